@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define TAM_ABI_VERSION 9
+#define TAM_ABI_VERSION 10
 #define TAM_BLOCK_SIZE 128 /* elements per quantisation / CoState block */
 
 /* error codes */
@@ -318,6 +318,48 @@ int tam_v_compress(const float* v, uint64_t n, uint32_t v_bits, int stochastic, 
  * quotient in[2i] / in[2i + 1] of n pairs).  No counterpart in the reference: it lets
  * a caller confirm the device math equals the host. */
 int tam_math_eval(int fn, const float* in, float* out, uint64_t n, void* stream);
+
+/* ---- layers: the forward and backward passes that give the step its
+ * gradients.  No counterpart in the reference, which has an optimizer only.
+ * Sums and statistics are fp32; each output is rounded to its type once. ---- */
+
+/* TamLinear.activation */
+#define TAM_ACT_NONE 0
+#define TAM_ACT_RELU 1
+#define TAM_ACT_GELU 2      /* 0.5 z (1 + erf(z / sqrt 2))                            */
+#define TAM_ACT_GELU_TANH 3 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))        */
+#define TAM_ACT_SILU 4      /* z / (1 + exp(-z))                                      */
+
+/* A linear layer: z = x w^T + bias, y = act(z) + residual, and its gradients.
+ * Every array is of `dtype`; arrays without a stride are contiguous.  Arrays
+ * may lie at any element's address; rows that are not whole 16 bytes on
+ * 16-byte addresses are first copied to the workspace. */
+typedef struct TamLinear {
+  const void* x;        /* [rows][inputs], row stride ldx                          */
+  const void* w;        /* [outputs][inputs], or [inputs][outputs] with w_in_out;  */
+                        /* row stride ldw                                          */
+  const void* bias;     /* [outputs] or NULL                                       */
+  const void* residual; /* [rows][outputs] or NULL                                 */
+  void* y;              /* forward: [rows][outputs]                                */
+  void* z;              /* [rows][outputs]: forward: written, or NULL; backward:   */
+                        /* read (the forward's), unless activation is NONE         */
+  const void* dy;       /* backward: [rows][outputs]                               */
+  void* dx;             /* backward: [rows][inputs] contiguous, or NULL            */
+  void* dw;             /* backward: laid out as w, contiguous, or NULL            */
+  void* db;             /* backward: [outputs], or NULL                            */
+  uint64_t rows, inputs, outputs;
+  uint64_t ldx, ldw;    /* elements                                                */
+  uint32_t dtype;       /* TAM_DTYPE_*                                             */
+  uint32_t activation;  /* TAM_ACT_*                                               */
+  uint32_t w_in_out;    /* w lies as [inputs][outputs]                             */
+  uint32_t reserved;
+} TamLinear;
+
+/* Bytes of workspace (256-byte aligned) of the two calls below. */
+int tam_linear_workspace(const TamLinear* d, int backward_pass, size_t* bytes);
+int tam_linear(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream);
+/* dx, dw and db (those that are not NULL); dresidual is dy. */
+int tam_linear_backward(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

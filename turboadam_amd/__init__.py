@@ -11,6 +11,7 @@ except PackageNotFoundError:
     __version__ = "0.1.0"
 
 from .checkpoint import load_reference_checkpoint  # noqa: E402
+from .layers import linear  # noqa: E402
 from .optimizer import TurboAdam  # noqa: E402
 
-__all__ = ["TurboAdam", "load_reference_checkpoint"]
+__all__ = ["TurboAdam", "linear", "load_reference_checkpoint"]

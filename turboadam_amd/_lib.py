@@ -28,7 +28,7 @@ TAM_FLAG_EF = 0x10
 TAM_FLAG_HAS_EF = 0x20
 TAM_FLAG_DEVICE_STEP = 0x40
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 # workspace of tam_multi_tensor_step_static (include/turboadam_amd.h)
 TAM_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -113,6 +113,30 @@ class TamStepInfo(ctypes.Structure):
     ]
 
 
+class TamLinear(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("z", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("db", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("inputs", ctypes.c_uint64),
+        ("outputs", ctypes.c_uint64),
+        ("ldx", ctypes.c_uint64),
+        ("ldw", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32),
+        ("activation", ctypes.c_uint32),
+        ("w_in_out", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 # Every symbol include/turboadam_amd.h declares, with its ctypes signature.
 _VP = ctypes.c_void_p
 SIGNATURES = {
@@ -176,6 +200,9 @@ SIGNATURES = {
         [_VP, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint64, _VP,
          _VP, _VP, ctypes.c_size_t, _VP],
     ),
+    "tam_linear_workspace": (ctypes.c_int, [ctypes.POINTER(TamLinear), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_linear": (ctypes.c_int, [ctypes.POINTER(TamLinear), _VP, ctypes.c_size_t, _VP]),
+    "tam_linear_backward": (ctypes.c_int, [ctypes.POINTER(TamLinear), _VP, ctypes.c_size_t, _VP]),
 }
 
 _lib = None

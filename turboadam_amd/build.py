@@ -1,7 +1,8 @@
 """Build recipe for the gfx950 library (and, for tests, the CPU oracle).
 
-``python -m turboadam_amd.build`` compiles ``csrc/tam_step.hip`` with hipcc
-into ``turboadam_amd/_build/libturboadam_amd.so``.  Flags:
+``python -m turboadam_amd.build`` compiles ``csrc/tam_step.hip`` (the packed-state
+step) and the layers' and Muon's sources with hipcc into
+``turboadam_amd/_build/libturboadam_amd.so``.  Flags:
   -ffp-contract=off      no implicit fma: every fma in the kernels is explicit,
                          matching where the reference's torch ops fuse;
   -packed-fp32-ops off   no v_pk_*_f32 (hipcc would otherwise form them);
@@ -11,12 +12,15 @@ into ``turboadam_amd/_build/libturboadam_amd.so``.  Flags:
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(BUILD_DIR, "libturboadam_amd.so")
-SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_step.hip")]
+STEP_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_step.hip")]
+OPERATOR_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_linear.hip",)]
+SOURCES = STEP_SOURCES + OPERATOR_SOURCES
 # streaming kernels that bench.py times as the bandwidth ceiling (not part of the library's ABI)
 STREAM_LIB_PATH = os.path.join(BUILD_DIR, "libtam_stream.so")
 STREAM_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_stream.hip")]
@@ -35,21 +39,35 @@ HIP_FLAGS = [
 ]
 
 
-def _hipcc(sources, out: str, verbose: bool, extra=()) -> str:
-    os.makedirs(BUILD_DIR, exist_ok=True)
-    tmp = out + ".tmp"
-    cmd = [HIPCC, *HIP_FLAGS, *extra, "-o", tmp, *sources]
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stderr}")
+
+
+def _hipcc(sources, out: str, verbose: bool, extra=()) -> str:
+    """Compile the sources (at once, where there are several) and link them into `out`."""
+    os.makedirs(BUILD_DIR, exist_ok=True)
+    tmp = out + ".tmp"
+    if len(sources) == 1:
+        _run([HIPCC, *HIP_FLAGS, *extra, "-o", tmp, *sources], verbose)
+    else:
+        flags = [f for f in HIP_FLAGS if f != "-shared"]
+        objects = [f"{out}.{os.path.basename(s)}.o" for s in sources]
+        with ThreadPoolExecutor(min(len(sources), os.cpu_count() or 1)) as pool:
+            list(pool.map(lambda so: _run([HIPCC, *flags, *extra, "-c", "-o", so[1], so[0]], verbose),
+                          zip(sources, objects)))
+        _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objects], verbose)
+        for o in objects:
+            os.remove(o)
     os.replace(tmp, out)
     return out
 
 
 def build_library(verbose: bool = False) -> str:
-    """The optimizer library, the host module of steady steps and the
+    """The library, the host module of steady steps and the
     streaming-kernel library bench.py uses."""
     _hipcc(STREAM_SOURCES, STREAM_LIB_PATH, verbose)
     build_host_module(verbose)
@@ -85,7 +103,7 @@ STATS_LIB_PATH = os.path.join(BUILD_DIR, "libturboadam_amd_stats.so")
 
 
 def build_stats_library(verbose: bool = False) -> str:
-    return _hipcc(SOURCES, STATS_LIB_PATH, verbose, ["-DTAM_STATS=1"])
+    return _hipcc(STEP_SOURCES, STATS_LIB_PATH, verbose, ["-DTAM_STATS=1"])
 
 
 if __name__ == "__main__":

@@ -1,0 +1,696 @@
+// tam_linear.hip -- linear layer of the C ABI: y = act(x w^T + bias) + residual
+// and its gradients, on the tile core of tam_gemm.h.
+//
+//   z = x w^T + bias,  y = act(z) + residual
+//   dz = dy act'(z),   dx = dz w,  dw = dz^T x,  dbias = sum over rows of dz
+//
+// Kernels:
+//   tam_k_gemm   one tile of a product; the forward epilogue adds the bias, keeps
+//                z (rounded to the type) for the backward pass, applies the
+//                activation and adds the residual, all in fp32, and rounds once;
+//   tam_k_split  the same epilogue over the partial sums of a product whose k was
+//                cut among workgroups (few tiles);
+//   tam_k_few    the forward product of up to 32 rows: every wave reads its part
+//                of 16 weight rows once, straight to the matrix cores;
+//   tam_k_slope  dz and its column sums;  tam_k_column_sum: the sums' end;
+//   tam_k_align  rows copied to 16-byte-aligned rows (zeros behind them), for
+//                operands whose rows are not.
+#include "tam_gemm.h"
+
+#include <math.h>
+
+#include <type_traits>
+
+#define TAM_ACT_MAX TAM_ACT_SILU
+
+// ---------------------------------------------------------------------------
+// activations (fp32)
+// ---------------------------------------------------------------------------
+// gelu_tanh: 0.5 z (1 + tanh u) = z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3)
+#define TAM_GELU_2U 1.5957691216057308f
+#define TAM_GELU_C 0.044715f
+
+__device__ __forceinline__ float tam_sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+__device__ __forceinline__ float tam_act(float z, uint32_t act) {
+  switch (act) {
+    case TAM_ACT_RELU: return z < 0.0f ? 0.0f : z;  // a NaN stays
+    case TAM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case TAM_ACT_GELU_TANH: return z * tam_sigmoid(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
+    case TAM_ACT_SILU: return z * tam_sigmoid(z);
+    default: return z;
+  }
+}
+
+__device__ __forceinline__ float tam_act_slope(float z, uint32_t act) {
+  switch (act) {
+    case TAM_ACT_RELU: return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
+    case TAM_ACT_GELU:
+      return __builtin_fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z),
+                            0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+    case TAM_ACT_GELU_TANH: {
+      const float s = tam_sigmoid(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
+      return __builtin_fmaf(z * s * (1.0f - s), TAM_GELU_2U * __builtin_fmaf(3.0f * TAM_GELU_C * z, z, 1.0f), s);
+    }
+    case TAM_ACT_SILU: {
+      const float s = tam_sigmoid(z);
+      return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// epilogue
+// ---------------------------------------------------------------------------
+struct tam_epilogue {
+  void* out;            // [rows][cols], contiguous
+  const void* bias;     // [cols] or null
+  const void* residual; // [rows][cols] or null
+  void* z;              // [rows][cols] or null
+  uint32_t rows, cols, act;
+};
+
+// v holds columns col .. col + 7 of a row of the product.
+template <typename T>
+__device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, uint32_t col, float (&v)[8]) {
+  const uint64_t at = (uint64_t)row * e.cols + col;
+  if (col + 8 <= e.cols) {
+    float t[8];
+    if (e.bias) {
+      tam_load8(static_cast<const T*>(e.bias) + col, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    if (e.z) tam_store8(static_cast<T*>(e.z) + at, v);
+    if (e.act != TAM_ACT_NONE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = tam_act(v[j], e.act);
+    }
+    if (e.residual) {
+      tam_load8(static_cast<const T*>(e.residual) + at, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    tam_store8(static_cast<T*>(e.out) + at, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (col + j >= e.cols) break;
+      float x = v[j];
+      if (e.bias) x += tam_to_f(static_cast<const T*>(e.bias)[col + j]);
+      if (e.z) static_cast<T*>(e.z)[at + j] = tam_from_f<T>(x);
+      x = tam_act(x, e.act);
+      if (e.residual) x += tam_to_f(static_cast<const T*>(e.residual)[at + j]);
+      static_cast<T*>(e.out)[at + j] = tam_from_f<T>(x);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+struct tam_gemm_args {
+  tam_operand P, Q;   // P: the columns' operand, Q: the rows'
+  uint64_t k, k_part; // the sum's length; of one of the parts it is cut into
+  uint32_t tm, tn;    // tiles
+  float* partial;     // [part][rows][cols] fp32, or null: one part
+  tam_epilogue e;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK>
+__global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 2 : (BM == 128 ? 3 : 4)) void tam_k_gemm(tam_gemm_args a) {
+  typedef tam_tile<T, BM, BN, WM, WN, PK, QK> Tile;
+  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  uint32_t m, n;
+  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
+  const uint64_t k0 = blockIdx.y * a.k_part;
+  const uint64_t k1 = k0 + a.k_part < a.k ? k0 + a.k_part : a.k;
+  Tile t;
+  t.zero();
+  t.run(a.P, a.Q, n * BN, m * BM, k0, k1, smem);
+  t.each(
+      smem,
+      [&](uint32_t row, uint32_t col, float(&v)[8]) {
+        row += m * BM;
+        col += n * BN;
+        if (row >= a.e.rows || col >= a.e.cols) return;
+        if (a.partial) {
+          float* p = a.partial + ((uint64_t)blockIdx.y * a.e.rows + row) * a.e.cols + col;
+          if (col + 8 <= a.e.cols) {
+            tam_store8(p, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < a.e.cols) p[j] = v[j];
+          }
+        } else {
+          tam_finish<T>(a.e, row, col, v);
+        }
+      },
+      [](uint32_t, uint32_t, const float*, int) {});
+}
+
+// The parts' sums in their order, then the epilogue: a thread takes 8 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_split(const float* partial, uint32_t parts, tam_epilogue e) {
+  const uint32_t per = (e.cols + 7) / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (uint64_t)per * e.rows) return;
+  const uint32_t row = (uint32_t)(i / per), col = (uint32_t)(i - (uint64_t)row * per) * 8;
+  const uint64_t at = (uint64_t)row * e.cols + col, step = (uint64_t)e.rows * e.cols;
+  float v[8] = {};
+  if (col + 8 <= e.cols) {
+    for (uint32_t p = 0; p < parts; ++p) {
+      float t[8];
+      tam_load8(partial + p * step + at, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+  } else {
+    for (uint32_t p = 0; p < parts; ++p)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < e.cols) v[j] += partial[p * step + at + j];
+  }
+  tam_finish<T>(e, row, col, v);
+}
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+// One workgroup: 16 columns of y (16 weight rows) for up to 16 * MT rows of x.
+// Its 8 waves take the k axis in turns of 4 chunks to a lane; a lane of fragment
+// row i loads the chunks at k0 + 8 * (4 u + lane / 16), u = 0..3: a wave's four
+// loads of a row are 256 consecutive bytes. Bound by reading w once; x stays in
+// the caches. The waves' sums meet in LDS in wave order.
+// Chunk k .. of a row; GUARD: elements from K on are zeros and not read.
+template <typename T, bool GUARD>
+__device__ __forceinline__ void tam_few_load(tam_frag<T>& f, const T* row, uint64_t k, uint64_t K) {
+  constexpr int N = 16 / (int)sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(N)));
+  struct __attribute__((packed, aligned(sizeof(T)))) any {
+    vec v;
+  };
+  if (!GUARD || k + N <= K) {
+    f.v = __builtin_bit_cast(decltype(f.v), reinterpret_cast<const any*>(row + k)->v);
+  } else {
+    vec v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = k + j < K ? row[k + j] : (T)0.0f;
+    f.v = __builtin_bit_cast(decltype(f.v), v);
+  }
+}
+
+struct tam_few_args {
+  const void* x;
+  const void* w;
+  uint64_t ldx, ldw, k;  // elements
+  tam_epilogue e;
+};
+
+#define TAM_FEW_WAVES 8
+
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_few(tam_few_args a) {
+  constexpr int N = 16 / (int)sizeof(T), U = 4;
+  constexpr uint64_t TURN = 4 * U * N;  // k of a wave's turn
+  __shared__ float sum[TAM_FEW_WAVES][MT * 16][20];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t i = lane & 15, q = lane >> 4, n = blockIdx.x * 16 + i;
+  // rows past the last one read the first one's elements; their sums go nowhere
+  const T* w = static_cast<const T*>(a.w) + (n < a.e.cols ? (uint64_t)n * a.ldw : 0);
+  const T* x[MT];
+  tam_f4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    x[m] = static_cast<const T*>(a.x) + (m * 16 + i < a.e.rows ? (uint64_t)(m * 16 + i) * a.ldx : 0);
+    acc[m] = tam_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto turn = [&](uint64_t k0, auto guard) {
+    constexpr bool G = decltype(guard)::value;
+    tam_frag<T> fw[U], fx[MT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) tam_few_load<T, G>(fw[u], w, k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) tam_few_load<T, G>(fx[m][u], x[m], k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc[m] = tam_mfma(fw[u], fx[m][u], acc[m]);
+  };
+  uint64_t k0 = wave * TURN;
+#pragma unroll 2
+  for (; k0 + TURN <= a.k; k0 += TAM_FEW_WAVES * TURN) turn(k0, std::false_type());
+  if (k0 < a.k) turn(k0, std::true_type());
+#pragma unroll
+  for (int m = 0; m < MT; ++m)  // row m * 16 + i, columns 4 q ..
+    *reinterpret_cast<tam_f4*>(&sum[wave][m * 16 + i][q * 4]) = acc[m];
+  __syncthreads();
+  const uint32_t t = threadIdx.x, row = t / 2, col = (t % 2) * 8;
+  if (t < MT * 32 && row < a.e.rows && blockIdx.x * 16 + col < a.e.cols) {
+    float v[8] = {};
+    for (int s = 0; s < TAM_FEW_WAVES; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += sum[s][row][col + j];
+    tam_finish<T>(a.e, row, blockIdx.x * 16 + col, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the backward pass's elementwise part
+// ---------------------------------------------------------------------------
+// A workgroup takes 512 columns (8 to a lane) of a run of rows, its waves every
+// fourth row; dz leaves rounded to the type, and the columns' sums of dz in fp32,
+// one row of `sums` to a run. dz == null: the sums alone (of dy).
+struct tam_slope_args {
+  const void* dy;
+  const void* z;
+  void* dz;
+  float* sums;     // [runs][cols] or null
+  uint64_t ld_dz;  // elements
+  uint32_t rows, cols, run, act;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_slope(tam_slope_args a) {
+  __shared__ float part[3][64][8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t col = blockIdx.x * 512 + lane * 8;
+  const uint32_t r0 = blockIdx.y * a.run, r1 = a.rows - r0 < a.run ? a.rows : r0 + a.run;
+  const bool whole = col + 8 <= a.cols;
+  float s[8] = {};
+  if (col < a.cols) {
+    for (uint32_t r = r0 + wave; r < r1; r += 4) {
+      const uint64_t at = (uint64_t)r * a.cols + col;
+      float d[8] = {}, z[8] = {};
+      if (whole) {
+        tam_load8(static_cast<const T*>(a.dy) + at, d);
+        if (a.act != TAM_ACT_NONE) tam_load8(static_cast<const T*>(a.z) + at, z);
+      } else {
+        for (uint32_t j = 0; j < 8; ++j)
+          if (col + j < a.cols) {
+            d[j] = tam_to_f(static_cast<const T*>(a.dy)[at + j]);
+            if (a.act != TAM_ACT_NONE) z[j] = tam_to_f(static_cast<const T*>(a.z)[at + j]);
+          }
+      }
+      if (a.act != TAM_ACT_NONE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] *= tam_act_slope(z[j], a.act);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += d[j];
+      // rows of dz are whole 16 bytes: columns past the last one are zeros
+      if (a.dz) tam_store8(static_cast<T*>(a.dz) + (uint64_t)r * a.ld_dz + col, d);
+    }
+  }
+  if (!a.sums) return;
+  if (wave) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[wave - 1][lane][j] = s[j];
+  }
+  __syncthreads();
+  if (wave == 0 && col < a.cols) {
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += part[w][lane][j];
+    float* out = a.sums + (uint64_t)blockIdx.y * a.cols + col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + j < a.cols) out[j] = s[j];
+  }
+}
+
+// out[c] = sum over runs of sums[run][c]: 64 columns to a workgroup, its 4 waves
+// take every fourth run.
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_column_sum(const float* sums, uint32_t runs, uint32_t cols, T* out) {
+  __shared__ float part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t c = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < cols)
+    for (uint32_t r = wave; r < runs; r += 4) s += sums[(uint64_t)r * cols + c];
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < cols) out[c] = tam_from_f<T>(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_zero(T* out, uint32_t n) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = (T)0.0f;
+}
+
+// ---------------------------------------------------------------------------
+// alignment
+// ---------------------------------------------------------------------------
+// dst[r][0 .. ld_dst) = src[r][0 .. cols), zeros behind: a thread takes 8 elements.
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_align(const T* src, uint64_t ld_src, uint64_t rows, uint32_t cols, T* dst,
+                                                   uint32_t ld_dst) {
+  const uint32_t per = ld_dst / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (uint64_t)per * rows) return;
+  const uint64_t r = i / per;
+  const uint32_t c = (uint32_t)(i - r * per) * 8;
+  const T* s = src + r * ld_src + c;
+  float v[8] = {};
+  if (c + 8 <= cols) {
+    tam_load8(s, v);
+  } else {
+    for (uint32_t j = 0; j < 8; ++j)
+      if (c + j < cols) v[j] = tam_to_f(s[j]);
+  }
+  tam_store8(dst + r * ld_dst + c, v);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr uint32_t kSize[3] = {4, 2, 2};
+
+// One matrix as the products read it: rows of `cols` contiguous elements.
+struct matrix {
+  const void* p;
+  uint64_t ld, rows;
+  uint32_t cols;
+};
+
+bool aligned(const matrix& m, uint32_t size) {
+  return (uint64_t)m.cols * size % 16 == 0 && m.ld * size % 16 == 0 && (uintptr_t)m.p % 16 == 0;
+}
+
+uint32_t aligned_ld(uint32_t cols) { return (uint32_t)tam_up(cols, 8); }
+
+// The workspace is laid out by walking the call twice: once without memory, to
+// learn its size, and once with it.
+struct arena {
+  char* base;
+  uint64_t used;
+  void* take(uint64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += tam_up(bytes, 256);
+    return p;
+  }
+};
+
+struct call {
+  uint32_t dtype;
+  hipStream_t stream;
+  arena ws;
+  bool dry;  // lay out the workspace only
+};
+
+int check_linear(const TamLinear* d, bool backward) {
+  tam_op_begin();
+  if (!d) return tam_op_fail(TAM_E_INVALID, "null argument");
+  if (d->dtype > TAM_DTYPE_F16) return tam_op_fail(TAM_E_INVALID, "unknown dtype %u", d->dtype);
+  if (d->activation > TAM_ACT_MAX) return tam_op_fail(TAM_E_INVALID, "unknown activation %u", d->activation);
+  const uint64_t most = 1ull << 31;
+  if (d->rows >= most || d->inputs >= most || d->outputs >= most)
+    return tam_op_fail(TAM_E_UNSUPPORTED, "a size of 2^31 or more");
+  if (d->inputs && (d->ldx < d->inputs || d->ldw < (d->w_in_out ? d->outputs : d->inputs)))
+    return tam_op_fail(TAM_E_INVALID, "a row stride shorter than its row");
+  // a tile's offsets of up to 256 rows are 31-bit numbers of bytes
+  if ((d->ldx | d->ldw | d->inputs | d->outputs) >= 1ull << 21)
+    return tam_op_fail(TAM_E_UNSUPPORTED, "a row or row stride of 2^21 elements or more");
+  if (d->rows == 0 || d->outputs == 0) return TAM_OK;
+  if (d->inputs && (!d->x || !d->w)) return tam_op_fail(TAM_E_INVALID, "null x or w");
+  if (!backward && !d->y) return tam_op_fail(TAM_E_INVALID, "null y");
+  if (backward && !d->dy) return tam_op_fail(TAM_E_INVALID, "null dy");
+  if (backward && d->activation != TAM_ACT_NONE && !d->z) return tam_op_fail(TAM_E_INVALID, "null z");
+  return TAM_OK;
+}
+
+// ---- products ----
+
+struct shape {
+  int tile;        // rows and columns of a tile
+  uint32_t parts;  // the sum is cut into
+};
+
+// Which tile, and into how many parts the sum is cut. A product's time is about
+// rounds of tiles over the compute units times a tile's, and a tile's is its
+// multiplications at the rate that its size reaches when the chip is full
+// (measured, bf16, 8192 x 4096 x 4096 in TFLOP/s: see `rate`) plus what it
+// cannot hide; parts add their sums' way to memory and back and a launch.
+shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
+  const double cus = tam_op_cus(), f32 = dtype == TAM_DTYPE_F32 ? 8.0 : 1.0;
+  struct {
+    int tile;
+    double rate;   // TFLOP/s of 16-bit products
+    double start;  // us before and after a tile's sum
+  } const kind[3] = {{256, 1000.0, 4.0}, {128, 700.0, 2.5}, {64, 350.0, 1.5}};
+  shape best = {64, 1};
+  double least = 1e30;
+  for (const auto& t : kind) {
+    if (t.tile == 256 && dtype == TAM_DTYPE_F32) continue;
+    const double tiles = (double)tam_div_up(rows, t.tile) * (double)tam_div_up(cols, t.tile);
+    for (uint32_t parts = 1; parts <= 32; parts *= 2) {
+      if (parts > 1 && k / parts < 256) break;
+      const double rounds = tiles * parts / cus < 1.0 ? 1.0 : ceil(tiles * parts / cus);
+      const double one = 2.0 * t.tile * t.tile * ((double)k / parts) * cus / (t.rate * 1e6) * f32;
+      double us = rounds * (one + (rounds > 1.0 ? 0.5 : 1.0) * t.start);
+      if (parts > 1) us += 3.0 + (double)rows * cols * 4.0 * (2.0 * parts) / 3e6;
+      if (us < least) {
+        least = us;
+        best = {t.tile, parts};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, int TILE, int WM, int WN>
+void launch_tile(bool pk, bool qk, const tam_gemm_args& a, uint32_t parts, hipStream_t s) {
+  const dim3 grid(a.tm * a.tn, parts), block(64 * WM * WN);
+  if (pk && qk)
+    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, true, true>), grid, block, 0, s, a);
+  else if (qk)
+    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, false, true>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, false, false>), grid, block, 0, s, a);
+}
+
+template <typename T>
+void launch_gemm(int tile, bool pk, bool qk, const tam_gemm_args& a, uint32_t parts, hipStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (tile == 256) return launch_tile<T, 256, 2, 4>(pk, qk, a, parts, s);
+  if (tile == 128) return launch_tile<T, 128, 2, 2>(pk, qk, a, parts, s);
+  launch_tile<T, 64, 2, 2>(pk, qk, a, parts, s);
+}
+
+// out[rows][cols] = sum over k of Q's row and P's row: P and Q as they lie in
+// memory, p_k / q_k: rows of the matrix are the operand's rows (contiguous along k).
+int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint64_t k, const tam_epilogue& e) {
+  const shape s = choose(e.rows, e.cols, k, c.dtype);
+  float* partial = s.parts > 1 ? (float*)c.ws.take((uint64_t)s.parts * e.rows * e.cols * 4) : nullptr;
+  if (c.dry) return TAM_OK;
+  const uint32_t size = kSize[c.dtype];
+  tam_gemm_args a = {};
+  a.P = {(const char*)P.p, P.ld * size, e.cols};
+  a.Q = {(const char*)Q.p, Q.ld * size, e.rows};
+  a.k = k;
+  a.k_part = s.parts > 1 ? tam_up(tam_div_up(k, s.parts), 64) : k;
+  a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
+  a.tn = (uint32_t)tam_div_up(e.cols, s.tile);
+  a.partial = partial;
+  a.e = e;
+  if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+  if (c.dtype == TAM_DTYPE_BF16)
+    launch_gemm<tam_bf16>(s.tile, p_k, q_k, a, s.parts, c.stream);
+  else if (c.dtype == TAM_DTYPE_F16)
+    launch_gemm<tam_f16>(s.tile, p_k, q_k, a, s.parts, c.stream);
+  else
+    launch_gemm<float>(s.tile, p_k, q_k, a, s.parts, c.stream);
+  TAM_OP_LAUNCHED("the product");
+  if (s.parts > 1) {
+    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
+    if (c.dtype == TAM_DTYPE_BF16)
+      hipLaunchKernelGGL(tam_k_split<tam_bf16>, grid, block, 0, c.stream, partial, s.parts, e);
+    else if (c.dtype == TAM_DTYPE_F16)
+      hipLaunchKernelGGL(tam_k_split<tam_f16>, grid, block, 0, c.stream, partial, s.parts, e);
+    else
+      hipLaunchKernelGGL(tam_k_split<float>, grid, block, 0, c.stream, partial, s.parts, e);
+    TAM_OP_LAUNCHED("the parts' sum");
+  }
+  return TAM_OK;
+}
+
+// m, or a copy of it whose rows are whole 16 bytes on 16-byte addresses.
+int on_16_bytes(call& c, matrix& m) {
+  const uint32_t size = kSize[c.dtype];
+  if (aligned(m, size)) return TAM_OK;
+  const uint32_t ld = aligned_ld(m.cols);
+  void* p = c.ws.take(m.rows * ld * size);
+  if (!c.dry && m.rows) {
+    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
+    if (c.dtype == TAM_DTYPE_F32)
+      hipLaunchKernelGGL(tam_k_align<float>, grid, block, 0, c.stream, (const float*)m.p, m.ld, m.rows, m.cols,
+                         (float*)p, ld);
+    else if (c.dtype == TAM_DTYPE_BF16)
+      hipLaunchKernelGGL(tam_k_align<tam_bf16>, grid, block, 0, c.stream, (const tam_bf16*)m.p, m.ld, m.rows, m.cols,
+                         (tam_bf16*)p, ld);
+    else
+      hipLaunchKernelGGL(tam_k_align<tam_f16>, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld, m.rows, m.cols,
+                         (tam_f16*)p, ld);
+    TAM_OP_LAUNCHED("the aligned copy");
+  }
+  m.p = p;
+  m.ld = ld;
+  return TAM_OK;
+}
+
+matrix x_of(const TamLinear* d) { return {d->x, d->ldx, d->rows, (uint32_t)d->inputs}; }
+matrix w_of(const TamLinear* d) {
+  return {d->w, d->ldw, d->w_in_out ? d->inputs : d->outputs, (uint32_t)(d->w_in_out ? d->outputs : d->inputs)};
+}
+
+int forward(const TamLinear* d, call& c) {
+  if (d->rows == 0 || d->outputs == 0) return TAM_OK;
+  tam_epilogue e = {d->y, d->bias, d->residual, d->z, (uint32_t)d->rows, (uint32_t)d->outputs, d->activation};
+  if (d->rows <= 32 && !d->w_in_out) {
+    if (c.dry) return TAM_OK;
+    const tam_few_args a = {d->x, d->w, d->ldx, d->ldw, d->inputs, e};
+    const dim3 grid((uint32_t)tam_div_up(d->outputs, 16)), block(64 * TAM_FEW_WAVES);
+#define TAM_FEW(T)                                                                   \
+  if (d->rows <= 16)                                                                 \
+    hipLaunchKernelGGL((tam_k_few<T, 1>), grid, block, 0, c.stream, a);              \
+  else                                                                               \
+    hipLaunchKernelGGL((tam_k_few<T, 2>), grid, block, 0, c.stream, a)
+    if (c.dtype == TAM_DTYPE_F32) {
+      TAM_FEW(float);
+    } else if (c.dtype == TAM_DTYPE_BF16) {
+      TAM_FEW(tam_bf16);
+    } else {
+      TAM_FEW(tam_f16);
+    }
+    TAM_OP_LAUNCHED("the product of few rows");
+    return TAM_OK;
+  }
+  matrix x = x_of(d), w = w_of(d);
+  int rc = on_16_bytes(c, x);
+  if (rc == TAM_OK) rc = on_16_bytes(c, w);
+  if (rc == TAM_OK) rc = product(c, w, !d->w_in_out, x, true, d->inputs, e);
+  return rc;
+}
+
+// Rows of one run of tam_k_slope: about four workgroups to a compute unit, at
+// least 16 rows (4 to a wave).
+uint32_t slope_run(uint64_t rows, uint64_t cols) {
+  const uint64_t across = tam_div_up(cols, 512), runs = tam_div_up(4ull * tam_op_cus(), across);
+  const uint64_t run = tam_div_up(rows, runs);
+  return (uint32_t)tam_up(run < 16 ? 16 : run, 4);
+}
+
+int backward(const TamLinear* d, call& c) {
+  if (d->outputs == 0 && d->inputs == 0) return TAM_OK;
+  const uint32_t size = kSize[c.dtype];
+  matrix dz = {d->dy, d->outputs, d->rows, (uint32_t)d->outputs};
+  const bool products = (d->dx || d->dw) && d->inputs;
+  const bool keep = products && (d->activation != TAM_ACT_NONE || !aligned(dz, size));
+  if (d->rows && d->outputs && (keep || d->db)) {
+    tam_slope_args a = {d->dy, d->z, nullptr, nullptr, 0, (uint32_t)d->rows, (uint32_t)d->outputs, 0, d->activation};
+    if (keep) {
+      dz.ld = a.ld_dz = aligned_ld((uint32_t)d->outputs);
+      dz.p = a.dz = c.ws.take(d->rows * dz.ld * size);
+    }
+    a.run = slope_run(d->rows, d->outputs);
+    const uint32_t runs = (uint32_t)tam_div_up(d->rows, a.run);
+    if (d->db) a.sums = (float*)c.ws.take((uint64_t)runs * d->outputs * 4);
+    if (!c.dry) {
+      const dim3 grid((uint32_t)tam_div_up(d->outputs, 512), runs), block(256), sums((uint32_t)tam_div_up(d->outputs, 64));
+#define TAM_SLOPE(T)                                                                                               \
+  do {                                                                                                             \
+    hipLaunchKernelGGL(tam_k_slope<T>, grid, block, 0, c.stream, a);                                               \
+    TAM_OP_LAUNCHED("the activation's gradient");                                                                  \
+    if (d->db) {                                                                                                   \
+      hipLaunchKernelGGL(tam_k_column_sum<T>, sums, block, 0, c.stream, a.sums, runs, (uint32_t)d->outputs, (T*)d->db); \
+      TAM_OP_LAUNCHED("the bias's gradient");                                                                      \
+    }                                                                                                              \
+  } while (0)
+      if (c.dtype == TAM_DTYPE_F32)
+        TAM_SLOPE(float);
+      else if (c.dtype == TAM_DTYPE_BF16)
+        TAM_SLOPE(tam_bf16);
+      else
+        TAM_SLOPE(tam_f16);
+    }
+  } else if (d->db && d->outputs && !c.dry) {  // no rows: an empty sum
+    const dim3 grid((uint32_t)tam_div_up(d->outputs, 256)), block(256);
+    if (size == 4)
+      hipLaunchKernelGGL(tam_k_zero<float>, grid, block, 0, c.stream, (float*)d->db, (uint32_t)d->outputs);
+    else  // zero has the same 16 bits in both types
+      hipLaunchKernelGGL(tam_k_zero<tam_f16>, grid, block, 0, c.stream, (tam_f16*)d->db, (uint32_t)d->outputs);
+    TAM_OP_LAUNCHED("the bias's gradient");
+  }
+  if (!products) return TAM_OK;
+  if (d->dx && d->rows) {
+    matrix w = w_of(d);
+    int rc = d->outputs ? on_16_bytes(c, w) : TAM_OK;
+    const tam_epilogue e = {d->dx, nullptr, nullptr, nullptr, (uint32_t)d->rows, (uint32_t)d->inputs, TAM_ACT_NONE};
+    if (rc == TAM_OK) rc = product(c, w, d->w_in_out != 0, dz, true, d->outputs, e);
+    if (rc != TAM_OK) return rc;
+  }
+  if (d->dw && d->outputs) {
+    matrix x = x_of(d);
+    const int rc = d->rows ? on_16_bytes(c, x) : TAM_OK;
+    if (rc != TAM_OK) return rc;
+    // dw lies as w does: [outputs][inputs], or [inputs][outputs]
+    tam_epilogue e = {d->dw, nullptr, nullptr, nullptr, (uint32_t)d->outputs, (uint32_t)d->inputs, TAM_ACT_NONE};
+    if (!d->w_in_out) return product(c, x, false, dz, false, d->rows, e);
+    e.rows = (uint32_t)d->inputs;
+    e.cols = (uint32_t)d->outputs;
+    return product(c, dz, false, x, false, d->rows, e);
+  }
+  return TAM_OK;
+}
+
+int linear(const TamLinear* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need) {
+  int rc = check_linear(d, back);
+  if (rc != TAM_OK) return rc;
+  call c = {d->dtype, (hipStream_t)stream, {nullptr, 0}, true};
+  rc = back ? backward(d, c) : forward(d, c);
+  if (rc != TAM_OK) return rc;
+  if (need) {
+    *need = c.ws.used;
+    return TAM_OK;
+  }
+  if (c.ws.used > ws_bytes || (c.ws.used && !workspace))
+    return tam_op_fail(TAM_E_WORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes,
+                       (unsigned long long)c.ws.used);
+  if ((uintptr_t)workspace & 255u) return tam_op_fail(TAM_E_INVALID, "workspace not on 256 bytes");
+  c = {d->dtype, (hipStream_t)stream, {(char*)workspace, 0}, false};
+  return back ? backward(d, c) : forward(d, c);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tam_linear_workspace(const TamLinear* d, int backward_pass, size_t* bytes) {
+  if (!bytes) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  uint64_t need = 0;
+  const int rc = linear(d, backward_pass != 0, nullptr, 0, nullptr, &need);
+  *bytes = (size_t)need;
+  return rc;
+}
+
+int tam_linear(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream) {
+  return linear(d, false, workspace, ws_bytes, stream, nullptr);
+}
+
+int tam_linear_backward(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream) {
+  return linear(d, true, workspace, ws_bytes, stream, nullptr);
+}
+
+}  // extern "C"

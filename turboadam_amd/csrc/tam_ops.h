@@ -1,0 +1,101 @@
+// tam_ops.h -- what the operators' sources (tam_norm.hip, tam_linear.hip,
+// tam_muon.hip) share: error reporting, element types and launch helpers.
+#ifndef TAM_OPS_H
+#define TAM_OPS_H
+
+#include <hip/hip_runtime.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/turboadam_amd.h"
+
+// The thread's message lies in tam_step.hip, which hands it out as
+// tam_last_error(): 512 bytes, written here by every failing call too.
+#define TAM_ERR_BYTES 512
+
+__attribute__((format(printf, 2, 3))) static inline int tam_op_fail(int code, const char* fmt, ...) {
+  va_list args;
+  va_start(args, fmt);
+  vsnprintf(const_cast<char*>(tam_last_error()), TAM_ERR_BYTES, fmt, args);
+  va_end(args);
+  return code;
+}
+
+static inline void tam_op_begin() { const_cast<char*>(tam_last_error())[0] = 0; }
+
+#define TAM_OP_LAUNCHED(what)                                                                       \
+  do {                                                                                              \
+    const hipError_t e_ = hipGetLastError();                                                        \
+    if (e_ != hipSuccess) return tam_op_fail(TAM_E_HIP, "HIP error at %s: code %d", what, (int)e_); \
+  } while (0)
+
+static inline uint64_t tam_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+static inline uint64_t tam_div_up(uint64_t x, uint64_t by) { return (x + by - 1) / by; }
+
+// Compute units of the current device; 256 (an MI355X) where it cannot be asked.
+static inline uint32_t tam_op_cus() {
+  static const uint32_t cus = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+      return 256u;
+    return n > 0 ? (uint32_t)n : 256u;
+  }();
+  return cus;
+}
+
+// ---------------------------------------------------------------------------
+// element types
+// ---------------------------------------------------------------------------
+typedef __bf16 tam_bf16;
+typedef _Float16 tam_f16;
+typedef float tam_f4 __attribute__((ext_vector_type(4)));
+
+// N elements that may lie at any element's address (gfx950 moves 16 bytes at
+// any address; the claimed alignment is the element's own).
+template <typename T, int N>
+struct tam_pack {
+  T v[N];
+};
+
+template <typename T>
+__device__ __forceinline__ float tam_to_f(T x) {
+  return (float)x;
+}
+template <typename T>
+__device__ __forceinline__ T tam_from_f(float x) {
+  return (T)x;  // round to nearest even
+}
+
+// 8 consecutive elements at p to fp32 and back, 16 (32 for fp32) bytes at once.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) tam_oct {
+  T v __attribute__((ext_vector_type(8)));
+};
+template <>
+struct __attribute__((packed, aligned(2))) tam_oct<tam_bf16> {
+  tam_bf16 v __attribute__((ext_vector_type(8)));
+};
+
+template <typename T>
+__device__ __forceinline__ void tam_load8(const T* p, float (&x)[8]) {
+  const tam_oct<T> o = *reinterpret_cast<const tam_oct<T>*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)o.v[i];
+}
+template <typename T>
+__device__ __forceinline__ void tam_store8(T* p, const float (&x)[8]) {
+  tam_oct<T> o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o.v[i] = (T)x[i];
+  *reinterpret_cast<tam_oct<T>*>(p) = o;
+}
+
+// Sum over the wave's 64 lanes; every lane gets it.
+__device__ __forceinline__ float tam_wave_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
+#endif  // TAM_OPS_H
