@@ -361,6 +361,68 @@ int tam_linear(const TamLinear* d, void* workspace, size_t ws_bytes, void* strea
 /* dx, dw and db (those that are not NULL); dresidual is dy. */
 int tam_linear_backward(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream);
 
+/* Layer norm over rows of n elements (at most 32768): y = (x - mean) rstd w + b
+ * with rstd = 1 / sqrt(var + eps), var the mean squared distance from the mean;
+ * and its gradients.  Every array but stats is of `dtype`, contiguous but for
+ * x's row stride, at any element's address. */
+typedef struct TamNorm {
+  const void* x;        /* [rows][n], row stride ldx                               */
+  const void* w;        /* [n] or NULL (ones)                                      */
+  const void* b;        /* [n] or NULL (zeros); forward only                       */
+  void* y;              /* forward: [rows][n]                                      */
+  float* stats;         /* f32[rows][2] mean and rstd: forward: written, or NULL;  */
+                        /* backward: read                                          */
+  const void* dy;       /* backward: [rows][n]                                     */
+  void* dx;             /* backward: [rows][n] or NULL                             */
+  void* dw;             /* backward: [n] or NULL                                   */
+  void* db;             /* backward: [n] or NULL                                   */
+  uint64_t rows, n, ldx;
+  uint32_t dtype;       /* TAM_DTYPE_*                                             */
+  float eps;
+} TamNorm;
+
+/* Bytes of workspace of the backward pass (0 for the forward). */
+int tam_norm_workspace(const TamNorm* d, int backward_pass, size_t* bytes);
+int tam_norm(const TamNorm* d, void* stream);
+int tam_norm_backward(const TamNorm* d, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- Muon: matrices stepped by their orthogonalised momentum.  No counterpart
+ * in the reference. ---- */
+
+/* TamMatrix.flags */
+#define TAM_MATRIX_UPDATE 0x1u   /* step the parameter `out`; else write the direction to it */
+#define TAM_MATRIX_NESTEROV 0x2u /* u looks one step ahead of the momentum                   */
+
+/* One matrix: u = g without a momentum; with one, m = keep m + (1 - keep) g and
+ * u = m, or (1 - keep) g + keep m (NESTEROV).  x = u / max(|u|, eps) with the
+ * Frobenius norm, then `steps` times x = a x + b q x + c q q x with q = x x^T
+ * (x^T x where rows > cols: the same polynomial).  out = x, or with UPDATE
+ * out = decay out - rate x.  Products run on the fp16 matrix cores with fp32
+ * sums: for bf16, x has a high and a low part and the products take the high
+ * ones; for fp32 and fp16 every factor has both, and a product is three
+ * (22 bits).  Each result is rounded to its type once. */
+typedef struct TamMatrix {
+  void* out;            /* [rows][cols] of dtype, contiguous                       */
+  const void* grad;     /* [rows][cols] of dtype, contiguous                       */
+  float* momentum;      /* f32[rows][cols] or NULL                                 */
+  uint64_t rows, cols;  /* 1 to 65536 each                                         */
+  uint32_t dtype;       /* TAM_DTYPE_*                                             */
+  uint32_t flags;       /* TAM_MATRIX_*                                            */
+  float keep, one_minus_keep;
+  float eps;            /* above 0                                                 */
+  float decay, rate;    /* UPDATE: 1 - lr * weight decay; the adjusted lr          */
+  uint32_t reserved;
+} TamMatrix;
+
+/* Bytes of workspace (256-byte aligned) of tam_orthogonalize: about 8 per
+ * element of the matrices and 4 or 8 per element of their smaller squares. */
+int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes);
+/* All n matrices (a host array, read before the call returns) in the same 2 +
+ * 3 * steps launches, beside their descriptors' upload. coefficients: a, b, c;
+ * steps 1 to 64. */
+int tam_orthogonalize(const TamMatrix* matrices, int n, const float* coefficients, int steps, void* workspace,
+                      size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

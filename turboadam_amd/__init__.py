@@ -11,7 +11,8 @@ except PackageNotFoundError:
     __version__ = "0.1.0"
 
 from .checkpoint import load_reference_checkpoint  # noqa: E402
-from .layers import linear  # noqa: E402
+from .layers import layer_norm, linear  # noqa: E402
+from .muon import Muon, orthogonalize  # noqa: E402
 from .optimizer import TurboAdam  # noqa: E402
 
-__all__ = ["TurboAdam", "linear", "load_reference_checkpoint"]
+__all__ = ["Muon", "TurboAdam", "layer_norm", "linear", "load_reference_checkpoint", "orthogonalize"]

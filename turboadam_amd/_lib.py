@@ -137,6 +137,47 @@ class TamLinear(ctypes.Structure):
     ]
 
 
+class TamNorm(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("db", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("n", ctypes.c_uint64),
+        ("ldx", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+TAM_MATRIX_UPDATE = 0x1
+TAM_MATRIX_NESTEROV = 0x2
+
+
+class TamMatrix(ctypes.Structure):
+    _fields_ = [
+        ("out", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("momentum", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("cols", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32),
+        ("flags", ctypes.c_uint32),
+        ("keep", ctypes.c_float),
+        ("one_minus_keep", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("decay", ctypes.c_float),
+        ("rate", ctypes.c_float),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 # Every symbol include/turboadam_amd.h declares, with its ctypes signature.
 _VP = ctypes.c_void_p
 SIGNATURES = {
@@ -203,6 +244,14 @@ SIGNATURES = {
     "tam_linear_workspace": (ctypes.c_int, [ctypes.POINTER(TamLinear), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_linear": (ctypes.c_int, [ctypes.POINTER(TamLinear), _VP, ctypes.c_size_t, _VP]),
     "tam_linear_backward": (ctypes.c_int, [ctypes.POINTER(TamLinear), _VP, ctypes.c_size_t, _VP]),
+    "tam_norm_workspace": (ctypes.c_int, [ctypes.POINTER(TamNorm), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_norm": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP]),
+    "tam_norm_backward": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP, ctypes.c_size_t, _VP]),
+    "tam_orthogonalize_workspace": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_orthogonalize": (
+        ctypes.c_int,
+        [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_float), ctypes.c_int, _VP, ctypes.c_size_t, _VP],
+    ),
 }
 
 _lib = None

@@ -19,7 +19,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(BUILD_DIR, "libturboadam_amd.so")
 STEP_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_step.hip")]
-OPERATOR_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_linear.hip",)]
+OPERATOR_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_linear.hip", "tam_norm.hip", "tam_muon.hip")]
 SOURCES = STEP_SOURCES + OPERATOR_SOURCES
 # streaming kernels that bench.py times as the bandwidth ceiling (not part of the library's ABI)
 STREAM_LIB_PATH = os.path.join(BUILD_DIR, "libtam_stream.so")

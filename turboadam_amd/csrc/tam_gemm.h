@@ -168,9 +168,16 @@ struct tam_stage {
   }
 };
 
+// A product of operands in two parts, high + low: the sum of high * high, high *
+// low and low * high runs as one sum over three times k.  p, q: bytes from an
+// operand's high part to its low part (the same layout).
+struct tam_parts {
+  uint32_t terms;  // 1 (high * high alone) or 3
+  int64_t p, q;
+};
+
 // One workgroup's tile: BM rows (operand Q) by BN columns (operand P), WM by
-// WN waves.  STAGE2: the loads of a second pair of operands follow the first
-// pair's (used where a product is a sum of products).
+// WN waves.
 template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK>
 struct tam_tile {
   static constexpr int NW = WM * WN;
@@ -223,8 +230,9 @@ struct tam_tile {
   }
 
   // Adds the products of k0 <= k < k1 to the tile at rows r0, columns c0.
+  template <bool PARTS = false>
   __device__ __forceinline__ void run(const tam_operand& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
-                                      uint64_t k1, char* smem) {
+                                      uint64_t k1, char* smem, tam_parts parts = {1, 0, 0}) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     tam_lds_char* lds = (tam_lds_char*)smem;
@@ -232,9 +240,20 @@ struct tam_tile {
     SQ sq;
     sp.init(P, c0, k0, wave, lane);
     sq.init(Q, r0, k0, wave, lane);
-    int64_t left = k1 > k0 ? (int64_t)(k1 - k0) : 0;  // k from the next stage to load on
-    const uint32_t pairs = (uint32_t)((left + 2 * BK - 1) / (2 * BK));
+    const char *const p0 = sp.base, *const q0 = sq.base;
+    const int64_t length = k1 > k0 ? (int64_t)(k1 - k0) : 0;
+    int64_t left = length;  // k from the next stage to load on
+    uint32_t steps = (uint32_t)((length + BK - 1) / BK), term = 0;
+    if constexpr (PARTS) steps *= parts.terms;
+    const uint32_t pairs = (steps + 1) / 2;
     auto load = [&](uint32_t buf) {
+      if constexpr (PARTS)
+        if (left <= 0 && term + 1 < parts.terms) {
+          ++term;
+          left = length;
+          sp.base = p0 + (term == 2 ? parts.p : 0);
+          sq.base = q0 + (term == 1 ? parts.q : 0);
+        }
       sp.load(lds + buf * STAGE, wave, left);
       sq.load(lds + buf * STAGE + SP::BYTES, wave, left);
       left -= BK;

@@ -1,0 +1,641 @@
+// tam_muon.hip -- momentum, orthogonalisation by Newton-Schulz products and
+// parameter update of a list of matrices (C ABI: tam_orthogonalize).
+//
+// With s the smaller and l the larger side, x (s x l or, tall, l x s) and
+// q = x x^T (tall: x^T x), a step is x <- (a I + b q + c q q) x (tall: from the
+// right), three products; the first two are symmetric, and only the tiles on
+// and below the diagonal are computed, each stored twice.
+//
+// Numbers.  The norm makes every singular value of x at most 1, and the step's
+// polynomial keeps them near 1, so x, q and p = a I + b q + c q q are held as
+// fp16 times 2^12: entries up to 16, and 11 bits down to 1.5e-8 of x's scale,
+// at the rate of bf16 with an eighth of its error.  What a step's rounding adds
+// in x's small singular directions the next steps amplify like the directions
+// themselves (a per step), so x keeps a low fp16 part, and x' = p x_high + diag(p)
+// x_low: p x_low with p's diagonal alone, since p is near diagonal where x_low
+// matters.  Rounding a I into p, instead of adding a x, keeps the diagonal's
+// rounding at the size of the result.  That is the scheme for bf16 matrices (error
+// about 1e-3 of the result's norm, below bf16's own rounding 1.7e-3).  fp32 and
+// fp16 matrices have high and low parts of x, q and p, and every product is high
+// high + high low + low high: 22 bits, errors near those of fp32 sums.
+//
+// Launches (whole list each): tam_k_mu_momentum (momentum, partial squares of
+// u), tam_k_mu_start (x = u / |u|, in parts), then per step tam_k_mu_square
+// twice (q, p) and tam_k_mu_apply (x, the last one: the output).
+#include "tam_gemm.h"
+
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+namespace {
+
+constexpr float kScale = 4096.f;        // what fp16 entries are multiplied by
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMostPartials = 512; // of a matrix's squares
+constexpr uint64_t kMostSide = 65536;
+
+// A matrix as the kernels take it.  Unit counts run over the list: units of
+// phase f of matrix i are first[f] .. first[f] of i + 1.
+enum { MOMENTUM, START, SQUARE, APPLY, PHASES };
+
+struct mat {
+  void* out;
+  const void* grad;
+  float* momentum;
+  tam_f16* x[2];      // [rows][ldx] high parts, in turns; the low part `low` behind
+  tam_f16 *q, *p;     // [s][lds]
+  float* diag;        // p's diagonal, fp32
+  float* partial;     // squares of u
+  uint64_t elements;
+  int64_t x_low, s_low;  // elements from a high part to its low part (s_low 0: none)
+  uint32_t rows, cols, s, ldx, lds;
+  uint32_t tall, split, dtype, flags;
+  uint32_t first[PHASES];
+  uint32_t partials, chunk;  // partial squares; elements of each
+  float keep, one_minus_keep, eps, decay, rate;
+};
+
+struct list {
+  const mat* m;
+  uint32_t n;
+  uint32_t units[PHASES];
+};
+
+// The matrix whose unit of phase F b is: the last one whose first unit is not
+// past b.  64 matrices are looked at at once.
+template <int F>
+__device__ __forceinline__ uint32_t owner(const list& l, uint32_t b) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t found = 0;
+  for (uint32_t i = 0; i < l.n; i += 64) {
+    const bool in = i + lane < l.n && l.m[i + lane].first[F] <= b;
+    const uint64_t mask = __ballot(in);
+    if (!mask) break;
+    found = i + 63u - (uint32_t)__builtin_clzll(mask);
+    if (mask != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(found);
+}
+
+// ---------------------------------------------------------------------------
+// descriptors
+// ---------------------------------------------------------------------------
+constexpr int kPut = 16;  // descriptors that one launch carries as arguments
+struct put_args {
+  mat m[kPut];
+};
+static_assert(sizeof(put_args) <= 3968, "kernel arguments");
+
+__global__ __launch_bounds__(256) void tam_k_mu_put(put_args a, mat* to, uint32_t n) {
+  const uint32_t words = n * (uint32_t)(sizeof(mat) / 4);
+  for (uint32_t i = threadIdx.x; i < words; i += 256)
+    reinterpret_cast<uint32_t*>(to)[i] = reinterpret_cast<const uint32_t*>(&a)[i];
+}
+
+// ---------------------------------------------------------------------------
+// u
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void grad8(const mat& m, uint64_t at, uint32_t count, float (&g)[8]) {
+  const T* p = static_cast<const T*>(m.grad) + at;
+  if (count == 8) {
+    tam_load8(p, g);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) g[j] = j < count ? tam_to_f(p[j]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void load_grad(const mat& m, uint64_t at, uint32_t count, float (&g)[8]) {
+  if (m.dtype == TAM_DTYPE_F32)
+    grad8<float>(m, at, count, g);
+  else if (m.dtype == TAM_DTYPE_BF16)
+    grad8<tam_bf16>(m, at, count, g);
+  else
+    grad8<tam_f16>(m, at, count, g);
+}
+
+__device__ __forceinline__ void load_f32(const float* p, uint32_t count, float (&v)[8]) {
+  if (count == 8) {
+    tam_load8(p, v);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) v[j] = j < count ? p[j] : 0.f;
+  }
+}
+
+// u of elements whose gradient is g and whose (new) momentum is m.
+__device__ __forceinline__ void direction(const mat& d, const float (&g)[8], const float (&m)[8], float (&u)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    u[j] = !d.momentum ? g[j]
+           : d.flags & TAM_MATRIX_NESTEROV ? __builtin_fmaf(d.keep, m[j], d.one_minus_keep * g[j])
+                                           : m[j];
+}
+
+// Sum over the workgroup; every thread gets it.
+__device__ __forceinline__ float group_sum(float x, float* lds) {
+  x = tam_wave_sum(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// A unit is `chunk` consecutive elements.
+__global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
+  __shared__ float lds[4];
+  const mat& d = l.m[owner<MOMENTUM>(l, blockIdx.x)];
+  const uint32_t unit = blockIdx.x - d.first[MOMENTUM];
+  const uint64_t begin = (uint64_t)unit * d.chunk, end = begin + d.chunk < d.elements ? begin + d.chunk : d.elements;
+  float sum = 0.f;
+  for (uint64_t at = begin + threadIdx.x * 8u; at < end; at += kThreads * 8u) {
+    const uint32_t count = end - at < 8 ? (uint32_t)(end - at) : 8u;
+    float g[8], m[8] = {}, u[8];
+    load_grad(d, at, count, g);
+    if (d.momentum) {
+      load_f32(d.momentum + at, count, m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m[j] = __builtin_fmaf(d.one_minus_keep, g[j], d.keep * m[j]);
+      if (count == 8) {
+        tam_store8(d.momentum + at, m);
+      } else {
+        for (uint32_t j = 0; j < 8; ++j)
+          if (j < count) d.momentum[at + j] = m[j];
+      }
+    }
+    direction(d, g, m, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(u[j], u[j], sum);
+  }
+  sum = group_sum(sum, lds);
+  if (threadIdx.x == 0) d.partial[unit] = sum;
+}
+
+__device__ __forceinline__ void store_parts(tam_f16* high, int64_t low, const float (&v)[8]) {
+  float h[8], r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // The fp32 value itself: the compiler otherwise rounds a product that v is
+    // straight to fp16 for one of its uses (v_fma_mixlo_f16) and by way of fp32
+    // for the other, and where the two differ, high + low is off by high's last bit.
+    float x = v[j];
+    asm("" : "+v"(x));
+    h[j] = (float)(tam_f16)x;
+    r[j] = x - h[j];  // exact
+  }
+  tam_store8(high, h);
+  if (low) tam_store8(high + low, r);
+}
+
+// x = u / max(|u|, eps) times 2^12, in parts.  A unit is 2048 elements of x's
+// rows of ldx; the columns past the matrix are zeros.
+constexpr uint32_t kStart = 2048;
+
+__global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
+  __shared__ float lds[4];
+  const mat& d = l.m[owner<START>(l, blockIdx.x)];
+  float sum = 0.f;
+  for (uint32_t i = threadIdx.x; i < d.partials; i += kThreads) sum += d.partial[i];
+  const float norm = sqrtf(group_sum(sum, lds)), scale = kScale / (norm < d.eps ? d.eps : norm);
+  const uint64_t at = (uint64_t)(blockIdx.x - d.first[START]) * kStart + threadIdx.x * 8u;
+  if (at >= (uint64_t)d.rows * d.ldx) return;
+  const uint32_t row = (uint32_t)(at / d.ldx), col = (uint32_t)(at - (uint64_t)row * d.ldx);
+  const uint32_t count = d.cols - col < 8 ? d.cols - col : 8u;
+  const uint64_t from = (uint64_t)row * d.cols + col;
+  float g[8], m[8] = {}, u[8];
+  load_grad(d, from, count, g);
+  if (d.momentum) load_f32(d.momentum + from, count, m);
+  direction(d, g, m, u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u[j] *= scale;
+  store_parts(d.x[0] + at, d.x_low, u);
+}
+
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ tam_operand operand(const tam_f16* p, uint32_t ld, uint32_t count) {
+  return {reinterpret_cast<const char*>(p), (uint64_t)ld * 2u, count};
+}
+
+struct coefficients {
+  float a, b, c;
+};
+
+// Tile t of the lower triangle, row by row: rows m, columns n <= m.
+__device__ __forceinline__ void triangle(uint32_t t, uint32_t& m, uint32_t& n) {
+  m = (uint32_t)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+  while (m * (m + 1) / 2 > t) --m;
+  while ((m + 1) * (m + 2) / 2 <= t) ++m;
+  n = t - m * (m + 1) / 2;
+}
+
+// GRAM: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q.
+template <int TILE, int WM, int WN, bool GRAM>
+__global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 4)) void tam_k_mu_square(
+    list l, uint32_t turn, coefficients co) {
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, true, true> Rows;
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, false, false> Columns;
+  __shared__ __attribute__((aligned(16))) char smem[Rows::LDS > Columns::LDS ? Rows::LDS : Columns::LDS];
+  const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
+  const mat& d = l.m[owner<SQUARE>(l, unit)];
+  uint32_t tm, tn;
+  triangle(unit - d.first[SQUARE], tm, tn);
+  const uint32_t r0 = tm * TILE, c0 = tn * TILE;
+  auto finish = [&](auto& t) {
+    tam_f16* out = GRAM ? d.q : d.p;
+    t.each(
+        smem,
+        [&](uint32_t row, uint32_t col, float(&v)[8]) {
+          row += r0;
+          col += c0;
+          if (row >= d.s || col >= d.lds) return;
+          const uint64_t at = (uint64_t)row * d.lds + col;
+          if constexpr (GRAM) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
+          } else {
+            float q[8];
+            tam_load8(d.q + at, q);
+            if (d.s_low) {
+              float r[8];
+              tam_load8(d.q + at + d.s_low, r);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) q[j] += r[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(co.b, q[j], co.c / kScale * v[j]);
+            if (row - col < 8) {
+#pragma unroll
+              for (uint32_t j = 0; j < 8; ++j)
+                if (row - col == j) {
+                  v[j] += co.a * kScale;
+                  d.diag[row] = v[j] * (1.f / kScale);
+                }
+            }
+          }
+          store_parts(out + at, d.s_low, v);
+        },
+        [&](uint32_t row, uint32_t col, const float* turned, int pitch) {
+          // off the diagonal, the mirrored tile: element (row, col) also goes to (col, row)
+          if (tm == tn) return;
+          typedef typename std::remove_reference<decltype(t)>::type Tile;
+          const int lane = threadIdx.x & 63;
+          // a lane takes 8 rows of one column: 4 lanes to a column's 32 rows
+#pragma unroll 1
+          for (int c = lane >> 2; c < Tile::COLS; c += 16) {
+            const uint32_t to_row = c0 + col + c, to_col = r0 + row + (lane & 3) * 8;
+            if (to_row >= d.s || to_col >= d.lds) continue;
+            const uint64_t at = (uint64_t)to_row * d.lds + to_col;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = turned[((lane & 3) * 8 + j) * pitch + c];
+            if constexpr (GRAM) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
+            } else {
+              float q[8];
+              tam_load8(d.q + at, q);
+              if (d.s_low) {
+                float r[8];
+                tam_load8(d.q + at + d.s_low, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] += r[j];
+              }
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(co.b, q[j], co.c / kScale * v[j]);
+            }
+            store_parts(out + at, d.s_low, v);
+          }
+        });
+  };
+  if (GRAM && d.tall) {
+    Columns t;
+    t.zero();
+    const tam_operand x = operand(d.x[turn], d.ldx, d.ldx);
+    t.template run<true>(x, x, c0, r0, 0, d.rows, smem, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
+    finish(t);
+  } else {
+    Rows t;
+    t.zero();
+    const tam_operand x = GRAM ? operand(d.x[turn], d.ldx, d.rows) : operand(d.q, d.lds, d.s);
+    const int64_t low = (GRAM ? d.x_low : d.s_low) * 2;
+    t.template run<true>(x, x, c0, r0, 0, GRAM ? d.ldx : d.lds, smem, {d.split ? 3u : 1u, low, low});
+    finish(t);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t col, float (&v)[8]) {
+  T* out = static_cast<T*>(d.out) + (uint64_t)row * d.cols + col;
+  const bool update = d.flags & TAM_MATRIX_UPDATE;
+  if (col + 8 <= d.cols) {
+    if (update) {
+      float p[8];
+      tam_load8(out, p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(-d.rate, v[j], d.decay * p[j]);
+    }
+    tam_store8(out, v);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (col + j < d.cols)
+        out[j] = tam_from_f<T>(update ? __builtin_fmaf(-d.rate, v[j], d.decay * tam_to_f(out[j])) : v[j]);
+  }
+}
+
+// x' = p x (tall: x p); LAST: the output instead.
+template <int TILE, int WM, int WN, bool LAST>
+__global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 4)) void tam_k_mu_apply(list l,
+                                                                                                       uint32_t turn) {
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, false, true> Wide;
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, true, true> Tall;
+  __shared__ __attribute__((aligned(16))) char smem[Wide::LDS > Tall::LDS ? Wide::LDS : Tall::LDS];
+  const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
+  const mat& d = l.m[owner<APPLY>(l, unit)];
+  uint32_t tm, tn;
+  tam_tile_at(unit - d.first[APPLY], (d.rows + TILE - 1) / TILE, (d.cols + TILE - 1) / TILE, tm, tn);
+  const uint32_t r0 = tm * TILE, c0 = tn * TILE;
+  const tam_f16* x = d.x[turn];
+  auto finish = [&](auto& t) {
+    t.each(
+        smem,
+        [&](uint32_t row, uint32_t col, float(&v)[8]) {
+          row += r0;
+          col += c0;
+          if (row >= d.rows || col >= d.cols) return;
+          const uint64_t at = (uint64_t)row * d.ldx + col;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
+          if (!d.split) {
+            float r[8];
+            tam_load8(x + at + d.x_low, r);
+            if (d.tall) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (col + j < d.cols) v[j] = __builtin_fmaf(d.diag[col + j], r[j], v[j]);
+            } else {
+              const float p = d.diag[row];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(p, r[j], v[j]);
+            }
+          }
+          if constexpr (LAST) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
+            if (d.dtype == TAM_DTYPE_F32)
+              write_out<float>(d, row, col, v);
+            else if (d.dtype == TAM_DTYPE_BF16)
+              write_out<tam_bf16>(d, row, col, v);
+            else
+              write_out<tam_f16>(d, row, col, v);
+          } else {
+            store_parts(d.x[turn ^ 1u] + at, d.x_low, v);
+          }
+        },
+        [](uint32_t, uint32_t, const float*, int) {});
+  };
+  const tam_operand p = operand(d.p, d.lds, d.s);
+  const uint32_t terms = d.split ? 3u : 1u;
+  if (d.tall) {
+    Tall t;
+    t.zero();
+    t.template run<true>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.lds, smem, {terms, d.s_low * 2, d.x_low * 2});
+    finish(t);
+  } else {
+    Wide t;
+    t.zero();
+    t.template run<true>(operand(x, d.ldx, d.ldx), p, c0, r0, 0, d.rows, smem, {terms, d.x_low * 2, d.s_low * 2});
+    finish(t);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct plan {
+  std::vector<mat> m;
+  uint64_t bytes;
+  int tile[PHASES];
+  uint32_t units[PHASES];
+};
+
+int check(const TamMatrix* m, int n) {
+  tam_op_begin();
+  if (n < 0 || (n > 0 && !m)) return tam_op_fail(TAM_E_INVALID, "null argument");
+  for (int i = 0; i < n; ++i) {
+    const TamMatrix& d = m[i];
+    if (!d.out || !d.grad) return tam_op_fail(TAM_E_INVALID, "matrix %d: null out or grad", i);
+    if (!d.rows || !d.cols) return tam_op_fail(TAM_E_INVALID, "matrix %d has no elements", i);
+    if (d.rows > kMostSide || d.cols > kMostSide)
+      return tam_op_fail(TAM_E_UNSUPPORTED, "matrix %d: a side of more than %llu", i, (unsigned long long)kMostSide);
+    if (d.dtype > TAM_DTYPE_F16) return tam_op_fail(TAM_E_INVALID, "matrix %d: unknown dtype %u", i, d.dtype);
+    if (!(d.eps > 0.f)) return tam_op_fail(TAM_E_INVALID, "matrix %d: eps must be above 0", i);
+    if ((uintptr_t)d.momentum & 3u) return tam_op_fail(TAM_E_INVALID, "matrix %d: misaligned momentum", i);
+  }
+  return TAM_OK;
+}
+
+uint64_t tiles(uint64_t rows, uint64_t cols, int t) { return tam_div_up(rows, t) * tam_div_up(cols, t); }
+uint64_t triangle_tiles(uint64_t s, int t) { return tam_div_up(s, t) * (tam_div_up(s, t) + 1) / 2; }
+
+// The tile of a phase: the time of a launch is about the work of its tiles at
+// the rate that their size reaches, over the compute units, in whole rounds.
+int pick_tile(const std::vector<mat>& m, bool square) {
+  const double cus = tam_op_cus();
+  const struct {
+    int tile;
+    double rate, start;
+  } kind[3] = {{256, 1000.0, 4.0}, {128, 700.0, 2.5}, {64, 350.0, 1.5}};
+  int best = 64;
+  double least = 1e30;
+  for (const auto& t : kind) {
+    double work = 0, longest = 0;  // us of one compute unit
+    for (const mat& d : m) {
+      // q's sum runs over the longer side, p's and x's over the shorter one
+      const double k = (square ? std::max(d.rows, d.cols) : d.s) * (d.split ? 3.0 : 1.0);
+      const double one = 2.0 * t.tile * t.tile * k * cus / (t.rate * 1e6) + t.start;
+      work += one * (double)(square ? triangle_tiles(d.s, t.tile) : tiles(d.rows, d.cols, t.tile));
+      longest = std::max(longest, one);
+    }
+    const double us = std::max(longest, work / cus) + (work / cus > longest ? longest * 0.5 : 0.0);
+    if (us < least) {
+      least = us;
+      best = t.tile;
+    }
+  }
+  return best;
+}
+
+// Lays the list out: the largest sums first, so that no long tile starts last.
+int make(const TamMatrix* in, int n, char* base, plan& out) {
+  std::vector<int> order(n);
+  for (int i = 0; i < n; ++i) order[i] = i;
+  auto larger = [&](int i) { return std::max(in[i].rows, in[i].cols); };
+  std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return larger(i) > larger(j); });
+  out.m.resize(n);
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    char* p = (char*)((uintptr_t)base + at);
+    at += tam_up(bytes, 256);
+    return p;
+  };
+  take((uint64_t)n * sizeof(mat));
+  for (int k = 0; k < n; ++k) {
+    const TamMatrix& d = in[order[k]];
+    mat& m = out.m[k];
+    m = mat{};
+    m.out = d.out;
+    m.grad = d.grad;
+    m.momentum = d.momentum;
+    m.rows = (uint32_t)d.rows;
+    m.cols = (uint32_t)d.cols;
+    m.elements = d.rows * d.cols;
+    m.tall = d.rows > d.cols;
+    m.s = m.tall ? m.cols : m.rows;
+    m.ldx = (uint32_t)tam_up(d.cols, 8);
+    m.lds = (uint32_t)tam_up(m.s, 8);
+    m.dtype = d.dtype;
+    m.flags = d.flags;
+    m.split = d.dtype != TAM_DTYPE_BF16;
+    m.keep = d.keep;
+    m.one_minus_keep = d.one_minus_keep;
+    m.eps = d.eps;
+    m.decay = d.decay;
+    m.rate = d.rate;
+    m.x_low = (int64_t)tam_up((uint64_t)m.rows * m.ldx, 128);
+    const int64_t square = (int64_t)tam_up((uint64_t)m.s * m.lds, 128);
+    m.s_low = m.split ? square : 0;
+    for (int i = 0; i < 2; ++i) m.x[i] = (tam_f16*)take(m.x_low * 4);
+    m.q = (tam_f16*)take(square * (m.split ? 4 : 2));
+    m.p = (tam_f16*)take(square * (m.split ? 4 : 2));
+    m.diag = (float*)take((uint64_t)m.s * 4);
+    m.chunk = (uint32_t)tam_up(tam_div_up(m.elements, kMostPartials), kThreads * 8);
+    m.partials = (uint32_t)tam_div_up(m.elements, m.chunk);
+    m.partial = (float*)take((uint64_t)m.partials * 4);
+  }
+  out.bytes = at;
+  out.tile[SQUARE] = pick_tile(out.m, true);
+  out.tile[APPLY] = pick_tile(out.m, false);
+  uint64_t units[PHASES] = {};
+  for (mat& m : out.m) {
+    for (int f = 0; f < PHASES; ++f) m.first[f] = (uint32_t)units[f];
+    units[MOMENTUM] += m.partials;
+    units[START] += tam_div_up((uint64_t)m.rows * m.ldx, kStart);
+    units[SQUARE] += triangle_tiles(m.s, out.tile[SQUARE]);
+    units[APPLY] += tiles(m.rows, m.cols, out.tile[APPLY]);
+  }
+  for (int f = 0; f < PHASES; ++f) {
+    if (units[f] >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "matrices of too many elements for one call");
+    out.units[f] = (uint32_t)units[f];
+  }
+  return TAM_OK;
+}
+
+template <bool GRAM>
+void launch_square(int tile, const list& l, uint32_t turn, coefficients co, hipStream_t s) {
+  const dim3 grid(l.units[SQUARE]);
+  if (tile == 256)
+    hipLaunchKernelGGL((tam_k_mu_square<256, 2, 4, GRAM>), grid, dim3(512), 0, s, l, turn, co);
+  else if (tile == 128)
+    hipLaunchKernelGGL((tam_k_mu_square<128, 2, 2, GRAM>), grid, dim3(256), 0, s, l, turn, co);
+  else
+    hipLaunchKernelGGL((tam_k_mu_square<64, 2, 2, GRAM>), grid, dim3(256), 0, s, l, turn, co);
+}
+
+template <bool LAST>
+void launch_apply(int tile, const list& l, uint32_t turn, hipStream_t s) {
+  const dim3 grid(l.units[APPLY]);
+  if (tile == 256)
+    hipLaunchKernelGGL((tam_k_mu_apply<256, 2, 4, LAST>), grid, dim3(512), 0, s, l, turn);
+  else if (tile == 128)
+    hipLaunchKernelGGL((tam_k_mu_apply<128, 2, 2, LAST>), grid, dim3(256), 0, s, l, turn);
+  else
+    hipLaunchKernelGGL((tam_k_mu_apply<64, 2, 2, LAST>), grid, dim3(256), 0, s, l, turn);
+}
+
+int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* workspace, size_t ws_bytes,
+                  hipStream_t s, size_t* need) {
+  int rc = check(in, n);
+  if (rc != TAM_OK) return rc;
+  plan p;
+  p.bytes = 0;
+  if (n) rc = make(in, n, (char*)workspace, p);
+  if (rc != TAM_OK) return rc;
+  if (need) {
+    *need = (size_t)p.bytes;
+    return TAM_OK;
+  }
+  if (!c) return tam_op_fail(TAM_E_INVALID, "null argument");
+  if (!(fabsf(c[0]) < 64.f && fabsf(c[1]) < 64.f && fabsf(c[2]) < 64.f))
+    return tam_op_fail(TAM_E_INVALID, "a coefficient of 64 or more, or none");
+  if (steps < 1 || steps > 64) return tam_op_fail(TAM_E_INVALID, "steps must be 1 to 64");
+  if (n == 0) return TAM_OK;
+  if (p.bytes > ws_bytes || !workspace)
+    return tam_op_fail(TAM_E_WORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes,
+                       (unsigned long long)p.bytes);
+  if ((uintptr_t)workspace & 255u) return tam_op_fail(TAM_E_INVALID, "workspace not on 256 bytes");
+  mat* table = (mat*)workspace;
+  for (int i = 0; i < n; i += kPut) {
+    put_args a;
+    const int k = n - i < kPut ? n - i : kPut;
+    for (int j = 0; j < kPut; ++j) a.m[j] = j < k ? p.m[i + j] : mat{};
+    hipLaunchKernelGGL(tam_k_mu_put, dim3(1), dim3(256), 0, s, a, table + i, (uint32_t)k);
+    TAM_OP_LAUNCHED("the descriptors");
+  }
+  list l = {table, (uint32_t)n, {}};
+  for (int f = 0; f < PHASES; ++f) l.units[f] = p.units[f];
+  hipLaunchKernelGGL(tam_k_mu_momentum, dim3(l.units[MOMENTUM]), dim3(kThreads), 0, s, l);
+  TAM_OP_LAUNCHED("the momentum");
+  hipLaunchKernelGGL(tam_k_mu_start, dim3(l.units[START]), dim3(kThreads), 0, s, l);
+  TAM_OP_LAUNCHED("the normalisation");
+  const coefficients co = {c[0], c[1], c[2]};
+  for (int i = 0; i < steps; ++i) {
+    const uint32_t turn = i & 1;
+    launch_square<true>(p.tile[SQUARE], l, turn, co, s);
+    TAM_OP_LAUNCHED("the Gram product");
+    launch_square<false>(p.tile[SQUARE], l, turn, co, s);
+    TAM_OP_LAUNCHED("the polynomial");
+    if (i + 1 < steps)
+      launch_apply<false>(p.tile[APPLY], l, turn, s);
+    else
+      launch_apply<true>(p.tile[APPLY], l, turn, s);
+    TAM_OP_LAUNCHED("the polynomial's product");
+  }
+  return TAM_OK;
+}
+
+// No exception leaves the library: the plan's memory is all that can fail.
+int guarded(const TamMatrix* in, int n, const float* c, int steps, void* ws, size_t bytes, hipStream_t s,
+            size_t* need) {
+  try {
+    return orthogonalize(in, n, c, steps, ws, bytes, s, need);
+  } catch (const std::bad_alloc&) {
+    return tam_op_fail(TAM_E_INVALID, "no host memory for %d matrices", n);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes) {
+  if (!bytes) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  return guarded(matrices, n, nullptr, 0, nullptr, 0, nullptr, bytes);
+}
+
+int tam_orthogonalize(const TamMatrix* matrices, int n, const float* coefficients, int steps, void* workspace,
+                      size_t ws_bytes, void* stream) {
+  return guarded(matrices, n, coefficients, steps, workspace, ws_bytes, (hipStream_t)stream, nullptr);
+}
+
+}  // extern "C"

@@ -51,13 +51,6 @@ typedef __bf16 tam_bf16;
 typedef _Float16 tam_f16;
 typedef float tam_f4 __attribute__((ext_vector_type(4)));
 
-// N elements that may lie at any element's address (gfx950 moves 16 bytes at
-// any address; the claimed alignment is the element's own).
-template <typename T, int N>
-struct tam_pack {
-  T v[N];
-};
-
 template <typename T>
 __device__ __forceinline__ float tam_to_f(T x) {
   return (float)x;
@@ -68,13 +61,11 @@ __device__ __forceinline__ T tam_from_f(float x) {
 }
 
 // 8 consecutive elements at p to fp32 and back, 16 (32 for fp32) bytes at once.
+// They may lie at any element's address: gfx950 moves 16 bytes at any address,
+// and the alignment claimed to the compiler is the element's own.
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) tam_oct {
   T v __attribute__((ext_vector_type(8)));
-};
-template <>
-struct __attribute__((packed, aligned(2))) tam_oct<tam_bf16> {
-  tam_bf16 v __attribute__((ext_vector_type(8)));
 };
 
 template <typename T>
@@ -91,11 +82,24 @@ __device__ __forceinline__ void tam_store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<tam_oct<T>*>(p) = o;
 }
 
-// Sum over the wave's 64 lanes; every lane gets it.
+// Sum over the wave's 64 lanes; every lane gets the same bits.
+template <int CTRL>
+__device__ __forceinline__ float tam_dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float tam_wave_sum(float x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
+  x = tam_dpp_add<0xb1>(x);   // quad_perm [1, 0, 3, 2]
+  x = tam_dpp_add<0x4e>(x);   // quad_perm [2, 3, 0, 1]
+  x = tam_dpp_add<0x141>(x);  // row_half_mirror
+  x = tam_dpp_add<0x140>(x);  // row_mirror
+  const uint32_t i = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
+  const uint32_t j = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(j, j, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
 }
 
 #endif  // TAM_OPS_H

@@ -164,3 +164,85 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None, *, 
     if _need(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act)
     return _linear_forward(x, weight, bias, residual, act, False)[0]
+
+
+# -------------------------------------------------------------- layer norm
+_MOST_NORM = 32768  # elements of a row the kernels take (include/turboadam_amd.h)
+
+
+def _norm_operands(x, weight, bias, eps):
+    d = _lib.TamNorm()
+    n = x.shape[-1]
+    x2, ldx = _rows(x, n)
+    weight = None if weight is None else _plain(weight)
+    bias = None if bias is None else _plain(bias)
+    d.x, d.w, d.b = x2.data_ptr(), _ptr(weight), _ptr(bias)
+    d.rows, d.n, d.ldx, d.dtype, d.eps = x2.shape[0], n, ldx, _lib.DTYPES[x.dtype], eps
+    return d, (x2, weight, bias)
+
+
+def _norm_forward(x, weight, bias, eps, keep):
+    lib = _lib.load()
+    d, operands = _norm_operands(x, weight, bias, eps)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((d.rows, 2), dtype=torch.float32, device=x.device) if keep else None
+    d.y, d.stats = y.data_ptr(), _ptr(stats)
+    with torch.cuda.device(x.device):
+        _lib.check(lib.tam_norm(ctypes.byref(d), _lib.stream_of(x.device)), "tam_norm")
+    del operands
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.eps = eps
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        lib = _lib.load()
+        d, operands = _norm_operands(x, weight, None, ctx.eps)
+        n, dev = x.shape[-1], x.device
+        g = _plain(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        dw = torch.empty(n, dtype=x.dtype, device=dev) if need_w else None
+        db = torch.empty(n, dtype=x.dtype, device=dev) if need_b else None
+        d.dy, d.stats, d.dx, d.dw, d.db = g.data_ptr(), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db)
+        with torch.cuda.device(dev):
+            need = ctypes.c_size_t()
+            _lib.check(lib.tam_norm_workspace(ctypes.byref(d), 1, ctypes.byref(need)), "tam_norm_workspace")
+            ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+            _lib.check(lib.tam_norm_backward(ctypes.byref(d), _ptr(ws), need.value, _lib.stream_of(dev)),
+                       "tam_norm_backward")
+        del operands
+        return dx, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor = None, *,
+               eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension.
+
+    x (..., n) with n at most 32768, weight and bias (n) or None, all of one
+    dtype.  The mean and the variance (the mean squared distance from the mean)
+    are fp32 sums over a row held in registers, kept in fp32 for the backward
+    pass, which gives the gradients of x, weight and bias; those of weight and
+    bias are summed over the rows in a fixed order."""
+    _check("layer_norm", x, (("weight", weight), ("bias", bias)))
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MOST_NORM:
+        raise ValueError(f"turboadam_amd.layer_norm: x must have rows of 1 to {_MOST_NORM} elements, got "
+                         f"{tuple(x.shape)}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.shape != x.shape[-1:]:
+            raise ValueError(f"turboadam_amd.layer_norm: {name} must have shape ({x.shape[-1]},), got "
+                             f"{tuple(t.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"turboadam_amd.layer_norm: eps must be 0 or more, got {eps}")
+    if _need(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _norm_forward(x, weight, bias, float(eps), False)[0]
