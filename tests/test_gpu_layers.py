@@ -1,0 +1,394 @@
+"""GPU: linear and layer_norm with their gradients against the formulas in 64
+bits, element by element.
+
+Bounds (fixed before the first run).  u: the dtype's rounding (2^-24, 2^-8,
+2^-11); a sum of n products in fp32 is off by at most (n + 16) 2^-23 times the
+sum of their absolute values, whatever its order; elementary functions by 2^-20
+of their result.  The backward pass of an activation sees z rounded once and
+rounds dz once; the activations' second derivatives are below 1.2."""
+
+import math
+import zlib
+
+import pytest
+import torch
+
+from tests.helpers import log
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+UNIT = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+TINY = {"f32": 1e-37, "bf16": 1e-37, "f16": 2.0 ** -24}  # fp16's smallest numbers
+F = torch.nn.functional
+ACT = {None: lambda z: z, "relu": torch.relu, "gelu": F.gelu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"),
+       "silu": F.silu}
+
+
+def _gen(*key):
+    return torch.Generator(device="cuda").manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def _sum_error(n):
+    return (n + 16) * 2.0 ** -23
+
+
+def _within(got, want, bound, what):
+    got, want = got.detach().double(), want.double()
+    assert got.shape == want.shape, what
+    over = (got - want).abs() > bound
+    assert not bool(over.any()) and bool(torch.isfinite(got).all()), (
+        f"{what}: {int(over.sum())} of {over.numel()} over the bound, worst {float(((got - want).abs() - bound).max())}")
+
+
+# ------------------------------------------------------------------ linear
+def _linear_case(m, k, n, dt, act, bias, residual, in_out, integers=False):
+    g, d = _gen(m, k, n, dt, act), DTYPES[dt]
+
+    def rand(*shape):
+        if integers:
+            return torch.randint(-3, 4, shape, generator=g, device="cuda").to(d)
+        return torch.randn(shape, generator=g, device="cuda").to(d)
+
+    x = rand(m, k)
+    w = rand(k, n) if in_out else rand(n, k)
+    if not integers:
+        w = w * max(k, 1) ** -0.5
+    w = w.t() if in_out else w
+    return x, w, rand(n) if bias else None, rand(m, n) if residual else None, rand(m, n)
+
+
+def _check_linear(x, w, b, r, dy, dt, act):
+    from turboadam_amd import linear
+
+    m, n, k, u, t = x.shape[0], w.shape[0], x.shape[1], UNIT[dt], TINY[dt]
+    args = [v for v in (x, w, b, r) if v is not None]
+    leaves = [v.detach().requires_grad_() for v in args]
+    it = iter(leaves)
+    xl, wl, bl, rl = next(it), next(it), next(it) if b is not None else None, next(it) if r is not None else None
+    y = linear(xl, wl, bl, activation=act, residual=rl)
+    assert y.dtype == x.dtype and y.shape == (m, n)
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        assert torch.equal(linear(x, w, b, activation=act, residual=r), y)  # the call without gradients
+    X, W, DY = x.double(), w.double(), dy.double()
+    z = X @ W.t() + (0 if b is None else b.double())
+    z_err = _sum_error(k) * (X.abs() @ W.abs().t() + (0 if b is None else b.double().abs()))
+    z.requires_grad_()
+    a = ACT[act](z)
+    slope = torch.autograd.grad(a.sum(), z)[0]
+    z, a = z.detach(), a.detach()
+    ref = a + (0 if r is None else r.double())
+    smooth = 0.0 if act is None else 2.0 ** -20
+    _within(y, ref, u * ref.abs() + (1 + u) * (1.2 * z_err + smooth * (a.abs() + z.abs())
+                                               + 2.0 ** -23 * ref.abs()) + t, "y")
+    if act is None:
+        dz, dz_err = DY, torch.zeros_like(DY)
+    else:
+        dz = DY * slope
+        seen = 0.0 if act == "relu" else 1.2 * (z_err + u * z.abs() + t)
+        dz_err = DY.abs() * (seen + smooth) * (1 + u) + u * dz.abs() + t
+    # the bias's gradient is summed before dz is rounded; the bound with its rounding holds too
+    want = {"dx": (dz @ W, dz_err @ W.abs() + _sum_error(n) * (dz.abs() @ W.abs())),
+            "dw": (dz.t() @ X, dz_err.t() @ X.abs() + _sum_error(m) * (dz.abs().t() @ X.abs()))}
+    if b is not None:
+        want["db"] = (dz.sum(0), dz_err.sum(0) + _sum_error(m) * dz.abs().sum(0))
+    for (name, (v, err)), got in zip(want.items(), grads):
+        _within(got, v, u * v.abs() + (1 + u) * err + t, name)
+    if r is not None:
+        assert torch.equal(grads[-1], dy)
+    assert grads[1].stride() == w.stride() or 1 in w.shape
+
+
+SHAPES = [(1, 1, 1), (1, 64, 16), (2, 4096, 130), (7, 33, 5), (16, 1000, 17), (32, 129, 64), (33, 64, 64),
+          (64, 64, 64), (100, 200, 300), (129, 257, 65), (255, 40, 1), (260, 512, 264), (1, 3, 1000), (700, 8, 12),
+          (40, 8192, 72), (1100, 520, 776)]
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_linear_and_gradients(m, k, n, dt):
+    for act, bias, residual, in_out in [(None, False, False, False), ("gelu", True, True, True),
+                                        ("silu", True, False, False), ("gelu_tanh", False, True, True),
+                                        (None, True, True, True)]:
+        log(f"linear {m}x{k}x{n} {dt} {act} bias={bias} residual={residual} in_out={in_out}")
+        _check_linear(*_linear_case(m, k, n, dt, act, bias, residual, in_out), dt, act)
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_linear_relu_of_whole_numbers(dt):
+    # small whole numbers: z is exact, and its slope at 0 is 0 on both sides
+    log(f"linear relu {dt}")
+    _check_linear(*_linear_case(200, 24, 130, dt, "relu", True, True, False, integers=True), dt, "relu")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_linear_large_tiles_and_split_sums(dt):
+    # many tiles of the largest size, and few tiles of a long sum
+    for m, k, n in [(2048, 512, 2304), (96, 16384, 160), (2050, 1030, 1030)]:
+        log(f"linear {m}x{k}x{n} {dt}")
+        _check_linear(*_linear_case(m, k, n, dt, "gelu", True, True, False), dt, "gelu")
+
+
+def test_linear_views_strides_and_leading_dimensions():
+    from turboadam_amd import linear
+
+    g = _gen("views")
+    base = torch.randn(6, 50, 96, generator=g, device="cuda").bfloat16()
+    w = torch.randn(70, 96, generator=g, device="cuda").bfloat16()
+    b = torch.randn(140, generator=g, device="cuda").bfloat16()
+    whole = linear(base.reshape(300, 96), w, b[:70]).reshape(6, 50, 70)
+    log("linear on leading dimensions")
+    assert torch.equal(linear(base, w, b[:70]), whole)
+    log("linear on strided rows, an odd offset and every other bias element")
+    wide = torch.zeros(300, 131, device="cuda", dtype=torch.bfloat16)
+    wide[:, 3:99] = base.reshape(300, 96)
+    assert torch.equal(linear(wide[:, 3:99], w, b[:70]), whole.reshape(300, 70))
+    far = torch.zeros(70, 200, device="cuda", dtype=torch.bfloat16)
+    far[:, 8:104] = w
+    assert torch.equal(linear(base, far[:, 8:104], b[:70]), whole)
+    every = torch.zeros(96, 2, device="cuda", dtype=torch.bfloat16)
+    every[:, 0] = base[0, 0]
+    assert torch.equal(linear(every[:, 0], w), linear(base[0, 0], w))
+    log("linear on a transposed input, an expanded one and a broadcast residual")
+    t = base.reshape(300, 96).t().contiguous().t()
+    assert torch.equal(linear(t, w), linear(base.reshape(300, 96), w))
+    row = base[0, :1].expand(300, 96)
+    assert torch.equal(linear(row, w, residual=b[:70].expand(300, 70)),
+                       linear(row.contiguous(), w, residual=b[:70].expand(300, 70).contiguous()))
+
+
+def test_linear_gradient_of_a_broadcast_input():
+    from turboadam_amd import linear
+
+    g = _gen("broadcast")
+    x = torch.randn(1, 64, generator=g, device="cuda").requires_grad_()
+    w = torch.randn(48, 64, generator=g, device="cuda").requires_grad_()
+    r = torch.randn(48, generator=g, device="cuda").requires_grad_()
+    dy = torch.randn(40, 48, generator=g, device="cuda")
+    dx, dw, dr = torch.autograd.grad(linear(x.expand(40, 64), w, residual=r.expand(40, 48)), (x, w, r), dy)
+    D = dy.double()
+    assert torch.allclose(dx.double(), (D @ w.double()).sum(0, keepdim=True), rtol=1e-5, atol=1e-4)
+    assert torch.allclose(dw.double(), D.t() @ x.double().expand(40, 64), rtol=1e-5, atol=1e-4)
+    assert torch.allclose(dr.double(), D.sum(0), rtol=1e-5, atol=1e-4)
+
+
+@pytest.mark.parametrize("m,k,n", [(0, 8, 8), (5, 0, 9), (40, 0, 9), (5, 8, 0), (40, 8, 0), (0, 0, 4)])
+def test_linear_empty_sizes(m, k, n):
+    from turboadam_amd import linear
+
+    log(f"linear {m}x{k}x{n}")
+    x = torch.ones(m, k, device="cuda", requires_grad=True)
+    w = torch.ones(n, k, device="cuda", requires_grad=True)
+    b = torch.full((n,), 2.0, device="cuda", requires_grad=True)
+    y = linear(x, w, b, activation="relu")
+    assert y.shape == (m, n) and bool((y == k + 2).all())
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert bool((dx == n).all()) and bool((dw == m).all()) and bool((db == m).all())
+    assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
+
+
+@pytest.mark.parametrize("rows", [3, 80])
+def test_linear_infinities_and_nan_stay_in_their_rows(rows):
+    from turboadam_amd import linear
+
+    x = torch.ones(rows, 72, device="cuda")
+    x[1, 5], x[2, 71] = math.inf, math.nan
+    w = torch.ones(40, 72, device="cuda")
+    for act in (None, "relu", "gelu", "silu", "gelu_tanh"):
+        y = linear(x, w, activation=act)
+        assert bool((y[1] == math.inf).all()) and bool(y[2].isnan().all()), act
+        assert bool(y[0].isfinite().all()) and bool(y[3:].isfinite().all()), act
+    assert bool((linear(-x, w, activation="relu")[1] == 0).all())
+
+
+def test_linear_gradient_against_differences():
+    """fp32 directional derivatives by central differences in 64 bits of the same function of the outputs."""
+    from turboadam_amd import linear
+
+    g = _gen("differences")
+    for act in ("gelu", "gelu_tanh", "silu"):
+        leaves = [torch.randn(s, generator=g, device="cuda") for s in ((50, 40), (30, 40), (30,), (50, 30))]
+        leaves[1] *= 40 ** -0.5
+        dy = torch.randn(50, 30, generator=g, device="cuda")
+        x, w, b, r = [v.clone().requires_grad_() for v in leaves]
+        grads = torch.autograd.grad(linear(x, w, b, activation=act, residual=r), (x, w, b, r), dy)
+
+        def value(x, w, b, r):
+            return ((ACT[act](x @ w.t() + b) + r) * dy.double()).sum()
+
+        for i, grad in enumerate(grads):
+            step = torch.randn(leaves[i].shape, generator=g, device="cuda", dtype=torch.float64)
+            at = [v.double() for v in leaves]
+            up, down = list(at), list(at)
+            up[i], down[i] = at[i] + 1e-5 * step, at[i] - 1e-5 * step
+            want = (value(*up) - value(*down)) / 2e-5
+            scale = float(grad.double().norm() * step.norm())
+            assert abs(float((grad.double() * step).sum() - want)) < 1e-5 * scale, (act, i)
+
+
+def test_linear_same_bits_every_time_and_on_another_stream():
+    from turboadam_amd import linear
+
+    x, w, b, r, dy = _linear_case(900, 1000, 264, "bf16", "gelu", True, True, False)
+    x, w, b = x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+
+    def call():
+        y = linear(x, w, b, activation="gelu", residual=r)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, b), dy)]
+
+    first = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = call()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, c in zip(first, second):
+        assert torch.equal(a, c)
+
+
+def test_layers_in_a_captured_graph():
+    from turboadam_amd import layer_norm, linear
+
+    x, w, b, r, dy = _linear_case(300, 264, 130, "bf16", "silu", True, True, False)
+    s = torch.ones(264, device="cuda", dtype=torch.bfloat16)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b, s)]
+
+    def call():
+        y = linear(layer_norm(leaves[0], leaves[3]), leaves[1], leaves[2], activation="silu", residual=r)
+        return [y, *torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(300, 264, generator=_gen(i), device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, call()):
+            assert torch.equal(a, c), f"replay {i}"
+
+
+# -------------------------------------------------------------- layer norm
+def _check_norm(x, w, b, dy, dt, eps=1e-5):
+    from turboadam_amd import layer_norm
+
+    u, t, n = UNIT[dt], TINY[dt], x.shape[-1]
+    leaves = [v.detach().requires_grad_() for v in (x, w, b) if v is not None]
+    it = iter(leaves)
+    y = layer_norm(next(it), next(it) if w is not None else None, next(it) if b is not None else None, eps=eps)
+    grads = torch.autograd.grad(y, leaves, dy)
+    X, DY = x.double(), dy.double()
+    W = torch.ones(n, device="cuda", dtype=torch.float64) if w is None else w.double()
+    c = X - X.mean(1, keepdim=True)
+    rstd = (c.square().mean(1, keepdim=True) + eps).rsqrt()
+    h = c * rstd
+    # the mean is off by mean_err, each distance by that and a rounding; rstd by the sum's
+    # error and what the distances' errors make of the variance
+    mean_err = _sum_error(n) * X.abs().mean(1, keepdim=True) + 2.0 ** -23 * X.mean(1, keepdim=True).abs()
+    c_err = mean_err + 2.0 ** -23 * c.abs()
+    rstd_rel = _sum_error(n) + 2.0 ** -20 + rstd.square() * (c.abs() * c_err + c_err.square()).mean(1, keepdim=True)
+    h_err = c_err * rstd + h.abs() * (rstd_rel + 2.0 ** -22)
+    y_ref = h * W + (0 if b is None else b.double())
+    _within(y, y_ref, u * y_ref.abs() + (1 + u) * (h_err * W.abs() + 2.0 ** -22 * ((h * W).abs() + y_ref.abs())) + t, "y")
+    T = DY * W
+    m0, m1 = T.mean(1, keepdim=True), (T * h).mean(1, keepdim=True)
+    dx = rstd * (T - m0 - h * m1)
+    m0_err = (_sum_error(n) + 2.0 ** -22) * T.abs().mean(1, keepdim=True)
+    m1_err = (_sum_error(n) + 2.0 ** -22) * (T * h).abs().mean(1, keepdim=True) + (T.abs() * h_err).mean(1, keepdim=True)
+    part = T.abs() + m0.abs() + (h * m1).abs()
+    dx_err = rstd * (m0_err + h.abs() * m1_err + h_err * (m1.abs() + m1_err) + (rstd_rel + 2.0 ** -20) * part)
+    _within(grads[0], dx, u * dx.abs() + (1 + u) * dx_err + t, "dx")
+    rows = x.shape[0]
+    if w is not None:
+        dw = (DY * h).sum(0)
+        err = (DY.abs() * h_err).sum(0) + _sum_error(rows) * (DY * h).abs().sum(0)
+        _within(grads[1], dw, u * dw.abs() + (1 + u) * err + t, "dweight")
+    if b is not None:
+        db = DY.sum(0)
+        _within(grads[-1], db, u * db.abs() + (1 + u) * _sum_error(rows) * DY.abs().sum(0) + t, "dbias")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 7), (1, 4096), (5, 512), (130, 513), (1000, 768), (17, 1013),
+                                    (300, 1500), (40, 4095), (33, 4097), (9, 8192), (7, 12001), (3, 16384),
+                                    (5, 20000), (2, 32768)])
+def test_layer_norm_and_gradients(rows, n, dt):
+    g, d = _gen(rows, n, dt), DTYPES[dt]
+    x = (torch.randn(rows, n, generator=g, device="cuda") * 2 + 1).to(d)
+    w = torch.randn(n, generator=g, device="cuda").to(d)
+    b = torch.randn(n, generator=g, device="cuda").to(d)
+    dy = torch.randn(rows, n, generator=g, device="cuda").to(d)
+    for use_w, use_b in ((True, True), (True, False), (False, True), (False, False)):
+        log(f"layer_norm {rows}x{n} {dt} weight={use_w} bias={use_b}")
+        _check_norm(x, w if use_w else None, b if use_b else None, dy, dt)
+
+
+def test_layer_norm_of_rows_far_from_zero_and_of_equal_elements():
+    g = _gen("far")
+    x = 1000 + torch.randn(20, 600, generator=g, device="cuda")
+    dy = torch.randn(20, 600, generator=g, device="cuda")
+    log("layer_norm of a large mean")
+    _check_norm(x, None, None, dy, "f32")
+    from turboadam_amd import layer_norm
+
+    log("layer_norm of equal elements")
+    flat = torch.full((4, 600), 3.0, device="cuda", requires_grad=True)
+    y = layer_norm(flat, eps=1e-5)
+    assert bool((y == 0).all())
+    assert bool(torch.autograd.grad(y.sum(), flat)[0].isfinite().all())
+
+
+def test_layer_norm_views_empty_rows_and_bad_rows():
+    from turboadam_amd import layer_norm
+
+    g = _gen("norm views")
+    x = torch.randn(3, 10, 131, generator=g, device="cuda").half()
+    whole = layer_norm(x[..., 2:99].contiguous())
+    log("layer_norm on strided rows and leading dimensions")
+    assert torch.equal(layer_norm(x[..., 2:99]), whole)
+    assert torch.equal(layer_norm(x[1, :, 2:99]), whole[1])
+    assert torch.equal(layer_norm(x[1, 4, 2:99]), whole[1, 4])
+    log("layer_norm of no rows")
+    none = torch.zeros(0, 40, device="cuda", requires_grad=True)
+    w = torch.ones(40, device="cuda", requires_grad=True)
+    dx, dw = torch.autograd.grad(layer_norm(none, w), (none, w), torch.zeros(0, 40, device="cuda"))
+    assert dx.shape == (0, 40) and bool((dw == 0).all())
+    log("layer_norm: a NaN or infinity stays in its row")
+    y = torch.randn(5, 97, generator=g, device="cuda")
+    good = layer_norm(y)
+    y[1, 3], y[3, 0] = math.nan, math.inf
+    bad = layer_norm(y)
+    assert bool(bad[1].isnan().all()) and bool(bad[3].isnan().all())
+    assert torch.equal(bad[[0, 2, 4]], good[[0, 2, 4]])
+
+
+def test_layers_refuse_what_they_cannot_take():
+    from turboadam_amd import layer_norm, linear
+
+    x = torch.ones(4, 8, device="cuda")
+    w = torch.ones(6, 8, device="cuda")
+    for args, kw, error, text in [
+        ((x.cpu(), w), {}, RuntimeError, "MI355X"), ((x, w.cpu()), {}, RuntimeError, "weight"),
+        ((x.double(), w.double()), {}, ValueError, "float32"), ((x, w.half()), {}, ValueError, "weight must be"),
+        ((x, w.t()), {}, ValueError, "inputs"), ((x, w[0]), {}, ValueError, "inputs"),
+        ((x, w, x[0]), {}, ValueError, "bias"), ((x, w), {"residual": x}, ValueError, "residual"),
+        ((x, w), {"activation": "tanh"}, ValueError, "activation"),
+    ]:
+        with pytest.raises(error, match=text):
+            linear(*args, **kw)
+    for args, kw, error, text in [
+        ((x.cpu(),), {}, RuntimeError, "MI355X"), ((x, w[0].half()), {}, ValueError, "weight must be"),
+        ((x, x[:, 0]), {}, ValueError, "shape"), ((x, None, x[:, 0]), {}, ValueError, "shape"),
+        ((x,), {"eps": -1.0}, ValueError, "eps"), ((x.long(),), {}, ValueError, "float32"),
+        ((torch.ones(2, 32769, device="cuda"),), {}, ValueError, "32768"),
+        ((torch.ones(2, 0, device="cuda"),), {}, ValueError, "1 to"),
+    ]:
+        with pytest.raises(error, match=text):
+            layer_norm(*args, **kw)

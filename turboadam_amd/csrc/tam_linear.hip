@@ -526,10 +526,10 @@ int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint6
 // m, or a copy of it whose rows are whole 16 bytes on 16-byte addresses.
 int on_16_bytes(call& c, matrix& m) {
   const uint32_t size = kSize[c.dtype];
-  if (aligned(m, size)) return TAM_OK;
+  if (aligned(m, size) || !m.cols || !m.rows) return TAM_OK;  // of no elements: nothing is read
   const uint32_t ld = aligned_ld(m.cols);
   void* p = c.ws.take(m.rows * ld * size);
-  if (!c.dry && m.rows) {
+  if (!c.dry) {
     const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
     if (c.dtype == TAM_DTYPE_F32)
       hipLaunchKernelGGL(tam_k_align<float>, grid, block, 0, c.stream, (const float*)m.p, m.ld, m.rows, m.cols,

@@ -7,6 +7,7 @@ type once.  No counterpart in the reference, which has an optimizer only.
 """
 
 import ctypes
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -41,8 +42,8 @@ def _plain(t: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor, width: int):
     """t as (rows, width) with contiguous rows, and the stride between them."""
-    t = t.resolve_neg().reshape(-1, width)
-    n = t.shape[0]
+    n = math.prod(t.shape[:-1])
+    t = t.resolve_neg().reshape(n, width)
     if width != 1 and t.stride(1) != 1 or n > 1 and not width <= t.stride(0) < _MOST_STRIDE:
         t = t.contiguous()
     return t, (t.stride(0) if n > 1 else max(width, 1))

@@ -147,7 +147,7 @@ class Muon(Optimizer):
 
     def _row(self, p, group):
         """One parameter's row of the table (TamMatrix without its last field)."""
-        g, st = p.grad, self.state[p]
+        g = p.grad
         if not p.is_cuda:
             raise RuntimeError(f"turboadam_amd.Muon: parameters must be on an MI355X (HIP) device, got {p.device}")
         if p.dtype not in _lib.DTYPES:
@@ -158,6 +158,7 @@ class Muon(Optimizer):
             raise RuntimeError(f"turboadam_amd.Muon: the gradient of a {p.dtype} parameter {tuple(p.shape)} on "
                                f"{p.device} must be dense and like it, got {g.layout} {g.dtype} {tuple(g.shape)} on "
                                f"{g.device}")
+        st = self.state[p]
         m = st.get("momentum_buffer")
         if m is None:
             m = st["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
