@@ -2,37 +2,40 @@
 // of D[r][c] = sum_k Q[r][k] * P[c][k] on the matrix cores, for bf16, fp16 and
 // fp32 operands that are contiguous along k or along their own index.
 //
-// Stages.  The k axis is cut into stages of 64 bytes of a row: 32 16-bit or 16
-// fp32 elements.  A stage of an operand is (rows * 64) bytes of LDS, written by
-// buffer loads that go to LDS directly, 1 KB to a wave and instruction:
-//   k-contiguous operand: [row][64 bytes], 16-byte chunk c of row r at place
-//     c ^ (r >> 1 & 3): eight consecutive rows' chunks cover all 32 banks, so
-//     the 16-byte fragment reads are free of conflicts;
+// Stages.  The k axis is cut into stages of 128 bytes of a row, a whole cache
+// line: 64 16-bit or 32 fp32 elements.  A stage of an operand is (rows * 128)
+// bytes of LDS, written by buffer loads that go to LDS directly, 1 KB to a wave
+// and instruction:
+//   k-contiguous operand: [row][128 bytes], 16-byte chunk c of row r at place
+//     c ^ (r >> 1 & 7): the 16-byte fragment reads are free of conflicts;
 //   operand contiguous along its own index ("m-major"): [k][rows], read with
-//     the transposing LDS read (16 bits) or in single words (fp32); chunk c of
-//     row k lies at c ^ 2 * (k & 3) (16 bits), c ^ 4 * (k >> 2 & 1) (fp32), so
-//     that the 4 rows that a 16-lane group reads lie in different banks.
+//     the transposing LDS read (16 bits) or in single words (fp32). LDS has 64
+//     banks (256 bytes); a read's 32 (fp32: 64) lanes that go together hold 8 (4)
+//     k rows, and chunk c of row k lies at c ^ swizzle(k), which puts them into
+//     different banks. (With the rows of 16 lanes alone apart, each transposing
+//     read took 4 cycles for 2: 1352 us for 8192 x 14336 x 4096, both operands.)
 // Chunks outside the operand have an offset past the buffer's end, which the
 // load returns as zeros: no size needs a tail loop, and the stages past the
-// last one are zeros too, so every step issues the same loads and waits for
-// the same count.
+// last one are zeros too, so every step issues the same loads.
 //
-// Pipeline.  TAM_GEMM_STAGES buffers.  Step t: wait for stage t+1 (all but
-// the youngest loads) and for the own LDS reads of stage t, barrier; issue the
-// loads of stage t+3 into the buffer of stage t, whose fragments are in every
-// wave's registers by then; read the fragments of stage t+1 among the matrix
-// instructions of stage t.  One barrier a step, and nothing waits for a load
-// issued less than two steps before.
+// Pipeline.  Two buffers, fragments of half a stage in registers twice.  Step t:
+// read the second half's fragments of stage t among the matrix instructions of the
+// first half; wait for stage t+1 and for the own reads, barrier: nobody reads
+// stage t's buffer any more; issue the loads of stage t+2 into it; read the first
+// half of stage t+1 among the matrix instructions of the second half of t.  One
+// barrier a step, and a load has a whole step to arrive.
 //
 // Fragments.  mfma 16x16x32 (16 bits) or four 16x16x4 (fp32), P as the left
 // operand: a lane then holds 4 consecutive columns c of one row r.
 #ifndef TAM_GEMM_H
 #define TAM_GEMM_H
 
+#include <type_traits>
+
 #include "tam_ops.h"
 
-#define TAM_GEMM_STAGES 3
-#define TAM_GEMM_ROW 64  // bytes of a row in a stage
+#define TAM_GEMM_STAGES 2
+#define TAM_GEMM_ROW 128  // bytes of a row in a stage
 
 typedef short tam_s4 __attribute__((ext_vector_type(4)));
 typedef short tam_s8 __attribute__((ext_vector_type(8)));
@@ -40,7 +43,6 @@ typedef __bf16 tam_bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 tam_h8 __attribute__((ext_vector_type(8)));
 typedef int tam_i4 __attribute__((ext_vector_type(4)));
 
-typedef __attribute__((address_space(3))) void tam_lds_void;
 typedef __attribute__((address_space(3))) char tam_lds_char;
 typedef __attribute__((address_space(3))) tam_s4 tam_lds_s4;
 typedef __attribute__((address_space(3))) tam_s8 tam_lds_s8;
@@ -55,7 +57,7 @@ struct tam_operand {
   uint32_t count;  // i < count
 };
 
-// Fragment of 16 rows by one stage: 8 16-bit or 4 fp32 elements a lane.
+// Fragment of 16 rows by half a stage: 8 16-bit or 4 fp32 elements a lane.
 template <typename T>
 struct tam_frag {
   tam_s8 v;
@@ -73,7 +75,7 @@ __device__ __forceinline__ tam_f4 tam_mfma(const tam_frag<tam_f16>& a, const tam
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(tam_h8, a.v), __builtin_bit_cast(tam_h8, b.v), c, 0,
                                                 0, 0);
 }
-// fp32: the lane's 4 elements are k = 4 * (lane / 16) + 0..3 of the stage; the
+// fp32: the lane's 4 elements are k = 4 * (lane / 16) + 0..3 of the half; the
 // j-th instruction sums k = j, 4 + j, 8 + j, 12 + j, the same for both operands.
 __device__ __forceinline__ tam_f4 tam_mfma(const tam_frag<float>& a, const tam_frag<float>& b, tam_f4 c) {
 #pragma unroll
@@ -96,10 +98,12 @@ struct tam_stage {
   const char* base;      // of the next stage to load
   uint64_t step;         // bytes from one stage to the next
   uint32_t off[LOADS];   // the lane's offsets; 2^31 where its row or column lies outside
-  uint32_t lane_k[KC ? 1 : LOADS];
+  uint32_t lane_k[LOADS];
 
   __device__ __forceinline__ static uint32_t swizzle(uint32_t k) {
-    return sizeof(T) == 2 ? 2u * (k & 3u) : 4u * (k >> 2 & 1u);
+    if constexpr (sizeof(T) == 4) return 4u * (k >> 2 & 3u);
+    if constexpr (CPR == 8) return 2u * (k >> 1 & 1u) | 4u * (k >> 3 & 1u);
+    return 2u * (k & 3u) | 8u * (k >> 3 & 1u);
   }
 
   // first: the tile's first row; k0: the first k
@@ -107,11 +111,11 @@ struct tam_stage {
     if constexpr (KC) {
       base = o.base + (uint64_t)first * o.ld + k0 * sizeof(T);
       step = TAM_GEMM_ROW;
-      const uint32_t chunk = (lane & 3u) ^ (lane >> 3 & 3u);
-      lane_k[0] = chunk * EPC;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const uint32_t row = (uint32_t)(wave * LOADS + i) * 16u + (uint32_t)(lane >> 2);
+        const uint32_t row = (uint32_t)(wave * LOADS + i) * 8u + (uint32_t)(lane >> 3);
+        const uint32_t chunk = (lane & 7u) ^ (row >> 1 & 7u);
+        lane_k[i] = chunk * EPC;
         off[i] = first + row < o.count ? (uint32_t)(row * o.ld) + chunk * 16u : 0x80000000u;
       }
     } else {
@@ -127,41 +131,42 @@ struct tam_stage {
     }
   }
 
-  // Loads the next stage into LDS at `lds`; k_left: how many k are left from its
-  // first one on (0 or less: zeros).
-  __device__ __forceinline__ void load(tam_lds_char* lds, int wave, int64_t k_left) {
-    const uint32_t left = k_left <= 0 ? 0u : (k_left > BK ? (uint32_t)BK : (uint32_t)k_left);
-    const __amdgpu_buffer_rsrc_t rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x80000000u, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const uint32_t voff = lane_k[KC ? 0 : i] < left ? off[i] : 0x80000000u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (tam_lds_void*)(lds + (wave * LOADS + i) * 1024), 16, voff, 0, 0,
-                                               0);
-    }
-    base += step;
+  // Load `i` of the next stage into LDS at `lds`; left: how many k are left from the
+  // stage's first one on, at most BK (zeros come past them).
+  // The compiler does not know that the asm writes LDS, or of its count in vmcnt: the
+  // pipeline waits for it (sync), and no wait is put before the reads of other
+  // buffers (as a builtin load gets one before every transposing read: 1.7 times the
+  // time for two m-major operands). m0 takes a wait state before it is used.
+  __device__ __forceinline__ void load(int i, uint32_t lds, int wave, uint32_t left) const {
+    const uint64_t b = (uint64_t)base;
+    const tam_i4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)0x80000000u, 0x00020000};
+    const uint32_t voff = lane_k[i] < left ? off[i] : 0x80000000u, at = lds + (uint32_t)(wave * LOADS + i) * 1024u;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(at), "v"(voff), "s"(rsrc)
+                 : "m0");
   }
 
-  // The fragment of rows row0 .. row0 + 15 of the stage at `lds`.
-  __device__ __forceinline__ static void read(tam_frag<T>& f, const tam_lds_char* lds, int row0, int lane) {
+  // The fragment of rows row0 .. row0 + 15 and half `h` of the stage at `lds`.
+  __device__ __forceinline__ static void read(tam_frag<T>& f, const tam_lds_char* lds, int row0, int h, int lane) {
     const uint32_t i = lane & 15u, q = (uint32_t)lane >> 4;
     if constexpr (KC) {
-      const uint32_t place = q ^ (i >> 1 & 3u);
+      const uint32_t place = (4u * h + q) ^ (i >> 1 & 7u);
       const tam_lds_char* p = lds + (row0 + i) * TAM_GEMM_ROW + place * 16u;
       f.v = *(const __attribute__((address_space(3))) decltype(f.v)*)p;
     } else if constexpr (sizeof(T) == 2) {
-      // k rows 8q + 4h + i/4, columns row0 + 4 * (i % 4): the transposing read gives
+      // k rows 8q + 4g + i/4, columns row0 + 4 * (i % 4): the transposing read gives
       // lane i the 4 k of column row0 + i
       const uint32_t jr = i >> 2;
-      const uint32_t chunk = ((uint32_t)row0 / 8u + (i >> 1 & 1u)) ^ (2u * jr);
-      const tam_lds_char* p = lds + (8u * q + jr) * (ROWS * 2u) + chunk * 16u + (i & 1u) * 8u;
+      const uint32_t chunk = ((uint32_t)row0 / 8u + (i >> 1 & 1u)) ^ swizzle(8u * q + jr);
+      const tam_lds_char* p = lds + (32u * h + 8u * q + jr) * (ROWS * 2u) + chunk * 16u + (i & 1u) * 8u;
       const tam_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tam_lds_s4*)p);
       const tam_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tam_lds_s4*)(p + 4u * (ROWS * 2u)));
       f.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       const uint32_t col = (uint32_t)row0 + i;
-      const uint32_t chunk = (col / 4u) ^ (4u * (q & 1u));
-      const tam_lds_char* p = lds + 4u * q * (ROWS * 4u) + chunk * 16u + (col & 3u) * 4u;
+      const uint32_t chunk = (col / 4u) ^ swizzle(4u * q);
+      const tam_lds_char* p = lds + (16u * h + 4u * q) * (ROWS * 4u) + chunk * 16u + (col & 3u) * 4u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) f.v[j] = *(const tam_lds_float*)(p + j * (ROWS * 4u));
     }
@@ -209,20 +214,6 @@ struct tam_tile {
     tam_frag<T> p[TN], q[TM];
   };
 
-  __device__ __forceinline__ static void read_all(frags& f, const tam_lds_char* lds, int wm, int wn, int lane) {
-#pragma unroll
-    for (int n = 0; n < TN; ++n) SP::read(f.p[n], lds, (wn * TN + n) * 16, lane);
-#pragma unroll
-    for (int m = 0; m < TM; ++m) SQ::read(f.q[m], lds + SP::BYTES, (wm * TM + m) * 16, lane);
-  }
-
-  __device__ __forceinline__ void multiply(const frags& f) {
-#pragma unroll
-    for (int m = 0; m < TM; ++m)
-#pragma unroll
-      for (int n = 0; n < TN; ++n) acc[n][m] = tam_mfma(f.p[n], f.q[m], acc[n][m]);
-  }
-
   // wait until at most N loads are in flight and every LDS read has returned; barrier
   template <int N>
   __device__ __forceinline__ static void sync() {
@@ -236,67 +227,79 @@ struct tam_tile {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     tam_lds_char* lds = (tam_lds_char*)smem;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
     SP sp;
     SQ sq;
     sp.init(P, c0, k0, wave, lane);
     sq.init(Q, r0, k0, wave, lane);
     const char *const p0 = sp.base, *const q0 = sq.base;
     const int64_t length = k1 > k0 ? (int64_t)(k1 - k0) : 0;
-    int64_t left = length;  // k from the next stage to load on
-    uint32_t steps = (uint32_t)((length + BK - 1) / BK), term = 0;
+    int64_t ahead = length;  // k from the next stage to load on
+    uint32_t left = 0, steps = (uint32_t)((length + BK - 1) / BK), term = 0;
     if constexpr (PARTS) steps *= parts.terms;
-    const uint32_t pairs = (steps + 1) / 2;
-    auto load = [&](uint32_t buf) {
-      if constexpr (PARTS)
-        if (left <= 0 && term + 1 < parts.terms) {
-          ++term;
-          left = length;
-          sp.base = p0 + (term == 2 ? parts.p : 0);
-          sq.base = q0 + (term == 1 ? parts.q : 0);
-        }
-      sp.load(lds + buf * STAGE, wave, left);
-      sq.load(lds + buf * STAGE + SP::BYTES, wave, left);
-      left -= BK;
+    // load i of the next stage into buffer `buf`: the first one looks at what is left,
+    // the last one moves on
+    auto load = [&](int i, uint32_t buf) {
+      if (i == 0) {
+        if constexpr (PARTS)
+          if (ahead <= 0 && term + 1 < parts.terms) {
+            ++term;
+            ahead = length;
+            sp.base = p0 + (term == 2 ? parts.p : 0);
+            sq.base = q0 + (term == 1 ? parts.q : 0);
+          }
+        left = ahead <= 0 ? 0u : (ahead > BK ? (uint32_t)BK : (uint32_t)ahead);
+        ahead -= BK;
+      }
+      if (i < SP::LOADS)
+        sp.load(i, lds0 + buf * STAGE, wave, left);
+      else
+        sq.load(i - SP::LOADS, lds0 + buf * STAGE + SP::BYTES, wave, left);
+      if (i == LOADS - 1) {
+        sp.base += sp.step;
+        sq.base += sq.step;
+      }
+    };
+    // Half a step: the fragments of half h of buffer `from` are read, and the loads into
+    // buffer `to` issued (GLOBAL), among the products of `f`, whose rows take a group each
+    // of about as many loads, reads and matrix instructions. Issued at once, the loads
+    // would hold up every matrix instruction behind them until the address unit has taken
+    // them, and the reads would queue.
+    auto half = [&](const frags& f, frags& next, uint32_t from, int h, uint32_t to, auto global) {
+      constexpr bool GLOBAL = decltype(global)::value;
+      const tam_lds_char* src = lds + from * STAGE;
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+#pragma unroll
+        for (int n = m * TN / TM; n < (m + 1) * TN / TM; ++n) SP::read(next.p[n], src, (wn * TN + n) * 16, h, lane);
+        SQ::read(next.q[m], src + SP::BYTES, (wm * TM + m) * 16, h, lane);
+        if constexpr (GLOBAL)
+#pragma unroll
+          for (int i = m * LOADS / TM; i < (m + 1) * LOADS / TM; ++i) load(i, to);
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[n][m] = tam_mfma(f.p[n], f.q[m], acc[n][m]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     __syncthreads();  // the LDS may hold what another tile's epilogue still reads
-    load(0);
-    load(1);
-    load(2);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(i, 0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(i, 1);
     frags a, b;
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
-    read_all(a, lds, wm, wn, lane);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+#pragma unroll
+    for (int n = 0; n < TN; ++n) SP::read(a.p[n], lds, (wn * TN + n) * 16, 0, lane);
+#pragma unroll
+    for (int m = 0; m < TM; ++m) SQ::read(a.q[m], lds + SP::BYTES, (wm * TM + m) * 16, 0, lane);
     uint32_t cur = 0;  // buffer of stage t
-    for (uint32_t t = 0; t < pairs; ++t) {
-      uint32_t next = cur == 2 ? 0 : cur + 1;
-      sync<LOADS>();
-      load(cur);
-      read_all(b, lds + next * STAGE, wm, wn, lane);
-      multiply(a);
-      interleave();
-      cur = next;
-      next = cur == 2 ? 0 : cur + 1;
-      sync<LOADS>();
-      load(cur);
-      read_all(a, lds + next * STAGE, wm, wn, lane);
-      multiply(b);
-      interleave();
-      cur = next;
+    for (uint32_t t = 0; t < steps; ++t) {
+      half(a, b, cur, 1, 0, std::false_type());
+      sync<0>();
+      half(b, a, cur ^ 1u, 0, cur, std::true_type());
+      cur ^= 1u;
     }
     sync<0>();  // the LDS is the epilogue's
-  }
-
-  // LDS reads spread among the matrix instructions of a step
-  __device__ __forceinline__ static void interleave() {
-    constexpr int READS = (PK ? 1 : sizeof(T) == 2 ? 2 : 4) * TN + (QK ? 1 : sizeof(T) == 2 ? 2 : 4) * TM;
-    constexpr int MFMAS = TN * TM * (sizeof(T) == 2 ? 1 : 4);
-    constexpr int EACH = MFMAS / READS > 0 ? MFMAS / READS : 1;
-#pragma unroll
-    for (int i = 0; i < READS; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);     // one LDS read
-      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // matrix instructions
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);  // the rest: the last reads return behind them
-    __builtin_amdgcn_sched_barrier(0);
   }
 
   // Hands the tile to f(row, col, v): 8 consecutive columns of one row, in fp32,
