@@ -74,25 +74,28 @@ def build_library(verbose: bool = False) -> str:
     return _hipcc(SOURCES, LIB_PATH, verbose)
 
 
-# The host side of a steady step in C++ (csrc/tam_host.cpp), a torch extension
-# module imported from _build/host by turboadam_amd.optimizer.
+# The host side of a steady step (csrc/tam_host.cpp) and of the layers
+# (csrc/tam_layers.cpp) in C++, a torch extension module imported from
+# _build/host by turboadam_amd.optimizer.
 HOST_BUILD_DIR = os.path.join(BUILD_DIR, "host")
-HOST_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_host.cpp")]
+HOST_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_host.cpp", "tam_layers.cpp")]
+ROCM_INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")  # of torch's HIP streams
 HOST_MODULE_PATH = os.path.join(HOST_BUILD_DIR, "_tam_host.so")
 
 
 def build_host_module(verbose: bool = False) -> str:
-    """Compile csrc/tam_host.cpp against torch's C++ API (the CPU compiler;
-    no device code)."""
+    """Compile the host sources against torch's C++ API (the CPU compiler; no
+    device code)."""
     from torch.utils import cpp_extension
 
     os.makedirs(HOST_BUILD_DIR, exist_ok=True)
-    for name in ("_tam_host.so", "tam_host.o"):  # compile every time, as the other libraries
+    for name in ("_tam_host.so", "tam_host.o", "tam_layers.o"):  # compile every time, as the other libraries
         path = os.path.join(HOST_BUILD_DIR, name)
         if os.path.exists(path):
             os.remove(path)
     cpp_extension.load(name="_tam_host", sources=HOST_SOURCES, build_directory=HOST_BUILD_DIR,
-                       extra_cflags=["-O2"], verbose=verbose)
+                       extra_cflags=["-O2"], extra_include_paths=[ROCM_INCLUDE], extra_ldflags=["-lc10_hip"],
+                       verbose=verbose)
     return HOST_MODULE_PATH
 
 

@@ -575,8 +575,11 @@ void advance_steps(py::list states) {
   }
 }
 
+void tam_register_layers(py::module_& m);  // tam_layers.cpp
+
 PYBIND11_MODULE(_tam_host, m) {
-  m.doc() = "Host side of a steady TurboAdam step (turboadam_amd.optimizer)";
+  m.doc() = "Host side of a steady TurboAdam step (turboadam_amd.optimizer) and of the layers (turboadam_amd.layers)";
+  tam_register_layers(m);
   m.def("tensor_addresses", &tensor_addresses, py::arg("tensors"));
   m.def("set_group_fields", &set_group_fields, py::arg("table"), py::arg("gsel"), py::arg("group_rows"),
         py::arg("wd"));
