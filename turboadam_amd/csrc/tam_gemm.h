@@ -359,4 +359,35 @@ __device__ __forceinline__ void tam_tile_at(uint32_t t, uint32_t tm, uint32_t tn
   m = g * GROUP + left - n * rows;
 }
 
+// ---------------------------------------------------------------------------
+// host side: what a launch of tiles takes
+// ---------------------------------------------------------------------------
+// Measured on one MI355X, tiles of k = 256 .. 4096 in launches of 16 to 1024 tiles
+// (bf16; fp32 in the second table): a launch that leaves half of the compute units
+// empty takes start + k * half us; with r tiles on each unit (at most `resident`
+// fit: 128, 64 and 32 KB of LDS) start + k * per_k[r - 1]. At k = 4096 and many
+// tiles that is 1460 TFLOP/s for 256, 980 for 128 and 690 for 64 (fp32: 133 for
+// both); 16 tiles of k = 256 take 10.4, 6.1 and 3.5 us.
+struct tam_tile_rate {
+  int tile, resident;
+  double start, half, per_k[4];
+};
+static const tam_tile_rate tam_rates_16[3] = {{256, 1, 5.0, 0.0168, {0.0224}},
+                                              {128, 2, 3.5, 0.0091, {0.0111, 0.0163}},
+                                              {64, 4, 2.4, 0.0040, {0.0048, 0.0064, 0.0090, 0.0116}}};
+static const tam_tile_rate tam_rates_32[2] = {{128, 2, 4.5, 0.0700, {0.0715, 0.1270}},
+                                              {64, 4, 2.4, 0.0182, {0.0188, 0.0330, 0.0480, 0.0633}}};
+
+// us of `tiles` tiles of k: whole rounds, then what is left.
+static inline double tam_tiles_us(const tam_tile_rate& t, double tiles, double k, double cus) {
+  const double round = cus * t.resident;
+  const double full = (double)(uint64_t)(tiles / round), rest = tiles - full * round;
+  double us = full * (0.5 * t.start + k * t.per_k[t.resident - 1]);
+  if (rest > 0) {
+    const int r = (int)((rest + cus - 1) / cus);
+    us += t.start + k * (rest <= 0.5 * cus ? t.half : t.per_k[r - 1]);
+  }
+  return us;
+}
+
 #endif  // TAM_GEMM_H

@@ -324,19 +324,26 @@ __global__ __launch_bounds__(256) void tam_k_slope(tam_slope_args a) {
   }
 }
 
-// out[c] = sum over runs of sums[run][c]: 64 columns to a workgroup, its 4 waves
-// take every fourth run.
+// out[c] = sum over runs of sums[run][c]: 64 columns to a workgroup, its 16 waves
+// take every 16th run.
 template <typename T>
-__global__ __launch_bounds__(256) void tam_k_column_sum(const float* sums, uint32_t runs, uint32_t cols, T* out) {
-  __shared__ float part[4][64];
+__global__ __launch_bounds__(1024) void tam_k_column_sum(const float* sums, uint32_t runs, uint32_t cols, T* out) {
+  __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t c = blockIdx.x * 64 + lane;
   float s = 0.f;
-  if (c < cols)
-    for (uint32_t r = wave; r < runs; r += 4) s += sums[(uint64_t)r * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (uint32_t r = wave; r < runs; r += 16) s += sums[(uint64_t)r * cols + c];
+  }
   part[wave][lane] = s;
   __syncthreads();
-  if (wave == 0 && c < cols) out[c] = tam_from_f<T>(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]);
+  if (wave == 0 && c < cols) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) v += part[w][lane];
+    out[c] = tam_from_f<T>(v);
+  }
 }
 
 template <typename T>
@@ -435,32 +442,24 @@ struct shape {
   uint32_t parts;  // the sum is cut into
 };
 
-// Which tile, and into how many parts the sum is cut. A product's time is about
-// rounds of tiles over the compute units times a tile's, and a tile's is its
-// multiplications at the rate that its size reaches when the chip is full
-// (measured, bf16, 8192 x 4096 x 4096 in TFLOP/s: see `rate`) plus what it
-// cannot hide; parts add their sums' way to memory and back and a launch.
+// Which tile, and into how many parts the sum is cut: the least of the measured
+// times (tam_tiles_us). Parts add their sums' way to memory and back (about 4 TB/s)
+// and a launch.
 shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
-  const double cus = tam_op_cus(), f32 = dtype == TAM_DTYPE_F32 ? 8.0 : 1.0;
-  struct {
-    int tile;
-    double rate;   // TFLOP/s of 16-bit products
-    double start;  // us before and after a tile's sum
-  } const kind[3] = {{256, 1000.0, 4.0}, {128, 700.0, 2.5}, {64, 350.0, 1.5}};
+  const double cus = tam_op_cus();
+  const bool f32 = dtype == TAM_DTYPE_F32;
+  const tam_tile_rate* rate = f32 ? tam_rates_32 : tam_rates_16;
   shape best = {64, 1};
   double least = 1e30;
-  for (const auto& t : kind) {
-    if (t.tile == 256 && dtype == TAM_DTYPE_F32) continue;
-    const double tiles = (double)tam_div_up(rows, t.tile) * (double)tam_div_up(cols, t.tile);
-    for (uint32_t parts = 1; parts <= 32; parts *= 2) {
-      if (parts > 1 && k / parts < 256) break;
-      const double rounds = tiles * parts / cus < 1.0 ? 1.0 : ceil(tiles * parts / cus);
-      const double one = 2.0 * t.tile * t.tile * ((double)k / parts) * cus / (t.rate * 1e6) * f32;
-      double us = rounds * (one + (rounds > 1.0 ? 0.5 : 1.0) * t.start);
-      if (parts > 1) us += 3.0 + (double)rows * cols * 4.0 * (2.0 * parts) / 3e6;
+  for (int i = 0; i < (f32 ? 2 : 3); ++i) {
+    const double tiles = (double)tam_div_up(rows, rate[i].tile) * (double)tam_div_up(cols, rate[i].tile);
+    for (uint32_t parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (parts > 1 && k / parts < 128) break;
+      double us = tam_tiles_us(rate[i], tiles * parts, (double)k / parts, cus);
+      if (parts > 1) us += 3.0 + (double)rows * cols * 8.0 * parts / 4e6;
       if (us < least) {
         least = us;
-        best = {t.tile, parts};
+        best = {rate[i].tile, parts};
       }
     }
   }
@@ -611,7 +610,7 @@ int backward(const TamLinear* d, call& c) {
     hipLaunchKernelGGL(tam_k_slope<T>, grid, block, 0, c.stream, a);                                               \
     TAM_OP_LAUNCHED("the activation's gradient");                                                                  \
     if (d->db) {                                                                                                   \
-      hipLaunchKernelGGL(tam_k_column_sum<T>, sums, block, 0, c.stream, a.sums, runs, (uint32_t)d->outputs, (T*)d->db); \
+      hipLaunchKernelGGL(tam_k_column_sum<T>, sums, dim3(1024), 0, c.stream, a.sums, runs, (uint32_t)d->outputs, (T*)d->db); \
       TAM_OP_LAUNCHED("the bias's gradient");                                                                      \
     }                                                                                                              \
   } while (0)

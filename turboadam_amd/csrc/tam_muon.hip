@@ -445,26 +445,23 @@ int check(const TamMatrix* m, int n) {
 uint64_t tiles(uint64_t rows, uint64_t cols, int t) { return tam_div_up(rows, t) * tam_div_up(cols, t); }
 uint64_t triangle_tiles(uint64_t s, int t) { return tam_div_up(s, t) * (tam_div_up(s, t) + 1) / 2; }
 
-// The tile of a phase: the time of a launch is about the work of its tiles at
-// the rate that their size reaches, over the compute units, in whole rounds.
+// The tile of a phase: the least of what its launch takes at the measured rates
+// (tam_tiles_us), for all tiles as if of one k, and no less than the longest one.
 int pick_tile(const std::vector<mat>& m, bool square) {
   const double cus = tam_op_cus();
-  const struct {
-    int tile;
-    double rate, start;
-  } kind[3] = {{256, 1000.0, 4.0}, {128, 700.0, 2.5}, {64, 350.0, 1.5}};
   int best = 64;
   double least = 1e30;
-  for (const auto& t : kind) {
-    double work = 0, longest = 0;  // us of one compute unit
+  for (const tam_tile_rate& t : tam_rates_16) {
+    double count = 0, sum = 0, longest = 0;
     for (const mat& d : m) {
       // q's sum runs over the longer side, p's and x's over the shorter one
       const double k = (square ? std::max(d.rows, d.cols) : d.s) * (d.split ? 3.0 : 1.0);
-      const double one = 2.0 * t.tile * t.tile * k * cus / (t.rate * 1e6) + t.start;
-      work += one * (double)(square ? triangle_tiles(d.s, t.tile) : tiles(d.rows, d.cols, t.tile));
-      longest = std::max(longest, one);
+      const double n = (double)(square ? triangle_tiles(d.s, t.tile) : tiles(d.rows, d.cols, t.tile));
+      count += n;
+      sum += n * k;
+      longest = std::max(longest, k);
     }
-    const double us = std::max(longest, work / cus) + (work / cus > longest ? longest * 0.5 : 0.0);
+    const double us = std::max(tam_tiles_us(t, count, sum / count, cus), t.start + longest * t.half);
     if (us < least) {
       least = us;
       best = t.tile;

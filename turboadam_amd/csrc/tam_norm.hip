@@ -30,19 +30,27 @@ struct norm_args {
   float eps;
 };
 
-// Elements at .. at + 7 of a row of n; zeros past its end.
+// Elements at .. at + 7 of a row of n as they lie in memory; zeros past its end.
 template <typename T>
-__device__ __forceinline__ void row_load(const T* row, uint32_t at, uint32_t n, float (&v)[8]) {
+__device__ __forceinline__ tam_oct<T> row_raw(const T* row, uint32_t at, uint32_t n) {
+  tam_oct<T> o;
   if (at + 8 <= n) {
-    tam_load8(row + at, v);
+    o = *reinterpret_cast<const tam_oct<T>*>(row + at);
   } else {
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) v[j] = 0.f;
+    for (uint32_t j = 0; j < 8; ++j) o.v[j] = (T)0.f;
     if (at < n)
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j)
-        if (at + j < n) v[j] = tam_to_f(row[at + j]);
+        if (at + j < n) o.v[j] = row[at + j];
   }
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ void row_load(const T* row, uint32_t at, uint32_t n, float (&v)[8]) {
+  const tam_oct<T> o = row_raw(row, at, n);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)o.v[j];
 }
 
 template <typename T>
@@ -169,25 +177,42 @@ __global__ __launch_bounds__((norm_shape<WPR, CH>::THREADS)) void tam_k_norm_bac
     if (a.w && at[c] < a.n) row_load(static_cast<const T*>(a.w), at[c], a.n, w[c]);
   }
   const float inv = 1.f / (float)a.n;
-  for (uint64_t first = (uint64_t)blockIdx.x * S::ROWS; first < a.rows; first += (uint64_t)gridDim.x * S::ROWS) {
-    const uint64_t row = first + wave / WPR, safe = row < a.rows ? row : 0;
+  // the next row's elements are on their way while a row's sums go through the waves
+  const uint64_t stride = (uint64_t)gridDim.x * S::ROWS;
+  tam_oct<T> rx[CH], rdy[CH];
+  float mean, rstd;
+  auto fetch = [&](uint64_t row) {
+    const uint64_t safe = row < a.rows ? row : 0;
     const uint32_t n = row < a.rows ? a.n : 0;
-    const T* x = static_cast<const T*>(a.x) + safe * a.ldx;
-    const T* dy = static_cast<const T*>(a.dy) + safe * a.n;
-    const float mean = a.stats[2 * safe], rstd = a.stats[2 * safe + 1];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      rx[c] = row_raw(static_cast<const T*>(a.x) + safe * a.ldx, at[c], n);
+      rdy[c] = row_raw(static_cast<const T*>(a.dy) + safe * a.n, at[c], n);
+    }
+    mean = a.stats[2 * safe];
+    rstd = a.stats[2 * safe + 1];
+  };
+  fetch((uint64_t)blockIdx.x * S::ROWS + wave / WPR);
+  for (uint64_t first = (uint64_t)blockIdx.x * S::ROWS; first < a.rows; first += stride) {
+    const uint64_t row = first + wave / WPR;
+    const uint32_t n = row < a.rows ? a.n : 0;
+    const float mu = mean, rs = rstd;
     float h[CH][8], t[CH][8];
     float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      row_load(x, at[c], n, h[c]);
-      row_load(dy, at[c], n, t[c]);
-    }
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        h[c][j] = (float)rx[c].v[j];
+        t[c][j] = (float)rdy[c].v[j];
+      }
+    if (first + stride < a.rows) fetch(row + stride);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         // past the row's end dy is 0 and h is not used
-        h[c][j] = (h[c][j] - mean) * rstd;
+        h[c][j] = (h[c][j] - mu) * rs;
         db[c][j] += t[c][j];
         if (at[c] + j < n) dw[c][j] = __builtin_fmaf(t[c][j], h[c][j], dw[c][j]);
         t[c][j] *= w[c][j];
@@ -202,7 +227,7 @@ __global__ __launch_bounds__((norm_shape<WPR, CH>::THREADS)) void tam_k_norm_bac
     for (int c = 0; c < CH; ++c) {
       if (at[c] >= a.n) continue;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[c][j] = rstd * (t[c][j] - m0 - h[c][j] * m1);
+      for (int j = 0; j < 8; ++j) t[c][j] = rs * (t[c][j] - m0 - h[c][j] * m1);
       row_store(dx, at[c], a.n, t[c]);
     }
   }
@@ -247,8 +272,10 @@ __global__ __launch_bounds__(1024) void tam_k_norm_sums(const float* sums, uint3
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint64_t c = (uint64_t)blockIdx.x * 64 + lane;
   float s = 0.f;
-  if (c < 2ull * n)
+  if (c < 2ull * n) {
+#pragma unroll 8
     for (uint32_t g = wave; g < groups; g += 16) s += sums[(uint64_t)g * 2 * n + c];
+  }
   part[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < 2ull * n) {
