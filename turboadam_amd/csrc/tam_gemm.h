@@ -302,19 +302,48 @@ struct tam_tile {
     sync<0>();  // the LDS is the epilogue's
   }
 
-  // Hands the tile to f(row, col, v): 8 consecutive columns of one row, in fp32,
-  // turned through LDS so that consecutive lanes hold consecutive columns.
-  // Rows and columns are the tile's own; every one is handed out once.
+  // Hands the tile to finish(row, col, v, pre): 8 consecutive columns of one row, in
+  // fp32, turned through LDS so that consecutive lanes hold consecutive columns.
+  // Rows and columns are the tile's own; every one is handed out once. pre is what
+  // load(row, col) returned for them earlier: the global loads that finish needs,
+  // issued a pass ahead (or, UNROLL, a round of passes), because a load behind each
+  // pass's stores costs its whole latency, 16 times a tile.
   // piece(rows0, cols0, lds, pitch): after each 32 rows of the wave, what it holds in LDS.
-  template <typename F, typename G>
-  __device__ __forceinline__ void each(char* smem, F f, G piece) {
+  template <bool UNROLL, typename L, typename F, typename G>
+  __device__ __forceinline__ void each(char* smem, L load, F finish, G piece) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     float* turn = reinterpret_cast<float*>(smem) + wave * ROUND * PITCH;
-    constexpr int LPR = COLS / 8;   // lanes of a row
-    constexpr int RPP = 64 / LPR;   // rows of a pass
+    constexpr int LPR = COLS / 8;         // lanes of a row
+    constexpr int RPP = 64 / LPR;         // rows of a pass
+    constexpr int PASSES = ROUND / RPP;
+    typedef decltype(load(0u, 0u)) Pre;
+    const int r0 = lane / LPR, c0 = (lane % LPR) * 8;
+    const uint32_t col = (uint32_t)(wn * COLS + c0);
+    auto row = [&](int m, int pass) { return (uint32_t)((wm * TM + m) * 16 + pass * RPP + r0); };
+    auto take = [&](int pass, float(&v)[8]) {
+      const float* from = turn + (pass * RPP + r0) * PITCH + c0;
+      const tam_f4 lo = *reinterpret_cast<const tam_f4*>(from), hi = *reinterpret_cast<const tam_f4*>(from + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = lo[j];
+        v[4 + j] = hi[j];
+      }
+    };
+    Pre pre[2][UNROLL ? PASSES : 1];
+    if constexpr (UNROLL) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) pre[0][p] = load(row(0, p), col);
+    }
 #pragma unroll
     for (int m = 0; m < TM; m += 2) {
+      if constexpr (UNROLL) {
+        if (m + 2 < TM)
+#pragma unroll
+          for (int p = 0; p < PASSES; ++p) pre[(m / 2 + 1) & 1][p] = load(row(m + 2, p), col);
+      } else {
+        pre[0][0] = load(row(m, 0), col);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -322,18 +351,22 @@ struct tam_tile {
           *reinterpret_cast<tam_f4*>(turn + (h * 16 + (lane & 15)) * PITCH + n * 16 + (lane >> 4) * 4) = acc[n][m + h];
       __builtin_amdgcn_wave_barrier();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-      for (int r = lane / LPR; r < ROUND; r += RPP) {
-        const int c = (lane % LPR) * 8;
-        float v[8];
-        const tam_f4 lo = *reinterpret_cast<const tam_f4*>(turn + r * PITCH + c);
-        const tam_f4 hi = *reinterpret_cast<const tam_f4*>(turn + r * PITCH + c + 4);
+      if constexpr (UNROLL) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = lo[j];
-          v[4 + j] = hi[j];
+        for (int p = 0; p < PASSES; ++p) {
+          float v[8];
+          take(p, v);
+          finish(row(m, p), col, v, pre[m / 2 & 1][p]);
         }
-        f((uint32_t)((wm * TM + m) * 16 + r), (uint32_t)(wn * COLS + c), v);
+      } else {
+#pragma unroll 1
+        for (int p = 0; p < PASSES; ++p) {
+          const Pre now = pre[0][0];
+          if (p + 1 < PASSES) pre[0][0] = load(row(m, p + 1), col);
+          float v[8];
+          take(p, v);
+          finish(row(m, p), col, v, now);
+        }
       }
       piece((uint32_t)((wm * TM + m) * 16), (uint32_t)(wn * COLS), turn, PITCH);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -342,12 +375,14 @@ struct tam_tile {
   }
 };
 
-// Workgroup b of n in the order in which one XCD's workgroups take consecutive
-// tiles (workgroups go to the 8 XCDs in turn): neighbours share rows of Q or P
-// in that XCD's L2.
+// Workgroup b of n -> tile. Workgroups go to the 8 XCDs in turn; of each 256, which
+// run together, an XCD takes 32 consecutive tiles: neighbours share rows of Q or P
+// in its L2, and all of them in the memory-side cache. The tiles' order from one
+// 256 to the next stays, longest first where their sums differ.
 __device__ __forceinline__ uint32_t tam_xcd_order(uint32_t b, uint32_t n) {
-  const uint32_t x = b & 7u, q = n >> 3, r = n & 7u;
-  return x * q + (x < r ? x : r) + (b >> 3);
+  const uint32_t base = b & ~255u, in = b & 255u, count = n - base < 256u ? n - base : 256u;
+  const uint32_t x = in & 7u, q = count >> 3, r = count & 7u;
+  return base + x * q + (x < r ? x : r) + (in >> 3);
 }
 
 // Tile t of tm x tn in groups of GROUP rows, column by column inside a group.

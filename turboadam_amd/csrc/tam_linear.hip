@@ -71,26 +71,37 @@ struct tam_epilogue {
   uint32_t rows, cols, act;
 };
 
-// v holds columns col .. col + 7 of a row of the product.
+// Eight elements of the residual, loaded ahead of their use.
 template <typename T>
-__device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, uint32_t col, float (&v)[8]) {
+__device__ __forceinline__ tam_oct<T> tam_residual(const tam_epilogue& e, uint32_t row, uint32_t col) {
+  tam_oct<T> r;
+  if (e.residual && row < e.rows && col + 8 <= e.cols)
+    r = *reinterpret_cast<const tam_oct<T>*>(static_cast<const T*>(e.residual) + (uint64_t)row * e.cols + col);
+  return r;
+}
+
+// v holds columns col .. col + 7 of a row of the product, r what tam_residual gave.
+template <typename T>
+__device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, uint32_t col, float (&v)[8],
+                                           const tam_oct<T>& r) {
   const uint64_t at = (uint64_t)row * e.cols + col;
   if (col + 8 <= e.cols) {
-    float t[8];
     if (e.bias) {
+      float t[8];
       tam_load8(static_cast<const T*>(e.bias) + col, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += t[j];
     }
+    // rounded to the type: half of the memory of fp32, and an error of one rounding of z
+    // times the activation's second derivative
     if (e.z) tam_store8(static_cast<T*>(e.z) + at, v);
     if (e.act != TAM_ACT_NONE) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = tam_act(v[j], e.act);
     }
     if (e.residual) {
-      tam_load8(static_cast<const T*>(e.residual) + at, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += t[j];
+      for (int j = 0; j < 8; ++j) v[j] += (float)r.v[j];
     }
     tam_store8(static_cast<T*>(e.out) + at, v);
   } else {
@@ -129,9 +140,9 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 2 : (BM == 128 ? 3 : 4)) 
   Tile t;
   t.zero();
   t.run(a.P, a.Q, n * BN, m * BM, k0, k1, smem);
-  t.each(
-      smem,
-      [&](uint32_t row, uint32_t col, float(&v)[8]) {
+  t.template each<false>(
+      smem, [&](uint32_t row, uint32_t col) { return tam_residual<T>(a.e, row + m * BM, col + n * BN); },
+      [&](uint32_t row, uint32_t col, float(&v)[8], const tam_oct<T>& r) {
         row += m * BM;
         col += n * BN;
         if (row >= a.e.rows || col >= a.e.cols) return;
@@ -145,7 +156,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 2 : (BM == 128 ? 3 : 4)) 
               if (col + j < a.e.cols) p[j] = v[j];
           }
         } else {
-          tam_finish<T>(a.e, row, col, v);
+          tam_finish<T>(a.e, row, col, v, r);
         }
       },
       [](uint32_t, uint32_t, const float*, int) {});
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(256) void tam_k_split(const float* partial, uint32_
       for (int j = 0; j < 8; ++j)
         if (col + j < e.cols) v[j] += partial[p * step + at + j];
   }
-  tam_finish<T>(e, row, col, v);
+  tam_finish<T>(e, row, col, v, tam_residual<T>(e, row, col));
 }
 
 // ---------------------------------------------------------------------------
@@ -255,7 +266,7 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_few(tam_few_args a) 
     for (int s = 0; s < TAM_FEW_WAVES; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += sum[s][row][col + j];
-    tam_finish<T>(a.e, row, blockIdx.x * 16 + col, v);
+    tam_finish<T>(a.e, row, blockIdx.x * 16 + col, v, tam_residual<T>(a.e, row, blockIdx.x * 16 + col));
   }
 }
 

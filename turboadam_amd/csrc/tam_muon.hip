@@ -247,70 +247,62 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
   uint32_t tm, tn;
   triangle(unit - d.first[SQUARE], tm, tn);
   const uint32_t r0 = tm * TILE, c0 = tn * TILE;
-  auto finish = [&](auto& t) {
-    tam_f16* out = GRAM ? d.q : d.p;
-    t.each(
-        smem,
-        [&](uint32_t row, uint32_t col, float(&v)[8]) {
-          row += r0;
-          col += c0;
-          if (row >= d.s || col >= d.lds) return;
-          const uint64_t at = (uint64_t)row * d.lds + col;
-          if constexpr (GRAM) {
+  struct parts {
+    tam_oct<tam_f16> high, low;
+  };
+  // q where p is made from it
+  auto load = [&](uint32_t row, uint32_t col) {
+    parts q;
+    if (!GRAM && row < d.s && col < d.lds) {
+      const tam_f16* from = d.q + (uint64_t)row * d.lds + col;
+      q.high = *reinterpret_cast<const tam_oct<tam_f16>*>(from);
+      if (d.s_low) q.low = *reinterpret_cast<const tam_oct<tam_f16>*>(from + d.s_low);
+    }
+    return q;
+  };
+  auto store = [&](uint32_t row, uint32_t col, float(&v)[8], const parts& q) {
+    if (row >= d.s || col >= d.lds) return;
+    if constexpr (GRAM) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
-          } else {
-            float q[8];
-            tam_load8(d.q + at, q);
-            if (d.s_low) {
-              float r[8];
-              tam_load8(d.q + at + d.s_low, r);
+      for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
+    } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) q[j] += r[j];
-            }
+      for (int j = 0; j < 8; ++j) {
+        const float x = (float)q.high.v[j] + (d.s_low ? (float)q.low.v[j] : 0.f);
+        v[j] = __builtin_fmaf(co.b, x, co.c / kScale * v[j]);
+      }
+      if (row - col < 8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(co.b, q[j], co.c / kScale * v[j]);
-            if (row - col < 8) {
-#pragma unroll
-              for (uint32_t j = 0; j < 8; ++j)
-                if (row - col == j) {
-                  v[j] += co.a * kScale;
-                  d.diag[row] = v[j] * (1.f / kScale);
-                }
-            }
+        for (uint32_t j = 0; j < 8; ++j)
+          if (row - col == j) {
+            v[j] += co.a * kScale;
+            d.diag[row] = v[j] * (1.f / kScale);
           }
-          store_parts(out + at, d.s_low, v);
-        },
+      }
+    }
+    store_parts((GRAM ? d.q : d.p) + (uint64_t)row * d.lds + col, d.s_low, v);
+  };
+  auto finish = [&](auto& t) {
+    typedef typename std::remove_reference<decltype(t)>::type Tile;
+    t.template each<true>(
+        smem, [&](uint32_t row, uint32_t col) { return load(row + r0, col + c0); },
+        [&](uint32_t row, uint32_t col, float(&v)[8], const parts& q) { store(row + r0, col + c0, v, q); },
         [&](uint32_t row, uint32_t col, const float* turned, int pitch) {
-          // off the diagonal, the mirrored tile: element (row, col) also goes to (col, row)
+          // off the diagonal, the mirrored tile: element (row, col) also goes to (col, row).
+          // A lane takes 8 rows of one column: 4 lanes to a column's 32 rows.
           if (tm == tn) return;
-          typedef typename std::remove_reference<decltype(t)>::type Tile;
-          const int lane = threadIdx.x & 63;
-          // a lane takes 8 rows of one column: 4 lanes to a column's 32 rows
-#pragma unroll 1
-          for (int c = lane >> 2; c < Tile::COLS; c += 16) {
-            const uint32_t to_row = c0 + col + c, to_col = r0 + row + (lane & 3) * 8;
-            if (to_row >= d.s || to_col >= d.lds) continue;
-            const uint64_t at = (uint64_t)to_row * d.lds + to_col;
+          const uint32_t lane = threadIdx.x & 63, from = (lane & 3) * 8, to_col = r0 + row + from;
+          constexpr int N = Tile::COLS / 16;
+          parts q[N];
+#pragma unroll
+          for (int i = 0; i < N; ++i) q[i] = load(c0 + col + i * 16 + (lane >> 2), to_col);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const uint32_t c = i * 16 + (lane >> 2);
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = turned[((lane & 3) * 8 + j) * pitch + c];
-            if constexpr (GRAM) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
-            } else {
-              float q[8];
-              tam_load8(d.q + at, q);
-              if (d.s_low) {
-                float r[8];
-                tam_load8(d.q + at + d.s_low, r);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] += r[j];
-              }
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(co.b, q[j], co.c / kScale * v[j]);
-            }
-            store_parts(out + at, d.s_low, v);
+            for (int j = 0; j < 8; ++j) v[j] = turned[(from + j) * pitch + c];
+            store(c0 + col + c, to_col, v, q[i]);
           }
         });
   };
@@ -330,16 +322,30 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
   }
 }
 
+// What the last product's epilogue needs of the parameter, loaded ahead.
+struct held {
+  tam_oct<tam_f16> low;  // of x
+  float p;               // wide: p's diagonal at the row
+  tam_oct<float> out;    // the parameter: 16 or 32 bytes
+};
+
 template <typename T>
-__device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t col, float (&v)[8]) {
+__device__ __forceinline__ void hold(const mat& d, uint32_t row, uint32_t col, held& h) {
+  const T* out = static_cast<const T*>(d.out) + (uint64_t)row * d.cols + col;
+  const tam_oct<T> o = *reinterpret_cast<const tam_oct<T>*>(out);
+  __builtin_memcpy(&h.out, &o, sizeof(o));
+}
+
+template <typename T>
+__device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t col, float (&v)[8], const held& h) {
   T* out = static_cast<T*>(d.out) + (uint64_t)row * d.cols + col;
   const bool update = d.flags & TAM_MATRIX_UPDATE;
   if (col + 8 <= d.cols) {
     if (update) {
-      float p[8];
-      tam_load8(out, p);
+      tam_oct<T> p;
+      __builtin_memcpy(&p, &h.out, sizeof(p));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(-d.rate, v[j], d.decay * p[j]);
+      for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(-d.rate, v[j], d.decay * (float)p.v[j]);
     }
     tam_store8(out, v);
   } else {
@@ -364,39 +370,54 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
   const uint32_t r0 = tm * TILE, c0 = tn * TILE;
   const tam_f16* x = d.x[turn];
   auto finish = [&](auto& t) {
-    t.each(
+    typedef typename std::remove_reference<decltype(t)>::type Tile;
+    float diag[8] = {};  // tall: p's diagonal at the lane's columns, the same in every row
+    if (d.tall && !d.split) {
+      const uint32_t lane = threadIdx.x & 63, col = c0 + ((threadIdx.x >> 6) % WN) * Tile::COLS + lane % (Tile::COLS / 8) * 8;
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) diag[j] = col + j < d.cols ? d.diag[col + j] : 0.f;
+    }
+    // the last product also holds the parameter: a round of passes ahead it would spill
+    t.template each<!LAST>(
         smem,
-        [&](uint32_t row, uint32_t col, float(&v)[8]) {
+        [&](uint32_t row, uint32_t col) {
+          held h;
+          row += r0;
+          col += c0;
+          if (row >= d.rows || col >= d.cols) return h;
+          if (!d.split) {
+            h.low = *reinterpret_cast<const tam_oct<tam_f16>*>(x + (uint64_t)row * d.ldx + col + d.x_low);
+            if (!d.tall) h.p = d.diag[row];
+          }
+          if (LAST && (d.flags & TAM_MATRIX_UPDATE) && col + 8 <= d.cols) {
+            if (d.dtype == TAM_DTYPE_F32)
+              hold<float>(d, row, col, h);
+            else
+              hold<tam_f16>(d, row, col, h);  // 16 bytes of either 16-bit type
+          }
+          return h;
+        },
+        [&](uint32_t row, uint32_t col, float(&v)[8], const held& h) {
           row += r0;
           col += c0;
           if (row >= d.rows || col >= d.cols) return;
-          const uint64_t at = (uint64_t)row * d.ldx + col;
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
           if (!d.split) {
-            float r[8];
-            tam_load8(x + at + d.x_low, r);
-            if (d.tall) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (col + j < d.cols) v[j] = __builtin_fmaf(d.diag[col + j], r[j], v[j]);
-            } else {
-              const float p = d.diag[row];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(p, r[j], v[j]);
-            }
+            for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(d.tall ? diag[j] : h.p, (float)h.low.v[j], v[j]);
           }
           if constexpr (LAST) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
             if (d.dtype == TAM_DTYPE_F32)
-              write_out<float>(d, row, col, v);
+              write_out<float>(d, row, col, v, h);
             else if (d.dtype == TAM_DTYPE_BF16)
-              write_out<tam_bf16>(d, row, col, v);
+              write_out<tam_bf16>(d, row, col, v, h);
             else
-              write_out<tam_f16>(d, row, col, v);
+              write_out<tam_f16>(d, row, col, v, h);
           } else {
-            store_parts(d.x[turn ^ 1u] + at, d.x_low, v);
+            store_parts(d.x[turn ^ 1u] + (uint64_t)row * d.ldx + col, d.x_low, v);
           }
         },
         [](uint32_t, uint32_t, const float*, int) {});
