@@ -398,8 +398,8 @@ int tam_norm_backward(const TamNorm* d, void* workspace, size_t ws_bytes, void* 
  * Frobenius norm, then `steps` times x = a x + b q x + c q q x with q = x x^T
  * (x^T x where rows > cols: the same polynomial).  out = x, or with UPDATE
  * out = decay out - rate x.  Products run on the fp16 matrix cores with fp32
- * sums: for bf16, x has a high and a low part and the products take the high
- * ones; for fp32 and fp16 every factor has both, and a product is three
+ * sums: for bf16, x has a high and a low part (3 bytes) and the products take the
+ * high ones; for fp32 and fp16 every factor has both, and a product is three
  * (22 bits).  Each result is rounded to its type once. */
 typedef struct TamMatrix {
   void* out;            /* [rows][cols] of dtype, contiguous                       */
@@ -414,8 +414,8 @@ typedef struct TamMatrix {
   uint32_t reserved;
 } TamMatrix;
 
-/* Bytes of workspace (256-byte aligned) of tam_orthogonalize: about 8 per
- * element of the matrices and 4 or 8 per element of their smaller squares. */
+/* Bytes of workspace (256-byte aligned) of tam_orthogonalize: about 6 (bf16) or 8
+ * per element of the matrices and 4 or 8 per element of their smaller squares. */
 int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes);
 /* All n matrices (a host array, read before the call returns) in the same 2 +
  * 3 * steps launches, beside their descriptors' upload. coefficients: a, b, c;

@@ -11,13 +11,17 @@
 // fp16 times 2^12: entries up to 16, and 11 bits down to 1.5e-8 of x's scale,
 // at the rate of bf16 with an eighth of its error.  What a step's rounding adds
 // in x's small singular directions the next steps amplify like the directions
-// themselves (a per step), so x keeps a low fp16 part, and x' = p x_high + diag(p)
+// themselves (a per step), so x keeps a low part, and x' = p x_high + diag(p)
 // x_low: p x_low with p's diagonal alone, since p is near diagonal where x_low
-// matters.  Rounding a I into p, instead of adding a x, keeps the diagonal's
+// matters.  The low part is a byte (5 exponent and 2 fraction bits: the upper half
+// of an fp16 number), 3 bits more than x_high: singular values over 5 decades
+// come out 1e-3 of the result's norm off, 2e-2 without it and 7e-4 with 11 bits, and
+// the products' epilogues, which all compute units reach together, move 4 bytes an
+// element for 6.  Rounding a I into p, instead of adding a x, keeps the diagonal's
 // rounding at the size of the result.  That is the scheme for bf16 matrices (error
 // about 1e-3 of the result's norm, below bf16's own rounding 1.7e-3).  fp32 and
-// fp16 matrices have high and low parts of x, q and p, and every product is high
-// high + high low + low high: 22 bits, errors near those of fp32 sums.
+// fp16 matrices have high and low fp16 parts of x, q and p, and every product is
+// high high + high low + low high: 22 bits, errors near those of fp32 sums.
 //
 // Launches (whole list each): tam_k_mu_momentum (momentum, partial squares of
 // u), tam_k_mu_start (x = u / |u|, in parts), then per step tam_k_mu_square
@@ -46,7 +50,8 @@ struct mat {
   void* out;
   const void* grad;
   float* momentum;
-  tam_f16* x[2];      // [rows][ldx] high parts, in turns; the low part `low` behind
+  tam_f16* x[2];      // [rows][ldx] high parts, in turns; the low parts (split: fp16, else
+                      // bytes) x_low elements behind
   tam_f16 *q, *p;     // [s][lds]
   float* diag;        // p's diagonal, fp32
   float* partial;     // squares of u
@@ -192,6 +197,45 @@ __device__ __forceinline__ void store_parts(tam_f16* high, int64_t low, const fl
   if (low) tam_store8(high + low, r);
 }
 
+// Bytes of 5 exponent and 2 fraction bits: 8 of them from fp32, rounded, and back.
+struct bytes8 {
+  uint32_t w[2];
+};
+__device__ __forceinline__ bytes8 to_bytes(const float (&v)[8]) {
+  bytes8 b;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * i], v[4 * i + 1], 0, false);
+    b.w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(v[4 * i + 2], v[4 * i + 3], w, true);
+  }
+  return b;
+}
+__device__ __forceinline__ float from_byte(const bytes8& b, int j) {
+  const uint16_t bits = (uint16_t)((b.w[j / 4] >> (8 * (j % 4)) & 255u) << 8);
+  return (float)__builtin_bit_cast(tam_f16, bits);
+}
+
+__device__ __forceinline__ uint8_t* low_bytes(const mat& d, const tam_f16* x) {
+  return reinterpret_cast<uint8_t*>(const_cast<tam_f16*>(x) + d.x_low);
+}
+
+// 8 elements of x (times 2^12) in its parts.
+__device__ __forceinline__ void store_x(const mat& d, tam_f16* x, uint64_t at, const float (&v)[8]) {
+  if (d.split) {
+    store_parts(x + at, d.x_low, v);
+  } else {
+    float y[8], r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      y[j] = v[j];
+      asm("" : "+v"(y[j]));  // as in store_parts
+      r[j] = y[j] - (float)(tam_f16)y[j];
+    }
+    tam_store8(x + at, y);
+    *reinterpret_cast<bytes8*>(low_bytes(d, x) + at) = to_bytes(r);
+  }
+}
+
 // x = u / max(|u|, eps) times 2^12, in parts.  A unit is 2048 elements of x's
 // rows of ldx; the columns past the matrix are zeros.
 constexpr uint32_t kStart = 2048;
@@ -213,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
   direction(d, g, m, u);
 #pragma unroll
   for (int j = 0; j < 8; ++j) u[j] *= scale;
-  store_parts(d.x[0] + at, d.x_low, u);
+  store_x(d, d.x[0], at, u);
 }
 
 // ---------------------------------------------------------------------------
@@ -324,7 +368,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
 
 // What the last product's epilogue needs of the parameter, loaded ahead.
 struct held {
-  tam_oct<tam_f16> low;  // of x
+  bytes8 low;            // of x, where it is bytes
   float p;               // wide: p's diagonal at the row
   tam_oct<float> out;    // the parameter: 16 or 32 bytes
 };
@@ -386,7 +430,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
           col += c0;
           if (row >= d.rows || col >= d.cols) return h;
           if (!d.split) {
-            h.low = *reinterpret_cast<const tam_oct<tam_f16>*>(x + (uint64_t)row * d.ldx + col + d.x_low);
+            h.low = *reinterpret_cast<const bytes8*>(low_bytes(d, x) + (uint64_t)row * d.ldx + col);
             if (!d.tall) h.p = d.diag[row];
           }
           if (LAST && (d.flags & TAM_MATRIX_UPDATE) && col + 8 <= d.cols) {
@@ -405,7 +449,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
           for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
           if (!d.split) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(d.tall ? diag[j] : h.p, (float)h.low.v[j], v[j]);
+            for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(d.tall ? diag[j] : h.p, from_byte(h.low, j), v[j]);
           }
           if constexpr (LAST) {
 #pragma unroll
@@ -417,7 +461,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
             else
               write_out<tam_f16>(d, row, col, v, h);
           } else {
-            store_parts(d.x[turn ^ 1u] + (uint64_t)row * d.ldx + col, d.x_low, v);
+            store_x(d, d.x[turn ^ 1u], (uint64_t)row * d.ldx + col, v);
           }
         },
         [](uint32_t, uint32_t, const float*, int) {});
@@ -530,7 +574,7 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
     m.x_low = (int64_t)tam_up((uint64_t)m.rows * m.ldx, 128);
     const int64_t square = (int64_t)tam_up((uint64_t)m.s * m.lds, 128);
     m.s_low = m.split ? square : 0;
-    for (int i = 0; i < 2; ++i) m.x[i] = (tam_f16*)take(m.x_low * 4);
+    for (int i = 0; i < 2; ++i) m.x[i] = (tam_f16*)take(m.x_low * (m.split ? 4 : 3));
     m.q = (tam_f16*)take(square * (m.split ? 4 : 2));
     m.p = (tam_f16*)take(square * (m.split ? 4 : 2));
     m.diag = (float*)take((uint64_t)m.s * 4);
