@@ -418,7 +418,8 @@ typedef struct TamMatrix {
  * per element of the matrices and 4 or 8 per element of their smaller squares. */
 int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes);
 /* All n matrices (a host array, read before the call returns) in the same 2 +
- * 3 * steps launches, beside their descriptors' upload. coefficients: a, b, c;
+ * 3 * steps launches (steps more where q's sums are cut among workgroups), those
+ * with sides of up to 128 in one of their own, beside their descriptors' upload. coefficients: a, b, c;
  * steps 1 to 64. */
 int tam_orthogonalize(const TamMatrix* matrices, int n, const float* coefficients, int steps, void* workspace,
                       size_t ws_bytes, void* stream);

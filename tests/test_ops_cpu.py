@@ -129,12 +129,12 @@ def test_orthogonalize_rejects(kw, code, text):
 
 def test_orthogonalize_workspace_and_settings():
     lib = _lib.load()
-    m = _matrices((100, 60), (33, 70))
+    m = _matrices((200, 60), (33, 270))
     rc, need, _ = _ns(m)
     # two turns of x in two fp16 parts; q and p in two parts (fp32)
-    assert rc == 0 and need >= 8 * (100 * 64 + 33 * 72) + 8 * (60 * 64 + 33 * 40)
-    half = _ns(_matrices((100, 60), (33, 70), dtype=_lib.TAM_DTYPE_BF16))[1]
-    assert need > half >= 6 * (100 * 64 + 33 * 72) + 4 * (60 * 64 + 33 * 40)
+    assert rc == 0 and need >= 8 * (200 * 64 + 33 * 272) + 8 * (60 * 64 + 33 * 40)
+    half = _ns(_matrices((200, 60), (33, 270), dtype=_lib.TAM_DTYPE_BF16))[1]
+    assert need > half >= 6 * (200 * 64 + 33 * 272) + 4 * (60 * 64 + 33 * 40)
     co = (ctypes.c_float * 3)(3.4445, -4.775, 2.0315)
     bad = (ctypes.c_float * 3)(3.4445, float("nan"), 2.0315)
     at = ctypes.addressof(m)

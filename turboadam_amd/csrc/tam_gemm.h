@@ -83,6 +83,22 @@ __device__ __forceinline__ tam_f4 tam_mfma(const tam_frag<float>& a, const tam_f
   return c;
 }
 
+// 16 bytes a lane from rsrc's base + voff to LDS at `lds` + 16 * lane.
+__device__ __forceinline__ void tam_to_lds(uint32_t lds, uint32_t voff, tam_i4 rsrc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(rsrc)
+               : "m0");
+}
+
+// A word a lane, to LDS at `lds` + 4 * lane.
+__device__ __forceinline__ void tam_word_to_lds(uint32_t lds, uint32_t voff, tam_i4 rsrc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(rsrc)
+               : "m0");
+}
+
 // Loading and reading one operand's stages.  ROWS: its rows in the tile; NW:
 // the workgroup's waves; KC: contiguous along k.
 template <typename T, int ROWS, int NW, bool KC>
@@ -141,10 +157,7 @@ struct tam_stage {
     const uint64_t b = (uint64_t)base;
     const tam_i4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)0x80000000u, 0x00020000};
     const uint32_t voff = lane_k[i] < left ? off[i] : 0x80000000u, at = lds + (uint32_t)(wave * LOADS + i) * 1024u;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(at), "v"(voff), "s"(rsrc)
-                 : "m0");
+    tam_to_lds(at, voff, rsrc);
   }
 
   // The fragment of rows row0 .. row0 + 15 and half `h` of the stage at `lds`.
@@ -181,6 +194,20 @@ struct tam_parts {
   int64_t p, q;
 };
 
+// How far ahead of its use the epilogue loads (tam_tile::each).
+enum tam_ahead { TAM_AHEAD_PASS, TAM_AHEAD_ROUND, TAM_AHEAD_ALL };
+
+// What the epilogue will read of an array laid out like the tile: a word of each line
+// of it is fetched in the last step but one (to LDS, where nobody reads it: that takes
+// no registers). Otherwise all compute units, whose tiles end together, wait for
+// memory: of 45 us that a tile of k = 256 took, 11 were the wait for x's low part.
+struct tam_soon {
+  const char* base;         // of the tile's first element, on 4 bytes; null: nothing
+  uint64_t ld;              // bytes, a multiple of 4
+  uint32_t rows, bytes;     // from there on
+  uint32_t width;           // bytes of a tile's row: a power of two from 64 to 1024
+};
+
 // One workgroup's tile: BM rows (operand Q) by BN columns (operand P), WM by
 // WN waves.
 template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK>
@@ -198,7 +225,8 @@ struct tam_tile {
   static constexpr int COLS = BN / WN;                    // a wave's columns
   static constexpr int PITCH = COLS + 4;                  // floats of a turned row
   static constexpr int TURN = NW * ROUND * PITCH * 4;
-  static constexpr int LDS = TAM_GEMM_STAGES * STAGE > TURN ? TAM_GEMM_STAGES * STAGE : TURN;
+  static constexpr int DUMP = TAM_GEMM_STAGES * STAGE > TURN ? TAM_GEMM_STAGES * STAGE : TURN;
+  static constexpr int LDS = DUMP + NW * 256;  // the words that `soon` fetches
   static_assert(TM % 2 == 0, "rounds of 32 rows");
 
   tam_f4 acc[TN][TM];
@@ -223,7 +251,7 @@ struct tam_tile {
   // Adds the products of k0 <= k < k1 to the tile at rows r0, columns c0.
   template <bool PARTS = false>
   __device__ __forceinline__ void run(const tam_operand& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
-                                      uint64_t k1, char* smem, tam_parts parts = {1, 0, 0}) {
+                                      uint64_t k1, char* smem, const tam_soon& soon, tam_parts parts = {1, 0, 0}) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     tam_lds_char* lds = (tam_lds_char*)smem;
@@ -260,6 +288,16 @@ struct tam_tile {
         sq.base += sq.step;
       }
     };
+    auto fetch = [&]() {
+      const uint32_t lines = soon.width > 128u ? soon.width / 128u : 1u;  // of a row
+      const uint64_t b = (uint64_t)soon.base;
+      const tam_i4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)0x80000000u, 0x00020000};
+      for (uint32_t i = wave * 64; i < BM * lines; i += NW * 64) {
+        const uint32_t line = i + lane, row = line / lines, in = line % lines * 128u;
+        const bool inside = row < soon.rows && row < BM && in + 4u <= soon.bytes;
+        tam_word_to_lds(lds0 + DUMP + (uint32_t)wave * 256u, inside ? (uint32_t)(row * soon.ld) + in : 0x80000000u, rsrc);
+      }
+    };
     // Half a step: the fragments of half h of buffer `from` are read, and the loads into
     // buffer `to` issued (GLOBAL), among the products of `f`, whose rows take a group each
     // of about as many loads, reads and matrix instructions. Issued at once, the loads
@@ -293,9 +331,11 @@ struct tam_tile {
 #pragma unroll
     for (int m = 0; m < TM; ++m) SQ::read(a.q[m], lds + SP::BYTES, (wm * TM + m) * 16, 0, lane);
     uint32_t cur = 0;  // buffer of stage t
+    const uint32_t last = steps > 2 && soon.base ? steps - 2 : ~0u;
     for (uint32_t t = 0; t < steps; ++t) {
       half(a, b, cur, 1, 0, std::false_type());
       sync<0>();
+      if (t == last) fetch();
       half(b, a, cur ^ 1u, 0, cur, std::true_type());
       cur ^= 1u;
     }
@@ -305,11 +345,13 @@ struct tam_tile {
   // Hands the tile to finish(row, col, v, pre): 8 consecutive columns of one row, in
   // fp32, turned through LDS so that consecutive lanes hold consecutive columns.
   // Rows and columns are the tile's own; every one is handed out once. pre is what
-  // load(row, col) returned for them earlier: the global loads that finish needs,
-  // issued a pass ahead (or, UNROLL, a round of passes), because a load behind each
-  // pass's stores costs its whole latency, 16 times a tile.
+  // load(row, col) returned for them earlier: the global loads that finish needs. A
+  // load behind each pass's stores costs its whole latency, 16 times a tile; and as
+  // loads and stores are counted in order, a load issued behind stores is not there
+  // before they have reached memory. AHEAD: all (every load before the first store),
+  // round (a round of 32 rows ahead), or pass (one pass; the code of one pass).
   // piece(rows0, cols0, lds, pitch): after each 32 rows of the wave, what it holds in LDS.
-  template <bool UNROLL, typename L, typename F, typename G>
+  template <tam_ahead AHEAD, typename L, typename F, typename G>
   __device__ __forceinline__ void each(char* smem, L load, F finish, G piece) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -330,18 +372,22 @@ struct tam_tile {
         v[4 + j] = hi[j];
       }
     };
-    Pre pre[2][UNROLL ? PASSES : 1];
+    constexpr bool UNROLL = AHEAD != TAM_AHEAD_PASS;
+    constexpr int ROUNDS = TM / 2, DEPTH = AHEAD == TAM_AHEAD_ALL ? ROUNDS : 2;
+    Pre pre[DEPTH][UNROLL ? PASSES : 1];
     if constexpr (UNROLL) {
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) pre[0][p] = load(row(0, p), col);
+      for (int i = 0; i < DEPTH - (AHEAD == TAM_AHEAD_ROUND); ++i)
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) pre[i][p] = load(row(2 * i, p), col);
     }
 #pragma unroll
     for (int m = 0; m < TM; m += 2) {
-      if constexpr (UNROLL) {
+      if constexpr (AHEAD == TAM_AHEAD_ROUND) {
         if (m + 2 < TM)
 #pragma unroll
-          for (int p = 0; p < PASSES; ++p) pre[(m / 2 + 1) & 1][p] = load(row(m + 2, p), col);
-      } else {
+          for (int p = 0; p < PASSES; ++p) pre[(m / 2 + 1) % DEPTH][p] = load(row(m + 2, p), col);
+      } else if constexpr (AHEAD == TAM_AHEAD_PASS) {
         pre[0][0] = load(row(m, 0), col);
       }
 #pragma unroll
@@ -356,7 +402,7 @@ struct tam_tile {
         for (int p = 0; p < PASSES; ++p) {
           float v[8];
           take(p, v);
-          finish(row(m, p), col, v, pre[m / 2 & 1][p]);
+          finish(row(m, p), col, v, pre[m / 2 % DEPTH][p]);
         }
       } else {
 #pragma unroll 1

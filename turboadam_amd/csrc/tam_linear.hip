@@ -139,8 +139,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 2 : (BM == 128 ? 3 : 4)) 
   const uint64_t k1 = k0 + a.k_part < a.k ? k0 + a.k_part : a.k;
   Tile t;
   t.zero();
-  t.run(a.P, a.Q, n * BN, m * BM, k0, k1, smem);
-  t.template each<false>(
+  tam_soon soon = {};
+  if (a.e.residual && !a.partial) {
+    const uint64_t ld = (uint64_t)a.e.cols * sizeof(T);
+    soon = {static_cast<const char*>(a.e.residual) + m * BM * ld + n * BN * sizeof(T), ld, a.e.rows - m * BM,
+            (a.e.cols - n * BN) * (uint32_t)sizeof(T), BN * (uint32_t)sizeof(T)};
+    if (((uintptr_t)soon.base | ld) & 3u) soon.base = nullptr;
+  }
+  t.run(a.P, a.Q, n * BN, m * BM, k0, k1, smem, soon);
+  t.template each<TAM_AHEAD_PASS>(
       smem, [&](uint32_t row, uint32_t col) { return tam_residual<T>(a.e, row + m * BM, col + n * BN); },
       [&](uint32_t row, uint32_t col, float(&v)[8], const tam_oct<T>& r) {
         row += m * BM;

@@ -25,7 +25,9 @@
 //
 // Launches (whole list each): tam_k_mu_momentum (momentum, partial squares of
 // u), tam_k_mu_start (x = u / |u|, in parts), then per step tam_k_mu_square
-// twice (q, p) and tam_k_mu_apply (x, the last one: the output).
+// twice (q, p; tam_k_mu_join between them where q's sums are cut among workgroups)
+// and tam_k_mu_apply (x, the last one: the output).  Small matrices take one launch
+// of their own, tam_k_mu_small.
 #include "tam_gemm.h"
 
 #include <math.h>
@@ -44,7 +46,7 @@ constexpr uint64_t kMostSide = 65536;
 
 // A matrix as the kernels take it.  Unit counts run over the list: units of
 // phase f of matrix i are first[f] .. first[f] of i + 1.
-enum { MOMENTUM, START, SQUARE, APPLY, PHASES };
+enum { MOMENTUM, START, GRAM, SQUARE, APPLY, PHASES };
 
 struct mat {
   void* out;
@@ -68,6 +70,8 @@ struct list {
   const mat* m;
   uint32_t n;
   uint32_t units[PHASES];
+  uint32_t parts;  // of the Gram products' sums, and where they go: 64 x 64 tiles
+  float* sums;     // [unit][part]
 };
 
 // The matrix whose unit of phase F b is: the last one whose first unit is not
@@ -279,25 +283,32 @@ __device__ __forceinline__ void triangle(uint32_t t, uint32_t& m, uint32_t& n) {
   n = t - m * (m + 1) / 2;
 }
 
-// GRAM: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q.
-template <int TILE, int WM, int WN, bool GRAM>
+// FIRST: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q.
+template <int TILE, int WM, int WN, bool FIRST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 4)) void tam_k_mu_square(
     list l, uint32_t turn, coefficients co) {
   typedef tam_tile<tam_f16, TILE, TILE, WM, WN, true, true> Rows;
   typedef tam_tile<tam_f16, TILE, TILE, WM, WN, false, false> Columns;
   __shared__ __attribute__((aligned(16))) char smem[Rows::LDS > Columns::LDS ? Rows::LDS : Columns::LDS];
   const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
-  const mat& d = l.m[owner<SQUARE>(l, unit)];
+  const mat& d = l.m[owner<FIRST ? GRAM : SQUARE>(l, unit)];
   uint32_t tm, tn;
-  triangle(unit - d.first[SQUARE], tm, tn);
+  triangle(unit - d.first[FIRST ? GRAM : SQUARE], tm, tn);
   const uint32_t r0 = tm * TILE, c0 = tn * TILE;
+  // the part of the sum that is this workgroup's (FIRST: blockIdx.y of l.parts)
+  uint64_t k0 = 0, k1 = FIRST ? (d.tall ? d.rows : d.ldx) : d.lds;
+  if (FIRST && l.parts > 1) {
+    const uint64_t each = (k1 + l.parts * 64u - 1) / (l.parts * 64u) * 64u;
+    k0 = blockIdx.y * each < k1 ? blockIdx.y * each : k1;
+    k1 = k0 + each < k1 ? k0 + each : k1;
+  }
   struct parts {
     tam_oct<tam_f16> high, low;
   };
   // q where p is made from it
   auto load = [&](uint32_t row, uint32_t col) {
     parts q;
-    if (!GRAM && row < d.s && col < d.lds) {
+    if (!FIRST && row < d.s && col < d.lds) {
       const tam_f16* from = d.q + (uint64_t)row * d.lds + col;
       q.high = *reinterpret_cast<const tam_oct<tam_f16>*>(from);
       if (d.s_low) q.low = *reinterpret_cast<const tam_oct<tam_f16>*>(from + d.s_low);
@@ -306,7 +317,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
   };
   auto store = [&](uint32_t row, uint32_t col, float(&v)[8], const parts& q) {
     if (row >= d.s || col >= d.lds) return;
-    if constexpr (GRAM) {
+    if constexpr (FIRST) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
     } else {
@@ -324,11 +335,21 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
           }
       }
     }
-    store_parts((GRAM ? d.q : d.p) + (uint64_t)row * d.lds + col, d.s_low, v);
+    store_parts((FIRST ? d.q : d.p) + (uint64_t)row * d.lds + col, d.s_low, v);
   };
   auto finish = [&](auto& t) {
     typedef typename std::remove_reference<decltype(t)>::type Tile;
-    t.template each<true>(
+    if constexpr (FIRST && TILE == 64) {
+      if (l.parts > 1) {
+        float* out = l.sums + ((uint64_t)unit * l.parts + blockIdx.y) * (64 * 64);
+        t.template each<TAM_AHEAD_PASS>(
+            smem, [](uint32_t, uint32_t) { return 0; },
+            [&](uint32_t row, uint32_t col, float(&v)[8], int) { tam_store8(out + row * 64 + col, v); },
+            [](uint32_t, uint32_t, const float*, int) {});
+        return;
+      }
+    }
+    t.template each<TAM_AHEAD_ROUND>(
         smem, [&](uint32_t row, uint32_t col) { return load(row + r0, col + c0); },
         [&](uint32_t row, uint32_t col, float(&v)[8], const parts& q) { store(row + r0, col + c0, v, q); },
         [&](uint32_t row, uint32_t col, const float* turned, int pitch) {
@@ -350,19 +371,58 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
           }
         });
   };
-  if (GRAM && d.tall) {
+  tam_soon soon = {};  // q, where p is made from it
+  if (!FIRST)
+    soon = {reinterpret_cast<const char*>(d.q + (uint64_t)r0 * d.lds + c0), (uint64_t)d.lds * 2u, d.s - r0,
+            (d.lds - c0) * 2u, TILE * 2u};
+  if (FIRST && d.tall) {
     Columns t;
     t.zero();
     const tam_operand x = operand(d.x[turn], d.ldx, d.ldx);
-    t.template run<true>(x, x, c0, r0, 0, d.rows, smem, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
+    t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
     finish(t);
   } else {
     Rows t;
     t.zero();
-    const tam_operand x = GRAM ? operand(d.x[turn], d.ldx, d.rows) : operand(d.q, d.lds, d.s);
-    const int64_t low = (GRAM ? d.x_low : d.s_low) * 2;
-    t.template run<true>(x, x, c0, r0, 0, GRAM ? d.ldx : d.lds, smem, {d.split ? 3u : 1u, low, low});
+    const tam_operand x = FIRST ? operand(d.x[turn], d.ldx, d.rows) : operand(d.q, d.lds, d.s);
+    const int64_t low = (FIRST ? d.x_low : d.s_low) * 2;
+    t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, low, low});
     finish(t);
+  }
+}
+
+// q from the parts' sums of its tiles, added in their order.
+__global__ __launch_bounds__(kThreads) void tam_k_mu_join(list l) {
+  __shared__ float tile[64][65];
+  const mat& d = l.m[owner<GRAM>(l, blockIdx.x)];
+  uint32_t tm, tn;
+  triangle(blockIdx.x - d.first[GRAM], tm, tn);
+  const float* from = l.sums + (uint64_t)blockIdx.x * l.parts * (64 * 64);
+  const uint32_t col = (threadIdx.x & 7u) * 8u;
+  for (uint32_t row = threadIdx.x >> 3; row < 64; row += kThreads / 8) {
+    float v[8] = {};
+    for (uint32_t p = 0; p < l.parts; ++p) {
+      float s[8];
+      tam_load8(from + p * (64 * 64) + row * 64 + col, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += s[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] *= 1.f / kScale;
+      tile[row][col + j] = v[j];
+    }
+    const uint32_t r = tm * 64 + row, c = tn * 64 + col;
+    if (r < d.s && c < d.lds) store_parts(d.q + (uint64_t)r * d.lds + c, d.s_low, v);
+  }
+  if (tm == tn) return;
+  __syncthreads();
+  for (uint32_t row = threadIdx.x >> 3; row < 64; row += kThreads / 8) {
+    const uint32_t r = tn * 64 + row, c = tm * 64 + col;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = tile[col + j][row];
+    if (r < d.s && c < d.lds) store_parts(d.q + (uint64_t)r * d.lds + c, d.s_low, v);
   }
 }
 
@@ -421,8 +481,8 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) diag[j] = col + j < d.cols ? d.diag[col + j] : 0.f;
     }
-    // the last product also holds the parameter: a round of passes ahead it would spill
-    t.template each<!LAST>(
+    // (the last product also holds the parameter: all of it would not fit the registers)
+    t.template each<LAST ? TAM_AHEAD_ROUND : TAM_AHEAD_ALL>(
         smem,
         [&](uint32_t row, uint32_t col) {
           held h;
@@ -468,16 +528,240 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
   };
   const tam_operand p = operand(d.p, d.lds, d.s);
   const uint32_t terms = d.split ? 3u : 1u;
+  // x's low bytes; with high and low products the last epilogue's parameter instead
+  tam_soon soon = {};
+  if (!d.split) {
+    soon = {reinterpret_cast<const char*>(low_bytes(d, x)) + (uint64_t)r0 * d.ldx + c0, d.ldx, d.rows - r0, d.ldx - c0, TILE};
+    if (d.ldx & 3u) soon.base = nullptr;
+  } else if (LAST && (d.flags & TAM_MATRIX_UPDATE)) {
+    const uint32_t size = d.dtype == TAM_DTYPE_F32 ? 4u : 2u;
+    const uint64_t ld = (uint64_t)d.cols * size;
+    soon = {static_cast<const char*>(d.out) + r0 * ld + (uint64_t)c0 * size, ld, d.rows - r0, (d.cols - c0) * size, TILE * size};
+    if (((uintptr_t)soon.base | ld) & 3u) soon.base = nullptr;
+  }
   if (d.tall) {
     Tall t;
     t.zero();
-    t.template run<true>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.lds, smem, {terms, d.s_low * 2, d.x_low * 2});
+    t.template run<true>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.lds, smem, soon, {terms, d.s_low * 2, d.x_low * 2});
     finish(t);
   } else {
     Wide t;
     t.zero();
-    t.template run<true>(operand(x, d.ldx, d.ldx), p, c0, r0, 0, d.rows, smem, {terms, d.x_low * 2, d.s_low * 2});
+    t.template run<true>(operand(x, d.ldx, d.ldx), p, c0, r0, 0, d.rows, smem, soon, {terms, d.x_low * 2, d.s_low * 2});
     finish(t);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// small matrices: everything in one workgroup
+// ---------------------------------------------------------------------------
+// Sides of up to 128: x, and q and then p in its place, with their low parts, lie in
+// LDS (128 KB), s rows of up to 128 columns (a tall matrix transposed), and the
+// three products of a step run on the 8 waves, 16 rows of the result to each, with
+// barriers between them. All types take the three products of parts. One launch for
+// any number of such matrices: 128 x 96 in fp32 took 110 us in 18 launches of 4 to
+// 8 us each, most of that the way to memory and back between them.
+constexpr uint32_t kSmall = 128;
+constexpr uint32_t kSmallThreads = 512;
+
+// Rows of 256 bytes, 16-byte chunk c of row r at place c ^ (r & 15).
+__device__ __forceinline__ uint32_t small_at(uint32_t row, uint32_t col) {
+  return row * 256u + (((col >> 3) ^ (row & 15u)) << 4) + (col & 7u) * 2u;
+}
+
+// Rows row0 .. + 15, k = k0 .. k0 + 31 along the row.
+__device__ __forceinline__ tam_frag<tam_f16> small_rows(const tam_lds_char* m, uint32_t row0, uint32_t k0, uint32_t lane) {
+  tam_frag<tam_f16> f;
+  f.v = *(const tam_lds_s8*)(m + small_at(row0 + (lane & 15u), k0 + 8u * (lane >> 4)));
+  return f;
+}
+
+// Columns col0 .. + 15, k = k0 .. k0 + 31 down the rows (the transposing read).
+__device__ __forceinline__ tam_frag<tam_f16> small_columns(const tam_lds_char* m, uint32_t col0, uint32_t k0, uint32_t lane) {
+  const uint32_t i = lane & 15u, k = k0 + 8u * (lane >> 4) + (i >> 2), col = col0 + 4u * (i & 3u);
+  const tam_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tam_lds_s4*)(m + small_at(k, col)));
+  const tam_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tam_lds_s4*)(m + small_at(k + 4u, col)));
+  tam_frag<tam_f16> f;
+  f.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return f;
+}
+
+// 4 elements (times 2^12) at row, col in both parts.
+__device__ __forceinline__ void small_store(char* high, char* low, uint32_t row, uint32_t col, const tam_f4& v) {
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  f16x4 h, r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float x = v[j];
+    asm("" : "+v"(x));  // as in store_parts
+    h[j] = (tam_f16)x;
+    r[j] = (tam_f16)(x - (float)h[j]);
+  }
+  *reinterpret_cast<f16x4*>(high + small_at(row, col)) = h;
+  *reinterpret_cast<f16x4*>(low + small_at(row, col)) = r;
+}
+
+template <typename T>
+__device__ __forceinline__ void small_out(const mat& d, uint32_t row, uint32_t col, float v) {
+  T* out = static_cast<T*>(d.out) + (uint64_t)row * d.cols + col;
+  *out = tam_from_f<T>(d.flags & TAM_MATRIX_UPDATE ? __builtin_fmaf(-d.rate, v, d.decay * tam_to_f(*out)) : v);
+}
+
+__global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list, coefficients co, uint32_t steps) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * 32768];
+  __shared__ float lds[8];
+  char *const xh = smem, *const xl = smem + 32768, *const qh = smem + 65536, *const ql = smem + 98304;
+  const tam_lds_char *const Xh = (tam_lds_char*)xh, *const Xl = (tam_lds_char*)xl;
+  const tam_lds_char *const Qh = (tam_lds_char*)qh, *const Ql = (tam_lds_char*)ql;
+  const mat& d = list[blockIdx.x];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t s = d.s, width = d.tall ? d.rows : d.cols;
+  // elements past the matrix are zeros in every factor
+  for (uint32_t i = threadIdx.x; i < sizeof(smem) / 16; i += kSmallThreads)
+    reinterpret_cast<tam_i4*>(smem)[i] = tam_i4{0, 0, 0, 0};
+  constexpr int GROUPS = kSmall * kSmall / 8 / kSmallThreads;
+  float u[GROUPS][8];
+  float sum = 0.f;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const uint64_t at = (uint64_t)(g * kSmallThreads + threadIdx.x) * 8u;
+    const uint32_t count = at >= d.elements ? 0u : (d.elements - at < 8 ? (uint32_t)(d.elements - at) : 8u);
+    float gr[8], m[8] = {};
+    load_grad(d, at, count, gr);
+    if (d.momentum) {
+      load_f32(d.momentum + at, count, m);
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        m[j] = __builtin_fmaf(d.one_minus_keep, gr[j], d.keep * m[j]);
+        if (j < count) d.momentum[at + j] = m[j];
+      }
+    }
+    direction(d, gr, m, u[g]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(u[g][j], u[g][j], sum);
+  }
+  sum = tam_wave_sum(sum);
+  if (lane == 0) lds[wave] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += lds[w];
+  const float norm = sqrtf(sum), scale = kScale / (norm < d.eps ? d.eps : norm);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const uint32_t at = (g * kSmallThreads + threadIdx.x) * 8u;
+    uint32_t row = at / d.cols, col = at - row * d.cols;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      if (at + j < d.elements) {
+        float x = u[g][j] * scale;
+        asm("" : "+v"(x));  // as in store_parts
+        const tam_f16 h = (tam_f16)x;
+        const uint32_t to = d.tall ? small_at(col, row) : small_at(row, col);
+        *reinterpret_cast<tam_f16*>(xh + to) = h;
+        *reinterpret_cast<tam_f16*>(xl + to) = (tam_f16)(x - (float)h);
+      }
+      if (++col == d.cols) {
+        col = 0;
+        ++row;
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t row0 = wave * 16, rows = (s + 15) / 16, columns = (width + 15) / 16;
+  const uint32_t row = row0 + (lane & 15u), quad = (lane >> 4) * 4u;
+  const bool works = wave < rows;
+  for (uint32_t step = 0; step < steps; ++step) {
+    tam_f4 acc[kSmall / 16];
+    if (works) {  // q = x x^T
+#pragma unroll
+      for (uint32_t n = 0; n < kSmall / 16; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t k = 0; k < width; k += 32) {
+        const tam_frag<tam_f16> h = small_rows(Xh, row0, k, lane), r = small_rows(Xl, row0, k, lane);
+#pragma unroll
+        for (uint32_t n = 0; n < kSmall / 16; ++n)
+          if (n < rows) {
+            const tam_frag<tam_f16> ch = small_rows(Xh, n * 16, k, lane), cr = small_rows(Xl, n * 16, k, lane);
+            acc[n] = tam_mfma(ch, h, acc[n]);
+            acc[n] = tam_mfma(ch, r, acc[n]);
+            acc[n] = tam_mfma(cr, h, acc[n]);
+          }
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < kSmall / 16; ++n)
+        if (n < rows) small_store(qh, ql, row, n * 16 + quad, acc[n] * (1.f / kScale));
+    }
+    __syncthreads();
+    if (works) {  // p = a I + b q + c q q
+#pragma unroll
+      for (uint32_t n = 0; n < kSmall / 16; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t k = 0; k < s; k += 32) {
+        const tam_frag<tam_f16> h = small_rows(Qh, row0, k, lane), r = small_rows(Ql, row0, k, lane);
+#pragma unroll
+        for (uint32_t n = 0; n < kSmall / 16; ++n)
+          if (n < rows) {
+            const tam_frag<tam_f16> ch = small_rows(Qh, n * 16, k, lane), cr = small_rows(Ql, n * 16, k, lane);
+            acc[n] = tam_mfma(ch, h, acc[n]);
+            acc[n] = tam_mfma(ch, r, acc[n]);
+            acc[n] = tam_mfma(cr, h, acc[n]);
+          }
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < kSmall / 16; ++n)
+        if (n < rows) {
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t col = n * 16 + quad + j, from = small_at(row, col);
+            const float q = (float)*reinterpret_cast<const tam_f16*>(qh + from) + (float)*reinterpret_cast<const tam_f16*>(ql + from);
+            acc[n][j] = __builtin_fmaf(co.b, q, co.c / kScale * acc[n][j]) + (col == row && row < s ? co.a * kScale : 0.f);
+          }
+        }
+    }
+    __syncthreads();  // q is read
+    if (works) {
+#pragma unroll
+      for (uint32_t n = 0; n < kSmall / 16; ++n)
+        if (n < rows) small_store(qh, ql, row, n * 16 + quad, acc[n]);
+    }
+    __syncthreads();
+    if (works) {  // p x
+#pragma unroll
+      for (uint32_t n = 0; n < kSmall / 16; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t k = 0; k < s; k += 32) {
+        const tam_frag<tam_f16> h = small_rows(Qh, row0, k, lane), r = small_rows(Ql, row0, k, lane);
+#pragma unroll
+        for (uint32_t n = 0; n < kSmall / 16; ++n)
+          if (n < columns) {
+            const tam_frag<tam_f16> ch = small_columns(Xh, n * 16, k, lane), cr = small_columns(Xl, n * 16, k, lane);
+            acc[n] = tam_mfma(ch, h, acc[n]);
+            acc[n] = tam_mfma(ch, r, acc[n]);
+            acc[n] = tam_mfma(cr, h, acc[n]);
+          }
+      }
+    }
+    __syncthreads();  // x is read
+    if (!works) continue;
+#pragma unroll
+    for (uint32_t n = 0; n < kSmall / 16; ++n) {
+      if (n >= columns) continue;
+      if (step + 1 < steps) {
+        small_store(xh, xl, row, n * 16 + quad, acc[n] * (1.f / kScale));
+        continue;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t col = n * 16 + quad + j, r = d.tall ? col : row, c = d.tall ? row : col;
+        if (r >= d.rows || c >= d.cols) continue;
+        const float v = acc[n][j] * (1.f / kScale) * (1.f / kScale);
+        if (d.dtype == TAM_DTYPE_F32)
+          small_out<float>(d, r, c, v);
+        else if (d.dtype == TAM_DTYPE_BF16)
+          small_out<tam_bf16>(d, r, c, v);
+        else
+          small_out<tam_f16>(d, r, c, v);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -485,10 +769,13 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 
 // host side
 // ---------------------------------------------------------------------------
 struct plan {
-  std::vector<mat> m;
+  std::vector<mat> m;  // `large` ones, then the small ones
+  int large;
   uint64_t bytes;
   int tile[PHASES];
   uint32_t units[PHASES];
+  uint32_t parts;      // of the Gram products' sums
+  float* sums;
 };
 
 int check(const TamMatrix* m, int n) {
@@ -510,26 +797,38 @@ int check(const TamMatrix* m, int n) {
 uint64_t tiles(uint64_t rows, uint64_t cols, int t) { return tam_div_up(rows, t) * tam_div_up(cols, t); }
 uint64_t triangle_tiles(uint64_t s, int t) { return tam_div_up(s, t) * (tam_div_up(s, t) + 1) / 2; }
 
-// The tile of a phase: the least of what its launch takes at the measured rates
-// (tam_tiles_us), for all tiles as if of one k, and no less than the longest one.
-int pick_tile(const std::vector<mat>& m, bool square) {
+// The tile of a phase, and (GRAM) the parts that its sums are cut into: the least of
+// what the launches take at the measured rates (tam_tiles_us), for all tiles as if of
+// one k, and no less than the longest one. Parts are of 64 x 64 tiles, and their sums
+// go to memory and back (about 4 TB/s) through one launch more.
+struct shape {
+  int tile;
+  uint32_t parts;
+};
+
+shape pick(const mat* m, int n, int phase) {
   const double cus = tam_op_cus();
-  int best = 64;
+  shape best = {64, 1};
   double least = 1e30;
   for (const tam_tile_rate& t : tam_rates_16) {
     double count = 0, sum = 0, longest = 0;
-    for (const mat& d : m) {
+    for (int i = 0; i < n; ++i) {
+      const mat& d = m[i];
       // q's sum runs over the longer side, p's and x's over the shorter one
-      const double k = (square ? std::max(d.rows, d.cols) : d.s) * (d.split ? 3.0 : 1.0);
-      const double n = (double)(square ? triangle_tiles(d.s, t.tile) : tiles(d.rows, d.cols, t.tile));
-      count += n;
-      sum += n * k;
+      const double k = (phase == GRAM ? std::max(d.rows, d.cols) : d.s) * (d.split ? 3.0 : 1.0);
+      const double c = (double)(phase == APPLY ? tiles(d.rows, d.cols, t.tile) : triangle_tiles(d.s, t.tile));
+      count += c;
+      sum += c * k;
       longest = std::max(longest, k);
     }
-    const double us = std::max(tam_tiles_us(t, count, sum / count, cus), t.start + longest * t.half);
-    if (us < least) {
-      least = us;
-      best = t.tile;
+    for (uint32_t parts : {1, 2, 4, 8, 16, 32}) {
+      if (parts > 1 && (phase != GRAM || t.tile != 64 || longest / parts < 256)) break;
+      double us = std::max(tam_tiles_us(t, count * parts, sum / count / parts, cus), t.start + longest / parts * t.half);
+      if (parts > 1) us += 4.0 + count * parts * (64 * 64 * 8) / 4e6;
+      if (us < least) {
+        least = us;
+        best = {t.tile, parts};
+      }
     }
   }
   return best;
@@ -542,6 +841,7 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
   auto larger = [&](int i) { return std::max(in[i].rows, in[i].cols); };
   std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return larger(i) > larger(j); });
   out.m.resize(n);
+  out.large = 0;
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     char* p = (char*)((uintptr_t)base + at);
@@ -571,6 +871,8 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
     m.eps = d.eps;
     m.decay = d.decay;
     m.rate = d.rate;
+    if (std::max(m.rows, m.cols) <= kSmall) continue;  // these come last
+    out.large = k + 1;
     m.x_low = (int64_t)tam_up((uint64_t)m.rows * m.ldx, 128);
     const int64_t square = (int64_t)tam_up((uint64_t)m.s * m.lds, 128);
     m.s_low = m.split ? square : 0;
@@ -582,14 +884,18 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
     m.partials = (uint32_t)tam_div_up(m.elements, m.chunk);
     m.partial = (float*)take((uint64_t)m.partials * 4);
   }
-  out.bytes = at;
-  out.tile[SQUARE] = pick_tile(out.m, true);
-  out.tile[APPLY] = pick_tile(out.m, false);
+  for (int f = GRAM; f < PHASES; ++f) {
+    const shape s = pick(out.m.data(), out.large, f);
+    out.tile[f] = s.tile;
+    if (f == GRAM) out.parts = s.parts;
+  }
   uint64_t units[PHASES] = {};
-  for (mat& m : out.m) {
+  for (int i = 0; i < out.large; ++i) {
+    mat& m = out.m[i];
     for (int f = 0; f < PHASES; ++f) m.first[f] = (uint32_t)units[f];
     units[MOMENTUM] += m.partials;
     units[START] += tam_div_up((uint64_t)m.rows * m.ldx, kStart);
+    units[GRAM] += triangle_tiles(m.s, out.tile[GRAM]);
     units[SQUARE] += triangle_tiles(m.s, out.tile[SQUARE]);
     units[APPLY] += tiles(m.rows, m.cols, out.tile[APPLY]);
   }
@@ -597,18 +903,20 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
     if (units[f] >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "matrices of too many elements for one call");
     out.units[f] = (uint32_t)units[f];
   }
+  out.sums = out.parts > 1 ? (float*)take(units[GRAM] * out.parts * (64 * 64 * 4)) : nullptr;
+  out.bytes = at;
   return TAM_OK;
 }
 
-template <bool GRAM>
+template <bool FIRST>
 void launch_square(int tile, const list& l, uint32_t turn, coefficients co, hipStream_t s) {
-  const dim3 grid(l.units[SQUARE]);
+  const dim3 grid(l.units[FIRST ? GRAM : SQUARE], FIRST ? l.parts : 1);
   if (tile == 256)
-    hipLaunchKernelGGL((tam_k_mu_square<256, 2, 4, GRAM>), grid, dim3(512), 0, s, l, turn, co);
+    hipLaunchKernelGGL((tam_k_mu_square<256, 2, 4, FIRST>), grid, dim3(512), 0, s, l, turn, co);
   else if (tile == 128)
-    hipLaunchKernelGGL((tam_k_mu_square<128, 2, 2, GRAM>), grid, dim3(256), 0, s, l, turn, co);
+    hipLaunchKernelGGL((tam_k_mu_square<128, 2, 2, FIRST>), grid, dim3(256), 0, s, l, turn, co);
   else
-    hipLaunchKernelGGL((tam_k_mu_square<64, 2, 2, GRAM>), grid, dim3(256), 0, s, l, turn, co);
+    hipLaunchKernelGGL((tam_k_mu_square<64, 2, 2, FIRST>), grid, dim3(256), 0, s, l, turn, co);
 }
 
 template <bool LAST>
@@ -651,17 +959,27 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
     hipLaunchKernelGGL(tam_k_mu_put, dim3(1), dim3(256), 0, s, a, table + i, (uint32_t)k);
     TAM_OP_LAUNCHED("the descriptors");
   }
-  list l = {table, (uint32_t)n, {}};
+  const coefficients co = {c[0], c[1], c[2]};
+  if (p.large < n) {
+    hipLaunchKernelGGL(tam_k_mu_small, dim3((uint32_t)(n - p.large)), dim3(kSmallThreads), 0, s, table + p.large, co,
+                       (uint32_t)steps);
+    TAM_OP_LAUNCHED("the small matrices");
+  }
+  if (!p.large) return TAM_OK;
+  list l = {table, (uint32_t)p.large, {}, p.parts, p.sums};
   for (int f = 0; f < PHASES; ++f) l.units[f] = p.units[f];
   hipLaunchKernelGGL(tam_k_mu_momentum, dim3(l.units[MOMENTUM]), dim3(kThreads), 0, s, l);
   TAM_OP_LAUNCHED("the momentum");
   hipLaunchKernelGGL(tam_k_mu_start, dim3(l.units[START]), dim3(kThreads), 0, s, l);
   TAM_OP_LAUNCHED("the normalisation");
-  const coefficients co = {c[0], c[1], c[2]};
   for (int i = 0; i < steps; ++i) {
     const uint32_t turn = i & 1;
-    launch_square<true>(p.tile[SQUARE], l, turn, co, s);
+    launch_square<true>(p.tile[GRAM], l, turn, co, s);
     TAM_OP_LAUNCHED("the Gram product");
+    if (p.parts > 1) {
+      hipLaunchKernelGGL(tam_k_mu_join, dim3(l.units[GRAM]), dim3(kThreads), 0, s, l);
+      TAM_OP_LAUNCHED("the Gram product's sums");
+    }
     launch_square<false>(p.tile[SQUARE], l, turn, co, s);
     TAM_OP_LAUNCHED("the polynomial");
     if (i + 1 < steps)
