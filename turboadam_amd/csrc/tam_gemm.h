@@ -18,12 +18,12 @@
 // load returns as zeros: no size needs a tail loop, and the stages past the
 // last one are zeros too, so every step issues the same loads.
 //
-// Pipeline.  Two buffers, fragments of half a stage in registers twice.  Step t:
+// Pipeline.  STAGES buffers, fragments of half a stage in registers twice.  Step t:
 // read the second half's fragments of stage t among the matrix instructions of the
 // first half; wait for stage t+1 and for the own reads, barrier: nobody reads
-// stage t's buffer any more; issue the loads of stage t+2 into it; read the first
+// stage t's buffer any more; issue the loads of stage t+STAGES into it; read the first
 // half of stage t+1 among the matrix instructions of the second half of t.  One
-// barrier a step, and a load has a whole step to arrive.
+// barrier a step, and a load has STAGES-1 steps to arrive.
 //
 // Fragments.  mfma 16x16x32 (16 bits) or four 16x16x4 (fp32), P as the left
 // operand: a lane then holds 4 consecutive columns c of one row r.
@@ -34,7 +34,6 @@
 
 #include "tam_ops.h"
 
-#define TAM_GEMM_STAGES 2
 #define TAM_GEMM_ROW 128  // bytes of a row in a stage
 
 typedef short tam_s4 __attribute__((ext_vector_type(4)));
@@ -208,9 +207,17 @@ struct tam_soon {
   uint32_t width;           // bytes of a tile's row: a power of two from 64 to 1024
 };
 
+// Stages of a tile in LDS: two, but three of the small tiles of 16-bit types, whose
+// steps are shorter than the way to memory (k = 4096, 64 tiles: 32 us with two, 18
+// with three; 128-wide tiles gain nothing from more, and lose a neighbour).
+template <typename T, int TILE>
+constexpr int tam_stages() {
+  return TILE == 64 && sizeof(T) == 2 ? 3 : 2;
+}
+
 // One workgroup's tile: BM rows (operand Q) by BN columns (operand P), WM by
 // WN waves.
-template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK>
 struct tam_tile {
   static constexpr int NW = WM * WN;
   static constexpr int THREADS = 64 * NW;
@@ -225,7 +232,7 @@ struct tam_tile {
   static constexpr int COLS = BN / WN;                    // a wave's columns
   static constexpr int PITCH = COLS + 4;                  // floats of a turned row
   static constexpr int TURN = NW * ROUND * PITCH * 4;
-  static constexpr int DUMP = TAM_GEMM_STAGES * STAGE > TURN ? TAM_GEMM_STAGES * STAGE : TURN;
+  static constexpr int DUMP = STAGES * STAGE > TURN ? STAGES * STAGE : TURN;
   static constexpr int LDS = DUMP + NW * 256;  // the words that `soon` fetches
   static_assert(TM % 2 == 0, "rounds of 32 rows");
 
@@ -321,11 +328,11 @@ struct tam_tile {
     };
     __syncthreads();  // the LDS may hold what another tile's epilogue still reads
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) load(i, 0);
+    for (int s = 0; s < STAGES; ++s)
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) load(i, 1);
+      for (int i = 0; i < LOADS; ++i) load(i, s);
     frags a, b;
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * LOADS) : "memory");
 #pragma unroll
     for (int n = 0; n < TN; ++n) SP::read(a.p[n], lds, (wn * TN + n) * 16, 0, lane);
 #pragma unroll
@@ -333,11 +340,12 @@ struct tam_tile {
     uint32_t cur = 0;  // buffer of stage t
     const uint32_t last = steps > 2 && soon.base ? steps - 2 : ~0u;
     for (uint32_t t = 0; t < steps; ++t) {
+      const uint32_t next = cur + 1 == STAGES ? 0 : cur + 1;
       half(a, b, cur, 1, 0, std::false_type());
-      sync<0>();
+      sync<(STAGES - 2) * LOADS>();
       if (t == last) fetch();
-      half(b, a, cur ^ 1u, 0, cur, std::true_type());
-      cur ^= 1u;
+      half(b, a, next, 0, cur, std::true_type());
+      cur = next;
     }
     sync<0>();  // the LDS is the epilogue's
   }
@@ -446,18 +454,18 @@ __device__ __forceinline__ void tam_tile_at(uint32_t t, uint32_t tm, uint32_t tn
 // Measured on one MI355X, tiles of k = 256 .. 4096 in launches of 16 to 1024 tiles
 // (bf16; fp32 in the second table): a launch that leaves half of the compute units
 // empty takes start + k * half us; with r tiles on each unit (at most `resident`
-// fit: 128, 64 and 32 KB of LDS) start + k * per_k[r - 1]. At k = 4096 and many
-// tiles that is 1460 TFLOP/s for 256, 980 for 128 and 690 for 64 (fp32: 133 for
-// both); 16 tiles of k = 256 take 10.4, 6.1 and 3.5 us.
+// fit: 136, 68 and 49, fp32 33, KB of LDS) start + k * per_k[r - 1]. At k = 4096 and
+// 1024 tiles that is 1430 TFLOP/s for 256, 1150 for 128 and 640 for 64 (fp32: 145 and
+// 134); 16 tiles of k = 256 take 12, 6 and 4 us.
 struct tam_tile_rate {
   int tile, resident;
   double start, half, per_k[4];
 };
-static const tam_tile_rate tam_rates_16[3] = {{256, 1, 5.0, 0.0168, {0.0224}},
-                                              {128, 2, 3.5, 0.0091, {0.0111, 0.0163}},
-                                              {64, 4, 2.4, 0.0040, {0.0048, 0.0064, 0.0090, 0.0116}}};
-static const tam_tile_rate tam_rates_32[2] = {{128, 2, 4.5, 0.0700, {0.0715, 0.1270}},
-                                              {64, 4, 2.4, 0.0182, {0.0188, 0.0330, 0.0480, 0.0633}}};
+static const tam_tile_rate tam_rates_16[3] = {{256, 1, 6.0, 0.0166, {0.0225}},
+                                              {128, 2, 3.9, 0.0085, {0.0095, 0.0140}},
+                                              {64, 3, 2.6, 0.0038, {0.0040, 0.0056, 0.0085}}};
+static const tam_tile_rate tam_rates_32[2] = {{128, 2, 6.0, 0.0600, {0.0612, 0.1155}},
+                                              {64, 4, 2.8, 0.0180, {0.0184, 0.0315, 0.0470, 0.0622}}};
 
 // us of `tiles` tiles of k: whole rounds, then what is left.
 static inline double tam_tiles_us(const tam_tile_rate& t, double tiles, double k, double cus) {

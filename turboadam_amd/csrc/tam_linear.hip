@@ -130,8 +130,8 @@ struct tam_gemm_args {
 };
 
 template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK>
-__global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 2 : (BM == 128 ? 3 : 4)) void tam_k_gemm(tam_gemm_args a) {
-  typedef tam_tile<T, BM, BN, WM, WN, PK, QK> Tile;
+__global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam_gemm_args a) {
+  typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, QK> Tile;
   __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
   uint32_t m, n;
   tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);

@@ -285,10 +285,10 @@ __device__ __forceinline__ void triangle(uint32_t t, uint32_t& m, uint32_t& n) {
 
 // FIRST: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q.
 template <int TILE, int WM, int WN, bool FIRST>
-__global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 4)) void tam_k_mu_square(
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_square(
     list l, uint32_t turn, coefficients co) {
-  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, true, true> Rows;
-  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, false, false> Columns;
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), true, true> Rows;
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), false, false> Columns;
   __shared__ __attribute__((aligned(16))) char smem[Rows::LDS > Columns::LDS ? Rows::LDS : Columns::LDS];
   const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
   const mat& d = l.m[owner<FIRST ? GRAM : SQUARE>(l, unit)];
@@ -462,10 +462,10 @@ __device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t c
 
 // x' = p x (tall: x p); LAST: the output instead.
 template <int TILE, int WM, int WN, bool LAST>
-__global__ __launch_bounds__(64 * WM * WN, TILE == 256 ? 2 : (TILE == 128 ? 3 : 4)) void tam_k_mu_apply(list l,
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_apply(list l,
                                                                                                        uint32_t turn) {
-  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, false, true> Wide;
-  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, true, true> Tall;
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), false, true> Wide;
+  typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), true, true> Tall;
   __shared__ __attribute__((aligned(16))) char smem[Wide::LDS > Tall::LDS ? Wide::LDS : Tall::LDS];
   const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
   const mat& d = l.m[owner<APPLY>(l, unit)];
@@ -607,6 +607,9 @@ __device__ __forceinline__ void small_out(const mat& d, uint32_t row, uint32_t c
   *out = tam_from_f<T>(d.flags & TAM_MATRIX_UPDATE ? __builtin_fmaf(-d.rate, v, d.decay * tam_to_f(*out)) : v);
 }
 
+// BLOCKS: 16-column blocks of the largest matrix (2, 4 or 8); all of them are
+// computed, zeros or not, so that the reads of one k run ahead of its products.
+template <int BLOCKS>
 __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list, coefficients co, uint32_t steps) {
   __shared__ __attribute__((aligned(16))) char smem[4 * 32768];
   __shared__ float lds[8];
@@ -619,7 +622,7 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list,
   // elements past the matrix are zeros in every factor
   for (uint32_t i = threadIdx.x; i < sizeof(smem) / 16; i += kSmallThreads)
     reinterpret_cast<tam_i4*>(smem)[i] = tam_i4{0, 0, 0, 0};
-  constexpr int GROUPS = kSmall * kSmall / 8 / kSmallThreads;
+  constexpr int GROUPS = (BLOCKS * BLOCKS * 32 + (int)kSmallThreads - 1) / (int)kSmallThreads;  // of 8 elements a thread
   float u[GROUPS][8];
   float sum = 0.f;
 #pragma unroll
@@ -672,42 +675,40 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list,
   const uint32_t row = row0 + (lane & 15u), quad = (lane >> 4) * 4u;
   const bool works = wave < rows;
   for (uint32_t step = 0; step < steps; ++step) {
-    tam_f4 acc[kSmall / 16];
+    tam_f4 acc[BLOCKS];
     if (works) {  // q = x x^T
 #pragma unroll
-      for (uint32_t n = 0; n < kSmall / 16; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t n = 0; n < BLOCKS; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
       for (uint32_t k = 0; k < width; k += 32) {
         const tam_frag<tam_f16> h = small_rows(Xh, row0, k, lane), r = small_rows(Xl, row0, k, lane);
 #pragma unroll
-        for (uint32_t n = 0; n < kSmall / 16; ++n)
-          if (n < rows) {
-            const tam_frag<tam_f16> ch = small_rows(Xh, n * 16, k, lane), cr = small_rows(Xl, n * 16, k, lane);
-            acc[n] = tam_mfma(ch, h, acc[n]);
-            acc[n] = tam_mfma(ch, r, acc[n]);
-            acc[n] = tam_mfma(cr, h, acc[n]);
-          }
+        for (uint32_t n = 0; n < BLOCKS; ++n) {
+          const tam_frag<tam_f16> ch = small_rows(Xh, n * 16, k, lane), cr = small_rows(Xl, n * 16, k, lane);
+          acc[n] = tam_mfma(ch, h, acc[n]);
+          acc[n] = tam_mfma(ch, r, acc[n]);
+          acc[n] = tam_mfma(cr, h, acc[n]);
+        }
       }
 #pragma unroll
-      for (uint32_t n = 0; n < kSmall / 16; ++n)
+      for (uint32_t n = 0; n < BLOCKS; ++n)
         if (n < rows) small_store(qh, ql, row, n * 16 + quad, acc[n] * (1.f / kScale));
     }
     __syncthreads();
     if (works) {  // p = a I + b q + c q q
 #pragma unroll
-      for (uint32_t n = 0; n < kSmall / 16; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t n = 0; n < BLOCKS; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
       for (uint32_t k = 0; k < s; k += 32) {
         const tam_frag<tam_f16> h = small_rows(Qh, row0, k, lane), r = small_rows(Ql, row0, k, lane);
 #pragma unroll
-        for (uint32_t n = 0; n < kSmall / 16; ++n)
-          if (n < rows) {
-            const tam_frag<tam_f16> ch = small_rows(Qh, n * 16, k, lane), cr = small_rows(Ql, n * 16, k, lane);
-            acc[n] = tam_mfma(ch, h, acc[n]);
-            acc[n] = tam_mfma(ch, r, acc[n]);
-            acc[n] = tam_mfma(cr, h, acc[n]);
-          }
+        for (uint32_t n = 0; n < BLOCKS; ++n) {
+          const tam_frag<tam_f16> ch = small_rows(Qh, n * 16, k, lane), cr = small_rows(Ql, n * 16, k, lane);
+          acc[n] = tam_mfma(ch, h, acc[n]);
+          acc[n] = tam_mfma(ch, r, acc[n]);
+          acc[n] = tam_mfma(cr, h, acc[n]);
+        }
       }
 #pragma unroll
-      for (uint32_t n = 0; n < kSmall / 16; ++n)
+      for (uint32_t n = 0; n < BLOCKS; ++n)
         if (n < rows) {
 #pragma unroll
           for (uint32_t j = 0; j < 4; ++j) {
@@ -720,45 +721,44 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list,
     __syncthreads();  // q is read
     if (works) {
 #pragma unroll
-      for (uint32_t n = 0; n < kSmall / 16; ++n)
+      for (uint32_t n = 0; n < BLOCKS; ++n)
         if (n < rows) small_store(qh, ql, row, n * 16 + quad, acc[n]);
     }
     __syncthreads();
     if (works) {  // p x
 #pragma unroll
-      for (uint32_t n = 0; n < kSmall / 16; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t n = 0; n < BLOCKS; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
       for (uint32_t k = 0; k < s; k += 32) {
         const tam_frag<tam_f16> h = small_rows(Qh, row0, k, lane), r = small_rows(Ql, row0, k, lane);
 #pragma unroll
-        for (uint32_t n = 0; n < kSmall / 16; ++n)
-          if (n < columns) {
-            const tam_frag<tam_f16> ch = small_columns(Xh, n * 16, k, lane), cr = small_columns(Xl, n * 16, k, lane);
-            acc[n] = tam_mfma(ch, h, acc[n]);
-            acc[n] = tam_mfma(ch, r, acc[n]);
-            acc[n] = tam_mfma(cr, h, acc[n]);
-          }
+        for (uint32_t n = 0; n < BLOCKS; ++n) {
+          const tam_frag<tam_f16> ch = small_columns(Xh, n * 16, k, lane), cr = small_columns(Xl, n * 16, k, lane);
+          acc[n] = tam_mfma(ch, h, acc[n]);
+          acc[n] = tam_mfma(ch, r, acc[n]);
+          acc[n] = tam_mfma(cr, h, acc[n]);
+        }
       }
     }
     __syncthreads();  // x is read
-    if (!works) continue;
+    if (works) {
 #pragma unroll
-    for (uint32_t n = 0; n < kSmall / 16; ++n) {
-      if (n >= columns) continue;
-      if (step + 1 < steps) {
-        small_store(xh, xl, row, n * 16 + quad, acc[n] * (1.f / kScale));
-        continue;
-      }
+      for (uint32_t n = 0; n < BLOCKS; ++n) {
+        if (step + 1 < steps) {
+          if (n < columns) small_store(xh, xl, row, n * 16 + quad, acc[n] * (1.f / kScale));
+          continue;
+        }
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t col = n * 16 + quad + j, r = d.tall ? col : row, c = d.tall ? row : col;
-        if (r >= d.rows || c >= d.cols) continue;
-        const float v = acc[n][j] * (1.f / kScale) * (1.f / kScale);
-        if (d.dtype == TAM_DTYPE_F32)
-          small_out<float>(d, r, c, v);
-        else if (d.dtype == TAM_DTYPE_BF16)
-          small_out<tam_bf16>(d, r, c, v);
-        else
-          small_out<tam_f16>(d, r, c, v);
+        for (uint32_t j = 0; j < 4; ++j) {
+          const uint32_t col = n * 16 + quad + j, r = d.tall ? col : row, c = d.tall ? row : col;
+          if (r >= d.rows || c >= d.cols) continue;
+          const float v = acc[n][j] * (1.f / kScale) * (1.f / kScale);
+          if (d.dtype == TAM_DTYPE_F32)
+            small_out<float>(d, r, c, v);
+          else if (d.dtype == TAM_DTYPE_BF16)
+            small_out<tam_bf16>(d, r, c, v);
+          else
+            small_out<tam_f16>(d, r, c, v);
+        }
       }
     }
     __syncthreads();
@@ -961,8 +961,14 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
   }
   const coefficients co = {c[0], c[1], c[2]};
   if (p.large < n) {
-    hipLaunchKernelGGL(tam_k_mu_small, dim3((uint32_t)(n - p.large)), dim3(kSmallThreads), 0, s, table + p.large, co,
-                       (uint32_t)steps);
+    const uint32_t side = std::max(p.m[p.large].rows, p.m[p.large].cols);  // the list's largest
+    const dim3 grid((uint32_t)(n - p.large)), block(kSmallThreads);
+    if (side <= 32)
+      hipLaunchKernelGGL(tam_k_mu_small<2>, grid, block, 0, s, table + p.large, co, (uint32_t)steps);
+    else if (side <= 64)
+      hipLaunchKernelGGL(tam_k_mu_small<4>, grid, block, 0, s, table + p.large, co, (uint32_t)steps);
+    else
+      hipLaunchKernelGGL(tam_k_mu_small<8>, grid, block, 0, s, table + p.large, co, (uint32_t)steps);
     TAM_OP_LAUNCHED("the small matrices");
   }
   if (!p.large) return TAM_OK;
