@@ -557,10 +557,11 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
 // ---------------------------------------------------------------------------
 // Sides of up to 128: x, and q and then p in its place, with their low parts, lie in
 // LDS (128 KB), s rows of up to 128 columns (a tall matrix transposed), and the
-// three products of a step run on the 8 waves, 16 rows of the result to each, with
-// barriers between them. All types take the three products of parts. One launch for
-// any number of such matrices: 128 x 96 in fp32 took 110 us in 18 launches of 4 to
-// 8 us each, most of that the way to memory and back between them.
+// three products of a step run on the 8 waves, 32 rows by half of the columns of the
+// result to each, with barriers between them. One launch for any number of such matrices: 128 x 96 in
+// fp32 took 110 us in 18 launches of 4 to 8 us each, most of that the way to memory
+// and back between them; here it takes 17 us and 7 us a step, of which the matrix
+// instructions of one compute unit are 4.
 constexpr uint32_t kSmall = 128;
 constexpr uint32_t kSmallThreads = 512;
 
@@ -610,13 +611,13 @@ __device__ __forceinline__ void small_out(const mat& d, uint32_t row, uint32_t c
 // BLOCKS: 16-column blocks of the largest matrix (2, 4 or 8); all of them are
 // computed, zeros or not, so that the reads of one k run ahead of its products.
 template <int BLOCKS>
-__global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list, coefficients co, uint32_t steps) {
+__global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const mat* list, coefficients co, uint32_t steps) {
   __shared__ __attribute__((aligned(16))) char smem[4 * 32768];
   __shared__ float lds[8];
   char *const xh = smem, *const xl = smem + 32768, *const qh = smem + 65536, *const ql = smem + 98304;
   const tam_lds_char *const Xh = (tam_lds_char*)xh, *const Xl = (tam_lds_char*)xl;
   const tam_lds_char *const Qh = (tam_lds_char*)qh, *const Ql = (tam_lds_char*)ql;
-  const mat& d = list[blockIdx.x];
+  const mat& d = list ? list[blockIdx.x] : only;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t s = d.s, width = d.tall ? d.rows : d.cols;
   // elements past the matrix are zeros in every factor
@@ -671,98 +672,111 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(const mat* list,
     }
   }
   __syncthreads();
-  const uint32_t row0 = wave * 16, rows = (s + 15) / 16, columns = (width + 15) / 16;
-  const uint32_t row = row0 + (lane & 15u), quad = (lane >> 4) * 4u;
-  const bool works = wave < rows;
-  for (uint32_t step = 0; step < steps; ++step) {
-    tam_f4 acc[BLOCKS];
-    if (works) {  // q = x x^T
+  // A wave's part of a result: 32 rows by half of the blocks' columns.
+  constexpr int CB = BLOCKS / 2;
+  const uint32_t row0 = wave / 2 * 32, col0 = wave % 2 * (CB * 16);
+  const uint32_t lane_row = lane & 15u, quad = (lane >> 4) * 4u;
+  const bool works = row0 < s;
+  tam_f4 acc[CB][2];
+  const bool split = d.split;
+  // acc = sum over k of left's rows (of the result) and right's columns, in parts (bf16:
+  // of the high parts)
+  auto product = [&](const tam_lds_char* lh, const tam_lds_char* ll, const tam_lds_char* rh, const tam_lds_char* rl,
+                     uint32_t length, auto right) {
 #pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
-      for (uint32_t k = 0; k < width; k += 32) {
-        const tam_frag<tam_f16> h = small_rows(Xh, row0, k, lane), r = small_rows(Xl, row0, k, lane);
+    for (int n = 0; n < CB; ++n)
 #pragma unroll
-        for (uint32_t n = 0; n < BLOCKS; ++n) {
-          const tam_frag<tam_f16> ch = small_rows(Xh, n * 16, k, lane), cr = small_rows(Xl, n * 16, k, lane);
-          acc[n] = tam_mfma(ch, h, acc[n]);
-          acc[n] = tam_mfma(ch, r, acc[n]);
-          acc[n] = tam_mfma(cr, h, acc[n]);
-        }
+      for (int m = 0; m < 2; ++m) acc[n][m] = tam_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (uint32_t k = 0; k < length; k += 32) {
+      tam_frag<tam_f16> h[2], r[2], ch[CB], cr[CB];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        h[m] = small_rows(lh, row0 + m * 16, k, lane);
+        if (split) r[m] = small_rows(ll, row0 + m * 16, k, lane);
       }
 #pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n)
-        if (n < rows) small_store(qh, ql, row, n * 16 + quad, acc[n] * (1.f / kScale));
+      for (int n = 0; n < CB; ++n) {
+        ch[n] = right(rh, col0 + n * 16, k);
+        if (split) cr[n] = right(rl, col0 + n * 16, k);
+      }
+      // term by term: a sum's next product comes after all the others'
+#pragma unroll
+      for (int n = 0; n < CB; ++n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[n][m] = tam_mfma(ch[n], h[m], acc[n][m]);
+      if (!split) continue;
+#pragma unroll
+      for (int n = 0; n < CB; ++n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[n][m] = tam_mfma(ch[n], r[m], acc[n][m]);
+#pragma unroll
+      for (int n = 0; n < CB; ++n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[n][m] = tam_mfma(cr[n], h[m], acc[n][m]);
+    }
+  };
+  auto in_rows = [&](const tam_lds_char* m, uint32_t first, uint32_t k) { return small_rows(m, first, k, lane); };
+  auto in_columns = [&](const tam_lds_char* m, uint32_t first, uint32_t k) { return small_columns(m, first, k, lane); };
+  // f(row, first of 4 columns, acc) over what the wave holds
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int n = 0; n < CB; ++n)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) f(row0 + m * 16 + lane_row, col0 + n * 16 + quad, acc[n][m]);
+  };
+  for (uint32_t step = 0; step < steps; ++step) {
+    if (works) {  // q = x x^T
+      product(Xh, Xl, Xh, Xl, width, in_rows);
+      each([&](uint32_t row, uint32_t col, tam_f4& v) { small_store(qh, ql, row, col, v * (1.f / kScale)); });
     }
     __syncthreads();
     if (works) {  // p = a I + b q + c q q
+      product(Qh, Ql, Qh, Ql, s, in_rows);
+      each([&](uint32_t row, uint32_t col, tam_f4& v) {
+        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+        const f16x4 h = *reinterpret_cast<const f16x4*>(qh + small_at(row, col));
+        const f16x4 r = *reinterpret_cast<const f16x4*>(ql + small_at(row, col));
 #pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
-      for (uint32_t k = 0; k < s; k += 32) {
-        const tam_frag<tam_f16> h = small_rows(Qh, row0, k, lane), r = small_rows(Ql, row0, k, lane);
-#pragma unroll
-        for (uint32_t n = 0; n < BLOCKS; ++n) {
-          const tam_frag<tam_f16> ch = small_rows(Qh, n * 16, k, lane), cr = small_rows(Ql, n * 16, k, lane);
-          acc[n] = tam_mfma(ch, h, acc[n]);
-          acc[n] = tam_mfma(ch, r, acc[n]);
-          acc[n] = tam_mfma(cr, h, acc[n]);
-        }
-      }
-#pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n)
-        if (n < rows) {
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t col = n * 16 + quad + j, from = small_at(row, col);
-            const float q = (float)*reinterpret_cast<const tam_f16*>(qh + from) + (float)*reinterpret_cast<const tam_f16*>(ql + from);
-            acc[n][j] = __builtin_fmaf(co.b, q, co.c / kScale * acc[n][j]) + (col == row && row < s ? co.a * kScale : 0.f);
-          }
-        }
+        for (uint32_t j = 0; j < 4; ++j)
+          v[j] = __builtin_fmaf(co.b, (float)h[j] + (float)r[j], co.c / kScale * v[j]) +
+                 (col + j == row && row < s ? co.a * kScale : 0.f);
+      });
     }
     __syncthreads();  // q is read
-    if (works) {
-#pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n)
-        if (n < rows) small_store(qh, ql, row, n * 16 + quad, acc[n]);
-    }
+    if (works) each([&](uint32_t row, uint32_t col, tam_f4& v) { small_store(qh, ql, row, col, v); });
     __syncthreads();
     if (works) {  // p x
+      product(Qh, Ql, Xh, Xl, s, in_columns);
+      if (!split)
+        each([&](uint32_t row, uint32_t col, tam_f4& v) {  // and p's diagonal times x's low part
+          typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+          const float p = (float)*reinterpret_cast<const tam_f16*>(qh + small_at(row, row));
+          const f16x4 r = *reinterpret_cast<const f16x4*>(xl + small_at(row, col));
 #pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n) acc[n] = tam_f4{0.f, 0.f, 0.f, 0.f};
-      for (uint32_t k = 0; k < s; k += 32) {
-        const tam_frag<tam_f16> h = small_rows(Qh, row0, k, lane), r = small_rows(Ql, row0, k, lane);
-#pragma unroll
-        for (uint32_t n = 0; n < BLOCKS; ++n) {
-          const tam_frag<tam_f16> ch = small_columns(Xh, n * 16, k, lane), cr = small_columns(Xl, n * 16, k, lane);
-          acc[n] = tam_mfma(ch, h, acc[n]);
-          acc[n] = tam_mfma(ch, r, acc[n]);
-          acc[n] = tam_mfma(cr, h, acc[n]);
-        }
-      }
+          for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(p, (float)r[j], v[j]);
+        });
     }
     __syncthreads();  // x is read
-    if (works) {
-#pragma unroll
-      for (uint32_t n = 0; n < BLOCKS; ++n) {
-        if (step + 1 < steps) {
-          if (n < columns) small_store(xh, xl, row, n * 16 + quad, acc[n] * (1.f / kScale));
-          continue;
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          const uint32_t col = n * 16 + quad + j, r = d.tall ? col : row, c = d.tall ? row : col;
-          if (r >= d.rows || c >= d.cols) continue;
-          const float v = acc[n][j] * (1.f / kScale) * (1.f / kScale);
-          if (d.dtype == TAM_DTYPE_F32)
-            small_out<float>(d, r, c, v);
-          else if (d.dtype == TAM_DTYPE_BF16)
-            small_out<tam_bf16>(d, r, c, v);
-          else
-            small_out<tam_f16>(d, r, c, v);
-        }
-      }
-    }
+    if (works && step + 1 < steps)
+      each([&](uint32_t row, uint32_t col, tam_f4& v) { small_store(xh, xl, row, col, v * (1.f / kScale)); });
     __syncthreads();
   }
+  if (!works) return;
+  each([&](uint32_t row, uint32_t col, tam_f4& v) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t r = d.tall ? col + j : row, c = d.tall ? row : col + j;
+      if (r >= d.rows || c >= d.cols) continue;
+      const float x = v[j] * (1.f / kScale) * (1.f / kScale);
+      if (d.dtype == TAM_DTYPE_F32)
+        small_out<float>(d, r, c, x);
+      else if (d.dtype == TAM_DTYPE_BF16)
+        small_out<tam_bf16>(d, r, c, x);
+      else
+        small_out<tam_f16>(d, r, c, x);
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -952,7 +966,8 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
                        (unsigned long long)p.bytes);
   if ((uintptr_t)workspace & 255u) return tam_op_fail(TAM_E_INVALID, "workspace not on 256 bytes");
   mat* table = (mat*)workspace;
-  for (int i = 0; i < n; i += kPut) {
+  const bool only = n == 1 && !p.large;  // one small matrix goes as an argument
+  for (int i = 0; i < n && !only; i += kPut) {
     put_args a;
     const int k = n - i < kPut ? n - i : kPut;
     for (int j = 0; j < kPut; ++j) a.m[j] = j < k ? p.m[i + j] : mat{};
@@ -963,12 +978,13 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
   if (p.large < n) {
     const uint32_t side = std::max(p.m[p.large].rows, p.m[p.large].cols);  // the list's largest
     const dim3 grid((uint32_t)(n - p.large)), block(kSmallThreads);
+    const mat* list = only ? nullptr : table + p.large;
     if (side <= 32)
-      hipLaunchKernelGGL(tam_k_mu_small<2>, grid, block, 0, s, table + p.large, co, (uint32_t)steps);
+      hipLaunchKernelGGL(tam_k_mu_small<2>, grid, block, 0, s, p.m[p.large], list, co, (uint32_t)steps);
     else if (side <= 64)
-      hipLaunchKernelGGL(tam_k_mu_small<4>, grid, block, 0, s, table + p.large, co, (uint32_t)steps);
+      hipLaunchKernelGGL(tam_k_mu_small<4>, grid, block, 0, s, p.m[p.large], list, co, (uint32_t)steps);
     else
-      hipLaunchKernelGGL(tam_k_mu_small<8>, grid, block, 0, s, table + p.large, co, (uint32_t)steps);
+      hipLaunchKernelGGL(tam_k_mu_small<8>, grid, block, 0, s, p.m[p.large], list, co, (uint32_t)steps);
     TAM_OP_LAUNCHED("the small matrices");
   }
   if (!p.large) return TAM_OK;
