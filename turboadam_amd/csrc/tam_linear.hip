@@ -298,22 +298,14 @@ __global__ __launch_bounds__(256) void tam_k_slope(tam_slope_args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t col = blockIdx.x * 512 + lane * 8;
   const uint32_t r0 = blockIdx.y * a.run, r1 = a.rows - r0 < a.run ? a.rows : r0 + a.run;
-  const bool whole = col + 8 <= a.cols;
+  const uint32_t count = col < a.cols ? a.cols - col : 0;
   float s[8] = {};
   if (col < a.cols) {
     for (uint32_t r = r0 + wave; r < r1; r += 4) {
       const uint64_t at = (uint64_t)r * a.cols + col;
-      float d[8] = {}, z[8] = {};
-      if (whole) {
-        tam_load8(static_cast<const T*>(a.dy) + at, d);
-        if (a.act != TAM_ACT_NONE) tam_load8(static_cast<const T*>(a.z) + at, z);
-      } else {
-        for (uint32_t j = 0; j < 8; ++j)
-          if (col + j < a.cols) {
-            d[j] = tam_to_f(static_cast<const T*>(a.dy)[at + j]);
-            if (a.act != TAM_ACT_NONE) z[j] = tam_to_f(static_cast<const T*>(a.z)[at + j]);
-          }
-      }
+      float d[8], z[8];
+      tam_load_some(static_cast<const T*>(a.dy) + at, count, d);
+      if (a.act != TAM_ACT_NONE) tam_load_some(static_cast<const T*>(a.z) + at, count, z);
       if (a.act != TAM_ACT_NONE) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[j] *= tam_act_slope(z[j], a.act);
@@ -382,15 +374,7 @@ __global__ __launch_bounds__(256) void tam_k_align(const T* src, uint64_t ld_src
   if (i >= (uint64_t)per * rows) return;
   const uint64_t r = i / per;
   const uint32_t c = (uint32_t)(i - r * per) * 8;
-  const T* s = src + r * ld_src + c;
-  float v[8] = {};
-  if (c + 8 <= cols) {
-    tam_load8(s, v);
-  } else {
-    for (uint32_t j = 0; j < 8; ++j)
-      if (c + j < cols) v[j] = tam_to_f(s[j]);
-  }
-  tam_store8(dst + r * ld_dst + c, v);
+  *reinterpret_cast<tam_oct<T>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -411,7 +395,8 @@ bool aligned(const matrix& m, uint32_t size) {
   return (uint64_t)m.cols * size % 16 == 0 && m.ld * size % 16 == 0 && (uintptr_t)m.p % 16 == 0;
 }
 
-uint32_t aligned_ld(uint32_t cols) { return (uint32_t)tam_up(cols, 8); }
+// Rows of a copy: whole 128-byte lines (a tile's row then touches no line more than it fills).
+uint32_t aligned_ld(uint32_t cols, uint32_t size) { return (uint32_t)tam_up(cols, 128 / size); }
 
 // The workspace is laid out by walking the call twice: once without memory, to
 // learn its size, and once with it.
@@ -544,7 +529,7 @@ int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint6
 int on_16_bytes(call& c, matrix& m) {
   const uint32_t size = kSize[c.dtype];
   if (aligned(m, size) || !m.cols || !m.rows) return TAM_OK;  // of no elements: nothing is read
-  const uint32_t ld = aligned_ld(m.cols);
+  const uint32_t ld = aligned_ld(m.cols, size);
   void* p = c.ws.take(m.rows * ld * size);
   if (!c.dry) {
     const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
@@ -615,7 +600,7 @@ int backward(const TamLinear* d, call& c) {
   if (d->rows && d->outputs && (keep || d->db)) {
     tam_slope_args a = {d->dy, d->z, nullptr, nullptr, 0, (uint32_t)d->rows, (uint32_t)d->outputs, 0, d->activation};
     if (keep) {
-      dz.ld = a.ld_dz = aligned_ld((uint32_t)d->outputs);
+      dz.ld = a.ld_dz = aligned_ld((uint32_t)d->outputs, size);
       dz.p = a.dz = c.ws.take(d->rows * dz.ld * size);
     }
     a.run = slope_run(d->rows, d->outputs);

@@ -59,7 +59,9 @@ struct mat {
   float* partial;     // squares of u
   uint64_t elements;
   int64_t x_low, s_low;  // elements from a high part to its low part (s_low 0: none)
-  uint32_t rows, cols, s, ldx, lds;
+  uint32_t rows, cols, s;
+  uint32_t ldx, lds;  // of x, and of q and p: whole 128-byte lines
+  uint32_t wx, ws;    // cols and s in whole 16 bytes: what a row holds, zeros behind the matrix
   uint32_t tall, split, dtype, flags;
   uint32_t first[PHASES];
   uint32_t partials, chunk;  // partial squares; elements of each
@@ -108,33 +110,13 @@ __global__ __launch_bounds__(256) void tam_k_mu_put(put_args a, mat* to, uint32_
 // ---------------------------------------------------------------------------
 // u
 // ---------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void grad8(const mat& m, uint64_t at, uint32_t count, float (&g)[8]) {
-  const T* p = static_cast<const T*>(m.grad) + at;
-  if (count == 8) {
-    tam_load8(p, g);
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) g[j] = j < count ? tam_to_f(p[j]) : 0.f;
-  }
-}
-
 __device__ __forceinline__ void load_grad(const mat& m, uint64_t at, uint32_t count, float (&g)[8]) {
   if (m.dtype == TAM_DTYPE_F32)
-    grad8<float>(m, at, count, g);
+    tam_load_some(static_cast<const float*>(m.grad) + at, count, g);
   else if (m.dtype == TAM_DTYPE_BF16)
-    grad8<tam_bf16>(m, at, count, g);
+    tam_load_some(static_cast<const tam_bf16*>(m.grad) + at, count, g);
   else
-    grad8<tam_f16>(m, at, count, g);
-}
-
-__device__ __forceinline__ void load_f32(const float* p, uint32_t count, float (&v)[8]) {
-  if (count == 8) {
-    tam_load8(p, v);
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) v[j] = j < count ? p[j] : 0.f;
-  }
+    tam_load_some(static_cast<const tam_f16*>(m.grad) + at, count, g);
 }
 
 // u of elements whose gradient is g and whose (new) momentum is m.
@@ -167,15 +149,10 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
     float g[8], m[8] = {}, u[8];
     load_grad(d, at, count, g);
     if (d.momentum) {
-      load_f32(d.momentum + at, count, m);
+      tam_load_some<float>(d.momentum + at, count, m);
 #pragma unroll
       for (int j = 0; j < 8; ++j) m[j] = __builtin_fmaf(d.one_minus_keep, g[j], d.keep * m[j]);
-      if (count == 8) {
-        tam_store8(d.momentum + at, m);
-      } else {
-        for (uint32_t j = 0; j < 8; ++j)
-          if (j < count) d.momentum[at + j] = m[j];
-      }
+      tam_store_some(d.momentum + at, count, m);
     }
     direction(d, g, m, u);
 #pragma unroll
@@ -241,7 +218,7 @@ __device__ __forceinline__ void store_x(const mat& d, tam_f16* x, uint64_t at, c
 }
 
 // x = u / max(|u|, eps) times 2^12, in parts.  A unit is 2048 elements of x's
-// rows of ldx; the columns past the matrix are zeros.
+// rows of ldx; the columns past the matrix are zeros up to wx.
 constexpr uint32_t kStart = 2048;
 
 __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
@@ -253,11 +230,12 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
   const uint64_t at = (uint64_t)(blockIdx.x - d.first[START]) * kStart + threadIdx.x * 8u;
   if (at >= (uint64_t)d.rows * d.ldx) return;
   const uint32_t row = (uint32_t)(at / d.ldx), col = (uint32_t)(at - (uint64_t)row * d.ldx);
+  if (col >= d.wx) return;
   const uint32_t count = d.cols - col < 8 ? d.cols - col : 8u;
   const uint64_t from = (uint64_t)row * d.cols + col;
   float g[8], m[8] = {}, u[8];
   load_grad(d, from, count, g);
-  if (d.momentum) load_f32(d.momentum + from, count, m);
+  if (d.momentum) tam_load_some<float>(d.momentum + from, count, m);
   direction(d, g, m, u);
 #pragma unroll
   for (int j = 0; j < 8; ++j) u[j] *= scale;
@@ -296,7 +274,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
   triangle(unit - d.first[FIRST ? GRAM : SQUARE], tm, tn);
   const uint32_t r0 = tm * TILE, c0 = tn * TILE;
   // the part of the sum that is this workgroup's (FIRST: blockIdx.y of l.parts)
-  uint64_t k0 = 0, k1 = FIRST ? (d.tall ? d.rows : d.ldx) : d.lds;
+  uint64_t k0 = 0, k1 = FIRST ? (d.tall ? d.rows : d.wx) : d.ws;
   if (FIRST && l.parts > 1) {
     const uint64_t each = (k1 + l.parts * 64u - 1) / (l.parts * 64u) * 64u;
     k0 = blockIdx.y * each < k1 ? blockIdx.y * each : k1;
@@ -308,7 +286,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
   // q where p is made from it
   auto load = [&](uint32_t row, uint32_t col) {
     parts q;
-    if (!FIRST && row < d.s && col < d.lds) {
+    if (!FIRST && row < d.s && col < d.ws) {
       const tam_f16* from = d.q + (uint64_t)row * d.lds + col;
       q.high = *reinterpret_cast<const tam_oct<tam_f16>*>(from);
       if (d.s_low) q.low = *reinterpret_cast<const tam_oct<tam_f16>*>(from + d.s_low);
@@ -316,7 +294,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
     return q;
   };
   auto store = [&](uint32_t row, uint32_t col, float(&v)[8], const parts& q) {
-    if (row >= d.s || col >= d.lds) return;
+    if (row >= d.s || col >= d.ws) return;
     if constexpr (FIRST) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
@@ -374,11 +352,11 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
   tam_soon soon = {};  // q, where p is made from it
   if (!FIRST)
     soon = {reinterpret_cast<const char*>(d.q + (uint64_t)r0 * d.lds + c0), (uint64_t)d.lds * 2u, d.s - r0,
-            (d.lds - c0) * 2u, TILE * 2u};
+            (d.ws - c0) * 2u, TILE * 2u};
   if (FIRST && d.tall) {
     Columns t;
     t.zero();
-    const tam_operand x = operand(d.x[turn], d.ldx, d.ldx);
+    const tam_operand x = operand(d.x[turn], d.ldx, d.wx);
     t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
     finish(t);
   } else {
@@ -413,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_join(list l) {
       tile[row][col + j] = v[j];
     }
     const uint32_t r = tm * 64 + row, c = tn * 64 + col;
-    if (r < d.s && c < d.lds) store_parts(d.q + (uint64_t)r * d.lds + c, d.s_low, v);
+    if (r < d.s && c < d.ws) store_parts(d.q + (uint64_t)r * d.lds + c, d.s_low, v);
   }
   if (tm == tn) return;
   __syncthreads();
@@ -422,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_join(list l) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = tile[col + j][row];
-    if (r < d.s && c < d.lds) store_parts(d.q + (uint64_t)r * d.lds + c, d.s_low, v);
+    if (r < d.s && c < d.ws) store_parts(d.q + (uint64_t)r * d.lds + c, d.s_low, v);
   }
 }
 
@@ -531,8 +509,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
   // x's low bytes; with high and low products the last epilogue's parameter instead
   tam_soon soon = {};
   if (!d.split) {
-    soon = {reinterpret_cast<const char*>(low_bytes(d, x)) + (uint64_t)r0 * d.ldx + c0, d.ldx, d.rows - r0, d.ldx - c0, TILE};
-    if (d.ldx & 3u) soon.base = nullptr;
+    soon = {reinterpret_cast<const char*>(low_bytes(d, x)) + (uint64_t)r0 * d.ldx + c0, d.ldx, d.rows - r0, d.wx - c0, TILE};
   } else if (LAST && (d.flags & TAM_MATRIX_UPDATE)) {
     const uint32_t size = d.dtype == TAM_DTYPE_F32 ? 4u : 2u;
     const uint64_t ld = (uint64_t)d.cols * size;
@@ -542,12 +519,12 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
   if (d.tall) {
     Tall t;
     t.zero();
-    t.template run<true>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.lds, smem, soon, {terms, d.s_low * 2, d.x_low * 2});
+    t.template run<true>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.ws, smem, soon, {terms, d.s_low * 2, d.x_low * 2});
     finish(t);
   } else {
     Wide t;
     t.zero();
-    t.template run<true>(operand(x, d.ldx, d.ldx), p, c0, r0, 0, d.rows, smem, soon, {terms, d.x_low * 2, d.s_low * 2});
+    t.template run<true>(operand(x, d.ldx, d.wx), p, c0, r0, 0, d.rows, smem, soon, {terms, d.x_low * 2, d.s_low * 2});
     finish(t);
   }
 }
@@ -633,12 +610,10 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
     float gr[8], m[8] = {};
     load_grad(d, at, count, gr);
     if (d.momentum) {
-      load_f32(d.momentum + at, count, m);
+      tam_load_some<float>(d.momentum + at, count, m);
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        m[j] = __builtin_fmaf(d.one_minus_keep, gr[j], d.keep * m[j]);
-        if (j < count) d.momentum[at + j] = m[j];
-      }
+      for (int j = 0; j < 8; ++j) m[j] = __builtin_fmaf(d.one_minus_keep, gr[j], d.keep * m[j]);
+      tam_store_some(d.momentum + at, count, m);
     }
     direction(d, gr, m, u[g]);
 #pragma unroll
@@ -875,8 +850,10 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
     m.elements = d.rows * d.cols;
     m.tall = d.rows > d.cols;
     m.s = m.tall ? m.cols : m.rows;
-    m.ldx = (uint32_t)tam_up(d.cols, 8);
-    m.lds = (uint32_t)tam_up(m.s, 8);
+    m.wx = (uint32_t)tam_up(d.cols, 8);
+    m.ws = (uint32_t)tam_up(m.s, 8);
+    m.ldx = (uint32_t)tam_up(d.cols, 64);
+    m.lds = (uint32_t)tam_up(m.s, 64);
     m.dtype = d.dtype;
     m.flags = d.flags;
     m.split = d.dtype != TAM_DTYPE_BF16;

@@ -30,38 +30,18 @@ struct norm_args {
   float eps;
 };
 
-// Elements at .. at + 7 of a row of n as they lie in memory; zeros past its end.
+// Elements at .. at + 7 of a row of n; zeros past its end.
 template <typename T>
 __device__ __forceinline__ tam_oct<T> row_raw(const T* row, uint32_t at, uint32_t n) {
-  tam_oct<T> o;
-  if (at + 8 <= n) {
-    o = *reinterpret_cast<const tam_oct<T>*>(row + at);
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) o.v[j] = (T)0.f;
-    if (at < n)
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j)
-        if (at + j < n) o.v[j] = row[at + j];
-  }
-  return o;
+  return tam_some(row + at, at < n ? n - at : 0);
 }
 template <typename T>
 __device__ __forceinline__ void row_load(const T* row, uint32_t at, uint32_t n, float (&v)[8]) {
-  const tam_oct<T> o = row_raw(row, at, n);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (float)o.v[j];
+  tam_load_some(row + at, at < n ? n - at : 0, v);
 }
-
 template <typename T>
 __device__ __forceinline__ void row_store(T* row, uint32_t at, uint32_t n, const float (&v)[8]) {
-  if (at + 8 <= n) {
-    tam_store8(row + at, v);
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
-      if (at + j < n) row[at + j] = tam_from_f<T>(v[j]);
-  }
+  tam_store_some(row + at, at < n ? n - at : 0, v);
 }
 
 // A workgroup's shape: at least 4 waves, WPR of them to a row.

@@ -82,6 +82,42 @@ __device__ __forceinline__ void tam_store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<tam_oct<T>*>(p) = o;
 }
 
+// The first `count` of 8 elements at p (all of them from 8 on), zeros behind: the
+// loads of a short count do not wait for each other.
+template <typename T>
+__device__ __forceinline__ tam_oct<T> tam_some(const T* p, uint32_t count) {
+  tam_oct<T> o;
+  if (count >= 8) {
+    o = *reinterpret_cast<const tam_oct<T>*>(p);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) o.v[j] = (T)0.f;
+    if (count)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) o.v[j] = p[j < count ? j : 0];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (j >= count) o.v[j] = (T)0.f;
+  }
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ void tam_load_some(const T* p, uint32_t count, float (&x)[8]) {
+  const tam_oct<T> o = tam_some(p, count);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)o.v[i];
+}
+template <typename T>
+__device__ __forceinline__ void tam_store_some(T* p, uint32_t count, const float (&x)[8]) {
+  if (count >= 8) {
+    tam_store8(p, x);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (j < count) p[j] = (T)x[j];
+  }
+}
+
 // Sum over the wave's 64 lanes; every lane gets the same bits.
 template <int CTRL>
 __device__ __forceinline__ float tam_dpp_add(float x) {

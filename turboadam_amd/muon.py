@@ -33,7 +33,7 @@ def _check_products(what: str, coefficients, steps, eps) -> None:
 def _workspace_of(table) -> np.ndarray:
     """About the bytes of workspace of each matrix."""
     small = np.minimum(table["rows"], table["cols"]).astype(np.float64)
-    return 8.0 * table["rows"] * (table["cols"] + 8) + 8.0 * small * (small + 8)
+    return 8.0 * table["rows"] * (table["cols"] + 64) + 8.0 * small * (small + 64)
 
 
 def _launch(table, coefficients, steps: int, device) -> None:
