@@ -30,30 +30,42 @@
 #define TAM_GELU_2U 1.5957691216057308f
 #define TAM_GELU_C 0.044715f
 
-__device__ __forceinline__ float tam_sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// FAST (16-bit results): the hardware's 2^x and reciprocal, 1 ulp each, 4 instructions
+// for about 30: 2^-20 of the result at |x| < 16. At 8192 x 768 x 3072 the epilogue's
+// arithmetic took longer than its stores.
+template <bool FAST>
+__device__ __forceinline__ float tam_sigmoid(float x) {
+  if constexpr (FAST)
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+  else
+    return 1.0f / (1.0f + expf(-x));
+}
 
+template <bool FAST>
 __device__ __forceinline__ float tam_act(float z, uint32_t act) {
   switch (act) {
     case TAM_ACT_RELU: return z < 0.0f ? 0.0f : z;  // a NaN stays
     case TAM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case TAM_ACT_GELU_TANH: return z * tam_sigmoid(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
-    case TAM_ACT_SILU: return z * tam_sigmoid(z);
+    case TAM_ACT_GELU_TANH: return z * tam_sigmoid<FAST>(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
+    case TAM_ACT_SILU: return z * tam_sigmoid<FAST>(z);
     default: return z;
   }
 }
 
+template <bool FAST>
 __device__ __forceinline__ float tam_act_slope(float z, uint32_t act) {
   switch (act) {
     case TAM_ACT_RELU: return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
-    case TAM_ACT_GELU:
-      return __builtin_fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z),
-                            0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+    case TAM_ACT_GELU: {
+      const float e = FAST ? __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z) : expf(-0.5f * z * z);
+      return __builtin_fmaf(z * 0.39894228040143268f, e, 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+    }
     case TAM_ACT_GELU_TANH: {
-      const float s = tam_sigmoid(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
+      const float s = tam_sigmoid<FAST>(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
       return __builtin_fmaf(z * s * (1.0f - s), TAM_GELU_2U * __builtin_fmaf(3.0f * TAM_GELU_C * z, z, 1.0f), s);
     }
     case TAM_ACT_SILU: {
-      const float s = tam_sigmoid(z);
+      const float s = tam_sigmoid<FAST>(z);
       return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
     }
     default: return 1.0f;
@@ -97,7 +109,7 @@ __device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, 
     if (e.z) tam_store8(static_cast<T*>(e.z) + at, v);
     if (e.act != TAM_ACT_NONE) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = tam_act(v[j], e.act);
+      for (int j = 0; j < 8; ++j) v[j] = tam_act<sizeof(T) == 2>(v[j], e.act);
     }
     if (e.residual) {
 #pragma unroll
@@ -111,7 +123,7 @@ __device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, 
       float x = v[j];
       if (e.bias) x += tam_to_f(static_cast<const T*>(e.bias)[col + j]);
       if (e.z) static_cast<T*>(e.z)[at + j] = tam_from_f<T>(x);
-      x = tam_act(x, e.act);
+      x = tam_act<sizeof(T) == 2>(x, e.act);
       if (e.residual) x += tam_to_f(static_cast<const T*>(e.residual)[at + j]);
       static_cast<T*>(e.out)[at + j] = tam_from_f<T>(x);
     }
@@ -308,7 +320,7 @@ __global__ __launch_bounds__(256) void tam_k_slope(tam_slope_args a) {
       if (a.act != TAM_ACT_NONE) tam_load_some(static_cast<const T*>(a.z) + at, count, z);
       if (a.act != TAM_ACT_NONE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] *= tam_act_slope(z[j], a.act);
+        for (int j = 0; j < 8; ++j) d[j] *= tam_act_slope<sizeof(T) == 2>(z[j], a.act);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += d[j];
