@@ -332,8 +332,8 @@ int tam_math_eval(int fn, const float* in, float* out, uint64_t n, void* stream)
 
 /* A linear layer: z = x w^T + bias, y = act(z) + residual, and its gradients.
  * Every array is of `dtype`; arrays without a stride are contiguous.  Arrays
- * may lie at any element's address; rows that are not whole 16 bytes on
- * 16-byte addresses are first copied to the workspace. */
+ * may lie at any element's address; 16-bit rows that do not begin and end on 4
+ * bytes are first copied to the workspace. */
 typedef struct TamLinear {
   const void* x;        /* [rows][inputs], row stride ldx                          */
   const void* w;        /* [outputs][inputs], or [inputs][outputs] with w_in_out;  */

@@ -158,6 +158,26 @@ def test_linear_views_strides_and_leading_dimensions():
                        linear(row.contiguous(), w, residual=b[:70].expand(300, 70).contiguous()))
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("m,k,n", [(66, 130, 70), (300, 1026, 34), (35, 2, 6), (2050, 1030, 1030)])
+def test_linear_rows_on_words_amid_nan(m, k, n, dt):
+    # rows that begin and end on 4 bytes but not on 16, with NaN on every side of them
+    for act, in_out in [(None, False), ("gelu", True)]:
+        x, w, b, r, dy = _linear_case(m, k, n, dt, act, True, False, False)
+
+        def amid(v):
+            wide = torch.full((v.shape[0] + 1, v.shape[1] + 6), float("nan"), device="cuda", dtype=v.dtype)
+            inner = wide[:-1, 2:2 + v.shape[1]]
+            inner.copy_(v)
+            return inner
+
+        log(f"linear amid nan {m}x{k}x{n} {dt} {act} in_out={in_out}")
+        flat = torch.full((w.numel() + 10,), float("nan"), device="cuda", dtype=w.dtype)
+        flat[2:-8] = (w.t() if in_out else w).reshape(-1)
+        w = flat[2:-8].view(k, n).t() if in_out else flat[2:-8].view(n, k)
+        _check_linear(amid(x), w, b, r, dy, dt, act)
+
+
 def test_linear_gradient_of_a_broadcast_input():
     from turboadam_amd import linear
 

@@ -47,13 +47,17 @@ typedef __attribute__((address_space(3))) tam_s4 tam_lds_s4;
 typedef __attribute__((address_space(3))) tam_s8 tam_lds_s8;
 typedef __attribute__((address_space(3))) float tam_lds_float;
 
-// One operand of a product: element (i, k) at base + (i * ld + k) * size
-// (k-contiguous) or base + (k * ld + i) * size (m-major).  The contiguous
-// extent is a multiple of 16 bytes, and base and rows lie on 16 bytes.
+// One operand of a product: element (i, k) at base + i * ld + k * size
+// (k-contiguous) or base + k * ld + i * size (m-major). base and ld are multiples of
+// 4. A product's k is a multiple of 16 bytes of its k-contiguous operands, or their
+// rows are zeros up to one; the rest of a sum is tam_tile::tail's. Loads take 16 bytes
+// from any multiple of 4; in an EXACT tile the words of an m-major operand from `end`
+// on come as zeros (each word for itself).
 struct tam_operand {
   const char* base;
-  uint64_t ld;     // bytes from one row to the next
-  uint32_t count;  // i < count
+  uint64_t ld;      // bytes from one row to the next
+  uint32_t count;   // i < count
+  const char* end;
 };
 
 // Fragment of 16 rows by half a stage: 8 16-bit or 4 fp32 elements a lane.
@@ -99,8 +103,9 @@ __device__ __forceinline__ void tam_word_to_lds(uint32_t lds, uint32_t voff, tam
 }
 
 // Loading and reading one operand's stages.  ROWS: its rows in the tile; NW:
-// the workgroup's waves; KC: contiguous along k.
-template <typename T, int ROWS, int NW, bool KC>
+// the workgroup's waves; KC: contiguous along k; EXACT: nothing is read past the
+// operand's end (see tam_tile).
+template <typename T, int ROWS, int NW, bool KC, bool EXACT>
 struct tam_stage {
   static constexpr int EPC = 16 / (int)sizeof(T);             // elements of a chunk
   static constexpr int BK = TAM_GEMM_ROW / (int)sizeof(T);    // k of a stage
@@ -111,6 +116,7 @@ struct tam_stage {
   static_assert(LOADS >= 1 && BYTES % (1024 * NW) == 0, "whole loads");
 
   const char* base;      // of the next stage to load
+  const char* end;
   uint64_t step;         // bytes from one stage to the next
   uint32_t off[LOADS];   // the lane's offsets; 2^31 where its row or column lies outside
   uint32_t lane_k[LOADS];
@@ -123,6 +129,7 @@ struct tam_stage {
 
   // first: the tile's first row; k0: the first k
   __device__ __forceinline__ void init(const tam_operand& o, uint32_t first, uint64_t k0, int wave, int lane) {
+    if constexpr (EXACT) end = o.end;
     if constexpr (KC) {
       base = o.base + (uint64_t)first * o.ld + k0 * sizeof(T);
       step = TAM_GEMM_ROW;
@@ -154,7 +161,12 @@ struct tam_stage {
   // time for two m-major operands). m0 takes a wait state before it is used.
   __device__ __forceinline__ void load(int i, uint32_t lds, int wave, uint32_t left) const {
     const uint64_t b = (uint64_t)base;
-    const tam_i4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)0x80000000u, 0x00020000};
+    uint32_t records = 0x80000000u;
+    if constexpr (EXACT) {
+      const int64_t rest = end - base;
+      records = rest <= 0 ? 0u : (rest < 0x80000000ll ? (uint32_t)rest : 0x80000000u);
+    }
+    const tam_i4 rsrc = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)records, 0x00020000};
     const uint32_t voff = lane_k[i] < left ? off[i] : 0x80000000u, at = lds + (uint32_t)(wave * LOADS + i) * 1024u;
     tam_to_lds(at, voff, rsrc);
   }
@@ -217,14 +229,16 @@ constexpr int tam_stages() {
 
 // One workgroup's tile: BM rows (operand Q) by BN columns (operand P), WM by
 // WN waves.
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK>
+// EXACT: m-major operands whose rows may end inside 16 bytes: the last row's last
+// load stops at the operand's `end` (a k-contiguous one never passes it).
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool EXACT = false>
 struct tam_tile {
   static constexpr int NW = WM * WN;
   static constexpr int THREADS = 64 * NW;
   static constexpr int TM = BM / WM / 16;  // a wave's fragments of Q
   static constexpr int TN = BN / WN / 16;  // and of P
-  typedef tam_stage<T, BN, NW, PK> SP;
-  typedef tam_stage<T, BM, NW, QK> SQ;
+  typedef tam_stage<T, BN, NW, PK, EXACT && !PK> SP;
+  typedef tam_stage<T, BM, NW, QK, EXACT && !QK> SQ;
   static constexpr int BK = SP::BK;
   static constexpr int STAGE = SP::BYTES + SQ::BYTES;
   static constexpr int LOADS = SP::LOADS + SQ::LOADS;
@@ -348,6 +362,33 @@ struct tam_tile {
       cur = next;
     }
     sync<0>();  // the LDS is the epilogue's
+  }
+
+  // Adds the products of k0 <= k < k1, a few of them, element by element.
+  __device__ __forceinline__ void tail(const tam_operand& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
+                                       uint64_t k1) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+    for (uint64_t k = k0; k < k1; ++k) {
+      float p[TN][4], q[TM];
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const uint32_t at = r0 + (wm * TM + m) * 16 + (lane & 15u), i = at < Q.count ? at : Q.count - 1;
+        q[m] = (float)*reinterpret_cast<const T*>(QK ? Q.base + i * Q.ld + k * sizeof(T) : Q.base + k * Q.ld + i * sizeof(T));
+      }
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          const uint32_t at = c0 + (wn * TN + n) * 16 + (lane >> 4) * 4 + j, i = at < P.count ? at : P.count - 1;
+          p[n][j] = (float)*reinterpret_cast<const T*>(PK ? P.base + i * P.ld + k * sizeof(T) : P.base + k * P.ld + i * sizeof(T));
+        }
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[n][m][j] = __builtin_fmaf(p[n][j], q[m], acc[n][m][j]);
+    }
   }
 
   // Hands the tile to finish(row, col, v, pre): 8 consecutive columns of one row, in

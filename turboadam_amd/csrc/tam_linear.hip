@@ -14,7 +14,7 @@
 //                of 16 weight rows once, straight to the matrix cores;
 //   tam_k_slope  dz and its column sums;  tam_k_column_sum: the sums' end;
 //   tam_k_align  rows copied to 16-byte-aligned rows (zeros behind them), for
-//                operands whose rows are not.
+//                16-bit operands whose rows do not begin and end on 4 bytes.
 #include "tam_gemm.h"
 
 #include <math.h>
@@ -135,15 +135,17 @@ __device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, 
 // ---------------------------------------------------------------------------
 struct tam_gemm_args {
   tam_operand P, Q;   // P: the columns' operand, Q: the rows'
-  uint64_t k, k_part; // the sum's length; of one of the parts it is cut into
+  uint64_t k, k_part; // of the tiles' sums; of one of the parts they are cut into
+  uint64_t k_all;     // of the whole sum: what is left is the first part's
   uint32_t tm, tn;    // tiles
   float* partial;     // [part][rows][cols] fp32, or null: one part
   tam_epilogue e;
 };
 
-template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK>
+// REST: operands whose rows may end inside 16 bytes.
+template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool REST>
 __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam_gemm_args a) {
-  typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, QK> Tile;
+  typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, QK, REST> Tile;
   __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
   uint32_t m, n;
   tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
@@ -159,6 +161,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam
     if (((uintptr_t)soon.base | ld) & 3u) soon.base = nullptr;
   }
   t.run(a.P, a.Q, n * BN, m * BM, k0, k1, smem, soon);
+  if (REST && blockIdx.y == 0) t.tail(a.P, a.Q, n * BN, m * BM, a.k, a.k_all);
   t.template each<TAM_AHEAD_PASS>(
       smem, [&](uint32_t row, uint32_t col) { return tam_residual<T>(a.e, row + m * BM, col + n * BN); },
       [&](uint32_t row, uint32_t col, float(&v)[8], const tam_oct<T>& r) {
@@ -377,16 +380,16 @@ __global__ __launch_bounds__(256) void tam_k_zero(T* out, uint32_t n) {
 // ---------------------------------------------------------------------------
 // alignment
 // ---------------------------------------------------------------------------
-// dst[r][0 .. ld_dst) = src[r][0 .. cols), zeros behind: a thread takes 8 elements.
-template <typename T>
-__global__ __launch_bounds__(256) void tam_k_align(const T* src, uint64_t ld_src, uint64_t rows, uint32_t cols, T* dst,
-                                                   uint32_t ld_dst) {
+// dst[r][0 .. ld_dst) = src[r][0 .. cols) of 16-bit elements, zeros behind: a thread
+// moves 8 elements and none of their bits.
+__global__ __launch_bounds__(256) void tam_k_align(const tam_f16* src, uint64_t ld_src, uint64_t rows, uint32_t cols,
+                                                   tam_f16* dst, uint32_t ld_dst) {
   const uint32_t per = ld_dst / 8;
   const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (uint64_t)per * rows) return;
   const uint64_t r = i / per;
   const uint32_t c = (uint32_t)(i - r * per) * 8;
-  *reinterpret_cast<tam_oct<T>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
+  *reinterpret_cast<tam_oct<tam_f16>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -396,15 +399,22 @@ namespace {
 
 constexpr uint32_t kSize[3] = {4, 2, 2};
 
-// One matrix as the products read it: rows of `cols` contiguous elements.
+// One matrix as the products read it: rows of `cols` contiguous elements; whole: they
+// are 16 bytes, or zeros follow up to that.
 struct matrix {
   const void* p;
   uint64_t ld, rows;
   uint32_t cols;
+  bool whole;
 };
 
-bool aligned(const matrix& m, uint32_t size) {
-  return (uint64_t)m.cols * size % 16 == 0 && m.ld * size % 16 == 0 && (uintptr_t)m.p % 16 == 0;
+// Whether the products' loads can take m as it lies: rows that begin and end on 4 bytes.
+bool in_words(const matrix& m, uint32_t size) {
+  return (uint64_t)m.cols * size % 4 == 0 && m.ld * size % 4 == 0 && (uintptr_t)m.p % 4 == 0;
+}
+
+matrix matrix_of(const void* p, uint64_t ld, uint64_t rows, uint64_t cols, uint32_t size) {
+  return {p, ld, rows, (uint32_t)cols, cols * size % 16 == 0};
 }
 
 // Rows of a copy: whole 128-byte lines (a tile's row then touches no line more than it fills).
@@ -481,48 +491,77 @@ shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
   return best;
 }
 
-template <typename T, int TILE, int WM, int WN>
+// m, or a copy of it whose rows are whole lines. Rows that may end inside 16 bytes
+// have kernels of their own (REST), as the bound on their loads and the rest of their
+// sums would cost the others 1% (x [8192, 768], w [768, 3072], bf16, both ways: 206 -> 208
+// us), and a copy of [2018, 13611] fp32 would be 25 of 110 us. The 256 tile is for
+// products so large that the copy is less than 3% of them.
+int readable(call& c, matrix& m, const shape& s) {
+  const uint32_t size = kSize[c.dtype];
+  if ((in_words(m, size) && (m.whole || s.tile != 256)) || !m.cols || !m.rows) return TAM_OK;  // no elements: nothing is read
+  const uint32_t ld = aligned_ld(m.cols, size);
+  void* p = c.ws.take(m.rows * ld * size);
+  if (!c.dry) {
+    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
+    hipLaunchKernelGGL(tam_k_align, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld, m.rows, m.cols, (tam_f16*)p, ld);
+    TAM_OP_LAUNCHED("the aligned copy");
+  }
+  m = {p, ld, m.rows, m.cols, true};
+  return TAM_OK;
+}
+
+template <typename T, int TILE, int WM, int WN, bool REST>
 void launch_tile(bool pk, bool qk, const tam_gemm_args& a, uint32_t parts, hipStream_t s) {
   const dim3 grid(a.tm * a.tn, parts), block(64 * WM * WN);
   if (pk && qk)
-    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, true, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, true, true, REST>), grid, block, 0, s, a);
   else if (qk)
-    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, false, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, false, true, REST>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, false, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((tam_k_gemm<T, TILE, TILE, WM, WN, false, false, REST>), grid, block, 0, s, a);
 }
 
 template <typename T>
-void launch_gemm(int tile, bool pk, bool qk, const tam_gemm_args& a, uint32_t parts, hipStream_t s) {
+void launch_gemm(int tile, bool pk, bool qk, bool rest, const tam_gemm_args& a, uint32_t parts, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (tile == 256) return launch_tile<T, 256, 2, 4>(pk, qk, a, parts, s);
-  if (tile == 128) return launch_tile<T, 128, 2, 2>(pk, qk, a, parts, s);
-  launch_tile<T, 64, 2, 2>(pk, qk, a, parts, s);
+    if (tile == 256) return launch_tile<T, 256, 2, 4, false>(pk, qk, a, parts, s);
+  if (tile == 128)
+    return rest ? launch_tile<T, 128, 2, 2, true>(pk, qk, a, parts, s) : launch_tile<T, 128, 2, 2, false>(pk, qk, a, parts, s);
+  rest ? launch_tile<T, 64, 2, 2, true>(pk, qk, a, parts, s) : launch_tile<T, 64, 2, 2, false>(pk, qk, a, parts, s);
 }
 
 // out[rows][cols] = sum over k of Q's row and P's row: P and Q as they lie in
 // memory, p_k / q_k: rows of the matrix are the operand's rows (contiguous along k).
-int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint64_t k, const tam_epilogue& e) {
+int product(call& c, matrix P, bool p_k, matrix Q, bool q_k, uint64_t k, const tam_epilogue& e) {
   const shape s = choose(e.rows, e.cols, k, c.dtype);
+  int rc = readable(c, P, s);
+  if (rc == TAM_OK) rc = readable(c, Q, s);
+  if (rc != TAM_OK) return rc;
   float* partial = s.parts > 1 ? (float*)c.ws.take((uint64_t)s.parts * e.rows * e.cols * 4) : nullptr;
   if (c.dry) return TAM_OK;
   const uint32_t size = kSize[c.dtype];
+  auto operand = [&](const matrix& m, uint32_t count) {
+    const char* base = (const char*)m.p;
+    const uint64_t bytes = m.rows ? (m.rows - 1) * m.ld * size + tam_up((uint64_t)m.cols * size, m.whole ? 16 : 1) : 0;
+    return tam_operand{base, m.ld * size, count, base + bytes};
+  };
   tam_gemm_args a = {};
-  a.P = {(const char*)P.p, P.ld * size, e.cols};
-  a.Q = {(const char*)Q.p, Q.ld * size, e.rows};
-  a.k = k;
-  a.k_part = s.parts > 1 ? tam_up(tam_div_up(k, s.parts), 64) : k;
+  a.P = operand(P, e.cols);
+  a.Q = operand(Q, e.rows);
+  a.k_all = k;
+  a.k = (!p_k || P.whole) && (!q_k || Q.whole) ? k : k - k % (16 / size);
+  a.k_part = s.parts > 1 ? tam_up(tam_div_up(a.k, s.parts), 64) : a.k;
   a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
   a.tn = (uint32_t)tam_div_up(e.cols, s.tile);
   a.partial = partial;
   a.e = e;
   if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
   if (c.dtype == TAM_DTYPE_BF16)
-    launch_gemm<tam_bf16>(s.tile, p_k, q_k, a, s.parts, c.stream);
+    launch_gemm<tam_bf16>(s.tile, p_k, q_k, !(P.whole && Q.whole), a, s.parts, c.stream);
   else if (c.dtype == TAM_DTYPE_F16)
-    launch_gemm<tam_f16>(s.tile, p_k, q_k, a, s.parts, c.stream);
+    launch_gemm<tam_f16>(s.tile, p_k, q_k, !(P.whole && Q.whole), a, s.parts, c.stream);
   else
-    launch_gemm<float>(s.tile, p_k, q_k, a, s.parts, c.stream);
+    launch_gemm<float>(s.tile, p_k, q_k, !(P.whole && Q.whole), a, s.parts, c.stream);
   TAM_OP_LAUNCHED("the product");
   if (s.parts > 1) {
     const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
@@ -537,33 +576,10 @@ int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint6
   return TAM_OK;
 }
 
-// m, or a copy of it whose rows are whole 16 bytes on 16-byte addresses.
-int on_16_bytes(call& c, matrix& m) {
-  const uint32_t size = kSize[c.dtype];
-  if (aligned(m, size) || !m.cols || !m.rows) return TAM_OK;  // of no elements: nothing is read
-  const uint32_t ld = aligned_ld(m.cols, size);
-  void* p = c.ws.take(m.rows * ld * size);
-  if (!c.dry) {
-    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
-    if (c.dtype == TAM_DTYPE_F32)
-      hipLaunchKernelGGL(tam_k_align<float>, grid, block, 0, c.stream, (const float*)m.p, m.ld, m.rows, m.cols,
-                         (float*)p, ld);
-    else if (c.dtype == TAM_DTYPE_BF16)
-      hipLaunchKernelGGL(tam_k_align<tam_bf16>, grid, block, 0, c.stream, (const tam_bf16*)m.p, m.ld, m.rows, m.cols,
-                         (tam_bf16*)p, ld);
-    else
-      hipLaunchKernelGGL(tam_k_align<tam_f16>, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld, m.rows, m.cols,
-                         (tam_f16*)p, ld);
-    TAM_OP_LAUNCHED("the aligned copy");
-  }
-  m.p = p;
-  m.ld = ld;
-  return TAM_OK;
-}
-
-matrix x_of(const TamLinear* d) { return {d->x, d->ldx, d->rows, (uint32_t)d->inputs}; }
+matrix x_of(const TamLinear* d) { return matrix_of(d->x, d->ldx, d->rows, d->inputs, kSize[d->dtype]); }
 matrix w_of(const TamLinear* d) {
-  return {d->w, d->ldw, d->w_in_out ? d->inputs : d->outputs, (uint32_t)(d->w_in_out ? d->outputs : d->inputs)};
+  return matrix_of(d->w, d->ldw, d->w_in_out ? d->inputs : d->outputs, d->w_in_out ? d->outputs : d->inputs,
+                   kSize[d->dtype]);
 }
 
 int forward(const TamLinear* d, call& c) {
@@ -588,11 +604,7 @@ int forward(const TamLinear* d, call& c) {
     TAM_OP_LAUNCHED("the product of few rows");
     return TAM_OK;
   }
-  matrix x = x_of(d), w = w_of(d);
-  int rc = on_16_bytes(c, x);
-  if (rc == TAM_OK) rc = on_16_bytes(c, w);
-  if (rc == TAM_OK) rc = product(c, w, !d->w_in_out, x, true, d->inputs, e);
-  return rc;
+  return product(c, w_of(d), !d->w_in_out, x_of(d), true, d->inputs, e);
 }
 
 // Rows of one run of tam_k_slope: about four workgroups to a compute unit, at
@@ -606,14 +618,15 @@ uint32_t slope_run(uint64_t rows, uint64_t cols) {
 int backward(const TamLinear* d, call& c) {
   if (d->outputs == 0 && d->inputs == 0) return TAM_OK;
   const uint32_t size = kSize[c.dtype];
-  matrix dz = {d->dy, d->outputs, d->rows, (uint32_t)d->outputs};
+  matrix dz = matrix_of(d->dy, d->outputs, d->rows, d->outputs, size);
   const bool products = (d->dx || d->dw) && d->inputs;
-  const bool keep = products && (d->activation != TAM_ACT_NONE || !aligned(dz, size));
+  const bool keep = products && (d->activation != TAM_ACT_NONE || !in_words(dz, size) || (size == 2 && !dz.whole));
   if (d->rows && d->outputs && (keep || d->db)) {
     tam_slope_args a = {d->dy, d->z, nullptr, nullptr, 0, (uint32_t)d->rows, (uint32_t)d->outputs, 0, d->activation};
     if (keep) {
       dz.ld = a.ld_dz = aligned_ld((uint32_t)d->outputs, size);
       dz.p = a.dz = c.ws.take(d->rows * dz.ld * size);
+      dz.whole = true;
     }
     a.run = slope_run(d->rows, d->outputs);
     const uint32_t runs = (uint32_t)tam_div_up(d->rows, a.run);
@@ -646,16 +659,12 @@ int backward(const TamLinear* d, call& c) {
   }
   if (!products) return TAM_OK;
   if (d->dx && d->rows) {
-    matrix w = w_of(d);
-    int rc = d->outputs ? on_16_bytes(c, w) : TAM_OK;
     const tam_epilogue e = {d->dx, nullptr, nullptr, nullptr, (uint32_t)d->rows, (uint32_t)d->inputs, TAM_ACT_NONE};
-    if (rc == TAM_OK) rc = product(c, w, d->w_in_out != 0, dz, true, d->outputs, e);
+    const int rc = product(c, w_of(d), d->w_in_out != 0, dz, true, d->outputs, e);
     if (rc != TAM_OK) return rc;
   }
   if (d->dw && d->outputs) {
-    matrix x = x_of(d);
-    const int rc = d->rows ? on_16_bytes(c, x) : TAM_OK;
-    if (rc != TAM_OK) return rc;
+    const matrix x = x_of(d);
     // dw lies as w does: [outputs][inputs], or [inputs][outputs]
     tam_epilogue e = {d->dw, nullptr, nullptr, nullptr, (uint32_t)d->outputs, (uint32_t)d->inputs, TAM_ACT_NONE};
     if (!d->w_in_out) return product(c, x, false, dz, false, d->rows, e);

@@ -246,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
 // products
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ tam_operand operand(const tam_f16* p, uint32_t ld, uint32_t count) {
-  return {reinterpret_cast<const char*>(p), (uint64_t)ld * 2u, count};
+  return {reinterpret_cast<const char*>(p), (uint64_t)ld * 2u, count, nullptr};
 }
 
 struct coefficients {
