@@ -608,11 +608,12 @@ int forward(const TamLinear* d, call& c) {
 }
 
 // Rows of one run of tam_k_slope: about four workgroups to a compute unit, at
-// least 16 rows (4 to a wave).
+// least 8 rows (2 to a wave; 1531 x 777 fp32, gelu: 13.2 us with 16, 9.6 with 8, and
+// the sums' 4 us grow below that).
 uint32_t slope_run(uint64_t rows, uint64_t cols) {
   const uint64_t across = tam_div_up(cols, 512), runs = tam_div_up(4ull * tam_op_cus(), across);
   const uint64_t run = tam_div_up(rows, runs);
-  return (uint32_t)tam_up(run < 16 ? 16 : run, 4);
+  return (uint32_t)tam_up(run < 8 ? 8 : run, 4);
 }
 
 int backward(const TamLinear* d, call& c) {
