@@ -332,8 +332,9 @@ int tam_math_eval(int fn, const float* in, float* out, uint64_t n, void* stream)
 
 /* A linear layer: z = x w^T + bias, y = act(z) + residual, and its gradients.
  * Every array is of `dtype`; arrays without a stride are contiguous.  Arrays
- * may lie at any element's address; 16-bit rows that do not begin and end on 4
- * bytes are first copied to the workspace. */
+ * may lie at any element's address. 16-bit rows that do not begin and end on 4
+ * bytes, or in large products on 16, are first copied to the workspace: ask for its
+ * size with the pointers and strides of the call. */
 typedef struct TamLinear {
   const void* x;        /* [rows][inputs], row stride ldx                          */
   const void* w;        /* [outputs][inputs], or [inputs][outputs] with w_in_out;  */
