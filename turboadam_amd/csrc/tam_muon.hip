@@ -92,6 +92,31 @@ __device__ __forceinline__ uint32_t owner(const list& l, uint32_t b) {
   return __builtin_amdgcn_readfirstlane(found);
 }
 
+// A pointer of a descriptor: to global memory. (The compiler cannot know, and its
+// flat stores count as LDS work too, which the epilogues' turns through LDS wait for.)
+template <typename T>
+__device__ __forceinline__ T* global(T* p) {
+  return (T*)(__attribute__((address_space(1))) T*)(uint64_t)p;
+}
+
+// A descriptor in registers. Read where it lies, every field would be read again
+// after each store (which might have changed it), behind that store: the products'
+// epilogues had 300 such loads, 16 trips to memory one after another (seven matrices of
+// 4096 by 14336: 15.7 ms a step, 14.4 without; one of 128 x 96: 56 us, 49 without).
+__device__ __forceinline__ mat fetch(const mat& from) {
+  mat d = from;
+  d.out = global(d.out);
+  d.grad = global(d.grad);
+  d.momentum = global(d.momentum);
+  d.x[0] = global(d.x[0]);
+  d.x[1] = global(d.x[1]);
+  d.q = global(d.q);
+  d.p = global(d.p);
+  d.diag = global(d.diag);
+  d.partial = global(d.partial);
+  return d;
+}
+
 // ---------------------------------------------------------------------------
 // descriptors
 // ---------------------------------------------------------------------------
@@ -142,7 +167,7 @@ __device__ __forceinline__ float group_sum(float x, float* lds) {
 // 10 bytes an element.
 __global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
   __shared__ float lds[4];
-  const mat& d = l.m[owner<MOMENTUM>(l, blockIdx.x)];
+  const mat d = fetch(l.m[owner<MOMENTUM>(l, blockIdx.x)]);
   const uint32_t unit = blockIdx.x - d.first[MOMENTUM];
   const uint64_t begin = (uint64_t)unit * d.chunk, end = begin + d.chunk < d.elements ? begin + d.chunk : d.elements;
   float sum = 0.f;
@@ -227,7 +252,7 @@ constexpr uint32_t kStart = 2048;
 
 __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
   __shared__ float lds[4];
-  const mat& d = l.m[owner<START>(l, blockIdx.x)];
+  const mat d = fetch(l.m[owner<START>(l, blockIdx.x)]);
   float sum = 0.f;
   for (uint32_t i = threadIdx.x; i < d.partials; i += kThreads) sum += d.partial[i];
   const float norm = sqrtf(group_sum(sum, lds)), scale = kScale / (norm < d.eps ? d.eps : norm);
@@ -276,7 +301,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
   typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), false, false> Columns;
   __shared__ __attribute__((aligned(16))) char smem[Rows::LDS > Columns::LDS ? Rows::LDS : Columns::LDS];
   const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
-  const mat& d = l.m[owner<FIRST ? GRAM : SQUARE>(l, unit)];
+  const mat d = fetch(l.m[owner<FIRST ? GRAM : SQUARE>(l, unit)]);
   uint32_t tm, tn;
   triangle(unit - d.first[FIRST ? GRAM : SQUARE], tm, tn);
   const uint32_t r0 = tm * TILE, c0 = tn * TILE;
@@ -363,13 +388,13 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
   if (FIRST && d.tall) {
     Columns t;
     t.zero();
-    const tam_operand x = operand(d.x[turn], d.ldx, d.wx);
+    const tam_operand x = operand((turn ? d.x[1] : d.x[0]), d.ldx, d.wx);
     t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
     finish(t);
   } else {
     Rows t;
     t.zero();
-    const tam_operand x = FIRST ? operand(d.x[turn], d.ldx, d.rows) : operand(d.q, d.lds, d.s);
+    const tam_operand x = FIRST ? operand((turn ? d.x[1] : d.x[0]), d.ldx, d.rows) : operand(d.q, d.lds, d.s);
     const int64_t low = (FIRST ? d.x_low : d.s_low) * 2;
     t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, low, low});
     finish(t);
@@ -379,7 +404,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
 // q from the parts' sums of its tiles, added in their order.
 __global__ __launch_bounds__(kThreads) void tam_k_mu_join(list l) {
   __shared__ float tile[64][65];
-  const mat& d = l.m[owner<GRAM>(l, blockIdx.x)];
+  const mat d = fetch(l.m[owner<GRAM>(l, blockIdx.x)]);
   uint32_t tm, tn;
   triangle(blockIdx.x - d.first[GRAM], tm, tn);
   const float* from = l.sums + (uint64_t)blockIdx.x * l.parts * (64 * 64);
@@ -455,11 +480,11 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
   typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), true, true> Tall;
   __shared__ __attribute__((aligned(16))) char smem[Wide::LDS > Tall::LDS ? Wide::LDS : Tall::LDS];
   const uint32_t unit = tam_xcd_order(blockIdx.x, gridDim.x);
-  const mat& d = l.m[owner<APPLY>(l, unit)];
+  const mat d = fetch(l.m[owner<APPLY>(l, unit)]);
   uint32_t tm, tn;
   tam_tile_at(unit - d.first[APPLY], (d.rows + TILE - 1) / TILE, (d.cols + TILE - 1) / TILE, tm, tn);
   const uint32_t r0 = tm * TILE, c0 = tn * TILE;
-  const tam_f16* x = d.x[turn];
+  const tam_f16* x = (turn ? d.x[1] : d.x[0]);
   auto finish = [&](auto& t) {
     typedef typename std::remove_reference<decltype(t)>::type Tile;
     float diag[8] = {};  // tall: p's diagonal at the lane's columns, the same in every row
@@ -508,7 +533,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
             else
               write_out<tam_f16>(d, row, col, v, h);
           } else {
-            store_x(d, d.x[turn ^ 1u], (uint64_t)row * d.ldx + col, v);
+            store_x(d, (turn ? d.x[0] : d.x[1]), (uint64_t)row * d.ldx + col, v);
           }
         },
         [](uint32_t, uint32_t, const float*, int) {});
@@ -603,7 +628,7 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
   char *const xh = smem, *const xl = smem + 32768, *const qh = smem + 65536, *const ql = smem + 98304;
   const tam_lds_char *const Xh = (tam_lds_char*)xh, *const Xl = (tam_lds_char*)xl;
   const tam_lds_char *const Qh = (tam_lds_char*)qh, *const Ql = (tam_lds_char*)ql;
-  const mat& d = list ? list[blockIdx.x] : only;
+  const mat d = fetch(list ? list[blockIdx.x] : only);
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t s = d.s, width = d.tall ? d.rows : d.cols;
   // elements past the matrix are zeros in every factor
