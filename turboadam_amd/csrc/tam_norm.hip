@@ -283,24 +283,27 @@ __global__ __launch_bounds__(1024) void tam_k_norm_sums(const float* sums, uint3
 // ---------------------------------------------------------------------------
 // Waves of a row and chunks of a lane. The fewest lanes without work first; one
 // wave where a row fits 16 elements a lane (no barriers), 16 elements a lane
-// beyond as far as the waves go.
+// beyond as far as the waves go, but 8 waves of 32 elements for the backward pass of
+// rows past 8192: 16 waves leave a lane 128 registers, and its six rows of 16 elements
+// spill (4096 x 16384 bf16: 523 us, 132 with 8 waves; forward 48 with 16 waves, 62
+// with 8). Past 16384 there is no room for either, and the spills stay.
 struct pick {
   int wpr, ch;
 };
 constexpr uint32_t kMost = 32768;
 
-pick pick_shape(uint32_t n) {
+pick pick_shape(uint32_t n, bool backward) {
   if (n <= 512) return {1, 1};
   if (n <= 1024) return {1, 2};
   if (n <= 2048) return {4, 1};
   if (n <= 4096) return {4, 2};
   if (n <= 8192) return {4, 4};
-  if (n <= 16384) return {16, 2};
+  if (n <= 16384) return backward ? pick{8, 4} : pick{16, 2};
   return {16, 4};
 }
 
 uint32_t norm_grid(const TamNorm* d, bool backward) {
-  const pick p = pick_shape((uint32_t)d->n);
+  const pick p = pick_shape((uint32_t)d->n, backward);
   const uint64_t rows = p.wpr >= 4 ? 1 : 4, need = tam_div_up(d->rows, rows);
   const uint64_t most = (uint64_t)tam_op_cus() * (p.wpr == 16 ? 2 : (backward ? 2 : 8));
   return (uint32_t)(need < most ? need : most);
@@ -308,22 +311,26 @@ uint32_t norm_grid(const TamNorm* d, bool backward) {
 
 template <typename T>
 void launch_norm(const norm_args& a, pick p, uint32_t grid, bool backward, hipStream_t s) {
-#define TAM_NORM(W, C)                                                                                             \
-  if (p.wpr == W && p.ch == C) {                                                                                   \
-    const dim3 block(norm_shape<W, C>::THREADS);                                                                \
-    if (backward)                                                                                                  \
-      hipLaunchKernelGGL((tam_k_norm_backward<T, W, C>), dim3(grid), block, 0, s, a);                              \
-    else                                                                                                           \
-      hipLaunchKernelGGL((tam_k_norm<T, W, C>), dim3(grid), block, 0, s, a);                                       \
-    return;                                                                                                        \
+#define TAM_NORM(KERNEL, W, C)  \
+  if (p.wpr == W && p.ch == C)  \
+  hipLaunchKernelGGL((KERNEL<T, W, C>), dim3(grid), dim3(norm_shape<W, C>::THREADS), 0, s, a)
+  if (backward) {
+    TAM_NORM(tam_k_norm_backward, 1, 1);
+    TAM_NORM(tam_k_norm_backward, 1, 2);
+    TAM_NORM(tam_k_norm_backward, 4, 1);
+    TAM_NORM(tam_k_norm_backward, 4, 2);
+    TAM_NORM(tam_k_norm_backward, 4, 4);
+    TAM_NORM(tam_k_norm_backward, 8, 4);
+    TAM_NORM(tam_k_norm_backward, 16, 4);
+  } else {
+    TAM_NORM(tam_k_norm, 1, 1);
+    TAM_NORM(tam_k_norm, 1, 2);
+    TAM_NORM(tam_k_norm, 4, 1);
+    TAM_NORM(tam_k_norm, 4, 2);
+    TAM_NORM(tam_k_norm, 4, 4);
+    TAM_NORM(tam_k_norm, 16, 2);
+    TAM_NORM(tam_k_norm, 16, 4);
   }
-  TAM_NORM(1, 1)
-  TAM_NORM(1, 2)
-  TAM_NORM(4, 1)
-  TAM_NORM(4, 2)
-  TAM_NORM(4, 4)
-  TAM_NORM(16, 2)
-  TAM_NORM(16, 4)
 #undef TAM_NORM
 }
 
@@ -363,7 +370,7 @@ int norm(const TamNorm* d, bool backward, void* workspace, size_t ws_bytes, hipS
   const bool sums = backward && (d->dw || d->db);
   const norm_args a = {d->x,  d->w, d->b, d->y, d->stats, d->dy, d->dx, sums ? (float*)workspace : nullptr, d->ldx,
                        (uint32_t)d->rows, (uint32_t)d->n, d->eps};
-  const pick p = pick_shape((uint32_t)d->n);
+  const pick p = pick_shape((uint32_t)d->n, backward);
   if (grid) {
     if (d->dtype == TAM_DTYPE_F32)
       launch_norm<float>(a, p, grid, backward, s);
