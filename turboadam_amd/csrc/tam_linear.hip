@@ -92,17 +92,25 @@ __device__ __forceinline__ tam_oct<T> tam_residual(const tam_epilogue& e, uint32
   return r;
 }
 
-// v holds columns col .. col + 7 of a row of the product, r what tam_residual gave.
+// Eight elements of the bias: a lane's columns are the same in every row of a tile.
+// (Loaded for each row they came behind the row's stores, 16 times a tile.)
+template <typename T>
+__device__ __forceinline__ tam_oct<T> tam_bias(const tam_epilogue& e, uint32_t col) {
+  tam_oct<T> b;
+  if (e.bias && col + 8 <= e.cols) b = *reinterpret_cast<const tam_oct<T>*>(static_cast<const T*>(e.bias) + col);
+  return b;
+}
+
+// v holds columns col .. col + 7 of a row of the product, r what tam_residual gave and
+// b what tam_bias gave.
 template <typename T>
 __device__ __forceinline__ void tam_finish(const tam_epilogue& e, uint32_t row, uint32_t col, float (&v)[8],
-                                           const tam_oct<T>& r) {
+                                           const tam_oct<T>& r, const tam_oct<T>& b) {
   const uint64_t at = (uint64_t)row * e.cols + col;
   if (col + 8 <= e.cols) {
     if (e.bias) {
-      float t[8];
-      tam_load8(static_cast<const T*>(e.bias) + col, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += t[j];
+      for (int j = 0; j < 8; ++j) v[j] += (float)b.v[j];
     }
     // rounded to the type: half of the memory of fp32, and an error of one rounding of z
     // times the activation's second derivative
@@ -169,6 +177,9 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam
   }
   t.run(a.P, a.Q, n * BN, m * BM, k0, k1, smem, soon);
   if (REST && blockIdx.y == 0) t.tail(a.P, a.Q, n * BN, m * BM, a.k, a.k_all);
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  tam_oct<T> bias;
+  if (!a.partial) bias = tam_bias<T>(a.e, n * BN + wave % WN * Tile::COLS + lane % (Tile::COLS / 8) * 8);
   t.template each<TAM_AHEAD_PASS>(
       smem, [&](uint32_t row, uint32_t col) { return tam_residual<T>(a.e, row + m * BM, col + n * BN); },
       [&](uint32_t row, uint32_t col, float(&v)[8], const tam_oct<T>& r) {
@@ -185,7 +196,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam
               if (col + j < a.e.cols) p[j] = v[j];
           }
         } else {
-          tam_finish<T>(a.e, row, col, v, r);
+          tam_finish<T>(a.e, row, col, v, r, bias);
         }
       },
       [](uint32_t, uint32_t, const float*, int) {});
@@ -215,7 +226,7 @@ __global__ __launch_bounds__(256) void tam_k_split(const float* partial, uint32_
       for (int j = 0; j < 8; ++j)
         if (col + j < e.cols) v[j] += partial[p * step + at + j];
   }
-  tam_finish<T>(e, row, col, v, tam_residual<T>(e, row, col));
+  tam_finish<T>(e, row, col, v, tam_residual<T>(e, row, col), tam_bias<T>(e, col));
 }
 
 // ---------------------------------------------------------------------------
@@ -291,13 +302,15 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_few(tam_few_args a) 
   for (int m = 0; m < MT; ++m)  // row m * 16 + i, columns 4 q ..
     *reinterpret_cast<tam_f4*>(&sum[wave][m * 16 + i][q * 4]) = acc[m];
   __syncthreads();
-  const uint32_t t = threadIdx.x, row = t / 2, col = (t % 2) * 8;
+  const uint32_t t = threadIdx.x, row = t / 2;
+  uint32_t col = (t % 2) * 8;
   if (t < MT * 32 && row < a.e.rows && blockIdx.x * 16 + col < a.e.cols) {
     float v[8] = {};
     for (int s = 0; s < TAM_FEW_WAVES; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += sum[s][row][col + j];
-    tam_finish<T>(a.e, row, blockIdx.x * 16 + col, v, tam_residual<T>(a.e, row, blockIdx.x * 16 + col));
+    col += blockIdx.x * 16;
+    tam_finish<T>(a.e, row, col, v, tam_residual<T>(a.e, row, col), tam_bias<T>(a.e, col));
   }
 }
 
