@@ -153,7 +153,7 @@ struct tam_gemm_args {
 // Bound by the matrix cores and, beside them, by LDS (operands in, fragments out).
 // 8192 x 14336 x 4096 bf16, 256 tiles: 742 us with both operands along k (1296
 // TFLOP/s), 734 for dx (one m-major), 810 for dw (both); a library product reaches
-// 1654 TFLOP/s at this size. 8192 x 768 x 3072, 128 tiles: 73 us for y and z (its 100 MB
+// 1654 TFLOP/s at this size. 8192 x 768 x 3072, 128 tiles: 70 us for y and z (its 100 MB
 // of stores are the second bound), 47 for dx and dw each. fp32 1531 x 1001 x 777, 64
 // tiles: 30, 33 and 39 us; 17 are its operations at 143 TFLOP/s, the rest is 312 to 416
 // tiles on 256 compute units and single-word reads of m-major fragments.

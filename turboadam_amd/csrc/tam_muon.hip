@@ -163,8 +163,8 @@ __device__ __forceinline__ float group_sum(float x, float* lds) {
 }
 
 // A unit is `chunk` consecutive elements. Memory bounds it: the seven matrices of a
-// layer of 4096 by 14336, 218M elements, bf16 with fp32 momentum: 541 us, 4.0 TB/s of
-// 10 bytes an element.
+// layer of 4096 by 14336, 218M elements, bf16 with fp32 momentum: 445 us, 4.9 TB/s of
+// 10 bytes an element (a large copy: 5.1).
 __global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
   __shared__ float lds[4];
   const mat d = fetch(l.m[owner<MOMENTUM>(l, blockIdx.x)]);
@@ -246,7 +246,7 @@ __device__ __forceinline__ void store_x(const mat& d, tam_f16* x, uint64_t at, c
 
 // x = u / max(|u|, eps) times 2^12, in parts.  A unit is 2048 elements of x's
 // rows of ldx; the columns past the matrix are zeros up to wx. Memory bounds it (the
-// same list: 335 us, 5.9 TB/s): u is made again from the gradient and the momentum, 6
+// same list: 361 us, 5.4 TB/s): u is made again from the gradient and the momentum, 6
 // bytes an element, for 4 to write and 4 to read of a copy of u.
 constexpr uint32_t kStart = 2048;
 
@@ -291,9 +291,9 @@ __device__ __forceinline__ void triangle(uint32_t t, uint32_t& m, uint32_t& n) {
 }
 
 // FIRST: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q. Bound by the matrix
-// cores: the same list's q 843 us (1030 TFLOP/s of the triangles' operations), p 434
-// (800: 700 tiles are 2.7 rounds of 256 workgroups, and a tile of k = 4096 has an
-// epilogue that stores it twice).
+// cores: the same list's q 826 us (1050 TFLOP/s of the triangles' operations), p 364
+// (950: 700 tiles are 2.7 rounds of 256 workgroups, and a tile's epilogue stores it
+// twice).
 template <int TILE, int WM, int WN, bool FIRST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_square(
     list l, uint32_t turn, coefficients co) {
@@ -471,8 +471,8 @@ __device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t c
 }
 
 // x' = p x (tall: x p); LAST: the output instead. Bound by the matrix cores: the same
-// list 1648 us, 1054 TFLOP/s, LAST 1802 (it reads the parameter and writes it back); the
-// epilogues, which all workgroups of a round reach together, are a sixth of that.
+// list 1515 us, 1146 TFLOP/s, LAST 1534 (it reads the parameter and writes it back); the
+// epilogues, which all workgroups of a round reach together, are a tenth of that.
 template <int TILE, int WM, int WN, bool LAST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_apply(list l,
                                                                                                        uint32_t turn) {
