@@ -222,6 +222,34 @@ def test_linear_infinities_and_nan_stay_in_their_rows(rows):
     assert bool((linear(-x, w, activation="relu")[1] == 0).all())
 
 
+@pytest.mark.parametrize("dt,size", [("f16", 1e4), ("f16", 6e4), ("bf16", 1e4), ("bf16", 2e20), ("f32", 2e20)])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_linear_gradient_where_z_passes_every_range(act, dt, size):
+    """z = -8 size (for fp16 past its numbers, in y a 0; for 2e20 one whose cube is past fp32's) and, where y can hold it,
+    8 size: slopes of 0 and 1, and no row or column beside them is touched."""
+    from turboadam_amd import linear
+
+    log(f"linear {act} {dt} z = 8 x {size}")
+    d = DTYPES[dt]
+    x = torch.full((40, 8), 0.25, device="cuda", dtype=d)
+    x[3], x[5] = size, -size
+    w = torch.full((18, 8), -1.0, device="cuda", dtype=d)
+    w[9:] = 0.125
+    if dt == "f16":  # there y's own infinities are right: only z far below 0
+        x[5], w[9:] = 0.25, -0.5
+    x, w = x.requires_grad_(), w.requires_grad_()
+    b = torch.zeros(18, device="cuda", dtype=d, requires_grad=True)
+    y = linear(x, w, b, activation=act)
+    assert bool(y.isfinite().all())
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    z = (x.detach().double() @ w.detach().double().t()).requires_grad_()
+    slope = torch.autograd.grad(ACT[act](z).sum(), z)[0]
+    assert bool(slope.isfinite().all())
+    for got, want in ((dx, slope @ w.detach().double()), (dw, slope.t() @ x.detach().double()), (db, slope.sum(0))):
+        assert bool(got.isfinite().all())
+        assert float((got.double() - want).norm()) <= (4 * UNIT[dt] + 2.0 ** -17) * float(want.norm())
+
+
 def test_linear_gradient_against_differences():
     """fp32 directional derivatives by central differences in 64 bits of the same function of the outputs."""
     from turboadam_amd import linear

@@ -52,8 +52,12 @@ __device__ __forceinline__ float tam_act(float z, uint32_t act) {
   }
 }
 
+// Past +-128 the smooth activations' slopes are 0 and 1 in fp32, and so they are at
+// the infinities: a z that the layer's type cannot hold (below -65504 in fp16, where y is
+// a finite 0) or whose cube passes fp32's range would give 0 * inf. A NaN stays.
 template <bool FAST>
 __device__ __forceinline__ float tam_act_slope(float z, uint32_t act) {
+  if (act != TAM_ACT_RELU) z = z > 128.0f ? 128.0f : z < -128.0f ? -128.0f : z;
   switch (act) {
     case TAM_ACT_RELU: return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
     case TAM_ACT_GELU: {
