@@ -440,3 +440,40 @@ def test_layers_refuse_what_they_cannot_take():
     ]:
         with pytest.raises(error, match=text):
             layer_norm(*args, **kw)
+
+
+def test_layers_and_orthogonalize_refuse_tangents():
+    """Forward-mode derivatives are not computed: a dual argument raises, and with it a dual gradient."""
+    import torch.autograd.forward_ad as forward
+
+    from turboadam_amd import layer_norm, linear, orthogonalize
+
+    g = _gen("tangents")
+    x, w = torch.randn(40, 24, generator=g, device="cuda"), torch.randn(16, 24, generator=g, device="cuda")
+    b, r, s = w[:, 0].contiguous(), torch.ones(40, 16, device="cuda"), torch.ones(24, device="cuda")
+    plain = [linear(x, w, b, residual=r), layer_norm(x, s, s), orthogonalize(x)]
+    leaf, weight = x.clone().requires_grad_(), w.clone().requires_grad_()
+    graphs = [(linear(leaf, w), leaf), (linear(x, weight), weight), (layer_norm(leaf), leaf)]
+    with forward.dual_level():
+        def dual(v):
+            return forward.make_dual(v, torch.ones_like(v))
+
+        def calls():
+            return (lambda: linear(dual(x), w), lambda: linear(x, dual(w)), lambda: linear(x, w, dual(b)),
+                    lambda: linear(x, w, residual=dual(r)), lambda: linear(dual(x), weight),
+                    lambda: layer_norm(dual(x)), lambda: layer_norm(x, dual(s)), lambda: layer_norm(x, s, dual(s)),
+                    lambda: layer_norm(dual(x), s.clone().requires_grad_()), lambda: orthogonalize(dual(x)))
+
+        for i, call in enumerate(calls()):
+            for enabled in (True, False):
+                log(f"a dual argument, call {i}, gradients {enabled}")
+                with torch.set_grad_enabled(enabled), pytest.raises(RuntimeError, match="dual"):
+                    call()
+        for i, (y, at) in enumerate(graphs):
+            log(f"a dual gradient, call {i}")
+            with pytest.raises(RuntimeError, match="dual"):
+                torch.autograd.grad(y, at, dual(torch.ones_like(y)))
+        # a level without a tangent on any argument changes nothing
+        now = [linear(x, w, b, residual=r), layer_norm(x, s, s), orthogonalize(x)]
+    for a, c in zip(plain, now):
+        assert torch.equal(a, c)

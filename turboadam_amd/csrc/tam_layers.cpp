@@ -102,6 +102,15 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 
 bool wants_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// What the kernels write has no tangent: a dual tensor's would be lost, and everything
+// behind the result would see a zero derivative. (Also under no_grad, where forward
+// mode stays on, and in a backward pass whose gradient is dual.)
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined())
+      refuse(c10::str(what, ": has no forward-mode derivative, and an argument is a dual tensor"));
+}
+
 // The results of these backward passes come from raw memory: they have no graph.
 void not_twice(const char* what) {
   if (at::GradMode::is_enabled())
@@ -197,6 +206,7 @@ struct Linear : torch::autograd::Function<Linear> {
     not_twice("linear");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &z = saved[2], dy = grads[0];
+    refuse_tangents("linear", {&dy});
     const int64_t wants = ctx->saved_data["wants"].toInt();
     Tensor dx, dw, db;
     if (dy.defined() && (wants & 7)) {
@@ -241,10 +251,12 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
       refuse_value(c10::str("linear: residual must have the result's shape (", at::IntArrayRef(sizes), "), got ",
                             shape(*residual)));
   }
+  const Tensor b = given(bias), r = given(residual);
+  refuse_tangents("linear", {&x, &weight, &b, &r});
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() ||
                                      (bias && bias->requires_grad()) || (residual && residual->requires_grad())))
     return Linear::apply(x, weight, bias, residual, activation);
-  return linear_forward(x, weight, given(bias), given(residual), activation, nullptr);
+  return linear_forward(x, weight, b, r, activation, nullptr);
 }
 
 // -------------------------------------------------------------- layer norm
@@ -298,6 +310,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     not_twice("layer_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], dy = grads[0];
+    refuse_tangents("layer_norm", {&dy});
     const int64_t wants = ctx->saved_data["wants"].toInt();
     Tensor dx, dw, db;
     if (dy.defined() && wants) {
@@ -333,11 +346,16 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
       if (t->dim() != 1 || t->size(0) != x.size(-1))
         refuse_value(c10::str("layer_norm: ", name, " must have shape (", x.size(-1), ",), got ", shape(*t)));
     }
+  const Tensor w = given(weight), b = given(bias);
+  refuse_tangents("layer_norm", {&x, &w, &b});
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
     return LayerNorm::apply(x, weight, bias, eps);
-  return norm_forward(x, given(weight), given(bias), eps, nullptr);
+  return norm_forward(x, w, b, eps, nullptr);
 }
+
+// The same checks for an entry whose host work is in Python.
+void check_call(const std::string& what, const Tensor& t) { refuse_tangents(what.c_str(), {&t}); }
 
 template <typename F>
 void take(const py::dict& at, const char* name, F& f) {
@@ -358,5 +376,6 @@ void tam_register_layers(py::module_& m) {
   }, py::arg("addresses"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("residual"),
         py::arg("activation"));
+  m.def("check_call", &check_call, py::arg("what"), py::arg("tensor"));
   m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
 }

@@ -14,6 +14,7 @@ import torch
 from torch.optim import Optimizer
 
 from . import _lib
+from .optimizer import _host
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _MATRIX = np.dtype(_lib.TamMatrix)
@@ -80,6 +81,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
         raise ValueError(f"turboadam_amd.orthogonalize: g must be (..., rows, cols) with sides of at most "
                          f"{_MOST_SIDE}, got {tuple(g.shape)}")
     _check_products("orthogonalize", coefficients, steps, eps)
+    _host().check_call("orthogonalize", g)
     g = g.detach().resolve_neg().contiguous()
     out = torch.empty_like(g)
     rows, cols = g.shape[-2:]
