@@ -477,3 +477,35 @@ def test_layers_and_orthogonalize_refuse_tangents():
         now = [linear(x, w, b, residual=r), layer_norm(x, s, s), orthogonalize(x)]
     for a, c in zip(plain, now):
         assert torch.equal(a, c)
+
+
+def test_layers_and_orthogonalize_refuse_to_be_recorded():
+    """A recorder of torch operations sees only the allocation of what the kernels write: its graph would return
+    uninitialised memory."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from turboadam_amd import layer_norm, linear, orthogonalize
+
+    g = _gen("recorded")
+    x, w = torch.randn(40, 24, generator=g, device="cuda"), torch.randn(16, 24, generator=g, device="cuda")
+    leaf = x.clone().requires_grad_()
+    y, h = linear(leaf, w), layer_norm(leaf)
+
+    def ortho(t):
+        return orthogonalize(t)
+
+    for name, call in (("linear", lambda t: linear(t, w)), ("layer_norm", lambda t: layer_norm(t)),
+                       ("orthogonalize", ortho),
+                       ("linear's gradient", lambda t: torch.autograd.grad(y, leaf, t[:, :16], retain_graph=True)[0]),
+                       ("layer_norm's gradient", lambda t: torch.autograd.grad(h, leaf, t, retain_graph=True)[0])):
+        log(f"make_fx of {name}")
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(call)(x)
+        if "gradient" not in name:
+            log(f"make_fx before dispatch of {name}")
+            with pytest.raises(RuntimeError, match="recorded"):
+                make_fx(call, pre_dispatch=True)(x)
+            log(f"trace of {name}")
+            with pytest.raises(RuntimeError, match="recorded"):
+                torch.jit.trace(call, (x,), check_trace=False)
+            assert torch.equal(call(x), call(x))

@@ -10,6 +10,8 @@
 // that the rest of the package has loaded.
 #include <torch/extension.h>
 
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <string>
@@ -101,6 +103,14 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 bool wants_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A recorder of torch operations (torch.jit.trace, make_fx) would see the allocation of
+// the output and not the kernel that fills it: its graph returns memory as it finds it.
+void refuse_recording(const char* what) {
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(at::DispatchKey::PreDispatch) ||
+      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+    refuse(c10::str(what, ": cannot be recorded by torch.jit.trace or make_fx"));
+}
 
 // What the kernels write has no tangent: a dual tensor's would be lost, and everything
 // behind the result would see a zero derivative. (Also under no_grad, where forward
@@ -204,6 +214,7 @@ struct Linear : torch::autograd::Function<Linear> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     not_twice("linear");
+    refuse_recording("linear");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &z = saved[2], dy = grads[0];
     refuse_tangents("linear", {&dy});
@@ -234,6 +245,7 @@ struct Linear : torch::autograd::Function<Linear> {
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
               int64_t activation) {
   check_first("linear", x);
+  refuse_recording("linear");
   check_other("linear", "weight", weight, x);
   if (weight.dim() != 2 || x.dim() < 1 || x.size(-1) != weight.size(1))
     refuse_value(c10::str("linear: x ", shape(x), " and weight ", shape(weight),
@@ -308,6 +320,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     not_twice("layer_norm");
+    refuse_recording("layer_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], dy = grads[0];
     refuse_tangents("layer_norm", {&dy});
@@ -337,6 +350,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   check_first("layer_norm", x);
+  refuse_recording("layer_norm");
   if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > kMostNorm)
     refuse_value(c10::str("layer_norm: x must have rows of 1 to ", kMostNorm, " elements, got ", shape(x)));
   if (!(eps >= 0)) refuse_value(c10::str("layer_norm: eps must be 0 or more, got ", eps));
@@ -355,7 +369,10 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 }
 
 // The same checks for an entry whose host work is in Python.
-void check_call(const std::string& what, const Tensor& t) { refuse_tangents(what.c_str(), {&t}); }
+void check_call(const std::string& what, const Tensor& t) {
+  refuse_recording(what.c_str());
+  refuse_tangents(what.c_str(), {&t});
+}
 
 template <typename F>
 void take(const py::dict& at, const char* name, F& f) {

@@ -75,13 +75,13 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     if not isinstance(g, torch.Tensor) or not g.is_cuda:
         got = g.device if isinstance(g, torch.Tensor) else type(g).__name__
         raise RuntimeError(f"turboadam_amd.orthogonalize: tensors must be on an MI355X (HIP) device, got {got}")
+    _host().check_call("orthogonalize", g)
     if g.dtype not in _lib.DTYPES:
         raise ValueError(f"turboadam_amd.orthogonalize: g must be float32, bfloat16 or float16, got {g.dtype}")
     if g.dim() < 2 or max(g.shape[-2:]) > _MOST_SIDE:
         raise ValueError(f"turboadam_amd.orthogonalize: g must be (..., rows, cols) with sides of at most "
                          f"{_MOST_SIDE}, got {tuple(g.shape)}")
     _check_products("orthogonalize", coefficients, steps, eps)
-    _host().check_call("orthogonalize", g)
     g = g.detach().resolve_neg().contiguous()
     out = torch.empty_like(g)
     rows, cols = g.shape[-2:]
