@@ -308,6 +308,20 @@ def test_muon_and_orthogonalize_refuse_what_they_cannot_take():
         Muon([q]).step()
 
 
+def test_orthogonalize_refuses_to_drop_a_gradient():
+    from turboadam_amd import orthogonalize
+
+    x = _matrix(_gen("gradient"), 20, 30, "noise")
+    want = orthogonalize(x)
+    leaf = x.clone().requires_grad_()
+    for g in (leaf, leaf * 1.0):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            orthogonalize(g)
+        assert torch.equal(orthogonalize(g.detach()), want)
+        with torch.no_grad():
+            assert torch.equal(orthogonalize(g), want)
+
+
 def test_example_trains_a_block():
     import importlib.util
     import os

@@ -71,10 +71,14 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     of fp16 factors with fp32 sums, an error of about 1e-3 of the result's norm
     beside the result's own rounding; fp32 and fp16: factors of 22 bits.  With
     coefficients under which an iterate's entries pass 16 the result is not
-    finite."""
+    finite.  It has no backward pass: a g that requires gradients is refused
+    where they are on (under no_grad, or detached, it is a constant)."""
     if not isinstance(g, torch.Tensor) or not g.is_cuda:
         got = g.device if isinstance(g, torch.Tensor) else type(g).__name__
         raise RuntimeError(f"turboadam_amd.orthogonalize: tensors must be on an MI355X (HIP) device, got {got}")
+    if g.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("turboadam_amd.orthogonalize: has no backward pass, and g requires gradients: pass "
+                           "g.detach() where it is meant as a constant")
     _host().check_call("orthogonalize", g)
     if g.dtype not in _lib.DTYPES:
         raise ValueError(f"turboadam_amd.orthogonalize: g must be float32, bfloat16 or float16, got {g.dtype}")
