@@ -217,6 +217,27 @@ def test_muon_groups_types_and_odd_addresses_in_one_step():
     assert torch.equal(flat[kept], rest[kept])
 
 
+def test_muon_step_is_seen_by_graphs_that_kept_the_parameter():
+    from turboadam_amd import Muon, linear
+
+    g = _gen("versions")
+    w, other = (torch.nn.Parameter(torch.randn(30, 20, generator=g, device="cuda")) for _ in range(2))
+    x = torch.randn(8, 20, generator=g, device="cuda", requires_grad=True)
+    opt = Muon([w, other])
+    w.grad = torch.randn(30, 20, generator=g, device="cuda")
+    y = linear(x, w)
+    before = [t._version for t in (w, other)]
+    opt.step()
+    assert w._version > before[0] and other._version == before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    m = opt.state[w]["momentum_buffer"]
+    at = m._version
+    opt.step()
+    assert m._version > at
+    linear(x, w).sum().backward()
+
+
 def test_muon_state_dict_keeps_fp32_momentum():
     from turboadam_amd import Muon
 

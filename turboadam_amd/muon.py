@@ -196,11 +196,14 @@ class Muon(Optimizer):
                     continue
                 row, g = self._row(p, group)
                 key = (p.device, tuple(group["ns_coefficients"]), int(group["ns_steps"]))
-                rows, held = calls.setdefault(key, ([], []))
+                rows, held, written = calls.setdefault(key, ([], [], []))
                 rows.append(row)
                 held.append(g)
-        for (device, coefficients, steps), (rows, held) in calls.items():
+                written += (p, self.state[p]["momentum_buffer"])
+        for (device, coefficients, steps), (rows, held, written) in calls.items():
             _launch(np.array(rows, dtype=_MATRIX), coefficients, steps, device)
+            # a graph that kept one of them must not use it as if it were what it was
+            torch.autograd.graph.increment_version(written)
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:
