@@ -205,3 +205,26 @@ def test_add_param_group_mid_run():
     log("add_param_group: steps 6 and 1")
     bad = compare_with_oracle(opt, [x, y], orc, oparams, "after add_param_group")
     assert not bad, "\n".join(bad[:20])
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_step_is_seen_by_graphs_that_kept_the_parameter(capturable):
+    """The first, the full and the steady steps advance the version of each parameter they write, and of no other:
+    a backward pass through the weight as it was raises."""
+    from turboadam_amd import TurboAdam
+
+    torch.manual_seed(0)
+    w, other = (torch.nn.Parameter(torch.randn(96, 64, device="cuda:0")) for _ in range(2))
+    x = torch.randn(8, 64, device="cuda:0", requires_grad=True)
+    opt = TurboAdam([w, other], lr=1e-3, capturable=capturable)
+    for s in range(4):
+        w.grad = torch.randn_like(w)
+        y = torch.nn.functional.linear(x, w)
+        before = w._version, other._version
+        opt.step()
+        log(f"capturable {capturable} step {s}: versions {before} -> {w._version, other._version}")
+        assert w._version > before[0] and other._version == before[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    assert (opt._fast is None) == capturable  # the last steps were steady ones
+    torch.nn.functional.linear(x, w).sum().backward()

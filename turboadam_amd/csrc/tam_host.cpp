@@ -14,9 +14,10 @@
 // steady_rows() returns False, with nothing written, when any check fails
 // (the optimizer then takes its full path, which validates and raises where
 // something is wrong); steady_groups() writes the fields the parameter groups
-// set (numpy column writes took 20 us a step); advance_steps() adds 1 to each
-// state's step counter once the step has been launched.  state_addresses() checks
-// the state arrays of a table that is being built.
+// set (numpy column writes took 20 us a step); advance_steps() advances each
+// parameter's version and each state's step counter once the step has been
+// launched.  state_addresses() checks the state arrays of a table that is being
+// built.
 #include <torch/extension.h>
 
 #include <array>
@@ -558,9 +559,15 @@ bool steady_groups(py::handle f, uint64_t table_addr, int64_t rows, uint64_t gse
   return true;
 }
 
-// state["step"] += 1 for each state dict (once the step has been launched).
-void advance_steps(py::list states) {
+// Once the step has been launched: the rows' parameters' versions, for graphs that
+// kept one of them (the kernels write through addresses, which autograd does not see;
+// an inference tensor has no version), and state["step"] += 1 for each state dict.
+void advance_steps(py::list states, py::list params) {
   const Keys& K = keys();
+  for (py::handle p : params) {
+    at::TensorImpl* t = THPVariable_Unpack(p.ptr()).unsafeGetTensorImpl();
+    if (!t->is_inference()) t->bump_version();
+  }
   for (py::handle st : states) {
     PyObject* s = item(st.ptr(), K.step);
     if (!s) throw py::key_error("step");
@@ -586,7 +593,7 @@ PYBIND11_MODULE(_tam_host, m) {
   m.def("state_addresses", &state_addresses, py::arg("params"), py::arg("tensors"), py::arg("table"));
   m.def("steady_rows", &steady_rows, py::arg("f"), py::arg("table_addr"), py::arg("bias_map"), py::arg("bias_keys"),
         py::arg("bias_out"));
-  m.def("advance_steps", &advance_steps, py::arg("states"));
+  m.def("advance_steps", &advance_steps, py::arg("states"), py::arg("params"));
   m.def("values_kept", &values_kept, py::arg("map"), py::arg("kept"));
   m.def("steady_groups", &steady_groups, py::arg("f"), py::arg("table_addr"), py::arg("rows"), py::arg("gsel_addr"),
         py::arg("flags_addr"), py::arg("bc_addr"));

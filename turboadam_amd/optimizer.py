@@ -254,6 +254,7 @@ class _FastStep:
         self.dev_index = device.index if device.index is not None else torch.cuda.current_device()
         self.params = params      # every parameter of the optimizer, in order
         self.absent = absent      # [p.grad is None] of the step this was built from
+        self.written = [params[i] for i in rows]  # the rows' parameters
         self.states = states      # their state dicts
         self.grads = grads        # the last step's gradient objects, per row (kept alive until the next)
         self.pdtypes = pdtypes    # their parameters' dtypes
@@ -841,6 +842,8 @@ class TurboAdam(Optimizer):
         else:
             self._refresh(plan, device, items)
         self._submit(lib, device, plan, bufs, capturing)
+        # a graph that kept a parameter must not use it as if it were what it was
+        torch.autograd.graph.increment_version([it[0] for it in items])
         for p, state, group, group_idx, tid in items:
             if not group.get("capturable"):
                 state["step"] += 1  # capturable: the step's first launch counts it
@@ -946,7 +949,7 @@ class TurboAdam(Optimizer):
         else:
             with torch.cuda.device(f.device):
                 self._submit_fast(lib, f)
-        host.advance_steps(f.states)
+        host.advance_steps(f.states, f.written)
         return True
 
     def _steady_groups(self, f) -> None:
