@@ -420,8 +420,10 @@ typedef struct TamMatrix {
 int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes);
 /* All n matrices (a host array, read before the call returns) in the same 2 +
  * 3 * steps launches (steps more where q's sums are cut among workgroups), those
- * with sides of up to 128 in one of their own, beside their descriptors' upload. coefficients: a, b, c;
- * steps 1 to 64. */
+ * with sides of up to 128 in one of their own, beside their descriptors' upload. coefficients: a, b, c
+ * below 64; steps 1 to 64.  Results are finite as long as singular values s stay below 4
+ * before the last step, and a + b s^2 + c s^4 below 15 (255 where |a| + |b| + |c| is 15
+ * or more). */
 int tam_orthogonalize(const TamMatrix* matrices, int n, const float* coefficients, int steps, void* workspace,
                       size_t ws_bytes, void* stream);
 

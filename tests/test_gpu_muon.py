@@ -329,6 +329,23 @@ def test_muon_and_orthogonalize_refuse_what_they_cannot_take():
         Muon([q]).step()
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows,cols", [(30, 40), (40, 30), (150, 200), (200, 150)])
+def test_orthogonalize_large_coefficients(rows, cols, dt):
+    """Coefficients whose polynomial passes 16 (fp16's numbers at 2^-12): its sums fit, and a zero matrix stays one."""
+    from turboadam_amd import orthogonalize
+
+    x = _matrix(_gen("large coefficients", rows, cols), rows, cols, "noise").to(DTYPES[dt])
+    assert bool(orthogonalize(torch.ones(1, 1, device="cuda"), steps=1, coefficients=(63.9, 63.9, 63.9)).isfinite())
+    for co in ((16.0, 0.0, 0.0), (20.0, -3.0, 1.0), (63.9, -60.0, 1.0), (0.0, 63.9, 0.0), (0.0, 0.0, 63.9),
+               (-63.9, 63.9, 63.9), (15.0, 0.0, 0.0)):
+        log(f"orthogonalize {rows}x{cols} {dt} {co}")
+        for steps in (1, 5):
+            assert bool((orthogonalize(torch.zeros_like(x), steps=steps, coefficients=co) == 0).all())
+        off = _off(orthogonalize(x, steps=1, coefficients=co), _reference(x, 1, co))
+        assert off <= BOUND[dt], (co, off)
+
+
 def test_orthogonalize_refuses_to_drop_a_gradient():
     from turboadam_amd import orthogonalize
 

@@ -8,7 +8,7 @@
 //
 // Numbers.  The norm makes every singular value of x at most 1, and the step's
 // polynomial keeps them near 1, so x, q and p = a I + b q + c q q are held as
-// fp16 times 2^12: entries up to 16, and 11 bits down to 1.5e-8 of x's scale,
+// fp16 times 2^12 (p times 2^8 where the coefficients are large): entries up to 16, and 11 bits down to 1.5e-8 of x's scale,
 // at the rate of bf16 with an eighth of its error.  What a step's rounding adds
 // in x's small singular directions the next steps amplify like the directions
 // themselves (a per step), so x keeps a low part, and x' = p x_high + diag(p)
@@ -39,7 +39,7 @@
 
 namespace {
 
-constexpr float kScale = 4096.f;        // what fp16 entries are multiplied by
+constexpr float kScale = 4096.f;        // what fp16 entries are multiplied by (p's: see coefficients)
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMostPartials = 512; // of a matrix's squares
 constexpr uint64_t kMostSide = 65536;
@@ -278,8 +278,12 @@ __device__ __forceinline__ tam_operand operand(const tam_f16* p, uint32_t ld, ui
   return {reinterpret_cast<const char*>(p), (uint64_t)ld * 2u, count, nullptr};
 }
 
+// The polynomial's coefficients as p's sums take them, of q q times 2^24, q times 2^12
+// and 1, for p times its scale; back: 1 / scale. p's entries reach |a| + |b| + |c|
+// where x's singular values are at most 1 (a alone where they are small: a zero
+// matrix's p is a I): the scale is 2^12, or 2^8 (entries up to 255) from 15 on.
 struct coefficients {
-  float a, b, c;
+  float qq, q, one, back;
 };
 
 // Tile t of the lower triangle, row by row: rows m, columns n <= m.
@@ -334,14 +338,14 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float x = (float)q.high.v[j] + (d.s_low ? (float)q.low.v[j] : 0.f);
-        v[j] = __builtin_fmaf(co.b, x, co.c / kScale * v[j]);
+        v[j] = __builtin_fmaf(co.q, x, co.qq * v[j]);
       }
       if (row - col < 8) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j)
           if (row - col == j) {
-            v[j] += co.a * kScale;
-            d.diag[row] = v[j] * (1.f / kScale);
+            v[j] += co.one;
+            d.diag[row] = v[j] * co.back;
           }
       }
     }
@@ -470,12 +474,11 @@ __device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t c
   }
 }
 
-// x' = p x (tall: x p); LAST: the output instead. Bound by the matrix cores: the same
+// x' = p x (tall: x p); LAST: the output instead. back: coefficients::back. Bound by the matrix cores: the same
 // list 1515 us, 1146 TFLOP/s, LAST 1534 (it reads the parameter and writes it back); the
 // epilogues, which all workgroups of a round reach together, are a tenth of that.
 template <int TILE, int WM, int WN, bool LAST>
-__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_apply(list l,
-                                                                                                       uint32_t turn) {
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_apply(list l, uint32_t turn, float back) {
   typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), false, true> Wide;
   typedef tam_tile<tam_f16, TILE, TILE, WM, WN, tam_stages<tam_f16, TILE>(), true, true> Tall;
   __shared__ __attribute__((aligned(16))) char smem[Wide::LDS > Tall::LDS ? Wide::LDS : Tall::LDS];
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
           col += c0;
           if (row >= d.rows || col >= d.cols) return;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= 1.f / kScale;
+          for (int j = 0; j < 8; ++j) v[j] *= back;
           if (!d.split) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(d.tall ? diag[j] : h.p, from_byte(h.low, j), v[j]);
@@ -748,8 +751,8 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
         const f16x4 r = *reinterpret_cast<const f16x4*>(ql + small_at(row, col));
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j)
-          v[j] = __builtin_fmaf(co.b, (float)h[j] + (float)r[j], co.c / kScale * v[j]) +
-                 (col + j == row && row < s ? co.a * kScale : 0.f);
+          v[j] = __builtin_fmaf(co.q, (float)h[j] + (float)r[j], co.qq * v[j]) +
+                 (col + j == row && row < s ? co.one : 0.f);
       });
     }
     __syncthreads();  // q is read
@@ -768,7 +771,7 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
     }
     __syncthreads();  // x is read
     if (works && step + 1 < steps)
-      each([&](uint32_t row, uint32_t col, tam_f4& v) { small_store(xh, xl, row, col, v * (1.f / kScale)); });
+      each([&](uint32_t row, uint32_t col, tam_f4& v) { small_store(xh, xl, row, col, v * co.back); });
     __syncthreads();
   }
   if (!works) return;
@@ -777,7 +780,7 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
     for (uint32_t j = 0; j < 4; ++j) {
       const uint32_t r = d.tall ? col + j : row, c = d.tall ? row : col + j;
       if (r >= d.rows || c >= d.cols) continue;
-      const float x = v[j] * (1.f / kScale) * (1.f / kScale);
+      const float x = v[j] * co.back * (1.f / kScale);
       if (d.dtype == TAM_DTYPE_F32)
         small_out<float>(d, r, c, x);
       else if (d.dtype == TAM_DTYPE_BF16)
@@ -945,14 +948,14 @@ void launch_square(int tile, const list& l, uint32_t turn, coefficients co, hipS
 }
 
 template <bool LAST>
-void launch_apply(int tile, const list& l, uint32_t turn, hipStream_t s) {
+void launch_apply(int tile, const list& l, uint32_t turn, float back, hipStream_t s) {
   const dim3 grid(l.units[APPLY]);
   if (tile == 256)
-    hipLaunchKernelGGL((tam_k_mu_apply<256, 2, 4, LAST>), grid, dim3(512), 0, s, l, turn);
+    hipLaunchKernelGGL((tam_k_mu_apply<256, 2, 4, LAST>), grid, dim3(512), 0, s, l, turn, back);
   else if (tile == 128)
-    hipLaunchKernelGGL((tam_k_mu_apply<128, 2, 2, LAST>), grid, dim3(256), 0, s, l, turn);
+    hipLaunchKernelGGL((tam_k_mu_apply<128, 2, 2, LAST>), grid, dim3(256), 0, s, l, turn, back);
   else
-    hipLaunchKernelGGL((tam_k_mu_apply<64, 2, 2, LAST>), grid, dim3(256), 0, s, l, turn);
+    hipLaunchKernelGGL((tam_k_mu_apply<64, 2, 2, LAST>), grid, dim3(256), 0, s, l, turn, back);
 }
 
 int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* workspace, size_t ws_bytes,
@@ -985,7 +988,8 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
     hipLaunchKernelGGL(tam_k_mu_put, dim3(1), dim3(256), 0, s, a, table + i, (uint32_t)k);
     TAM_OP_LAUNCHED("the descriptors");
   }
-  const coefficients co = {c[0], c[1], c[2]};
+  const float scale = fabsf(c[0]) + fabsf(c[1]) + fabsf(c[2]) < 15.f ? kScale : 256.f;
+  const coefficients co = {c[2] * scale / (kScale * kScale), c[1] * scale / kScale, c[0] * scale, 1.f / scale};
   if (p.large < n) {
     const uint32_t side = std::max(p.m[p.large].rows, p.m[p.large].cols);  // the list's largest
     const dim3 grid((uint32_t)(n - p.large)), block(kSmallThreads);
@@ -1016,9 +1020,9 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
     launch_square<false>(p.tile[SQUARE], l, turn, co, s);
     TAM_OP_LAUNCHED("the polynomial");
     if (i + 1 < steps)
-      launch_apply<false>(p.tile[APPLY], l, turn, s);
+      launch_apply<false>(p.tile[APPLY], l, turn, co.back, s);
     else
-      launch_apply<true>(p.tile[APPLY], l, turn, s);
+      launch_apply<true>(p.tile[APPLY], l, turn, co.back, s);
     TAM_OP_LAUNCHED("the polynomial's product");
   }
   return TAM_OK;

@@ -69,9 +69,10 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     x = a x + b (x x^T) x + c (x x^T)^2 x with (a, b, c) = coefficients, on the
     shorter side.  fp32, bf16 or fp16; the result has g's dtype.  bf16: products
     of fp16 factors with fp32 sums, an error of about 1e-3 of the result's norm
-    beside the result's own rounding; fp32 and fp16: factors of 22 bits.  With
-    coefficients under which an iterate's entries pass 16 the result is not
-    finite.  It has no backward pass: a g that requires gradients is refused
+    beside the result's own rounding; fp32 and fp16: factors of 22 bits.  The
+    coefficients are below 64.  The factors are held in a range: the result is
+    not finite where a singular value s passes 4 before the last step, or
+    a + b s^2 + c s^4 passes 15 (255 where |a| + |b| + |c| is 15 or more).  It has no backward pass: a g that requires gradients is refused
     where they are on (under no_grad, or detached, it is a constant)."""
     if not isinstance(g, torch.Tensor) or not g.is_cuda:
         got = g.device if isinstance(g, torch.Tensor) else type(g).__name__
