@@ -346,6 +346,42 @@ def test_orthogonalize_large_coefficients(rows, cols, dt):
         assert off <= BOUND[dt], (co, off)
 
 
+@pytest.mark.parametrize("rows,cols", [(20, 30), (150, 200), (200, 150)])
+def test_orthogonalize_any_norm_and_eps(rows, cols):
+    """|u| and eps anywhere in fp32's range: squares are summed in 64 bits, and no factor of the quotient leaves it."""
+    from turboadam_amd import orthogonalize
+
+    x = torch.randn(rows, cols, generator=_gen("norms", rows, cols), device="cuda")
+    zero = torch.zeros_like(x)
+    for scale, eps in ((1e-22, 1e-30), (1e-30, 1e-38), (1e-36, 1e-44), (1e-20, 1e-7), (1e-30, 1e-28), (1e18, 1e-7),
+                       (1e25, 1e-7), (1e37, 1e-7), (1e36, 1e30), (1e-3, 1e38)):
+        log(f"orthogonalize {rows}x{cols} scale {scale} eps {eps}")
+        y = x * scale
+        want = _reference(y, eps=eps)
+        # denormal numbers of u are right to their last bit, 2^-149
+        bound = BOUND["f32"] * float(want.norm()) + 2.0 ** -149 / max(scale, eps) * 500 * want.norm()
+        # below 2^-24 / 2^12 of 1 the factors' low parts have no bits: such a result is near 0 and no more
+        assert float((orthogonalize(y, eps=eps).double() - want).norm()) <= float(bound) + 1e-6, (scale, eps)
+        assert bool((orthogonalize(zero, eps=eps) == 0).all())
+    for dt in DTYPES.values():
+        assert bool((orthogonalize(zero.to(dt), eps=1e-38) == 0).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 30), (150, 200)])
+def test_muon_of_a_huge_gradient(rows, cols):
+    from turboadam_amd import Muon
+
+    kw = dict(lr=0.02, weight_decay=0.1, momentum=0.9, nesterov=True, adjust_lr="original")
+    g = _gen("huge", rows)
+    p = torch.nn.Parameter(torch.randn(rows, cols, generator=g, device="cuda"))
+    p0, m0 = p.detach().clone(), torch.zeros(rows, cols, device="cuda")
+    p.grad = 1e30 * torch.randn(rows, cols, generator=g, device="cuda")
+    Muon([p], **kw).step()
+    want, _, rate = _muon_reference(p0, p.grad, m0, kw)
+    bound = BOUND["f32"] * rate * 1.2 * math.sqrt(rows) + 2.0 ** -21 * float(want.norm())
+    assert float((p.detach().double() - want).norm()) <= bound
+
+
 def test_orthogonalize_refuses_to_drop_a_gradient():
     from turboadam_amd import orthogonalize
 

@@ -56,7 +56,7 @@ struct mat {
                       // bytes) x_low elements behind
   tam_f16 *q, *p;     // [s][lds]
   float* diag;        // p's diagonal, fp32
-  float* partial;     // squares of u
+  double* partial;    // squares of u
   uint64_t elements;
   int64_t x_low, s_low;  // elements from a high part to its low part (s_low 0: none)
   uint32_t rows, cols, s;
@@ -153,24 +153,79 @@ __device__ __forceinline__ void direction(const mat& d, const float (&g)[8], con
                                            : m[j];
 }
 
+// The squares of u are summed in 64 bits: in 32 they leave the range where an element
+// passes 2^64, or all of them stay below 2^-75 (and eps, if it is as small, does not
+// take over).
+typedef uint32_t halves __attribute__((ext_vector_type(2)));
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double x) {
+  halves h = __builtin_bit_cast(halves, x);
+  h.x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)h.x, CTRL, 0xf, 0xf, true);
+  h.y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)h.y, CTRL, 0xf, 0xf, true);
+  return x + __builtin_bit_cast(double, h);
+}
+__device__ __forceinline__ double wave_sum(double x) {  // as tam_wave_sum
+  x = dpp_add<0xb1>(x);
+  x = dpp_add<0x4e>(x);
+  x = dpp_add<0x141>(x);
+  x = dpp_add<0x140>(x);
+  halves h = __builtin_bit_cast(halves, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(h.x, h.x, false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap(h.y, h.y, false, false);
+  const halves l0 = {a[0], b[0]}, l1 = {a[1], b[1]};
+  x = __builtin_bit_cast(double, l0) + __builtin_bit_cast(double, l1);
+  h = __builtin_bit_cast(halves, x);
+  const auto c = __builtin_amdgcn_permlane32_swap(h.x, h.x, false, false);
+  const auto e = __builtin_amdgcn_permlane32_swap(h.y, h.y, false, false);
+  const halves h0 = {c[0], e[0]}, h1 = {c[1], e[1]};
+  return __builtin_bit_cast(double, h0) + __builtin_bit_cast(double, h1);
+}
+
 // Sum over the workgroup; every thread gets it.
-__device__ __forceinline__ float group_sum(float x, float* lds) {
-  x = tam_wave_sum(x);
+__device__ __forceinline__ double group_sum(double x, double* lds) {
+  x = wave_sum(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
   __syncthreads();
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
+// 8 squares onto a sum, in four chains.
+__device__ __forceinline__ double add_squares(double sum, const float (&u)[8]) {
+  double s[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] = __builtin_fma((double)u[j + 4], (double)u[j + 4], (double)u[j] * (double)u[j]);
+  return sum + ((s[0] + s[1]) + (s[2] + s[3]));
+}
+
+// What brings u to x times 2^12: u 2^shift times `by`. (One factor for both would pass
+// fp32's range, and with it 0 / eps be a NaN.)
+struct normal {
+  float by;
+  int shift;
+  __device__ __forceinline__ float operator()(float u) const { return __builtin_ldexpf(u, shift) * by; }
+};
+
+__device__ __forceinline__ normal normalise(double squares, float eps) {
+  // |u| = n 2^k, n = the root of a number in [1/4, 1) (infinity and NaN stay in n)
+  const int e = __builtin_amdgcn_frexp_exp(squares), k = (e + 1) >> 1;
+  const float n = sqrtf((float)__builtin_ldexp(squares, -2 * k));
+  if (__builtin_ldexp((double)n, k) < (double)eps) {
+    const int ke = __builtin_amdgcn_frexp_exp((double)eps);
+    return {kScale / __builtin_ldexpf(eps, -ke), -ke};
+  }
+  return {kScale / n, -k};
+}
+
 // A unit is `chunk` consecutive elements. Memory bounds it: the seven matrices of a
 // layer of 4096 by 14336, 218M elements, bf16 with fp32 momentum: 445 us, 4.9 TB/s of
 // 10 bytes an element (a large copy: 5.1).
 __global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
-  __shared__ float lds[4];
+  __shared__ double lds[4];
   const mat d = fetch(l.m[owner<MOMENTUM>(l, blockIdx.x)]);
   const uint32_t unit = blockIdx.x - d.first[MOMENTUM];
   const uint64_t begin = (uint64_t)unit * d.chunk, end = begin + d.chunk < d.elements ? begin + d.chunk : d.elements;
-  float sum = 0.f;
+  double sum = 0.;
   for (uint64_t at = begin + threadIdx.x * 8u; at < end; at += kThreads * 8u) {
     const uint32_t count = end - at < 8 ? (uint32_t)(end - at) : 8u;
     float g[8], m[8] = {}, u[8];
@@ -182,8 +237,7 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
       tam_store_some(d.momentum + at, count, m);
     }
     direction(d, g, m, u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(u[j], u[j], sum);
+    sum = add_squares(sum, u);
   }
   sum = group_sum(sum, lds);
   if (threadIdx.x == 0) d.partial[unit] = sum;
@@ -251,11 +305,11 @@ __device__ __forceinline__ void store_x(const mat& d, tam_f16* x, uint64_t at, c
 constexpr uint32_t kStart = 2048;
 
 __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
-  __shared__ float lds[4];
+  __shared__ double lds[4];
   const mat d = fetch(l.m[owner<START>(l, blockIdx.x)]);
-  float sum = 0.f;
+  double sum = 0.;
   for (uint32_t i = threadIdx.x; i < d.partials; i += kThreads) sum += d.partial[i];
-  const float norm = sqrtf(group_sum(sum, lds)), scale = kScale / (norm < d.eps ? d.eps : norm);
+  const normal to_x = normalise(group_sum(sum, lds), d.eps);
   const uint64_t at = (uint64_t)(blockIdx.x - d.first[START]) * kStart + threadIdx.x * 8u;
   if (at >= (uint64_t)d.rows * d.ldx) return;
   const uint32_t row = (uint32_t)(at / d.ldx), col = (uint32_t)(at - (uint64_t)row * d.ldx);
@@ -267,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void tam_k_mu_start(list l) {
   if (d.momentum) tam_load_some<float>(d.momentum + from, count, m);
   direction(d, g, m, u);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] *= scale;
+  for (int j = 0; j < 8; ++j) u[j] = to_x(u[j]);
   store_x(d, d.x[0], at, u);
 }
 
@@ -627,7 +681,7 @@ __device__ __forceinline__ void small_out(const mat& d, uint32_t row, uint32_t c
 template <int BLOCKS>
 __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const mat* list, coefficients co, uint32_t steps) {
   __shared__ __attribute__((aligned(16))) char smem[4 * 32768];
-  __shared__ float lds[8];
+  __shared__ double lds[8];
   char *const xh = smem, *const xl = smem + 32768, *const qh = smem + 65536, *const ql = smem + 98304;
   const tam_lds_char *const Xh = (tam_lds_char*)xh, *const Xl = (tam_lds_char*)xl;
   const tam_lds_char *const Qh = (tam_lds_char*)qh, *const Ql = (tam_lds_char*)ql;
@@ -639,7 +693,7 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
     reinterpret_cast<tam_i4*>(smem)[i] = tam_i4{0, 0, 0, 0};
   constexpr int GROUPS = (BLOCKS * BLOCKS * 32 + (int)kSmallThreads - 1) / (int)kSmallThreads;  // of 8 elements a thread
   float u[GROUPS][8];
-  float sum = 0.f;
+  double sum = 0.;
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
     const uint64_t at = (uint64_t)(g * kSmallThreads + threadIdx.x) * 8u;
@@ -653,16 +707,15 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
       tam_store_some(d.momentum + at, count, m);
     }
     direction(d, gr, m, u[g]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(u[g][j], u[g][j], sum);
+    sum = add_squares(sum, u[g]);
   }
-  sum = tam_wave_sum(sum);
+  sum = wave_sum(sum);
   if (lane == 0) lds[wave] = sum;
   __syncthreads();
-  sum = 0.f;
+  sum = 0.;
 #pragma unroll
   for (int w = 0; w < 8; ++w) sum += lds[w];
-  const float norm = sqrtf(sum), scale = kScale / (norm < d.eps ? d.eps : norm);
+  const normal to_x = normalise(sum, d.eps);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
     const uint32_t at = (g * kSmallThreads + threadIdx.x) * 8u;
@@ -670,7 +723,7 @@ __global__ __launch_bounds__(kSmallThreads) void tam_k_mu_small(mat only, const 
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       if (at + j < d.elements) {
-        float x = u[g][j] * scale;
+        float x = to_x(u[g][j]);
         asm("" : "+v"(x));  // as in store_parts
         const tam_f16 h = (tam_f16)x;
         const uint32_t to = d.tall ? small_at(col, row) : small_at(row, col);
@@ -910,7 +963,7 @@ int make(const TamMatrix* in, int n, char* base, plan& out) {
     m.diag = (float*)take((uint64_t)m.s * 4);
     m.chunk = (uint32_t)tam_up(tam_div_up(m.elements, kMostPartials), kThreads * 8);
     m.partials = (uint32_t)tam_div_up(m.elements, m.chunk);
-    m.partial = (float*)take((uint64_t)m.partials * 4);
+    m.partial = (double*)take((uint64_t)m.partials * 8);
   }
   for (int f = GRAM; f < PHASES; ++f) {
     const shape s = pick(out.m.data(), out.large, f);
