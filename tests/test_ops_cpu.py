@@ -172,3 +172,13 @@ def test_muon_checks_its_settings():
         opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(3))]})
     assert len(opt.param_groups) == 1
     assert opt.defaults["ns_steps"] == 5
+
+
+def test_muon_refuses_an_eps_that_is_zero_to_the_kernels():
+    from turboadam_amd import Muon
+
+    p = torch.nn.Parameter(torch.ones(4, 6))
+    for eps in (1e-50, 0.0, -1e-7, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            Muon([p], eps=eps)
+    Muon([p], eps=1e-44)

@@ -27,8 +27,8 @@ def _check_products(what: str, coefficients, steps, eps) -> None:
         raise ValueError(f"turboadam_amd.{what}: coefficients must be three numbers below 64, got {coefficients!r}")
     if int(steps) != steps or not 1 <= steps <= 64:
         raise ValueError(f"turboadam_amd.{what}: steps must be 1 to 64, got {steps}")
-    if not eps > 0:
-        raise ValueError(f"turboadam_amd.{what}: eps must be above 0, got {eps}")
+    if not ctypes.c_float(float(eps)).value > 0:  # as the kernels take it
+        raise ValueError(f"turboadam_amd.{what}: eps must be above 0 in float32, got {eps}")
 
 
 def _workspace_of(table) -> np.ndarray:
