@@ -182,3 +182,14 @@ def test_muon_refuses_an_eps_that_is_zero_to_the_kernels():
         with pytest.raises(ValueError, match="eps"):
             Muon([p], eps=eps)
     Muon([p], eps=1e-44)
+
+
+def test_counting_library_holds_what_the_binding_loads(monkeypatch):
+    """_lib.load binds every symbol, of the counting build too: it is linked of the library's sources, all of them."""
+    from turboadam_amd import build
+
+    calls = []
+    monkeypatch.setattr(build, "_hipcc", lambda sources, out, verbose, extra=(): calls.append((list(sources), out, extra)))
+    build.build_stats_library()
+    (sources, out, extra), = calls
+    assert sources == build.SOURCES and out == build.STATS_LIB_PATH and "-DTAM_STATS=1" in extra

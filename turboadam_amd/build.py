@@ -18,9 +18,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(BUILD_DIR, "libturboadam_amd.so")
-STEP_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_step.hip")]
-OPERATOR_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_linear.hip", "tam_norm.hip", "tam_muon.hip")]
-SOURCES = STEP_SOURCES + OPERATOR_SOURCES
+SOURCES = [os.path.join(PKG_DIR, "csrc", name)
+           for name in ("tam_step.hip", "tam_linear.hip", "tam_norm.hip", "tam_muon.hip")]
 # streaming kernels that bench.py times as the bandwidth ceiling (not part of the library's ABI)
 STREAM_LIB_PATH = os.path.join(BUILD_DIR, "libtam_stream.so")
 STREAM_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_stream.hip")]
@@ -106,7 +105,7 @@ STATS_LIB_PATH = os.path.join(BUILD_DIR, "libturboadam_amd_stats.so")
 
 
 def build_stats_library(verbose: bool = False) -> str:
-    return _hipcc(STEP_SOURCES, STATS_LIB_PATH, verbose, ["-DTAM_STATS=1"])
+    return _hipcc(SOURCES, STATS_LIB_PATH, verbose, ["-DTAM_STATS=1"])
 
 
 if __name__ == "__main__":
