@@ -193,3 +193,16 @@ def test_counting_library_holds_what_the_binding_loads(monkeypatch):
     build.build_stats_library()
     (sources, out, extra), = calls
     assert sources == build.SOURCES and out == build.STATS_LIB_PATH and "-DTAM_STATS=1" in extra
+
+
+@pytest.mark.parametrize("kw", [{"ns_coefficients": None}, {"lr": "fast"}, {"ns_steps": "many"}, {"eps": None},
+                                {"lr": -1.0}])
+def test_muon_keeps_no_group_that_it_refuses(kw):
+    from turboadam_amd import Muon
+
+    opt = Muon([torch.nn.Parameter(torch.ones(4, 6))])
+    p = torch.nn.Parameter(torch.ones(3, 5))
+    with pytest.raises((TypeError, ValueError)):
+        opt.add_param_group({"params": [p], **kw})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [p]})  # and so the parameter is free

@@ -130,7 +130,7 @@ class Muon(Optimizer):
         group = self.param_groups[-1]
         try:
             self._check_group(group)
-        except ValueError:
+        except Exception:  # also a setting of a wrong type
             self.param_groups.pop()
             raise
 
