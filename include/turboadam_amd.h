@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define TAM_ABI_VERSION 10
+#define TAM_ABI_VERSION 11
 #define TAM_BLOCK_SIZE 128 /* elements per quantisation / CoState block */
 
 /* error codes */
@@ -358,6 +358,11 @@ typedef struct TamLinear {
 
 /* Bytes of workspace (256-byte aligned) of the two calls below. */
 int tam_linear_workspace(const TamLinear* d, int backward_pass, size_t* bytes);
+/* How the products of the two calls below are cut (no GPU work; a self-check, for tests
+ * and measurements): tiles[0] the tile's rows and columns, tiles[1] the parts of its sums,
+ * of y or of dx; [2] and [3] of dw. Zeros where there is no such product (y of up to 32
+ * rows has a kernel without tiles). */
+int tam_linear_tiles(const TamLinear* d, int backward_pass, uint32_t* tiles);
 int tam_linear(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream);
 /* dx, dw and db (those that are not NULL); dresidual is dy. */
 int tam_linear_backward(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream);
@@ -418,6 +423,10 @@ typedef struct TamMatrix {
 /* Bytes of workspace (256-byte aligned) of tam_orthogonalize: about 6 (bf16) or 8
  * per element of the matrices and 4 or 8 per element of their smaller squares. */
 int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes);
+/* How tam_orthogonalize cuts its products (no GPU work; a self-check): tiles[0] and [1]
+ * the tile and parts of q, [2] the tile of p, [3] of x; zeros where all matrices are
+ * small. */
+int tam_orthogonalize_tiles(const TamMatrix* matrices, int n, uint32_t* tiles);
 /* All n matrices (a host array, read before the call returns) in the same 2 +
  * 3 * steps launches (steps more where q's sums are cut among workgroups), those
  * with sides of up to 128 in one of their own, beside their descriptors' upload. coefficients: a, b, c

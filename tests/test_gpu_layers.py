@@ -509,3 +509,94 @@ def test_layers_and_orthogonalize_refuse_to_be_recorded():
             with pytest.raises(RuntimeError, match="recorded"):
                 torch.jit.trace(call, (x,), check_trace=False)
             assert torch.equal(call(x), call(x))
+
+
+# -------------------------------------------------- every tile and every term
+def _tiles(m, k, n, dt, in_out):
+    """The tiles of y, dx and dw, as the library would choose them for this call."""
+    import ctypes
+
+    from turboadam_amd import _lib
+
+    lib, tiles = _lib.load(), []
+    for backward in (0, 1):
+        d = _lib.TamLinear(rows=m, inputs=k, outputs=n, ldx=k, ldw=n if in_out else k, w_in_out=in_out,
+                           dtype=_lib.DTYPES[DTYPES[dt]])
+        for name in ("x", "w", "y", "z", "dy", "dx", "dw"):
+            setattr(d, name, 0x10000)
+        out = (ctypes.c_uint32 * 4)()
+        assert lib.tam_linear_tiles(ctypes.byref(d), backward, out) == 0
+        tiles += [out[0]] if not backward else [out[0], out[2]]
+    return tuple(tiles)
+
+
+# sizes that reach each tile with remainders: rows in whole 16 bytes, rows on words (which the largest tile copies), neither
+LARGE = [("bf16", 8200, 520, 8200, 256, 128, 128), ("f16", 8200, 520, 8200, 256, 128, 128),
+         ("bf16", 8202, 518, 8198, 256, 128, 128), ("f16", 8201, 519, 8199, 256, 128, 128),
+         ("bf16", 3000, 4104, 3000, 128, 256, 256), ("f16", 3002, 4102, 3010, 128, 256, 256),
+         ("bf16", 3001, 4101, 3003, 128, 256, 256), ("bf16", 4099, 2050, 4102, 128, 128, 128),
+         ("f16", 4099, 2050, 4102, 128, 128, 128), ("f32", 6000, 1032, 6000, 128, 128, 128),
+         ("f32", 6003, 1031, 6005, 128, 128, 128)]
+
+
+@pytest.mark.parametrize("in_out", [False, True])
+@pytest.mark.parametrize("dt,m,k,n,y_tile,dx_tile,dw_tile", LARGE)
+def test_linear_in_every_large_tile(dt, m, k, n, y_tile, dx_tile, dw_tile, in_out):
+    log(f"linear {m}x{k}x{n} {dt} in_out={in_out}, tiles of {y_tile}, {dx_tile}, {dw_tile}")
+    assert _tiles(m, k, n, dt, in_out) == (y_tile, dx_tile, dw_tile)
+    _check_linear(*_linear_case(m, k, n, dt, "gelu", True, True, in_out), dt, "gelu")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("m,k,n", [(96, 16384, 160), (40, 8192, 72), (2, 4096, 130), (32, 16383, 48), (17, 5003, 33),
+                                   (1, 16384, 300), (300, 9001, 65), (160, 96, 16384), (130, 70, 9001),
+                                   (16384, 96, 160), (9001, 70, 130), (2050, 1030, 1030), (8202, 518, 8198),
+                                   (3002, 4102, 3010), (6003, 1031, 6005)])
+def test_linear_of_whole_numbers_loses_no_term(m, k, n, dt):
+    """Small whole numbers, whose sums are exact in fp32 in any order and in any parts: the results are the exact ones,
+    rounded.  One term lost or taken twice in a sum of thousands shows."""
+    from turboadam_amd import linear
+
+    for in_out in (False, True):
+        log(f"linear of whole numbers {m}x{k}x{n} {dt} in_out={in_out}")
+        x, w, b, r, dy = _linear_case(m, k, n, dt, None, True, True, in_out, integers=True)
+        x, w, b = x.requires_grad_(), w.detach().requires_grad_(), b.requires_grad_()
+        y = linear(x, w, b, residual=r)
+        got = [y, *torch.autograd.grad(y, (x, w, b), dy)]
+        X, W, D = x.detach().double(), w.detach().double(), dy.double()
+        want = [X @ W.t() + b.detach().double() + r.double(), D @ W, D.t() @ X, D.sum(0)]
+        for name, a, c in zip(("y", "dx", "dw", "db"), got, want):
+            assert torch.equal(a.detach(), c.to(a.dtype)), name
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("n", [768, 1013, 4096, 4097, 8192, 12001, 16384, 20000, 32768])
+def test_layer_norm_sees_every_element(n, dt):
+    """Rows of one element that is not 0, and dy of another one: a lost or repeated chunk of a row changes the mean, the
+    variance or the gradient's sums at once, where long random sums would hide it."""
+    from turboadam_amd import layer_norm
+
+    log(f"layer_norm of single elements {n} {dt}")
+    at = sorted({i for i in (0, 1, 7, 8, 63, 511, 512, 1023, 2047, 2048, 4095, 4096, 8191, 8192, 16383, 16384, n // 2,
+                             n - 9, n - 8, n - 1) if i < n})
+    rows = torch.arange(len(at), device="cuda")
+    cols = torch.tensor(at, device="cuda")
+    x = torch.zeros(len(at), n, device="cuda", dtype=DTYPES[dt])
+    dy = torch.zeros_like(x)
+    x[rows, cols] = 3.0
+    dy[rows, cols.flip(0)] = 2.0
+    w = torch.ones(n, device="cuda", dtype=DTYPES[dt])
+    leaves = [x.requires_grad_(), w.requires_grad_(), torch.zeros_like(w).requires_grad_()]
+    y = layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    X, T = x.detach().double(), dy.double()
+    c = X - X.mean(1, keepdim=True)
+    rstd = (c.square().mean(1, keepdim=True) + 1e-5).rsqrt()
+    h = c * rstd
+    m0, m1 = T.mean(1, keepdim=True), (T * h).mean(1, keepdim=True)
+    u, t, e = UNIT[dt], TINY[dt], 2.0 ** -18  # of the terms: a few roundings of fp32
+    _within(y, h, (u + e) * h.abs() + t, "y")
+    ref = rstd * (T - m0 - h * m1)
+    _within(dx, ref, u * ref.abs() + (1 + u) * e * rstd * (T.abs() + m0.abs() + (h * m1).abs()) + t, "dx")
+    _within(dw, (T * h).sum(0), (u + e) * (T * h).abs().sum(0) + t, "dw")
+    _within(db, T.sum(0), u * T.abs().sum(0) + t, "db")

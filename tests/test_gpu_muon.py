@@ -382,6 +382,68 @@ def test_muon_of_a_huge_gradient(rows, cols):
     assert float((p.detach().double() - want).norm()) <= bound
 
 
+# lists that reach each tile (of q, p and x) with remainders, wide and tall
+TILES = [([(1507, 1601), (1603, 1500), (1500, 1600)], (128, 128, 128)), ([(5001, 4201)], (128, 128, 256)),
+         ([(4201, 5003)], (128, 128, 256)), ([(1281, 1922)] * 5 + [(1923, 1282)] * 5, (256, 256, 256)),
+         ([(1030, 1033)] * 8 + [(1035, 1031)] * 7, (256, 256, 128))]
+
+
+def _tiles(shapes, dt):
+    import ctypes
+
+    from turboadam_amd import _lib
+
+    m, out = (_lib.TamMatrix * len(shapes))(), (ctypes.c_uint32 * 4)()
+    for d, (rows, cols) in zip(m, shapes):
+        d.out = d.grad = 0x10000
+        d.rows, d.cols, d.eps, d.dtype = rows, cols, 1e-7, _lib.DTYPES[DTYPES[dt]]
+    assert _lib.load().tam_orthogonalize_tiles(ctypes.addressof(m), len(shapes), out) == 0
+    return out[0], out[2], out[3]
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("shapes,tiles", TILES)
+def test_muon_in_every_large_tile(shapes, tiles, dt):
+    from turboadam_amd import Muon
+
+    log(f"muon {len(shapes)} matrices like {shapes[0]} {dt}, tiles of {tiles}")
+    assert _tiles(shapes, dt) == tiles
+    kw = dict(lr=0.5, weight_decay=0.1, momentum=0.9, nesterov=True, adjust_lr="original")
+    g = _gen("tiles", len(shapes), dt)
+    params = [torch.nn.Parameter((0.01 * torch.randn(s, generator=g, device="cuda")).to(DTYPES[dt])) for s in shapes]
+    before = [p.detach().clone() for p in params]
+    for p in params:
+        p.grad = _matrix(g, *p.shape, "strong").to(DTYPES[dt])
+    Muon(params, **kw).step()
+    unit = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dt]
+    for i, (p, p0) in enumerate(zip(params, before)):
+        want, _, rate = _muon_reference(p0, p.grad, torch.zeros_like(p0, dtype=torch.float32), kw)
+        bound = BOUND[dt] * rate * 1.2 * math.sqrt(min(p.shape)) + (unit + 2.0 ** -22) * float(want.norm())
+        assert float((p.detach().double() - want).norm()) <= bound, i
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("batch,rows,cols,tiles", [(3, 1507, 1601, (128, 128, 128)), (1, 5001, 4201, (128, 128, 256)),
+                                                   (10, 1281, 1922, (256, 256, 256)), (10, 1922, 1281, (256, 256, 256)),
+                                                   (15, 1030, 1033, (256, 256, 128))])
+def test_orthogonalize_in_every_large_tile(batch, rows, cols, tiles, dt):
+    from turboadam_amd import orthogonalize
+
+    log(f"orthogonalize {batch}x{rows}x{cols} {dt}, tiles of {tiles}")
+    assert _tiles([(rows, cols)] * batch, dt) == tiles
+    g = _gen("tiles", batch, rows, cols)
+    x = torch.stack([_matrix(g, rows, cols, "strong") for _ in range(batch)]).to(DTYPES[dt])
+    out = orthogonalize(x)
+    for i in {0, batch // 2, batch - 1}:
+        want = _reference(x[i])
+        off = _off(out[i], want)
+        assert off <= BOUND[dt], (i, off)
+        # no row or column is left far behind the others (the bound above is over the whole matrix)
+        for dim in (0, 1):
+            far = (out[i].double() - want).norm(dim=dim) / want.norm(dim=dim)
+            assert float(far.max()) <= 8 * BOUND[dt], (i, dim, int(far.argmax()))
+
+
 def test_orthogonalize_refuses_to_drop_a_gradient():
     from turboadam_amd import orthogonalize
 

@@ -206,3 +206,20 @@ def test_muon_keeps_no_group_that_it_refuses(kw):
         opt.add_param_group({"params": [p], **kw})
     assert len(opt.param_groups) == 1
     opt.add_param_group({"params": [p]})  # and so the parameter is free
+
+
+def test_tiles_are_told():
+    lib, out = _lib.load(), (ctypes.c_uint32 * 4)(9, 9, 9, 9)
+    assert lib.tam_linear_tiles(ctypes.byref(_linear(rows=32)), 0, out) == 0 and list(out) == [0, 0, 0, 0]
+    assert lib.tam_linear_tiles(ctypes.byref(_linear(rows=33)), 0, out) == 0 and list(out) == [64, 1, 0, 0]
+    assert lib.tam_linear_tiles(ctypes.byref(_linear()), 1, out) == 0 and out[0] == 64 and out[2] == 64
+    assert lib.tam_linear_tiles(ctypes.byref(_linear(dx=None)), 1, out) == 0 and out[0] == 0 and out[2] == 64
+    assert lib.tam_linear_tiles(ctypes.byref(_linear(dw=None)), 1, out) == 0 and out[0] == 64 and out[2] == 0
+    assert lib.tam_linear_tiles(ctypes.byref(_linear(dtype=3)), 0, out) == 1
+    assert lib.tam_linear_tiles(ctypes.byref(_linear()), 0, None) == 1
+    small, large = _matrices((128, 128), (9, 7)), _matrices((129, 128))
+    assert lib.tam_orthogonalize_tiles(ctypes.addressof(small), 2, out) == 0 and list(out) == [0, 0, 0, 0]
+    assert lib.tam_orthogonalize_tiles(ctypes.addressof(large), 1, out) == 0 and list(out) == [64, 1, 64, 64]
+    assert lib.tam_orthogonalize_tiles(None, 0, out) == 0 and list(out) == [0, 0, 0, 0]
+    assert lib.tam_orthogonalize_tiles(ctypes.addressof(large), -1, out) == 1
+    assert lib.tam_orthogonalize_tiles(ctypes.addressof(large), 1, None) == 1

@@ -28,7 +28,7 @@ TAM_FLAG_EF = 0x10
 TAM_FLAG_HAS_EF = 0x20
 TAM_FLAG_DEVICE_STEP = 0x40
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 # workspace of tam_multi_tensor_step_static (include/turboadam_amd.h)
 TAM_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -242,12 +242,14 @@ SIGNATURES = {
          _VP, _VP, ctypes.c_size_t, _VP],
     ),
     "tam_linear_workspace": (ctypes.c_int, [ctypes.POINTER(TamLinear), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_linear_tiles": (ctypes.c_int, [ctypes.POINTER(TamLinear), ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     "tam_linear": (ctypes.c_int, [ctypes.POINTER(TamLinear), _VP, ctypes.c_size_t, _VP]),
     "tam_linear_backward": (ctypes.c_int, [ctypes.POINTER(TamLinear), _VP, ctypes.c_size_t, _VP]),
     "tam_norm_workspace": (ctypes.c_int, [ctypes.POINTER(TamNorm), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_norm": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP]),
     "tam_norm_backward": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP, ctypes.c_size_t, _VP]),
     "tam_orthogonalize_workspace": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_orthogonalize_tiles": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     "tam_orthogonalize": (
         ctypes.c_int,
         [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_float), ctypes.c_int, _VP, ctypes.c_size_t, _VP],

@@ -464,6 +464,7 @@ struct call {
   hipStream_t stream;
   arena ws;
   bool dry;  // lay out the workspace only
+  uint32_t* tiles;  // where a product's tile and parts are told (tam_linear_tiles), or null
 };
 
 int check_linear(const TamLinear* d, bool backward) {
@@ -561,6 +562,10 @@ void launch_gemm(int tile, bool pk, bool qk, bool rest, const tam_gemm_args& a, 
 // memory, p_k / q_k: rows of the matrix are the operand's rows (contiguous along k).
 int product(call& c, matrix P, bool p_k, matrix Q, bool q_k, uint64_t k, const tam_epilogue& e) {
   const shape s = choose(e.rows, e.cols, k, c.dtype);
+  if (c.tiles) {
+    c.tiles[0] = (uint32_t)s.tile;
+    c.tiles[1] = s.parts;
+  }
   int rc = readable(c, P, s);
   if (rc == TAM_OK) rc = readable(c, Q, s);
   if (rc != TAM_OK) return rc;
@@ -692,6 +697,7 @@ int backward(const TamLinear* d, call& c) {
     if (rc != TAM_OK) return rc;
   }
   if (d->dw && d->outputs) {
+    if (c.tiles) c.tiles += 2;
     const matrix x = x_of(d);
     // dw lies as w does: [outputs][inputs], or [inputs][outputs]
     tam_epilogue e = {d->dw, nullptr, nullptr, nullptr, (uint32_t)d->outputs, (uint32_t)d->inputs, TAM_ACT_NONE};
@@ -703,10 +709,11 @@ int backward(const TamLinear* d, call& c) {
   return TAM_OK;
 }
 
-int linear(const TamLinear* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need) {
+int linear(const TamLinear* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need,
+           uint32_t* tiles = nullptr) {
   int rc = check_linear(d, back);
   if (rc != TAM_OK) return rc;
-  call c = {d->dtype, (hipStream_t)stream, {nullptr, 0}, true};
+  call c = {d->dtype, (hipStream_t)stream, {nullptr, 0}, true, tiles};
   rc = back ? backward(d, c) : forward(d, c);
   if (rc != TAM_OK) return rc;
   if (need) {
@@ -717,7 +724,7 @@ int linear(const TamLinear* d, bool back, void* workspace, uint64_t ws_bytes, vo
     return tam_op_fail(TAM_E_WORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes,
                        (unsigned long long)c.ws.used);
   if ((uintptr_t)workspace & 255u) return tam_op_fail(TAM_E_INVALID, "workspace not on 256 bytes");
-  c = {d->dtype, (hipStream_t)stream, {(char*)workspace, 0}, false};
+  c = {d->dtype, (hipStream_t)stream, {(char*)workspace, 0}, false, nullptr};
   return back ? backward(d, c) : forward(d, c);
 }
 
@@ -734,6 +741,16 @@ int tam_linear_workspace(const TamLinear* d, int backward_pass, size_t* bytes) {
   const int rc = linear(d, backward_pass != 0, nullptr, 0, nullptr, &need);
   *bytes = (size_t)need;
   return rc;
+}
+
+int tam_linear_tiles(const TamLinear* d, int backward_pass, uint32_t* tiles) {
+  if (!tiles) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  for (int i = 0; i < 4; ++i) tiles[i] = 0;
+  uint64_t need = 0;
+  return linear(d, backward_pass != 0, nullptr, 0, nullptr, &need, tiles);
 }
 
 int tam_linear(const TamLinear* d, void* workspace, size_t ws_bytes, void* stream) {

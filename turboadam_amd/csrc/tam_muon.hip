@@ -1012,7 +1012,7 @@ void launch_apply(int tile, const list& l, uint32_t turn, float back, hipStream_
 }
 
 int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* workspace, size_t ws_bytes,
-                  hipStream_t s, size_t* need) {
+                  hipStream_t s, size_t* need, uint32_t* tiles) {
   int rc = check(in, n);
   if (rc != TAM_OK) return rc;
   plan p;
@@ -1021,6 +1021,10 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
   if (rc != TAM_OK) return rc;
   if (need) {
     *need = (size_t)p.bytes;
+    if (tiles && n && p.large) {
+      const uint32_t told[4] = {(uint32_t)p.tile[GRAM], p.parts, (uint32_t)p.tile[SQUARE], (uint32_t)p.tile[APPLY]};
+      std::copy(told, told + 4, tiles);
+    }
     return TAM_OK;
   }
   if (!c) return tam_op_fail(TAM_E_INVALID, "null argument");
@@ -1083,9 +1087,9 @@ int orthogonalize(const TamMatrix* in, int n, const float* c, int steps, void* w
 
 // No exception leaves the library: the plan's memory is all that can fail.
 int guarded(const TamMatrix* in, int n, const float* c, int steps, void* ws, size_t bytes, hipStream_t s,
-            size_t* need) {
+            size_t* need, uint32_t* tiles = nullptr) {
   try {
-    return orthogonalize(in, n, c, steps, ws, bytes, s, need);
+    return orthogonalize(in, n, c, steps, ws, bytes, s, need, tiles);
   } catch (const std::bad_alloc&) {
     return tam_op_fail(TAM_E_INVALID, "no host memory for %d matrices", n);
   }
@@ -1101,6 +1105,16 @@ int tam_orthogonalize_workspace(const TamMatrix* matrices, int n, size_t* bytes)
     return tam_op_fail(TAM_E_INVALID, "null argument");
   }
   return guarded(matrices, n, nullptr, 0, nullptr, 0, nullptr, bytes);
+}
+
+int tam_orthogonalize_tiles(const TamMatrix* matrices, int n, uint32_t* tiles) {
+  if (!tiles) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  std::fill(tiles, tiles + 4, 0u);
+  size_t need = 0;
+  return guarded(matrices, n, nullptr, 0, nullptr, 0, nullptr, &need, tiles);
 }
 
 int tam_orthogonalize(const TamMatrix* matrices, int n, const float* coefficients, int steps, void* workspace,
