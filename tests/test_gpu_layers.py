@@ -600,3 +600,31 @@ def test_layer_norm_sees_every_element(n, dt):
     _within(dx, ref, u * ref.abs() + (1 + u) * e * rstd * (T.abs() + m0.abs() + (h * m1).abs()) + t, "dx")
     _within(dw, (T * h).sum(0), (u + e) * (T * h).abs().sum(0) + t, "dw")
     _within(db, T.sum(0), u * T.abs().sum(0) + t, "db")
+
+
+def test_layers_take_zero_tensors_as_zeros():
+    """autograd's zero tensors have no memory; they are arguments like any other."""
+    from turboadam_amd import layer_norm, linear
+
+    g = _gen("zero tensors")
+    x, w = torch.randn(5, 24, generator=g, device="cuda"), torch.randn(7, 24, generator=g, device="cuda")
+
+    def none(*shape):
+        return torch._efficientzerotensor(shape, device="cuda", dtype=torch.float32)
+
+    def real(*shape):
+        return torch.zeros(shape, device="cuda")
+
+    for name, call in (("layer_norm's weight", lambda z: layer_norm(x, z(24), w[0])),
+                       ("layer_norm's bias", lambda z: layer_norm(x, w[0], z(24))),
+                       ("layer_norm's x", lambda z: layer_norm(z(5, 24), w[0], w[1])),
+                       ("linear's x", lambda z: linear(z(5, 24), w, w[:, 0])),
+                       ("linear's weight", lambda z: linear(x, z(7, 24), w[:, 0])),
+                       ("linear's bias", lambda z: linear(x, w, z(7))),
+                       ("linear's residual", lambda z: linear(x, w, residual=z(5, 7)))):
+        log(name)
+        assert torch.equal(call(none), call(real)), name
+    leaf = x.clone().requires_grad_()
+    for y in (linear(leaf, w), layer_norm(leaf)):
+        dx, = torch.autograd.grad(y, leaf, none(*y.shape))
+        assert bool((dx == 0).all()) and dx.shape == x.shape

@@ -78,17 +78,21 @@ Tensor given(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// t as memory holds it: contiguous, its negative bit resolved.
-Tensor plain(const Tensor& t) {
-  if (!t.defined()) return t;
-  return (t.is_neg() ? t.resolve_neg() : t).contiguous();
+// t as memory holds it: its negative bit resolved, and zeros where it is one of
+// autograd's zero tensors, which have no memory (a null address means "not given" to the
+// kernels, and a missing weight is ones).
+Tensor solid(const Tensor& t) {
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+  return t.is_neg() ? t.resolve_neg() : t;
 }
+
+Tensor plain(const Tensor& t) { return t.defined() ? solid(t).contiguous() : t; }
 
 // t as rows of `width` contiguous elements, and the stride between them.
 Tensor rows_of(const Tensor& t, int64_t width, int64_t& ld) {
   int64_t n = 1;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
-  Tensor r = t.is_neg() ? t.resolve_neg() : t;
+  Tensor r = solid(t);
   if (r.dim() != 2) r = r.reshape({n, width});
   if ((width != 1 && r.stride(1) != 1) || (n > 1 && (r.stride(0) < width || r.stride(0) >= kMostStride)))
     r = r.contiguous();
@@ -131,7 +135,7 @@ void not_twice(const char* what) {
 // The weight, its row stride, and whether its rows are the inputs: a weight stored
 // as (inputs, outputs) and passed as its transpose stays where it is.
 Tensor weight_of(const Tensor& weight, int64_t& ld, bool& in_out) {
-  Tensor w = weight.is_neg() ? weight.resolve_neg() : weight;
+  Tensor w = solid(weight);
   const int64_t outputs = w.size(0), inputs = w.size(1);
   in_out = false;
   if ((inputs == 1 || w.stride(1) == 1) &&
