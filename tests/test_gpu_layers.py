@@ -628,3 +628,20 @@ def test_layers_take_zero_tensors_as_zeros():
     for y in (linear(leaf, w), layer_norm(leaf)):
         dx, = torch.autograd.grad(y, leaf, none(*y.shape))
         assert bool((dx == 0).all()) and dx.shape == x.shape
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_linear_gradient_of_infinite_and_missing_z(dt):
+    """A NaN in a row of x makes that row's gradient NaN, whatever the activation, and an infinity gives the slopes' limits."""
+    from turboadam_amd import linear
+
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        log(f"linear {act} {dt}: NaN and infinities in rows")
+        x = torch.ones(70, 24, device="cuda", dtype=DTYPES[dt])
+        x[1, 5], x[2, 23], x[3, 0] = math.nan, math.inf, -math.inf
+        x = x.requires_grad_()
+        w = torch.ones(40, 24, device="cuda", dtype=DTYPES[dt])
+        dx, = torch.autograd.grad(linear(x, w, activation=act), x, torch.ones(70, 40, device="cuda", dtype=DTYPES[dt]))
+        assert bool(dx[1].isnan().all()), act
+        assert bool((dx[2] == 40).all()) and bool((dx[3] == 0).all()), act
+        assert bool(dx[[0, *range(4, 70)]].isfinite().all()), act

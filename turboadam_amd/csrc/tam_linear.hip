@@ -54,23 +54,24 @@ __device__ __forceinline__ float tam_act(float z, uint32_t act) {
 
 // Past +-128 the smooth activations' slopes are 0 and 1 in fp32, and so they are at
 // the infinities: a z that the layer's type cannot hold (below -65504 in fp16, where y is
-// a finite 0) or whose cube passes fp32's range would give 0 * inf. A NaN stays.
+// a finite 0) or whose cube passes fp32's range would give 0 * inf as a factor, so `near`
+// is the factor. (One instruction, which loses a NaN: that comes from s or e.)
 template <bool FAST>
 __device__ __forceinline__ float tam_act_slope(float z, uint32_t act) {
-  if (act != TAM_ACT_RELU) z = z > 128.0f ? 128.0f : z < -128.0f ? -128.0f : z;
+  const float near = __builtin_amdgcn_fmed3f(z, -128.0f, 128.0f);
   switch (act) {
     case TAM_ACT_RELU: return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
     case TAM_ACT_GELU: {
       const float e = FAST ? __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z) : expf(-0.5f * z * z);
-      return __builtin_fmaf(z * 0.39894228040143268f, e, 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+      return __builtin_fmaf(near * 0.39894228040143268f, e, 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
     }
     case TAM_ACT_GELU_TANH: {
       const float s = tam_sigmoid<FAST>(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
-      return __builtin_fmaf(z * s * (1.0f - s), TAM_GELU_2U * __builtin_fmaf(3.0f * TAM_GELU_C * z, z, 1.0f), s);
+      return __builtin_fmaf(near * s * (1.0f - s), TAM_GELU_2U * __builtin_fmaf(3.0f * TAM_GELU_C * near, near, 1.0f), s);
     }
     case TAM_ACT_SILU: {
       const float s = tam_sigmoid<FAST>(z);
-      return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+      return s * __builtin_fmaf(near, 1.0f - s, 1.0f);
     }
     default: return 1.0f;
   }
