@@ -330,7 +330,9 @@ int tam_math_eval(int fn, const float* in, float* out, uint64_t n, void* stream)
 #define TAM_ACT_GELU_TANH 3 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))        */
 #define TAM_ACT_SILU 4      /* z / (1 + exp(-z))                                      */
 
-/* A linear layer: z = x w^T + bias, y = act(z) + residual, and its gradients.
+/* A linear layer: z = x w^T + bias, y = act(z) + residual, and its gradients. The
+ * backward pass sees z rounded to dtype, and dy act'(z) is rounded to it before the
+ * products that make dx and dw (db is its sum in fp32).
  * Every array is of `dtype`; arrays without a stride are contiguous.  Arrays
  * may lie at any element's address. 16-bit rows that do not begin and end on 4
  * bytes, or in large products on 16, are first copied to the workspace: ask for its

@@ -156,11 +156,11 @@ struct tam_gemm_args {
 };
 
 // Bound by the matrix cores and, beside them, by LDS (operands in, fragments out).
-// 8192 x 14336 x 4096 bf16, 256 tiles: 742 us with both operands along k (1296
-// TFLOP/s), 734 for dx (one m-major), 810 for dw (both); a library product reaches
-// 1654 TFLOP/s at this size. 8192 x 768 x 3072, 128 tiles: 70 us for y and z (its 100 MB
-// of stores are the second bound), 47 for dx and dw each. fp32 1531 x 1001 x 777, 64
-// tiles: 30, 33 and 39 us; 17 are its operations at 143 TFLOP/s, the rest is 312 to 416
+// 8192 x 14336 x 4096 bf16, 256 tiles (means over 300 passes, from card to card 5%
+// either way): 745 us with both operands along k (1290 TFLOP/s), 729 for dx (one
+// m-major), 816 for dw (both); a library product reaches 1654 TFLOP/s at this size.
+// 8192 x 768 x 3072, 128 tiles: 70 us for y and z (its 100 MB of stores are the second
+// bound), 47 for dx and dw each. fp32 1531 x 1001 x 777, 64 tiles: 30, 34 and 39 us; 17 are its operations at 143 TFLOP/s, the rest is 312 to 416
 // tiles on 256 compute units and single-word reads of m-major fragments.
 // REST: operands whose rows may end inside 16 bytes.
 template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool REST>
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam
 }
 
 // The parts' sums in their order, then the epilogue: a thread takes 8 columns. Two
-// parts of 1531 x 777 fp32, gelu and residual: 8.3 us, and the products they join 30 (43
+// parts of 1531 x 777 fp32, gelu and residual: 8.9 us, and the products they join 30 (43
 // uncut).
 template <typename T>
 __global__ __launch_bounds__(256) void tam_k_split(const float* partial, uint32_t parts, tam_epilogue e) {
@@ -324,8 +324,10 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_few(tam_few_args a) 
 // ---------------------------------------------------------------------------
 // A workgroup takes 512 columns (8 to a lane) of a run of rows, its waves every
 // fourth row; dz leaves rounded to the type, and the columns' sums of dz in fp32,
-// one row of `sums` to a run. dz == null: the sums alone (of dy). Memory bounds it:
-// 8192 x 3072 bf16, gelu_tanh: 33 us, 4.6 TB/s.
+// one row of `sums` to a run. dz == null: the sums alone (of dy). The rounding is
+// what dx's and dw's matrix instructions take: in bf16 it brings their errors from
+// 1.7e-3 of the result (its own rounding) to 2.4e-3; two parts of dz would double both
+// products. Memory bounds it: 8192 x 3072 bf16, gelu_tanh: 33 us, 4.5 TB/s.
 struct tam_slope_args {
   const void* dy;
   const void* z;

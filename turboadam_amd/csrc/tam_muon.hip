@@ -218,7 +218,7 @@ __device__ __forceinline__ normal normalise(double squares, float eps) {
 }
 
 // A unit is `chunk` consecutive elements. Memory bounds it: the seven matrices of a
-// layer of 4096 by 14336, 218M elements, bf16 with fp32 momentum: 445 us, 4.9 TB/s of
+// layer of 4096 by 14336, 218M elements, bf16 with fp32 momentum: 448 us, 4.9 TB/s of
 // 10 bytes an element (a large copy: 5.1).
 __global__ __launch_bounds__(kThreads) void tam_k_mu_momentum(list l) {
   __shared__ double lds[4];
@@ -300,7 +300,7 @@ __device__ __forceinline__ void store_x(const mat& d, tam_f16* x, uint64_t at, c
 
 // x = u / max(|u|, eps) times 2^12, in parts.  A unit is 2048 elements of x's
 // rows of ldx; the columns past the matrix are zeros up to wx. Memory bounds it (the
-// same list: 361 us, 5.4 TB/s): u is made again from the gradient and the momentum, 6
+// same list: 366 us, 5.4 TB/s): u is made again from the gradient and the momentum, 6
 // bytes an element, for 4 to write and 4 to read of a copy of u.
 constexpr uint32_t kStart = 2048;
 
@@ -349,8 +349,8 @@ __device__ __forceinline__ void triangle(uint32_t t, uint32_t& m, uint32_t& n) {
 }
 
 // FIRST: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q. Bound by the matrix
-// cores: the same list's q 826 us (1050 TFLOP/s of the triangles' operations), p 364
-// (950: 700 tiles are 2.7 rounds of 256 workgroups, and a tile's epilogue stores it
+// cores: the same list's q 847 us (1020 TFLOP/s of the triangles' operations), p 378
+// (915: 700 tiles are 2.7 rounds of 256 workgroups, and a tile's epilogue stores it
 // twice).
 template <int TILE, int WM, int WN, bool FIRST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_square(
@@ -529,7 +529,7 @@ __device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t c
 }
 
 // x' = p x (tall: x p); LAST: the output instead. back: coefficients::back. Bound by the matrix cores: the same
-// list 1515 us, 1146 TFLOP/s, LAST 1534 (it reads the parameter and writes it back); the
+// list 1540 us, 1127 TFLOP/s, LAST 1555 (it reads the parameter and writes it back); the
 // epilogues, which all workgroups of a round reach together, are a tenth of that.
 template <int TILE, int WM, int WN, bool LAST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_apply(list l, uint32_t turn, float back) {
@@ -628,8 +628,9 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
 // three products of a step run on the 8 waves, 32 rows by half of the columns of the
 // result to each, with barriers between them. One launch for any number of such matrices: 128 x 96 in
 // fp32 took 110 us in 18 launches of 4 to 8 us each, most of that the way to memory
-// and back between them; here it takes 17 us and 7 us a step, of which the matrix
-// instructions of one compute unit are 4.
+// and back between them; here it takes 49, about 7 a step. Of the 16 x 16
+// blocks that a step multiplies at 128 x 96, two fifths are not needed (columns 96 to 127
+// of q and p, and one triangle of each), and two of the eight waves have no rows.
 constexpr uint32_t kSmall = 128;
 constexpr uint32_t kSmallThreads = 512;
 

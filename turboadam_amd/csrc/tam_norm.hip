@@ -78,7 +78,7 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* lds, uint32_t& tur
 }
 
 // Reads x and writes y, nothing else. 16384 x 4096 bf16: 50 us, 5.4 TB/s (a large copy:
-// 5.1); 8192 x 768 fp32: 11 us, 4.5 TB/s; one row of 4096: 2.9 us, the way to memory
+// 5.1); 8192 x 768 fp32: 11 us, 4.5 TB/s; one row of 4096: 3.0 us, the way to memory
 // and back and two sums over the waves.
 template <typename T, int WPR, int CH>
 __global__ __launch_bounds__((norm_shape<WPR, CH>::THREADS)) void tam_k_norm(norm_args a) {
@@ -144,7 +144,7 @@ __global__ __launch_bounds__((norm_shape<WPR, CH>::THREADS)) void tam_k_norm(nor
 // Reads x and dy and writes dx. Two workgroups to a compute unit: their rows of `sums`
 // are few (the weight's and bias's gradients stay in registers over all of a
 // workgroup's rows), and the row fetched ahead hides what more of them would.
-// 16384 x 4096 bf16: 79 us, 5.1 TB/s; 8192 x 768 fp32: 17 us, 4.4 TB/s.
+// 16384 x 4096 bf16: 80 us, 5.0 TB/s; 8192 x 768 fp32: 17 us, 4.4 TB/s.
 template <typename T, int WPR, int CH>
 __global__ __launch_bounds__((norm_shape<WPR, CH>::THREADS)) void tam_k_norm_backward(norm_args a) {
   typedef norm_shape<WPR, CH> S;
@@ -285,8 +285,11 @@ __global__ __launch_bounds__(1024) void tam_k_norm_sums(const float* sums, uint3
 // wave where a row fits 16 elements a lane (no barriers), 16 elements a lane
 // beyond as far as the waves go, but 8 waves of 32 elements for the backward pass of
 // rows past 8192: 16 waves leave a lane 128 registers, and its six rows of 16 elements
-// spill (4096 x 16384 bf16: 523 us, 132 with 8 waves; forward 48 with 16 waves, 62
-// with 8). Past 16384 there is no room for either, and the spills stay.
+// spill (4096 x 16384 bf16: 523 us, 135 with 8 waves; forward 49 with 16 waves, 62
+// with 8). 8 waves spill less, not nothing: 30 registers of 256 in 16 bits and 105 in
+// fp32, 3.0 and 3.2 TB/s there. Past 16384 the rows fit neither: the backward pass
+// spills 514 to 705 registers and the forward pass 114 to 168 (4096 x 32768 bf16: 2160 us,
+// 0.4 TB/s, and 248, 2.2).
 struct pick {
   int wpr, ch;
 };

@@ -3,8 +3,10 @@
 Each is one function with a backward pass on hand-written gfx950 kernels
 (csrc/tam_linear.hip, csrc/tam_norm.hip); csrc/tam_layers.cpp checks the
 arguments and holds the autograd nodes.  Tensors are fp32, bf16 or fp16 on a HIP
-device; sums and statistics are fp32, and every result is rounded to its type
-once.  No counterpart in the reference, which has an optimizer only.
+device, all of a call of one type (autocast casts nothing here); sums and
+statistics are fp32, and every result is rounded to its type once.  Forward-mode
+derivatives, a second backward pass and recording by torch.jit.trace or make_fx
+raise.  No counterpart in the reference, which has an optimizer only.
 """
 
 import ctypes
@@ -39,8 +41,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None, *, 
     outputs), all of one dtype; the result is (..., outputs).  activation: None,
     "relu", "gelu" (by erf), "gelu_tanh" or "silu".  A weight kept as (inputs,
     outputs) is passed as its transposed view and read in place.  The backward
-    pass gives the gradients of every argument; where there is an activation,
-    the forward pass keeps its argument, rounded to the dtype, for it."""
+    pass gives the gradients of every argument.  Where there is an activation,
+    the forward pass keeps its argument z for it, and it hands dy act'(z) to
+    the products that make dx and dweight, both rounded to the dtype: in bf16
+    these are about 2.4e-3 of their norm off, 1.7e-3 of it their own rounding."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"turboadam_amd.linear: activation must be one of {sorted(k for k in _ACTIVATIONS if k)}, "
                          f"got {activation!r}")
