@@ -645,3 +645,66 @@ def test_linear_gradient_of_infinite_and_missing_z(dt):
         assert bool(dx[1].isnan().all()), act
         assert bool((dx[2] == 40).all()) and bool((dx[3] == 0).all()), act
         assert bool(dx[[0, *range(4, 70)]].isfinite().all()), act
+
+
+# ------------------------------------------------- offsets past 32 bits
+def _whole(g, *shape):
+    return torch.randint(-3, 4, shape, generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+
+
+def test_linear_offsets_past_32_bits():
+    """Outputs and gradients of 2.3e9 elements, in whole numbers: rows at both ends and the sums over all of them."""
+    from turboadam_amd import linear
+
+    g = _gen("long")
+    m, k, n = 70001, 24, 32768
+    x, w, dy = _whole(g, m, k).requires_grad_(), _whole(g, n, k).requires_grad_(), _whole(g, m, n)
+    b, r = _whole(g, n).requires_grad_(), dy.roll(1, 0)
+    log(f"linear {m}x{k}x{n}")
+    y = linear(x, w, b, activation="relu", residual=r)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    X, W = x.detach().double(), w.detach().double()
+    sum_w, sum_b = torch.zeros_like(W), torch.zeros(n, device="cuda", dtype=torch.float64)
+    for i in range(0, m, 5000):
+        rows = slice(i, min(i + 5000, m))
+        z = X[rows] @ W.t() + b.detach().double()
+        dz = dy[rows].double() * (z > 0)
+        assert torch.equal(y[rows], (z.relu() + r[rows].double()).to(y.dtype)), i
+        assert torch.equal(dx[rows], (dz @ W).to(dx.dtype)), i
+        sum_w += dz.t() @ X[rows]
+        sum_b += dz.sum(0)
+    assert torch.equal(dw, sum_w.to(dw.dtype)) and torch.equal(db, sum_b.to(db.dtype))
+
+
+@pytest.mark.parametrize("rows,in_out", [(1, False), (20, False), (40, False), (1, True), (40, True)])
+def test_linear_weight_past_32_bits(rows, in_out):
+    from turboadam_amd import linear
+
+    g = _gen("long weight")
+    k, n = 18000, 128256
+    x = _whole(g, rows, k)
+    w = _whole(g, k, n).t() if in_out else _whole(g, n, k)
+    log(f"linear {rows}x{k}x{n} in_out={in_out}")
+    y = linear(x, w)
+    X = x.double()
+    for i in range(0, n, 16384):
+        part = slice(i, min(i + 16384, n))
+        assert torch.equal(y[:, part], (X @ w[part].double().t()).to(y.dtype)), i
+
+
+def test_layer_norm_offsets_past_32_bits():
+    from turboadam_amd import layer_norm
+
+    g = _gen("long norm")
+    rows, n = 540001, 4096
+    x = torch.randn(rows, n, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(rows, n, generator=g, device="cuda", dtype=torch.bfloat16)
+    log(f"layer_norm {rows}x{n}")
+    y = layer_norm(x)
+    dx, = torch.autograd.grad(y, x, dy)
+    for i in (0, 261000, 524288, rows - 3000):  # the same rows by themselves, whose results other tests pin
+        part = x.detach()[i:i + 3000].clone().requires_grad_()
+        z = layer_norm(part)
+        assert torch.equal(y[i:i + 3000], z), i
+        assert torch.equal(dx[i:i + 3000], torch.autograd.grad(z, part, dy[i:i + 3000])[0]), i
+

@@ -444,6 +444,33 @@ def test_orthogonalize_in_every_large_tile(batch, rows, cols, tiles, dt):
             assert float(far.max()) <= 8 * BOUND[dt], (i, dim, int(far.argmax()))
 
 
+@pytest.mark.parametrize("rows,cols", [(65536, 33001), (33001, 65535)])
+def test_orthogonalize_offsets_past_32_bits(rows, cols):
+    """2.2e9 elements: one step of a polynomial that leaves the normalised matrix, and one that scales each of its rows
+    (columns, where it is tall) by q's diagonal, q being diagonal here."""
+    from turboadam_amd import orthogonalize
+
+    log(f"orthogonalize {rows}x{cols}")
+    x = torch.randn(rows, cols, generator=_gen("long", rows), device="cuda", dtype=torch.bfloat16)
+    out = orthogonalize(x, steps=1, coefficients=(1.0, 0.0, 0.0))
+    squares = sum(float(p.double().square().sum()) for p in x.split(4096))
+    for p, o in zip(x.split(4096), out.split(4096)):
+        want = p.double() / math.sqrt(squares)
+        assert float((o.double() - want).norm()) <= BOUND["bf16"] * float(want.norm())
+    # one element to each of the last 40 lines of the shorter side: q = diag(e^2) / |e|^2, x' = (1 + 40 q) x
+    x.zero_()
+    at = torch.arange(min(rows, cols) - 40, min(rows, cols), device="cuda")
+    other = (at * 1601) % max(rows, cols)
+    e = 1.0 + (at % 13).float()
+    i, j = (at, other) if rows <= cols else (other, at)
+    x[i, j] = e.to(x.dtype)
+    out = orthogonalize(x, steps=1, coefficients=(1.0, 40.0, 0.0))
+    n = e.double() / e.double().norm()
+    want = (1 + 40 * n * n) * n
+    assert float((out[i, j].double() - want).norm()) <= BOUND["bf16"] * float(want.norm())
+    assert int(out.count_nonzero()) == len(at)
+
+
 def test_orthogonalize_refuses_to_drop_a_gradient():
     from turboadam_amd import orthogonalize
 
