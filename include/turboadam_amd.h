@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define TAM_ABI_VERSION 11
+#define TAM_ABI_VERSION 12
 #define TAM_BLOCK_SIZE 128 /* elements per quantisation / CoState block */
 
 /* error codes */
@@ -393,6 +393,121 @@ typedef struct TamNorm {
 int tam_norm_workspace(const TamNorm* d, int backward_pass, size_t* bytes);
 int tam_norm(const TamNorm* d, void* stream);
 int tam_norm_backward(const TamNorm* d, void* workspace, size_t ws_bytes, void* stream);
+
+/* The first half of a gated feed-forward block: h = act(x gate^T) * (x up^T), and its
+ * gradients.  Both products are one; the backward pass sees g = x gate^T and u = x up^T
+ * rounded to dtype, and dg = dh u act'(g) and du = dh act(g) are rounded to it before the
+ * products that make dx, dgate and dup.  Every array is of `dtype`; arrays without a stride
+ * are contiguous.  Arrays may lie at any element's address; operands whose rows are not
+ * whole 16 bytes on 4 bytes are first copied to the workspace: ask for its size with the
+ * pointers and strides of the call. */
+typedef struct TamGated {
+  const void* x;        /* [rows][inputs], row stride ldx                          */
+  const void* gate;     /* [outputs][inputs], or [inputs][outputs] with w_in_out;  */
+  const void* up;       /* row stride ldw of both                                  */
+  void* h;              /* forward: [rows][outputs]                                */
+  void* g;              /* [rows][outputs]: forward: written, or NULL; backward:   */
+  void* u;              /* read (the forward's)                                    */
+  const void* dh;       /* backward: [rows][outputs]                               */
+  void* dx;             /* backward: [rows][inputs], or NULL                       */
+  void* dgate;          /* backward: laid out as the weights, contiguous, or NULL  */
+  void* dup;
+  uint64_t rows, inputs, outputs;
+  uint64_t ldx, ldw;    /* elements                                                */
+  uint32_t dtype;       /* TAM_DTYPE_*                                             */
+  uint32_t activation;  /* TAM_ACT_*                                               */
+  uint32_t w_in_out;    /* the weights lie as [inputs][outputs]                    */
+  uint32_t reserved;
+} TamGated;
+
+/* Bytes of workspace (256-byte aligned) of the two calls below. */
+int tam_gated_workspace(const TamGated* d, int backward_pass, size_t* bytes);
+/* How their products are cut, as tam_linear_tiles tells it: h or dx, then dgate with dup. */
+int tam_gated_tiles(const TamGated* d, int backward_pass, uint32_t* tiles);
+int tam_gated(const TamGated* d, void* workspace, size_t ws_bytes, void* stream);
+/* dx, dgate and dup (those that are not NULL). */
+int tam_gated_backward(const TamGated* d, void* workspace, size_t ws_bytes, void* stream);
+
+/* TamCross.reduction */
+#define TAM_CROSS_NONE 0 /* a loss for each row                                     */
+#define TAM_CROSS_SUM 1
+#define TAM_CROSS_MEAN 2 /* the sum over the number of counted rows (0 where it is 0) */
+
+/* An output projection with softmax cross entropy: z = x w^T, loss_i = log(sum over the
+ * vocabulary of exp(z_i)) - z_i[target_i], and its gradients.  z is never in memory as a
+ * whole: the forward pass keeps a maximum and a sum of each row of a tile, the backward pass
+ * makes z again in pieces of the vocabulary.  Rows whose target is `ignored` have no loss
+ * and no gradient, whatever x holds there, and cost nothing in passes with more than 32
+ * rows; another target outside the vocabulary makes the row's loss NaN, and with it the
+ * gradients.  x, w and their gradients are of `dtype`, the rest fp32.  The backward pass
+ * rounds (softmax - onehot) times the row's gradient to dtype before the products that make
+ * dx and dw (scaled, so that fp16 holds it). */
+typedef struct TamCross {
+  const void* x;         /* [rows][inputs], row stride ldx                         */
+  const void* w;         /* [vocabulary][inputs], row stride ldw                   */
+  const int64_t* target; /* [rows]                                                 */
+  float* loss;           /* forward: [rows], or one number where reduced           */
+  void* kept;            /* tam_cross_kept(rows) bytes, 256-byte aligned: forward:  */
+                         /* written; backward: read (the forward's)                */
+  const float* dloss;    /* backward: as loss; row i's at i * dloss_stride         */
+  void* dx;              /* backward: [rows][inputs], or NULL                      */
+  void* dw;              /* backward: [vocabulary][inputs], or NULL                */
+  uint64_t rows, inputs, vocabulary;
+  uint64_t ldx, ldw;     /* elements                                               */
+  int64_t ignored;       /* the target of rows that do not count                   */
+  int64_t dloss_stride;  /* elements                                               */
+  uint32_t dtype;        /* TAM_DTYPE_*                                            */
+  uint32_t reduction;    /* TAM_CROSS_*                                            */
+  uint64_t piece;        /* columns of a piece of the vocabulary; 0: chosen        */
+} TamCross;
+
+/* Bytes that the forward pass keeps for the backward pass. */
+size_t tam_cross_kept(uint64_t rows);
+/* Bytes of workspace (256-byte aligned) of the two calls below. */
+int tam_cross_workspace(const TamCross* d, int backward_pass, size_t* bytes);
+/* How their products are cut (as tam_linear_tiles tells it): tiles[0] the tile of z, [1] the
+ * columns of a piece (forward: 0), [2] the tile of dx, [3] of dw. */
+int tam_cross_tiles(const TamCross* d, int backward_pass, uint32_t* tiles);
+int tam_cross(const TamCross* d, void* workspace, size_t ws_bytes, void* stream);
+/* dx and dw (those that are not NULL). */
+int tam_cross_backward(const TamCross* d, void* workspace, size_t ws_bytes, void* stream);
+
+/* The heads of queries or keys: `heads` rows of dim elements at each token.  x_b, x_t and
+ * x_h are the strides of batch, token and head, in elements; a head's own are contiguous. */
+typedef struct TamHeads {
+  const void* x;        /* the heads (backward: where w is given)                  */
+  const void* w;        /* [dim]: weight of the head's norm, or NULL: no norm      */
+  const void* dy;       /* backward                                                */
+  void* y;              /* forward: the result; backward: dx                       */
+  void* dw;             /* backward: [dim], or NULL                                */
+  uint64_t heads;       /* 0: none of these                                        */
+  int64_t x_b, x_t, x_h;
+  int64_t y_b, y_t, y_h;
+  int64_t dy_b, dy_t, dy_h;
+} TamHeads;
+
+/* Rotary positions: n = x / sqrt(mean(x^2) + eps) * w over a head (n = x without w), then
+ * the pairs (a, b) of its first `rotated` elements turn by the angle position * frequency:
+ * magnitude * (a cos - b sin, a sin + b cos).  Pairs are elements i and i + rotated / 2, or
+ * 2 i and 2 i + 1 with `interleaved`.  Angles are 64-bit products.  Squares and their sums
+ * are fp32.  Results may not overlap their inputs. */
+typedef struct TamRotary {
+  TamHeads q, k;
+  const void* positions;     /* i64 or i32 at [batch * pos_b + token * pos_t]      */
+  const double* frequencies; /* f64[rotated / 2], radians a position               */
+  int64_t pos_b, pos_t;      /* elements                                           */
+  uint64_t batch, tokens, dim, rotated;
+  uint32_t dtype;            /* TAM_DTYPE_*                                        */
+  uint32_t positions64;      /* positions are i64                                  */
+  uint32_t interleaved;
+  float eps, magnitude;
+  uint32_t reserved;
+} TamRotary;
+
+/* Bytes of workspace of the backward pass (0 for the forward). */
+int tam_rotary_workspace(const TamRotary* d, int backward_pass, size_t* bytes);
+int tam_rotary(const TamRotary* d, void* stream);
+int tam_rotary_backward(const TamRotary* d, void* workspace, size_t ws_bytes, void* stream);
 
 /* ---- Muon: matrices stepped by their orthogonalised momentum.  No counterpart
  * in the reference. ---- */

@@ -28,7 +28,7 @@ TAM_FLAG_EF = 0x10
 TAM_FLAG_HAS_EF = 0x20
 TAM_FLAG_DEVICE_STEP = 0x40
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 # workspace of tam_multi_tensor_step_static (include/turboadam_amd.h)
 TAM_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -156,6 +156,97 @@ class TamNorm(ctypes.Structure):
     ]
 
 
+class TamGated(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("up", ctypes.c_void_p),
+        ("h", ctypes.c_void_p),
+        ("g", ctypes.c_void_p),
+        ("u", ctypes.c_void_p),
+        ("dh", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dgate", ctypes.c_void_p),
+        ("dup", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("inputs", ctypes.c_uint64),
+        ("outputs", ctypes.c_uint64),
+        ("ldx", ctypes.c_uint64),
+        ("ldw", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32),
+        ("activation", ctypes.c_uint32),
+        ("w_in_out", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+TAM_CROSS_NONE, TAM_CROSS_SUM, TAM_CROSS_MEAN = 0, 1, 2
+
+
+class TamCross(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("target", ctypes.c_void_p),
+        ("loss", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("dloss", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("inputs", ctypes.c_uint64),
+        ("vocabulary", ctypes.c_uint64),
+        ("ldx", ctypes.c_uint64),
+        ("ldw", ctypes.c_uint64),
+        ("ignored", ctypes.c_int64),
+        ("dloss_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_uint32),
+        ("reduction", ctypes.c_uint32),
+        ("piece", ctypes.c_uint64),
+    ]
+
+
+class TamHeads(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("heads", ctypes.c_uint64),
+        ("x_b", ctypes.c_int64),
+        ("x_t", ctypes.c_int64),
+        ("x_h", ctypes.c_int64),
+        ("y_b", ctypes.c_int64),
+        ("y_t", ctypes.c_int64),
+        ("y_h", ctypes.c_int64),
+        ("dy_b", ctypes.c_int64),
+        ("dy_t", ctypes.c_int64),
+        ("dy_h", ctypes.c_int64),
+    ]
+
+
+class TamRotary(ctypes.Structure):
+    _fields_ = [
+        ("q", TamHeads),
+        ("k", TamHeads),
+        ("positions", ctypes.c_void_p),
+        ("frequencies", ctypes.c_void_p),
+        ("pos_b", ctypes.c_int64),
+        ("pos_t", ctypes.c_int64),
+        ("batch", ctypes.c_uint64),
+        ("tokens", ctypes.c_uint64),
+        ("dim", ctypes.c_uint64),
+        ("rotated", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32),
+        ("positions64", ctypes.c_uint32),
+        ("interleaved", ctypes.c_uint32),
+        ("eps", ctypes.c_float),
+        ("magnitude", ctypes.c_float),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 TAM_MATRIX_UPDATE = 0x1
 TAM_MATRIX_NESTEROV = 0x2
 
@@ -248,6 +339,18 @@ SIGNATURES = {
     "tam_norm_workspace": (ctypes.c_int, [ctypes.POINTER(TamNorm), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_norm": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP]),
     "tam_norm_backward": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP, ctypes.c_size_t, _VP]),
+    "tam_gated_workspace": (ctypes.c_int, [ctypes.POINTER(TamGated), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_gated_tiles": (ctypes.c_int, [ctypes.POINTER(TamGated), ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
+    "tam_gated": (ctypes.c_int, [ctypes.POINTER(TamGated), _VP, ctypes.c_size_t, _VP]),
+    "tam_gated_backward": (ctypes.c_int, [ctypes.POINTER(TamGated), _VP, ctypes.c_size_t, _VP]),
+    "tam_cross_kept": (ctypes.c_size_t, [ctypes.c_uint64]),
+    "tam_cross_workspace": (ctypes.c_int, [ctypes.POINTER(TamCross), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_cross_tiles": (ctypes.c_int, [ctypes.POINTER(TamCross), ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
+    "tam_cross": (ctypes.c_int, [ctypes.POINTER(TamCross), _VP, ctypes.c_size_t, _VP]),
+    "tam_cross_backward": (ctypes.c_int, [ctypes.POINTER(TamCross), _VP, ctypes.c_size_t, _VP]),
+    "tam_rotary_workspace": (ctypes.c_int, [ctypes.POINTER(TamRotary), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "tam_rotary": (ctypes.c_int, [ctypes.POINTER(TamRotary), _VP]),
+    "tam_rotary_backward": (ctypes.c_int, [ctypes.POINTER(TamRotary), _VP, ctypes.c_size_t, _VP]),
     "tam_orthogonalize_workspace": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_orthogonalize_tiles": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     "tam_orthogonalize": (

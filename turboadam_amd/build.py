@@ -19,7 +19,8 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(BUILD_DIR, "libturboadam_amd.so")
 SOURCES = [os.path.join(PKG_DIR, "csrc", name)
-           for name in ("tam_step.hip", "tam_linear.hip", "tam_norm.hip", "tam_muon.hip")]
+           for name in ("tam_step.hip", "tam_linear.hip", "tam_norm.hip", "tam_muon.hip", "tam_gated.hip", "tam_cross.hip",
+                     "tam_rotary.hip")]
 # streaming kernels that bench.py times as the bandwidth ceiling (not part of the library's ABI)
 STREAM_LIB_PATH = os.path.join(BUILD_DIR, "libtam_stream.so")
 STREAM_SOURCES = [os.path.join(PKG_DIR, "csrc", "tam_stream.hip")]
@@ -74,10 +75,10 @@ def build_library(verbose: bool = False) -> str:
 
 
 # The host side of a steady step (csrc/tam_host.cpp) and of the layers
-# (csrc/tam_layers.cpp) in C++, a torch extension module imported from
+# (csrc/tam_layers.cpp, tam_decoder.cpp) in C++, a torch extension module imported from
 # _build/host by turboadam_amd.optimizer.
 HOST_BUILD_DIR = os.path.join(BUILD_DIR, "host")
-HOST_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_host.cpp", "tam_layers.cpp")]
+HOST_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("tam_host.cpp", "tam_layers.cpp", "tam_decoder.cpp")]
 ROCM_INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")  # of torch's HIP streams
 HOST_MODULE_PATH = os.path.join(HOST_BUILD_DIR, "_tam_host.so")
 
@@ -88,7 +89,7 @@ def build_host_module(verbose: bool = False) -> str:
     from torch.utils import cpp_extension
 
     os.makedirs(HOST_BUILD_DIR, exist_ok=True)
-    for name in ("_tam_host.so", "tam_host.o", "tam_layers.o"):  # compile every time, as the other libraries
+    for name in ("_tam_host.so", "tam_host.o", "tam_layers.o", "tam_decoder.o"):  # compile every time, as the other libraries
         path = os.path.join(HOST_BUILD_DIR, name)
         if os.path.exists(path):
             os.remove(path)

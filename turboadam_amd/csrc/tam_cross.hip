@@ -1,0 +1,911 @@
+// tam_cross.hip -- output projection with softmax cross entropy of the C ABI, on the tile
+// core of tam_gemm.h:
+//
+//   z = x w^T,  lse_i = log sum_v exp(z_iv),  loss_i = lse_i - z_i,target_i
+//   dz = (exp(z - lse) - onehot) dloss_i,  dx = dz w,  dw = dz^T x
+//
+// z (rows x vocabulary) is never in memory as a whole.
+//
+// Forward.  A tile of z stays in the matrix cores' registers and leaves a maximum and a sum
+// of exponentials of each of its rows, 8 bytes for its 64 to 256 columns
+// (tam_k_cross_logits); tam_k_cross_join makes lse and the loss of them.  Up to 32 rows read
+// the weight once, straight to the matrix cores (tam_k_cross_few).
+//
+// Backward.  Pieces of the vocabulary: z again, and dz of a piece, rounded to the type, goes
+// to memory (tam_k_cross_logits); then the piece's rows of dw, whole sums, and its share of
+// dx, added to fp32 sums that tam_k_cross_dx rounds at the end.  To make z again costs a
+// third of the gradients' products; to keep it would cost rows * vocabulary.
+//
+// Rows that do not count take no part: tam_k_cross_rows numbers the others, x is gathered
+// into rows of whole lines (the one copy of it; 26 us of 27 ms for 8192 x 4096), and every
+// later kernel reads their number from the device: its tiles of rows past it return at once, and
+// sums over rows end there.  So NaN in a padded row reaches nothing.
+//
+// dz is held as (exp(z - lse) - onehot) * w, |w| <= 1 (fp16: times 2^14, as a softmax
+// over 10^5 words lies below fp16's numbers otherwise), and the results are multiplied by
+// the power of two or the factor that is missing (scale) when they are rounded.
+#include "tam_few.h"
+#include "tam_products.h"
+
+#include <math.h>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T>
+__device__ __forceinline__ float cross_exp(float x) {
+  if constexpr (sizeof(T) == 2)  // 2^-22 of the result more than expf, below 2^-9 of the rounding
+    return __builtin_amdgcn_exp2f(kLog2e * x);
+  else
+    return expf(x);
+}
+
+// exp(z - m), 0 where z is -inf (also where m is), NaN where z is
+template <typename T>
+__device__ __forceinline__ float cross_term(float z, float m) {
+  return z == -INFINITY ? 0.0f : cross_exp<T>(z - m);
+}
+
+// What the forward pass keeps, and what every kernel reads: all by the row's own number but
+// `index` and `target`, which are by its number among those that count.
+struct cross_rows {
+  uint32_t* count;
+  uint32_t* index;   // -> row
+  int32_t* place;    // of a row -> number, or -1
+  int32_t* target;   // -1: outside the vocabulary
+  float* lse;
+};
+
+struct cross_rows_args {
+  cross_rows r;
+  const int64_t* targets;
+  float* loss;       // zeros for rows that do not count, or null
+  int64_t ignored;
+  uint32_t rows;
+  int64_t vocabulary;
+};
+
+// One workgroup numbers the rows that count, 8192 a turn in their order: 8 rows to a
+// thread, sums of the threads' numbers over waves and workgroup.
+__global__ __launch_bounds__(1024) void tam_k_cross_rows(cross_rows_args a) {
+  __shared__ uint32_t part[16];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t base = 0;
+  for (uint64_t first = 0; first < a.rows; first += 8192) {
+    const uint64_t row0 = first + threadIdx.x * 8;
+    int64_t t[8];
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      t[i] = row0 + i < a.rows ? a.targets[row0 + i] : a.ignored;
+      n += t[i] != a.ignored;
+    }
+    uint32_t upto = n;  // of the wave's lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t v = __shfl_up(upto, d);
+      upto += lane >= (uint32_t)d ? v : 0;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    uint32_t at = base + upto - n;
+    for (uint32_t w = 0; w < 16; ++w) {
+      at += w < wave ? part[w] : 0;
+      base += part[w];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (row0 + i < a.rows) {
+        const bool counts = t[i] != a.ignored;
+        if (counts) {
+          a.r.index[at] = (uint32_t)(row0 + i);
+          a.r.target[at] = t[i] >= 0 && t[i] < a.vocabulary ? (int32_t)t[i] : -1;
+        } else if (a.loss) {
+          a.loss[row0 + i] = 0.f;
+        }
+        a.r.place[row0 + i] = counts ? (int32_t)at : -1;
+        at += counts;
+      }
+  }
+  if (threadIdx.x == 0) *a.r.count = base;
+}
+
+// to[j] = the j-th row of x that counts, zeros behind it: 8 16-bit units to a thread.
+__global__ __launch_bounds__(256) void tam_k_cross_gather(const tam_f16* x, uint64_t ldx, uint32_t cols, cross_rows r,
+                                                          uint32_t rows, tam_f16* to, uint32_t ld) {
+  const uint32_t per = ld / 8, count = *r.count;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint64_t j = i / per;
+  if (j >= count || j >= rows) return;
+  const uint32_t c = (uint32_t)(i - j * per) * 8;
+  *reinterpret_cast<tam_oct<tam_f16>*>(to + j * ld + c) =
+      tam_some(x + (uint64_t)r.index[j] * ldx + c, c < cols ? cols - c : 0);
+}
+
+// ---------------------------------------------------------------------------
+// z
+// ---------------------------------------------------------------------------
+struct cross_logits_args {
+  tam_operand P, Q;    // rows of w of the piece; gathered rows of x
+  uint64_t k;
+  uint32_t tm, tn;
+  cross_rows r;
+  uint32_t first;      // column of the piece's first one
+  uint32_t cols;       // of the piece
+  uint64_t rows;       // of every array here
+  float2* parts;       // forward: [tn][rows] maximum and sum of a tile's row
+  float* hit;          // forward: [rows] z of the target
+  const struct cross_row* row;  // backward: [rows]
+  void* dz;            // backward: [rows][ld]
+  uint64_t ld;
+};
+
+// A row that counts, by its number, as dz takes it.
+struct cross_row {
+  float lse, w;
+  int32_t target;
+  uint32_t unused;
+};
+
+template <typename T, int TILE, int WM, int WN, bool BACK>
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_logits(cross_logits_args a) {
+  typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), true, true> Tile;
+  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  const uint32_t count = *a.r.count;
+  uint32_t m, n;
+  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
+  if (m * TILE >= count) return;
+  a.Q.count = count;
+  Tile t;
+  t.zero();
+  t.run(a.P, a.Q, n * TILE, m * TILE, 0, a.k, smem, tam_soon{});
+  if constexpr (BACK) {
+    t.template each<TAM_AHEAD_PASS>(
+        smem,
+        [&](uint32_t row, uint32_t) {
+          row += m * TILE;
+          return a.row[row < count ? row : count - 1];
+        },
+        [&](uint32_t row, uint32_t col, float(&v)[8], const cross_row& of) {
+          row += m * TILE;
+          col += n * TILE;
+          if (row >= count || col >= a.cols) return;
+          const uint32_t hit = (uint32_t)of.target - a.first - col;
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j) {
+            const float p = cross_exp<T>(v[j] - of.lse) - (hit == j ? 1.0f : 0.0f);
+            // columns past the last one are zeros: the sum over columns takes whole 16 bytes
+            v[j] = col + j < a.cols ? p * of.w : 0.0f;
+          }
+          tam_store8(static_cast<T*>(a.dz) + (uint64_t)row * a.ld + col, v);
+        },
+        [](uint32_t, uint32_t, const float*, int) {});
+  } else {
+    // a lane holds 4 consecutive columns of a row in each of its fragments: its 4 TN
+    // columns, then the row's 4 lanes, then the tile's waves side by side
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+    float2* at = reinterpret_cast<float2*>(smem);  // [TILE][WN]
+#pragma unroll
+    for (int f = 0; f < Tile::TM; ++f) {
+      const uint32_t in = (wm * Tile::TM + f) * 16 + (lane & 15), row = m * TILE + in;
+      const int32_t target = row < count ? a.r.target[row] : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < Tile::TN; ++c)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          const uint32_t col = n * TILE + (wn * Tile::TN + c) * 16 + (lane >> 4) * 4 + j;
+          const float z = col < a.cols ? t.acc[c][f][j] : -INFINITY;
+          t.acc[c][f][j] = z;
+          if ((int32_t)col == target) a.hit[row] = z;
+          top = fmaxf(top, z);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < Tile::TN; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += cross_term<T>(t.acc[c][f][j], top);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (lane < 16) at[in * WN + wn] = float2{top, sum};
+    }
+    __syncthreads();
+    const uint32_t row = m * TILE + threadIdx.x;
+    if (threadIdx.x < TILE && row < count) {
+      float2 all = {-INFINITY, 0.f};
+#pragma unroll
+      for (int w = 0; w < WN; ++w) all.x = fmaxf(all.x, at[threadIdx.x * WN + w].x);
+#pragma unroll
+      for (int w = 0; w < WN; ++w) {
+        const float2 p = at[threadIdx.x * WN + w];
+        if (p.y != 0.f) all.y += p.y * cross_exp<T>(p.x - all.x);
+      }
+      a.parts[(uint64_t)n * a.rows + row] = all;
+    }
+  }
+}
+
+struct cross_join_args {
+  cross_rows r;
+  const float2* parts;  // [tiles][rows], or of few rows [rows][tiles]
+  const float* hit;
+  float* loss;          // by row, or where they are added by number
+  uint64_t rows;
+  uint32_t tiles;
+  bool by_number;
+  const int64_t* targets;  // few rows: read here
+  int64_t ignored, vocabulary;
+};
+
+// The sum of parts p0, p0 + step, .. with the common maximum.
+__device__ __forceinline__ float2 cross_add(const float2& a, const float2& b) {
+  const float top = fmaxf(a.x, b.x);
+  return {top, (a.y != 0.f ? a.y * expf(a.x - top) : 0.f) + (b.y != 0.f ? b.y * expf(b.x - top) : 0.f)};
+}
+
+// 64 rows to a workgroup, 16 threads to a row, whose sums meet in their order.
+__global__ __launch_bounds__(1024) void tam_k_cross_join(cross_join_args a) {
+  __shared__ float2 at[16][64];
+  const uint32_t lane = threadIdx.x & 63, run = threadIdx.x >> 6, count = *a.r.count;
+  const uint32_t j = blockIdx.x * 64 + lane;
+  if (blockIdx.x * 64 >= count) return;
+  float2 s = {-INFINITY, 0.f};
+  if (j < count)
+#pragma unroll 8
+    for (uint32_t t = run; t < a.tiles; t += 16) s = cross_add(s, a.parts[(uint64_t)t * a.rows + j]);
+  at[run][lane] = s;
+  __syncthreads();
+  if (run == 0 && j < count) {
+    for (int w = 1; w < 16; ++w) s = cross_add(s, at[w][lane]);
+    const uint32_t row = a.r.index[j];
+    const float lse = a.r.target[j] < 0 ? NAN : s.x + logf(s.y);
+    a.r.lse[row] = lse;
+    a.loss[a.by_number ? j : row] = lse - a.hit[j];
+  }
+}
+
+// Few rows: a workgroup to a row.
+__global__ __launch_bounds__(256) void tam_k_cross_join_few(cross_join_args a) {
+  __shared__ float2 at[256];
+  const uint32_t row = blockIdx.x;
+  const int64_t target = a.targets[row];
+  float2 s = {-INFINITY, 0.f};
+#pragma unroll 8
+  for (uint32_t t = threadIdx.x; t < a.tiles; t += 256) s = cross_add(s, a.parts[(uint64_t)row * a.tiles + t]);
+  at[threadIdx.x] = s;
+  for (int half = 128; half >= 1; half /= 2) {
+    __syncthreads();
+    if ((int)threadIdx.x < half) at[threadIdx.x] = cross_add(at[threadIdx.x], at[threadIdx.x + half]);
+  }
+  if (threadIdx.x == 0) {
+    s = at[0];
+    const bool inside = target >= 0 && target < a.vocabulary;
+    const float lse = inside ? s.x + logf(s.y) : NAN;
+    if (a.r.lse) a.r.lse[row] = lse;
+    a.loss[row] = target == a.ignored ? 0.f : lse - (inside ? a.hit[row] : 0.f);
+  }
+}
+
+// The losses' sum in 64 bits, in a fixed order, over their number where it is a mean.
+__global__ __launch_bounds__(1024) void tam_k_cross_sum(const float* losses, const uint32_t* count, const int64_t* targets,
+                                                        int64_t ignored, uint32_t rows, bool mean, float* loss) {
+  __shared__ double at[1024];
+  __shared__ uint32_t number[1024];
+  // few rows: by row, and those that count are counted here
+  const uint32_t n = count ? *count : rows;
+  double s = 0.;
+  uint32_t c = 0;
+  for (uint32_t j = threadIdx.x; j < n; j += 1024) {
+    s += (double)losses[j];
+    c += count || targets[j] != ignored;
+  }
+  at[threadIdx.x] = s;
+  number[threadIdx.x] = c;
+  for (int half = 512; half >= 1; half /= 2) {
+    __syncthreads();
+    if ((int)threadIdx.x < half) {
+      at[threadIdx.x] += at[threadIdx.x + half];
+      number[threadIdx.x] += number[threadIdx.x + half];
+    }
+  }
+  if (threadIdx.x == 0) *loss = (float)(mean ? at[0] / (double)(number[0] ? number[0] : 1u) : at[0]);
+}
+
+struct cross_few_args {
+  const void* x;
+  const void* w;
+  uint64_t ldx, ldw, k;
+  const int64_t* targets;
+  float2* parts;  // [rows][workgroups]
+  float* hit;
+  uint32_t rows, cols;
+};
+
+// One workgroup: 16 columns of z for up to 16 * MT rows of x, as tam_k_few.
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_args a) {
+  constexpr int N = 16 / (int)sizeof(T), U = 4;
+  constexpr uint64_t TURN = 4 * U * N;  // k of a wave's turn
+  __shared__ float sum[TAM_FEW_WAVES][MT * 16][20];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t i = lane & 15, q = lane >> 4, n = blockIdx.x * 16 + i;
+  // rows past the last one read the first one's elements; their sums go nowhere
+  const T* w = static_cast<const T*>(a.w) + (n < a.cols ? (uint64_t)n * a.ldw : 0);
+  const T* x[MT];
+  tam_f4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    x[m] = static_cast<const T*>(a.x) + (m * 16 + i < a.rows ? (uint64_t)(m * 16 + i) * a.ldx : 0);
+    acc[m] = tam_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto turn = [&](uint64_t k0, auto guard) {
+    constexpr bool G = decltype(guard)::value;
+    tam_frag<T> fw[U], fx[MT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) tam_few_load<T, G>(fw[u], w, k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) tam_few_load<T, G>(fx[m][u], x[m], k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc[m] = tam_mfma(fw[u], fx[m][u], acc[m]);
+  };
+  uint64_t k0 = wave * TURN;
+#pragma unroll 2
+  for (; k0 + TURN <= a.k; k0 += TAM_FEW_WAVES * TURN) turn(k0, std::false_type());
+  if (k0 < a.k) turn(k0, std::true_type());
+#pragma unroll
+  for (int m = 0; m < MT; ++m)  // row m * 16 + i, columns 4 q ..
+    *reinterpret_cast<tam_f4*>(&sum[wave][m * 16 + i][q * 4]) = acc[m];
+  __syncthreads();
+  const uint32_t t = threadIdx.x, row = t / 2, col = blockIdx.x * 16 + (t % 2) * 8;
+  if (t < MT * 32) {
+    float v[8] = {};
+    for (int s = 0; s < TAM_FEW_WAVES; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += sum[s][row][(t % 2) * 8 + j];
+    const int64_t target = row < a.rows ? a.targets[row] : -1;
+    float top = -INFINITY, all = 0.f;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      if (col + j >= a.cols) v[j] = -INFINITY;
+      else if (target == (int64_t)(col + j)) a.hit[row] = v[j];
+      top = fmaxf(top, v[j]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 1));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) all += cross_term<T>(v[j], top);
+    all += __shfl_xor(all, 1);
+    if (t % 2 == 0 && row < a.rows) a.parts[(uint64_t)row * gridDim.x + blockIdx.x] = float2{top, all};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// gradients
+// ---------------------------------------------------------------------------
+struct cross_weights_args {
+  cross_rows r;
+  const float* dloss;
+  int64_t stride;
+  uint32_t reduction;
+  float lift;     // of dz
+  cross_row* row; // [rows]
+  float* scale;   // what the products are multiplied by
+};
+
+// Each row's weight, and scale. A gradient for each row: scale is the least power of two above the
+// largest finite one, so that dividing by it rounds nothing.
+__global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a) {
+  __shared__ float top[1024];
+  const uint32_t count = *a.r.count;
+  if (a.reduction != TAM_CROSS_NONE) {
+    for (uint32_t j = threadIdx.x; j < count; j += 1024) a.row[j] = {a.r.lse[a.r.index[j]], a.lift, a.r.target[j], 0};
+    if (threadIdx.x == 0)
+      *a.scale = (a.reduction == TAM_CROSS_MEAN ? a.dloss[0] / (float)(count ? count : 1u) : a.dloss[0]) / a.lift;
+    return;
+  }
+  float most = 0.f;
+  for (uint32_t j = threadIdx.x; j < count; j += 1024) {
+    const float d = fabsf(a.dloss[(int64_t)a.r.index[j] * a.stride]);
+    if (d < INFINITY) most = fmaxf(most, d);
+  }
+  top[threadIdx.x] = most;
+  for (int half = 512; half >= 1; half /= 2) {
+    __syncthreads();
+    if ((int)threadIdx.x < half) top[threadIdx.x] = fmaxf(top[threadIdx.x], top[threadIdx.x + half]);
+  }
+  __syncthreads();
+  int power;
+  frexpf(top[0], &power);
+  power = power < -100 ? -100 : power;
+  for (uint32_t j = threadIdx.x; j < count; j += 1024) {
+    const uint32_t row = a.r.index[j];
+    a.row[j] = {a.r.lse[row], ldexpf(a.dloss[(int64_t)row * a.stride], -power) * a.lift, a.r.target[j], 0};
+  }
+  if (threadIdx.x == 0) *a.scale = ldexpf(1.0f, power) / a.lift;
+}
+
+struct cross_product_args {
+  tam_operand P, Q;
+  uint64_t k, k_part;      // dw: k is the rows that count, k_part of all rows
+  uint32_t tm, tn;
+  const uint32_t* count;
+  const float* scale;
+  uint32_t rows, cols;
+  float* sums;             // [part][rows][cols], or null: dw's own
+  bool add;                // to what the sums hold
+  void* dw;
+};
+
+// dx's share of a piece (WEIGHT false: fp32 sums) or the piece's rows of dw.
+template <typename T, int TILE, int WM, int WN, bool WEIGHT>
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_product(cross_product_args a) {
+  typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, !WEIGHT> Tile;
+  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  const uint32_t count = *a.count;
+  uint32_t m, n;
+  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
+  const uint32_t rows = WEIGHT ? a.rows : count;
+  if (m * TILE >= rows) return;
+  if (!WEIGHT) a.Q.count = count;
+  const uint64_t k = WEIGHT ? count : a.k, k0 = blockIdx.y * a.k_part;
+  const uint64_t k1 = k0 + a.k_part < k ? k0 + a.k_part : k;
+  float* sums = a.sums ? a.sums + (uint64_t)blockIdx.y * a.rows * a.cols : nullptr;
+  Tile t;
+  t.zero();
+  tam_soon soon = {};
+  if (a.add) {
+    const uint64_t ld = (uint64_t)a.cols * 4;
+    soon = {reinterpret_cast<const char*>(sums) + m * TILE * ld + n * TILE * 4, ld, rows - m * TILE, (a.cols - n * TILE) * 4,
+            TILE * 4};
+  }
+  t.run(a.P, a.Q, n * TILE, m * TILE, k0, k1, smem, soon);
+  const float scale = WEIGHT ? *a.scale : 1.0f;
+  t.template each<TAM_AHEAD_PASS>(
+      smem,
+      [&](uint32_t row, uint32_t col) {
+        tam_oct<float> s = {};
+        row += m * TILE;
+        col += n * TILE;
+        if (!WEIGHT && a.add && row < rows && col < a.cols)
+          s = tam_some(sums + (uint64_t)row * a.cols + col, a.cols - col);
+        return s;
+      },
+      [&](uint32_t row, uint32_t col, float(&v)[8], const tam_oct<float>& s) {
+        row += m * TILE;
+        col += n * TILE;
+        if (row >= rows || col >= a.cols) return;
+        const uint64_t at = (uint64_t)row * a.cols + col;
+        if (WEIGHT && !sums) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= scale;
+          tam_store_some(static_cast<T*>(a.dw) + at, a.cols - col, v);
+        } else {
+          if (!WEIGHT && a.add)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += s.v[j];
+          tam_store_some(sums + at, a.cols - col, v);
+        }
+      },
+      [](uint32_t, uint32_t, const float*, int) {});
+}
+
+// out[row] = the parts' sums of the row's number in their order, times scale; zeros for
+// rows that do not count. place == null: a row's number is its own.
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_cross_out(const float* sums, uint32_t parts, uint64_t rows, uint32_t cols,
+                                                       const int32_t* place, const float* scale, T* out) {
+  const uint32_t per = (cols + 7) / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= per * rows) return;
+  const uint64_t row = i / per;
+  const uint32_t col = (uint32_t)(i - row * per) * 8;
+  const int64_t at = place ? place[row] : (int64_t)row;
+  float v[8] = {};
+  if (at >= 0) {
+    const float s = *scale;
+    for (uint32_t p = 0; p < parts; ++p) {
+      float t[8];
+      tam_load_some(sums + (p * rows + at) * cols + col, cols - col, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= s;
+  }
+  tam_store_some(out + row * cols + col, cols - col, v);
+}
+
+__global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n) {
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = (tam_f16)0.0f;  // zero has the same bits in every type
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr uint64_t kFew = 32;
+constexpr uint64_t kPieceBytes = 512ull << 20;  // of dz
+constexpr uint64_t kMostPiece = 1ull << 20;     // a tile's offsets are 31-bit numbers of bytes
+
+int check_cross(const TamCross* d, bool back) {
+  tam_op_begin();
+  if (!d) return tam_op_fail(TAM_E_INVALID, "null argument");
+  if (d->dtype > TAM_DTYPE_F16) return tam_op_fail(TAM_E_INVALID, "unknown dtype %u", d->dtype);
+  if (d->reduction > TAM_CROSS_MEAN) return tam_op_fail(TAM_E_INVALID, "unknown reduction %u", d->reduction);
+  const uint64_t most = 1ull << 31;
+  if (d->rows >= most || d->inputs >= most || d->vocabulary >= most - 256)
+    return tam_op_fail(TAM_E_UNSUPPORTED, "a size of 2^31 or more");
+  if (d->inputs && (d->ldx < d->inputs || d->ldw < d->inputs))
+    return tam_op_fail(TAM_E_INVALID, "a row stride shorter than its row");
+  if ((d->ldx | d->ldw | d->inputs) >= 1ull << 21)
+    return tam_op_fail(TAM_E_UNSUPPORTED, "a row or row stride of 2^21 elements or more");
+  if (d->piece % 256 || d->piece > kMostPiece)
+    return tam_op_fail(TAM_E_INVALID, "a piece that is no multiple of 256, or above 2^20");
+  if (!d->rows && (back || d->reduction == TAM_CROSS_NONE)) return TAM_OK;
+  if (d->rows && d->vocabulary == 0) return tam_op_fail(TAM_E_INVALID, "an empty vocabulary");
+  if (d->rows && d->inputs && (!d->x || !d->w)) return tam_op_fail(TAM_E_INVALID, "null x or w");
+  if (d->rows && !d->target) return tam_op_fail(TAM_E_INVALID, "null target");
+  if (!back && !d->loss) return tam_op_fail(TAM_E_INVALID, "null loss");
+  if (back && (!d->kept || !d->dloss)) return tam_op_fail(TAM_E_INVALID, "null dloss, or what the forward pass kept");
+  if ((uintptr_t)d->kept & 255u) return tam_op_fail(TAM_E_INVALID, "kept memory not on 256 bytes");
+  return TAM_OK;
+}
+
+uint64_t kept_bytes(uint64_t rows) { return 256 + tam_up(16 * rows, 256); }
+
+cross_rows rows_in(void* kept, uint64_t rows) {
+  if (!kept) return {};
+  uint32_t* p = (uint32_t*)((char*)kept + 256);
+  return {(uint32_t*)kept, p, (int32_t*)(p + rows), (int32_t*)(p + 2 * rows), (float*)(p + 3 * rows)};
+}
+
+int number_rows(const TamCross* d, const cross_rows& r, float* loss, hipStream_t s) {
+  const cross_rows_args a = {r, d->target, loss, d->ignored, (uint32_t)d->rows, (int64_t)d->vocabulary};
+  hipLaunchKernelGGL(tam_k_cross_rows, dim3(1), dim3(1024), 0, s, a);
+  TAM_OP_LAUNCHED("the rows' numbers");
+  return TAM_OK;
+}
+
+#define TAM_OF_TYPE(c, CALL)                               \
+  do {                                                     \
+    if ((c).dtype == TAM_DTYPE_F32) {                      \
+      CALL(float);                                         \
+    } else if ((c).dtype == TAM_DTYPE_BF16) {              \
+      CALL(tam_bf16);                                      \
+    } else {                                               \
+      CALL(tam_f16);                                       \
+    }                                                      \
+  } while (0)
+
+// The rows of x that count, and w, as the tiles read them.
+int operands(const TamCross* d, call& c, const cross_rows& r, matrix& x, matrix& w) {
+  const uint32_t size = kSize[c.dtype], halves = size / 2, inputs = (uint32_t)d->inputs;
+  w = matrix_of(d->w, d->ldw, d->vocabulary, d->inputs, size);
+  const int rc = whole_rows(c, w);
+  if (rc != TAM_OK) return rc;
+  const uint32_t ld = aligned_ld(inputs, size);
+  x = {c.ws.take(d->rows * ld * size), ld, d->rows, inputs, true};
+  if (!c.dry && inputs) {
+    const dim3 grid((uint32_t)tam_div_up(d->rows * (ld * halves / 8), 256)), block(256);
+    hipLaunchKernelGGL(tam_k_cross_gather, grid, block, 0, c.stream, (const tam_f16*)d->x, d->ldx * halves, inputs * halves, r,
+                       (uint32_t)d->rows, (tam_f16*)x.p, ld * halves);
+    TAM_OP_LAUNCHED("the rows' copy");
+  }
+  return TAM_OK;
+}
+
+template <typename T, bool BACK>
+void launch_logits(int tile, const cross_logits_args& a, hipStream_t s) {
+  const dim3 grid(a.tm * a.tn);
+  if constexpr (sizeof(T) == 2)
+    if (tile == 256) {
+      hipLaunchKernelGGL((tam_k_cross_logits<T, 256, 2, 4, BACK>), grid, dim3(512), 0, s, a);
+      return;
+    }
+  if (tile == 128)
+    hipLaunchKernelGGL((tam_k_cross_logits<T, 128, 2, 2, BACK>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((tam_k_cross_logits<T, 64, 2, 2, BACK>), grid, dim3(256), 0, s, a);
+}
+
+template <typename T, bool WEIGHT>
+void launch_product(int tile, const cross_product_args& a, uint32_t parts, hipStream_t s) {
+  const dim3 grid(a.tm * a.tn, parts);
+  if constexpr (sizeof(T) == 2)
+    if (tile == 256) {
+      hipLaunchKernelGGL((tam_k_cross_product<T, 256, 2, 4, WEIGHT>), grid, dim3(512), 0, s, a);
+      return;
+    }
+  if (tile == 128)
+    hipLaunchKernelGGL((tam_k_cross_product<T, 128, 2, 2, WEIGHT>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((tam_k_cross_product<T, 64, 2, 2, WEIGHT>), grid, dim3(256), 0, s, a);
+}
+
+// The tile of a product that is not cut into parts.
+int tile_of(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
+  const double cus = tam_op_cus();
+  const bool f32 = dtype == TAM_DTYPE_F32;
+  const tam_tile_rate* rate = f32 ? tam_rates_32 : tam_rates_16;
+  int best = 64;
+  double least = 1e30;
+  for (int i = 0; i < (f32 ? 2 : 3); ++i) {
+    const double us = tam_tiles_us(
+        rate[i], (double)tam_div_up(rows, rate[i].tile) * (double)tam_div_up(cols, rate[i].tile), (double)k, cus);
+    if (us < least) {
+      least = us;
+      best = rate[i].tile;
+    }
+  }
+  return best;
+}
+
+cross_logits_args logits_of(const TamCross* d, const matrix& x, const matrix& w, const cross_rows& r, uint64_t first,
+                            uint64_t cols, int tile, uint32_t size) {
+  cross_logits_args a = {};
+  a.P = operand_of(w, (uint32_t)cols, size);
+  a.P.base += first * w.ld * size;
+  a.Q = operand_of(x, (uint32_t)d->rows, size);
+  a.k = d->inputs;
+  a.tm = (uint32_t)tam_div_up(d->rows, tile);
+  a.tn = (uint32_t)tam_div_up(cols, tile);
+  a.r = r;
+  a.first = (uint32_t)first;
+  a.cols = (uint32_t)cols;
+  a.rows = d->rows;
+  return a;
+}
+
+int forward(const TamCross* d, call& c) {
+  const bool reduced = d->reduction != TAM_CROSS_NONE;
+  const uint32_t rows = (uint32_t)d->rows;
+  if (rows == 0 && !reduced) return TAM_OK;
+  cross_join_args j = {};
+  j.targets = d->target;
+  j.ignored = d->ignored;
+  j.vocabulary = (int64_t)d->vocabulary;
+  j.rows = rows;
+  float* losses = d->loss;
+  if (reduced) losses = (float*)c.ws.take(4ull * rows);
+  const bool few = rows <= kFew;
+  if (rows) {
+    float* hit = (float*)c.ws.take(4ull * rows);
+    cross_rows r = rows_in(d->kept, rows);
+    if (few) {
+      const uint32_t groups = (uint32_t)tam_div_up(d->vocabulary, 16);
+      float2* parts = (float2*)c.ws.take(8ull * rows * groups);
+      if (!c.dry) {
+        if (d->kept) {
+          const int rc = number_rows(d, r, nullptr, c.stream);
+          if (rc != TAM_OK) return rc;
+        }
+        const cross_few_args a = {d->x, d->w, d->ldx, d->ldw, d->inputs, d->target, parts, hit, rows, (uint32_t)d->vocabulary};
+        const dim3 grid(groups), block(64 * TAM_FEW_WAVES);
+#define TAM_FEW(T)                                                             \
+  if (rows <= 16)                                                              \
+    hipLaunchKernelGGL((tam_k_cross_few<T, 1>), grid, block, 0, c.stream, a);  \
+  else                                                                         \
+    hipLaunchKernelGGL((tam_k_cross_few<T, 2>), grid, block, 0, c.stream, a)
+        TAM_OF_TYPE(c, TAM_FEW);
+        TAM_OP_LAUNCHED("the logits of few rows");
+        j.r = r;
+        j.parts = parts;
+        j.hit = hit;
+        j.loss = losses;
+        j.tiles = groups;
+        hipLaunchKernelGGL(tam_k_cross_join_few, dim3(rows), dim3(256), 0, c.stream, j);
+        TAM_OP_LAUNCHED("the losses");
+      }
+    } else {
+      if (!d->kept) r = rows_in(c.ws.take(kept_bytes(rows)), rows);
+      if (!c.dry) {
+        const int rc = number_rows(d, r, reduced ? nullptr : d->loss, c.stream);
+        if (rc != TAM_OK) return rc;
+      }
+      const int tile = tile_of(rows, d->vocabulary, d->inputs, c.dtype);
+      if (c.tiles) c.tiles[0] = (uint32_t)tile;
+      matrix x, w;
+      const int rc = operands(d, c, r, x, w);
+      if (rc != TAM_OK) return rc;
+      cross_logits_args a = logits_of(d, x, w, r, 0, d->vocabulary, tile, kSize[c.dtype]);
+      if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+      a.parts = (float2*)c.ws.take(8ull * rows * a.tn);
+      a.hit = hit;
+      if (!c.dry) {
+#define TAM_LOGITS(T) launch_logits<T, false>(tile, a, c.stream)
+        TAM_OF_TYPE(c, TAM_LOGITS);
+        TAM_OP_LAUNCHED("the logits");
+        j.r = r;
+        j.parts = a.parts;
+        j.hit = hit;
+        j.loss = losses;
+        j.by_number = reduced;
+        j.tiles = a.tn;
+        hipLaunchKernelGGL(tam_k_cross_join, dim3((uint32_t)tam_div_up(rows, 64)), dim3(1024), 0, c.stream, j);
+        TAM_OP_LAUNCHED("the losses");
+      }
+    }
+    j.r = r;
+  }
+  if (reduced && !c.dry) {
+    hipLaunchKernelGGL(tam_k_cross_sum, dim3(1), dim3(1024), 0, c.stream, losses, few ? nullptr : j.r.count, d->target, d->ignored,
+                       rows, d->reduction == TAM_CROSS_MEAN, d->loss);
+    TAM_OP_LAUNCHED("the losses' sum");
+  }
+  return TAM_OK;
+}
+
+// Columns of a piece: as even as they come, in whole tiles, of at most kPieceBytes of dz.
+uint64_t piece_of(const TamCross* d, uint32_t size) {
+  if (d->piece) return d->piece;
+  uint64_t most = kPieceBytes / (d->rows * size) / 256 * 256;
+  most = most < 256 ? 256 : (most > kMostPiece ? kMostPiece : most);
+  return tam_up(tam_div_up(d->vocabulary, tam_div_up(d->vocabulary, most)), 256);
+}
+
+int zero(const call& c, void* p, uint64_t elements) {
+  if (c.dry || !p || !elements) return TAM_OK;
+  const uint64_t halves = elements * (kSize[c.dtype] / 2);
+  hipLaunchKernelGGL(tam_k_cross_zero, dim3((uint32_t)tam_div_up(halves, 256)), dim3(256), 0, c.stream, (tam_f16*)p, halves);
+  TAM_OP_LAUNCHED("an empty sum");
+  return TAM_OK;
+}
+
+int backward(const TamCross* d, call& c) {
+  if (!d->dx && !d->dw) return TAM_OK;
+  const uint32_t rows = (uint32_t)d->rows, inputs = (uint32_t)d->inputs, size = kSize[c.dtype];
+  if (!rows || !inputs) return zero(c, d->dw, d->vocabulary * d->inputs);
+  const cross_rows r = rows_in(d->kept, rows);
+  cross_row* row = (cross_row*)c.ws.take(sizeof(cross_row) * (uint64_t)rows);
+  float* scale = (float*)c.ws.take(4);
+  if (!c.dry) {
+    const float lift = c.dtype == TAM_DTYPE_F16 ? 16384.0f : 1.0f;
+    const cross_weights_args a = {r, d->dloss, d->dloss_stride, d->reduction, lift, row, scale};
+    hipLaunchKernelGGL(tam_k_cross_weights, dim3(1), dim3(1024), 0, c.stream, a);
+    TAM_OP_LAUNCHED("the rows' weights");
+  }
+  matrix x, w;
+  int rc = operands(d, c, r, x, w);
+  if (rc != TAM_OK) return rc;
+  const uint64_t piece = piece_of(d, size), widest = d->vocabulary < piece ? d->vocabulary : piece;
+  const uint32_t ld = aligned_ld((uint32_t)widest, size);
+  void* dz = c.ws.take((uint64_t)rows * ld * size);
+  const int tile_z = tile_of(rows, widest, inputs, c.dtype);
+  const shape sx = choose(rows, inputs, widest, c.dtype), sw = choose(widest, inputs, rows, c.dtype);
+  if (c.tiles) {
+    c.tiles[0] = (uint32_t)tile_z;
+    c.tiles[1] = (uint32_t)piece;
+    if (d->dx) c.tiles[2] = (uint32_t)sx.tile;
+    if (d->dw) c.tiles[3] = (uint32_t)sw.tile;
+  }
+  float* dx_sums = d->dx ? (float*)c.ws.take(4ull * sx.parts * rows * inputs) : nullptr;
+  float* dw_sums = d->dw && sw.parts > 1 ? (float*)c.ws.take(4ull * sw.parts * widest * inputs) : nullptr;
+  if (c.dry) return TAM_OK;
+  for (uint64_t first = 0; first < d->vocabulary; first += piece) {
+    const uint32_t cols = (uint32_t)(d->vocabulary - first < piece ? d->vocabulary - first : piece);
+    cross_logits_args a = logits_of(d, x, w, r, first, cols, tile_z, size);
+    if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+    a.row = row;
+    a.dz = dz;
+    a.ld = ld;
+#define TAM_DZ(T) launch_logits<T, true>(tile_z, a, c.stream)
+    TAM_OF_TYPE(c, TAM_DZ);
+    TAM_OP_LAUNCHED("the logits' gradient");
+    const matrix z = {dz, ld, rows, cols, true};
+    if (d->dx) {
+      cross_product_args p = {};
+      p.P = operand_of(w, inputs, size);
+      p.P.base += first * w.ld * size;
+      p.Q = operand_of(z, rows, size);
+      p.k = cols;
+      p.k_part = sx.parts > 1 ? tam_up(tam_div_up(cols, sx.parts), 64) : cols;
+      p.tm = (uint32_t)tam_div_up(rows, sx.tile);
+      p.tn = (uint32_t)tam_div_up(inputs, sx.tile);
+      p.count = r.count;
+      p.scale = scale;
+      p.rows = rows;
+      p.cols = inputs;
+      p.sums = dx_sums;
+      p.add = first != 0;
+#define TAM_DX(T) launch_product<T, false>(sx.tile, p, sx.parts, c.stream)
+      TAM_OF_TYPE(c, TAM_DX);
+      TAM_OP_LAUNCHED("dx");
+    }
+    if (d->dw) {
+      cross_product_args p = {};
+      p.P = operand_of(x, inputs, size);
+      p.Q = operand_of(z, cols, size);
+      p.k = rows;
+      p.k_part = sw.parts > 1 ? tam_up(tam_div_up(rows, sw.parts), 64) : rows;
+      p.tm = (uint32_t)tam_div_up(cols, sw.tile);
+      p.tn = (uint32_t)tam_div_up(inputs, sw.tile);
+      p.count = r.count;
+      p.scale = scale;
+      p.rows = cols;
+      p.cols = inputs;
+      p.sums = dw_sums;
+      p.dw = (char*)d->dw + first * inputs * size;
+#define TAM_DW(T) launch_product<T, true>(sw.tile, p, sw.parts, c.stream)
+      TAM_OF_TYPE(c, TAM_DW);
+      TAM_OP_LAUNCHED("dw");
+      if (dw_sums) {
+        const dim3 grid((uint32_t)tam_div_up((uint64_t)cols * tam_div_up(inputs, 8), 256)), block(256);
+#define TAM_DW_OUT(T) \
+  hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dw_sums, sw.parts, (uint64_t)cols, inputs, nullptr, scale, (T*)p.dw)
+        TAM_OF_TYPE(c, TAM_DW_OUT);
+        TAM_OP_LAUNCHED("dw's sum");
+      }
+    }
+  }
+  if (d->dx) {
+    const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * tam_div_up(inputs, 8), 256)), block(256);
+#define TAM_DX_OUT(T) \
+  hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dx_sums, sx.parts, (uint64_t)rows, inputs, r.place, scale, (T*)d->dx)
+    TAM_OF_TYPE(c, TAM_DX_OUT);
+    TAM_OP_LAUNCHED("dx's sum");
+  }
+  return TAM_OK;
+}
+
+int cross(const TamCross* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need,
+          uint32_t* tiles = nullptr) {
+  int rc = check_cross(d, back);
+  if (rc != TAM_OK) return rc;
+  call c = {d->dtype, (hipStream_t)stream, {nullptr, 0}, true, tiles};
+  rc = back ? backward(d, c) : forward(d, c);
+  if (rc != TAM_OK) return rc;
+  if (need) {
+    *need = c.ws.used;
+    return TAM_OK;
+  }
+  if (c.ws.used > ws_bytes || (c.ws.used && !workspace))
+    return tam_op_fail(TAM_E_WORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes,
+                       (unsigned long long)c.ws.used);
+  if ((uintptr_t)workspace & 255u) return tam_op_fail(TAM_E_INVALID, "workspace not on 256 bytes");
+  c = {d->dtype, (hipStream_t)stream, {(char*)workspace, 0}, false, nullptr};
+  return back ? backward(d, c) : forward(d, c);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tam_cross_kept(uint64_t rows) { return (size_t)kept_bytes(rows); }
+
+int tam_cross_workspace(const TamCross* d, int backward_pass, size_t* bytes) {
+  if (!bytes) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  uint64_t need = 0;
+  const int rc = cross(d, backward_pass != 0, nullptr, 0, nullptr, &need);
+  *bytes = (size_t)need;
+  return rc;
+}
+
+int tam_cross_tiles(const TamCross* d, int backward_pass, uint32_t* tiles) {
+  if (!tiles) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  for (int i = 0; i < 4; ++i) tiles[i] = 0;
+  uint64_t need = 0;
+  return cross(d, backward_pass != 0, nullptr, 0, nullptr, &need, tiles);
+}
+
+int tam_cross(const TamCross* d, void* workspace, size_t ws_bytes, void* stream) {
+  return cross(d, false, workspace, ws_bytes, stream, nullptr);
+}
+
+int tam_cross_backward(const TamCross* d, void* workspace, size_t ws_bytes, void* stream) {
+  return cross(d, true, workspace, ws_bytes, stream, nullptr);
+}
+
+}  // extern "C"

@@ -1,0 +1,560 @@
+// tam_gated.hip -- the first half of a gated feed-forward block of the C ABI, on the tile
+// core of tam_gemm.h:
+//
+//   g = x gate^T,  u = x up^T,  h = act(g) u
+//   dg = dh u act'(g),  du = dh act(g)
+//   dx = dg gate + du up,  dgate = dg^T x,  dup = du^T x
+//
+// Kernels:
+//   tam_k_gated      one tile of both products: half of its columns are of g and half of
+//                    u, the same ones, so that one lane ends up with both and the
+//                    product is formed in registers (x is staged once for both);
+//   tam_k_gated_few  the forward products of up to 32 rows: every wave reads its part of
+//                    16 rows of either weight once, straight to the matrix cores;
+//   tam_k_gated_join the same epilogue over the partial sums of products whose k was cut
+//                    among workgroups (few tiles);
+//   tam_k_gated_slope dg and du, side by side in one row: then dgate and dup are one
+//                    product of twice the rows, and dx is one sum of twice the length
+//                    (TAM_TWO_PRODUCTS);
+//   tam_k_gated_product, tam_k_gated_sum  those products.
+#include "tam_act.h"
+#include "tam_few.h"
+#include "tam_products.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+struct gated_epilogue {
+  void* h;  // [rows][cols], contiguous
+  void* g;  // or null
+  void* u;  // or null
+  uint32_t rows, cols, act;
+};
+
+// a, b: columns col .. col + 7 of a row of g and u. h is formed of both as they are in
+// fp32; they are kept rounded to the type (half of the memory).
+template <typename T>
+__device__ __forceinline__ void gated_finish(const gated_epilogue& e, uint32_t row, uint32_t col, const float (&a)[8],
+                                             const float (&b)[8]) {
+  const uint64_t at = (uint64_t)row * e.cols + col;
+  const uint32_t count = e.cols - col;
+  if (e.g) tam_store_some(static_cast<T*>(e.g) + at, count, a);
+  if (e.u) tam_store_some(static_cast<T*>(e.u) + at, count, b);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = tam_act<sizeof(T) == 2>(a[j], e.act) * b[j];
+  tam_store_some(static_cast<T*>(e.h) + at, count, v);
+}
+
+struct gated_args {
+  tam_operand_pair P;  // gate, up
+  tam_operand Q;       // x
+  uint64_t k, k_part;
+  uint32_t tm, tn;     // tiles: BM rows, BN / 2 columns of h
+  float* partial;      // [part][2][rows][cols] fp32, or null: one part
+  gated_epilogue e;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool PK>
+__global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gated(gated_args a) {
+  typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, true, false, true> Tile;
+  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  uint32_t m, n;
+  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
+  const uint64_t k0 = blockIdx.y * a.k_part;
+  const uint64_t k1 = k0 + a.k_part < a.k ? k0 + a.k_part : a.k;
+  Tile t;
+  t.zero();
+  t.run(a.P, a.Q, n * (BN / 2), m * BM, k0, k1, smem, tam_soon{});
+  t.pairs(smem, [&](uint32_t row, uint32_t col, const float(&g)[8], const float(&u)[8]) {
+    row += m * BM;
+    col += n * (BN / 2);
+    if (row >= a.e.rows || col >= a.e.cols) return;
+    if (a.partial) {
+      const uint64_t plane = (uint64_t)a.e.rows * a.e.cols;
+      float* p = a.partial + 2 * blockIdx.y * plane + (uint64_t)row * a.e.cols + col;
+      tam_store_some(p, a.e.cols - col, g);
+      tam_store_some(p + plane, a.e.cols - col, u);
+    } else {
+      gated_finish<T>(a.e, row, col, g, u);
+    }
+  });
+}
+
+// The parts' sums in their order, then the epilogue: a thread takes 8 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_gated_join(const float* partial, uint32_t parts, gated_epilogue e) {
+  const uint32_t per = (e.cols + 7) / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (uint64_t)per * e.rows) return;
+  const uint32_t row = (uint32_t)(i / per), col = (uint32_t)(i - (uint64_t)row * per) * 8;
+  const uint64_t at = (uint64_t)row * e.cols + col, plane = (uint64_t)e.rows * e.cols;
+  float g[8] = {}, u[8] = {};
+  for (uint32_t p = 0; p < parts; ++p) {
+    float a[8], b[8];
+    tam_load_some(partial + 2 * p * plane + at, e.cols - col, a);
+    tam_load_some(partial + (2 * p + 1) * plane + at, e.cols - col, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      g[j] += a[j];
+      u[j] += b[j];
+    }
+  }
+  gated_finish<T>(e, row, col, g, u);
+}
+
+struct gated_few_args {
+  const void* x;
+  const void* gate;
+  const void* up;
+  uint64_t ldx, ldw, k;  // elements
+  gated_epilogue e;
+};
+
+// One workgroup: 16 columns of h for up to 16 * MT rows of x, as tam_k_few; a wave's
+// turn of k is half as long, as it loads two weights.
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_gated_few(gated_few_args a) {
+  constexpr int N = 16 / (int)sizeof(T), U = 4;
+  constexpr uint64_t TURN = 4 * U * N;  // k of a wave's turn
+  __shared__ float sum[2][TAM_FEW_WAVES][MT * 16][20];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t i = lane & 15, q = lane >> 4, n = blockIdx.x * 16 + i;
+  // rows past the last one read the first one's elements; their sums go nowhere
+  const uint64_t at = n < a.e.cols ? (uint64_t)n * a.ldw : 0;
+  const T *wg = static_cast<const T*>(a.gate) + at, *wu = static_cast<const T*>(a.up) + at;
+  const T* x[MT];
+  tam_f4 ag[MT], au[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    x[m] = static_cast<const T*>(a.x) + (m * 16 + i < a.e.rows ? (uint64_t)(m * 16 + i) * a.ldx : 0);
+    ag[m] = au[m] = tam_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto turn = [&](uint64_t k0, auto guard) {
+    constexpr bool G = decltype(guard)::value;
+    tam_frag<T> fg[U], fu[U], fx[MT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) tam_few_load<T, G>(fg[u], wg, k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int u = 0; u < U; ++u) tam_few_load<T, G>(fu[u], wu, k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) tam_few_load<T, G>(fx[m][u], x[m], k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ag[m] = tam_mfma(fg[u], fx[m][u], ag[m]);
+        au[m] = tam_mfma(fu[u], fx[m][u], au[m]);
+      }
+  };
+  uint64_t k0 = wave * TURN;
+#pragma unroll 2
+  for (; k0 + TURN <= a.k; k0 += TAM_FEW_WAVES * TURN) turn(k0, std::false_type());
+  if (k0 < a.k) turn(k0, std::true_type());
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {  // row m * 16 + i, columns 4 q ..
+    *reinterpret_cast<tam_f4*>(&sum[0][wave][m * 16 + i][q * 4]) = ag[m];
+    *reinterpret_cast<tam_f4*>(&sum[1][wave][m * 16 + i][q * 4]) = au[m];
+  }
+  __syncthreads();
+  const uint32_t t = threadIdx.x, row = t / 2, col = (t % 2) * 8;
+  if (t < MT * 32 && row < a.e.rows && blockIdx.x * 16 + col < a.e.cols) {
+    float g[8] = {}, u[8] = {};
+    for (int s = 0; s < TAM_FEW_WAVES; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] += sum[0][s][row][col + j];
+        u[j] += sum[1][s][row][col + j];
+      }
+    gated_finish<T>(a.e, row, blockIdx.x * 16 + col, g, u);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+struct gated_slope_args {
+  const void* dh;
+  const void* g;
+  const void* u;
+  void* out;         // [rows][2][ld]: dg, du; up to 8 columns past the last one are zeros
+  uint64_t rows;
+  uint32_t cols, ld, act;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_gated_slope(gated_slope_args a) {
+  const uint32_t per = (a.cols + 7) / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= per * a.rows) return;
+  const uint64_t row = i / per;
+  const uint32_t col = (uint32_t)(i - row * per) * 8, count = a.cols - col;
+  const uint64_t at = row * a.cols + col;
+  float d[8], g[8], u[8];
+  tam_load_some(static_cast<const T*>(a.dh) + at, count, d);
+  tam_load_some(static_cast<const T*>(a.g) + at, count, g);
+  tam_load_some(static_cast<const T*>(a.u) + at, count, u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float s = tam_act_slope<sizeof(T) == 2>(g[j], a.act), v = tam_act<sizeof(T) == 2>(g[j], a.act);
+    g[j] = d[j] * u[j] * s;
+    u[j] = d[j] * v;
+  }
+  T* out = static_cast<T*>(a.out) + 2 * row * a.ld + col;
+  tam_store8(out, g);
+  tam_store8(out + a.ld, u);
+}
+
+// Where a product goes: its rows (or columns) from `half` on are those of the second array.
+struct gated_out {
+  void* out[2];         // [rows][cols] each, contiguous; null: not wanted
+  uint32_t rows, cols;  // of the product
+  uint32_t half, each;  // and of one array's rows (columns), behind which its padding lies
+  bool by_cols;
+};
+
+template <typename T>
+__device__ __forceinline__ void gated_put(const gated_out& e, uint32_t row, uint32_t col, const float (&v)[8]) {
+  uint32_t width = e.cols, second;
+  if (e.by_cols) {
+    second = col >= e.half;
+    col -= second ? e.half : 0;
+    width = e.each;
+    if (col >= width) return;
+  } else {
+    second = row >= e.half;
+    row -= second ? e.half : 0;
+    if (row >= e.each) return;
+  }
+  T* out = static_cast<T*>(e.out[second]);
+  if (out) tam_store_some(out + (uint64_t)row * width + col, width - col, v);
+}
+
+struct gated_product_args {
+  tam_operand P, Q;
+  tam_parts terms;
+  uint64_t k, k_part;
+  uint32_t tm, tn;
+  float* partial;       // [part][rows][cols] fp32, or null
+  gated_out e;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, int TERMS>
+__global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gated_product(gated_product_args a) {
+  typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, QK> Tile;
+  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  uint32_t m, n;
+  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
+  const uint64_t k0 = blockIdx.y * a.k_part;
+  const uint64_t k1 = k0 + a.k_part < a.k ? k0 + a.k_part : a.k;
+  Tile t;
+  t.zero();
+  t.template run<TERMS>(a.P, a.Q, n * BN, m * BM, k0, k1, smem, tam_soon{}, a.terms);
+  t.template each<TAM_AHEAD_PASS>(
+      smem, [](uint32_t, uint32_t) { return 0; },
+      [&](uint32_t row, uint32_t col, const float(&v)[8], int) {
+        row += m * BM;
+        col += n * BN;
+        if (row >= a.e.rows || col >= a.e.cols) return;
+        if (a.partial)
+          tam_store_some(a.partial + ((uint64_t)blockIdx.y * a.e.rows + row) * a.e.cols + col, a.e.cols - col, v);
+        else
+          gated_put<T>(a.e, row, col, v);
+      },
+      [](uint32_t, uint32_t, const float*, int) {});
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_gated_sum(const float* partial, uint32_t parts, gated_out e) {
+  const uint32_t per = (e.cols + 7) / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (uint64_t)per * e.rows) return;
+  const uint32_t row = (uint32_t)(i / per), col = (uint32_t)(i - (uint64_t)row * per) * 8;
+  const uint64_t at = (uint64_t)row * e.cols + col, step = (uint64_t)e.rows * e.cols;
+  float v[8] = {};
+  for (uint32_t p = 0; p < parts; ++p) {
+    float t[8];
+    tam_load_some(partial + p * step + at, e.cols - col, t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += t[j];
+  }
+  gated_put<T>(e, row, col, v);
+}
+
+__global__ __launch_bounds__(256) void tam_k_gated_zero(uint32_t* out, uint64_t words, uint64_t halves) {
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < words) out[i] = 0;
+  if (i == 0 && halves & 1) reinterpret_cast<uint16_t*>(out)[halves - 1] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+int check_gated(const TamGated* d, bool back) {
+  tam_op_begin();
+  if (!d) return tam_op_fail(TAM_E_INVALID, "null argument");
+  if (d->dtype > TAM_DTYPE_F16) return tam_op_fail(TAM_E_INVALID, "unknown dtype %u", d->dtype);
+  if (d->activation > TAM_ACT_MAX) return tam_op_fail(TAM_E_INVALID, "unknown activation %u", d->activation);
+  const uint64_t most = 1ull << 31;
+  if (d->rows >= most || d->inputs >= most || d->outputs >= most)
+    return tam_op_fail(TAM_E_UNSUPPORTED, "a size of 2^31 or more");
+  if (d->inputs && (d->ldx < d->inputs || d->ldw < (d->w_in_out ? d->outputs : d->inputs)))
+    return tam_op_fail(TAM_E_INVALID, "a row stride shorter than its row");
+  // a tile's offsets of up to 256 rows are 31-bit numbers of bytes, of dg and du side by side too
+  if ((d->ldx | d->ldw | d->inputs) >= 1ull << 21 || d->outputs >= (1ull << 20) - 64)
+    return tam_op_fail(TAM_E_UNSUPPORTED, "a row or row stride of 2^21 elements or more, or 2^20 - 64 outputs or more");
+  if (d->rows == 0 || d->outputs == 0) return TAM_OK;
+  if (d->inputs && (!d->x || !d->gate || !d->up)) return tam_op_fail(TAM_E_INVALID, "null x, gate or up");
+  if (!back && !d->h) return tam_op_fail(TAM_E_INVALID, "null h");
+  if (back && (!d->dh || !d->g || !d->u)) return tam_op_fail(TAM_E_INVALID, "null dh, g or u");
+  return TAM_OK;
+}
+
+matrix x_of(const TamGated* d) { return matrix_of(d->x, d->ldx, d->rows, d->inputs, kSize[d->dtype]); }
+matrix w_of(const TamGated* d, const void* w) {
+  return matrix_of(w, d->ldw, d->w_in_out ? d->inputs : d->outputs, d->w_in_out ? d->outputs : d->inputs, kSize[d->dtype]);
+}
+
+#define TAM_OF_TYPE(c, CALL)                               \
+  do {                                                     \
+    if ((c).dtype == TAM_DTYPE_F32) {                      \
+      CALL(float);                                         \
+    } else if ((c).dtype == TAM_DTYPE_BF16) {              \
+      CALL(tam_bf16);                                      \
+    } else {                                               \
+      CALL(tam_f16);                                       \
+    }                                                      \
+  } while (0)
+
+template <typename T>
+void launch_gated(int tile, bool pk, const gated_args& a, uint32_t parts, hipStream_t s) {
+  const dim3 grid(a.tm * a.tn, parts);
+#define TAM_TILE(TILE, WM, WN)                                                                                      \
+  do {                                                                                                              \
+    if (pk)                                                                                                         \
+      hipLaunchKernelGGL((tam_k_gated<T, TILE, TILE, WM, WN, true>), grid, dim3(64 * WM * WN), 0, s, a);            \
+    else                                                                                                            \
+      hipLaunchKernelGGL((tam_k_gated<T, TILE, TILE, WM, WN, false>), grid, dim3(64 * WM * WN), 0, s, a);           \
+  } while (0)
+  if constexpr (sizeof(T) == 2)
+    if (tile == 256) {
+      TAM_TILE(256, 2, 4);
+      return;
+    }
+  if (tile == 128)
+    TAM_TILE(128, 2, 2);
+  else
+    TAM_TILE(64, 2, 2);
+#undef TAM_TILE
+}
+
+template <typename T, int TILE, int WM, int WN>
+void launch_product_tile(bool pk, bool qk, const gated_product_args& a, uint32_t parts, hipStream_t s) {
+  const dim3 grid(a.tm * a.tn, parts), block(64 * WM * WN);
+  if (pk)  // dx of weights stored [inputs][outputs]
+    hipLaunchKernelGGL((tam_k_gated_product<T, TILE, TILE, WM, WN, true, true, TAM_TWO_PRODUCTS>), grid, block, 0, s, a);
+  else if (qk)  // dx
+    hipLaunchKernelGGL((tam_k_gated_product<T, TILE, TILE, WM, WN, false, true, TAM_TWO_PRODUCTS>), grid, block, 0, s, a);
+  else  // the weights' gradients
+    hipLaunchKernelGGL((tam_k_gated_product<T, TILE, TILE, WM, WN, false, false, TAM_ONE_TERM>), grid, block, 0, s, a);
+}
+
+template <typename T>
+void launch_product(int tile, bool pk, bool qk, const gated_product_args& a, uint32_t parts, hipStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (tile == 256) return launch_product_tile<T, 256, 2, 4>(pk, qk, a, parts, s);
+  tile == 128 ? launch_product_tile<T, 128, 2, 2>(pk, qk, a, parts, s) : launch_product_tile<T, 64, 2, 2>(pk, qk, a, parts, s);
+}
+
+int zero(call& c, void* p, uint64_t elements) {
+  if (c.dry || !p || !elements) return TAM_OK;
+  const uint64_t halves = elements * kSize[c.dtype] / 2;
+  hipLaunchKernelGGL(tam_k_gated_zero, dim3((uint32_t)tam_div_up(halves / 2 + 1, 256)), dim3(256), 0, c.stream, (uint32_t*)p,
+                     halves / 2, halves);
+  TAM_OP_LAUNCHED("an empty sum");
+  return TAM_OK;
+}
+
+int forward(const TamGated* d, call& c) {
+  if (d->rows == 0 || d->outputs == 0) return TAM_OK;
+  const gated_epilogue e = {d->h, d->g, d->u, (uint32_t)d->rows, (uint32_t)d->outputs, d->activation};
+  if (d->rows <= 32 && !d->w_in_out) {
+    if (c.dry) return TAM_OK;
+    const gated_few_args a = {d->x, d->gate, d->up, d->ldx, d->ldw, d->inputs, e};
+    const dim3 grid((uint32_t)tam_div_up(d->outputs, 16)), block(64 * TAM_FEW_WAVES);
+#define TAM_FEW(T)                                                              \
+  if (d->rows <= 16)                                                            \
+    hipLaunchKernelGGL((tam_k_gated_few<T, 1>), grid, block, 0, c.stream, a);   \
+  else                                                                          \
+    hipLaunchKernelGGL((tam_k_gated_few<T, 2>), grid, block, 0, c.stream, a)
+    TAM_OF_TYPE(c, TAM_FEW);
+    TAM_OP_LAUNCHED("the products of few rows");
+    return TAM_OK;
+  }
+  const uint32_t size = kSize[c.dtype];
+  const shape s = choose(d->rows, 2 * d->outputs, d->inputs, c.dtype);
+  if (c.tiles) {
+    c.tiles[0] = (uint32_t)s.tile;
+    c.tiles[1] = s.parts;
+  }
+  matrix x = x_of(d), gate = w_of(d, d->gate), up = w_of(d, d->up);
+  int rc = whole_rows(c, x);
+  if (rc == TAM_OK) rc = whole_rows(c, gate);
+  if (rc == TAM_OK) rc = whole_rows(c, up);
+  if (rc != TAM_OK) return rc;
+  gated_args a = {};
+  if (s.parts > 1) a.partial = (float*)c.ws.take(2ull * s.parts * e.rows * e.cols * 4);
+  if (c.dry) return TAM_OK;
+  a.P = {operand_of(gate, e.cols, size), operand_of(up, e.cols, size)};
+  a.Q = operand_of(x, e.rows, size);
+  a.k = d->inputs;
+  a.k_part = s.parts > 1 ? tam_up(tam_div_up(a.k, s.parts), 64) : a.k;
+  a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
+  a.tn = (uint32_t)tam_div_up(e.cols, s.tile / 2);
+  a.e = e;
+  if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+#define TAM_GATED(T) launch_gated<T>(s.tile, !d->w_in_out, a, s.parts, c.stream)
+  TAM_OF_TYPE(c, TAM_GATED);
+  TAM_OP_LAUNCHED("the gated products");
+  if (s.parts > 1) {
+    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
+#define TAM_JOIN(T) hipLaunchKernelGGL(tam_k_gated_join<T>, grid, block, 0, c.stream, a.partial, s.parts, e)
+    TAM_OF_TYPE(c, TAM_JOIN);
+    TAM_OP_LAUNCHED("the parts' sum");
+  }
+  return TAM_OK;
+}
+
+int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint64_t k, tam_parts terms, const gated_out& e) {
+  const uint32_t size = kSize[c.dtype];
+  const shape s = choose(e.rows, e.cols, k * terms.terms, c.dtype);
+  if (c.tiles) {
+    c.tiles[0] = (uint32_t)s.tile;
+    c.tiles[1] = s.parts;
+  }
+  gated_product_args a = {};
+  if (s.parts > 1) a.partial = (float*)c.ws.take((uint64_t)s.parts * e.rows * e.cols * 4);
+  if (c.dry) return TAM_OK;
+  a.P = operand_of(P, e.cols, size);
+  a.Q = operand_of(Q, e.rows, size);
+  a.terms = terms;
+  a.k = k;
+  a.k_part = s.parts > 1 ? tam_up(tam_div_up(k, s.parts), 64) : k;
+  a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
+  a.tn = (uint32_t)tam_div_up(e.cols, s.tile);
+  a.e = e;
+  if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+#define TAM_PRODUCT(T) launch_product<T>(s.tile, p_k, q_k, a, s.parts, c.stream)
+  TAM_OF_TYPE(c, TAM_PRODUCT);
+  TAM_OP_LAUNCHED("the product");
+  if (s.parts > 1) {
+    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
+#define TAM_SUM(T) hipLaunchKernelGGL(tam_k_gated_sum<T>, grid, block, 0, c.stream, a.partial, s.parts, e)
+    TAM_OF_TYPE(c, TAM_SUM);
+    TAM_OP_LAUNCHED("the parts' sum");
+  }
+  return TAM_OK;
+}
+
+int backward(const TamGated* d, call& c) {
+  const uint32_t size = kSize[c.dtype];
+  if (d->rows == 0 || d->outputs == 0 || d->inputs == 0) {  // empty sums
+    int rc = zero(c, d->dx, d->rows * d->inputs);
+    if (rc == TAM_OK) rc = zero(c, d->dgate, d->outputs * d->inputs);
+    return rc == TAM_OK ? zero(c, d->dup, d->outputs * d->inputs) : rc;
+  }
+  if (!d->dx && !d->dgate && !d->dup) return TAM_OK;
+  const uint32_t rows = (uint32_t)d->rows, inputs = (uint32_t)d->inputs, outputs = (uint32_t)d->outputs;
+  const uint32_t ld = aligned_ld(outputs, size);
+  const matrix both = {c.ws.take((uint64_t)rows * 2 * ld * size), 2ull * ld, rows, 2 * ld, true};
+  if (!c.dry) {
+    const gated_slope_args a = {d->dh, d->g, d->u, (void*)both.p, rows, outputs, ld, d->activation};
+    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(outputs, 8) * rows, 256)), block(256);
+#define TAM_SLOPE(T) hipLaunchKernelGGL(tam_k_gated_slope<T>, grid, block, 0, c.stream, a)
+    TAM_OF_TYPE(c, TAM_SLOPE);
+    TAM_OP_LAUNCHED("the activation's gradient");
+  }
+  if (d->dx) {
+    matrix gate = w_of(d, d->gate), up = w_of(d, d->up);
+    int rc = whole_rows(c, gate);
+    if (rc == TAM_OK) rc = whole_rows(c, up);
+    if (rc == TAM_OK && (gate.ld != up.ld)) rc = tam_op_fail(TAM_E_INVALID, "weights laid out in two ways");
+    if (rc != TAM_OK) return rc;
+    const tam_parts terms = {2, (int64_t)((intptr_t)up.p - (intptr_t)gate.p), (int64_t)ld * size};
+    const gated_out e = {{d->dx, nullptr}, rows, inputs, rows, rows, false};
+    rc = product(c, gate, d->w_in_out != 0, both, true, outputs, terms, e);
+    if (rc != TAM_OK) return rc;
+  }
+  if (d->dgate || d->dup) {
+    if (c.tiles) c.tiles += 2;
+    matrix x = x_of(d);
+    const int rc = whole_rows(c, x);
+    if (rc != TAM_OK) return rc;
+    const tam_parts one = {1, 0, 0};
+    gated_out e = {{d->dgate, d->dup}, 2 * ld, inputs, ld, outputs, false};
+    if (!d->w_in_out) return product(c, x, false, both, false, rows, one, e);
+    e.rows = inputs;
+    e.cols = 2 * ld;
+    e.by_cols = true;
+    return product(c, both, false, x, false, rows, one, e);
+  }
+  return TAM_OK;
+}
+
+int gated(const TamGated* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need,
+          uint32_t* tiles = nullptr) {
+  int rc = check_gated(d, back);
+  if (rc != TAM_OK) return rc;
+  call c = {d->dtype, (hipStream_t)stream, {nullptr, 0}, true, tiles};
+  rc = back ? backward(d, c) : forward(d, c);
+  if (rc != TAM_OK) return rc;
+  if (need) {
+    *need = c.ws.used;
+    return TAM_OK;
+  }
+  if (c.ws.used > ws_bytes || (c.ws.used && !workspace))
+    return tam_op_fail(TAM_E_WORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes,
+                       (unsigned long long)c.ws.used);
+  if ((uintptr_t)workspace & 255u) return tam_op_fail(TAM_E_INVALID, "workspace not on 256 bytes");
+  c = {d->dtype, (hipStream_t)stream, {(char*)workspace, 0}, false, nullptr};
+  return back ? backward(d, c) : forward(d, c);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tam_gated_workspace(const TamGated* d, int backward_pass, size_t* bytes) {
+  if (!bytes) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  uint64_t need = 0;
+  const int rc = gated(d, backward_pass != 0, nullptr, 0, nullptr, &need);
+  *bytes = (size_t)need;
+  return rc;
+}
+
+int tam_gated_tiles(const TamGated* d, int backward_pass, uint32_t* tiles) {
+  if (!tiles) {
+    tam_op_begin();
+    return tam_op_fail(TAM_E_INVALID, "null argument");
+  }
+  for (int i = 0; i < 4; ++i) tiles[i] = 0;
+  uint64_t need = 0;
+  return gated(d, backward_pass != 0, nullptr, 0, nullptr, &need, tiles);
+}
+
+int tam_gated(const TamGated* d, void* workspace, size_t ws_bytes, void* stream) {
+  return gated(d, false, workspace, ws_bytes, stream, nullptr);
+}
+
+int tam_gated_backward(const TamGated* d, void* workspace, size_t ws_bytes, void* stream) {
+  return gated(d, true, workspace, ws_bytes, stream, nullptr);
+}
+
+}  // extern "C"

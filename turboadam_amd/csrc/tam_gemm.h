@@ -122,7 +122,8 @@ struct tam_stage {
   uint32_t lane_k[LOADS];
 
   __device__ __forceinline__ static uint32_t swizzle(uint32_t k) {
-    if constexpr (sizeof(T) == 4) return 4u * (k >> 2 & 3u);
+    if constexpr (sizeof(T) == 4) return 4u * (k >> 2 & (CPR == 8 ? 1u : 3u));
+    if constexpr (CPR == 4) return 2u * (k >> 3 & 1u);
     if constexpr (CPR == 8) return 2u * (k >> 1 & 1u) | 4u * (k >> 3 & 1u);
     return 2u * (k & 3u) | 8u * (k >> 3 & 1u);
   }
@@ -171,6 +172,10 @@ struct tam_stage {
     tam_to_lds(at, voff, rsrc);
   }
 
+  __device__ __forceinline__ const char* at() const { return base; }
+  __device__ __forceinline__ void seek(const char* p) { base = p; }
+  __device__ __forceinline__ void next() { base += step; }
+
   // The fragment of rows row0 .. row0 + 15 and half `h` of the stage at `lds`.
   __device__ __forceinline__ static void read(tam_frag<T>& f, const tam_lds_char* lds, int row0, int h, int lane) {
     const uint32_t i = lane & 15u, q = (uint32_t)lane >> 4;
@@ -197,11 +202,51 @@ struct tam_stage {
   }
 };
 
+// Two operands that share a tile's columns: a wave's fragments are half of one's
+// columns and half of the same columns of the other, so that one lane holds both products.
+struct tam_operand_pair {
+  tam_operand a, b;
+};
+
+// Their stages: ROWS / 2 rows of each, one behind the other. TN: a wave's fragments.
+template <typename T, int ROWS, int NW, bool KC, int TN>
+struct tam_pair_stage {
+  typedef tam_stage<T, ROWS / 2, NW, KC, false> Half;
+  static constexpr int BK = Half::BK, BYTES = 2 * Half::BYTES, LOADS = 2 * Half::LOADS;
+  static_assert(TN % 2 == 0, "half of the fragments are of each operand");
+
+  Half a, b;
+
+  // first: the tile's first column of either operand
+  __device__ __forceinline__ void init(const tam_operand_pair& o, uint32_t first, uint64_t k0, int wave, int lane) {
+    a.init(o.a, first, k0, wave, lane);
+    b.init(o.b, first, k0, wave, lane);
+  }
+  __device__ __forceinline__ void load(int i, uint32_t lds, int wave, uint32_t left) const {
+    if (i < Half::LOADS)
+      a.load(i, lds, wave, left);
+    else
+      b.load(i - Half::LOADS, lds + Half::BYTES, wave, left);
+  }
+  __device__ __forceinline__ static void read(tam_frag<T>& f, const tam_lds_char* lds, int row0, int h, int lane) {
+    const int n = row0 / 16 % TN, row = (row0 / 16 / TN * (TN / 2) + n % (TN / 2)) * 16;
+    Half::read(f, n < TN / 2 ? lds : lds + Half::BYTES, row, h, lane);
+  }
+  __device__ __forceinline__ const char* at() const { return a.base; }
+  __device__ __forceinline__ void seek(const char*) {}
+  __device__ __forceinline__ void next() {
+    a.next();
+    b.next();
+  }
+};
+
 // A product of operands in two parts, high + low: the sum of high * high, high *
 // low and low * high runs as one sum over three times k.  p, q: bytes from an
 // operand's high part to its low part (the same layout).
+// Or the sum of two products, one behind the other: of operands p and q bytes apart.
+enum tam_terms { TAM_ONE_TERM, TAM_HIGH_LOW, TAM_TWO_PRODUCTS };
 struct tam_parts {
-  uint32_t terms;  // 1 (high * high alone) or 3
+  uint32_t terms;  // 1 (high * high alone) or 3; 2 products
   int64_t p, q;
 };
 
@@ -231,13 +276,14 @@ constexpr int tam_stages() {
 // WN waves.
 // EXACT: m-major operands whose rows may end inside 16 bytes: the last row's last
 // load stops at the operand's `end` (a k-contiguous one never passes it).
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool EXACT = false>
+// PAIR: the columns' operand is two (tam_operand_pair), BN / 2 columns of each.
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool EXACT = false, bool PAIR = false>
 struct tam_tile {
   static constexpr int NW = WM * WN;
   static constexpr int THREADS = 64 * NW;
   static constexpr int TM = BM / WM / 16;  // a wave's fragments of Q
   static constexpr int TN = BN / WN / 16;  // and of P
-  typedef tam_stage<T, BN, NW, PK, EXACT && !PK> SP;
+  typedef std::conditional_t<PAIR, tam_pair_stage<T, BN, NW, PK, TN>, tam_stage<T, BN, NW, PK, EXACT && !PK>> SP;
   typedef tam_stage<T, BM, NW, QK, EXACT && !QK> SQ;
   static constexpr int BK = SP::BK;
   static constexpr int STAGE = SP::BYTES + SQ::BYTES;
@@ -270,8 +316,8 @@ struct tam_tile {
   }
 
   // Adds the products of k0 <= k < k1 to the tile at rows r0, columns c0.
-  template <bool PARTS = false>
-  __device__ __forceinline__ void run(const tam_operand& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
+  template <int TERMS = TAM_ONE_TERM, typename Columns = tam_operand>
+  __device__ __forceinline__ void run(const Columns& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
                                       uint64_t k1, char* smem, const tam_soon& soon, tam_parts parts = {1, 0, 0}) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -281,21 +327,21 @@ struct tam_tile {
     SQ sq;
     sp.init(P, c0, k0, wave, lane);
     sq.init(Q, r0, k0, wave, lane);
-    const char *const p0 = sp.base, *const q0 = sq.base;
+    const char *const p0 = sp.at(), *const q0 = sq.at();
     const int64_t length = k1 > k0 ? (int64_t)(k1 - k0) : 0;
     int64_t ahead = length;  // k from the next stage to load on
     uint32_t left = 0, steps = (uint32_t)((length + BK - 1) / BK), term = 0;
-    if constexpr (PARTS) steps *= parts.terms;
+    if constexpr (TERMS != TAM_ONE_TERM) steps *= parts.terms;
     // load i of the next stage into buffer `buf`: the first one looks at what is left,
     // the last one moves on
     auto load = [&](int i, uint32_t buf) {
       if (i == 0) {
-        if constexpr (PARTS)
+        if constexpr (TERMS != TAM_ONE_TERM)
           if (ahead <= 0 && term + 1 < parts.terms) {
             ++term;
             ahead = length;
-            sp.base = p0 + (term == 2 ? parts.p : 0);
-            sq.base = q0 + (term == 1 ? parts.q : 0);
+            sp.seek(p0 + (TERMS == TAM_TWO_PRODUCTS || term == 2 ? parts.p : 0));
+            sq.seek(q0 + (term == 1 ? parts.q : 0));
           }
         left = ahead <= 0 ? 0u : (ahead > BK ? (uint32_t)BK : (uint32_t)ahead);
         ahead -= BK;
@@ -305,8 +351,8 @@ struct tam_tile {
       else
         sq.load(i - SP::LOADS, lds0 + buf * STAGE + SP::BYTES, wave, left);
       if (i == LOADS - 1) {
-        sp.base += sp.step;
-        sq.base += sq.step;
+        sp.next();
+        sq.next();
       }
     };
     auto fetch = [&]() {
@@ -388,6 +434,44 @@ struct tam_tile {
         for (int m = 0; m < TM; ++m)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[n][m][j] = __builtin_fmaf(p[n][j], q[m], acc[n][m][j]);
+    }
+  }
+
+  // PAIR: hands the tile to finish(row, col, a, b): 8 consecutive columns of one row of
+  // either product, in fp32; columns are 0 .. BN / 2 - 1.
+  template <typename F>
+  __device__ __forceinline__ void pairs(char* smem, F finish) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    float* turn = reinterpret_cast<float*>(smem) + wave * ROUND * PITCH;
+    constexpr int HALF = COLS / 2, LPR = HALF / 8, RPP = 64 / LPR, PASSES = ROUND / RPP;
+    const int r0 = lane / LPR, c0 = (lane % LPR) * 8;
+#pragma unroll
+    for (int m = 0; m < TM; m += 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+          *reinterpret_cast<tam_f4*>(turn + (h * 16 + (lane & 15)) * PITCH + n * 16 + (lane >> 4) * 4) = acc[n][m + h];
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const float* from = turn + (p * RPP + r0) * PITCH + c0;
+        float a[8], b[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const tam_f4 x = *reinterpret_cast<const tam_f4*>(from + j), y = *reinterpret_cast<const tam_f4*>(from + HALF + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            a[j + i] = x[i];
+            b[j + i] = y[i];
+          }
+        }
+        finish((uint32_t)((wm * TM + m) * 16 + p * RPP + r0), (uint32_t)(wn * HALF + c0), a, b);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
     }
   }
 

@@ -12,70 +12,10 @@
 //                cut among workgroups (few tiles);
 //   tam_k_few    the forward product of up to 32 rows: every wave reads its part
 //                of 16 weight rows once, straight to the matrix cores;
-//   tam_k_slope  dz and its column sums;  tam_k_column_sum: the sums' end;
-//   tam_k_align  rows copied to 16-byte-aligned rows (zeros behind them), for
-//                16-bit operands whose rows do not begin and end on 4 bytes.
-#include "tam_gemm.h"
-
-#include <math.h>
-
-#include <type_traits>
-
-#define TAM_ACT_MAX TAM_ACT_SILU
-
-// ---------------------------------------------------------------------------
-// activations (fp32)
-// ---------------------------------------------------------------------------
-// gelu_tanh: 0.5 z (1 + tanh u) = z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3)
-#define TAM_GELU_2U 1.5957691216057308f
-#define TAM_GELU_C 0.044715f
-
-// FAST (16-bit results): the hardware's 2^x and reciprocal, 1 ulp each, 4 instructions
-// for about 30: 2^-20 of the result at |x| < 16. At 8192 x 768 x 3072 the epilogue's
-// arithmetic took longer than its stores.
-template <bool FAST>
-__device__ __forceinline__ float tam_sigmoid(float x) {
-  if constexpr (FAST)
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
-  else
-    return 1.0f / (1.0f + expf(-x));
-}
-
-template <bool FAST>
-__device__ __forceinline__ float tam_act(float z, uint32_t act) {
-  switch (act) {
-    case TAM_ACT_RELU: return z < 0.0f ? 0.0f : z;  // a NaN stays
-    case TAM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case TAM_ACT_GELU_TANH: return z * tam_sigmoid<FAST>(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
-    case TAM_ACT_SILU: return z * tam_sigmoid<FAST>(z);
-    default: return z;
-  }
-}
-
-// Past +-128 the smooth activations' slopes are 0 and 1 in fp32, and so they are at
-// the infinities: a z that the layer's type cannot hold (below -65504 in fp16, where y is
-// a finite 0) or whose cube passes fp32's range would give 0 * inf as a factor, so `near`
-// is the factor. (One instruction, which loses a NaN: that comes from s or e.)
-template <bool FAST>
-__device__ __forceinline__ float tam_act_slope(float z, uint32_t act) {
-  const float near = __builtin_amdgcn_fmed3f(z, -128.0f, 128.0f);
-  switch (act) {
-    case TAM_ACT_RELU: return z > 0.0f ? 1.0f : (z == z ? 0.0f : z);
-    case TAM_ACT_GELU: {
-      const float e = FAST ? __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z) : expf(-0.5f * z * z);
-      return __builtin_fmaf(near * 0.39894228040143268f, e, 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
-    }
-    case TAM_ACT_GELU_TANH: {
-      const float s = tam_sigmoid<FAST>(TAM_GELU_2U * __builtin_fmaf(TAM_GELU_C * z * z, z, z));
-      return __builtin_fmaf(near * s * (1.0f - s), TAM_GELU_2U * __builtin_fmaf(3.0f * TAM_GELU_C * near, near, 1.0f), s);
-    }
-    case TAM_ACT_SILU: {
-      const float s = tam_sigmoid<FAST>(z);
-      return s * __builtin_fmaf(near, 1.0f - s, 1.0f);
-    }
-    default: return 1.0f;
-  }
-}
+//   tam_k_slope  dz and its column sums;  tam_k_column_sum: the sums' end.
+#include "tam_act.h"
+#include "tam_few.h"
+#include "tam_products.h"
 
 // ---------------------------------------------------------------------------
 // epilogue
@@ -242,32 +182,12 @@ __global__ __launch_bounds__(256) void tam_k_split(const float* partial, uint32_
 // row i loads the chunks at k0 + 8 * (4 u + lane / 16), u = 0..3: a wave's four
 // loads of a row are 256 consecutive bytes. Bound by reading w once; x stays in
 // the caches. The waves' sums meet in LDS in wave order.
-// Chunk k .. of a row; GUARD: elements from K on are zeros and not read.
-template <typename T, bool GUARD>
-__device__ __forceinline__ void tam_few_load(tam_frag<T>& f, const T* row, uint64_t k, uint64_t K) {
-  constexpr int N = 16 / (int)sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(N)));
-  struct __attribute__((packed, aligned(sizeof(T)))) any {
-    vec v;
-  };
-  if (!GUARD || k + N <= K) {
-    f.v = __builtin_bit_cast(decltype(f.v), reinterpret_cast<const any*>(row + k)->v);
-  } else {
-    vec v;
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = k + j < K ? row[k + j] : (T)0.0f;
-    f.v = __builtin_bit_cast(decltype(f.v), v);
-  }
-}
-
 struct tam_few_args {
   const void* x;
   const void* w;
   uint64_t ldx, ldw, k;  // elements
   tam_epilogue e;
 };
-
-#define TAM_FEW_WAVES 8
 
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_few(tam_few_args a) {
@@ -408,67 +328,9 @@ __global__ __launch_bounds__(256) void tam_k_zero(T* out, uint32_t n) {
 }
 
 // ---------------------------------------------------------------------------
-// alignment
-// ---------------------------------------------------------------------------
-// dst[r][0 .. ld_dst) = src[r][0 .. cols) of 16-bit elements, zeros behind: a thread
-// moves 8 elements and none of their bits.
-__global__ __launch_bounds__(256) void tam_k_align(const tam_f16* src, uint64_t ld_src, uint64_t rows, uint32_t cols,
-                                                   tam_f16* dst, uint32_t ld_dst) {
-  const uint32_t per = ld_dst / 8;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (uint64_t)per * rows) return;
-  const uint64_t r = i / per;
-  const uint32_t c = (uint32_t)(i - r * per) * 8;
-  *reinterpret_cast<tam_oct<tam_f16>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
-}
-
-// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 namespace {
-
-constexpr uint32_t kSize[3] = {4, 2, 2};
-
-// One matrix as the products read it: rows of `cols` contiguous elements; whole: they
-// are 16 bytes, or zeros follow up to that.
-struct matrix {
-  const void* p;
-  uint64_t ld, rows;
-  uint32_t cols;
-  bool whole;
-};
-
-// Whether the products' loads can take m as it lies: rows that begin and end on 4 bytes.
-bool in_words(const matrix& m, uint32_t size) {
-  return (uint64_t)m.cols * size % 4 == 0 && m.ld * size % 4 == 0 && (uintptr_t)m.p % 4 == 0;
-}
-
-matrix matrix_of(const void* p, uint64_t ld, uint64_t rows, uint64_t cols, uint32_t size) {
-  return {p, ld, rows, (uint32_t)cols, cols * size % 16 == 0};
-}
-
-// Rows of a copy: whole 128-byte lines (a tile's row then touches no line more than it fills).
-uint32_t aligned_ld(uint32_t cols, uint32_t size) { return (uint32_t)tam_up(cols, 128 / size); }
-
-// The workspace is laid out by walking the call twice: once without memory, to
-// learn its size, and once with it.
-struct arena {
-  char* base;
-  uint64_t used;
-  void* take(uint64_t bytes) {
-    void* p = base ? base + used : nullptr;
-    used += tam_up(bytes, 256);
-    return p;
-  }
-};
-
-struct call {
-  uint32_t dtype;
-  hipStream_t stream;
-  arena ws;
-  bool dry;  // lay out the workspace only
-  uint32_t* tiles;  // where a product's tile and parts are told (tam_linear_tiles), or null
-};
 
 int check_linear(const TamLinear* d, bool backward) {
   tam_op_begin();
@@ -492,54 +354,6 @@ int check_linear(const TamLinear* d, bool backward) {
 }
 
 // ---- products ----
-
-struct shape {
-  int tile;        // rows and columns of a tile
-  uint32_t parts;  // the sum is cut into
-};
-
-// Which tile, and into how many parts the sum is cut: the least of the measured
-// times (tam_tiles_us). Parts add their sums' way to memory and back (about 4 TB/s)
-// and a launch.
-shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
-  const double cus = tam_op_cus();
-  const bool f32 = dtype == TAM_DTYPE_F32;
-  const tam_tile_rate* rate = f32 ? tam_rates_32 : tam_rates_16;
-  shape best = {64, 1};
-  double least = 1e30;
-  for (int i = 0; i < (f32 ? 2 : 3); ++i) {
-    const double tiles = (double)tam_div_up(rows, rate[i].tile) * (double)tam_div_up(cols, rate[i].tile);
-    for (uint32_t parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (parts > 1 && k / parts < 128) break;
-      double us = tam_tiles_us(rate[i], tiles * parts, (double)k / parts, cus);
-      if (parts > 1) us += 3.0 + (double)rows * cols * 8.0 * parts / 4e6;
-      if (us < least) {
-        least = us;
-        best = {rate[i].tile, parts};
-      }
-    }
-  }
-  return best;
-}
-
-// m, or a copy of it whose rows are whole lines. Rows that may end inside 16 bytes
-// have kernels of their own (REST), as the bound on their loads and the rest of their
-// sums would cost the others 1% (x [8192, 768], w [768, 3072], bf16, both ways: 206 -> 208
-// us), and a copy of [2018, 13611] fp32 would be 25 of 110 us. The 256 tile is for
-// products so large that the copy is less than 3% of them.
-int readable(call& c, matrix& m, const shape& s) {
-  const uint32_t size = kSize[c.dtype];
-  if ((in_words(m, size) && (m.whole || s.tile != 256)) || !m.cols || !m.rows) return TAM_OK;  // no elements: nothing is read
-  const uint32_t ld = aligned_ld(m.cols, size);
-  void* p = c.ws.take(m.rows * ld * size);
-  if (!c.dry) {
-    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
-    hipLaunchKernelGGL(tam_k_align, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld, m.rows, m.cols, (tam_f16*)p, ld);
-    TAM_OP_LAUNCHED("the aligned copy");
-  }
-  m = {p, ld, m.rows, m.cols, true};
-  return TAM_OK;
-}
 
 template <typename T, int TILE, int WM, int WN, bool REST>
 void launch_tile(bool pk, bool qk, const tam_gemm_args& a, uint32_t parts, hipStream_t s) {
@@ -575,14 +389,9 @@ int product(call& c, matrix P, bool p_k, matrix Q, bool q_k, uint64_t k, const t
   float* partial = s.parts > 1 ? (float*)c.ws.take((uint64_t)s.parts * e.rows * e.cols * 4) : nullptr;
   if (c.dry) return TAM_OK;
   const uint32_t size = kSize[c.dtype];
-  auto operand = [&](const matrix& m, uint32_t count) {
-    const char* base = (const char*)m.p;
-    const uint64_t bytes = m.rows ? (m.rows - 1) * m.ld * size + tam_up((uint64_t)m.cols * size, m.whole ? 16 : 1) : 0;
-    return tam_operand{base, m.ld * size, count, base + bytes};
-  };
   tam_gemm_args a = {};
-  a.P = operand(P, e.cols);
-  a.Q = operand(Q, e.rows);
+  a.P = operand_of(P, e.cols, size);
+  a.Q = operand_of(Q, e.rows, size);
   a.k_all = k;
   a.k = (!p_k || P.whole) && (!q_k || Q.whole) ? k : k - k % (16 / size);
   a.k_part = s.parts > 1 ? tam_up(tam_div_up(a.k, s.parts), 64) : a.k;

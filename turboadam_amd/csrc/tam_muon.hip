@@ -447,14 +447,14 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_squ
     Columns t;
     t.zero();
     const tam_operand x = operand((turn ? d.x[1] : d.x[0]), d.ldx, d.wx);
-    t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
+    t.template run<TAM_HIGH_LOW>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, d.x_low * 2, d.x_low * 2});
     finish(t);
   } else {
     Rows t;
     t.zero();
     const tam_operand x = FIRST ? operand((turn ? d.x[1] : d.x[0]), d.ldx, d.rows) : operand(d.q, d.lds, d.s);
     const int64_t low = (FIRST ? d.x_low : d.s_low) * 2;
-    t.template run<true>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, low, low});
+    t.template run<TAM_HIGH_LOW>(x, x, c0, r0, k0, k1, smem, soon, {d.split ? 3u : 1u, low, low});
     finish(t);
   }
 }
@@ -610,12 +610,12 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_app
   if (d.tall) {
     Tall t;
     t.zero();
-    t.template run<true>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.ws, smem, soon, {terms, d.s_low * 2, d.x_low * 2});
+    t.template run<TAM_HIGH_LOW>(p, operand(x, d.ldx, d.rows), c0, r0, 0, d.ws, smem, soon, {terms, d.s_low * 2, d.x_low * 2});
     finish(t);
   } else {
     Wide t;
     t.zero();
-    t.template run<true>(operand(x, d.ldx, d.wx), p, c0, r0, 0, d.rows, smem, soon, {terms, d.x_low * 2, d.s_low * 2});
+    t.template run<TAM_HIGH_LOW>(operand(x, d.ldx, d.wx), p, c0, r0, 0, d.rows, smem, soon, {terms, d.x_low * 2, d.s_low * 2});
     finish(t);
   }
 }

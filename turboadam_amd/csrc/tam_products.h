@@ -1,0 +1,144 @@
+// tam_products.h -- host side of the layers' matrix products: operands as they lie in
+// memory, aligned copies of those that the tiles cannot read, workspaces, and the choice of
+// tile and parts.
+#ifndef TAM_PRODUCTS_H
+#define TAM_PRODUCTS_H
+
+#include "tam_gemm.h"
+
+// ---------------------------------------------------------------------------
+// alignment
+// ---------------------------------------------------------------------------
+// dst[r][0 .. ld_dst) = src[r][0 .. cols) of 16-bit elements, zeros behind: a thread
+// moves 8 elements and none of their bits.
+static __global__ __launch_bounds__(256) void tam_k_align(const tam_f16* src, uint64_t ld_src, uint64_t rows, uint32_t cols,
+                                                   tam_f16* dst, uint32_t ld_dst) {
+  const uint32_t per = ld_dst / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (uint64_t)per * rows) return;
+  const uint64_t r = i / per;
+  const uint32_t c = (uint32_t)(i - r * per) * 8;
+  *reinterpret_cast<tam_oct<tam_f16>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
+}
+
+namespace {
+
+constexpr uint32_t kSize[3] = {4, 2, 2};
+
+// One matrix as the products read it: rows of `cols` contiguous elements; whole: they
+// are 16 bytes, or zeros follow up to that.
+struct matrix {
+  const void* p;
+  uint64_t ld, rows;
+  uint32_t cols;
+  bool whole;
+};
+
+// Whether the products' loads can take m as it lies: rows that begin and end on 4 bytes.
+inline bool in_words(const matrix& m, uint32_t size) {
+  return (uint64_t)m.cols * size % 4 == 0 && m.ld * size % 4 == 0 && (uintptr_t)m.p % 4 == 0;
+}
+
+inline matrix matrix_of(const void* p, uint64_t ld, uint64_t rows, uint64_t cols, uint32_t size) {
+  return {p, ld, rows, (uint32_t)cols, cols * size % 16 == 0};
+}
+
+// Rows of a copy: whole 128-byte lines (a tile's row then touches no line more than it fills).
+inline uint32_t aligned_ld(uint32_t cols, uint32_t size) { return (uint32_t)tam_up(cols, 128 / size); }
+
+// The workspace is laid out by walking the call twice: once without memory, to
+// learn its size, and once with it.
+struct arena {
+  char* base;
+  uint64_t used;
+  void* take(uint64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += tam_up(bytes, 256);
+    return p;
+  }
+};
+
+struct call {
+  uint32_t dtype;
+  hipStream_t stream;
+  arena ws;
+  bool dry;  // lay out the workspace only
+  uint32_t* tiles;  // where a product's tile and parts are told (tam_linear_tiles), or null
+};
+
+// ---- products ----
+
+struct shape {
+  int tile;        // rows and columns of a tile
+  uint32_t parts;  // the sum is cut into
+};
+
+// Which tile, and into how many parts the sum is cut: the least of the measured
+// times (tam_tiles_us). Parts add their sums' way to memory and back (about 4 TB/s)
+// and a launch.
+inline shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
+  const double cus = tam_op_cus();
+  const bool f32 = dtype == TAM_DTYPE_F32;
+  const tam_tile_rate* rate = f32 ? tam_rates_32 : tam_rates_16;
+  shape best = {64, 1};
+  double least = 1e30;
+  for (int i = 0; i < (f32 ? 2 : 3); ++i) {
+    const double tiles = (double)tam_div_up(rows, rate[i].tile) * (double)tam_div_up(cols, rate[i].tile);
+    for (uint32_t parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (parts > 1 && k / parts < 128) break;
+      double us = tam_tiles_us(rate[i], tiles * parts, (double)k / parts, cus);
+      if (parts > 1) us += 3.0 + (double)rows * cols * 8.0 * parts / 4e6;
+      if (us < least) {
+        least = us;
+        best = {rate[i].tile, parts};
+      }
+    }
+  }
+  return best;
+}
+
+// m, or a copy of it whose rows are whole lines. Rows that may end inside 16 bytes
+// have kernels of their own (REST), as the bound on their loads and the rest of their
+// sums would cost the others 1% (x [8192, 768], w [768, 3072], bf16, both ways: 206 -> 208
+// us), and a copy of [2018, 13611] fp32 would be 25 of 110 us. The 256 tile is for
+// products so large that the copy is less than 3% of them.
+inline int readable(call& c, matrix& m, const shape& s) {
+  const uint32_t size = kSize[c.dtype];
+  if ((in_words(m, size) && (m.whole || s.tile != 256)) || !m.cols || !m.rows) return TAM_OK;  // no elements: nothing is read
+  const uint32_t ld = aligned_ld(m.cols, size);
+  void* p = c.ws.take(m.rows * ld * size);
+  if (!c.dry) {
+    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
+    hipLaunchKernelGGL(tam_k_align, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld, m.rows, m.cols, (tam_f16*)p, ld);
+    TAM_OP_LAUNCHED("the aligned copy");
+  }
+  m = {p, ld, m.rows, m.cols, true};
+  return TAM_OK;
+}
+
+// m, or a copy of it: rows of whole 16 bytes that begin on 4, for kernels without a REST form.
+inline int whole_rows(call& c, matrix& m) {
+  const uint32_t size = kSize[c.dtype], halves = size / 2;
+  if ((in_words(m, size) && m.whole) || !m.cols || !m.rows) return TAM_OK;
+  const uint32_t ld = aligned_ld(m.cols, size);
+  void* p = c.ws.take(m.rows * ld * size);
+  if (!c.dry) {
+    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld * halves / 8), 256)), block(256);
+    hipLaunchKernelGGL(tam_k_align, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld * halves, m.rows, m.cols * halves,
+                       (tam_f16*)p, ld * halves);
+    TAM_OP_LAUNCHED("the aligned copy");
+  }
+  m = {p, ld, m.rows, m.cols, true};
+  return TAM_OK;
+}
+
+// m as an operand of a product: `count` rows or columns of it are the operand's.
+inline tam_operand operand_of(const matrix& m, uint32_t count, uint32_t size) {
+  const char* base = (const char*)m.p;
+  const uint64_t bytes = m.rows ? (m.rows - 1) * m.ld * size + tam_up((uint64_t)m.cols * size, m.whole ? 16 : 1) : 0;
+  return {base, m.ld * size, count, base + bytes};
+}
+
+}  // namespace
+
+#endif  // TAM_PRODUCTS_H
