@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "tam_ops.h"
 
 #define TAM_ACT_MAX TAM_ACT_SILU
@@ -59,6 +61,22 @@ __device__ __forceinline__ float tam_act_slope(float z, uint32_t act) {
       return s * __builtin_fmaf(near, 1.0f - s, 1.0f);
     }
     default: return 1.0f;
+  }
+}
+
+// Eight of them, with one look at which it is.
+template <bool FAST>
+__device__ __forceinline__ void tam_act8(const float (&z)[8], uint32_t act, float (&y)[8]) {
+  auto each = [&](auto which) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = tam_act<FAST>(z[j], decltype(which)::value);
+  };
+  switch (act) {
+    case TAM_ACT_RELU: return each(std::integral_constant<uint32_t, TAM_ACT_RELU>());
+    case TAM_ACT_GELU: return each(std::integral_constant<uint32_t, TAM_ACT_GELU>());
+    case TAM_ACT_GELU_TANH: return each(std::integral_constant<uint32_t, TAM_ACT_GELU_TANH>());
+    case TAM_ACT_SILU: return each(std::integral_constant<uint32_t, TAM_ACT_SILU>());
+    default: return each(std::integral_constant<uint32_t, TAM_ACT_NONE>());
   }
 }
 

@@ -43,8 +43,9 @@ __device__ __forceinline__ void gated_finish(const gated_epilogue& e, uint32_t r
   if (e.g) tam_store_some(static_cast<T*>(e.g) + at, count, a);
   if (e.u) tam_store_some(static_cast<T*>(e.u) + at, count, b);
   float v[8];
+  tam_act8<sizeof(T) == 2>(a, e.act, v);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = tam_act<sizeof(T) == 2>(a[j], e.act) * b[j];
+  for (int j = 0; j < 8; ++j) v[j] *= b[j];
   tam_store_some(static_cast<T*>(e.h) + at, count, v);
 }
 
@@ -61,16 +62,12 @@ template <typename T, int BM, int BN, int WM, int WN, bool PK>
 __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gated(gated_args a) {
   typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, true, false, true> Tile;
   __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  const uint32_t tiles = a.tm * a.tn;
   uint32_t m, n;
-  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
+  tam_tile_at(tam_xcd_order(blockIdx.x, tiles), a.tm, a.tn, m, n);
   const uint64_t k0 = blockIdx.y * a.k_part;
   const uint64_t k1 = k0 + a.k_part < a.k ? k0 + a.k_part : a.k;
-  Tile t;
-  t.zero();
-  t.run(a.P, a.Q, n * (BN / 2), m * BM, k0, k1, smem, tam_soon{});
-  t.pairs(smem, [&](uint32_t row, uint32_t col, const float(&g)[8], const float(&u)[8]) {
-    row += m * BM;
-    col += n * (BN / 2);
+  auto put = [&](uint32_t row, uint32_t col, const float(&g)[8], const float(&u)[8]) {
     if (row >= a.e.rows || col >= a.e.cols) return;
     if (a.partial) {
       const uint64_t plane = (uint64_t)a.e.rows * a.e.cols;
@@ -80,7 +77,45 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gated(ga
     } else {
       gated_finish<T>(a.e, row, col, g, u);
     }
-  });
+  };
+  Tile t;
+  if constexpr (Tile::RING) {
+    // a workgroup to a compute unit, each of which takes every gridDim.x-th tile and begins
+    // the next one before it stores the last
+    typename Tile::ring r;
+    Tile::begin(r, a.P, a.Q, n * (BN / 2), m * BM, k0, k1, smem);
+    constexpr uint32_t HALF_COLS = Tile::COLS / 2, LPR = HALF_COLS / 8, RPP = 64 / LPR;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+    for (uint32_t tile = blockIdx.x;;) {
+      t.zero();
+      t.sum(r, smem);
+      const uint32_t row0 = m * BM + wm * Tile::TM * 16 + lane / LPR, col = n * (BN / 2) + wn * HALF_COLS + lane % LPR * 8;
+      tile += gridDim.x;
+      if (tile < tiles) {
+        tam_tile_at(tam_xcd_order(tile, tiles), a.tm, a.tn, m, n);
+        Tile::begin(r, a.P, a.Q, n * (BN / 2), m * BM, k0, k1, smem);
+      }
+#pragma unroll
+      for (int f = 0; f < Tile::TM; ++f) {
+        t.turn_in(smem, f);
+#pragma unroll
+        for (uint32_t p = 0; p < 16; p += RPP) {
+          float g[8], u[8];
+          t.turn_out(smem, p + lane / LPR, lane % LPR * 8, g);
+          t.turn_out(smem, p + lane / LPR, HALF_COLS + lane % LPR * 8, u);
+          put(row0 + f * 16 + p, col, g, u);
+        }
+        Tile::turned();
+      }
+      if (tile >= tiles) return;
+    }
+  } else {
+    t.zero();
+    t.run(a.P, a.Q, n * (BN / 2), m * BM, k0, k1, smem, tam_soon{});
+    t.pairs(smem, [&](uint32_t row, uint32_t col, const float(&g)[8], const float(&u)[8]) {
+      put(row + m * BM, col + n * (BN / 2), g, u);
+    });
+  }
 }
 
 // The parts' sums in their order, then the epilogue: a thread takes 8 columns.
@@ -332,7 +367,8 @@ matrix w_of(const TamGated* d, const void* w) {
 
 template <typename T>
 void launch_gated(int tile, bool pk, const gated_args& a, uint32_t parts, hipStream_t s) {
-  const dim3 grid(a.tm * a.tn, parts);
+  const uint32_t tiles = a.tm * a.tn, cus = tam_op_cus();
+  const dim3 grid(tile == 256 && tiles > cus ? cus : tiles, parts);
 #define TAM_TILE(TILE, WM, WN)                                                                                      \
   do {                                                                                                              \
     if (pk)                                                                                                         \

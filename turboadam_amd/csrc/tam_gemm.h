@@ -86,6 +86,25 @@ __device__ __forceinline__ tam_f4 tam_mfma(const tam_frag<float>& a, const tam_f
   return c;
 }
 
+// The same where a sum stays in its registers, and with a load to LDS issued behind it: m0,
+// which takes a wait state before it is used, has it in the matrix instruction. The wait states
+// before the sums are read are the caller's (tam_tile::settle).
+#define TAM_MFMA_IN(TYPE, NAME)                                                                                      \
+  __device__ __forceinline__ void tam_mfma_in(const tam_frag<TYPE>& a, const tam_frag<TYPE>& b, tam_f4& c) {         \
+    asm volatile("v_mfma_f32_16x16x32_" NAME " %0, %1, %2, %0" : "+v"(c) : "v"(a.v), "v"(b.v));                      \
+  }                                                                                                                  \
+  __device__ __forceinline__ void tam_mfma_load(const tam_frag<TYPE>& a, const tam_frag<TYPE>& b, tam_f4& c,         \
+                                                uint32_t lds, int place, uint32_t voff, tam_i4 rsrc) {               \
+    asm volatile("s_add_i32 m0, %1, %2\n\tv_mfma_f32_16x16x32_" NAME " %0, %5, %6, %0\n\t"                           \
+                 "buffer_load_dwordx4 %3, %4, 0 offen lds"                                                           \
+                 : "+v"(c)                                                                                           \
+                 : "s"(lds), "i"(place), "v"(voff), "s"(rsrc), "v"(a.v), "v"(b.v)                                    \
+                 : "m0", "scc");                                                                                     \
+  }
+TAM_MFMA_IN(tam_bf16, "bf16")
+TAM_MFMA_IN(tam_f16, "f16")
+#undef TAM_MFMA_IN
+
 // 16 bytes a lane from rsrc's base + voff to LDS at `lds` + 16 * lane.
 __device__ __forceinline__ void tam_to_lds(uint32_t lds, uint32_t voff, tam_i4 rsrc) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -172,6 +191,16 @@ struct tam_stage {
     tam_to_lds(at, voff, rsrc);
   }
 
+  // The parts of load(), for loads that are issued together with a matrix instruction: load i goes to
+  // wave * WAVE_BYTES + place(i) of the stage, from offset(i, left).
+  static constexpr int WAVE_BYTES = LOADS * 1024;
+  __device__ static constexpr int place(int i) { return i * 1024; }
+  __device__ __forceinline__ tam_i4 rsrc(int) const {
+    const uint64_t b = (uint64_t)base;
+    return tam_i4{(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)0x80000000u, 0x00020000};
+  }
+  __device__ __forceinline__ uint32_t offset(int i, uint32_t left) const { return lane_k[i] < left ? off[i] : 0x80000000u; }
+
   __device__ __forceinline__ const char* at() const { return base; }
   __device__ __forceinline__ void seek(const char* p) { base = p; }
   __device__ __forceinline__ void next() { base += step; }
@@ -232,6 +261,14 @@ struct tam_pair_stage {
     const int n = row0 / 16 % TN, row = (row0 / 16 / TN * (TN / 2) + n % (TN / 2)) * 16;
     Half::read(f, n < TN / 2 ? lds : lds + Half::BYTES, row, h, lane);
   }
+  static constexpr int WAVE_BYTES = Half::WAVE_BYTES;
+  __device__ static constexpr int place(int i) {
+    return i < Half::LOADS ? i * 1024 : Half::BYTES + (i - Half::LOADS) * 1024;
+  }
+  __device__ __forceinline__ tam_i4 rsrc(int i) const { return i < Half::LOADS ? a.rsrc(i) : b.rsrc(i); }
+  __device__ __forceinline__ uint32_t offset(int i, uint32_t left) const {
+    return i < Half::LOADS ? a.offset(i, left) : b.offset(i - Half::LOADS, left);
+  }
   __device__ __forceinline__ const char* at() const { return a.base; }
   __device__ __forceinline__ void seek(const char*) {}
   __device__ __forceinline__ void next() {
@@ -281,6 +318,7 @@ template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool 
 struct tam_tile {
   static constexpr int NW = WM * WN;
   static constexpr int THREADS = 64 * NW;
+  static constexpr bool RING = BM == 256;
   static constexpr int TM = BM / WM / 16;  // a wave's fragments of Q
   static constexpr int TN = BN / WN / 16;  // and of P
   typedef std::conditional_t<PAIR, tam_pair_stage<T, BN, NW, PK, TN>, tam_stage<T, BN, NW, PK, EXACT && !PK>> SP;
@@ -293,7 +331,7 @@ struct tam_tile {
   static constexpr int PITCH = COLS + 4;                  // floats of a turned row
   static constexpr int TURN = NW * ROUND * PITCH * 4;
   static constexpr int DUMP = STAGES * STAGE > TURN ? STAGES * STAGE : TURN;
-  static constexpr int LDS = DUMP + NW * 256;  // the words that `soon` fetches
+  static constexpr int LDS = RING ? 5 * SP::BYTES : DUMP + NW * 256;  // the words that `soon` fetches
   static_assert(TM % 2 == 0, "rounds of 32 rows");
 
   tam_f4 acc[TN][TM];
@@ -319,6 +357,7 @@ struct tam_tile {
   template <int TERMS = TAM_ONE_TERM, typename Columns = tam_operand>
   __device__ __forceinline__ void run(const Columns& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
                                       uint64_t k1, char* smem, const tam_soon& soon, tam_parts parts = {1, 0, 0}) {
+    if constexpr (RING) return run_ring<TERMS>(P, Q, c0, r0, k0, k1, smem, parts);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     tam_lds_char* lds = (tam_lds_char*)smem;
@@ -410,6 +449,148 @@ struct tam_tile {
     sync<0>();  // the LDS is the epilogue's
   }
 
+  // The same for the largest tiles, whose stages are 32 KB of each operand: a ring of five
+  // such halves in place of two stages, so that one operand's loads are in flight while the
+  // other's arrive. Step t: read the second half's fragments of stage t and issue the loads of
+  // P's stage t + 2 among the matrix instructions of the first half; wait for stage t + 1 and
+  // for the own reads, barrier; read the first half of stage t + 1 and issue the loads of Q's
+  // stage t + 2 (into what P's stage t held) among those of the second half.
+  // begin issues the first two stages into the first four halves, which nobody may be
+  // reading; sum waits for them and adds the products. So a workgroup can begin its next
+  // tile before it stores this one, by way of the fifth half (`spare`).
+  static constexpr int HALF = SP::BYTES, L = SP::LOADS;
+  struct ring {
+    SP sp;
+    SQ sq;
+    const char *p0, *q0;
+    int64_t length, ahead;      // k of a sum; from the next stage to load on
+    uint32_t steps, left, seen, term;
+    uint32_t off_p[L], off_q[L];  // of a stage with `left`: it is BK in all but the last stages of a sum
+    tam_parts parts;
+
+    template <int TERMS>
+    __device__ __forceinline__ void stage() {
+      if constexpr (TERMS != TAM_ONE_TERM)
+        if (ahead <= 0 && term + 1 < parts.terms) {
+          ++term;
+          ahead = length;
+          sp.seek(p0 + (TERMS == TAM_TWO_PRODUCTS || term == 2 ? parts.p : 0));
+          sq.seek(q0 + (term == 1 ? parts.q : 0));
+        }
+      left = ahead <= 0 ? 0u : (ahead > BK ? (uint32_t)BK : (uint32_t)ahead);
+      ahead -= BK;
+      if (left != seen) {
+        seen = left;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+          off_p[i] = sp.offset(i, left);
+          off_q[i] = sq.offset(i, left);
+        }
+      }
+    }
+  };
+
+  template <int TERMS = TAM_ONE_TERM, typename Columns = tam_operand>
+  __device__ __forceinline__ static void begin(ring& r, const Columns& P, const tam_operand& Q, uint32_t c0, uint32_t r0,
+                                               uint64_t k0, uint64_t k1, char* smem, tam_parts parts = {1, 0, 0}) {
+    static_assert(SP::BYTES == SQ::BYTES && SP::LOADS == SQ::LOADS, "halves of one size");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(tam_lds_char*)smem);
+    r.sp.init(P, c0, k0, wave, lane);
+    r.sq.init(Q, r0, k0, wave, lane);
+    r.p0 = r.sp.at();
+    r.q0 = r.sq.at();
+    r.length = r.ahead = k1 > k0 ? (int64_t)(k1 - k0) : 0;
+    r.steps = (uint32_t)((r.length + BK - 1) / BK);
+    if constexpr (TERMS != TAM_ONE_TERM) r.steps *= parts.terms;
+    r.parts = parts;
+    r.term = 0;
+    r.seen = ~0u;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      r.template stage<TERMS>();
+#pragma unroll
+      for (int i = 0; i < L; ++i) tam_to_lds(lds0 + 2 * s * HALF + wave * SP::WAVE_BYTES + SP::place(i), r.off_p[i], r.sp.rsrc(i));
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+        tam_to_lds(lds0 + (2 * s + 1) * HALF + wave * SQ::WAVE_BYTES + SQ::place(i), r.off_q[i], r.sq.rsrc(i));
+      r.sp.next();
+      r.sq.next();
+    }
+  }
+
+  // LATER: vector memory operations that every wave has issued since begin, at least.
+  template <int TERMS = TAM_ONE_TERM, int LATER = 0>
+  __device__ __forceinline__ void sum(ring& r, char* smem) {
+    constexpr int READS = TM + TN, SLOTS = TM * TN;
+    constexpr int READ_EVERY = SLOTS * 3 / 4 / READS, LOAD_EVERY = SLOTS / 2 / L;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    tam_lds_char* lds = (tam_lds_char*)smem;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+    const uint32_t lds_p = lds0 + (uint32_t)wave * SP::WAVE_BYTES, lds_q = lds0 + (uint32_t)wave * SQ::WAVE_BYTES;
+    // Half a step: fragments of half h out of buffers bp and bq, P's first as they are used
+    // first, spread over the first three quarters of the matrix instructions (their latency
+    // is over at the barrier); the loads over the first half.
+    auto half = [&](const frags& f, frags& next, uint32_t bp, uint32_t bq, int h, const auto& st, const uint32_t(&off)[L],
+                    uint32_t to) {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) {
+        if (s % READ_EVERY == 0 && s / READ_EVERY < READS) {
+          const int i = s / READ_EVERY;
+          if (i < TN)
+            SP::read(next.p[i], lds + bp * HALF, (wn * TN + i) * 16, h, lane);
+          else
+            SQ::read(next.q[i - TN], lds + bq * HALF, (wm * TM + i - TN) * 16, h, lane);
+        }
+        const int m = s / TN, n = s % TN, i = s / LOAD_EVERY;
+        if (s % LOAD_EVERY == 1 && i < L)
+          tam_mfma_load(f.p[n], f.q[m], acc[n][m], to, st.place(i), off[i], st.rsrc(i));
+        else
+          tam_mfma_in(f.p[n], f.q[m], acc[n][m]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    frags a, b;
+    constexpr int FIRST = 2 * L + LATER < 63 ? 2 * L + LATER : 63;
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(FIRST) : "memory");
+#pragma unroll
+    for (int n = 0; n < TN; ++n) SP::read(a.p[n], lds, (wn * TN + n) * 16, 0, lane);
+#pragma unroll
+    for (int m = 0; m < TM; ++m) SQ::read(a.q[m], lds + HALF, (wm * TM + m) * 16, 0, lane);
+    uint32_t bp = 0;  // buffer of P's stage t; those behind it, in the ring's order: Q's, and so on
+    auto behind = [&](uint32_t n) { return bp + n >= 5 ? bp + n - 5 : bp + n; };
+    for (uint32_t t = 0; t < r.steps; ++t) {
+      r.template stage<TERMS>();
+      half(a, b, bp, behind(1), 1, r.sp, r.off_p, lds_p + behind(4) * HALF);
+      sync<L>();
+      half(b, a, behind(2), behind(3), 0, r.sq, r.off_q, lds_q + bp * HALF);
+      r.sp.next();
+      r.sq.next();
+      bp = behind(2);
+    }
+    sync<0>();  // the LDS is the epilogue's
+    settle();
+  }
+
+  template <int TERMS = TAM_ONE_TERM, typename Columns = tam_operand>
+  __device__ __forceinline__ void run_ring(const Columns& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
+                                           uint64_t k1, char* smem, tam_parts parts = {1, 0, 0}) {
+    ring r;
+    __syncthreads();  // the LDS may hold what another tile's epilogue still reads
+    begin<TERMS>(r, P, Q, c0, r0, k0, k1, smem, parts);
+    sum<TERMS>(r, smem);
+  }
+
+  // Behind the last of tam_mfma_in: a result may be read 11 wait states after it.
+  __device__ __forceinline__ void settle() {
+    asm volatile("s_nop 15\n\ts_nop 7");
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+      for (int m = 0; m < TM; ++m) asm volatile("" : "+v"(acc[n][m]));
+  }
+
   // Adds the products of k0 <= k < k1, a few of them, element by element.
   __device__ __forceinline__ void tail(const tam_operand& P, const tam_operand& Q, uint32_t c0, uint32_t r0, uint64_t k0,
                                        uint64_t k1) {
@@ -473,6 +654,37 @@ struct tam_tile {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
     }
+  }
+
+  // Epilogue of a tile whose next one has begun: by 16 rows at a time through the fifth half,
+  // where a wave has room for them; 16-byte chunk c of row r lies at place c ^ r.
+  static constexpr int SPARE = 4 * HALF;
+  __device__ __forceinline__ tam_lds_char* spare(char* smem) const {
+    return (tam_lds_char*)smem + SPARE + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (HALF / NW);
+  }
+  // Fragment m as fp32, by rows: one of its 16 rows to LPR lanes.
+  __device__ __forceinline__ void turn_in(char* smem, int m) const {
+    const uint32_t lane = threadIdx.x & 63, row = lane & 15;
+    tam_lds_char* at = spare(smem) + row * (COLS * 4);
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+      *(__attribute__((address_space(3))) tam_f4*)(at + ((n * 4 + (lane >> 4)) ^ row) * 16) = acc[n][m];
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  // 8 columns of a row of it.
+  __device__ __forceinline__ void turn_out(char* smem, uint32_t row, uint32_t col, float (&v)[8]) const {
+    const tam_lds_char* at = spare(smem) + row * (COLS * 4);
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      const tam_f4 x = *(const __attribute__((address_space(3))) tam_f4*)(at + ((col / 4 + j) ^ row) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * j + i] = x[i];
+    }
+  }
+  __device__ __forceinline__ static void turned() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
   }
 
   // Hands the tile to finish(row, col, v, pre): 8 consecutive columns of one row, in
