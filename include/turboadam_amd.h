@@ -396,8 +396,8 @@ int tam_norm_backward(const TamNorm* d, void* workspace, size_t ws_bytes, void* 
 
 /* The first half of a gated feed-forward block: h = act(x gate^T) * (x up^T), and its
  * gradients.  Both products are one; the backward pass sees g = x gate^T and u = x up^T
- * rounded to dtype, and dg = dh u act'(g) and du = dh act(g) are rounded to it before the
- * products that make dx, dgate and dup.  Every array is of `dtype`; arrays without a stride
+ * with 8 bits more than dtype, and dg = dh u act'(g) and du = dh act(g) are rounded to it
+ * before the products that make dx, dgate and dup.  Every array is of `dtype`; arrays without a stride
  * are contiguous.  Arrays may lie at any element's address; operands whose rows are not
  * whole 16 bytes on 4 bytes are first copied to the workspace: ask for its size with the
  * pointers and strides of the call. */
@@ -406,8 +406,8 @@ typedef struct TamGated {
   const void* gate;     /* [outputs][inputs], or [inputs][outputs] with w_in_out;  */
   const void* up;       /* row stride ldw of both                                  */
   void* h;              /* forward: [rows][outputs]                                */
-  void* g;              /* [rows][outputs]: forward: written, or NULL; backward:   */
-  void* u;              /* read (the forward's)                                    */
+  void* kept;           /* tam_gated_kept(..) bytes, 16-byte aligned: forward:     */
+                        /* written, or NULL; backward: read (the forward's)        */
   const void* dh;       /* backward: [rows][outputs]                               */
   void* dx;             /* backward: [rows][inputs], or NULL                       */
   void* dgate;          /* backward: laid out as the weights, contiguous, or NULL  */
@@ -420,6 +420,8 @@ typedef struct TamGated {
   uint32_t reserved;
 } TamGated;
 
+/* Bytes that the forward pass keeps for the backward pass: 6 (fp32: 8) to an output. */
+size_t tam_gated_kept(uint64_t rows, uint64_t outputs, uint32_t dtype);
 /* Bytes of workspace (256-byte aligned) of the two calls below. */
 int tam_gated_workspace(const TamGated* d, int backward_pass, size_t* bytes);
 /* How their products are cut, as tam_linear_tiles tells it: h or dx, then dgate with dup. */

@@ -139,6 +139,21 @@ def test_gated_relu_of_whole_numbers(dt):
     _check_gated(x, wg, wu, dh, dt, "relu")
 
 
+@pytest.mark.parametrize("rows", [20, 100])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_gated_of_products_below_and_near_the_ends_of_the_range(rows, dt):
+    """Rows of x from 2^-24 to 1 and some zeros: products below fp16's normal numbers and below its smallest; and
+    products past the middle of a type's last place, either side of 0."""
+    x, wg, wu, dh = _gated_case(rows, 40, 50, dt)
+    x = (x.float() * torch.exp2(-(torch.arange(rows, device="cuda") % 25.0))[:, None]).to(DTYPES[dt])
+    x[3] = 0
+    for act in ("silu", "gelu", None):
+        log(f"gated small {rows} {dt} {act}")
+        _check_gated(x, wg, wu, dh, dt, act)
+    log(f"gated large {rows} {dt}")
+    _check_gated(x * (64 if dt == "f16" else 2.0 ** 30), wg, wu, dh * 2.0 ** -10, dt, "relu" if dt == "f32" else "silu")
+
+
 @pytest.mark.parametrize("rows", [5, 90])
 @pytest.mark.parametrize("dt", list(DTYPES))
 def test_gated_views_and_weights_of_two_layouts(rows, dt):

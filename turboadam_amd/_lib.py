@@ -162,8 +162,7 @@ class TamGated(ctypes.Structure):
         ("gate", ctypes.c_void_p),
         ("up", ctypes.c_void_p),
         ("h", ctypes.c_void_p),
-        ("g", ctypes.c_void_p),
-        ("u", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
         ("dh", ctypes.c_void_p),
         ("dx", ctypes.c_void_p),
         ("dgate", ctypes.c_void_p),
@@ -339,6 +338,7 @@ SIGNATURES = {
     "tam_norm_workspace": (ctypes.c_int, [ctypes.POINTER(TamNorm), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_norm": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP]),
     "tam_norm_backward": (ctypes.c_int, [ctypes.POINTER(TamNorm), _VP, ctypes.c_size_t, _VP]),
+    "tam_gated_kept": (ctypes.c_size_t, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32]),
     "tam_gated_workspace": (ctypes.c_int, [ctypes.POINTER(TamGated), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_gated_tiles": (ctypes.c_int, [ctypes.POINTER(TamGated), ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     "tam_gated": (ctypes.c_int, [ctypes.POINTER(TamGated), _VP, ctypes.c_size_t, _VP]),

@@ -56,17 +56,15 @@ struct GatedCall {
   }
 };
 
-Tensor gated_forward(const Tensor& x, const Tensor& gate, const Tensor& up, int64_t activation, Tensor* g, Tensor* u) {
+Tensor gated_forward(const Tensor& x, const Tensor& gate, const Tensor& up, int64_t activation, Tensor* kept) {
   const c10::DeviceGuard guard(x.device());
   GatedCall c(x, gate, up, activation);
   auto sizes = x.sizes().vec();
   sizes.back() = gate.size(0);
   const Tensor h = at::empty(sizes, x.options().requires_grad(false));
-  if (g) {
-    *g = at::empty(sizes, h.options());
-    *u = at::empty(sizes, h.options());
-    c.d.g = g->data_ptr();
-    c.d.u = u->data_ptr();
+  if (kept) {
+    *kept = workspace(lib.gated_kept(c.d.rows, c.d.outputs, c.d.dtype), x);
+    c.d.kept = ptr(*kept);
   }
   c.d.h = h.data_ptr();
   c.run(false);
@@ -76,9 +74,9 @@ Tensor gated_forward(const Tensor& x, const Tensor& gate, const Tensor& up, int6
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up, int64_t activation) {
     at::AutoDispatchBelowADInplaceOrView below;
-    Tensor g, u;
-    const Tensor h = gated_forward(x, gate, up, activation, &g, &u);
-    ctx->save_for_backward({x, gate, up, g, u});
+    Tensor kept;
+    const Tensor h = gated_forward(x, gate, up, activation, &kept);
+    ctx->save_for_backward({x, gate, up, kept});
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["wants"] =
         (int64_t)((wants_gradient(x) ? 1 : 0) | (wants_gradient(gate) ? 2 : 0) | (wants_gradient(up) ? 4 : 0));
@@ -106,8 +104,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
       if (wants & 2) dgate = weight();
       if (wants & 4) dup = weight();
       c.d.dh = d.data_ptr();
-      c.d.g = saved[3].data_ptr();
-      c.d.u = saved[4].data_ptr();
+      c.d.kept = ptr(saved[3]);
       c.d.dx = ptr(dx);
       c.d.dgate = ptr(dgate);
       c.d.dup = ptr(dup);
@@ -133,7 +130,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& gate, const Tensor& up, int64
     refuse_value(c10::str("gated_linear: up must have gate's shape ", shape(gate), ", got ", shape(up)));
   refuse_tangents("gated_linear", {&x, &gate, &up});
   if (any_gradient({&x, &gate, &up})) return GatedLinear::apply(x, gate, up, activation);
-  return gated_forward(x, gate, up, activation, nullptr, nullptr);
+  return gated_forward(x, gate, up, activation, nullptr);
 }
 
 // --------------------------------------------- projection and cross entropy

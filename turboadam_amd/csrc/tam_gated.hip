@@ -27,26 +27,86 @@ namespace {
 // forward
 // ---------------------------------------------------------------------------
 struct gated_epilogue {
-  void* h;  // [rows][cols], contiguous
-  void* g;  // or null
-  void* u;  // or null
+  void* h;     // [rows][cols], contiguous
+  char* kept;  // [rows][(cols + 7) / 8] records of g and u, or null
   uint32_t rows, cols, act;
 };
 
-// a, b: columns col .. col + 7 of a row of g and u. h is formed of both as they are in
-// fp32; they are kept rounded to the type (half of the memory).
+// What the forward pass keeps of g and u: for 8 columns a record of 64 bytes in fp32, of 48 in
+// 16 bits: 8 of g and 8 of u in the type and, one byte each, the next 8 bits of both. (Rounded
+// to the type alone, they bring dgate's, dup's and dx's errors in bf16 from 2.4e-3 of their norm to
+// 3.0e-3, 1.7e-3 of it their own rounding; the bytes cost 2% of a large training pass.)
+template <typename T>
+constexpr uint32_t gated_record = sizeof(T) == 4 ? 64 : 48;
+
+// The low byte of x past its rounding h: of the distance of their bits, in 2^-8 of the
+// type's last place.
+template <typename T>
+__device__ __forceinline__ uint32_t gated_low(float x, T h) {
+  const float f = (float)h;
+  int32_t d = (int32_t)(__builtin_bit_cast(uint32_t, x) - __builtin_bit_cast(uint32_t, f));
+  if constexpr (std::is_same_v<T, tam_f16>) {
+    // below fp16's normal numbers places are wider than 2^13 bits, up to those of x where h is
+    // 0: as near as a byte comes; an infinity that x is not stays one
+    d = d < -4096 ? -4096 : (d > 4095 ? 4095 : d);
+    d = __builtin_isinf(f) ? 0 : d * 8;
+  }
+  d += 128;
+  return (uint32_t)(d < 32767 ? d : 32767) >> 8 & 0xffu;
+}
+template <typename T>
+__device__ __forceinline__ float gated_value(T h, uint32_t low) {
+  const int32_t d = (int32_t)(low << 24) >> (std::is_same_v<T, tam_f16> ? 19 : 16);
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)h) + (uint32_t)d);
+}
+
+template <typename T>
+__device__ __forceinline__ void gated_keep(char* at, const float (&g)[8], const float (&u)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    tam_store8(reinterpret_cast<T*>(at), g);
+    tam_store8(reinterpret_cast<T*>(at) + 8, u);
+  } else {
+    tam_oct<T> hg, hu;
+    uint32_t low[4] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hg.v[j] = (T)g[j];
+      hu.v[j] = (T)u[j];
+      low[j / 4] |= gated_low<T>(g[j], hg.v[j]) << (j % 4 * 8);
+      low[2 + j / 4] |= gated_low<T>(u[j], hu.v[j]) << (j % 4 * 8);
+    }
+    *reinterpret_cast<tam_oct<T>*>(at) = hg;
+    *reinterpret_cast<tam_oct<T>*>(at + 16) = hu;
+    *reinterpret_cast<uint4*>(at + 32) = uint4{low[0], low[1], low[2], low[3]};
+  }
+}
+template <typename T>
+__device__ __forceinline__ void gated_recall(const char* at, float (&g)[8], float (&u)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    tam_load8(reinterpret_cast<const T*>(at), g);
+    tam_load8(reinterpret_cast<const T*>(at) + 8, u);
+  } else {
+    const tam_oct<T> hg = *reinterpret_cast<const tam_oct<T>*>(at), hu = *reinterpret_cast<const tam_oct<T>*>(at + 16);
+    const uint4 l = *reinterpret_cast<const uint4*>(at + 32);
+    const uint32_t low[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      g[j] = gated_value<T>(hg.v[j], low[j / 4] >> (j % 4 * 8));
+      u[j] = gated_value<T>(hu.v[j], low[2 + j / 4] >> (j % 4 * 8));
+    }
+  }
+}
+
+// a, b: columns col .. col + 7 of a row of g and u. h is formed of both as they are in fp32.
 template <typename T>
 __device__ __forceinline__ void gated_finish(const gated_epilogue& e, uint32_t row, uint32_t col, const float (&a)[8],
                                              const float (&b)[8]) {
-  const uint64_t at = (uint64_t)row * e.cols + col;
-  const uint32_t count = e.cols - col;
-  if (e.g) tam_store_some(static_cast<T*>(e.g) + at, count, a);
-  if (e.u) tam_store_some(static_cast<T*>(e.u) + at, count, b);
+  if (e.kept) gated_keep<T>(e.kept + ((uint64_t)row * ((e.cols + 7) / 8) + col / 8) * gated_record<T>, a, b);
   float v[8];
   tam_act8<sizeof(T) == 2>(a, e.act, v);
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] *= b[j];
-  tam_store_some(static_cast<T*>(e.h) + at, count, v);
+  tam_store_some(static_cast<T*>(e.h) + (uint64_t)row * e.cols + col, e.cols - col, v);
 }
 
 struct gated_args {
@@ -214,8 +274,7 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_gated_few(gated_few_
 // ---------------------------------------------------------------------------
 struct gated_slope_args {
   const void* dh;
-  const void* g;
-  const void* u;
+  const char* kept;
   void* out;         // [rows][2][ld]: dg, du; up to 8 columns past the last one are zeros
   uint64_t rows;
   uint32_t cols, ld, act;
@@ -231,13 +290,13 @@ __global__ __launch_bounds__(256) void tam_k_gated_slope(gated_slope_args a) {
   const uint64_t at = row * a.cols + col;
   float d[8], g[8], u[8];
   tam_load_some(static_cast<const T*>(a.dh) + at, count, d);
-  tam_load_some(static_cast<const T*>(a.g) + at, count, g);
-  tam_load_some(static_cast<const T*>(a.u) + at, count, u);
+  gated_recall<T>(a.kept + i * gated_record<T>, g, u);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float s = tam_act_slope<sizeof(T) == 2>(g[j], a.act), v = tam_act<sizeof(T) == 2>(g[j], a.act);
-    g[j] = d[j] * u[j] * s;
-    u[j] = d[j] * v;
+    // past the last column the record is what a tile holds there
+    g[j] = (uint32_t)j < count ? d[j] * u[j] * s : 0.0f;
+    u[j] = (uint32_t)j < count ? d[j] * v : 0.0f;
   }
   T* out = static_cast<T*>(a.out) + 2 * row * a.ld + col;
   tam_store8(out, g);
@@ -345,7 +404,8 @@ int check_gated(const TamGated* d, bool back) {
   if (d->rows == 0 || d->outputs == 0) return TAM_OK;
   if (d->inputs && (!d->x || !d->gate || !d->up)) return tam_op_fail(TAM_E_INVALID, "null x, gate or up");
   if (!back && !d->h) return tam_op_fail(TAM_E_INVALID, "null h");
-  if (back && (!d->dh || !d->g || !d->u)) return tam_op_fail(TAM_E_INVALID, "null dh, g or u");
+  if (back && (!d->dh || !d->kept)) return tam_op_fail(TAM_E_INVALID, "null dh, or what the forward pass kept");
+  if ((uintptr_t)d->kept & 15u) return tam_op_fail(TAM_E_INVALID, "kept memory not on 16 bytes");
   return TAM_OK;
 }
 
@@ -417,7 +477,7 @@ int zero(call& c, void* p, uint64_t elements) {
 
 int forward(const TamGated* d, call& c) {
   if (d->rows == 0 || d->outputs == 0) return TAM_OK;
-  const gated_epilogue e = {d->h, d->g, d->u, (uint32_t)d->rows, (uint32_t)d->outputs, d->activation};
+  const gated_epilogue e = {d->h, (char*)d->kept, (uint32_t)d->rows, (uint32_t)d->outputs, d->activation};
   if (d->rows <= 32 && !d->w_in_out) {
     if (c.dry) return TAM_OK;
     const gated_few_args a = {d->x, d->gate, d->up, d->ldx, d->ldw, d->inputs, e};
@@ -508,7 +568,7 @@ int backward(const TamGated* d, call& c) {
   const uint32_t ld = aligned_ld(outputs, size);
   const matrix both = {c.ws.take((uint64_t)rows * 2 * ld * size), 2ull * ld, rows, 2 * ld, true};
   if (!c.dry) {
-    const gated_slope_args a = {d->dh, d->g, d->u, (void*)both.p, rows, outputs, ld, d->activation};
+    const gated_slope_args a = {d->dh, (const char*)d->kept, (void*)both.p, rows, outputs, ld, d->activation};
     const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(outputs, 8) * rows, 256)), block(256);
 #define TAM_SLOPE(T) hipLaunchKernelGGL(tam_k_gated_slope<T>, grid, block, 0, c.stream, a)
     TAM_OF_TYPE(c, TAM_SLOPE);
@@ -563,6 +623,10 @@ int gated(const TamGated* d, bool back, void* workspace, uint64_t ws_bytes, void
 }  // namespace
 
 extern "C" {
+
+size_t tam_gated_kept(uint64_t rows, uint64_t outputs, uint32_t dtype) {
+  return (size_t)(rows * tam_div_up(outputs, 8) * (dtype == TAM_DTYPE_F32 ? gated_record<float> : gated_record<tam_f16>));
+}
 
 int tam_gated_workspace(const TamGated* d, int backward_pass, size_t* bytes) {
   if (!bytes) {

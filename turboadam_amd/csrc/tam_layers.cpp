@@ -257,6 +257,7 @@ void tam_register_layers(py::module_& m) {
     take(at, "tam_norm_workspace", lib.norm_workspace);
     take(at, "tam_norm", lib.norm);
     take(at, "tam_norm_backward", lib.norm_backward);
+    take(at, "tam_gated_kept", lib.gated_kept);
     take(at, "tam_gated_workspace", lib.gated_workspace);
     take(at, "tam_gated", lib.gated);
     take(at, "tam_gated_backward", lib.gated_backward);

@@ -27,6 +27,7 @@ struct Library {
   decltype(&tam_norm_workspace) norm_workspace = nullptr;
   decltype(&tam_norm) norm = nullptr;
   decltype(&tam_norm_backward) norm_backward = nullptr;
+  decltype(&tam_gated_kept) gated_kept = nullptr;
   decltype(&tam_gated_workspace) gated_workspace = nullptr;
   decltype(&tam_gated) gated = nullptr;
   decltype(&tam_gated_backward) gated_backward = nullptr;
