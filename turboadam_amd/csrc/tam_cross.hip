@@ -41,10 +41,22 @@ __device__ __forceinline__ float cross_exp(float x) {
     return expf(x);
 }
 
-// exp(z - m), 0 where z is -inf (also where m is), NaN where z is
-template <typename T>
-__device__ __forceinline__ float cross_term(float z, float m) {
-  return z == -INFINITY ? 0.0f : cross_exp<T>(z - m);
+// The sum of exp(z - top) over a lane's values, top their maximum or more. A top of -inf
+// (words that cannot be, or columns past the last one) counts as 0: exp(-inf) is 0; a
+// NaN or an infinity makes the sum NaN.
+template <typename T, int N>
+__device__ __forceinline__ float cross_terms(const float (&z)[N], float top) {
+  const float at = top == -INFINITY ? 0.0f : top;
+  float sum = 0.f;
+  if constexpr (sizeof(T) == 2) {  // one multiplication and addition ahead of the hardware's 2^x
+    const float shift = -kLog2e * at;
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], kLog2e, shift));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum += expf(z[j] - at);
+  }
+  return sum;
 }
 
 // What the forward pass keeps, and what every kernel reads: all by the row's own number but
@@ -149,82 +161,213 @@ struct cross_row {
   uint32_t unused;
 };
 
+// Over the four lanes whose numbers agree in their last four bits; all get the same bits.
+template <typename F>
+__device__ __forceinline__ float cross_rows4(float x, F f) {
+  const uint32_t i = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t j = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(j, j, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+// A lane holds 4 consecutive columns of a row in each of its fragments. Forward: the maximum
+// and the sum over its 4 TN columns, then the row's 4 lanes, then the tile's waves side by side
+// (`at`: [TILE][WN] in LDS), and the target's z if it is here.
+template <typename T, typename Tile, int TILE, int WN, typename Sync>
+__device__ __forceinline__ void cross_forward(const cross_logits_args& a, Tile& t, const int32_t (&target)[Tile::TM],
+                                              uint32_t m, uint32_t n, uint32_t count, float2* at, Sync sync) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+  const uint32_t col0 = n * TILE + wn * Tile::TN * 16 + (lane >> 4) * 4;  // the lane's first column
+  if (n * TILE + TILE > a.cols)
+#pragma unroll
+    for (uint32_t c = 0; c < Tile::TN; ++c)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (col0 + c * 16 + j >= a.cols)
+#pragma unroll
+          for (int f = 0; f < Tile::TM; ++f) t.acc[c][f][j] = -INFINITY;
+  bool here = false;  // a row's target is in its lane's columns: of 128 rows and 64 of 50257 columns, one wave in six
+#pragma unroll
+  for (int f = 0; f < Tile::TM; ++f) here |= target[f] >= 0 && (uint32_t)target[f] - col0 < Tile::TN * 16u;
+  if (__any(here))
+#pragma unroll
+    for (int f = 0; f < Tile::TM; ++f)
+#pragma unroll
+      for (uint32_t c = 0; c < Tile::TN; ++c)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          if (target[f] == (int32_t)(col0 + c * 16 + j))
+            a.hit[m * TILE + (wm * Tile::TM + f) * 16 + (lane & 15)] = t.acc[c][f][j];
+#pragma unroll
+  for (int f = 0; f < Tile::TM; ++f) {
+    float z[4 * Tile::TN];
+#pragma unroll
+    for (int c = 0; c < Tile::TN; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[4 * c + j] = t.acc[c][f][j];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4 * Tile::TN; ++i) top = fmaxf(top, z[i]);
+    top = cross_rows4(top, [](float x, float y) { return fmaxf(x, y); });
+    const float sum = cross_rows4(cross_terms<T>(z, top), [](float x, float y) { return x + y; });
+    if (lane < 16) at[((wm * Tile::TM + f) * 16 + lane) * WN + wn] = float2{top, sum};
+  }
+  sync();
+  const uint32_t row = m * TILE + threadIdx.x;
+  if (threadIdx.x < TILE && row < count) {
+    float2 all = {-INFINITY, 0.f};
+#pragma unroll
+    for (int w = 0; w < WN; ++w) all.x = fmaxf(all.x, at[threadIdx.x * WN + w].x);
+#pragma unroll
+    for (int w = 0; w < WN; ++w) {
+      const float2 p = at[threadIdx.x * WN + w];
+      if (p.y != 0.f) all.y += p.y * cross_exp<T>(p.x - all.x);
+    }
+    a.parts[(uint64_t)n * a.rows + row] = all;
+  }
+}
+
+// Backward, of a tile whose next one has begun: dz where the sums lie, in the type, and turned
+// in LDS by 16 rows, so that a row's 64 columns leave as one line.
+template <typename T, typename Tile, int TILE, int WN>
+__device__ __forceinline__ void cross_backward(const cross_logits_args& a, Tile& t, const float (&lse)[Tile::TM],
+                                               const float (&w)[Tile::TM], const int32_t (&target)[Tile::TM], uint32_t m,
+                                               uint32_t n, uint32_t count, char* smem) {
+  typedef T four __attribute__((ext_vector_type(4)));
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+  const uint32_t col0 = n * TILE + wn * Tile::TN * 16 + (lane >> 4) * 4, row = lane & 15;
+  T* const out = static_cast<T*>(a.dz);
+  bool some = n * TILE + TILE > a.cols;  // columns past the last one, or (a wave in six) a target in a lane's columns
+#pragma unroll
+  for (int f = 0; f < Tile::TM; ++f) some |= target[f] >= 0 && (uint32_t)target[f] - a.first - col0 < Tile::TN * 16u;
+  auto rows = [&](auto special) __attribute__((always_inline)) {
+#pragma unroll
+    for (int f = 0; f < Tile::TM; ++f) {
+      tam_lds_char* const turn = t.spare(smem) + f % 2 * 2048;
+      const uint32_t hit = (uint32_t)target[f] - a.first - col0;
+#pragma unroll
+      for (uint32_t c = 0; c < Tile::TN; ++c) {
+        four v;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          float p = cross_exp<T>(t.acc[c][f][j] - lse[f]);
+          if constexpr (decltype(special)::value) {
+            p -= hit == c * 16 + j ? 1.0f : 0.0f;
+            if (col0 + c * 16 + j >= a.cols) p = 0.0f;  // the sum over columns takes whole 16 bytes
+          }
+          v[j] = (T)(p * w[f]);
+        }
+        // 8 bytes; the 16 that they are half of lie at their place ^ row
+        *(__attribute__((address_space(3))) four*)(turn + row * 128 + ((c * 2 + (lane >> 5)) ^ (row & 7)) * 16 +
+                                                   (lane >> 4 & 1) * 8) = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t r = h * 8 + lane / 8, at = m * TILE + (wm * Tile::TM + f) * 16 + r;
+        const uint32_t col = n * TILE + wn * Tile::TN * 16 + lane % 8 * 8;
+        const tam_s8 v = *(const tam_lds_s8*)(turn + r * 128 + ((lane % 8) ^ (r & 7)) * 16);
+        if (at < count && col < a.cols) *reinterpret_cast<tam_s8*>(out + (uint64_t)at * a.ld + col) = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  if (__any(some))
+    rows(std::true_type());
+  else
+    rows(std::false_type());
+}
+
+// Bound by the matrix cores and, at small k, by what follows the sums: exponentials, and
+// in the backward pass the stores. 16-bit tiles of 256: a workgroup to a compute unit, which begins
+// its next tile before it goes through the last one's sums.
 template <typename T, int TILE, int WM, int WN, bool BACK>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_logits(cross_logits_args a) {
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), true, true> Tile;
   __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
-  const uint32_t count = *a.r.count;
+  const uint32_t count = *a.r.count, tm = (count + TILE - 1) / TILE, tiles = tm * a.tn;
+  if (blockIdx.x >= tiles) return;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN;
   uint32_t m, n;
-  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
-  if (m * TILE >= count) return;
+  tam_tile_at(tam_xcd_order(blockIdx.x, tiles), tm, a.tn, m, n);
   a.Q.count = count;
   Tile t;
-  t.zero();
-  t.run(a.P, a.Q, n * TILE, m * TILE, 0, a.k, smem, tam_soon{});
-  if constexpr (BACK) {
-    t.template each<TAM_AHEAD_PASS>(
-        smem,
-        [&](uint32_t row, uint32_t) {
-          row += m * TILE;
-          return a.row[row < count ? row : count - 1];
-        },
-        [&](uint32_t row, uint32_t col, float(&v)[8], const cross_row& of) {
-          row += m * TILE;
-          col += n * TILE;
-          if (row >= count || col >= a.cols) return;
-          const uint32_t hit = (uint32_t)of.target - a.first - col;
+  if constexpr (Tile::RING) {
+    typename Tile::ring r;
+    Tile::begin(r, a.P, a.Q, n * TILE, m * TILE, 0, a.k, smem);
+    for (uint32_t tile = blockIdx.x;;) {
+      t.zero();
+      t.sum(r, smem);
+      // ahead of the next tile's loads, behind which they would come
+      int32_t target[Tile::TM];
+      float lse[Tile::TM], w[Tile::TM];
 #pragma unroll
-          for (uint32_t j = 0; j < 8; ++j) {
-            const float p = cross_exp<T>(v[j] - of.lse) - (hit == j ? 1.0f : 0.0f);
-            // columns past the last one are zeros: the sum over columns takes whole 16 bytes
-            v[j] = col + j < a.cols ? p * of.w : 0.0f;
-          }
-          tam_store8(static_cast<T*>(a.dz) + (uint64_t)row * a.ld + col, v);
-        },
-        [](uint32_t, uint32_t, const float*, int) {});
-  } else {
-    // a lane holds 4 consecutive columns of a row in each of its fragments: its 4 TN
-    // columns, then the row's 4 lanes, then the tile's waves side by side
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-    float2* at = reinterpret_cast<float2*>(smem);  // [TILE][WN]
-#pragma unroll
-    for (int f = 0; f < Tile::TM; ++f) {
-      const uint32_t in = (wm * Tile::TM + f) * 16 + (lane & 15), row = m * TILE + in;
-      const int32_t target = row < count ? a.r.target[row] : -1;
-      float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < Tile::TN; ++c)
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          const uint32_t col = n * TILE + (wn * Tile::TN + c) * 16 + (lane >> 4) * 4 + j;
-          const float z = col < a.cols ? t.acc[c][f][j] : -INFINITY;
-          t.acc[c][f][j] = z;
-          if ((int32_t)col == target) a.hit[row] = z;
-          top = fmaxf(top, z);
+      for (int f = 0; f < Tile::TM; ++f) {
+        uint32_t row = m * TILE + (wm * Tile::TM + f) * 16 + (lane & 15);
+        row = row < count ? row : count - 1;  // whose sums go nowhere
+        if constexpr (BACK) {
+          const cross_row of = a.row[row];
+          lse[f] = of.lse;
+          w[f] = of.w;
+          target[f] = of.target;
+        } else {
+          target[f] = m * TILE + (wm * Tile::TM + f) * 16 + (lane & 15) < count ? a.r.target[row] : -1;
         }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < Tile::TN; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum += cross_term<T>(t.acc[c][f][j], top);
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      if (lane < 16) at[in * WN + wn] = float2{top, sum};
-    }
-    __syncthreads();
-    const uint32_t row = m * TILE + threadIdx.x;
-    if (threadIdx.x < TILE && row < count) {
-      float2 all = {-INFINITY, 0.f};
-#pragma unroll
-      for (int w = 0; w < WN; ++w) all.x = fmaxf(all.x, at[threadIdx.x * WN + w].x);
-#pragma unroll
-      for (int w = 0; w < WN; ++w) {
-        const float2 p = at[threadIdx.x * WN + w];
-        if (p.y != 0.f) all.y += p.y * cross_exp<T>(p.x - all.x);
       }
-      a.parts[(uint64_t)n * a.rows + row] = all;
+#pragma unroll
+      for (int f = 0; f < Tile::TM; ++f) {
+        if constexpr (BACK) asm volatile("" : "+v"(lse[f]), "+v"(w[f]));
+        asm volatile("" : "+v"(target[f]));
+      }
+      const uint32_t m0 = m, n0 = n;
+      tile += gridDim.x;
+      if (tile < tiles) {
+        tam_tile_at(tam_xcd_order(tile, tiles), tm, a.tn, m, n);
+        Tile::begin(r, a.P, a.Q, n * TILE, m * TILE, 0, a.k, smem);
+      }
+      if constexpr (BACK)
+        cross_backward<T, Tile, TILE, WN>(a, t, lse, w, target, m0, n0, count, smem);
+      else
+        cross_forward<T, Tile, TILE, WN>(a, t, target, m0, n0, count, reinterpret_cast<float2*>(smem + Tile::SPARE),
+                                         [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); });
+      if (tile >= tiles) return;
+    }
+  } else {
+    t.zero();
+    t.run(a.P, a.Q, n * TILE, m * TILE, 0, a.k, smem, tam_soon{});
+    if constexpr (BACK) {
+      t.template each<TAM_AHEAD_PASS>(
+          smem,
+          [&](uint32_t row, uint32_t) {
+            row += m * TILE;
+            return a.row[row < count ? row : count - 1];
+          },
+          [&](uint32_t row, uint32_t col, float(&v)[8], const cross_row& of) {
+            row += m * TILE;
+            col += n * TILE;
+            if (row >= count || col >= a.cols) return;
+            const uint32_t hit = (uint32_t)of.target - a.first - col;
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+              const float p = cross_exp<T>(v[j] - of.lse) - (hit == j ? 1.0f : 0.0f);
+              // columns past the last one are zeros: the sum over columns takes whole 16 bytes
+              v[j] = col + j < a.cols ? p * of.w : 0.0f;
+            }
+            tam_store8(static_cast<T*>(a.dz) + (uint64_t)row * a.ld + col, v);
+          },
+          [](uint32_t, uint32_t, const float*, int) {});
+    } else {
+      int32_t target[Tile::TM];
+#pragma unroll
+      for (int f = 0; f < Tile::TM; ++f) {
+        const uint32_t row = m * TILE + (wm * Tile::TM + f) * 16 + (lane & 15);
+        target[f] = row < count ? a.r.target[row] : -1;
+      }
+      cross_forward<T, Tile, TILE, WN>(a, t, target, m, n, count, reinterpret_cast<float2*>(smem), [] { __syncthreads(); });
     }
   }
 }
@@ -379,8 +522,7 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_
       top = fmaxf(top, v[j]);
     }
     top = fmaxf(top, __shfl_xor(top, 1));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) all += cross_term<T>(v[j], top);
+    all = cross_terms<T>(v, top);
     all += __shfl_xor(all, 1);
     if (t % 2 == 0 && row < a.rows) a.parts[(uint64_t)row * gridDim.x + blockIdx.x] = float2{top, all};
   }
@@ -603,7 +745,8 @@ int operands(const TamCross* d, call& c, const cross_rows& r, matrix& x, matrix&
 
 template <typename T, bool BACK>
 void launch_logits(int tile, const cross_logits_args& a, hipStream_t s) {
-  const dim3 grid(a.tm * a.tn);
+  const uint32_t tiles = a.tm * a.tn, cus = tam_op_cus();
+  const dim3 grid(tile == 256 && tiles > cus ? cus : tiles);
   if constexpr (sizeof(T) == 2)
     if (tile == 256) {
       hipLaunchKernelGGL((tam_k_cross_logits<T, 256, 2, 4, BACK>), grid, dim3(512), 0, s, a);
