@@ -828,3 +828,206 @@ def test_what_has_no_derivative_raises():
             call(fwd.make_dual(x.detach(), torch.ones_like(x)), fwd.make_dual(q.detach(), torch.ones_like(q)))
         with pytest.raises(RuntimeError, match="recorded"):
             torch.jit.trace(lambda x, q: call(x, q), (x.detach(), q.detach()), check_trace=False)
+
+
+# ------------------------------------------------- every tile, and offsets past 32 bits
+def _gated_tiles(m, k, n, dt, backward, in_out=False):
+    import ctypes
+
+    from turboadam_amd import _lib
+
+    d = _lib.TamGated()
+    d.x = d.gate = d.up = d.h = d.kept = d.dh = d.dx = d.dgate = d.dup = 0x10000
+    d.rows, d.inputs, d.outputs, d.ldx, d.ldw = m, k, n, k, n if in_out else k
+    d.w_in_out, d.dtype = in_out, _lib.DTYPES[DTYPES[dt]]
+    out = (ctypes.c_uint32 * 4)()
+    assert _lib.load().tam_gated_tiles(ctypes.byref(d), backward, out) == 0
+    return list(out)
+
+
+@pytest.mark.parametrize("m,k,n,dt,tiles", [
+    (4096, 512, 4000, "bf16", [256, 1]), (5000, 264, 1200, "f16", [256, 1]), (300, 200, 1000, "bf16", [64, 1]),
+    (96, 8192, 80, "bf16", [64, 32]), (1100, 8192, 520, "f16", [128, 3]), (2048, 512, 2048, "f32", [128, 1]),
+    (200, 2048, 130, "f32", [64, 12])])
+def test_gated_tiles_forward(m, k, n, dt, tiles):
+    # several tiles to a workgroup where they are the largest, ragged ones among them, sums in one part and in more
+    log(f"gated {m}x{k}x{n} {dt} tiles {_gated_tiles(m, k, n, dt, 0)}")
+    assert _gated_tiles(m, k, n, dt, 0)[:2] == tiles
+    _check_gated(*_gated_case(m, k, n, dt), dt, "silu")
+
+
+@pytest.mark.parametrize("m,k,n,dt,in_out,dx,dw", [
+    (6000, 2048, 3000, "bf16", False, 256, 256), (6000, 2048, 3000, "f16", True, 256, 256),
+    (2048, 2048, 4096, "bf16", False, 128, 256), (300, 200, 200, "bf16", True, 64, 64),
+    (1024, 1024, 2048, "f32", False, 64, 64)])
+def test_gated_tiles_backward(m, k, n, dt, in_out, dx, dw):
+    got = _gated_tiles(m, k, n, dt, 1, in_out)
+    log(f"gated {m}x{k}x{n} {dt} in_out={in_out} tiles {got}")
+    assert (got[0], got[2]) == (dx, dw)
+    _check_gated(*_gated_case(m, k, n, dt, in_out), dt, "gelu")
+
+
+def _cross_tiles(m, k, v, dt, backward):
+    import ctypes
+
+    from turboadam_amd import _lib
+
+    d = _lib.TamCross()
+    d.x = d.w = d.target = d.loss = d.kept = d.dloss = d.dx = d.dw = 0x10000
+    d.rows, d.inputs, d.vocabulary, d.ldx, d.ldw, d.dtype = m, k, v, k, k, _lib.DTYPES[DTYPES[dt]]
+    out = (ctypes.c_uint32 * 4)()
+    assert _lib.load().tam_cross_tiles(ctypes.byref(d), backward, out) == 0
+    return list(out)
+
+
+@pytest.mark.parametrize("m,k,v,dt,z,dx,dw", [
+    (4096, 264, 9973, "bf16", 256, 128, 128), (4096, 1032, 9973, "f16", 256, 256, 256), (1000, 300, 2100, "bf16", 64, 64, 64),
+    (8192, 40, 2100, "f16", 128, 64, 64), (4000, 1024, 4000, "f32", 128, 128, 128), (200, 100, 700, "f32", 64, 64, 64)])
+def test_cross_tiles(m, k, v, dt, z, dx, dw):
+    got = _cross_tiles(m, k, v, dt, 1)
+    log(f"cross {m}x{k}x{v} {dt} tiles {_cross_tiles(m, k, v, dt, 0)} and {got}")
+    assert _cross_tiles(m, k, v, dt, 0)[0] == z and [got[0], *got[2:]] == [z, dx, dw]
+    for ignored in (0.0, 0.6):
+        _check_cross(*_cross_case(m, k, v, dt, ignored), dt, "mean" if ignored else "none")
+
+
+def _whole(g, *shape):
+    return torch.randint(-3, 4, shape, generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+
+
+def test_gated_offsets_past_32_bits():
+    """Outputs of 2.3e9 elements, in whole numbers: every row, and the sums over all of them."""
+    from turboadam_amd import gated_linear
+
+    g = _gen("long")
+    m, k, n = 70001, 24, 32768
+    x, wg, wu, dh = _whole(g, m, k).requires_grad_(), _whole(g, n, k).requires_grad_(), _whole(g, n, k).requires_grad_(), \
+        _whole(g, m, n)
+    log(f"gated {m}x{k}x{n}")
+    h = gated_linear(x, wg, wu, activation="relu")
+    dx, dgate, dup = torch.autograd.grad(h, (x, wg, wu), dh)
+    X, G, U = x.detach().double(), wg.detach().double(), wu.detach().double()
+    sums = torch.zeros_like(G), torch.zeros_like(U)
+    for i in range(0, m, 5000):
+        rows = slice(i, min(i + 5000, m))
+        z, u, d = X[rows] @ G.t(), X[rows] @ U.t(), dh[rows].double()
+        assert torch.equal(h[rows], (z.relu() * u).to(h.dtype)), i
+        dz, du = (d * u * (z > 0)).bfloat16().double(), (d * z.relu()).bfloat16().double()
+        want = dz @ G + du @ U  # sums of whole numbers past fp32's: in any order within 2^-23 (n + 16) of their parts
+        slack = (dz.abs() @ G.abs() + du.abs() @ U.abs()) * _sum_error(2 * n) + want.abs() * UNIT["bf16"]
+        assert bool(((dx[rows].double() - want).abs() <= slack).all()), i
+        sums[0].add_(dz.t() @ X[rows])
+        sums[1].add_(du.t() @ X[rows])
+    for got, want in zip((dgate, dup), sums):  # of 70001 whole numbers up to 2^11
+        assert float((got.double() - want).norm()) <= (UNIT["bf16"] + 2.0 ** -18) * float(want.norm())
+
+
+def test_cross_offsets_past_32_bits():
+    from turboadam_amd import linear_cross_entropy
+
+    log("cross of 2.2e9 elements of x")
+    g = _gen("long cross")
+    m, k, v = 540001, 4096, 70
+    x = torch.randn(m, k, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    w = (torch.randn(v, k, generator=g, device="cuda") / 64).bfloat16().requires_grad_()
+    t = torch.randint(0, v, (m,), generator=g, device="cuda")
+    t[5::7] = -100
+    loss = linear_cross_entropy(x, w, t, reduction="none")
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss), retain_graph=True)
+    for i in (0, 262000, 524288, m - 3000):
+        part = x.detach()[i:i + 3000].clone().requires_grad_()
+        want = linear_cross_entropy(part, w.detach(), t[i:i + 3000], reduction="none")
+        assert float((loss.detach()[i:i + 3000] - want.detach()).abs().max()) < 2e-5, i
+        d, = torch.autograd.grad(want, part, torch.ones_like(want))
+        assert float((dx[i:i + 3000].double() - d.double()).norm()) <= 2 * UNIT["bf16"] * float(d.double().norm()), i
+    del dx, x
+    log("cross of 2.3e9 elements of w")
+    k, v = 18000, 128256
+    x, w = _whole(g, 40, k), _whole(g, v, k)
+    x = (x / 64).requires_grad_()
+    w.requires_grad_()
+    t = torch.randint(0, v, (40,), generator=g, device="cuda")
+    loss = linear_cross_entropy(x, w, t, reduction="sum")
+    dw, = torch.autograd.grad(loss, w)
+    z = torch.cat([x.detach().double() @ p.double().t() for p in w.detach().split(16384)], 1)
+    assert abs(float(loss.detach()) - float(F.cross_entropy(z, t, reduction="sum"))) < 1e-4 * float(loss.detach())
+    p = z.softmax(1)
+    p[torch.arange(40, device="cuda"), t] -= 1
+    for i in range(0, v, 16384):
+        want = p[:, i:i + 16384].t() @ x.detach().double()
+        assert float((dw[i:i + 16384].double() - want).norm()) <= 2 * UNIT["bf16"] * float(want.norm()) + 1e-6, i
+
+
+def test_rotary_offsets_past_32_bits():
+    from turboadam_amd import rotary, rotary_frequencies
+
+    g = _gen("long rotary")
+    t, h, d = 540001, 16, 256
+    log(f"rotary of {t}x{h}x{d}")
+    q = torch.randn(t, h, d, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    w = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).bfloat16()
+    f, p = rotary_frequencies(d, device="cuda"), torch.arange(t, device="cuda")
+    y = rotary(q, None, p, f, q_weight=w)
+    dq, = torch.autograd.grad(y, q, y)
+    for i in (0, 262000, 524288, t - 3000):  # the same rows by themselves, whose results other tests pin
+        part = q.detach()[i:i + 3000].clone().requires_grad_()
+        z = rotary(part, None, p[i:i + 3000], f, q_weight=w)
+        assert torch.equal(y[i:i + 3000], z), i
+        assert torch.equal(dq[i:i + 3000], torch.autograd.grad(z, part, z)[0]), i
+
+
+# ------------------------------------------------------------ the example
+def _example():
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_decoder.py")
+    spec = importlib.util.spec_from_file_location("train_decoder", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def test_example_runs():
+    mod = _example()
+    for dtype in ("bf16", "f32"):
+        losses = mod.train(dim=128, layers=1, words=300, sequences=4, length=33, steps=3, dtype=dtype, log=log)
+        assert len(losses) == 3 and all(math.isfinite(v) for v in losses)
+
+
+def test_example_gradients():
+    """The example's decoder in fp32: its loss and every gradient against the same network in 64 bits and plain torch.
+    Its sums have up to 512 terms of fp32 (2^-14 of their parts at most), its depth is a dozen of them: 1e-3 of a
+    gradient's norm is far above what they add up to, and far below a wrong term."""
+    mod = _example()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    model = mod.Decoder(128, 2, 200, torch.float32, g)
+    text = mod.make_text(g, torch.randint(0, 200, (200, 4), generator=g, device="cuda"), 3, 41)
+    names, params = zip(*model.named_parameters())
+    loss = model.loss(text, prompt=8)
+    grads = torch.autograd.grad(loss, params)
+    P = {n: p.detach().double().requires_grad_() for n, p in zip(names, params)}
+    head, f = mod.HEAD, model.frequencies
+
+    def turn(x, w):
+        x = x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+        return _turned(x, (torch.arange(40, device="cuda").double()[:, None] * f)[:, None, :], head, False, 1.0)[0]
+
+    x = P["embedding"][text[:, :-1]]
+    for i, layer in enumerate(model.layers):
+        at = {n: P[f"layers.{i}.{n}"] for n, _ in layer.named_parameters()}
+        n = F.layer_norm(x, (128,), at["norm1"])
+        q, k, v = (n @ at["qkv"].t()).unflatten(-1, (-1, head)).split((layer.heads, layer.kv_heads, layer.kv_heads), -2)
+        q, k = turn(q, at["q_norm"]), turn(k, at["k_norm"])
+        groups = layer.heads // layer.kv_heads
+        q, k, v = q.transpose(1, 2), k.repeat_interleave(groups, 2).transpose(1, 2), v.repeat_interleave(groups, 2).transpose(1, 2)
+        s = (q @ k.mT * head ** -0.5).masked_fill(torch.ones(40, 40, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+        x = x + (s.softmax(-1) @ v).transpose(1, 2).flatten(2) @ at["out"].t()
+        n = F.layer_norm(x, (128,), at["norm2"])
+        x = x + (F.silu(n @ at["gate"].t()) * (n @ at["up"].t())) @ at["down"].t()
+    target = text[:, 1:].clone()
+    target[:, :8] = -100
+    want = F.cross_entropy((F.layer_norm(x, (128,), P["norm"]) @ P["head"].t()).flatten(0, 1), target.flatten())
+    assert abs(float(loss.detach()) - float(want.detach())) < 1e-5 * float(want.detach())
+    for n, got, ref in zip(names, grads, torch.autograd.grad(want, list(P.values()))):
+        assert float((got.double() - ref).norm()) <= 1e-3 * float(ref.norm()), n
