@@ -24,25 +24,26 @@
 namespace {
 
 struct heads_args {
-  const void* x;      // or, in a backward pass without a norm, null
-  const void* w;      // or null: no norm
-  const void* dy;
-  void* y;            // forward: the result; backward: dx
-  int64_t x_b, x_t, x_h, dy_b, dy_t, dy_h, y_b, y_t, y_h;  // elements
+  const char* x;  // or, in a backward pass without a norm, what is turned back
+  const char* w;  // or null: no norm
+  const char* dy;
+  char* y;        // forward: the result; backward: dx
+  int64_t x_b, x_t, dy_b, dy_t, y_b, y_t;  // bytes
+  uint32_t x_h, dy_h, y_h;                 // bytes
+  uint32_t heads, turns;                   // rows; of a wave, at a time
 };
 
 struct rotary_args {
   heads_args part[2];  // queries, keys
-  const void* positions;
+  const char* positions;
   const double* frequencies;
-  float* sums;         // [workgroups][2][L * 16] or null
-  int64_t pos_b, pos_t;
-  uint32_t tokens;     // of a batch
-  uint32_t all;        // tokens of all batches
-  uint32_t heads_q, heads;
+  float* sums;         // [workgroups][2][lanes * 16] or null
+  int64_t pos_b, pos_t;  // bytes
+  uint32_t tokens, batches;
   uint32_t dim, rotated, units, lanes;
   uint32_t at_once;    // tokens of a wave
-  uint32_t split;      // waves that share a token's rows
+  uint32_t bundles;    // of at_once tokens, in a batch
+  uint32_t split;      // waves that share a bundle's rows
   uint32_t pos64;
   float eps, scale;    // scale: of the rotated part
   float sign;          // of the angles' sines: -1 turns back
@@ -85,9 +86,12 @@ struct two {
   tam_oct<T> lo, hi;
 };
 
+// The unit's elements of the row that lies `row` bytes behind a base that all lanes share: 32-bit
+// offsets of a lane, whose sums cost one instruction.
 template <typename T>
-__device__ __forceinline__ two<T> fetch(const T* row, const unit& u) {
-  return {tam_some(row + u.e0, u.n0), tam_some(row + u.e1, u.n1)};
+__device__ __forceinline__ two<T> fetch(const char* base, uint32_t row, const unit& u) {
+  return {tam_some(reinterpret_cast<const T*>(base + (row + u.e0 * (uint32_t)sizeof(T))), u.n0),
+          tam_some(reinterpret_cast<const T*>(base + (row + u.e1 * (uint32_t)sizeof(T))), u.n1)};
 }
 
 // The unit's pairs: of a[p] and b[p], whichever way they lie.
@@ -106,7 +110,7 @@ __device__ __forceinline__ void pairs(const two<T>& v, float (&a)[8], float (&b)
 }
 
 template <typename T, bool SIDE>
-__device__ __forceinline__ void store(T* row, const unit& u, const float (&a)[8], const float (&b)[8]) {
+__device__ __forceinline__ void store(char* base, uint32_t row, const unit& u, const float (&a)[8], const float (&b)[8]) {
   float lo[8], hi[8];
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
@@ -118,8 +122,8 @@ __device__ __forceinline__ void store(T* row, const unit& u, const float (&a)[8]
       hi[p] = b[p];
     }
   }
-  tam_store_some(row + u.e0, u.n0, lo);
-  tam_store_some(row + u.e1, u.n1, hi);
+  tam_store_some(reinterpret_cast<T*>(base + (row + u.e0 * (uint32_t)sizeof(T))), u.n0, lo);
+  tam_store_some(reinterpret_cast<T*>(base + (row + u.e1 * (uint32_t)sizeof(T))), u.n1, hi);
 }
 
 // Sum over a row's lanes (a power of two of them); all get the same bits.
@@ -143,57 +147,89 @@ __device__ __forceinline__ float lanes_sum(float x, uint32_t lanes) {
   return x;
 }
 
-// NORM: of the heads whose part has a weight. BACK: dx and the weights' sums of a norm's
-// backward pass (without a norm it is the forward pass with the angles' sign turned).
+// sin and cos of a number of turns: the quarter's number and what is left of it, both taken in 64
+// bits; Taylor's sums on [-pi/4, pi/4], off by 2^-25 (the first terms left out: y^11 / 11!, y^10 / 10!).
+__device__ __forceinline__ void sin_cos_turns(double turns, float& s, float& c) {
+  turns -= rint(turns);
+  const double quarters = rint(4.0 * turns);
+  const float y = (float)__builtin_fma(4.0, turns, -quarters) * 1.57079632679489662f, z = y * y;
+  const int q = (int)quarters;
+  float a = __builtin_fmaf(z, 2.75573192239858925e-6f, -1.98412698412698413e-4f);
+  a = __builtin_fmaf(z, a, 8.33333333333333322e-3f);
+  a = __builtin_fmaf(z, a, -1.66666666666666657e-1f);
+  a = __builtin_fmaf(y * z, a, y);
+  float b = __builtin_fmaf(z, 2.48015873015873016e-5f, -1.38888888888888894e-3f);
+  b = __builtin_fmaf(z, b, 4.16666666666666644e-2f);
+  b = __builtin_fmaf(z, b, -0.5f);
+  b = __builtin_fmaf(z, b, 1.0f);
+  const float u = q & 1 ? b : a, v = q & 1 ? a : b;
+  s = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, u) ^ ((uint32_t)q & 2u) << 30);
+  c = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) ^ ((uint32_t)(q + 1) & 2u) << 30);
+}
+
+// 1 / sqrt of a norm: of 16-bit results by the hardware's root, 2^-22.
+template <typename T>
+__device__ __forceinline__ float inverse_root(float x) {
+  if constexpr (sizeof(T) == 2)
+    return __builtin_amdgcn_rsqf(x);
+  else
+    return 1.0f / sqrtf(x);
+}
+
+// A wave takes a bundle's rows in turns, queries' first; a turn's rows are all of one part, and their
+// addresses a base that the lanes share and an offset that a lane keeps. Bound by memory and,
+// nearly as much, by the vector unit. NORM: both parts have a weight, or none. BACK: dx and the weights' sums of a
+// norm's backward pass (without a norm it is the forward pass with the angles' sign turned).
 template <typename T, bool SIDE, bool NORM, bool BACK>
-__global__ __launch_bounds__(256) void tam_k_rotary(rotary_args a) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_k_rotary(rotary_args a) {
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t u = lane & (a.lanes - 1), group = lane / a.lanes, groups = 64 / a.lanes;
   uint32_t rest;
   unit at = unit_at<SIDE>(u, a.dim, a.rotated, rest);
   if (u >= a.units) at.n0 = at.n1 = 0;
-  double turns[8];  // of a position step
-#pragma unroll
-  for (uint32_t p = 0; p < 8; ++p)
-    turns[p] = !rest && u * 8 + p < a.rotated / 2 ? a.frequencies[u * 8 + p] * 0.15915494309189535 : 0.0;
-  const uint32_t in = a.at_once > 1 ? group / a.heads : 0, first = a.at_once > 1 ? group - in * a.heads : group;
-  const uint32_t step = groups * a.split;
-  const uint32_t bundles = (a.all + a.at_once - 1) / a.at_once;
+  const uint32_t rows = a.at_once > 1 ? groups / a.at_once : groups;  // of a turn and token
+  const uint32_t in = group / rows, first = group - in * rows;
   const float inv = 1.0f / (float)a.dim;
+  const uint32_t turns = a.part[0].turns + a.part[1].turns, items = a.bundles * a.batches * a.split;
   float dw[2][16] = {};
-  for (uint64_t item = (uint64_t)blockIdx.x * 4 + wave; item < (uint64_t)bundles * a.split; item += (uint64_t)gridDim.x * 4) {
-    const uint32_t bundle = (uint32_t)(item / a.split), share = (uint32_t)(item - (uint64_t)bundle * a.split);
-    const uint32_t token = bundle * a.at_once + in;
-    const bool mine = in < a.at_once && token < a.all;
-    const uint32_t batch = mine ? token / a.tokens : 0, t = mine ? token - batch * a.tokens : 0;
-    const int64_t where = batch * a.pos_b + t * a.pos_t;
-    const double position =
-        a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[where] : (double)static_cast<const int32_t*>(a.positions)[where];
+  for (uint32_t item = blockIdx.x * 4 + wave; item < items; item += gridDim.x * 4) {
+    const uint32_t bundle = __builtin_amdgcn_readfirstlane(item / a.split);
+    const uint32_t batch = __builtin_amdgcn_readfirstlane(bundle / a.bundles), t0 = (bundle - batch * a.bundles) * a.at_once;
+    const bool mine = in < a.at_once && t0 + in < a.tokens;
+    const uint32_t t = mine ? in : 0;  // behind t0
+    const char* const where = a.positions + batch * a.pos_b + t0 * a.pos_t + (uint64_t)t * a.pos_t;
+    const double position = a.pos64 ? (double)*reinterpret_cast<const int64_t*>(where) : (double)*reinterpret_cast<const int32_t*>(where);
     float c[8], s[8];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      double turn = position * turns[p];
-      turn -= rint(turn);
-      sincospif(2.0f * (float)turn, &s[p], &c[p]);
+    for (uint32_t p = 0; p < 8; ++p) {
+      // in turns; the frequencies stay in the caches (in registers they would be 16 of them)
+      const bool turn = !rest && u * 8 + p < a.rotated / 2;
+      sin_cos_turns(position * (turn ? a.frequencies[u * 8 + p] * 0.15915494309189535 : 0.0), s[p], c[p]);
       s[p] *= a.sign * a.scale;
       c[p] *= rest ? 1.0f : a.scale;
     }
-    for (uint32_t row = first + share * groups; row < a.heads; row += step) {
-      if (!mine) break;
-      const bool key = row >= a.heads_q;
-      const uint32_t head = key ? row - a.heads_q : row;
-      const heads_args& h = a.part[0];
-      const heads_args& k = a.part[1];
-      auto base = [&](const void* hp, const void* kp, int64_t hb, int64_t kb, int64_t ht, int64_t kt, int64_t hh, int64_t kh) {
-        return (T*)(key ? kp : hp) + (batch * (key ? kb : hb) + t * (key ? kt : ht) + head * (key ? kh : hh));
+#pragma unroll 1
+    for (uint32_t turn = item - bundle * a.split; turn < turns; turn += a.split) {
+      const bool key = turn >= a.part[0].turns;
+      uint32_t which = __builtin_amdgcn_readfirstlane((uint32_t)key);
+      asm("" : "+s"(which));  // a part's arguments are read where they are used: both in registers were too many
+      const heads_args& h = a.part[which];
+      const uint32_t row0 = (key ? turn - a.part[0].turns : turn) * rows;
+      unit e = at;
+      if (!mine || row0 + first >= h.heads) e.n0 = e.n1 = 0;
+      const uint32_t row = e.n0 | e.n1 ? first : 0;
+      auto from = [&](const char* base, int64_t b, int64_t of_t, uint32_t of_h) {
+        return base + (batch * b + t0 * of_t + (int64_t)row0 * of_h);
       };
-      float x0[8], x1[8], d0[8], d1[8], w0[8], w1[8];
-      const T* w = NORM ? static_cast<const T*>(key ? k.w : h.w) : nullptr;
       two<T> xv, dv, wv;
-      if (!BACK || w) xv = fetch(base(h.x, k.x, h.x_b, k.x_b, h.x_t, k.x_t, h.x_h, k.x_h), at);
-      if (BACK) dv = fetch(base(h.dy, k.dy, h.dy_b, k.dy_b, h.dy_t, k.dy_t, h.dy_h, k.dy_h), at);
-      if (w) wv = fetch(w, at);
-      T* y = base(h.y, k.y, h.y_b, k.y_b, h.y_t, k.y_t, h.y_h, k.y_h);
+      xv = fetch<T>(from(h.x, h.x_b, h.x_t, h.x_h), t * (uint32_t)h.x_t + row * h.x_h, e);
+      if (BACK) dv = fetch<T>(from(h.dy, h.dy_b, h.dy_t, h.dy_h), t * (uint32_t)h.dy_t + row * h.dy_h, e);
+      if (NORM) wv = fetch<T>(h.w, 0, at);
+      char* const y = const_cast<char*>(from(h.y, h.y_b, h.y_t, h.y_h));
+      const uint32_t to = t * (uint32_t)h.y_t + row * h.y_h;
+      float x0[8], x1[8], d0[8], d1[8], w0[8], w1[8];
+      if (NORM) pairs<T, SIDE>(wv, w0, w1);
+      pairs<T, SIDE>(xv, x0, x1);
       if (BACK) {
         pairs<T, SIDE>(dv, d0, d1);
 #pragma unroll
@@ -202,48 +238,53 @@ __global__ __launch_bounds__(256) void tam_k_rotary(rotary_args a) {
           d0[p] = __builtin_fmaf(da, c[p], -d1[p] * s[p]);
           d1[p] = __builtin_fmaf(da, s[p], d1[p] * c[p]);
         }
-        float sx = 0.f, sg = 0.f;
-        if (w) {
-          pairs<T, SIDE>(xv, x0, x1);
-          pairs<T, SIDE>(wv, w0, w1);
+        {
+          float sx = 0.f, sg = 0.f;
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
+            w0[p] *= d0[p];
+            w1[p] *= d1[p];
             sx = __builtin_fmaf(x0[p], x0[p], __builtin_fmaf(x1[p], x1[p], sx));
-            sg = __builtin_fmaf(d0[p] * w0[p], x0[p], __builtin_fmaf(d1[p] * w1[p], x1[p], sg));
+            sg = __builtin_fmaf(w0[p], x0[p], __builtin_fmaf(w1[p], x1[p], sg));
           }
-        }
-        // a row's lanes are all here or none, and of one part: its sums cross no other row
-        sx = lanes_sum(sx, a.lanes);
-        sg = lanes_sum(sg, a.lanes);
-        if (w) {
-          const float rstd = 1.0f / sqrtf(__builtin_fmaf(sx, inv, a.eps)), mean = sg * inv * rstd * rstd;
+          sx = lanes_sum(sx, a.lanes);
+          sg = lanes_sum(sg, a.lanes);
+          const float rstd = inverse_root<T>(__builtin_fmaf(sx, inv, a.eps)), mean = -sg * inv * rstd * rstd * rstd;
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
-            const float g0 = d0[p] * x0[p] * rstd, g1 = d1[p] * x1[p] * rstd;
-            dw[0][p] += key ? 0.f : g0;
-            dw[0][8 + p] += key ? 0.f : g1;
-            dw[1][p] += key ? g0 : 0.f;
-            dw[1][8 + p] += key ? g1 : 0.f;
-            d0[p] = rstd * __builtin_fmaf(-x0[p], mean, d0[p] * w0[p]);
-            d1[p] = rstd * __builtin_fmaf(-x1[p], mean, d1[p] * w1[p]);
+            d0[p] *= rstd;
+            d1[p] *= rstd;
+          }
+          if (key)
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              dw[1][p] = __builtin_fmaf(d0[p], x0[p], dw[1][p]);
+              dw[1][8 + p] = __builtin_fmaf(d1[p], x1[p], dw[1][8 + p]);
+            }
+          else
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              dw[0][p] = __builtin_fmaf(d0[p], x0[p], dw[0][p]);
+              dw[0][8 + p] = __builtin_fmaf(d1[p], x1[p], dw[0][8 + p]);
+            }
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            d0[p] = __builtin_fmaf(x0[p], mean, w0[p] * rstd);
+            d1[p] = __builtin_fmaf(x1[p], mean, w1[p] * rstd);
           }
         }
-        store<T, SIDE>(y, at, d0, d1);
+        store<T, SIDE>(y, to, e, d0, d1);
       } else {
-        pairs<T, SIDE>(xv, x0, x1);
         if (NORM) {
           float sx = 0.f;
 #pragma unroll
           for (int p = 0; p < 8; ++p) sx = __builtin_fmaf(x0[p], x0[p], __builtin_fmaf(x1[p], x1[p], sx));
           sx = lanes_sum(sx, a.lanes);
-          if (w) {
-            pairs<T, SIDE>(wv, w0, w1);
-            const float rstd = 1.0f / sqrtf(__builtin_fmaf(sx, inv, a.eps));
+          const float rstd = inverse_root<T>(__builtin_fmaf(sx, inv, a.eps));
 #pragma unroll
-            for (int p = 0; p < 8; ++p) {
-              x0[p] *= rstd * w0[p];
-              x1[p] *= rstd * w1[p];
-            }
+          for (int p = 0; p < 8; ++p) {
+            x0[p] *= rstd * w0[p];
+            x1[p] *= rstd * w1[p];
           }
         }
 #pragma unroll
@@ -252,7 +293,7 @@ __global__ __launch_bounds__(256) void tam_k_rotary(rotary_args a) {
           x0[p] = __builtin_fmaf(xa, c[p], -x1[p] * s[p]);
           x1[p] = __builtin_fmaf(xa, s[p], x1[p] * c[p]);
         }
-        store<T, SIDE>(y, at, x0, x1);
+        store<T, SIDE>(y, to, e, x0, x1);
       }
     }
   }
@@ -317,7 +358,7 @@ __global__ __launch_bounds__(1024) void tam_k_rotary_weight(const float* sums, u
 // host side
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMostDim = 1024;  // a lane takes 16 elements of a head
-constexpr uint32_t kMostGroups = 512;  // whose sums tam_k_rotary_weight adds
+constexpr uint32_t kMostGroups = 768;  // whose sums tam_k_rotary_weight adds
 
 uint32_t power_of_two(uint32_t n) {
   uint32_t p = 1;
@@ -350,6 +391,10 @@ int check_rotary(const TamRotary* d, bool back) {
     if (!h->heads) continue;
     if (!h->y || (!back && !h->x) || (back && (!h->dy || (h->w && !h->x))))
       return tam_op_fail(TAM_E_INVALID, "null heads");
+    const uint64_t size = d->dtype == TAM_DTYPE_F32 ? 4 : 2, far = (1ull << 31) / size / 64;  // a lane's offsets are 32-bit numbers of bytes
+    for (const int64_t stride : {h->x_h, h->y_h, h->dy_h})
+      if (stride < 0 || (uint64_t)stride >= far)
+        return tam_op_fail(TAM_E_UNSUPPORTED, "heads %lld elements apart", (long long)stride);
     if (back && h->dw && !h->w) return tam_op_fail(TAM_E_INVALID, "a gradient of a weight that is not given");
   }
   return TAM_OK;
@@ -362,12 +407,22 @@ uint32_t plan(const TamRotary* d, bool back, rotary_args& a) {
   a.units = units_of(d);
   a.lanes = power_of_two(a.units);
   a.tokens = (uint32_t)d->tokens;
-  a.all = (uint32_t)(d->batch * d->tokens);
-  a.heads_q = (uint32_t)d->q.heads;
-  a.heads = (uint32_t)(d->q.heads + d->k.heads);
+  a.batches = (uint32_t)d->batch;
   const uint32_t groups = 64 / a.lanes;
-  a.at_once = a.heads < groups ? groups / a.heads : 1;
-  const uint64_t bundles = tam_div_up(a.all, a.at_once), turns = tam_div_up(a.heads, groups);
+  const uint64_t most_heads = d->q.heads > d->k.heads ? d->q.heads : d->k.heads;
+  // several tokens to a wave, unless they lie too far apart for a lane's 32-bit offsets
+  const int64_t size = d->dtype == TAM_DTYPE_F32 ? 4 : 2, far = (1ll << 31) / size / 64;
+  bool near = true;
+  for (const TamHeads* h : {&d->q, &d->k})
+    for (const int64_t stride : {h->x_t, h->y_t, h->dy_t}) near = near && (!h->heads || (stride >= 0 && stride < far));
+  a.at_once = 1;
+  if (near)
+    while (2 * a.at_once * most_heads <= groups && a.at_once < a.tokens) a.at_once *= 2;
+  const uint32_t rows = groups / a.at_once;
+  a.bundles = (uint32_t)tam_div_up(a.tokens, a.at_once);
+  a.part[0].turns = (uint32_t)tam_div_up(d->q.heads, rows);
+  a.part[1].turns = (uint32_t)tam_div_up(d->k.heads, rows);
+  const uint64_t bundles = (uint64_t)a.bundles * a.batches, turns = a.part[0].turns + a.part[1].turns;
   // few tokens: their heads go to waves of their own, until 16 waves are on every compute unit
   const uint64_t room = 16ull * tam_op_cus();
   a.split = (uint32_t)(bundles >= room ? 1 : (room / bundles < turns ? room / bundles : turns));
@@ -403,18 +458,30 @@ __global__ __launch_bounds__(256) void tam_k_rotary_zero(T* out, uint32_t n) {
   if (i < n) out[i] = (T)0.0f;
 }
 
+int launch(const TamRotary* d, bool back, void* workspace, hipStream_t s);
+
+bool normed(const TamHeads& h) { return h.heads && h.w; }
+
+// One part of a call of which the other has no norm, or has one alone.
+TamRotary part_of(const TamRotary* d, bool keys) {
+  TamRotary one = *d;
+  TamHeads& other = keys ? one.q : one.k;
+  other = TamHeads{};
+  return one;
+}
+
 int rotary(const TamRotary* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need) {
-  const int rc = check_rotary(d, back);
+  int rc = check_rotary(d, back);
   if (rc != TAM_OK) return rc;
   const hipStream_t s = (hipStream_t)stream;
   const bool empty = d->batch == 0 || d->tokens == 0 || d->q.heads + d->k.heads == 0;
-  rotary_args a = {};
-  uint32_t wgs = 0;
+  const bool apart = d->q.heads && d->k.heads && normed(d->q) != normed(d->k);
   uint64_t used = 0;
-  const bool norm = (d->q.w && d->q.heads) || (d->k.w && d->k.heads), sums = back && norm && (d->q.dw || d->k.dw);
-  if (!empty) {
-    wgs = plan(d, back, a);
-    if (sums) used = (uint64_t)wgs * 2 * a.lanes * 16 * 4;
+  if (!empty && back && ((normed(d->q) && d->q.dw) || (normed(d->k) && d->k.dw))) {
+    rotary_args a = {};
+    const TamRotary one = part_of(d, normed(d->k));
+    const uint32_t wgs = plan(apart ? &one : d, back, a);
+    used = (uint64_t)wgs * 2 * a.lanes * 16 * 4;
   }
   if (need) {
     *need = used;
@@ -435,28 +502,43 @@ int rotary(const TamRotary* d, bool back, void* workspace, uint64_t ws_bytes, vo
         TAM_OP_LAUNCHED("the weights' gradients");
       }
   if (empty) return TAM_OK;
+  if (!apart) return launch(d, back, workspace, s);
+  for (const bool keys : {false, true}) {
+    const TamRotary one = part_of(d, keys);
+    rc = launch(&one, back, workspace, s);
+    if (rc != TAM_OK) return rc;
+  }
+  return TAM_OK;
+}
+
+int launch(const TamRotary* d, bool back, void* workspace, hipStream_t s) {
+  rotary_args a = {};
+  const uint32_t wgs = plan(d, back, a);
+  const bool norm = normed(d->q) || normed(d->k), sums = back && norm && (d->q.dw || d->k.dw);
   const bool turned = back && !norm;  // the forward pass of dy with the angles' sign turned
+  const int64_t size = d->dtype == TAM_DTYPE_F32 ? 4 : 2;
   int i = 0;
   for (const TamHeads* h : {&d->q, &d->k}) {
     heads_args& p = a.part[i++];
-    p.x = turned ? h->dy : h->x;
-    p.w = h->w;
-    p.dy = h->dy;
-    p.y = h->y;
-    p.x_b = turned ? h->dy_b : h->x_b;
-    p.x_t = turned ? h->dy_t : h->x_t;
-    p.x_h = turned ? h->dy_h : h->x_h;
-    p.dy_b = h->dy_b;
-    p.dy_t = h->dy_t;
-    p.dy_h = h->dy_h;
-    p.y_b = h->y_b;
-    p.y_t = h->y_t;
-    p.y_h = h->y_h;
+    p.x = (const char*)(turned ? h->dy : h->x);
+    p.w = (const char*)h->w;
+    p.dy = (const char*)h->dy;
+    p.y = (char*)h->y;
+    p.x_b = (turned ? h->dy_b : h->x_b) * size;
+    p.x_t = (turned ? h->dy_t : h->x_t) * size;
+    p.x_h = (uint32_t)((turned ? h->dy_h : h->x_h) * size);
+    p.dy_b = h->dy_b * size;
+    p.dy_t = h->dy_t * size;
+    p.dy_h = (uint32_t)(h->dy_h * size);
+    p.y_b = h->y_b * size;
+    p.y_t = h->y_t * size;
+    p.y_h = (uint32_t)(h->y_h * size);
+    p.heads = (uint32_t)h->heads;
   }
-  a.positions = d->positions;
+  a.positions = (const char*)d->positions;
   a.frequencies = d->frequencies;
-  a.pos_b = d->pos_b;
-  a.pos_t = d->pos_t;
+  a.pos_b = d->pos_b * (d->positions64 ? 8 : 4);
+  a.pos_t = d->pos_t * (d->positions64 ? 8 : 4);
   a.pos64 = d->positions64;
   a.eps = d->eps;
   a.scale = d->magnitude;
