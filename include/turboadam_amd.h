@@ -467,8 +467,9 @@ typedef struct TamCross {
 size_t tam_cross_kept(uint64_t rows);
 /* Bytes of workspace (256-byte aligned) of the two calls below. */
 int tam_cross_workspace(const TamCross* d, int backward_pass, size_t* bytes);
-/* How their products are cut (as tam_linear_tiles tells it): tiles[0] the tile of z, [1] the
- * columns of a piece (forward: 0), [2] the tile of dx, [3] of dw. */
+/* How their products are cut (as tam_linear_tiles tells it): tiles[0] the tile of z; backward:
+ * [1] the columns of a piece, [2] the tile of dx and dw, [3] the parts of their sums, dx's
+ * times 2^16 and dw's. */
 int tam_cross_tiles(const TamCross* d, int backward_pass, uint32_t* tiles);
 int tam_cross(const TamCross* d, void* workspace, size_t ws_bytes, void* stream);
 /* dx and dw (those that are not NULL). */

@@ -880,15 +880,16 @@ def _cross_tiles(m, k, v, dt, backward):
     return list(out)
 
 
-@pytest.mark.parametrize("m,k,v,dt,z,dx,dw", [
-    (4096, 264, 9973, "bf16", 256, 128, 128), (4096, 1032, 9973, "f16", 256, 256, 256), (1000, 300, 2100, "bf16", 64, 64, 64),
-    (8192, 40, 2100, "f16", 128, 64, 64), (4000, 1024, 4000, "f32", 128, 128, 128), (200, 100, 700, "f32", 64, 64, 64)])
-def test_cross_tiles(m, k, v, dt, z, dx, dw):
+@pytest.mark.parametrize("m,k,v,dt,z,both,x_parts,w_parts", [
+    (4096, 264, 9973, "bf16", 256, 128, 2, 1), (4096, 1032, 9973, "f16", 256, 256, 3, 1), (1000, 300, 2100, "bf16", 64, 64, 2, 1),
+    (8192, 40, 2100, "f16", 128, 64, 2, 8), (4000, 1024, 4000, "f32", 128, 128, 1, 1), (200, 100, 700, "f32", 64, 64, 2, 1),
+    (8192, 768, 20011, "bf16", 256, 256, 2, 1), (5000, 24, 40, "f32", 64, 64, 1, 32)])
+def test_cross_tiles(m, k, v, dt, z, both, x_parts, w_parts):
     got = _cross_tiles(m, k, v, dt, 1)
     log(f"cross {m}x{k}x{v} {dt} tiles {_cross_tiles(m, k, v, dt, 0)} and {got}")
-    assert _cross_tiles(m, k, v, dt, 0)[0] == z and [got[0], *got[2:]] == [z, dx, dw]
-    for ignored in (0.0, 0.6):
-        _check_cross(*_cross_case(m, k, v, dt, ignored), dt, "mean" if ignored else "none")
+    assert _cross_tiles(m, k, v, dt, 0)[0] == z and [got[0], *got[2:]] == [z, both, x_parts << 16 | w_parts]
+    for ignored in (0.0, 0.6, 0.95):  # where few rows count, dx's sums are cut into more parts
+        _check_cross(*_cross_case(m, k, v, dt, ignored), dt, "none" if ignored == 0.6 else "mean")
 
 
 def _whole(g, *shape):

@@ -575,30 +575,49 @@ __global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a
 
 struct cross_product_args {
   tam_operand P, Q;
-  uint64_t k, k_part;      // dw: k is the rows that count, k_part of all rows
-  uint32_t tm, tn;
-  const uint32_t* count;
-  const float* scale;
+  uint64_t k, most_k;      // dx: of this piece, and of the widest one
+  uint32_t tm, tn, parts;  // tiles (of all rows), and what a sum is cut into
   uint32_t rows, cols;
   float* sums;             // [part][rows][cols], or null: dw's own
   bool add;                // to what the sums hold
   void* dw;
 };
 
+// A piece's products: units of dw, then units of dx's share, in one launch, so that neither leaves
+// compute units empty at its end.
+struct cross_products_args {
+  cross_product_args w, x;
+  uint32_t w_units;        // of w.tm * w.tn * w.parts
+  const uint32_t* count;
+  const float* scale;
+};
+
+// Into how many parts dx's sums are cut where `count` of `rows` count: as many as there is room
+// for, in the sums and in the launch, which were laid out for all of them.
+__device__ __forceinline__ uint32_t cross_parts(uint32_t parts, uint32_t rows, uint32_t count, uint32_t tile, uint64_t k) {
+  if (parts == 1 || count == 0) return parts;
+  const uint32_t all = (rows + tile - 1) / tile, now = (count + tile - 1) / tile;
+  const uint64_t room = (uint64_t)parts * rows / count, launch = (uint64_t)parts * all / now, least = k / 256;
+  uint64_t n = room < launch ? room : launch;
+  if (n > least) n = least;
+  return n > parts ? (uint32_t)n : parts;
+}
+
 // dx's share of a piece (WEIGHT false: fp32 sums) or the piece's rows of dw.
 template <typename T, int TILE, int WM, int WN, bool WEIGHT>
-__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_product(cross_product_args a) {
+__device__ __forceinline__ void cross_product(cross_product_args& a, uint32_t unit, uint32_t count, const float* of_scale,
+                                              char* smem) {
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, !WEIGHT> Tile;
-  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
-  const uint32_t count = *a.count;
+  const uint32_t rows = WEIGHT ? a.rows : count, tm = (rows + TILE - 1) / TILE, tiles = tm * a.tn;
+  const uint32_t parts = WEIGHT ? a.parts : cross_parts(a.parts, a.rows, count, TILE, a.most_k);
+  if (unit >= tiles * parts) return;
+  const uint32_t part = unit / tiles;
   uint32_t m, n;
-  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
-  const uint32_t rows = WEIGHT ? a.rows : count;
-  if (m * TILE >= rows) return;
+  tam_tile_at(tam_xcd_order(unit - part * tiles, tiles), tm, a.tn, m, n);
   if (!WEIGHT) a.Q.count = count;
-  const uint64_t k = WEIGHT ? count : a.k, k0 = blockIdx.y * a.k_part;
-  const uint64_t k1 = k0 + a.k_part < k ? k0 + a.k_part : k;
-  float* sums = a.sums ? a.sums + (uint64_t)blockIdx.y * a.rows * a.cols : nullptr;
+  const uint64_t k = WEIGHT ? count : a.k, per = parts > 1 ? (k / parts + 64) / 64 * 64 : k;
+  const uint64_t k0 = part * per < k ? part * per : k, k1 = k0 + per < k ? k0 + per : k;
+  float* const sums = a.sums ? a.sums + (uint64_t)part * rows * a.cols : nullptr;
   Tile t;
   t.zero();
   tam_soon soon = {};
@@ -608,7 +627,7 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_
             TILE * 4};
   }
   t.run(a.P, a.Q, n * TILE, m * TILE, k0, k1, smem, soon);
-  const float scale = WEIGHT ? *a.scale : 1.0f;
+  const float scale = WEIGHT ? *of_scale : 1.0f;
   t.template each<TAM_AHEAD_PASS>(
       smem,
       [&](uint32_t row, uint32_t col) {
@@ -638,11 +657,28 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_
       [](uint32_t, uint32_t, const float*, int) {});
 }
 
+template <typename T, int TILE, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_products(cross_products_args a) {
+  typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, true> Tile;
+  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+  const uint32_t count = *a.count;
+  if (blockIdx.x < a.w_units)
+    cross_product<T, TILE, WM, WN, true>(a.w, blockIdx.x, count, a.scale, smem);
+  else
+    cross_product<T, TILE, WM, WN, false>(a.x, blockIdx.x - a.w_units, count, a.scale, smem);
+}
+
 // out[row] = the parts' sums of the row's number in their order, times scale; zeros for
-// rows that do not count. place == null: a row's number is its own.
+// rows that do not count. place == null: a row's number is its own. tile, k: dx's.
 template <typename T>
 __global__ __launch_bounds__(256) void tam_k_cross_out(const float* sums, uint32_t parts, uint64_t rows, uint32_t cols,
-                                                       const int32_t* place, const float* scale, T* out) {
+                                                       const int32_t* place, const uint32_t* count, uint32_t tile, uint64_t k,
+                                                       const float* scale, T* out) {
+  uint64_t summed = rows;
+  if (place) {
+    summed = *count;
+    parts = cross_parts(parts, (uint32_t)rows, (uint32_t)summed, tile, k);
+  }
   const uint32_t per = (cols + 7) / 8;
   const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= per * rows) return;
@@ -654,7 +690,7 @@ __global__ __launch_bounds__(256) void tam_k_cross_out(const float* sums, uint32
     const float s = *scale;
     for (uint32_t p = 0; p < parts; ++p) {
       float t[8];
-      tam_load_some(sums + (p * rows + at) * cols + col, cols - col, t);
+      tam_load_some(sums + (p * summed + at) * cols + col, cols - col, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += t[j];
     }
@@ -758,18 +794,72 @@ void launch_logits(int tile, const cross_logits_args& a, hipStream_t s) {
     hipLaunchKernelGGL((tam_k_cross_logits<T, 64, 2, 2, BACK>), grid, dim3(256), 0, s, a);
 }
 
-template <typename T, bool WEIGHT>
-void launch_product(int tile, const cross_product_args& a, uint32_t parts, hipStream_t s) {
-  const dim3 grid(a.tm * a.tn, parts);
+template <typename T>
+void launch_products(int tile, const cross_products_args& a, uint32_t units, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
     if (tile == 256) {
-      hipLaunchKernelGGL((tam_k_cross_product<T, 256, 2, 4, WEIGHT>), grid, dim3(512), 0, s, a);
+      hipLaunchKernelGGL((tam_k_cross_products<T, 256, 2, 4>), dim3(units), dim3(512), 0, s, a);
       return;
     }
   if (tile == 128)
-    hipLaunchKernelGGL((tam_k_cross_product<T, 128, 2, 2, WEIGHT>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((tam_k_cross_products<T, 128, 2, 2>), dim3(units), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((tam_k_cross_product<T, 64, 2, 2, WEIGHT>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((tam_k_cross_products<T, 64, 2, 2>), dim3(units), dim3(256), 0, s, a);
+}
+
+// A piece's two products in one launch: their tile and parts.
+struct pair_shape {
+  int tile;
+  uint32_t w_parts, x_parts;
+};
+
+// us of n units of k one after another on the places of a card, behind `ahead` units of `ahead_k`
+// (the longer first): each unit to the place that is free first.
+double units_us(const tam_tile_rate& t, uint64_t n1, double k1, uint64_t n2, double k2, double cus) {
+  if (k1 < k2) return n2 ? units_us(t, n2, k2, n1, k1, cus) : units_us(t, n1, k2, 0, 0, cus);
+  const uint64_t places = (uint64_t)cus * t.resident, all = n1 + n2;
+  const int with = all >= places ? t.resident : (int)tam_div_up(all ? all : 1, (uint64_t)cus);  // on a compute unit
+  const double per = all <= (uint64_t)(0.5 * cus) ? t.half : t.per_k[with - 1];
+  const double d1 = 0.5 * t.start + k1 * per, d2 = 0.5 * t.start + k2 * per;
+  // two kinds of places: `late` of them have one unit more
+  uint64_t late = n1 % places, rounds = n1 / places;
+  double early_at = rounds * d1, late_at = late ? early_at + d1 : early_at;
+  uint64_t early = places - late;
+  while (n2) {
+    double& at = early_at <= late_at || !late ? early_at : late_at;
+    const uint64_t here = &at == &early_at ? early : late, take = n2 < here ? n2 : here;
+    if (take < here) return 0.5 * t.start + (at + d2 > late_at ? at + d2 : late_at);
+    at += d2;
+    n2 -= take;
+  }
+  return 0.5 * t.start + (late && late_at > early_at ? late_at : early_at);
+}
+
+pair_shape choose_pair(uint64_t rows, uint64_t inputs, uint64_t words, bool dw, bool dx, uint32_t dtype) {
+  const double cus = tam_op_cus();
+  const bool f32 = dtype == TAM_DTYPE_F32;
+  const tam_tile_rate* rate = f32 ? tam_rates_32 : tam_rates_16;
+  pair_shape best = {64, 1, 1};
+  double least = 1e30;
+  for (int i = 0; i < (f32 ? 2 : 3); ++i) {
+    const uint64_t t = rate[i].tile, across = tam_div_up(inputs, t);
+    for (uint32_t wp : {1, 2, 4, 8, 16, 32}) {
+      if (wp > 1 && (!dw || rows / wp < 128)) break;
+      for (uint32_t xp : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (xp > 1 && (!dx || words / xp < 256)) break;
+        const uint64_t nw = dw ? tam_div_up(words, t) * across * wp : 0, nx = dx ? tam_div_up(rows, t) * across * xp : 0;
+        double us = units_us(rate[i], nw, (double)rows / wp, nx, (double)words / xp, cus);
+        // parts' sums to memory and back (about 4 TB/s): dx's are there in any case, and added to
+        us += (double)rows * inputs * 8.0 * (dx ? xp : 0) / 4e6;
+        if (wp > 1) us += 3.0 + (double)words * inputs * 8.0 * wp / 4e6;
+        if (us < least) {
+          least = us;
+          best = {rate[i].tile, wp, xp};
+        }
+      }
+    }
+  }
+  return best;
 }
 
 // The tile of a product that is not cut into parts.
@@ -885,12 +975,51 @@ int forward(const TamCross* d, call& c) {
   return TAM_OK;
 }
 
-// Columns of a piece: as even as they come, in whole tiles, of at most kPieceBytes of dz.
+// us of the backward pass in pieces of `piece` columns.
+double pieces_us(const TamCross* d, uint64_t piece) {
+  const double cus = tam_op_cus();
+  const bool f32 = d->dtype == TAM_DTYPE_F32;
+  const pair_shape p = choose_pair(d->rows, d->inputs, piece < d->vocabulary ? piece : d->vocabulary, d->dw, d->dx, d->dtype);
+  const int tile = tile_of(d->rows, piece, d->inputs, d->dtype);
+  const tam_tile_rate *rate = f32 ? tam_rates_32 : tam_rates_16, *z = rate, *t = rate;
+  while (z->tile != tile) ++z;
+  while (t->tile != p.tile) ++t;
+  double us = 0;
+  const uint64_t across = tam_div_up(d->inputs, t->tile);
+  for (uint64_t first = 0, cols; first < d->vocabulary; first += cols) {
+    cols = d->vocabulary - first < piece ? d->vocabulary - first : piece;
+    us += tam_tiles_us(*z, (double)tam_div_up(d->rows, tile) * (double)tam_div_up(cols, tile), (double)d->inputs, cus);
+    us += units_us(*t, d->dw ? tam_div_up(cols, t->tile) * across * p.w_parts : 0, (double)d->rows / p.w_parts,
+                   d->dx ? tam_div_up(d->rows, t->tile) * across * p.x_parts : 0, (double)cols / p.x_parts, cus);
+    us += 6.0 + (double)d->rows * d->inputs * 8.0 * (d->dx ? p.x_parts : 0) / 4e6;
+  }
+  return us;
+}
+
+// Columns of a piece, of at most kPieceBytes of dz: as even as they come, in whole tiles; or, where
+// products are long enough for the choice to pay for itself, what is estimated to take the
+// least time of a few numbers of pieces and of pieces whose dw fills the card's rounds. (8192 x 768 of
+// 50257 bf16: two even pieces, 2.26 ms.)
 uint64_t piece_of(const TamCross* d, uint32_t size) {
   if (d->piece) return d->piece;
   uint64_t most = kPieceBytes / (d->rows * size) / 256 * 256;
   most = most < 256 ? 256 : (most > kMostPiece ? kMostPiece : most);
-  return tam_up(tam_div_up(d->vocabulary, tam_div_up(d->vocabulary, most)), 256);
+  const uint64_t fewest = tam_div_up(d->vocabulary, most);
+  uint64_t best = tam_up(tam_div_up(d->vocabulary, fewest), 256);
+  if ((double)d->rows * (double)d->inputs * (double)d->vocabulary < 2e11 || (!d->dx && !d->dw)) return best;
+  double least = pieces_us(d, best);
+  auto consider = [&](uint64_t piece) {
+    if (piece < 1024 || piece > most) return;
+    const double us = pieces_us(d, piece);
+    if (us < 0.98 * least) {
+      least = us;
+      best = piece;
+    }
+  };
+  for (uint64_t n = fewest + 1; n < fewest + 4; ++n) consider(tam_up(tam_div_up(d->vocabulary, n), 256));
+  const uint64_t across = tam_div_up(d->inputs, 256);
+  for (uint64_t rounds = 1; rounds <= 4; ++rounds) consider(tam_op_cus() * rounds / across * 256);
+  return best;
 }
 
 int zero(const call& c, void* p, uint64_t elements) {
@@ -921,15 +1050,16 @@ int backward(const TamCross* d, call& c) {
   const uint32_t ld = aligned_ld((uint32_t)widest, size);
   void* dz = c.ws.take((uint64_t)rows * ld * size);
   const int tile_z = tile_of(rows, widest, inputs, c.dtype);
-  const shape sx = choose(rows, inputs, widest, c.dtype), sw = choose(widest, inputs, rows, c.dtype);
+  const pair_shape both = choose_pair(rows, inputs, widest, d->dw, d->dx, c.dtype);
   if (c.tiles) {
     c.tiles[0] = (uint32_t)tile_z;
     c.tiles[1] = (uint32_t)piece;
-    if (d->dx) c.tiles[2] = (uint32_t)sx.tile;
-    if (d->dw) c.tiles[3] = (uint32_t)sw.tile;
+    c.tiles[2] = (uint32_t)both.tile;
+    c.tiles[3] = both.x_parts << 16 | both.w_parts;
   }
-  float* dx_sums = d->dx ? (float*)c.ws.take(4ull * sx.parts * rows * inputs) : nullptr;
-  float* dw_sums = d->dw && sw.parts > 1 ? (float*)c.ws.take(4ull * sw.parts * widest * inputs) : nullptr;
+  float* dx_sums = d->dx ? (float*)c.ws.take(4ull * both.x_parts * rows * inputs) : nullptr;
+  float* dw_sums = d->dw && both.w_parts > 1 ? (float*)c.ws.take(4ull * both.w_parts * widest * inputs) : nullptr;
+  const uint32_t across = (uint32_t)tam_div_up(inputs, both.tile);
   if (c.dry) return TAM_OK;
   for (uint64_t first = 0; first < d->vocabulary; first += piece) {
     const uint32_t cols = (uint32_t)(d->vocabulary - first < piece ? d->vocabulary - first : piece);
@@ -942,55 +1072,57 @@ int backward(const TamCross* d, call& c) {
     TAM_OF_TYPE(c, TAM_DZ);
     TAM_OP_LAUNCHED("the logits' gradient");
     const matrix z = {dz, ld, rows, cols, true};
-    if (d->dx) {
-      cross_product_args p = {};
-      p.P = operand_of(w, inputs, size);
-      p.P.base += first * w.ld * size;
-      p.Q = operand_of(z, rows, size);
-      p.k = cols;
-      p.k_part = sx.parts > 1 ? tam_up(tam_div_up(cols, sx.parts), 64) : cols;
-      p.tm = (uint32_t)tam_div_up(rows, sx.tile);
-      p.tn = (uint32_t)tam_div_up(inputs, sx.tile);
-      p.count = r.count;
-      p.scale = scale;
-      p.rows = rows;
-      p.cols = inputs;
-      p.sums = dx_sums;
-      p.add = first != 0;
-#define TAM_DX(T) launch_product<T, false>(sx.tile, p, sx.parts, c.stream)
-      TAM_OF_TYPE(c, TAM_DX);
-      TAM_OP_LAUNCHED("dx");
-    }
+    cross_products_args p = {};
+    p.count = r.count;
+    p.scale = scale;
+    uint64_t units = 0;
     if (d->dw) {
-      cross_product_args p = {};
-      p.P = operand_of(x, inputs, size);
-      p.Q = operand_of(z, cols, size);
-      p.k = rows;
-      p.k_part = sw.parts > 1 ? tam_up(tam_div_up(rows, sw.parts), 64) : rows;
-      p.tm = (uint32_t)tam_div_up(cols, sw.tile);
-      p.tn = (uint32_t)tam_div_up(inputs, sw.tile);
-      p.count = r.count;
-      p.scale = scale;
-      p.rows = cols;
-      p.cols = inputs;
-      p.sums = dw_sums;
-      p.dw = (char*)d->dw + first * inputs * size;
-#define TAM_DW(T) launch_product<T, true>(sw.tile, p, sw.parts, c.stream)
-      TAM_OF_TYPE(c, TAM_DW);
-      TAM_OP_LAUNCHED("dw");
-      if (dw_sums) {
-        const dim3 grid((uint32_t)tam_div_up((uint64_t)cols * tam_div_up(inputs, 8), 256)), block(256);
-#define TAM_DW_OUT(T) \
-  hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dw_sums, sw.parts, (uint64_t)cols, inputs, nullptr, scale, (T*)p.dw)
-        TAM_OF_TYPE(c, TAM_DW_OUT);
-        TAM_OP_LAUNCHED("dw's sum");
-      }
+      p.w.P = operand_of(x, inputs, size);
+      p.w.Q = operand_of(z, cols, size);
+      p.w.tm = (uint32_t)tam_div_up(cols, both.tile);
+      p.w.tn = across;
+      p.w.parts = both.w_parts;
+      p.w.rows = cols;
+      p.w.cols = inputs;
+      p.w.sums = dw_sums;
+      p.w.dw = (char*)d->dw + first * inputs * size;
+      units = (uint64_t)p.w.tm * across * both.w_parts;
+      p.w_units = (uint32_t)units;
+    }
+    if (d->dx) {
+      p.x.P = operand_of(w, inputs, size);
+      p.x.P.base += first * w.ld * size;
+      p.x.Q = operand_of(z, rows, size);
+      p.x.k = cols;
+      p.x.most_k = widest;
+      p.x.tm = (uint32_t)tam_div_up(rows, both.tile);
+      p.x.tn = across;
+      // a last piece of few words has fewer 64s to cut than parts: the others are empty sums
+      p.x.parts = both.x_parts;
+      p.x.rows = rows;
+      p.x.cols = inputs;
+      p.x.sums = dx_sums;
+      p.x.add = first != 0;
+      units += (uint64_t)p.x.tm * across * both.x_parts;
+    }
+    if (units >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+#define TAM_PRODUCTS(T) launch_products<T>(both.tile, p, (uint32_t)units, c.stream)
+    TAM_OF_TYPE(c, TAM_PRODUCTS);
+    TAM_OP_LAUNCHED("dx and dw");
+    if (dw_sums) {
+      const dim3 grid((uint32_t)tam_div_up((uint64_t)cols * tam_div_up(inputs, 8), 256)), block(256);
+#define TAM_DW_OUT(T)                                                                                                     \
+  hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dw_sums, both.w_parts, (uint64_t)cols, inputs, nullptr, \
+                     nullptr, 0u, 0ull, scale, (T*)p.w.dw)
+      TAM_OF_TYPE(c, TAM_DW_OUT);
+      TAM_OP_LAUNCHED("dw's sum");
     }
   }
   if (d->dx) {
     const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * tam_div_up(inputs, 8), 256)), block(256);
-#define TAM_DX_OUT(T) \
-  hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dx_sums, sx.parts, (uint64_t)rows, inputs, r.place, scale, (T*)d->dx)
+#define TAM_DX_OUT(T)                                                                                                        \
+  hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dx_sums, both.x_parts, (uint64_t)rows, inputs, r.place, \
+                     r.count, (uint32_t)both.tile, widest, scale, (T*)d->dx)
     TAM_OF_TYPE(c, TAM_DX_OUT);
     TAM_OP_LAUNCHED("dx's sum");
   }
