@@ -103,7 +103,7 @@ def _check_gated(x, wg, wu, dh, dt, act):
              "dup": (du.t() @ X, du_err.t() @ X.abs() + _sum_error(m) * (du.abs().t() @ X.abs()))}
     for (name, (v, err)), got in zip(names.items(), grads):
         _within(got, v, u * v.abs() + (1 + u) * err + t, name)
-    if wg.stride() == wu.stride():
+    if wg.stride() == wu.stride() and (wg.is_contiguous() or wg.t().is_contiguous()):
         for got in grads[1:]:
             assert got.stride() == wg.stride() or 1 in wg.shape
 
@@ -174,6 +174,23 @@ def test_gated_views_and_weights_of_two_layouts(rows, dt):
     for a, b in zip(torch.autograd.grad(gated_linear(*leaves), leaves, dh),
                     torch.autograd.grad(gated_linear(*mixed), mixed, dh)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("in_out", [False, True])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_gated_one_weight_at_an_odd_address(dt, in_out):
+    """Rows of whole 16 bytes, a stride of their own, and only one of the weights on 4 bytes."""
+    x, wg, wu, dh = _gated_case(70, 64, 48, dt, in_out)
+    for off, of_gate in ((0, 1), (1, 0)):
+        views = []
+        for w, at in ((wg, of_gate), (wu, off)):
+            m = w.t() if in_out else w
+            flat = torch.full((m.shape[0] * 80 + 2,), float("nan"), device="cuda", dtype=w.dtype)
+            v = flat[at:at + m.shape[0] * 80].view(m.shape[0], 80)[:, :m.shape[1]]
+            v.copy_(m)
+            views.append(v.t() if in_out else v)
+        log(f"gated odd address {dt} in_out={in_out}")
+        _check_gated(x, *views, dh, dt, "silu")
 
 
 @pytest.mark.parametrize("m,k,n", [(0, 8, 8), (5, 0, 9), (40, 0, 9), (5, 8, 0), (40, 8, 0), (0, 0, 4)])
@@ -856,14 +873,15 @@ def test_gated_tiles_forward(m, k, n, dt, tiles):
     _check_gated(*_gated_case(m, k, n, dt), dt, "silu")
 
 
-@pytest.mark.parametrize("m,k,n,dt,in_out,dx,dw", [
-    (6000, 2048, 3000, "bf16", False, 256, 256), (6000, 2048, 3000, "f16", True, 256, 256),
-    (2048, 2048, 4096, "bf16", False, 128, 256), (300, 200, 200, "bf16", True, 64, 64),
-    (1024, 1024, 2048, "f32", False, 64, 64)])
-def test_gated_tiles_backward(m, k, n, dt, in_out, dx, dw):
+@pytest.mark.parametrize("m,k,n,dt,in_out,tile,x_parts,w_parts", [
+    (6000, 2048, 3000, "bf16", False, 128, 1, 1), (6000, 2048, 3000, "f16", True, 128, 1, 1),
+    (2048, 2048, 4096, "bf16", False, 256, 2, 1), (2048, 2048, 4096, "f16", True, 256, 2, 1),
+    (300, 200, 200, "bf16", True, 64, 1, 1), (1024, 1024, 2048, "f32", False, 128, 4, 1),
+    (5000, 40, 60, "bf16", False, 64, 1, 32)])
+def test_gated_tiles_backward(m, k, n, dt, in_out, tile, x_parts, w_parts):
     got = _gated_tiles(m, k, n, dt, 1, in_out)
     log(f"gated {m}x{k}x{n} {dt} in_out={in_out} tiles {got}")
-    assert (got[0], got[2]) == (dx, dw)
+    assert got == [tile, x_parts, tile, w_parts]
     _check_gated(*_gated_case(m, k, n, dt, in_out), dt, "gelu")
 
 

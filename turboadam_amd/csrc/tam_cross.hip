@@ -766,7 +766,7 @@ int number_rows(const TamCross* d, const cross_rows& r, float* loss, hipStream_t
 int operands(const TamCross* d, call& c, const cross_rows& r, matrix& x, matrix& w) {
   const uint32_t size = kSize[c.dtype], halves = size / 2, inputs = (uint32_t)d->inputs;
   w = matrix_of(d->w, d->ldw, d->vocabulary, d->inputs, size);
-  const int rc = whole_rows(c, w);
+  const int rc = whole_rows(c, {&w});
   if (rc != TAM_OK) return rc;
   const uint32_t ld = aligned_ld(inputs, size);
   x = {c.ws.take(d->rows * ld * size), ld, d->rows, inputs, true};
@@ -812,28 +812,6 @@ struct pair_shape {
   int tile;
   uint32_t w_parts, x_parts;
 };
-
-// us of n units of k one after another on the places of a card, behind `ahead` units of `ahead_k`
-// (the longer first): each unit to the place that is free first.
-double units_us(const tam_tile_rate& t, uint64_t n1, double k1, uint64_t n2, double k2, double cus) {
-  if (k1 < k2) return n2 ? units_us(t, n2, k2, n1, k1, cus) : units_us(t, n1, k2, 0, 0, cus);
-  const uint64_t places = (uint64_t)cus * t.resident, all = n1 + n2;
-  const int with = all >= places ? t.resident : (int)tam_div_up(all ? all : 1, (uint64_t)cus);  // on a compute unit
-  const double per = all <= (uint64_t)(0.5 * cus) ? t.half : t.per_k[with - 1];
-  const double d1 = 0.5 * t.start + k1 * per, d2 = 0.5 * t.start + k2 * per;
-  // two kinds of places: `late` of them have one unit more
-  uint64_t late = n1 % places, rounds = n1 / places;
-  double early_at = rounds * d1, late_at = late ? early_at + d1 : early_at;
-  uint64_t early = places - late;
-  while (n2) {
-    double& at = early_at <= late_at || !late ? early_at : late_at;
-    const uint64_t here = &at == &early_at ? early : late, take = n2 < here ? n2 : here;
-    if (take < here) return 0.5 * t.start + (at + d2 > late_at ? at + d2 : late_at);
-    at += d2;
-    n2 -= take;
-  }
-  return 0.5 * t.start + (late && late_at > early_at ? late_at : early_at);
-}
 
 pair_shape choose_pair(uint64_t rows, uint64_t inputs, uint64_t words, bool dw, bool dx, uint32_t dtype) {
   const double cus = tam_op_cus();

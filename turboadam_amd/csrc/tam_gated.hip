@@ -16,7 +16,7 @@
 //   tam_k_gated_slope dg and du, side by side in one row: then dgate and dup are one
 //                    product of twice the rows, and dx is one sum of twice the length
 //                    (TAM_TWO_PRODUCTS);
-//   tam_k_gated_product, tam_k_gated_sum  those products.
+//   tam_k_gated_products, tam_k_gated_sum  those two products, in one launch.
 #include "tam_act.h"
 #include "tam_few.h"
 #include "tam_products.h"
@@ -337,29 +337,47 @@ struct gated_product_args {
   gated_out e;
 };
 
-template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, int TERMS>
-__global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gated_product(gated_product_args a) {
-  typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, QK> Tile;
-  __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
+// The weights' gradients, then dx, in one launch, so that neither leaves compute units empty at its end.
+struct gated_products_args {
+  gated_product_args w, x;
+  uint32_t w_units;     // of w.tm * w.tn and its parts
+};
+
+template <typename T, typename Tile, int TILE, int TERMS>
+__device__ __forceinline__ void gated_product(const gated_product_args& a, uint32_t unit, char* smem) {
+  const uint32_t tiles = a.tm * a.tn, part = unit / tiles;
   uint32_t m, n;
-  tam_tile_at(tam_xcd_order(blockIdx.x, gridDim.x), a.tm, a.tn, m, n);
-  const uint64_t k0 = blockIdx.y * a.k_part;
+  tam_tile_at(tam_xcd_order(unit - part * tiles, tiles), a.tm, a.tn, m, n);
+  const uint64_t k0 = part * a.k_part;
   const uint64_t k1 = k0 + a.k_part < a.k ? k0 + a.k_part : a.k;
   Tile t;
   t.zero();
-  t.template run<TERMS>(a.P, a.Q, n * BN, m * BM, k0, k1, smem, tam_soon{}, a.terms);
+  t.template run<TERMS>(a.P, a.Q, n * TILE, m * TILE, k0, k1, smem, tam_soon{}, a.terms);
   t.template each<TAM_AHEAD_PASS>(
       smem, [](uint32_t, uint32_t) { return 0; },
       [&](uint32_t row, uint32_t col, const float(&v)[8], int) {
-        row += m * BM;
-        col += n * BN;
+        row += m * TILE;
+        col += n * TILE;
         if (row >= a.e.rows || col >= a.e.cols) return;
         if (a.partial)
-          tam_store_some(a.partial + ((uint64_t)blockIdx.y * a.e.rows + row) * a.e.cols + col, a.e.cols - col, v);
+          tam_store_some(a.partial + ((uint64_t)part * a.e.rows + row) * a.e.cols + col, a.e.cols - col, v);
         else
           gated_put<T>(a.e, row, col, v);
       },
       [](uint32_t, uint32_t, const float*, int) {});
+}
+
+// IN_OUT: of weights stored [inputs][outputs], along which dx's sums run.
+template <typename T, int TILE, int WM, int WN, bool IN_OUT>
+__global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_gated_products(gated_products_args a) {
+  typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, false> Weight;
+  typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), IN_OUT, true> Input;
+  static_assert(Weight::LDS == Input::LDS, "one size");
+  __shared__ __attribute__((aligned(16))) char smem[Weight::LDS];
+  if (blockIdx.x < a.w_units)
+    gated_product<T, Weight, TILE, TAM_ONE_TERM>(a.w, blockIdx.x, smem);
+  else
+    gated_product<T, Input, TILE, TAM_TWO_PRODUCTS>(a.x, blockIdx.x - a.w_units, smem);
 }
 
 template <typename T>
@@ -449,21 +467,59 @@ void launch_gated(int tile, bool pk, const gated_args& a, uint32_t parts, hipStr
 }
 
 template <typename T, int TILE, int WM, int WN>
-void launch_product_tile(bool pk, bool qk, const gated_product_args& a, uint32_t parts, hipStream_t s) {
-  const dim3 grid(a.tm * a.tn, parts), block(64 * WM * WN);
-  if (pk)  // dx of weights stored [inputs][outputs]
-    hipLaunchKernelGGL((tam_k_gated_product<T, TILE, TILE, WM, WN, true, true, TAM_TWO_PRODUCTS>), grid, block, 0, s, a);
-  else if (qk)  // dx
-    hipLaunchKernelGGL((tam_k_gated_product<T, TILE, TILE, WM, WN, false, true, TAM_TWO_PRODUCTS>), grid, block, 0, s, a);
-  else  // the weights' gradients
-    hipLaunchKernelGGL((tam_k_gated_product<T, TILE, TILE, WM, WN, false, false, TAM_ONE_TERM>), grid, block, 0, s, a);
+void launch_products_tile(bool in_out, const gated_products_args& a, uint32_t units, hipStream_t s) {
+  if (in_out)
+    hipLaunchKernelGGL((tam_k_gated_products<T, TILE, WM, WN, true>), dim3(units), dim3(64 * WM * WN), 0, s, a);
+  else
+    hipLaunchKernelGGL((tam_k_gated_products<T, TILE, WM, WN, false>), dim3(units), dim3(64 * WM * WN), 0, s, a);
 }
 
 template <typename T>
-void launch_product(int tile, bool pk, bool qk, const gated_product_args& a, uint32_t parts, hipStream_t s) {
+void launch_products(int tile, bool in_out, const gated_products_args& a, uint32_t units, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (tile == 256) return launch_product_tile<T, 256, 2, 4>(pk, qk, a, parts, s);
-  tile == 128 ? launch_product_tile<T, 128, 2, 2>(pk, qk, a, parts, s) : launch_product_tile<T, 64, 2, 2>(pk, qk, a, parts, s);
+    if (tile == 256) return launch_products_tile<T, 256, 2, 4>(in_out, a, units, s);
+  tile == 128 ? launch_products_tile<T, 128, 2, 2>(in_out, a, units, s) : launch_products_tile<T, 64, 2, 2>(in_out, a, units, s);
+}
+
+// A product's rows, columns and sum; parts of its sum.
+struct extent {
+  uint64_t rows, cols, k;
+  uint32_t parts;
+  bool wanted;
+};
+
+// The tile of both products of the backward pass, and the parts of each: the least of the estimated times.
+int choose_both(extent& w, extent& x, uint32_t dtype) {
+  const double cus = tam_op_cus();
+  const bool f32 = dtype == TAM_DTYPE_F32;
+  const tam_tile_rate* rate = f32 ? tam_rates_32 : tam_rates_16;
+  int best = 64;
+  double least = 1e30;
+  uint32_t w_parts = 1, x_parts = 1;
+  auto units = [](const extent& e, uint64_t t, uint32_t parts) {
+    return e.wanted ? tam_div_up(e.rows, t) * tam_div_up(e.cols, t) * parts : 0;
+  };
+  auto join = [](const extent& e, uint32_t parts) {  // the sums' way to memory and back (about 4 TB/s) and a launch
+    return e.wanted && parts > 1 ? 3.0 + (double)e.rows * e.cols * 8.0 * parts / 4e6 : 0.0;
+  };
+  for (int i = 0; i < (f32 ? 2 : 3); ++i)
+    for (uint32_t wp : {1, 2, 3, 4, 8, 16, 32}) {
+      if (wp > 1 && (!w.wanted || w.k / wp < 128)) break;
+      for (uint32_t xp : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (xp > 1 && (!x.wanted || x.k / xp < 128)) break;
+        const double us = units_us(rate[i], units(w, rate[i].tile, wp), (double)w.k / wp, units(x, rate[i].tile, xp),
+                                   (double)x.k / xp, cus) + join(w, wp) + join(x, xp);
+        if (us < least) {
+          least = us;
+          best = rate[i].tile;
+          w_parts = wp;
+          x_parts = xp;
+        }
+      }
+    }
+  w.parts = w_parts;
+  x.parts = x_parts;
+  return best;
 }
 
 int zero(call& c, void* p, uint64_t elements) {
@@ -498,9 +554,7 @@ int forward(const TamGated* d, call& c) {
     c.tiles[1] = s.parts;
   }
   matrix x = x_of(d), gate = w_of(d, d->gate), up = w_of(d, d->up);
-  int rc = whole_rows(c, x);
-  if (rc == TAM_OK) rc = whole_rows(c, gate);
-  if (rc == TAM_OK) rc = whole_rows(c, up);
+  const int rc = whole_rows(c, {&x, &gate, &up});
   if (rc != TAM_OK) return rc;
   gated_args a = {};
   if (s.parts > 1) a.partial = (float*)c.ws.take(2ull * s.parts * e.rows * e.cols * 4);
@@ -525,34 +579,28 @@ int forward(const TamGated* d, call& c) {
   return TAM_OK;
 }
 
-int product(call& c, const matrix& P, bool p_k, const matrix& Q, bool q_k, uint64_t k, tam_parts terms, const gated_out& e) {
+// a's tiles and parts; the partial sums' memory, if there are parts. Returns its units.
+uint64_t lay_out(call& c, gated_product_args& a, const matrix& P, const matrix& Q, tam_parts terms, const extent& of, int tile,
+                 const gated_out& e) {
   const uint32_t size = kSize[c.dtype];
-  const shape s = choose(e.rows, e.cols, k * terms.terms, c.dtype);
-  if (c.tiles) {
-    c.tiles[0] = (uint32_t)s.tile;
-    c.tiles[1] = s.parts;
-  }
-  gated_product_args a = {};
-  if (s.parts > 1) a.partial = (float*)c.ws.take((uint64_t)s.parts * e.rows * e.cols * 4);
-  if (c.dry) return TAM_OK;
+  if (of.parts > 1) a.partial = (float*)c.ws.take((uint64_t)of.parts * e.rows * e.cols * 4);
   a.P = operand_of(P, e.cols, size);
   a.Q = operand_of(Q, e.rows, size);
   a.terms = terms;
-  a.k = k;
-  a.k_part = s.parts > 1 ? tam_up(tam_div_up(k, s.parts), 64) : k;
-  a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
-  a.tn = (uint32_t)tam_div_up(e.cols, s.tile);
+  a.k = of.k / terms.terms;
+  a.k_part = of.parts > 1 ? tam_up(tam_div_up(a.k, of.parts), 64) : a.k;
+  a.tm = (uint32_t)tam_div_up(e.rows, tile);
+  a.tn = (uint32_t)tam_div_up(e.cols, tile);
   a.e = e;
-  if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
-#define TAM_PRODUCT(T) launch_product<T>(s.tile, p_k, q_k, a, s.parts, c.stream)
-  TAM_OF_TYPE(c, TAM_PRODUCT);
-  TAM_OP_LAUNCHED("the product");
-  if (s.parts > 1) {
-    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
-#define TAM_SUM(T) hipLaunchKernelGGL(tam_k_gated_sum<T>, grid, block, 0, c.stream, a.partial, s.parts, e)
-    TAM_OF_TYPE(c, TAM_SUM);
-    TAM_OP_LAUNCHED("the parts' sum");
-  }
+  return (uint64_t)a.tm * a.tn * of.parts;
+}
+
+int join(call& c, const gated_product_args& a, uint32_t parts) {
+  if (parts == 1) return TAM_OK;
+  const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(a.e.cols, 8) * a.e.rows, 256)), block(256);
+#define TAM_SUM(T) hipLaunchKernelGGL(tam_k_gated_sum<T>, grid, block, 0, c.stream, a.partial, parts, a.e)
+  TAM_OF_TYPE(c, TAM_SUM);
+  TAM_OP_LAUNCHED("the parts' sum");
   return TAM_OK;
 }
 
@@ -574,31 +622,37 @@ int backward(const TamGated* d, call& c) {
     TAM_OF_TYPE(c, TAM_SLOPE);
     TAM_OP_LAUNCHED("the activation's gradient");
   }
-  if (d->dx) {
-    matrix gate = w_of(d, d->gate), up = w_of(d, d->up);
-    int rc = whole_rows(c, gate);
-    if (rc == TAM_OK) rc = whole_rows(c, up);
-    if (rc == TAM_OK && (gate.ld != up.ld)) rc = tam_op_fail(TAM_E_INVALID, "weights laid out in two ways");
-    if (rc != TAM_OK) return rc;
-    const tam_parts terms = {2, (int64_t)((intptr_t)up.p - (intptr_t)gate.p), (int64_t)ld * size};
-    const gated_out e = {{d->dx, nullptr}, rows, inputs, rows, rows, false};
-    rc = product(c, gate, d->w_in_out != 0, both, true, outputs, terms, e);
-    if (rc != TAM_OK) return rc;
+  matrix gate = w_of(d, d->gate), up = w_of(d, d->up), x = x_of(d);
+  const bool want_w = d->dgate || d->dup;
+  // dx's sum goes from one weight to the other in its stride: they are copied both or not at all
+  if (in_words(gate, size) != in_words(up, size)) gate.whole = up.whole = false;
+  int rc = d->dx && want_w ? whole_rows(c, {&gate, &up, &x}) : (d->dx ? whole_rows(c, {&gate, &up}) : whole_rows(c, {&x}));
+  if (rc != TAM_OK) return rc;
+  // dgate and dup lie as the weights do, one product: of dg's and du's columns, a row's padding between them
+  gated_out ew = {{d->dgate, d->dup}, 2 * ld, inputs, ld, outputs, false};
+  if (d->w_in_out) ew = {{d->dgate, d->dup}, inputs, 2 * ld, ld, outputs, true};
+  const gated_out ex = {{d->dx, nullptr}, rows, inputs, rows, rows, false};
+  extent w = {ew.rows, ew.cols, rows, 1, want_w}, in = {rows, inputs, 2ull * outputs, 1, d->dx != nullptr};
+  const int tile = choose_both(w, in, c.dtype);
+  if (c.tiles) {
+    if (d->dx) c.tiles[0] = (uint32_t)tile, c.tiles[1] = in.parts;
+    if (want_w) c.tiles[2] = (uint32_t)tile, c.tiles[3] = w.parts;
   }
-  if (d->dgate || d->dup) {
-    if (c.tiles) c.tiles += 2;
-    matrix x = x_of(d);
-    const int rc = whole_rows(c, x);
-    if (rc != TAM_OK) return rc;
-    const tam_parts one = {1, 0, 0};
-    gated_out e = {{d->dgate, d->dup}, 2 * ld, inputs, ld, outputs, false};
-    if (!d->w_in_out) return product(c, x, false, both, false, rows, one, e);
-    e.rows = inputs;
-    e.cols = 2 * ld;
-    e.by_cols = true;
-    return product(c, both, false, x, false, rows, one, e);
+  gated_products_args a = {};
+  uint64_t units = 0;
+  if (want_w) {
+    units = lay_out(c, a.w, d->w_in_out ? both : x, d->w_in_out ? x : both, {1, 0, 0}, w, tile, ew);
+    a.w_units = (uint32_t)units;
   }
-  return TAM_OK;
+  if (d->dx)
+    units += lay_out(c, a.x, gate, both, {2, (int64_t)((intptr_t)up.p - (intptr_t)gate.p), (int64_t)ld * size}, in, tile, ex);
+  if (c.dry) return TAM_OK;
+  if (units >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+#define TAM_PRODUCTS(T) launch_products<T>(tile, d->w_in_out != 0, a, (uint32_t)units, c.stream)
+  TAM_OF_TYPE(c, TAM_PRODUCTS);
+  TAM_OP_LAUNCHED("the gradients' products");
+  if (want_w) rc = join(c, a.w, w.parts);
+  return rc == TAM_OK && d->dx ? join(c, a.x, in.parts) : rc;
 }
 
 int gated(const TamGated* d, bool back, void* workspace, uint64_t ws_bytes, void* stream, uint64_t* need,

@@ -4,6 +4,8 @@
 #ifndef TAM_PRODUCTS_H
 #define TAM_PRODUCTS_H
 
+#include <initializer_list>
+
 #include "tam_gemm.h"
 
 // ---------------------------------------------------------------------------
@@ -19,6 +21,34 @@ static __global__ __launch_bounds__(256) void tam_k_align(const tam_f16* src, ui
   const uint64_t r = i / per;
   const uint32_t c = (uint32_t)(i - r * per) * 8;
   *reinterpret_cast<tam_oct<tam_f16>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
+}
+
+// Up to three matrices of 16-bit units, one behind the other.
+struct tam_align_item {
+  const tam_f16* src;
+  tam_f16* dst;
+  uint64_t ld_src, rows, first;  // first: the items' units of 8 before this one's
+  uint32_t cols, ld_dst;
+};
+struct tam_align_args {
+  tam_align_item item[3];
+  uint64_t units;
+  int n;
+};
+
+static __global__ __launch_bounds__(256) void tam_k_align_all(tam_align_args a) {
+  uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.units) return;
+  tam_align_item m = a.item[0];
+#pragma unroll
+  for (int n = 1; n < 3; ++n)
+    if (n < a.n && i >= a.item[n].first) m = a.item[n];
+  i -= m.first;
+  const uint32_t per = m.ld_dst / 8;
+  const uint64_t r = i / per;
+  const uint32_t c = (uint32_t)(i - r * per) * 8;
+  *reinterpret_cast<tam_oct<tam_f16>*>(m.dst + r * m.ld_dst + c) =
+      tam_some(m.src + r * m.ld_src + c, c < m.cols ? m.cols - c : 0);
 }
 
 namespace {
@@ -97,6 +127,28 @@ inline shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
   return best;
 }
 
+// us of n units of k one after another on the places of a card, behind `ahead` units of `ahead_k`
+// (the longer first): each unit to the place that is free first.
+inline double units_us(const tam_tile_rate& t, uint64_t n1, double k1, uint64_t n2, double k2, double cus) {
+  if (k1 < k2) return n2 ? units_us(t, n2, k2, n1, k1, cus) : units_us(t, n1, k2, 0, 0, cus);
+  const uint64_t places = (uint64_t)cus * t.resident, all = n1 + n2;
+  const int with = all >= places ? t.resident : (int)tam_div_up(all ? all : 1, (uint64_t)cus);  // on a compute unit
+  const double per = all <= (uint64_t)(0.5 * cus) ? t.half : t.per_k[with - 1];
+  const double d1 = 0.5 * t.start + k1 * per, d2 = 0.5 * t.start + k2 * per;
+  // two kinds of places: `late` of them have one unit more
+  uint64_t late = n1 % places, rounds = n1 / places;
+  double early_at = rounds * d1, late_at = late ? early_at + d1 : early_at;
+  uint64_t early = places - late;
+  while (n2) {
+    double& at = early_at <= late_at || !late ? early_at : late_at;
+    const uint64_t here = &at == &early_at ? early : late, take = n2 < here ? n2 : here;
+    if (take < here) return 0.5 * t.start + (at + d2 > late_at ? at + d2 : late_at);
+    at += d2;
+    n2 -= take;
+  }
+  return 0.5 * t.start + (late && late_at > early_at ? late_at : early_at);
+}
+
 // m, or a copy of it whose rows are whole lines. Rows that may end inside 16 bytes
 // have kernels of their own (REST), as the bound on their loads and the rest of their
 // sums would cost the others 1% (x [8192, 768], w [768, 3072], bf16, both ways: 206 -> 208
@@ -116,19 +168,23 @@ inline int readable(call& c, matrix& m, const shape& s) {
   return TAM_OK;
 }
 
-// m, or a copy of it: rows of whole 16 bytes that begin on 4, for kernels without a REST form.
-inline int whole_rows(call& c, matrix& m) {
+// The matrices, or copies of them: rows of whole 16 bytes that begin on 4, for kernels without a REST
+// form. All copies are one launch (three of 5 us each were a tenth of a small layer's time).
+inline int whole_rows(call& c, std::initializer_list<matrix*> all) {
   const uint32_t size = kSize[c.dtype], halves = size / 2;
-  if ((in_words(m, size) && m.whole) || !m.cols || !m.rows) return TAM_OK;
-  const uint32_t ld = aligned_ld(m.cols, size);
-  void* p = c.ws.take(m.rows * ld * size);
-  if (!c.dry) {
-    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld * halves / 8), 256)), block(256);
-    hipLaunchKernelGGL(tam_k_align, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld * halves, m.rows, m.cols * halves,
-                       (tam_f16*)p, ld * halves);
-    TAM_OP_LAUNCHED("the aligned copy");
+  tam_align_args a = {};
+  for (matrix* m : all) {
+    if ((in_words(*m, size) && m->whole) || !m->cols || !m->rows) continue;
+    const uint32_t ld = aligned_ld(m->cols, size);
+    void* p = c.ws.take(m->rows * ld * size);
+    a.item[a.n] = {(const tam_f16*)m->p, (tam_f16*)p, m->ld * halves, m->rows, a.units, m->cols * halves, ld * halves};
+    a.units += m->rows * (ld * halves / 8);
+    ++a.n;
+    *m = {p, ld, m->rows, m->cols, true};
   }
-  m = {p, ld, m.rows, m.cols, true};
+  if (c.dry || !a.n) return TAM_OK;
+  hipLaunchKernelGGL(tam_k_align_all, dim3((uint32_t)tam_div_up(a.units, 256)), dim3(256), 0, c.stream, a);
+  TAM_OP_LAUNCHED("the aligned copies");
   return TAM_OK;
 }
 
