@@ -439,18 +439,19 @@ int tam_gated_backward(const TamGated* d, void* workspace, size_t ws_bytes, void
  * vocabulary of exp(z_i)) - z_i[target_i], and its gradients.  z is never in memory as a
  * whole: the forward pass keeps a maximum and a sum of each row of a tile, the backward pass
  * makes z again in pieces of the vocabulary.  Rows whose target is `ignored` have no loss
- * and no gradient, whatever x holds there, and cost nothing in passes with more than 32
- * rows; another target outside the vocabulary makes the row's loss NaN, and with it the
+ * and no gradient, whatever x holds there, and cost nothing in the products of passes with
+ * more than 32 rows; another target outside the vocabulary makes the row's loss NaN, and with it the
  * gradients.  x, w and their gradients are of `dtype`, the rest fp32.  The backward pass
  * rounds (softmax - onehot) times the row's gradient to dtype before the products that make
  * dx and dw (scaled, so that fp16 holds it). */
 typedef struct TamCross {
-  const void* x;         /* [rows][inputs], row stride ldx                         */
+  const void* x;         /* [rows][inputs], row stride ldx (backward: see           */
+                         /* tam_cross_reads_x)                                     */
   const void* w;         /* [vocabulary][inputs], row stride ldw                   */
-  const int64_t* target; /* [rows]                                                 */
+  const int64_t* target; /* forward: [rows]                                        */
   float* loss;           /* forward: [rows], or one number where reduced           */
-  void* kept;            /* tam_cross_kept(rows) bytes, 256-byte aligned: forward:  */
-                         /* written; backward: read (the forward's)                */
+  void* kept;            /* tam_cross_kept(d) bytes, 256-byte aligned: forward:     */
+                         /* written, or NULL; backward: read (the forward's)       */
   const float* dloss;    /* backward: as loss; row i's at i * dloss_stride         */
   void* dx;              /* backward: [rows][inputs], or NULL                      */
   void* dw;              /* backward: [vocabulary][inputs], or NULL                */
@@ -463,8 +464,11 @@ typedef struct TamCross {
   uint64_t piece;        /* columns of a piece of the vocabulary; 0: chosen        */
 } TamCross;
 
-/* Bytes that the forward pass keeps for the backward pass. */
-size_t tam_cross_kept(uint64_t rows);
+/* Bytes that the forward pass keeps for the backward pass: numbers of the rows and, unless
+ * the backward pass reads x, a copy of its rows that count. */
+size_t tam_cross_kept(const TamCross* d);
+/* Whether the backward pass reads x: of up to 32 rows or up to 64 words. */
+int tam_cross_reads_x(const TamCross* d);
 /* Bytes of workspace (256-byte aligned) of the two calls below. */
 int tam_cross_workspace(const TamCross* d, int backward_pass, size_t* bytes);
 /* How their products are cut (as tam_linear_tiles tells it): tiles[0] the tile of z; backward:

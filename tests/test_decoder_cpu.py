@@ -102,7 +102,7 @@ def test_gated_missing_arrays_workspaces_and_nothing():
 
 @pytest.mark.parametrize("kw,code,text", [
     ({"dtype": 3}, 1, "dtype"), ({"reduction": 3}, 1, "reduction"), ({"x": None}, 1, "null"), ({"w": None}, 1, "null"),
-    ({"target": None}, 1, "null"), ({"ldx": 23}, 1, "stride"), ({"ldw": 23}, 1, "stride"), ({"rows": 1 << 31}, 4, "2^31"),
+    ({"ldx": 23}, 1, "stride"), ({"ldw": 23}, 1, "stride"), ({"rows": 1 << 31}, 4, "2^31"),
     ({"ldw": 1 << 21}, 4, "2^21"), ({"vocabulary": 0}, 1, "vocabulary"), ({"piece": 100}, 1, "256"),
     ({"piece": 1 << 21}, 1, "2^20"), ({"kept": 0x10010}, 1, "256 bytes"),
 ])
@@ -117,6 +117,7 @@ def test_cross_rejects(kw, code, text):
 def test_cross_missing_arrays_workspaces_and_nothing():
     lib = _lib.load()
     assert _need(lib.tam_cross_workspace, _cross(loss=None), 0)[0] == 1
+    assert _need(lib.tam_cross_workspace, _cross(target=None), 0)[0] == 1
     for k in ("kept", "dloss"):
         assert _need(lib.tam_cross_workspace, _cross(**{k: None}), 1)[0] == 1
     d = _cross()
@@ -130,7 +131,12 @@ def test_cross_missing_arrays_workspaces_and_nothing():
     assert lib.tam_cross_backward(ctypes.byref(_cross(dx=None, dw=None)), None, 0, None) == 0
     empty = dict(x=None, w=None, target=None, rows=0)
     assert lib.tam_cross(ctypes.byref(_cross(reduction=0, loss=None, **empty)), None, 0, None) == 0
-    assert lib.tam_cross_kept(100) >= 256 + 1600
+    assert lib.tam_cross_kept(ctypes.byref(_cross(rows=100, vocabulary=65))) >= 256 + 1600 + 100 * 64 * 2
+    assert lib.tam_cross_kept(ctypes.byref(_cross(rows=100, vocabulary=64))) < 256 + 1600 + 256
+    for kw, reads in (({"rows": 32, "vocabulary": 1000}, 1), ({"rows": 33, "vocabulary": 64}, 1), ({"rows": 33, "vocabulary": 65}, 0)):
+        assert lib.tam_cross_reads_x(ctypes.byref(_cross(**kw))) == reads
+    assert _need(lib.tam_cross_workspace, _cross(x=None, vocabulary=65), 1)[0] == 0  # its rows are kept
+    assert _need(lib.tam_cross_workspace, _cross(x=None, vocabulary=64), 1)[0] == 1
     # a piece's gradient of the logits stays within its bound, whatever the rows and words
     tiles = (ctypes.c_uint32 * 4)()
     for rows, words, size in ((8192, 128256, 2), (65536, 128256, 2), (65536, 128256, 4), (40, 1 << 22, 2), (8, 100, 4)):

@@ -324,7 +324,8 @@ def test_cross_and_gradients(m, k, v, dt):
 
 @pytest.mark.parametrize("dt", list(DTYPES))
 def test_cross_large_tiles_and_split_sums(dt):
-    for m, k, v in [(2048, 512, 4608), (2050, 1030, 1030), (64, 128, 30011), (5000, 24, 40)]:
+    for m, k, v in [(2048, 512, 4608), (2050, 1030, 1030), (64, 128, 30011), (5000, 24, 40), (700, 1001, 64), (701, 1001, 65),
+                    (20, 96, 40000)]:
         log(f"cross {m}x{k}x{v} {dt}")
         _check_cross(*_cross_case(m, k, v, dt, 0.3), dt, "mean")
 
@@ -476,7 +477,7 @@ def test_cross_in_pieces_of_the_vocabulary(dt):
     d.x, d.w, d.target = x.data_ptr(), w.data_ptr(), t.data_ptr()
     d.rows, d.inputs, d.vocabulary, d.ldx, d.ldw, d.ignored = m, k, v, k, k, -100
     d.dtype, d.reduction, d.piece = _lib.DTYPES[x.dtype], _lib.TAM_CROSS_SUM, 256
-    kept = torch.empty(lib.tam_cross_kept(m), dtype=torch.uint8, device="cuda")
+    kept = torch.empty(lib.tam_cross_kept(ctypes.byref(d)), dtype=torch.uint8, device="cuda")
     out, one = torch.empty((), device="cuda"), torch.ones((), device="cuda")
     dx, dw = torch.empty_like(x), torch.empty_like(w)
     d.loss, d.kept, d.dloss, d.dx, d.dw = out.data_ptr(), kept.data_ptr(), one.data_ptr(), dx.data_ptr(), dw.data_ptr()
@@ -901,7 +902,7 @@ def _cross_tiles(m, k, v, dt, backward):
 @pytest.mark.parametrize("m,k,v,dt,z,both,x_parts,w_parts", [
     (4096, 264, 9973, "bf16", 256, 128, 2, 1), (4096, 1032, 9973, "f16", 256, 256, 3, 1), (1000, 300, 2100, "bf16", 64, 64, 2, 1),
     (8192, 40, 2100, "f16", 128, 64, 2, 8), (4000, 1024, 4000, "f32", 128, 128, 1, 1), (200, 100, 700, "f32", 64, 64, 2, 1),
-    (8192, 768, 20011, "bf16", 256, 256, 2, 1), (5000, 24, 40, "f32", 64, 64, 1, 32)])
+    (8192, 768, 20011, "bf16", 256, 256, 2, 1), (5000, 24, 40, "f32", 0, 64, 1, 32)])
 def test_cross_tiles(m, k, v, dt, z, both, x_parts, w_parts):
     got = _cross_tiles(m, k, v, dt, 1)
     log(f"cross {m}x{k}x{v} {dt} tiles {_cross_tiles(m, k, v, dt, 0)} and {got}")

@@ -343,7 +343,8 @@ SIGNATURES = {
     "tam_gated_tiles": (ctypes.c_int, [ctypes.POINTER(TamGated), ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     "tam_gated": (ctypes.c_int, [ctypes.POINTER(TamGated), _VP, ctypes.c_size_t, _VP]),
     "tam_gated_backward": (ctypes.c_int, [ctypes.POINTER(TamGated), _VP, ctypes.c_size_t, _VP]),
-    "tam_cross_kept": (ctypes.c_size_t, [ctypes.c_uint64]),
+    "tam_cross_kept": (ctypes.c_size_t, [ctypes.POINTER(TamCross)]),
+    "tam_cross_reads_x": (ctypes.c_int, [ctypes.POINTER(TamCross)]),
     "tam_cross_workspace": (ctypes.c_int, [ctypes.POINTER(TamCross), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "tam_cross_tiles": (ctypes.c_int, [ctypes.POINTER(TamCross), ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     "tam_cross": (ctypes.c_int, [ctypes.POINTER(TamCross), _VP, ctypes.c_size_t, _VP]),

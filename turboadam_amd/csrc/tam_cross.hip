@@ -8,8 +8,8 @@
 //
 // Forward.  A tile of z stays in the matrix cores' registers and leaves a maximum and a sum
 // of exponentials of each of its rows, 8 bytes for its 64 to 256 columns
-// (tam_k_cross_logits); tam_k_cross_join makes lse and the loss of them.  Up to 32 rows read
-// the weight once, straight to the matrix cores (tam_k_cross_few).
+// (tam_k_cross_logits); tam_k_cross_join makes lse and the loss of them.  Up to 32 rows, and up
+// to 64 words, read the weight straight to the matrix cores (tam_k_cross_few).
 //
 // Backward.  Pieces of the vocabulary: z again, and dz of a piece, rounded to the type, goes
 // to memory (tam_k_cross_logits); then the piece's rows of dw, whole sums, and its share of
@@ -17,7 +17,7 @@
 // third of the gradients' products; to keep it would cost rows * vocabulary.
 //
 // Rows that do not count take no part: tam_k_cross_rows numbers the others, x is gathered
-// into rows of whole lines (the one copy of it; 26 us of 27 ms for 8192 x 4096), and every
+// into rows of whole lines (22 us of 24 ms for 8192 x 4096; the backward pass reads the same), and every
 // later kernel reads their number from the device: its tiles of rows past it return at once, and
 // sums over rows end there.  So NaN in a padded row reaches nothing.
 //
@@ -463,26 +463,36 @@ struct cross_few_args {
   const void* w;
   uint64_t ldx, ldw, k;
   const int64_t* targets;
-  float2* parts;  // [rows][workgroups]
+  float2* parts;  // [rows][groups of 16 columns]
   float* hit;
-  uint32_t rows, cols;
+  uint32_t rows, cols, groups;
+  // backward: rows by their numbers
+  cross_rows r;
+  const cross_row* row;
+  void* dz;
+  uint64_t ld;
 };
 
-// One workgroup: 16 columns of z for up to 16 * MT rows of x, as tam_k_few.
-template <typename T, int MT>
+// One workgroup: 16 columns of z for up to 16 * MT rows of x, the groups of columns first, as
+// tam_k_few. BACK: dz of rows that count, of the whole vocabulary.
+template <typename T, int MT, bool BACK>
 __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_args a) {
   constexpr int N = 16 / (int)sizeof(T), U = 4;
   constexpr uint64_t TURN = 4 * U * N;  // k of a wave's turn
   __shared__ float sum[TAM_FEW_WAVES][MT * 16][20];
+  const uint32_t across = blockIdx.x / a.groups, column = blockIdx.x - across * a.groups;
+  const uint32_t row0 = across * MT * 16, rows = BACK ? *a.r.count : a.rows;
+  if (row0 >= rows) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t i = lane & 15, q = lane >> 4, n = blockIdx.x * 16 + i;
+  const uint32_t i = lane & 15, q = lane >> 4, n = column * 16 + i;
   // rows past the last one read the first one's elements; their sums go nowhere
   const T* w = static_cast<const T*>(a.w) + (n < a.cols ? (uint64_t)n * a.ldw : 0);
   const T* x[MT];
   tam_f4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    x[m] = static_cast<const T*>(a.x) + (m * 16 + i < a.rows ? (uint64_t)(m * 16 + i) * a.ldx : 0);
+    const uint32_t at = row0 + m * 16 + i < rows ? row0 + m * 16 + i : row0;
+    x[m] = static_cast<const T*>(a.x) + (uint64_t)(BACK ? a.r.index[at] : at) * a.ldx;
     acc[m] = tam_f4{0.f, 0.f, 0.f, 0.f};
   }
   auto turn = [&](uint64_t k0, auto guard) {
@@ -507,24 +517,38 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_
   for (int m = 0; m < MT; ++m)  // row m * 16 + i, columns 4 q ..
     *reinterpret_cast<tam_f4*>(&sum[wave][m * 16 + i][q * 4]) = acc[m];
   __syncthreads();
-  const uint32_t t = threadIdx.x, row = t / 2, col = blockIdx.x * 16 + (t % 2) * 8;
+  const uint32_t t = threadIdx.x, row = row0 + t / 2, col = column * 16 + (t % 2) * 8;
   if (t < MT * 32) {
     float v[8] = {};
     for (int s = 0; s < TAM_FEW_WAVES; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += sum[s][row][(t % 2) * 8 + j];
-    const int64_t target = row < a.rows ? a.targets[row] : -1;
-    float top = -INFINITY, all = 0.f;
+      for (int j = 0; j < 8; ++j) v[j] += sum[s][t / 2][(t % 2) * 8 + j];
+    if constexpr (BACK) {
+      if (row < rows && col < a.cols) {
+        const cross_row of = a.row[row];
+        const uint32_t hit = (uint32_t)of.target - col;
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      if (col + j >= a.cols) v[j] = -INFINITY;
-      else if (target == (int64_t)(col + j)) a.hit[row] = v[j];
-      top = fmaxf(top, v[j]);
+        for (uint32_t j = 0; j < 8; ++j) {
+          const float p = cross_exp<T>(v[j] - of.lse) - (hit == j ? 1.0f : 0.0f);
+          // columns past the last one are zeros: the sum over columns takes whole 16 bytes
+          v[j] = col + j < a.cols ? p * of.w : 0.0f;
+        }
+        tam_store8(static_cast<T*>(a.dz) + (uint64_t)row * a.ld + col, v);
+      }
+    } else {
+      const int64_t target = row < rows ? a.targets[row] : -1;
+      float top = -INFINITY, all = 0.f;
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        if (col + j >= a.cols) v[j] = -INFINITY;
+        else if (target == (int64_t)(col + j)) a.hit[row] = v[j];
+        top = fmaxf(top, v[j]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 1));
+      all = cross_terms<T>(v, top);
+      all += __shfl_xor(all, 1);
+      if (t % 2 == 0 && row < rows) a.parts[(uint64_t)row * a.groups + column] = float2{top, all};
     }
-    top = fmaxf(top, __shfl_xor(top, 1));
-    all = cross_terms<T>(v, top);
-    all += __shfl_xor(all, 1);
-    if (t % 2 == 0 && row < a.rows) a.parts[(uint64_t)row * gridDim.x + blockIdx.x] = float2{top, all};
   }
 }
 
@@ -580,7 +604,8 @@ struct cross_product_args {
   uint32_t rows, cols;
   float* sums;             // [part][rows][cols], or null: dw's own
   bool add;                // to what the sums hold
-  void* dw;
+  void* out;               // dw's rows of the piece; dx, where one product makes it (no sums)
+  const uint32_t* index;   // of dx's rows
 };
 
 // A piece's products: units of dw, then units of dx's share, in one launch, so that neither leaves
@@ -627,7 +652,7 @@ __device__ __forceinline__ void cross_product(cross_product_args& a, uint32_t un
             TILE * 4};
   }
   t.run(a.P, a.Q, n * TILE, m * TILE, k0, k1, smem, soon);
-  const float scale = WEIGHT ? *of_scale : 1.0f;
+  const float scale = sums ? 1.0f : *of_scale;
   t.template each<TAM_AHEAD_PASS>(
       smem,
       [&](uint32_t row, uint32_t col) {
@@ -642,16 +667,16 @@ __device__ __forceinline__ void cross_product(cross_product_args& a, uint32_t un
         row += m * TILE;
         col += n * TILE;
         if (row >= rows || col >= a.cols) return;
-        const uint64_t at = (uint64_t)row * a.cols + col;
-        if (WEIGHT && !sums) {
+        if (!sums) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] *= scale;
-          tam_store_some(static_cast<T*>(a.dw) + at, a.cols - col, v);
+          const uint64_t at = (uint64_t)(WEIGHT ? row : a.index[row]) * a.cols + col;
+          tam_store_some(static_cast<T*>(a.out) + at, a.cols - col, v);
         } else {
           if (!WEIGHT && a.add)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += s.v[j];
-          tam_store_some(sums + at, a.cols - col, v);
+          tam_store_some(sums + (uint64_t)row * a.cols + col, a.cols - col, v);
         }
       },
       [](uint32_t, uint32_t, const float*, int) {});
@@ -700,6 +725,17 @@ __global__ __launch_bounds__(256) void tam_k_cross_out(const float* sums, uint32
   tam_store_some(out + row * cols + col, cols - col, v);
 }
 
+// Zeros for the rows of dx that do not count, 8 16-bit units to a thread.
+__global__ __launch_bounds__(256) void tam_k_cross_clear(tam_f16* dx, uint64_t rows, uint32_t cols, const int32_t* place) {
+  const uint32_t per = (cols + 7) / 8;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= per * rows) return;
+  const uint64_t row = i / per;
+  const uint32_t col = (uint32_t)(i - row * per) * 8;
+  const float v[8] = {};
+  if (place[row] < 0) tam_store_some(dx + row * cols + col, cols - col, v);
+}
+
 __global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n) {
   const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < n) out[i] = (tam_f16)0.0f;  // zero has the same bits in every type
@@ -708,7 +744,10 @@ __global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr uint64_t kFew = 32;
+// Passes that read the weight (and x) straight to the matrix cores: of few rows, and of so few words
+// that tiles would be few, or mostly empty (12496 x 7900 over 22 words, fp32, both ways: FEW_FIGURES).
+bool few(const TamCross* d) { return d->rows <= 32 || d->vocabulary <= 64; }
+
 constexpr uint64_t kPieceBytes = 512ull << 20;  // of dz
 constexpr uint64_t kMostPiece = 1ull << 20;     // a tile's offsets are 31-bit numbers of bytes
 
@@ -728,15 +767,21 @@ int check_cross(const TamCross* d, bool back) {
     return tam_op_fail(TAM_E_INVALID, "a piece that is no multiple of 256, or above 2^20");
   if (!d->rows && (back || d->reduction == TAM_CROSS_NONE)) return TAM_OK;
   if (d->rows && d->vocabulary == 0) return tam_op_fail(TAM_E_INVALID, "an empty vocabulary");
-  if (d->rows && d->inputs && (!d->x || !d->w)) return tam_op_fail(TAM_E_INVALID, "null x or w");
-  if (d->rows && !d->target) return tam_op_fail(TAM_E_INVALID, "null target");
+  if (d->rows && d->inputs && ((!d->x && (!back || few(d))) || !d->w)) return tam_op_fail(TAM_E_INVALID, "null x or w");
+  if (d->rows && !back && !d->target) return tam_op_fail(TAM_E_INVALID, "null target");
   if (!back && !d->loss) return tam_op_fail(TAM_E_INVALID, "null loss");
   if (back && (!d->kept || !d->dloss)) return tam_op_fail(TAM_E_INVALID, "null dloss, or what the forward pass kept");
   if ((uintptr_t)d->kept & 255u) return tam_op_fail(TAM_E_INVALID, "kept memory not on 256 bytes");
   return TAM_OK;
 }
 
-uint64_t kept_bytes(uint64_t rows) { return 256 + tam_up(16 * rows, 256); }
+uint64_t rows_bytes(uint64_t rows) { return 256 + tam_up(16 * rows, 256); }
+
+// Behind the rows' numbers the gathered rows of x: the backward pass reads them in place of x.
+uint64_t kept_bytes(const TamCross* d) {
+  const uint32_t size = kSize[d->dtype];
+  return rows_bytes(d->rows) + (few(d) ? 0 : d->rows * aligned_ld((uint32_t)d->inputs, size) * size);
+}
 
 cross_rows rows_in(void* kept, uint64_t rows) {
   if (!kept) return {};
@@ -762,15 +807,16 @@ int number_rows(const TamCross* d, const cross_rows& r, float* loss, hipStream_t
     }                                                      \
   } while (0)
 
-// The rows of x that count, and w, as the tiles read them.
-int operands(const TamCross* d, call& c, const cross_rows& r, matrix& x, matrix& w) {
+// The rows of x that count, and w, as the tiles read them. kept: where the rows lie, or are to lie (the
+// workspace where it is null).
+int operands(const TamCross* d, call& c, const cross_rows& r, void* kept, bool gather, matrix& x, matrix& w) {
   const uint32_t size = kSize[c.dtype], halves = size / 2, inputs = (uint32_t)d->inputs;
   w = matrix_of(d->w, d->ldw, d->vocabulary, d->inputs, size);
   const int rc = whole_rows(c, {&w});
   if (rc != TAM_OK) return rc;
   const uint32_t ld = aligned_ld(inputs, size);
-  x = {c.ws.take(d->rows * ld * size), ld, d->rows, inputs, true};
-  if (!c.dry && inputs) {
+  x = {kept ? (char*)kept + rows_bytes(d->rows) : c.ws.take(d->rows * ld * size), ld, d->rows, inputs, true};
+  if (!c.dry && inputs && gather) {
     const dim3 grid((uint32_t)tam_div_up(d->rows * (ld * halves / 8), 256)), block(256);
     hipLaunchKernelGGL(tam_k_cross_gather, grid, block, 0, c.stream, (const tam_f16*)d->x, d->ldx * halves, inputs * halves, r,
                        (uint32_t)d->rows, (tam_f16*)x.p, ld * halves);
@@ -885,11 +931,11 @@ int forward(const TamCross* d, call& c) {
   j.rows = rows;
   float* losses = d->loss;
   if (reduced) losses = (float*)c.ws.take(4ull * rows);
-  const bool few = rows <= kFew;
+  const bool is_few = few(d);
   if (rows) {
     float* hit = (float*)c.ws.take(4ull * rows);
     cross_rows r = rows_in(d->kept, rows);
-    if (few) {
+    if (is_few) {
       const uint32_t groups = (uint32_t)tam_div_up(d->vocabulary, 16);
       float2* parts = (float2*)c.ws.take(8ull * rows * groups);
       if (!c.dry) {
@@ -897,13 +943,24 @@ int forward(const TamCross* d, call& c) {
           const int rc = number_rows(d, r, nullptr, c.stream);
           if (rc != TAM_OK) return rc;
         }
-        const cross_few_args a = {d->x, d->w, d->ldx, d->ldw, d->inputs, d->target, parts, hit, rows, (uint32_t)d->vocabulary};
-        const dim3 grid(groups), block(64 * TAM_FEW_WAVES);
-#define TAM_FEW(T)                                                             \
-  if (rows <= 16)                                                              \
-    hipLaunchKernelGGL((tam_k_cross_few<T, 1>), grid, block, 0, c.stream, a);  \
-  else                                                                         \
-    hipLaunchKernelGGL((tam_k_cross_few<T, 2>), grid, block, 0, c.stream, a)
+        cross_few_args a = {};
+        a.x = d->x;
+        a.w = d->w;
+        a.ldx = d->ldx;
+        a.ldw = d->ldw;
+        a.k = d->inputs;
+        a.targets = d->target;
+        a.parts = parts;
+        a.hit = hit;
+        a.rows = rows;
+        a.cols = (uint32_t)d->vocabulary;
+        a.groups = groups;
+        const dim3 grid(groups * (uint32_t)tam_div_up(rows, 32)), block(64 * TAM_FEW_WAVES);
+#define TAM_FEW(T)                                                                    \
+  if (rows <= 16)                                                                     \
+    hipLaunchKernelGGL((tam_k_cross_few<T, 1, false>), grid, block, 0, c.stream, a);  \
+  else                                                                                \
+    hipLaunchKernelGGL((tam_k_cross_few<T, 2, false>), grid, block, 0, c.stream, a)
         TAM_OF_TYPE(c, TAM_FEW);
         TAM_OP_LAUNCHED("the logits of few rows");
         j.r = r;
@@ -915,7 +972,7 @@ int forward(const TamCross* d, call& c) {
         TAM_OP_LAUNCHED("the losses");
       }
     } else {
-      if (!d->kept) r = rows_in(c.ws.take(kept_bytes(rows)), rows);
+      if (!d->kept) r = rows_in(c.ws.take(rows_bytes(rows)), rows);
       if (!c.dry) {
         const int rc = number_rows(d, r, reduced ? nullptr : d->loss, c.stream);
         if (rc != TAM_OK) return rc;
@@ -923,7 +980,7 @@ int forward(const TamCross* d, call& c) {
       const int tile = tile_of(rows, d->vocabulary, d->inputs, c.dtype);
       if (c.tiles) c.tiles[0] = (uint32_t)tile;
       matrix x, w;
-      const int rc = operands(d, c, r, x, w);
+      const int rc = operands(d, c, r, d->kept, true, x, w);
       if (rc != TAM_OK) return rc;
       cross_logits_args a = logits_of(d, x, w, r, 0, d->vocabulary, tile, kSize[c.dtype]);
       if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
@@ -946,7 +1003,7 @@ int forward(const TamCross* d, call& c) {
     j.r = r;
   }
   if (reduced && !c.dry) {
-    hipLaunchKernelGGL(tam_k_cross_sum, dim3(1), dim3(1024), 0, c.stream, losses, few ? nullptr : j.r.count, d->target, d->ignored,
+    hipLaunchKernelGGL(tam_k_cross_sum, dim3(1), dim3(1024), 0, c.stream, losses, is_few ? nullptr : j.r.count, d->target, d->ignored,
                        rows, d->reduction == TAM_CROSS_MEAN, d->loss);
     TAM_OP_LAUNCHED("the losses' sum");
   }
@@ -1022,7 +1079,8 @@ int backward(const TamCross* d, call& c) {
     TAM_OP_LAUNCHED("the rows' weights");
   }
   matrix x, w;
-  int rc = operands(d, c, r, x, w);
+  const bool is_few = few(d);
+  int rc = operands(d, c, r, is_few ? nullptr : d->kept, is_few, x, w);
   if (rc != TAM_OK) return rc;
   const uint64_t piece = piece_of(d, size), widest = d->vocabulary < piece ? d->vocabulary : piece;
   const uint32_t ld = aligned_ld((uint32_t)widest, size);
@@ -1030,12 +1088,14 @@ int backward(const TamCross* d, call& c) {
   const int tile_z = tile_of(rows, widest, inputs, c.dtype);
   const pair_shape both = choose_pair(rows, inputs, widest, d->dw, d->dx, c.dtype);
   if (c.tiles) {
-    c.tiles[0] = (uint32_t)tile_z;
+    c.tiles[0] = is_few && widest == d->vocabulary ? 0 : (uint32_t)tile_z;
     c.tiles[1] = (uint32_t)piece;
     c.tiles[2] = (uint32_t)both.tile;
     c.tiles[3] = both.x_parts << 16 | both.w_parts;
   }
-  float* dx_sums = d->dx ? (float*)c.ws.take(4ull * both.x_parts * rows * inputs) : nullptr;
+  // one product makes all of dx where its sums are whole
+  const bool direct = d->dx && both.x_parts == 1 && widest == d->vocabulary;
+  float* dx_sums = d->dx && !direct ? (float*)c.ws.take(4ull * both.x_parts * rows * inputs) : nullptr;
   float* dw_sums = d->dw && both.w_parts > 1 ? (float*)c.ws.take(4ull * both.w_parts * widest * inputs) : nullptr;
   const uint32_t across = (uint32_t)tam_div_up(inputs, both.tile);
   if (c.dry) return TAM_OK;
@@ -1046,8 +1106,27 @@ int backward(const TamCross* d, call& c) {
     a.row = row;
     a.dz = dz;
     a.ld = ld;
+    if (is_few && cols == d->vocabulary) {
+      cross_few_args f = {};
+      f.x = d->x;
+      f.w = d->w;
+      f.ldx = d->ldx;
+      f.ldw = d->ldw;
+      f.k = inputs;
+      f.rows = rows;
+      f.cols = cols;
+      f.r = r;
+      f.row = row;
+      f.dz = dz;
+      f.ld = ld;
+      f.groups = (uint32_t)tam_div_up(cols, 16);
+      const dim3 grid(f.groups * (uint32_t)tam_div_up(rows, 32)), block(64 * TAM_FEW_WAVES);
+#define TAM_FEW_DZ(T) hipLaunchKernelGGL((tam_k_cross_few<T, 2, true>), grid, block, 0, c.stream, f)
+      TAM_OF_TYPE(c, TAM_FEW_DZ);
+    } else {
 #define TAM_DZ(T) launch_logits<T, true>(tile_z, a, c.stream)
-    TAM_OF_TYPE(c, TAM_DZ);
+      TAM_OF_TYPE(c, TAM_DZ);
+    }
     TAM_OP_LAUNCHED("the logits' gradient");
     const matrix z = {dz, ld, rows, cols, true};
     cross_products_args p = {};
@@ -1063,7 +1142,7 @@ int backward(const TamCross* d, call& c) {
       p.w.rows = cols;
       p.w.cols = inputs;
       p.w.sums = dw_sums;
-      p.w.dw = (char*)d->dw + first * inputs * size;
+      p.w.out = (char*)d->dw + first * inputs * size;
       units = (uint64_t)p.w.tm * across * both.w_parts;
       p.w_units = (uint32_t)units;
     }
@@ -1080,6 +1159,8 @@ int backward(const TamCross* d, call& c) {
       p.x.rows = rows;
       p.x.cols = inputs;
       p.x.sums = dx_sums;
+      p.x.out = d->dx;
+      p.x.index = r.index;
       p.x.add = first != 0;
       units += (uint64_t)p.x.tm * across * both.x_parts;
     }
@@ -1091,12 +1172,17 @@ int backward(const TamCross* d, call& c) {
       const dim3 grid((uint32_t)tam_div_up((uint64_t)cols * tam_div_up(inputs, 8), 256)), block(256);
 #define TAM_DW_OUT(T)                                                                                                     \
   hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dw_sums, both.w_parts, (uint64_t)cols, inputs, nullptr, \
-                     nullptr, 0u, 0ull, scale, (T*)p.w.dw)
+                     nullptr, 0u, 0ull, scale, (T*)p.w.out)
       TAM_OF_TYPE(c, TAM_DW_OUT);
       TAM_OP_LAUNCHED("dw's sum");
     }
   }
-  if (d->dx) {
+  if (direct) {
+    const uint32_t halves = inputs * (size / 2);
+    const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * tam_div_up(halves, 8), 256)), block(256);
+    hipLaunchKernelGGL(tam_k_cross_clear, grid, block, 0, c.stream, (tam_f16*)d->dx, (uint64_t)rows, halves, r.place);
+    TAM_OP_LAUNCHED("rows without a gradient");
+  } else if (d->dx) {
     const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * tam_div_up(inputs, 8), 256)), block(256);
 #define TAM_DX_OUT(T)                                                                                                        \
   hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dx_sums, both.x_parts, (uint64_t)rows, inputs, r.place, \
@@ -1130,7 +1216,9 @@ int cross(const TamCross* d, bool back, void* workspace, uint64_t ws_bytes, void
 
 extern "C" {
 
-size_t tam_cross_kept(uint64_t rows) { return (size_t)kept_bytes(rows); }
+size_t tam_cross_kept(const TamCross* d) { return d && d->dtype <= TAM_DTYPE_F16 ? (size_t)kept_bytes(d) : 0; }
+
+int tam_cross_reads_x(const TamCross* d) { return d && few(d); }
 
 int tam_cross_workspace(const TamCross* d, int backward_pass, size_t* bytes) {
   if (!bytes) {

@@ -138,19 +138,20 @@ struct CrossCall {
   TamCross d = {};
   Tensor x, w;  // what d points at
 
-  CrossCall(const Tensor& x0, const Tensor& weight, int64_t reduction, int64_t ignored) {
-    int64_t ldx, ldw;
-    x = rows_of(x0, x0.size(-1), ldx);
+  // x0: of `rows` rows, or undefined (a backward pass that does not read it)
+  CrossCall(const Tensor& x0, const Tensor& weight, int64_t rows, int64_t reduction, int64_t ignored) {
+    int64_t ldx = std::max<int64_t>(weight.size(1), 1), ldw;
+    if (x0.defined()) x = rows_of(x0, x0.size(-1), ldx);
     w = rows_of(weight, weight.size(1), ldw);
-    d.x = x.data_ptr();
+    d.x = ptr(x);
     d.w = w.data_ptr();
-    d.rows = x.size(0);
-    d.inputs = x.size(1);
+    d.rows = rows;
+    d.inputs = weight.size(1);
     d.vocabulary = w.size(0);
     d.ldx = ldx;
     d.ldw = ldw;
     d.ignored = ignored;
-    d.dtype = dtype_of(x);
+    d.dtype = dtype_of(w);
     d.reduction = (uint32_t)reduction;
   }
 
@@ -158,20 +159,21 @@ struct CrossCall {
     const char* what = backward ? "tam_cross_backward" : "tam_cross";
     size_t need = 0;
     check(lib.cross_workspace(&d, backward, &need), what);
-    const Tensor ws = workspace(need, x);
-    check((backward ? lib.cross_backward : lib.cross)(&d, ptr(ws), need, stream_of(x)), what);
+    const Tensor ws = workspace(need, w);
+    check((backward ? lib.cross_backward : lib.cross)(&d, ptr(ws), need, stream_of(w)), what);
   }
 };
 
 Tensor cross_forward(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t reduction, int64_t ignored,
-                     Tensor* kept) {
+                     Tensor* kept, bool* reads_x) {
   const c10::DeviceGuard guard(x.device());
-  CrossCall c(x, weight, reduction, ignored);
+  CrossCall c(x, weight, target.numel(), reduction, ignored);
   const auto options = x.options().requires_grad(false).dtype(at::kFloat);
   const Tensor loss = reduction == TAM_CROSS_NONE ? at::empty(target.sizes(), options) : at::empty({}, options);
   const Tensor t = plain(target);
   if (kept) {
-    *kept = workspace(lib.cross_kept(c.d.rows), x);
+    *kept = workspace(lib.cross_kept(&c.d), x);
+    *reads_x = lib.cross_reads_x(&c.d) != 0;
     c.d.kept = kept->data_ptr();
   }
   c.d.target = static_cast<const int64_t*>(t.data_ptr());
@@ -185,8 +187,11 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
                         int64_t ignored) {
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor kept;
-    const Tensor loss = cross_forward(x, weight, target, reduction, ignored, &kept);
-    ctx->save_for_backward({x, weight, kept});
+    bool reads_x = false;
+    const Tensor loss = cross_forward(x, weight, target, reduction, ignored, &kept, &reads_x);
+    // otherwise what is kept holds its rows that count
+    ctx->save_for_backward({reads_x ? x : Tensor(), weight, kept});
+    ctx->saved_data["sizes"] = x.sizes().vec();
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["ignored"] = ignored;
     ctx->saved_data["wants"] = (int64_t)((wants_gradient(x) ? 1 : 0) | (wants_gradient(weight) ? 2 : 0));
@@ -197,23 +202,25 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     not_twice("linear_cross_entropy");
     refuse_recording("linear_cross_entropy");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], dloss = grads[0];
+    const Tensor &x = saved[0], &weight = saved[1], dloss = grads[0];
     refuse_tangents("linear_cross_entropy", {&dloss});
     const int64_t wants = ctx->saved_data["wants"].toInt();
     Tensor dx, dw;
     if (dloss.defined() && wants) {
-      const c10::DeviceGuard guard(x.device());
-      CrossCall c(x, saved[1], ctx->saved_data["reduction"].toInt(), ctx->saved_data["ignored"].toInt());
-      const auto options = x.options().requires_grad(false);
+      const c10::DeviceGuard guard(weight.device());
+      const auto sizes = ctx->saved_data["sizes"].toIntVector();
+      int64_t rows = 1;
+      for (size_t i = 0; i + 1 < sizes.size(); ++i) rows *= sizes[i];
+      CrossCall c(x, weight, rows, ctx->saved_data["reduction"].toInt(), ctx->saved_data["ignored"].toInt());
+      const auto options = weight.options().requires_grad(false);
       Tensor d = solid(dloss);
       // a gradient of one number for all rows (that of a sum) is read as it is
       bool one = d.dim() > 0 && d.numel() > 0;
       for (int64_t i = 0; i < d.dim(); ++i) one = one && (d.size(i) == 1 || d.stride(i) == 0);
       if (!one) d = d.contiguous();
-      if (wants & 1) dx = at::empty(x.sizes(), options);
-      if (wants & 2) dw = at::empty(saved[1].sizes(), options);
+      if (wants & 1) dx = at::empty(sizes, options);
+      if (wants & 2) dw = at::empty(weight.sizes(), options);
       c.d.kept = saved[2].data_ptr();
-      c.d.target = reinterpret_cast<const int64_t*>(saved[2].data_ptr());  // not read: the rows are numbered
       c.d.dloss = static_cast<const float*>(d.data_ptr());
       c.d.dloss_stride = one ? 0 : 1;
       c.d.dx = ptr(dx);
@@ -239,7 +246,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   if (weight.size(0) == 0 && target.numel()) refuse_value(c10::str(me, ": the vocabulary is empty"));
   refuse_tangents(me, {&x, &weight});
   if (any_gradient({&x, &weight})) return CrossEntropy::apply(x, weight, target, reduction, ignored);
-  return cross_forward(x, weight, target, reduction, ignored, nullptr);
+  return cross_forward(x, weight, target, reduction, ignored, nullptr, nullptr);
 }
 
 // ------------------------------------------------------------------ rotary

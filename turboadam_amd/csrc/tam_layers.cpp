@@ -262,6 +262,7 @@ void tam_register_layers(py::module_& m) {
     take(at, "tam_gated", lib.gated);
     take(at, "tam_gated_backward", lib.gated_backward);
     take(at, "tam_cross_kept", lib.cross_kept);
+    take(at, "tam_cross_reads_x", lib.cross_reads_x);
     take(at, "tam_cross_workspace", lib.cross_workspace);
     take(at, "tam_cross", lib.cross);
     take(at, "tam_cross_backward", lib.cross_backward);

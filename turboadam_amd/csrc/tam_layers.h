@@ -32,6 +32,7 @@ struct Library {
   decltype(&tam_gated) gated = nullptr;
   decltype(&tam_gated_backward) gated_backward = nullptr;
   decltype(&tam_cross_kept) cross_kept = nullptr;
+  decltype(&tam_cross_reads_x) cross_reads_x = nullptr;
   decltype(&tam_cross_workspace) cross_workspace = nullptr;
   decltype(&tam_cross) cross = nullptr;
   decltype(&tam_cross_backward) cross_backward = nullptr;

@@ -19,7 +19,7 @@ from .optimizer import _host
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _ENTRIES = ("tam_linear_workspace", "tam_linear", "tam_linear_backward", "tam_norm_workspace", "tam_norm",
             "tam_norm_backward", "tam_gated_kept", "tam_gated_workspace", "tam_gated", "tam_gated_backward",
-            "tam_cross_kept", "tam_cross_workspace", "tam_cross", "tam_cross_backward", "tam_rotary_workspace", "tam_rotary",
+            "tam_cross_kept", "tam_cross_reads_x", "tam_cross_workspace", "tam_cross", "tam_cross_backward", "tam_rotary_workspace", "tam_rotary",
             "tam_rotary_backward", "tam_last_error")
 
 _bound = None
