@@ -996,6 +996,26 @@ def test_rotary_offsets_past_32_bits():
         assert torch.equal(dq[i:i + 3000], torch.autograd.grad(z, part, z)[0]), i
 
 
+@pytest.mark.parametrize("tokens", [(1 << 20) - 8, (1 << 20) + 8])
+def test_rotary_heads_far_apart(tokens):
+    """2 heads of 128, one whole behind the other: of 8 heads a wave's offsets would end before and past 2^31 bytes."""
+    from turboadam_amd import rotary, rotary_frequencies
+
+    g = _gen("far heads", tokens)
+    log(f"rotary of 2 heads {tokens} x 128 elements apart")
+    q = torch.randn(2, tokens, 128, generator=g, device="cuda", dtype=torch.bfloat16).transpose(0, 1).requires_grad_()
+    w = (1 + 0.1 * torch.randn(128, generator=g, device="cuda")).bfloat16()
+    f, p = rotary_frequencies(128, device="cuda"), torch.arange(tokens, device="cuda")
+    for weight in (None, w):
+        y = rotary(q, None, p, f, q_weight=weight)
+        dq, = torch.autograd.grad(y, q, y.detach())
+        for i in (0, 500000, tokens - 2000):  # the same rows by themselves, whose results other tests pin
+            part = q.detach()[i:i + 2000].contiguous().requires_grad_()
+            z = rotary(part, None, p[i:i + 2000], f, q_weight=weight)
+            assert torch.equal(y[i:i + 2000], z), i
+            assert torch.equal(dq[i:i + 2000], torch.autograd.grad(z, part, z)[0]), i
+
+
 # ------------------------------------------------------------ the example
 def _example():
     import importlib.util

@@ -255,8 +255,17 @@ struct Turn {
   double magnitude, eps;
 };
 
+// Elements between two heads that the kernels' 32-bit offsets do not reach: 2^31 bytes for the heads that a
+// wave of 64 lanes takes at once, of a lane to 16 elements.
+int64_t too_far(const Tensor& like, int64_t rotated) {
+  const int64_t units = (rotated / 2 + 7) / 8 + (like.size(-1) - rotated + 15) / 16;
+  int64_t lanes = 1;
+  while (lanes < units && lanes < 64) lanes *= 2;
+  return (int64_t(1) << 31) / like.element_size() / (64 / lanes);
+}
+
 // t as (batch, tokens, heads, dim) with contiguous heads, in place where its strides allow.
-Tensor heads_of(const Tensor& t0) {
+Tensor heads_of(const Tensor& t0, int64_t far) {
   Tensor t = solid(t0);
   const int64_t n = t.dim();
   if (n == 3) t = t.unsqueeze(0);
@@ -265,7 +274,7 @@ Tensor heads_of(const Tensor& t0) {
     for (int64_t i = 0; i + 3 < n; ++i) batch *= t.size(i);
     t = t.reshape({batch, t.size(n - 3), t.size(n - 2), t.size(n - 1)});
   }
-  return t.size(3) > 1 && t.stride(3) != 1 ? t.contiguous() : t;
+  return (t.size(3) > 1 && t.stride(3) != 1) || (t.size(2) > 1 && t.stride(2) >= far) ? t.contiguous() : t;
 }
 
 // A tensor for results in t's order of dimensions (in place of a slice: without its gaps).
@@ -278,6 +287,7 @@ Tensor result_of(const Tensor& t) {
 struct RotaryCall {
   TamRotary d = {};
   std::vector<Tensor> held;  // what d points at
+  int64_t far;
 
   RotaryCall(const Tensor& like, const Tensor& positions, const Tensor& frequencies, const Turn& turn) {
     const int64_t n = like.dim();
@@ -286,6 +296,7 @@ struct RotaryCall {
     for (int64_t i = 0; i + 3 < n; ++i) d.batch *= like.size(i);
     d.dim = like.size(n - 1);
     d.rotated = 2 * frequencies.size(0);
+    far = too_far(like, (int64_t)d.rotated);
     d.dtype = dtype_of(like);
     d.interleaved = turn.interleaved;
     d.magnitude = (float)turn.magnitude;
@@ -303,21 +314,21 @@ struct RotaryCall {
   }
 
   void input(TamHeads& h, const Tensor& x) {
-    const Tensor t = heads_of(x);
+    const Tensor t = heads_of(x, far);
     h.heads = t.size(2);
     h.x = t.data_ptr();
     h.x_b = t.stride(0);
     h.x_t = t.stride(1);
-    h.x_h = t.stride(2);
+    h.x_h = t.size(2) > 1 ? t.stride(2) : 0;
     held.push_back(t);
   }
   void gradient(TamHeads& h, const Tensor& dy) {
-    const Tensor t = heads_of(dy);
+    const Tensor t = heads_of(dy, far);
     h.heads = t.size(2);
     h.dy = t.data_ptr();
     h.dy_b = t.stride(0);
     h.dy_t = t.stride(1);
-    h.dy_h = t.stride(2);
+    h.dy_h = t.size(2) > 1 ? t.stride(2) : 0;
     held.push_back(t);
   }
   void weight(TamHeads& h, const Tensor& w) {
@@ -328,12 +339,12 @@ struct RotaryCall {
   }
   Tensor output(TamHeads& h, const Tensor& like) {
     Tensor y = result_of(like);
-    if (y.dim() > 4 && !y.is_contiguous()) y = at::empty(like.sizes(), y.options());
-    const Tensor t = heads_of(y);
+    if (!y.is_contiguous() && (y.dim() > 4 || y.stride(-2) >= far)) y = at::empty(like.sizes(), y.options());
+    const Tensor t = heads_of(y, far);
     h.y = t.data_ptr();
     h.y_b = t.stride(0);
     h.y_t = t.stride(1);
-    h.y_h = t.stride(2);
+    h.y_h = t.size(2) > 1 ? t.stride(2) : 0;
     return y;
   }
 };

@@ -391,7 +391,8 @@ int check_rotary(const TamRotary* d, bool back) {
     if (!h->heads) continue;
     if (!h->y || (!back && !h->x) || (back && (!h->dy || (h->w && !h->x))))
       return tam_op_fail(TAM_E_INVALID, "null heads");
-    const uint64_t size = d->dtype == TAM_DTYPE_F32 ? 4 : 2, far = (1ull << 31) / size / 64;  // a lane's offsets are 32-bit numbers of bytes
+    const uint64_t size = d->dtype == TAM_DTYPE_F32 ? 4 : 2;
+    const uint64_t far = (1ull << 31) / size / (64 / power_of_two(units_of(d)));  // a lane's offsets are 32-bit numbers of bytes
     for (const int64_t stride : {h->x_h, h->y_h, h->dy_h})
       if (stride < 0 || (uint64_t)stride >= far)
         return tam_op_fail(TAM_E_UNSUPPORTED, "heads %lld elements apart", (long long)stride);
