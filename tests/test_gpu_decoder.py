@@ -356,6 +356,20 @@ def test_cross_rows_that_do_not_count_reach_nothing(rows, reduction, dt):
         assert bool((grad == 0).all())
 
 
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("rows,vocabulary", [(5, 100), (70, 100), (70, 30), (0, 30)])
+def test_cross_of_no_row_that_counts_and_an_infinite_gradient(rows, vocabulary, reduction):
+    from turboadam_amd import linear_cross_entropy
+
+    x, w, t, _ = _cross_case(rows, 40, vocabulary, "bf16")
+    x, w, t = x.requires_grad_(), w.requires_grad_(), torch.full_like(t, -100)
+    log(f"cross of no row of {rows}, {vocabulary} words, {reduction}, an infinite gradient")
+    loss = linear_cross_entropy(x, w, t, reduction=reduction)
+    for value in (math.inf, math.nan):
+        for grad in torch.autograd.grad(loss, (x, w), torch.full_like(loss, value), retain_graph=True):
+            assert bool((grad == 0).all())
+
+
 @pytest.mark.parametrize("rows", [3, 70])
 def test_cross_targets_outside_the_vocabulary_are_nan(rows):
     from turboadam_amd import linear_cross_entropy

@@ -13,7 +13,7 @@
 //
 // Backward.  Pieces of the vocabulary: z again, and dz of a piece, rounded to the type, goes
 // to memory (tam_k_cross_logits); then the piece's rows of dw, whole sums, and its share of
-// dx, added to fp32 sums that tam_k_cross_dx rounds at the end.  To make z again costs a
+// dx, added to fp32 sums that tam_k_cross_out rounds at the end.  To make z again costs a
 // third of the gradients' products; to keep it would cost rows * vocabulary.
 //
 // Rows that do not count take no part: tam_k_cross_rows numbers the others, x is gathered
@@ -572,8 +572,8 @@ __global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a
   const uint32_t count = *a.r.count;
   if (a.reduction != TAM_CROSS_NONE) {
     for (uint32_t j = threadIdx.x; j < count; j += 1024) a.row[j] = {a.r.lse[a.r.index[j]], a.lift, a.r.target[j], 0};
-    if (threadIdx.x == 0)
-      *a.scale = (a.reduction == TAM_CROSS_MEAN ? a.dloss[0] / (float)(count ? count : 1u) : a.dloss[0]) / a.lift;
+    if (threadIdx.x == 0)  // no row: the sums are zeros, and stay that
+      *a.scale = count ? (a.reduction == TAM_CROSS_MEAN ? a.dloss[0] / (float)count : a.dloss[0]) / a.lift : 0.0f;
     return;
   }
   float most = 0.f;
@@ -745,8 +745,10 @@ __global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n
 // host side
 // ---------------------------------------------------------------------------
 // Passes that read the weight (and x) straight to the matrix cores: of few rows, and of so few words
-// that tiles would be few, or mostly empty (12496 x 7900 over 22 words, fp32, both ways: FEW_FIGURES).
-bool few(const TamCross* d) { return d->rows <= 32 || d->vocabulary <= 64; }
+// that tiles would be few, or mostly empty (fp32, both ways, tiles -> this: 12496 x 7900 over 22 words
+// 1079 -> 808 us, 42 x 5424 over 6 words 232 -> 76). A row has 256 threads of a launch, which takes
+// fewer than 2^32.
+bool few(const TamCross* d) { return d->rows <= 32 || (d->vocabulary <= 64 && d->rows < 1ull << 24); }
 
 constexpr uint64_t kPieceBytes = 512ull << 20;  // of dz
 constexpr uint64_t kMostPiece = 1ull << 20;     // a tile's offsets are 31-bit numbers of bytes
