@@ -79,7 +79,8 @@ struct cross_rows_args {
 };
 
 // One workgroup numbers the rows that count, 8192 a turn in their order: 8 rows to a
-// thread, sums of the threads' numbers over waves and workgroup.
+// thread, sums of the threads' numbers over waves and workgroup. Bound by its trips to memory: 8192
+// rows 14 us, of 8 to 24 ms; several workgroups would have to wait for each other, or be two launches.
 __global__ __launch_bounds__(1024) void tam_k_cross_rows(cross_rows_args a) {
   __shared__ uint32_t part[16];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -124,7 +125,8 @@ __global__ __launch_bounds__(1024) void tam_k_cross_rows(cross_rows_args a) {
   if (threadIdx.x == 0) *a.r.count = base;
 }
 
-// to[j] = the j-th row of x that counts, zeros behind it: 8 16-bit units to a thread.
+// to[j] = the j-th row of x that counts, zeros behind it: 8 16-bit units to a thread. Bound by
+// memory: 7680 of 8192 rows of 4096 bf16 22 us, 5.7 TB/s.
 __global__ __launch_bounds__(256) void tam_k_cross_gather(const tam_f16* x, uint64_t ldx, uint32_t cols, cross_rows r,
                                                           uint32_t rows, tam_f16* to, uint32_t ld) {
   const uint32_t per = ld / 8, count = *r.count;
@@ -284,7 +286,10 @@ __device__ __forceinline__ void cross_backward(const cross_logits_args& a, Tile&
 
 // Bound by the matrix cores and, at small k, by what follows the sums: exponentials, and
 // in the backward pass the stores. 16-bit tiles of 256: a workgroup to a compute unit, which begins
-// its next tile before it goes through the last one's sums.
+// its next tile before it goes through the last one's sums. bf16, 7680 rows that count x 4096 over
+// 128256 words: 6104 us (1322 TFLOP/s), in four pieces of dz 6362 (1268); 8192 x 768 over 50257 words
+// 587 (1077), two pieces of dz 651 (971, 1.3 TB/s written beside it). fp32 619 x 515 over 9973 words, 64
+// tiles: 68 and 70 (91 to 93 TFLOP/s).
 template <typename T, int TILE, int WM, int WN, bool BACK>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_logits(cross_logits_args a) {
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), true, true> Tile;
@@ -390,7 +395,8 @@ __device__ __forceinline__ float2 cross_add(const float2& a, const float2& b) {
   return {top, (a.y != 0.f ? a.y * expf(a.x - top) : 0.f) + (b.y != 0.f ? b.y * expf(b.x - top) : 0.f)};
 }
 
-// 64 rows to a workgroup, 16 threads to a row, whose sums meet in their order.
+// 64 rows to a workgroup, 16 threads to a row, whose sums meet in their order. Bound by memory and
+// its few workgroups: 7680 rows of 501 parts 17 us, 8192 of 197 8.6.
 __global__ __launch_bounds__(1024) void tam_k_cross_join(cross_join_args a) {
   __shared__ float2 at[16][64];
   const uint32_t lane = threadIdx.x & 63, run = threadIdx.x >> 6, count = *a.r.count;
@@ -411,25 +417,29 @@ __global__ __launch_bounds__(1024) void tam_k_cross_join(cross_join_args a) {
   }
 }
 
-// Few rows: a workgroup to a row.
-__global__ __launch_bounds__(256) void tam_k_cross_join_few(cross_join_args a) {
-  __shared__ float2 at[256];
+// Few rows: a workgroup to a row, of 1024 threads for many parts and of 64 for those of few words
+// (one row of 8016 parts: 9.5 us, with 256 threads 10.8; 12496 rows of 2: 8.7 us, with 256 17.3). Bound
+// by its trips to memory one after another.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void tam_k_cross_join_few(cross_join_args a) {
+  __shared__ float2 at[THREADS];
   const uint32_t row = blockIdx.x;
   const int64_t target = a.targets[row];
+  const bool inside = target >= 0 && target < a.vocabulary;
+  const float hit = inside ? a.hit[row] : 0.f;
   float2 s = {-INFINITY, 0.f};
 #pragma unroll 8
-  for (uint32_t t = threadIdx.x; t < a.tiles; t += 256) s = cross_add(s, a.parts[(uint64_t)row * a.tiles + t]);
+  for (uint32_t t = threadIdx.x; t < a.tiles; t += THREADS) s = cross_add(s, a.parts[(uint64_t)row * a.tiles + t]);
   at[threadIdx.x] = s;
-  for (int half = 128; half >= 1; half /= 2) {
+  for (int half = THREADS / 2; half >= 1; half /= 2) {
     __syncthreads();
     if ((int)threadIdx.x < half) at[threadIdx.x] = cross_add(at[threadIdx.x], at[threadIdx.x + half]);
   }
   if (threadIdx.x == 0) {
     s = at[0];
-    const bool inside = target >= 0 && target < a.vocabulary;
     const float lse = inside ? s.x + logf(s.y) : NAN;
     if (a.r.lse) a.r.lse[row] = lse;
-    a.loss[row] = target == a.ignored ? 0.f : lse - (inside ? a.hit[row] : 0.f);
+    a.loss[row] = target == a.ignored ? 0.f : lse - hit;
   }
 }
 
@@ -474,7 +484,10 @@ struct cross_few_args {
 };
 
 // One workgroup: 16 columns of z for up to 16 * MT rows of x, the groups of columns first, as
-// tam_k_few. BACK: dz of rows that count, of the whole vocabulary.
+// tam_k_few. BACK: dz of rows that count, of the whole vocabulary. Bound by memory: 1 x 4096 over 128256
+// words bf16 176 us, 6.0 TB/s; 8 x 7191 over 72376 480, 2.2, as rows that begin on odd addresses take
+// loads of their own. Many rows over few words read x more than the weight: 12496 x 7900 over 22 words
+// fp32 212 us, 1.9 TB/s, not at a limit.
 template <typename T, int MT, bool BACK>
 __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_args a) {
   constexpr int N = 16 / (int)sizeof(T), U = 4;
@@ -565,7 +578,7 @@ struct cross_weights_args {
   float* scale;   // what the products are multiplied by
 };
 
-// Each row's weight, and scale. A gradient for each row: scale is the least power of two above the
+// Each row's weight, and scale; 8192 rows 6.5 us, one workgroup's trips to memory. A gradient for each row: scale is the least power of two above the
 // largest finite one, so that dividing by it rounds nothing.
 __global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a) {
   __shared__ float top[1024];
@@ -682,6 +695,9 @@ __device__ __forceinline__ void cross_product(cross_product_args& a, uint32_t un
       [](uint32_t, uint32_t, const float*, int) {});
 }
 
+// Bound by the matrix cores: bf16, 7680 rows that count x 4096 over 128256 words, four pieces 11850 us
+// for 16.1 Tflop (1362 TFLOP/s); 8192 x 768 over 50257 words, two pieces 983 (1287). fp32 619 x 515 over 9973
+// words, 64 tiles: 140 (91).
 template <typename T, int TILE, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_products(cross_products_args a) {
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, true> Tile;
@@ -694,7 +710,8 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_
 }
 
 // out[row] = the parts' sums of the row's number in their order, times scale; zeros for
-// rows that do not count. place == null: a row's number is its own. tile, k: dx's.
+// rows that do not count. place == null: a row's number is its own. tile, k: dx's. Bound by memory: 8192 x
+// 4096 bf16 of one part 32 us, 5.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void tam_k_cross_out(const float* sums, uint32_t parts, uint64_t rows, uint32_t cols,
                                                        const int32_t* place, const uint32_t* count, uint32_t tile, uint64_t k,
@@ -725,15 +742,13 @@ __global__ __launch_bounds__(256) void tam_k_cross_out(const float* sums, uint32
   tam_store_some(out + row * cols + col, cols - col, v);
 }
 
-// Zeros for the rows of dx that do not count, 8 16-bit units to a thread.
+// Zeros for the rows of dx that do not count: a workgroup to a row at a time.
 __global__ __launch_bounds__(256) void tam_k_cross_clear(tam_f16* dx, uint64_t rows, uint32_t cols, const int32_t* place) {
-  const uint32_t per = (cols + 7) / 8;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= per * rows) return;
-  const uint64_t row = i / per;
-  const uint32_t col = (uint32_t)(i - row * per) * 8;
   const float v[8] = {};
-  if (place[row] < 0) tam_store_some(dx + row * cols + col, cols - col, v);
+  for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    if (place[row] >= 0) continue;
+    for (uint32_t col = threadIdx.x * 8; col < cols; col += 2048) tam_store_some(dx + row * cols + col, cols - col, v);
+  }
 }
 
 __global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n) {
@@ -746,9 +761,9 @@ __global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n
 // ---------------------------------------------------------------------------
 // Passes that read the weight (and x) straight to the matrix cores: of few rows, and of so few words
 // that tiles would be few, or mostly empty (fp32, both ways, tiles -> this: 12496 x 7900 over 22 words
-// 1079 -> 808 us, 42 x 5424 over 6 words 232 -> 76). A row has 256 threads of a launch, which takes
+// 1079 -> 784 us, 42 x 5424 over 6 words 232 -> 76). A row has up to 64 threads of a launch, which takes
 // fewer than 2^32.
-bool few(const TamCross* d) { return d->rows <= 32 || (d->vocabulary <= 64 && d->rows < 1ull << 24); }
+bool few(const TamCross* d) { return d->rows <= 32 || (d->vocabulary <= 64 && d->rows < 1ull << 25); }
 
 constexpr uint64_t kPieceBytes = 512ull << 20;  // of dz
 constexpr uint64_t kMostPiece = 1ull << 20;     // a tile's offsets are 31-bit numbers of bytes
@@ -970,7 +985,10 @@ int forward(const TamCross* d, call& c) {
         j.hit = hit;
         j.loss = losses;
         j.tiles = groups;
-        hipLaunchKernelGGL(tam_k_cross_join_few, dim3(rows), dim3(256), 0, c.stream, j);
+        if (groups > 64)
+          hipLaunchKernelGGL(tam_k_cross_join_few<1024>, dim3(rows), dim3(1024), 0, c.stream, j);
+        else
+          hipLaunchKernelGGL(tam_k_cross_join_few<64>, dim3(rows), dim3(64), 0, c.stream, j);
         TAM_OP_LAUNCHED("the losses");
       }
     } else {
@@ -1181,7 +1199,7 @@ int backward(const TamCross* d, call& c) {
   }
   if (direct) {
     const uint32_t halves = inputs * (size / 2);
-    const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * tam_div_up(halves, 8), 256)), block(256);
+    const dim3 grid(rows < 16384 ? rows : 16384), block(256);
     hipLaunchKernelGGL(tam_k_cross_clear, grid, block, 0, c.stream, (tam_f16*)d->dx, (uint64_t)rows, halves, r.place);
     TAM_OP_LAUNCHED("rows without a gradient");
   } else if (d->dx) {
