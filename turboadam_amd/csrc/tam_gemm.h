@@ -18,8 +18,8 @@
 // load returns as zeros: no size needs a tail loop, and the stages past the
 // last one are zeros too, so every step issues the same loads.
 //
-// Pipeline.  STAGES buffers, fragments of half a stage in registers twice.  Step t:
-// read the second half's fragments of stage t among the matrix instructions of the
+// Pipeline of the 64 and 128 tiles (that of the 256 ones: tam_tile::ring).  STAGES
+// buffers, fragments of half a stage in registers twice.  Step t: read the second half's fragments of stage t among the matrix instructions of the
 // first half; wait for stage t+1 and for the own reads, barrier: nobody reads
 // stage t's buffer any more; issue the loads of stage t+STAGES into it; read the first
 // half of stage t+1 among the matrix instructions of the second half of t.  One
@@ -458,6 +458,9 @@ struct tam_tile {
   // begin issues the first two stages into the first four halves, which nobody may be
   // reading; sum waits for them and adds the products. So a workgroup can begin its next
   // tile before it stores this one, by way of the fifth half (`spare`).
+  // (8192 x 14336 x 4096 bf16, two whole stages -> this: 745 -> 681 us with both operands along k, 816 ->
+  // 755 with neither. 4 waves of 128 x 128 in place of 8 of 128 x 64, which read less LDS: the same
+  // with both along k, slower otherwise.)
   static constexpr int HALF = SP::BYTES, L = SP::LOADS;
   struct ring {
     SP sp;
@@ -791,7 +794,7 @@ __device__ __forceinline__ void tam_tile_at(uint32_t t, uint32_t tm, uint32_t tn
 // Measured on one MI355X, tiles of k = 256 .. 4096 in launches of 16 to 1024 tiles
 // (bf16; fp32 in the second table): a launch that leaves half of the compute units
 // empty takes start + k * half us; with r tiles on each unit (at most `resident`
-// fit: 136, 68 and 49, fp32 33, KB of LDS) start + k * per_k[r - 1]. At k = 4096 and
+// fit: 160, 68 and 49, fp32 33, KB of LDS) start + k * per_k[r - 1]. At k = 4096 and
 // 1024 tiles that is 1430 TFLOP/s for 256, 1150 for 128 and 640 for 64 (fp32: 145 and
 // 134); 16 tiles of k = 256 take 12, 6 and 4 us.
 struct tam_tile_rate {

@@ -96,12 +96,14 @@ struct tam_gemm_args {
 };
 
 // Bound by the matrix cores and, beside them, by LDS (operands in, fragments out).
-// 8192 x 14336 x 4096 bf16, 256 tiles (means over 300 passes, from card to card 5%
-// either way): 745 us with both operands along k (1290 TFLOP/s), 729 for dx (one
-// m-major), 816 for dw (both); a library product reaches 1654 TFLOP/s at this size.
+// 8192 x 14336 x 4096 bf16, 256 tiles (means over 200 passes, from card to card 5%
+// either way): 681 us with both operands along k (1413 TFLOP/s), 715 for dx (one
+// m-major), 755 for dw (both); a library product of 8192^3 reaches 1398 TFLOP/s, and on
+// operands of zeros, at the clock that they leave, this one 1900.
 // 8192 x 768 x 3072, 128 tiles: 70 us for y and z (its 100 MB of stores are the second
-// bound), 47 for dx and dw each. fp32 1531 x 1001 x 777, 64 tiles: 30, 34 and 39 us; 17 are its operations at 143 TFLOP/s, the rest is 312 to 416
-// tiles on 256 compute units and single-word reads of m-major fragments.
+// bound), 47 for dx and dw each. fp32 1531 x 1001 x 777, 64 tiles: 30, 34 and 39 us;
+// 17 are its operations at 143 TFLOP/s, the rest is 312 to 416 tiles on 256 compute
+// units and single-word reads of m-major fragments.
 // REST: operands whose rows may end inside 16 bytes.
 template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool REST>
 __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gemm(tam_gemm_args a) {

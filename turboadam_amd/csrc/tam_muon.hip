@@ -349,8 +349,8 @@ __device__ __forceinline__ void triangle(uint32_t t, uint32_t& m, uint32_t& n) {
 }
 
 // FIRST: q = x x^T (tall: x^T x).  Otherwise p = a I + b q + c q q. Bound by the matrix
-// cores: the same list's q 847 us (1020 TFLOP/s of the triangles' operations), p 378
-// (915: 700 tiles are 2.7 rounds of 256 workgroups, and a tile's epilogue stores it
+// cores: the same list's q 796 us (1085 TFLOP/s of the triangles' operations), p 354
+// (976: 700 tiles are 2.7 rounds of 256 workgroups, and a tile's epilogue stores it
 // twice).
 template <int TILE, int WM, int WN, bool FIRST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_square(
@@ -529,7 +529,7 @@ __device__ __forceinline__ void write_out(const mat& d, uint32_t row, uint32_t c
 }
 
 // x' = p x (tall: x p); LAST: the output instead. back: coefficients::back. Bound by the matrix cores: the same
-// list 1540 us, 1127 TFLOP/s, LAST 1555 (it reads the parameter and writes it back); the
+// list 1422 us, 1220 TFLOP/s, LAST 1454 (it reads the parameter and writes it back); the
 // epilogues, which all workgroups of a round reach together, are a tenth of that.
 template <int TILE, int WM, int WN, bool LAST>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_mu_apply(list l, uint32_t turn, float back) {

@@ -178,8 +178,11 @@ __device__ __forceinline__ float inverse_root(float x) {
 
 // A wave takes a bundle's rows in turns, queries' first; a turn's rows are all of one part, and their
 // addresses a base that the lanes share and an offset that a lane keeps. Bound by memory and,
-// nearly as much, by the vector unit. NORM: both parts have a weight, or none. BACK: dx and the weights' sums of a
-// norm's backward pass (without a norm it is the forward pass with the angles' sign turned).
+// nearly as much, by the vector unit: 16384 tokens of 32 + 8 heads of 128 bf16 with norms 73 us forward
+// (4.6 TB/s), 111 backward (4.6). One token: 4.5, a launch and three trips to memory one after another
+// (position, heads, results). 8192 tokens of 24 heads of 64 fp32, pairs side by side: 27 (3.7).
+// NORM: both parts have a weight, or none. BACK: dx and the weights' sums of a norm's backward pass (without
+// a norm it is the forward pass with the angles' sign turned).
 template <typename T, bool SIDE, bool NORM, bool BACK>
 __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_k_rotary(rotary_args a) {
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_
 }
 
 // dw[e] = the workgroups' sums of the slot of element e, in their order: 16 elements to a
-// workgroup, 64 threads to an element.
+// workgroup, 64 threads to an element. 768 workgroups' sums of 128 elements, twice: 4.7 us, of it 2 the launch.
 template <typename T, bool SIDE>
 __global__ __launch_bounds__(1024) void tam_k_rotary_weight(const float* sums, uint32_t runs, uint32_t dim, uint32_t rotated,
                                                             uint32_t lanes, T* dq, T* dk) {

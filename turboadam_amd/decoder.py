@@ -44,8 +44,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     x (..., inputs) and weight (vocabulary, inputs) of one dtype, target (...) int64.  The
     loss is fp32: of each row (reduction="none", in target's shape), their sum, or their mean
     over the rows that count.  Rows whose target is ignore_index do not: their loss is 0, their
-    gradient is 0, whatever x holds there, and with more than 32 rows they cost nothing.  Where no
-    row counts the sum and the mean are 0.  A target outside the vocabulary that is not
+    gradient is 0, whatever x holds there, and with more than 32 rows and 64 words they cost nothing.
+    Where no row counts the sum and the mean are 0.  A target outside the vocabulary that is not
     ignore_index makes its row's loss NaN, and the gradients with it.  The backward pass makes the
     logits again, a piece of the vocabulary at a time (up to 512 MiB of their gradient), and gives
     the gradients of x and weight; softmax - onehot is rounded to the dtype before the products
@@ -64,8 +64,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, frequencie
     q (..., tokens, heads, dim) and k of the same shape but for its heads, or None (the result is
     then the queries alone, otherwise both); dim at most 1024 (1008 where the rotated part is no
     multiple of 16).  Any strides with contiguous heads are read in place: slices of a joint
-    projection, heads before tokens (passed as a transposed view); results keep the order of
-    dimensions.  positions (tokens,) or anything that broadcasts to (..., tokens), int64 or int32.
+    projection, heads before tokens (passed as a transposed view; heads of 128 that lie 256 MiB or more
+    apart are copied); results keep the order of dimensions.  positions (tokens,) or anything that broadcasts to (..., tokens), int64 or int32.
     frequencies (pairs,) float64, in radians a position (rotary_frequencies): the first 2 * pairs
     elements of a head turn, the rest stays.  Pairs are elements i and i + pairs, or 2 i and 2 i + 1
     (interleaved); angles are 64-bit products.  magnitude multiplies what turns.  With q_weight
