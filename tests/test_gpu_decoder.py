@@ -330,6 +330,31 @@ def test_cross_large_tiles_and_split_sums(dt):
         _check_cross(*_cross_case(m, k, v, dt, 0.3), dt, "mean")
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("m,k,v", [(1, 999, 16), (15, 333, 31), (31, 1025, 32), (33, 4100, 33), (48, 515, 1), (1000, 77, 48),
+                                   (97, 2050, 64), (513, 640, 15)])
+def test_cross_few_words(m, k, v, dt):
+    log(f"cross few words {m}x{k}x{v} {dt}")
+    for reduction in ("mean", "none"):
+        _check_cross(*_cross_case(m, k, v, dt, 0.3), dt, reduction)
+
+
+def test_cross_few_words_of_strided_rows_and_a_graph_kept():
+    from turboadam_amd import linear_cross_entropy
+
+    x, w, t, dl = _cross_case(70, 330, 30, "bf16", 0.3)
+    log("cross few words, rows inside others")
+    wide, tall = torch.full((70, 401), math.nan, device="cuda").bfloat16(), torch.full((30, 333), math.nan, device="cuda").bfloat16()
+    wide[:, 3:333], tall[:, 1:331] = x, w
+    for a, b in zip(_check_cross(wide[:, 3:333], tall[:, 1:331], t, dl, "bf16", "none"), _check_cross(x, w, t, dl, "bf16", "none")):
+        assert torch.equal(a, b)
+    xl, wl = x.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(xl, wl, t)
+    first, _ = torch.autograd.grad(loss, (xl, wl), retain_graph=True), linear_cross_entropy(xl * 2, wl, t)
+    for a, b in zip(first, torch.autograd.grad(loss, (xl, wl))):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("rows", [3, 32, 70])
 @pytest.mark.parametrize("dt", ["f32", "f16"])

@@ -4,12 +4,13 @@
 //   z = x w^T,  lse_i = log sum_v exp(z_iv),  loss_i = lse_i - z_i,target_i
 //   dz = (exp(z - lse) - onehot) dloss_i,  dx = dz w,  dw = dz^T x
 //
-// z (rows x vocabulary) is never in memory as a whole.
+// z (rows x vocabulary) is never in memory as a whole, but for up to 64 words.
 //
 // Forward.  A tile of z stays in the matrix cores' registers and leaves a maximum and a sum
 // of exponentials of each of its rows, 8 bytes for its 64 to 256 columns
-// (tam_k_cross_logits); tam_k_cross_join makes lse and the loss of them.  Up to 32 rows, and up
-// to 64 words, read the weight straight to the matrix cores (tam_k_cross_few).
+// (tam_k_cross_logits); tam_k_cross_join makes lse and the loss of them.  Up to 32 rows read the
+// weight straight to the matrix cores (tam_k_cross_few); up to 64 words are a row's end in one workgroup,
+// and their z, which is small beside x, is kept for the backward pass (tam_k_cross_words).
 //
 // Backward.  Pieces of the vocabulary: z again, and dz of a piece, rounded to the type, goes
 // to memory (tam_k_cross_logits); then the piece's rows of dw, whole sums, and its share of
@@ -417,21 +418,19 @@ __global__ __launch_bounds__(1024) void tam_k_cross_join(cross_join_args a) {
   }
 }
 
-// Few rows: a workgroup to a row, of 1024 threads for many parts and of 64 for those of few words
-// (one row of 8016 parts: 9.5 us, with 256 threads 10.8; 12496 rows of 2: 8.7 us, with 256 17.3). Bound
-// by its trips to memory one after another.
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void tam_k_cross_join_few(cross_join_args a) {
-  __shared__ float2 at[THREADS];
+// Few rows: a workgroup to a row. Bound by its trips to memory one after another: a row of 8016 parts
+// 9.5 us (with 256 threads 10.8).
+__global__ __launch_bounds__(1024) void tam_k_cross_join_few(cross_join_args a) {
+  __shared__ float2 at[1024];
   const uint32_t row = blockIdx.x;
   const int64_t target = a.targets[row];
   const bool inside = target >= 0 && target < a.vocabulary;
   const float hit = inside ? a.hit[row] : 0.f;
   float2 s = {-INFINITY, 0.f};
 #pragma unroll 8
-  for (uint32_t t = threadIdx.x; t < a.tiles; t += THREADS) s = cross_add(s, a.parts[(uint64_t)row * a.tiles + t]);
+  for (uint32_t t = threadIdx.x; t < a.tiles; t += 1024) s = cross_add(s, a.parts[(uint64_t)row * a.tiles + t]);
   at[threadIdx.x] = s;
-  for (int half = THREADS / 2; half >= 1; half /= 2) {
+  for (int half = 512; half >= 1; half /= 2) {
     __syncthreads();
     if ((int)threadIdx.x < half) at[threadIdx.x] = cross_add(at[threadIdx.x], at[threadIdx.x + half]);
   }
@@ -483,19 +482,16 @@ struct cross_few_args {
   uint64_t ld;
 };
 
-// One workgroup: 16 columns of z for up to 16 * MT rows of x, the groups of columns first, as
-// tam_k_few. BACK: dz of rows that count, of the whole vocabulary. Bound by memory: 1 x 4096 over 128256
-// words bf16 176 us, 6.0 TB/s; 8 x 7191 over 72376 480, 2.2, as rows that begin on odd addresses take
-// loads of their own. Many rows over few words read x more than the weight: 12496 x 7900 over 22 words
-// fp32 212 us, 1.9 TB/s, not at a limit.
+// One workgroup: 16 columns of z for up to 16 * MT rows of x, as tam_k_few. BACK: dz of rows that
+// count, of the whole vocabulary. Bound by memory: 1 x 4096 over 128256 words bf16 176 us, 6.0 TB/s; 8 x
+// 7191 over 72376 480, 2.2, as rows that begin on odd addresses take loads of their own.
 template <typename T, int MT, bool BACK>
 __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_args a) {
   constexpr int N = 16 / (int)sizeof(T), U = 4;
   constexpr uint64_t TURN = 4 * U * N;  // k of a wave's turn
   __shared__ float sum[TAM_FEW_WAVES][MT * 16][20];
-  const uint32_t across = blockIdx.x / a.groups, column = blockIdx.x - across * a.groups;
-  const uint32_t row0 = across * MT * 16, rows = BACK ? *a.r.count : a.rows;
-  if (row0 >= rows) return;
+  const uint32_t column = blockIdx.x, rows = BACK ? *a.r.count : a.rows;
+  if (rows == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t i = lane & 15, q = lane >> 4, n = column * 16 + i;
   // rows past the last one read the first one's elements; their sums go nowhere
@@ -504,7 +500,7 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_
   tam_f4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const uint32_t at = row0 + m * 16 + i < rows ? row0 + m * 16 + i : row0;
+    const uint32_t at = m * 16 + i < rows ? m * 16 + i : 0;
     x[m] = static_cast<const T*>(a.x) + (uint64_t)(BACK ? a.r.index[at] : at) * a.ldx;
     acc[m] = tam_f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -530,7 +526,7 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_
   for (int m = 0; m < MT; ++m)  // row m * 16 + i, columns 4 q ..
     *reinterpret_cast<tam_f4*>(&sum[wave][m * 16 + i][q * 4]) = acc[m];
   __syncthreads();
-  const uint32_t t = threadIdx.x, row = row0 + t / 2, col = column * 16 + (t % 2) * 8;
+  const uint32_t t = threadIdx.x, row = t / 2, col = column * 16 + (t % 2) * 8;
   if (t < MT * 32) {
     float v[8] = {};
     for (int s = 0; s < TAM_FEW_WAVES; ++s)
@@ -565,9 +561,125 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_
   }
 }
 
+struct cross_words_args {
+  const void* x;
+  const void* w;
+  uint64_t ldx, ldw, k;
+  const int64_t* targets;
+  int64_t ignored;
+  float* loss;  // by row
+  float* lse;   // or null: nothing is kept
+  float* z;     // [rows][ld] or null
+  uint32_t rows, words, ld;
+};
+
+// Rows of a workgroup: the weight is read once for them, which past 16 words is as much as x (12496 x 7900
+// over 22 words fp32: 160 us with 32 rows, 213 with 16; 8192 x 4096 over 10 words bf16: 21 and 17).
+constexpr int cross_words_rows(int nt) { return nt == 1 ? 16 : 32; }
+
+// Up to 16 * NT words: a workgroup makes z of its rows, whose sums over k meet in LDS in the waves'
+// order, their lse and their losses. Bound by the weight's way from the second cache and by x's from
+// memory: 8192 x 4096 bf16 over 10 words 17 us (3.9 TB/s of x), over 50 words 25 (2.7); 12496 x 7900 over 22
+// words fp32 160 (2.5). Turns' loads ahead of the products change nothing.
+template <typename T, int NT>
+__global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_words(cross_words_args a) {
+  constexpr int N = 16 / (int)sizeof(T), U = NT == 4 ? 2 : 4, MT = cross_words_rows(NT) / 16;
+  constexpr uint64_t TURN = 4 * U * N;  // k of a wave's turn
+  __shared__ float sum[TAM_FEW_WAVES][MT * 16][NT * 16 + 4];
+  const uint32_t row0 = blockIdx.x * MT * 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t i = lane & 15, q = lane >> 4;
+  const T *w[NT], *x[MT];
+  tam_f4 acc[MT][NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)  // words and rows past the last one read the first one's elements; their sums go nowhere
+    w[n] = static_cast<const T*>(a.w) + (n * 16 + i < a.words ? (uint64_t)(n * 16 + i) * a.ldw : 0);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    x[m] = static_cast<const T*>(a.x) + (uint64_t)(row0 + m * 16 + i < a.rows ? row0 + m * 16 + i : row0) * a.ldx;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = tam_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto turn = [&](uint64_t k0, auto guard) {
+    constexpr bool G = decltype(guard)::value;
+    tam_frag<T> fw[NT][U], fx[MT][U];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int u = 0; u < U; ++u) tam_few_load<T, G>(fx[m][u], x[m], k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < U; ++u) tam_few_load<T, G>(fw[n][u], w[n], k0 + (u * 4 + q) * N, a.k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc[m][n] = tam_mfma(fw[n][u], fx[m][u], acc[m][n]);
+  };
+  uint64_t k0 = wave * TURN;
+#pragma unroll 2
+  for (; k0 + TURN <= a.k; k0 += TAM_FEW_WAVES * TURN) turn(k0, std::false_type());
+  if (k0 < a.k) turn(k0, std::true_type());
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)  // row m * 16 + i, words n * 16 + 4 q ..
+      *reinterpret_cast<tam_f4*>(&sum[wave][m * 16 + i][n * 16 + q * 4]) = acc[m][n];
+  __syncthreads();
+  const uint32_t t = threadIdx.x, at = t / (2 * NT), col = t % (2 * NT) * 8, row = row0 + at;  // 2 NT lanes to a row
+  if (t >= MT * 16 * 2 * NT || row >= a.rows) return;
+  float v[8] = {};
+  for (int s = 0; s < TAM_FEW_WAVES; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += sum[s][at][col + j];
+  if (a.z && col < a.ld) tam_store8(a.z + (uint64_t)row * a.ld + col, v);
+  const int64_t target = a.targets[row];
+  float top = -INFINITY, hit = 0.f;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) {
+    if (col + j >= a.words) v[j] = -INFINITY;
+    else if (target == (int64_t)(col + j)) hit = v[j];
+    top = fmaxf(top, v[j]);
+  }
+#pragma unroll
+  for (int d = 1; d < 2 * NT; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  float all = cross_terms<T>(v, top);
+#pragma unroll
+  for (int d = 1; d < 2 * NT; d *= 2) {
+    all += __shfl_xor(all, d);
+    hit += __shfl_xor(hit, d);
+  }
+  if (t % (2 * NT) == 0) {
+    const float lse = target >= 0 && target < (int64_t)a.words ? top + logf(all) : NAN;
+    if (a.lse) a.lse[row] = lse;
+    a.loss[row] = target == a.ignored ? 0.f : lse - hit;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // gradients
 // ---------------------------------------------------------------------------
+// dz of rows that count, of few words: 8 columns of the z that was kept to a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void tam_k_cross_words_dz(const float* z, uint32_t ldz, uint32_t words, cross_rows r,
+                                                            const cross_row* rows, T* dz, uint64_t ld) {
+  const uint32_t per = ldz / 8, i = blockIdx.x * 256 + threadIdx.x, j = i / per, col = (i - j * per) * 8;
+  if (j >= *r.count) return;
+  const cross_row of = rows[j];
+  float v[8];
+  tam_load8(z + (uint64_t)r.index[j] * ldz + col, v);
+  const uint32_t hit = (uint32_t)of.target - col;
+#pragma unroll
+  for (uint32_t c = 0; c < 8; ++c) {
+    const float p = cross_exp<T>(v[c] - of.lse) - (hit == c ? 1.0f : 0.0f);
+    // columns past the last one are zeros: the sum over columns takes whole 16 bytes
+    v[c] = col + c < words ? p * of.w : 0.0f;
+  }
+  tam_store8(dz + j * ld + col, v);
+}
+
 struct cross_weights_args {
   cross_rows r;
   const float* dloss;
@@ -759,11 +871,12 @@ __global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Passes that read the weight (and x) straight to the matrix cores: of few rows, and of so few words
+// Passes that read the weight and x straight to the matrix cores: of few rows, and of so few words
 // that tiles would be few, or mostly empty (fp32, both ways, tiles -> this: 12496 x 7900 over 22 words
-// 1079 -> 784 us, 42 x 5424 over 6 words 232 -> 76). A row has up to 64 threads of a launch, which takes
-// fewer than 2^32.
-bool few(const TamCross* d) { return d->rows <= 32 || (d->vocabulary <= 64 && d->rows < 1ull << 25); }
+// 1079 -> 555 us, 42 x 5424 over 6 words 232 -> 80). 16 rows have 512 threads of a launch, which
+// takes fewer than 2^32.
+bool few_words(const TamCross* d) { return d->vocabulary <= 64 && d->rows < 1ull << 26; }
+bool few(const TamCross* d) { return d->rows <= 32 || few_words(d); }
 
 constexpr uint64_t kPieceBytes = 512ull << 20;  // of dz
 constexpr uint64_t kMostPiece = 1ull << 20;     // a tile's offsets are 31-bit numbers of bytes
@@ -794,10 +907,14 @@ int check_cross(const TamCross* d, bool back) {
 
 uint64_t rows_bytes(uint64_t rows) { return 256 + tam_up(16 * rows, 256); }
 
-// Behind the rows' numbers the gathered rows of x: the backward pass reads them in place of x.
+uint32_t words_ld(const TamCross* d) { return (uint32_t)tam_up(d->vocabulary, 8); }
+
+// Behind the rows' numbers the gathered rows of x: the backward pass reads them in place of x. Of few
+// words z, by row.
 uint64_t kept_bytes(const TamCross* d) {
   const uint32_t size = kSize[d->dtype];
-  return rows_bytes(d->rows) + (few(d) ? 0 : d->rows * aligned_ld((uint32_t)d->inputs, size) * size);
+  if (few(d)) return rows_bytes(d->rows) + (few_words(d) ? d->rows * words_ld(d) * 4ull : 0);
+  return rows_bytes(d->rows) + d->rows * aligned_ld((uint32_t)d->inputs, size) * size;
 }
 
 cross_rows rows_in(void* kept, uint64_t rows) {
@@ -950,9 +1067,30 @@ int forward(const TamCross* d, call& c) {
   if (reduced) losses = (float*)c.ws.take(4ull * rows);
   const bool is_few = few(d);
   if (rows) {
-    float* hit = (float*)c.ws.take(4ull * rows);
+    float* hit = few_words(d) ? nullptr : (float*)c.ws.take(4ull * rows);
     cross_rows r = rows_in(d->kept, rows);
-    if (is_few) {
+    if (few_words(d)) {
+      if (!c.dry) {
+        if (d->kept) {
+          const int rc = number_rows(d, r, nullptr, c.stream);
+          if (rc != TAM_OK) return rc;
+        }
+        float* const z = d->kept ? (float*)((char*)d->kept + rows_bytes(rows)) : nullptr;
+        const cross_words_args a = {d->x, d->w, d->ldx, d->ldw, d->inputs, d->target, d->ignored, losses, r.lse, z, rows,
+                                    (uint32_t)d->vocabulary, words_ld(d)};
+        const int nt = a.words <= 16 ? 1 : (a.words <= 32 ? 2 : 4);
+        const dim3 grid((uint32_t)tam_div_up(rows, cross_words_rows(nt))), block(64 * TAM_FEW_WAVES);
+#define TAM_WORDS(T)                                                             \
+  if (nt == 1)                                                                   \
+    hipLaunchKernelGGL((tam_k_cross_words<T, 1>), grid, block, 0, c.stream, a);  \
+  else if (nt == 2)                                                              \
+    hipLaunchKernelGGL((tam_k_cross_words<T, 2>), grid, block, 0, c.stream, a);  \
+  else                                                                           \
+    hipLaunchKernelGGL((tam_k_cross_words<T, 4>), grid, block, 0, c.stream, a)
+        TAM_OF_TYPE(c, TAM_WORDS);
+        TAM_OP_LAUNCHED("the logits of few words");
+      }
+    } else if (is_few) {
       const uint32_t groups = (uint32_t)tam_div_up(d->vocabulary, 16);
       float2* parts = (float2*)c.ws.take(8ull * rows * groups);
       if (!c.dry) {
@@ -972,7 +1110,7 @@ int forward(const TamCross* d, call& c) {
         a.rows = rows;
         a.cols = (uint32_t)d->vocabulary;
         a.groups = groups;
-        const dim3 grid(groups * (uint32_t)tam_div_up(rows, 32)), block(64 * TAM_FEW_WAVES);
+        const dim3 grid(groups), block(64 * TAM_FEW_WAVES);
 #define TAM_FEW(T)                                                                    \
   if (rows <= 16)                                                                     \
     hipLaunchKernelGGL((tam_k_cross_few<T, 1, false>), grid, block, 0, c.stream, a);  \
@@ -985,10 +1123,7 @@ int forward(const TamCross* d, call& c) {
         j.hit = hit;
         j.loss = losses;
         j.tiles = groups;
-        if (groups > 64)
-          hipLaunchKernelGGL(tam_k_cross_join_few<1024>, dim3(rows), dim3(1024), 0, c.stream, j);
-        else
-          hipLaunchKernelGGL(tam_k_cross_join_few<64>, dim3(rows), dim3(64), 0, c.stream, j);
+        hipLaunchKernelGGL(tam_k_cross_join_few, dim3(rows), dim3(1024), 0, c.stream, j);
         TAM_OP_LAUNCHED("the losses");
       }
     } else {
@@ -1126,7 +1261,14 @@ int backward(const TamCross* d, call& c) {
     a.row = row;
     a.dz = dz;
     a.ld = ld;
-    if (is_few && cols == d->vocabulary) {
+    if (few_words(d)) {
+      const uint32_t ldz = words_ld(d);
+      const float* const kept = (const float*)((const char*)d->kept + rows_bytes(rows));
+      const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * (ldz / 8), 256)), block(256);
+#define TAM_WORDS_DZ(T) \
+  hipLaunchKernelGGL(tam_k_cross_words_dz<T>, grid, block, 0, c.stream, kept, ldz, cols, r, row, (T*)dz, (uint64_t)ld)
+      TAM_OF_TYPE(c, TAM_WORDS_DZ);
+    } else if (is_few && cols == d->vocabulary) {
       cross_few_args f = {};
       f.x = d->x;
       f.w = d->w;
@@ -1140,7 +1282,7 @@ int backward(const TamCross* d, call& c) {
       f.dz = dz;
       f.ld = ld;
       f.groups = (uint32_t)tam_div_up(cols, 16);
-      const dim3 grid(f.groups * (uint32_t)tam_div_up(rows, 32)), block(64 * TAM_FEW_WAVES);
+      const dim3 grid(f.groups), block(64 * TAM_FEW_WAVES);
 #define TAM_FEW_DZ(T) hipLaunchKernelGGL((tam_k_cross_few<T, 2, true>), grid, block, 0, c.stream, f)
       TAM_OF_TYPE(c, TAM_FEW_DZ);
     } else {

@@ -39,7 +39,8 @@ def gated_linear(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, *, activ
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, reduction: str = "mean",
                          ignore_index: int = -100) -> torch.Tensor:
-    """Softmax cross entropy of the logits x @ weight.T, which are never in memory as a whole.
+    """Softmax cross entropy of the logits x @ weight.T, which are never in memory as a whole (but for
+    up to 64 words).
 
     x (..., inputs) and weight (vocabulary, inputs) of one dtype, target (...) int64.  The
     loss is fp32: of each row (reduction="none", in target's shape), their sum, or their mean
