@@ -438,10 +438,10 @@ int tam_gated_backward(const TamGated* d, void* workspace, size_t ws_bytes, void
 /* An output projection with softmax cross entropy: z = x w^T, loss_i = log(sum over the
  * vocabulary of exp(z_i)) - z_i[target_i], and its gradients.  z is never in memory as a
  * whole: the forward pass keeps a maximum and a sum of each row of a tile, the backward pass
- * makes z again in pieces of the vocabulary.  Rows whose target is `ignored` have no loss
- * and no gradient, whatever x holds there, and cost nothing in the products of passes with
- * more than 32 rows; another target outside the vocabulary makes the row's loss NaN, and with it the
- * gradients.  x, w and their gradients are of `dtype`, the rest fp32.  The backward pass
+ * makes z again in pieces of the vocabulary.  (Up to 64 words z is kept.)  Rows whose target
+ * is `ignored` have no loss and no gradient, whatever x holds there, and cost nothing in the
+ * products of passes with more than 32 rows and 64 words; another target outside the
+ * vocabulary makes the row's loss NaN, and with it the gradients.  x, w and their gradients are of `dtype`, the rest fp32.  The backward pass
  * rounds (softmax - onehot) times the row's gradient to dtype before the products that make
  * dx and dw (scaled, so that fp16 holds it). */
 typedef struct TamCross {
@@ -465,7 +465,7 @@ typedef struct TamCross {
 } TamCross;
 
 /* Bytes that the forward pass keeps for the backward pass: numbers of the rows and, unless
- * the backward pass reads x, a copy of its rows that count. */
+ * the backward pass reads x, a copy of its rows that count; of up to 64 words z, in fp32. */
 size_t tam_cross_kept(const TamCross* d);
 /* Whether the backward pass reads x: of up to 32 rows or up to 64 words. */
 int tam_cross_reads_x(const TamCross* d);

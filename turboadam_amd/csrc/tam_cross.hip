@@ -690,8 +690,9 @@ struct cross_weights_args {
   float* scale;   // what the products are multiplied by
 };
 
-// Each row's weight, and scale; 8192 rows 6.5 us, one workgroup's trips to memory. A gradient for each row: scale is the least power of two above the
-// largest finite one, so that dividing by it rounds nothing.
+// Each row's weight, and scale; 8192 rows 6.5 us, one workgroup's trips to memory. A gradient for
+// each row: scale is the least power of two above the largest finite one, so that dividing by it
+// rounds nothing.
 __global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a) {
   __shared__ float top[1024];
   const uint32_t count = *a.r.count;
@@ -1158,8 +1159,8 @@ int forward(const TamCross* d, call& c) {
     j.r = r;
   }
   if (reduced && !c.dry) {
-    hipLaunchKernelGGL(tam_k_cross_sum, dim3(1), dim3(1024), 0, c.stream, losses, is_few ? nullptr : j.r.count, d->target, d->ignored,
-                       rows, d->reduction == TAM_CROSS_MEAN, d->loss);
+    hipLaunchKernelGGL(tam_k_cross_sum, dim3(1), dim3(1024), 0, c.stream, losses, is_few ? nullptr : j.r.count, d->target,
+                       d->ignored, rows, d->reduction == TAM_CROSS_MEAN, d->loss);
     TAM_OP_LAUNCHED("the losses' sum");
   }
   return TAM_OK;

@@ -66,9 +66,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, frequencie
     then the queries alone, otherwise both); dim at most 1024 (1008 where the rotated part is no
     multiple of 16).  Any strides with contiguous heads are read in place: slices of a joint
     projection, heads before tokens (passed as a transposed view; heads of 128 that lie 256 MiB or more
-    apart are copied); results keep the order of dimensions.  positions (tokens,) or anything that broadcasts to (..., tokens), int64 or int32.
-    frequencies (pairs,) float64, in radians a position (rotary_frequencies): the first 2 * pairs
-    elements of a head turn, the rest stays.  Pairs are elements i and i + pairs, or 2 i and 2 i + 1
+    apart are copied); results keep the order of dimensions.  positions (tokens,) or anything that
+    broadcasts to (..., tokens), int64 or int32.  frequencies (pairs,) float64, in radians a position
+    (rotary_frequencies): the first 2 * pairs elements of a head turn, the rest stays.  Pairs are elements i and i + pairs, or 2 i and 2 i + 1
     (interleaved); angles are 64-bit products.  magnitude multiplies what turns.  With q_weight
     (dim,) a query head is first divided by sqrt(mean of squares + eps) and multiplied by it; k_weight
     likewise.  The backward pass gives the gradients of q, k and the weights, those of the weights
