@@ -831,6 +831,42 @@ def test_in_a_captured_graph():
             assert torch.equal(a, c), f"replay {i}"
 
 
+def test_two_streams_at_once_and_two_graphs_of_one_pool():
+    """Calls of one process that overlap, and captured ones whose workspaces share their memory: no call's
+    workspace is another's while it is needed."""
+    cases = [_streams_case(), _streams_case()]
+    with torch.no_grad():
+        for leaf in cases[1][0]:
+            leaf.mul_(0.5)
+    want = [[v.clone() for v in call()] for _, call in cases]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (_, call) in enumerate(cases):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(call())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            for a, c in zip(out, want[i]):
+                assert torch.equal(a, c), i
+    graphs, outs = [], []
+    for _, call in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(call())
+        graphs.append(graph)
+    for turn in range(3):
+        for i in range(2):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            for a, c in zip(outs[i], want[i]):
+                assert torch.equal(a, c), (turn, i)
+            for a, c in zip(cases[i][1](), want[i]):
+                assert torch.equal(a, c), (turn, i)
+
+
 def test_refusals():
     from turboadam_amd import gated_linear, linear_cross_entropy, rotary
 
