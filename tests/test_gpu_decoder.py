@@ -350,6 +350,9 @@ def test_cross_few_words_of_strided_rows_and_a_graph_kept():
         assert torch.equal(a, b)
     xl, wl = x.requires_grad_(), w.requires_grad_()
     loss = linear_cross_entropy(xl, wl, t)
+    both = torch.autograd.grad(loss, (xl, wl), retain_graph=True)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(xl, wl.detach(), t), xl)[0], both[0])
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(xl.detach(), wl, t), wl)[0], both[1])
     first, _ = torch.autograd.grad(loss, (xl, wl), retain_graph=True), linear_cross_entropy(xl * 2, wl, t)
     for a, b in zip(first, torch.autograd.grad(loss, (xl, wl))):
         assert torch.equal(a, b)

@@ -1236,7 +1236,8 @@ int backward(const TamCross* d, call& c) {
   }
   matrix x, w;
   const bool is_few = few(d);
-  int rc = operands(d, c, r, is_few ? nullptr : d->kept, is_few, x, w);
+  // of few words only dw reads x
+  int rc = operands(d, c, r, is_few ? nullptr : d->kept, few_words(d) ? d->dw != nullptr : is_few, x, w);
   if (rc != TAM_OK) return rc;
   const uint64_t piece = piece_of(d, size), widest = d->vocabulary < piece ? d->vocabulary : piece;
   const uint32_t ld = aligned_ld((uint32_t)widest, size);
