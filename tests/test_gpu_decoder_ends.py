@@ -1,0 +1,72 @@
+"""GPU: gated_linear, linear_cross_entropy and rotary at the ends of their ranges: infinities and NaN beside what
+does not touch them, an eps of 0, values that a type cannot hold, losses of large logits, gradients of 2^127 and more.
+
+Bounds (fixed before the first run) are derived beside each test."""
+
+import math
+
+import pytest
+import torch
+
+from tests.helpers import log
+from tests.test_gpu_decoder import DTYPES, TINY, UNIT, _check_rotary, _gen, _randn, _rotary_case, _turned, _within
+
+pytestmark = pytest.mark.gpu
+
+BITS = {torch.float32: torch.int32, torch.bfloat16: torch.int16, torch.float16: torch.int16}
+
+
+def _same_bits(a, b):
+    """Bit for bit, -0 from 0 too, but any NaN as any other."""
+    bits = BITS[a.dtype]
+    return a.shape == b.shape and bool(((a.contiguous().view(bits) == b.contiguous().view(bits)) | (a.isnan() & b.isnan())).all())
+
+
+# ------------------------------------------------------------------ rotary
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,pairs", [(40, 8), (33, 7), (64, 16), (24, 0), (300, 100)])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_rotary_what_does_not_turn_stays_as_it_is(d, pairs, interleaved, dt):
+    """Infinities, NaN and -0 behind the rotated part of heads without a norm: forward and backward they come out as they
+    went in, and no other element changes a bit."""
+    from turboadam_amd import rotary
+
+    q, k, p, f, _, dq, dk = _rotary_case(2, 9, 3, 2, d, pairs, dt, False, 3)
+    log(f"rotary rest of {d}, {pairs} pairs, {dt} interleaved={interleaved}")
+
+    def both(q, k, dq, dk):
+        leaves = [v.detach().requires_grad_() for v in (q, k)]
+        out = rotary(*leaves, p, f, interleaved=interleaved)
+        return [v.detach() for v in out] + list(torch.autograd.grad(out, leaves, (dq, dk)))
+
+    want = both(q, k, dq, dk)
+    special = (math.inf, -math.inf, math.nan, -0.0)
+    marked = []
+    for v in (q, k, dq, dk):
+        v = v.clone()
+        g = _gen("where", d, pairs, len(marked))
+        where = torch.rand(v.shape, generator=g, device="cuda") < 0.2
+        where[..., :2 * pairs] = False
+        v[where] = torch.tensor(special, device="cuda").to(v.dtype)[torch.arange(int(where.sum()), device="cuda") % 4]
+        marked.append(v)
+    for got, ref, v in zip(both(*marked), want, marked):
+        assert _same_bits(got[..., 2 * pairs:], v[..., 2 * pairs:])
+        assert _same_bits(got[..., :2 * pairs], ref[..., :2 * pairs])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_rotary_an_infinity_in_the_rest_of_a_normed_head(interleaved, dt):
+    """The norm divides by an infinite root: by the formula it is NaN itself and every other element of its head 0."""
+    from turboadam_amd import rotary
+
+    q, k, p, f, w, _, _ = _rotary_case(1, 9, 3, 2, 40, 8, dt, True, 3)
+    want = rotary(q, k, p, f, interleaved=interleaved, q_weight=w[0], k_weight=w[1])
+    q = q.clone()
+    q[0, 4, 1, 21] = math.inf
+    log(f"rotary of an infinity beside a norm {dt} interleaved={interleaved}")
+    got = rotary(q, k, p, f, interleaved=interleaved, q_weight=w[0], k_weight=w[1])
+    head = got[0][0, 4, 1]
+    assert bool(head[21].isnan()) and bool((head[torch.arange(40, device="cuda") != 21] == 0).all())
+    got[0][0, 4, 1] = want[0][0, 4, 1]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -7,7 +7,8 @@
 //   t x rstd,  dx = rstd (t w - x rstd^2 mean(t w x))
 //
 // Units.  A head's row is cut into units of 8 pairs: UR units of the rotated part (the
-// last one may be short), then units of the rest of the row, whose angle is 0.  L lanes,
+// last one may be short), then units of the rest of the row, which go past the rotation: with
+// an angle of 0 an infinity or a NaN would reach the element that it is paired with.  L lanes,
 // the next power of two, take a row, a unit each: two vectors of 8 elements, both halves
 // of its pairs.  So a pair lies in one lane, whichever way pairs are laid out, and only
 // the norm's sums cross lanes.  A wave takes 64 / L rows of a token at once (or several
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_
       const bool turn = !rest && u * 8 + p < a.rotated / 2;
       sin_cos_turns(position * (turn ? a.frequencies[u * 8 + p] * 0.15915494309189535 : 0.0), s[p], c[p]);
       s[p] *= a.sign * a.scale;
-      c[p] *= rest ? 1.0f : a.scale;
+      c[p] *= a.scale;
     }
 #pragma unroll 1
     for (uint32_t turn = item - bundle * a.split; turn < turns; turn += a.split) {
@@ -235,12 +236,13 @@ __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_
       pairs<T, SIDE>(xv, x0, x1);
       if (BACK) {
         pairs<T, SIDE>(dv, d0, d1);
+        if (!rest)
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const float da = d0[p];
-          d0[p] = __builtin_fmaf(da, c[p], -d1[p] * s[p]);
-          d1[p] = __builtin_fmaf(da, s[p], d1[p] * c[p]);
-        }
+          for (int p = 0; p < 8; ++p) {
+            const float da = d0[p];
+            d0[p] = __builtin_fmaf(da, c[p], -d1[p] * s[p]);
+            d1[p] = __builtin_fmaf(da, s[p], d1[p] * c[p]);
+          }
         {
           float sx = 0.f, sg = 0.f;
 #pragma unroll
@@ -290,12 +292,13 @@ __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_
             x1[p] *= rstd * w1[p];
           }
         }
+        if (!rest)
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const float xa = x0[p];
-          x0[p] = __builtin_fmaf(xa, c[p], -x1[p] * s[p]);
-          x1[p] = __builtin_fmaf(xa, s[p], x1[p] * c[p]);
-        }
+          for (int p = 0; p < 8; ++p) {
+            const float xa = x0[p];
+            x0[p] = __builtin_fmaf(xa, c[p], -x1[p] * s[p]);
+            x1[p] = __builtin_fmaf(xa, s[p], x1[p] * c[p]);
+          }
         store<T, SIDE>(y, to, e, x0, x1);
       }
     }
