@@ -70,3 +70,15 @@ def test_rotary_an_infinity_in_the_rest_of_a_normed_head(interleaved, dt):
     assert bool(head[21].isnan()) and bool((head[torch.arange(40, device="cuda") != 21] == 0).all())
     got[0][0, 4, 1] = want[0][0, 4, 1]
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("b,t,hq,hk,d,pairs", [(1, 5, 32, 4, 128, 64), (2, 7, 7, 3, 84, 42), (1, 33, 2, 1, 64, 16), (3, 3, 1, 5, 40, 0)])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_rotary_norm_of_an_eps_of_zero(b, t, hq, hk, d, pairs, dt):
+    """Heads that are no multiple of a wave's rows, and tokens that leave a wave's last ones empty: what has no row adds
+    nothing to the weights' gradients, though its own norm would divide by 0."""
+    q, k, p, f, w, dq, dk = _rotary_case(b, t, hq, hk, d, pairs, dt, True, 5)
+    for interleaved in (False, True):
+        log(f"rotary eps 0, {b}x{t} {hq}/{hk} heads of {d} {dt} interleaved={interleaved}")
+        _check_rotary(q, k, p, f, dt, interleaved, 1.0, w[0], w[1], eps=0.0, dq=dq, dk=dk)
+        _check_rotary(q, k, p, f, dt, interleaved, 1.0, w[0], None, eps=0.0, dq=dq, dk=dk)

@@ -220,7 +220,8 @@ __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_
       const heads_args& h = a.part[which];
       const uint32_t row0 = (key ? turn - a.part[0].turns : turn) * rows;
       unit e = at;
-      if (!mine || row0 + first >= h.heads) e.n0 = e.n1 = 0;
+      const bool here = mine && row0 + first < h.heads;
+      if (!here) e.n0 = e.n1 = 0;
       const uint32_t row = e.n0 | e.n1 ? first : 0;
       auto from = [&](const char* base, int64_t b, int64_t of_t, uint32_t of_h) {
         return base + (batch * b + t0 * of_t + (int64_t)row0 * of_h);
@@ -254,7 +255,8 @@ __global__ __launch_bounds__(256, BACK ? 3 : (sizeof(T) == 2 ? 5 : 4)) void tam_
           }
           sx = lanes_sum(sx, a.lanes);
           sg = lanes_sum(sg, a.lanes);
-          const float rstd = inverse_root<T>(__builtin_fmaf(sx, inv, a.eps)), mean = -sg * inv * rstd * rstd * rstd;
+          // lanes without a row have sums of zeros, whose root may be infinite: they add nothing to dw
+          const float rstd = here ? inverse_root<T>(__builtin_fmaf(sx, inv, a.eps)) : 0.0f, mean = -sg * inv * rstd * rstd * rstd;
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
             d0[p] *= rstd;
