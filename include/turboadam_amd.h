@@ -497,7 +497,7 @@ typedef struct TamHeads {
  * the pairs (a, b) of its first `rotated` elements turn by the angle position * frequency:
  * magnitude * (a cos - b sin, a sin + b cos).  Pairs are elements i and i + rotated / 2, or
  * 2 i and 2 i + 1 with `interleaved`.  Angles are 64-bit products.  Squares and their sums
- * are fp32.  Results may not overlap their inputs. */
+ * are fp32; eps is 0 or a normal number.  Results may not overlap their inputs. */
 typedef struct TamRotary {
   TamHeads q, k;
   const void* positions;     /* i64 or i32 at [batch * pos_b + token * pos_t]      */

@@ -82,3 +82,18 @@ def test_rotary_norm_of_an_eps_of_zero(b, t, hq, hk, d, pairs, dt):
         log(f"rotary eps 0, {b}x{t} {hq}/{hk} heads of {d} {dt} interleaved={interleaved}")
         _check_rotary(q, k, p, f, dt, interleaved, 1.0, w[0], w[1], eps=0.0, dq=dq, dk=dk)
         _check_rotary(q, k, p, f, dt, interleaved, 1.0, w[0], None, eps=0.0, dq=dq, dk=dk)
+
+
+def test_rotary_eps_is_zero_or_a_normal_number():
+    """A head of zeros is divided by sqrt(eps): an eps that float32 has not, or that the hardware's root takes for 0, would
+    make it NaN."""
+    from turboadam_amd import rotary
+
+    log("rotary eps at its ends")
+    f, p = torch.ones(4, dtype=torch.float64, device="cuda"), torch.arange(4, device="cuda")
+    for dt in DTYPES.values():
+        q, w = torch.zeros(4, 2, 8, device="cuda", dtype=dt), torch.ones(8, device="cuda", dtype=dt)
+        for eps in (1e-50, 2.0 ** -127, 1e39, math.inf, math.nan):
+            with pytest.raises(ValueError, match="eps"):
+                rotary(q, None, p, f, q_weight=w, eps=eps)
+        assert bool((rotary(q, None, p, f, q_weight=w, eps=2.0 ** -126) == 0).all())

@@ -3,6 +3,8 @@
 // the torch extension module _tam_host).
 #include "tam_layers.h"
 
+#include <cfloat>
+
 namespace {
 
 using namespace tam;
@@ -448,7 +450,9 @@ variable_list rotary(const Tensor& q, const OptTensor& k, const Tensor& position
     refuse_value(c10::str("rotary: frequencies must be float64 (pairs,) with at most ", q.size(n - 1) / 2, " pairs, got ",
                           frequencies.scalar_type(), " ", shape(frequencies)));
   if (frequencies.requires_grad() && at::GradMode::is_enabled()) refuse("rotary: frequencies have no gradient");
-  if (!(eps >= 0)) refuse_value(c10::str("rotary: eps must be 0 or more, got ", eps));
+  const float eps32 = (float)eps;  // as the kernels take it
+  if (!(eps == 0 || (eps32 >= FLT_MIN && eps32 <= FLT_MAX)))
+    refuse_value(c10::str("rotary: eps must be 0 or in float32's normal numbers, got ", eps));
   if (k_weight && !k) refuse_value("rotary: k_weight without k");
   for (const auto& [name, t] : {std::pair<const char*, const OptTensor&>("q_weight", q_weight), {"k_weight", k_weight}})
     if (t) {

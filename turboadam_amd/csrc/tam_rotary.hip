@@ -20,6 +20,7 @@
 // and cosine are taken in fp32: position 10^6 is as exact as position 1.
 #include "tam_ops.h"
 
+#include <float.h>
 #include <math.h>
 
 namespace {
@@ -385,7 +386,8 @@ int check_rotary(const TamRotary* d, bool back) {
   if (d->dim == 0) return tam_op_fail(TAM_E_INVALID, "heads of no elements");
   if (d->rotated % 2 || d->rotated > d->dim)
     return tam_op_fail(TAM_E_INVALID, "a rotated part that is odd or longer than a head");
-  if (!(d->eps >= 0)) return tam_op_fail(TAM_E_INVALID, "eps below 0");
+  if (!(d->eps == 0 || (d->eps >= FLT_MIN && d->eps <= FLT_MAX)))  // the hardware's root takes smaller ones for 0
+    return tam_op_fail(TAM_E_INVALID, "an eps that is neither 0 nor one of fp32's normal numbers above it");
   if (d->dim > kMostDim || units_of(d) > 64)
     return tam_op_fail(TAM_E_UNSUPPORTED, "heads of more than %u elements (%u where the rotated part is no multiple of 16)",
                        kMostDim, kMostDim - 16);

@@ -71,7 +71,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, frequencie
     (rotary_frequencies): the first 2 * pairs elements of a head turn, the rest stays.  Pairs are elements i and i + pairs, or 2 i and 2 i + 1
     (interleaved); angles are 64-bit products.  magnitude multiplies what turns.  With q_weight
     (dim,) a query head is first divided by sqrt(mean of squares + eps) and multiplied by it; k_weight
-    likewise.  The backward pass gives the gradients of q, k and the weights, those of the weights
+    likewise.  eps is 0 or one of float32's normal numbers, in which the mean is taken.  The backward pass gives the gradients of q, k and the weights, those of the weights
     summed in a fixed order."""
     out = (layers._bound or _layers()).rotary(q, k, positions, frequencies, interleaved, magnitude, q_weight, k_weight, eps)
     return out[0] if k is None else (out[0], out[1])
