@@ -97,3 +97,29 @@ def test_rotary_eps_is_zero_or_a_normal_number():
             with pytest.raises(ValueError, match="eps"):
                 rotary(q, None, p, f, q_weight=w, eps=eps)
         assert bool((rotary(q, None, p, f, q_weight=w, eps=2.0 ** -126) == 0).all())
+
+
+# ------------------------------------------------------------ gated linear
+@pytest.mark.parametrize("in_out", [False, True])
+@pytest.mark.parametrize("rows", [20, 100])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_gated_of_products_that_the_type_cannot_hold(rows, dt, in_out):
+    """g = a G and u = b U, of which fp16 holds neither in some rows (g of -2.6e5 or 2.6e5, u of 1e5 either sign) but h and
+    every gradient in all of them.  The bounds are those of the other gated tests."""
+    from tests.test_gpu_decoder import _check_gated
+
+    g = _gen("past the range", rows)
+    a = torch.tensor([-512.0, -300.0, 512.0, 16.0, -0.02], device="cuda")[torch.arange(rows, device="cuda") % 5]
+    b = torch.tensor([0.008, 1.0, 2.0 ** -12, 0.008, 200.0], device="cuda")[torch.arange(rows, device="cuda") % 5]
+    x = torch.zeros(rows, 8, device="cuda")
+    x[:, 0], x[:, 1] = a, b
+    gate, up = torch.zeros(2, 40, 8, device="cuda").unbind(0)
+    gate[:, 0] = torch.rand(40, generator=g, device="cuda") * 500 + 12
+    up[:, 1] = (torch.rand(40, generator=g, device="cuda") - 0.5) * 1000
+    x, gate, up = [v.to(DTYPES[dt]) for v in (x, gate, up)]
+    if in_out:
+        gate, up = [v.t().contiguous().t() for v in (gate, up)]
+    dh = (torch.randn(rows, 40, generator=g, device="cuda") * 2.0 ** -15).to(DTYPES[dt])
+    for act in ("silu", "gelu_tanh", "gelu", "relu"):
+        log(f"gated past the range {rows} {dt} {act} in_out={in_out}")
+        _check_gated(x, gate, up, dh, dt, act)

@@ -33,31 +33,20 @@ struct gated_epilogue {
 };
 
 // What the forward pass keeps of g and u: for 8 columns a record of 64 bytes in fp32, of 48 in
-// 16 bits: 8 of g and 8 of u in the type and, one byte each, the next 8 bits of both. (Rounded
-// to the type alone, they bring dgate's, dup's and dx's errors in bf16 from 2.4e-3 of their norm to
-// 3.0e-3, 1.7e-3 of it their own rounding; the bytes cost 2% of a large training pass.)
+// 16 bits: fp32's upper 24 bits of 8 of g and 8 of u, as bf16 and, one byte each, the next 8 bits. (Rounded
+// to bf16 alone, they bring dgate's, dup's and dx's errors in bf16 from 2.4e-3 of their norm to
+// 3.0e-3, 1.7e-3 of it their own rounding; the bytes cost 2% of a large training pass. fp16 would have 3 digits
+// more, 2^-17 being a 32nd of its rounding, but not the range: act(g) u may be one of its numbers where g or u is not.)
 template <typename T>
 constexpr uint32_t gated_record = sizeof(T) == 4 ? 64 : 48;
 
-// The low byte of x past its rounding h: of the distance of their bits, in 2^-8 of the
-// type's last place.
-template <typename T>
-__device__ __forceinline__ uint32_t gated_low(float x, T h) {
-  const float f = (float)h;
-  int32_t d = (int32_t)(__builtin_bit_cast(uint32_t, x) - __builtin_bit_cast(uint32_t, f));
-  if constexpr (std::is_same_v<T, tam_f16>) {
-    // below fp16's normal numbers places are wider than 2^13 bits, up to those of x where h is
-    // 0: as near as a byte comes; an infinity that x is not stays one
-    d = d < -4096 ? -4096 : (d > 4095 ? 4095 : d);
-    d = __builtin_isinf(f) ? 0 : d * 8;
-  }
-  d += 128;
+// The low byte of x past its rounding h: of the distance of their bits, in 2^-8 of bf16's last place.
+__device__ __forceinline__ uint32_t gated_low(float x, tam_bf16 h) {
+  const int32_t d = (int32_t)(__builtin_bit_cast(uint32_t, x) - __builtin_bit_cast(uint32_t, (float)h)) + 128;
   return (uint32_t)(d < 32767 ? d : 32767) >> 8 & 0xffu;
 }
-template <typename T>
-__device__ __forceinline__ float gated_value(T h, uint32_t low) {
-  const int32_t d = (int32_t)(low << 24) >> (std::is_same_v<T, tam_f16> ? 19 : 16);
-  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)h) + (uint32_t)d);
+__device__ __forceinline__ float gated_value(tam_bf16 h, uint32_t low) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)h) + (uint32_t)((int32_t)(low << 24) >> 16));
 }
 
 template <typename T>
@@ -66,17 +55,17 @@ __device__ __forceinline__ void gated_keep(char* at, const float (&g)[8], const 
     tam_store8(reinterpret_cast<T*>(at), g);
     tam_store8(reinterpret_cast<T*>(at) + 8, u);
   } else {
-    tam_oct<T> hg, hu;
+    tam_oct<tam_bf16> hg, hu;
     uint32_t low[4] = {};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      hg.v[j] = (T)g[j];
-      hu.v[j] = (T)u[j];
-      low[j / 4] |= gated_low<T>(g[j], hg.v[j]) << (j % 4 * 8);
-      low[2 + j / 4] |= gated_low<T>(u[j], hu.v[j]) << (j % 4 * 8);
+      hg.v[j] = (tam_bf16)g[j];
+      hu.v[j] = (tam_bf16)u[j];
+      low[j / 4] |= gated_low(g[j], hg.v[j]) << (j % 4 * 8);
+      low[2 + j / 4] |= gated_low(u[j], hu.v[j]) << (j % 4 * 8);
     }
-    *reinterpret_cast<tam_oct<T>*>(at) = hg;
-    *reinterpret_cast<tam_oct<T>*>(at + 16) = hu;
+    *reinterpret_cast<tam_oct<tam_bf16>*>(at) = hg;
+    *reinterpret_cast<tam_oct<tam_bf16>*>(at + 16) = hu;
     *reinterpret_cast<uint4*>(at + 32) = uint4{low[0], low[1], low[2], low[3]};
   }
 }
@@ -86,13 +75,14 @@ __device__ __forceinline__ void gated_recall(const char* at, float (&g)[8], floa
     tam_load8(reinterpret_cast<const T*>(at), g);
     tam_load8(reinterpret_cast<const T*>(at) + 8, u);
   } else {
-    const tam_oct<T> hg = *reinterpret_cast<const tam_oct<T>*>(at), hu = *reinterpret_cast<const tam_oct<T>*>(at + 16);
+    const tam_oct<tam_bf16> hg = *reinterpret_cast<const tam_oct<tam_bf16>*>(at);
+    const tam_oct<tam_bf16> hu = *reinterpret_cast<const tam_oct<tam_bf16>*>(at + 16);
     const uint4 l = *reinterpret_cast<const uint4*>(at + 32);
     const uint32_t low[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      g[j] = gated_value<T>(hg.v[j], low[j / 4] >> (j % 4 * 8));
-      u[j] = gated_value<T>(hu.v[j], low[2 + j / 4] >> (j % 4 * 8));
+      g[j] = gated_value(hg.v[j], low[j / 4] >> (j % 4 * 8));
+      u[j] = gated_value(hu.v[j], low[2 + j / 4] >> (j % 4 * 8));
     }
   }
 }

@@ -28,9 +28,9 @@ def gated_linear(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, *, activ
     activation: as linear's (None for a product of two projections).  Weights kept as
     (inputs, outputs) are passed as their transposed views and read in place, if both
     are.  The backward pass gives the gradients of every argument; for it the forward
-    pass keeps both products with 8 bits more than the dtype (6 bytes an output, 8 in
-    fp32), and their gradients are rounded to it before the products that make dx, dgate
-    and dup."""
+    pass keeps the upper 24 bits of both products' float32 (6 bytes an output; in fp32 all
+    of them, 8), and their gradients are rounded to the dtype, and have to lie in its range,
+    before the products that make dx, dgate and dup."""
     if activation not in _ACTIVATIONS:
         raise ValueError("turboadam_amd.gated_linear: activation must be one of "
                          f"{sorted(k for k in _ACTIVATIONS if k)}, got {activation!r}")
