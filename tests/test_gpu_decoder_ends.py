@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from tests.helpers import log
-from tests.test_gpu_decoder import DTYPES, TINY, UNIT, _check_rotary, _gen, _randn, _rotary_case, _turned, _within
+from tests.test_gpu_decoder import DTYPES, UNIT, _check_rotary, _gen, _rotary_case, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,66 @@ def test_gated_of_products_that_the_type_cannot_hold(rows, dt, in_out):
     for act in ("silu", "gelu_tanh", "gelu", "relu"):
         log(f"gated past the range {rows} {dt} {act} in_out={in_out}")
         _check_gated(x, gate, up, dh, dt, act)
+
+
+# --------------------------------------------- projection and cross entropy
+def _exact_case(rows, inputs, words, dt, scale):
+    """One column of x and w that is not zero: the logits are products of two numbers of the type, exact in fp32, so that
+    the loss alone is measured."""
+    g = _gen("exact", rows, words, scale)
+    x, w = torch.zeros(rows, inputs, device="cuda"), torch.zeros(words, inputs, device="cuda")
+    x[:, inputs // 2] = (1 + torch.rand(rows, generator=g, device="cuda")) * scale
+    w[:, inputs // 2] = 2 - torch.rand(words, generator=g, device="cuda") * 2.0 ** torch.randint(
+        -7, 3, (words,), generator=g, device="cuda")
+    few = torch.float16 if dt == "f16" else torch.bfloat16  # digits, in fp32 too
+    return [v.to(few).to(DTYPES[dt]) for v in (x, w)] + [torch.randint(0, words, (rows,), generator=g, device="cuda")]
+
+
+@pytest.mark.parametrize("scale", [1.0, 300.0, 9000.0])
+@pytest.mark.parametrize("rows,inputs,words", [(1, 9, 1000), (20, 64, 30011), (50, 24, 60), (40, 8, 10), (300, 40, 2777),
+                                               (700, 264, 5001), (4096, 264, 9973)])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_cross_loss_of_exact_logits_of_any_size(rows, inputs, words, dt, scale):
+    """Off by: a term's 2^x and its argument's rounding, 2^-23 (1 + |z - top|) of it, whose mean over the softmax is taken
+    here; fp32 sums, at most 16 + 4 + 8 terms in a part and parts / 16 + 26 of them one after another, 2^-24 a step, two
+    steps to a part (a factor and a sum); the difference to the target and the logarithm, 2^-23 of either."""
+    from turboadam_amd import linear_cross_entropy
+
+    x, w, t = _exact_case(rows, inputs, words, dt, scale)
+    log(f"cross of exact logits {rows}x{inputs}x{words} {dt} scale {scale}")
+    z = x.double() @ w.double().t()
+    assert torch.equal(z, (x.float() @ w.float().t()).double())  # exact
+    top, hit = z.amax(1), z.gather(1, t[:, None])[:, 0]
+    away = ((z - top[:, None]).exp() * (top[:, None] - z)).sum(1) / (z - top[:, None]).exp().sum(1)
+    want = z.logsumexp(1) - hit
+    log_sum = z.logsumexp(1) - top
+    bound = 2.0 ** -23 * (1 + away) + 2.0 ** -24 * (28 + 2 * (words / 256 + 26)) + 2.0 ** -23 * ((top - hit) + log_sum) + 2.0 ** -23 * want
+    _within(linear_cross_entropy(x, w, t, reduction="none"), want, bound, "loss")
+
+
+@pytest.mark.parametrize("rows,words", [(5, 1000), (60, 1000), (60, 40)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_cross_of_logits_near_the_end_of_float32(rows, words, dt):
+    """Logits of up to 1.5 * 2^127 either side of 0: far apart, so that a loss is the difference of two of them."""
+    from turboadam_amd import linear_cross_entropy
+
+    log(f"cross of the largest logits {rows} {words} {dt}")
+    x, w = torch.zeros(rows, 16, device="cuda"), torch.zeros(words, 16, device="cuda")
+    x[:, 3] = 2.0 ** 64
+    x[1::2, 3] = -(2.0 ** 64)
+    w[:, 3] = torch.arange(words, device="cuda") % 5 * 2.0 ** 60
+    w[17, 3], w[23, 3] = 1.5 * 2.0 ** 63, -1.25 * 2.0 ** 63
+    x, w = x.to(DTYPES[dt]).requires_grad_(), w.to(DTYPES[dt]).requires_grad_()
+    t = torch.arange(rows, device="cuda") % words
+    t[:4] = torch.tensor([17, 23, 2, 7], device="cuda")
+    odd = torch.arange(rows, device="cuda") % 2
+    t[(t == 17) & (odd == 1)] = t[(t == 23) & (odd == 0)] = 3  # whose losses float32 could not hold
+    z = x.detach().double() @ w.detach().double().t()
+    want = z.amax(1) - z.gather(1, t[:, None])[:, 0]
+    loss = linear_cross_entropy(x, w, t, reduction="none")
+    _within(loss, want, 2.0 ** -23 * want, "loss")
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    p = (z == z.amax(1, keepdim=True)).double()
+    p.scatter_add_(1, t[:, None], torch.full_like(want, -1.0)[:, None])
+    ref = p @ w.detach().double()  # two terms a row
+    _within(dx, ref, (UNIT[dt] + 2.0 ** -22) * ref.abs() + 2.0 ** -22 * (p.abs() @ w.detach().double().abs()), "dx")

@@ -34,31 +34,48 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// With the hardware's 2^x and the rounding of its argument off by up to 2^-23 (1 + |x|) of the result. That is below
+// 2^-16 for dz, which is rounded to 16 bits, wherever it is not 0; a sum's terms of a large |x| are as small as e^-|x|.
 template <typename T>
 __device__ __forceinline__ float cross_exp(float x) {
-  if constexpr (sizeof(T) == 2)  // 2^-22 of the result more than expf, below 2^-9 of the rounding
+  if constexpr (sizeof(T) == 2)
     return __builtin_amdgcn_exp2f(kLog2e * x);
   else
     return expf(x);
 }
 
-// The sum of exp(z - top) over a lane's values, top their maximum or more. A top of -inf
-// (words that cannot be, or columns past the last one) counts as 0: exp(-inf) is 0; a
-// NaN or an infinity makes the sum NaN.
+constexpr float kFarTop = 1073741824.0f;  // 2^30
+
+// The sum of exp(z - top) over a lane's values, top their maximum or more, but in 16-bit types for the
+// factor that cross_settled takes out. A top of -inf (words that cannot be, or columns past the last one) counts as
+// 0: exp(-inf) is 0; a NaN or an infinity makes the sum NaN.
 template <typename T, int N>
 __device__ __forceinline__ float cross_terms(const float (&z)[N], float top) {
   const float at = top == -INFINITY ? 0.0f : top;
   float sum = 0.f;
-  if constexpr (sizeof(T) == 2) {  // one multiplication and addition ahead of the hardware's 2^x
+  if (sizeof(T) == 2 && fabsf(at) < kFarTop) {  // one multiplication and addition ahead of the hardware's 2^x
     const float shift = -kLog2e * at;
 #pragma unroll
     for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], kLog2e, shift));
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum += expf(z[j] - at);
+    for (int j = 0; j < N; ++j) sum += cross_exp<T>(z[j] - at);
   }
   return sum;
 }
+
+// The sum without the rounding of log2e top, which all of its terms have alike: 2^-24 |top| of it, 6e-5 at logits of
+// 1000. Once for a row of a wave's or a workgroup's columns.
+template <typename T>
+__device__ __forceinline__ float cross_settled(float sum, float top) {
+  if constexpr (sizeof(T) == 2) {
+    if (fabsf(top) < kFarTop) sum *= __builtin_amdgcn_exp2f(__builtin_fmaf(-kLog2e, top, kLog2e * top));
+  }
+  return sum;
+}
+
+// log(sum of exp) - z of the target: the large numbers meet first, so that a loss is as exact at logits of 1000 as of 1.
+__device__ __forceinline__ float cross_loss(float top, float sum, float hit) { return (top - hit) + logf(sum); }
 
 // What the forward pass keeps, and what every kernel reads: all by the row's own number but
 // `index` and `target`, which are by its number among those that count.
@@ -227,7 +244,7 @@ __device__ __forceinline__ void cross_forward(const cross_logits_args& a, Tile& 
 #pragma unroll
     for (int w = 0; w < WN; ++w) {
       const float2 p = at[threadIdx.x * WN + w];
-      if (p.y != 0.f) all.y += p.y * cross_exp<T>(p.x - all.x);
+      if (p.y != 0.f) all.y += cross_settled<T>(p.y, p.x) * cross_exp<T>(p.x - all.x);
     }
     a.parts[(uint64_t)n * a.rows + row] = all;
   }
@@ -412,9 +429,9 @@ __global__ __launch_bounds__(1024) void tam_k_cross_join(cross_join_args a) {
   if (run == 0 && j < count) {
     for (int w = 1; w < 16; ++w) s = cross_add(s, at[w][lane]);
     const uint32_t row = a.r.index[j];
-    const float lse = a.r.target[j] < 0 ? NAN : s.x + logf(s.y);
-    a.r.lse[row] = lse;
-    a.loss[a.by_number ? j : row] = lse - a.hit[j];
+    const bool inside = a.r.target[j] >= 0;
+    a.r.lse[row] = inside ? s.x + logf(s.y) : NAN;
+    a.loss[a.by_number ? j : row] = inside ? cross_loss(s.x, s.y, a.hit[j]) : NAN;
   }
 }
 
@@ -436,9 +453,8 @@ __global__ __launch_bounds__(1024) void tam_k_cross_join_few(cross_join_args a) 
   }
   if (threadIdx.x == 0) {
     s = at[0];
-    const float lse = inside ? s.x + logf(s.y) : NAN;
-    if (a.r.lse) a.r.lse[row] = lse;
-    a.loss[row] = target == a.ignored ? 0.f : lse - hit;
+    if (a.r.lse) a.r.lse[row] = inside ? s.x + logf(s.y) : NAN;
+    a.loss[row] = target == a.ignored ? 0.f : (inside ? cross_loss(s.x, s.y, hit) : NAN);
   }
 }
 
@@ -556,7 +572,7 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_
       top = fmaxf(top, __shfl_xor(top, 1));
       all = cross_terms<T>(v, top);
       all += __shfl_xor(all, 1);
-      if (t % 2 == 0 && row < rows) a.parts[(uint64_t)row * a.groups + column] = float2{top, all};
+      if (t % 2 == 0 && row < rows) a.parts[(uint64_t)row * a.groups + column] = float2{top, cross_settled<T>(all, top)};
     }
   }
 }
@@ -652,9 +668,10 @@ __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_words(cross_wo
     hit += __shfl_xor(hit, d);
   }
   if (t % (2 * NT) == 0) {
-    const float lse = target >= 0 && target < (int64_t)a.words ? top + logf(all) : NAN;
-    if (a.lse) a.lse[row] = lse;
-    a.loss[row] = target == a.ignored ? 0.f : lse - hit;
+    const bool inside = target >= 0 && target < (int64_t)a.words;
+    all = cross_settled<T>(all, top);
+    if (a.lse) a.lse[row] = inside ? top + logf(all) : NAN;
+    a.loss[row] = target == a.ignored ? 0.f : (inside ? cross_loss(top, all, hit) : NAN);
   }
 }
 
