@@ -186,3 +186,22 @@ def test_cross_of_logits_near_the_end_of_float32(rows, words, dt):
     p.scatter_add_(1, t[:, None], torch.full_like(want, -1.0)[:, None])
     ref = p @ w.detach().double()  # two terms a row
     _within(dx, ref, (UNIT[dt] + 2.0 ** -22) * ref.abs() + 2.0 ** -22 * (p.abs() @ w.detach().double().abs()), "dx")
+
+
+@pytest.mark.parametrize("rows,words", [(6, 100), (70, 100), (70, 30)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_cross_gradients_of_the_largest_losses_gradients(rows, words, dt):
+    """Gradients of single losses past 2^127 (no power of two in fp32 lies above them) beside others, with a weight so
+    small that dx is finite: the same digits as of gradients 2^127 times smaller, which other tests pin."""
+    from tests.test_gpu_decoder import _cross_case
+    from turboadam_amd import linear_cross_entropy
+
+    log(f"cross of the largest gradients {rows} {words} {dt}")
+    x, w, t, dl = _cross_case(rows, 40, words, dt, 0.2, scale=2.0 ** -9)
+    dl[1], dl[3] = 1.75, -1.5
+    leaves = [v.requires_grad_() for v in (x, w)]
+    small = torch.autograd.grad(linear_cross_entropy(*leaves, t, reduction="none"), leaves, dl)
+    large = torch.autograd.grad(linear_cross_entropy(*leaves, t, reduction="none"), leaves[:1], dl * 2.0 ** 127)
+    for a, b in zip(large, small):  # a power of two changes no bit but of what lies below 2^-126 in the second
+        a, b = a.double() * 2.0 ** -127, b.double()
+        assert bool(torch.isfinite(a).all()) and bool(((a - b).abs() <= 2.0 ** -126).all())

@@ -22,7 +22,7 @@
 // later kernel reads their number from the device: its tiles of rows past it return at once, and
 // sums over rows end there.  So NaN in a padded row reaches nothing.
 //
-// dz is held as (exp(z - lse) - onehot) * w, |w| <= 1 (fp16: times 2^14, as a softmax
+// dz is held as (exp(z - lse) - onehot) * w, |w| < 2 (fp16: times 2^14, as a softmax
 // over 10^5 words lies below fp16's numbers otherwise), and the results are multiplied by
 // the power of two or the factor that is missing (scale) when they are rounded.
 #include "tam_few.h"
@@ -709,7 +709,7 @@ struct cross_weights_args {
 
 // Each row's weight, and scale; 8192 rows 6.5 us, one workgroup's trips to memory. A gradient for
 // each row: scale is the least power of two above the largest finite one, so that dividing by it
-// rounds nothing.
+// rounds nothing; but 2^127 for those above it (a row's weight is then up to 2), and 2^-100 at least.
 __global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a) {
   __shared__ float top[1024];
   const uint32_t count = *a.r.count;
@@ -732,7 +732,7 @@ __global__ __launch_bounds__(1024) void tam_k_cross_weights(cross_weights_args a
   __syncthreads();
   int power;
   frexpf(top[0], &power);
-  power = power < -100 ? -100 : power;
+  power = power < -100 ? -100 : (power > 127 ? 127 : power);
   for (uint32_t j = threadIdx.x; j < count; j += 1024) {
     const uint32_t row = a.r.index[j];
     a.row[j] = {a.r.lse[row], ldexpf(a.dloss[(int64_t)row * a.stride], -power) * a.lift, a.r.target[j], 0};
