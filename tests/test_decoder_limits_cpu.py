@@ -14,3 +14,22 @@ def test_rotary_eps_is_zero_or_a_normal_number(eps, code):
     for backward in (0, 1):
         rc, _, msg = _need(_lib.load().tam_rotary_workspace, _rotary(eps=eps), backward)
         assert rc == code and (rc == 0 or "eps" in msg), (rc, msg)
+
+
+def _tiles(fn, d):
+    out = (ctypes.c_uint32 * 4)()
+    assert fn(ctypes.byref(d), 1, out) == 0
+    return list(out)
+
+
+def test_weights_gradients_alone_are_cut_by_their_own_sums():
+    """Without dx the estimate takes the rows' sums, not those of the product that is not run: these calls' sums are cut, or
+    their pieces and tiles are those of the whole pass, where the other length had 1 part, 4096 words and tiles of 128."""
+    lib, bf16, f32 = _lib.load(), _lib.TAM_DTYPE_BF16, _lib.TAM_DTYPE_F32
+    one = _gated(rows=8192, inputs=256, outputs=8192, dtype=bf16, dx=None)
+    assert _tiles(lib.tam_gated_tiles, one) == [0, 0, 128, 2]
+    for kw, piece, tile, parts in ((dict(rows=8192, inputs=4096, vocabulary=128256, dtype=bf16), 32256, 256, 1),
+                                   (dict(rows=8192, inputs=768, vocabulary=50257, dtype=bf16), 21760, 256, 1),
+                                   (dict(rows=1237, inputs=515, vocabulary=9973, dtype=f32), 9984, 64, 2)):
+        got = _tiles(lib.tam_cross_tiles, _cross(dx=None, **kw))
+        assert got[1:] == [piece, tile, 1 << 16 | parts], (kw, got)

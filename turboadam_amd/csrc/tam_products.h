@@ -127,10 +127,10 @@ inline shape choose(uint64_t rows, uint64_t cols, uint64_t k, uint32_t dtype) {
   return best;
 }
 
-// us of n units of k one after another on the places of a card, behind `ahead` units of `ahead_k`
-// (the longer first): each unit to the place that is free first.
+// us of n1 units of k1 and n2 of k2 on the places of a card, the longer first: each unit to the place that
+// is free first.
 inline double units_us(const tam_tile_rate& t, uint64_t n1, double k1, uint64_t n2, double k2, double cus) {
-  if (k1 < k2) return n2 ? units_us(t, n2, k2, n1, k1, cus) : units_us(t, n1, k2, 0, 0, cus);
+  if (k1 < k2 && n2) return units_us(t, n2, k2, n1, k1, cus);
   const uint64_t places = (uint64_t)cus * t.resident, all = n1 + n2;
   const int with = all >= places ? t.resident : (int)tam_div_up(all ? all : 1, (uint64_t)cus);  // on a compute unit
   const double per = all <= (uint64_t)(0.5 * cus) ? t.half : t.per_k[with - 1];
