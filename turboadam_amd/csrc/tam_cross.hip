@@ -751,11 +751,12 @@ struct cross_product_args {
   const uint32_t* index;   // of dx's rows
 };
 
-// A piece's products: units of dw, then units of dx's share, in one launch, so that neither leaves
-// compute units empty at its end.
+// A piece's products: units of dw and units of dx's share in one launch, so that neither leaves
+// compute units empty at its end: those of the longer sums first, so that the shorter fill the last round.
 struct cross_products_args {
   cross_product_args w, x;
   uint32_t w_units;        // of w.tm * w.tn * w.parts
+  uint32_t w_first;        // the first one's workgroup: 0, or behind dx's
   const uint32_t* count;
   const float* scale;
 };
@@ -833,10 +834,10 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, true> Tile;
   __shared__ __attribute__((aligned(16))) char smem[Tile::LDS];
   const uint32_t count = *a.count;
-  if (blockIdx.x < a.w_units)
-    cross_product<T, TILE, WM, WN, true>(a.w, blockIdx.x, count, a.scale, smem);
+  if (blockIdx.x - a.w_first < a.w_units)
+    cross_product<T, TILE, WM, WN, true>(a.w, blockIdx.x - a.w_first, count, a.scale, smem);
   else
-    cross_product<T, TILE, WM, WN, false>(a.x, blockIdx.x - a.w_units, count, a.scale, smem);
+    cross_product<T, TILE, WM, WN, false>(a.x, blockIdx.x < a.w_first ? blockIdx.x : blockIdx.x - a.w_units, count, a.scale, smem);
 }
 
 // out[row] = the parts' sums of the row's number in their order, times scale; zeros for
@@ -1343,7 +1344,9 @@ int backward(const TamCross* d, call& c) {
       p.x.out = d->dx;
       p.x.index = r.index;
       p.x.add = first != 0;
-      units += (uint64_t)p.x.tm * across * both.x_parts;
+      const uint64_t x_units = (uint64_t)p.x.tm * across * both.x_parts;
+      if (units && (uint64_t)cols * both.w_parts > (uint64_t)rows * both.x_parts) p.w_first = (uint32_t)x_units;
+      units += x_units;
     }
     if (units >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
 #define TAM_PRODUCTS(T) launch_products<T>(both.tile, p, (uint32_t)units, c.stream)

@@ -333,10 +333,11 @@ struct gated_product_args {
   gated_out e;
 };
 
-// The weights' gradients, then dx, in one launch, so that neither leaves compute units empty at its end.
+// The weights' gradients and dx in one launch, so that neither leaves compute units empty at its end.
 struct gated_products_args {
   gated_product_args w, x;
   uint32_t w_units;     // of w.tm * w.tn and its parts
+  uint32_t w_first;     // the first one's workgroup: 0, or behind dx's
 };
 
 template <typename T, typename Tile, int TILE, int TERMS>
@@ -363,8 +364,9 @@ __device__ __forceinline__ void gated_product(const gated_product_args& a, uint3
       [](uint32_t, uint32_t, const float*, int) {});
 }
 
-// One launch for both products, the longer sums first, so that the second fills the places that
-// the first leaves empty in its last round. Bound by the matrix cores: 8192 x 4096 -> 14336 bf16 2739 us
+// One launch for both products, the longer sums first (dx's, where 2 outputs in its parts are more than the rows
+// in theirs), so that the second fills the places that the first leaves empty in its last round (2048 x 2048 -> 8192 bf16
+// both ways 387 us, 427 with dx behind). Bound by the matrix cores: 8192 x 4096 -> 14336 bf16 2739 us
 // for 3.85 Tflop, 1405 TFLOP/s; 2048 x 768 -> 2048 fp16 48, fp32 1531 x 777 -> 1001 104.
 // IN_OUT: of weights stored [inputs][outputs], along which dx's sums run.
 template <typename T, int TILE, int WM, int WN, bool IN_OUT>
@@ -373,10 +375,10 @@ __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_gated_
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), IN_OUT, true> Input;
   static_assert(Weight::LDS == Input::LDS, "one size");
   __shared__ __attribute__((aligned(16))) char smem[Weight::LDS];
-  if (blockIdx.x < a.w_units)
-    gated_product<T, Weight, TILE, TAM_ONE_TERM>(a.w, blockIdx.x, smem);
+  if (blockIdx.x - a.w_first < a.w_units)
+    gated_product<T, Weight, TILE, TAM_ONE_TERM>(a.w, blockIdx.x - a.w_first, smem);
   else
-    gated_product<T, Input, TILE, TAM_TWO_PRODUCTS>(a.x, blockIdx.x - a.w_units, smem);
+    gated_product<T, Input, TILE, TAM_TWO_PRODUCTS>(a.x, blockIdx.x < a.w_first ? blockIdx.x : blockIdx.x - a.w_units, smem);
 }
 
 // The parts' sums in their order: 8 columns to a thread.
@@ -644,8 +646,12 @@ int backward(const TamGated* d, call& c) {
     units = lay_out(c, a.w, d->w_in_out ? both : x, d->w_in_out ? x : both, {1, 0, 0}, w, tile, ew);
     a.w_units = (uint32_t)units;
   }
-  if (d->dx)
-    units += lay_out(c, a.x, gate, both, {2, (int64_t)((intptr_t)up.p - (intptr_t)gate.p), (int64_t)ld * size}, in, tile, ex);
+  if (d->dx) {
+    const uint64_t x_units =
+        lay_out(c, a.x, gate, both, {2, (int64_t)((intptr_t)up.p - (intptr_t)gate.p), (int64_t)ld * size}, in, tile, ex);
+    if (units && in.k / in.parts > w.k / w.parts) a.w_first = (uint32_t)x_units;
+    units += x_units;
+  }
   if (c.dry) return TAM_OK;
   if (units >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
 #define TAM_PRODUCTS(T) launch_products<T>(tile, d->w_in_out != 0, a, (uint32_t)units, c.stream)
