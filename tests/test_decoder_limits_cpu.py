@@ -33,3 +33,24 @@ def test_weights_gradients_alone_are_cut_by_their_own_sums():
                                    (dict(rows=1237, inputs=515, vocabulary=9973, dtype=f32), 9984, 64, 2)):
         got = _tiles(lib.tam_cross_tiles, _cross(dx=None, **kw))
         assert got[1:] == [piece, tile, 1 << 16 | parts], (kw, got)
+
+
+def test_cross_takes_no_memory_for_copies_that_nothing_reads():
+    """x's rows are copied for dw and for tiles of logits, w's (odd ones) for dx and those: a pass without either takes
+    its gradient of the logits and a few bytes a row."""
+    lib, bf16 = _lib.load(), _lib.TAM_DTYPE_BF16
+
+    def need(**kw):
+        rc, bytes_, msg = _need(lib.tam_cross_workspace, _cross(dtype=bf16, **kw), 1)
+        assert rc == 0, msg
+        return bytes_
+
+    many = dict(rows=540001, inputs=4096, vocabulary=40)
+    assert need(dw=None, **many) < 540001 * (128 + 16) + 4096
+    assert need(**many) > 540001 * 4096 * 2
+    few = dict(rows=8, inputs=7191, vocabulary=72376)
+    dz, w = 8 * (72376 + 64) * 2, 72376 * 7191 * 2
+    assert need(dx=None, **few) < dz + 8 * 7232 * 2 + 4096  # with x's rows
+    assert w < need(dw=None, **few) < w + 72376 * 82 + dz + 33 * 8 * 7191 * 4  # with w's, and dx's sums in parts
+    assert need(dw=None, rows=8, inputs=8000, vocabulary=40) < 8 * 128 + 4096
+    assert need(dw=None, dx=None, **few) == 0

@@ -205,3 +205,22 @@ def test_cross_gradients_of_the_largest_losses_gradients(rows, words, dt):
     for a, b in zip(large, small):  # a power of two changes no bit but of what lies below 2^-126 in the second
         a, b = a.double() * 2.0 ** -127, b.double()
         assert bool(torch.isfinite(a).all()) and bool(((a - b).abs() <= 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("rows,inputs,words", [(8, 331, 5003), (30, 64, 700), (70, 331, 40), (90, 48, 333)])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_cross_gradients_of_one_argument(rows, inputs, words, dt):
+    """Passes for dx or dw alone, which copy nothing that they do not read; their sums may be cut otherwise than those of
+    both, so either is within its rounding and 2^-18 of its norm of the other (sums of up to 5003 terms, 2^-23 of their
+    parts a step, of random signs)."""
+    from tests.test_gpu_decoder import _cross_case
+    from turboadam_amd import linear_cross_entropy
+
+    log(f"cross of one gradient {rows}x{inputs}x{words} {dt}")
+    x, w, t, _ = _cross_case(rows, inputs, words, dt, 0.2)
+    leaves = [v.requires_grad_() for v in (x, w)]
+    both = torch.autograd.grad(linear_cross_entropy(*leaves, t), leaves)
+    for i in range(2):
+        some = [v.detach().requires_grad_(j == i) for j, v in enumerate((x, w))]
+        got, = torch.autograd.grad(linear_cross_entropy(*some, t), [some[i]])
+        assert float((got.double() - both[i].double()).norm()) <= (2 * UNIT[dt] + 2.0 ** -18) * float(both[i].double().norm()), i

@@ -960,16 +960,19 @@ int number_rows(const TamCross* d, const cross_rows& r, float* loss, hipStream_t
     }                                                      \
   } while (0)
 
-// The rows of x that count, and w, as the tiles read them. kept: where the rows lie, or are to lie (the
-// workspace where it is null).
-int operands(const TamCross* d, call& c, const cross_rows& r, void* kept, bool gather, matrix& x, matrix& w) {
-  const uint32_t size = kSize[c.dtype], halves = size / 2, inputs = (uint32_t)d->inputs;
-  w = matrix_of(d->w, d->ldw, d->vocabulary, d->inputs, size);
-  const int rc = whole_rows(c, {&w});
-  if (rc != TAM_OK) return rc;
-  const uint32_t ld = aligned_ld(inputs, size);
+// The rows of x that count, and w, as the tiles read them, where a product does. kept: where the rows lie or, in
+// the forward pass, are to lie (the workspace where it is null).
+int operands(const TamCross* d, call& c, const cross_rows& r, void* kept, bool back, bool read_x, bool read_w, matrix& x,
+             matrix& w) {
+  const uint32_t size = kSize[c.dtype], halves = size / 2, inputs = (uint32_t)d->inputs, ld = aligned_ld(inputs, size);
+  if (read_w) {
+    w = matrix_of(d->w, d->ldw, d->vocabulary, d->inputs, size);
+    const int rc = whole_rows(c, {&w});
+    if (rc != TAM_OK) return rc;
+  }
+  if (!read_x) return TAM_OK;
   x = {kept ? (char*)kept + rows_bytes(d->rows) : c.ws.take(d->rows * ld * size), ld, d->rows, inputs, true};
-  if (!c.dry && inputs && gather) {
+  if (!c.dry && inputs && !(back && kept)) {
     const dim3 grid((uint32_t)tam_div_up(d->rows * (ld * halves / 8), 256)), block(256);
     hipLaunchKernelGGL(tam_k_cross_gather, grid, block, 0, c.stream, (const tam_f16*)d->x, d->ldx * halves, inputs * halves, r,
                        (uint32_t)d->rows, (tam_f16*)x.p, ld * halves);
@@ -1154,7 +1157,7 @@ int forward(const TamCross* d, call& c) {
       const int tile = tile_of(rows, d->vocabulary, d->inputs, c.dtype);
       if (c.tiles) c.tiles[0] = (uint32_t)tile;
       matrix x, w;
-      const int rc = operands(d, c, r, d->kept, true, x, w);
+      const int rc = operands(d, c, r, d->kept, false, true, true, x, w);
       if (rc != TAM_OK) return rc;
       cross_logits_args a = logits_of(d, x, w, r, 0, d->vocabulary, tile, kSize[c.dtype]);
       if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
@@ -1252,18 +1255,18 @@ int backward(const TamCross* d, call& c) {
     hipLaunchKernelGGL(tam_k_cross_weights, dim3(1), dim3(1024), 0, c.stream, a);
     TAM_OP_LAUNCHED("the rows' weights");
   }
-  matrix x, w;
-  const bool is_few = few(d);
-  // of few words only dw reads x
-  int rc = operands(d, c, r, is_few ? nullptr : d->kept, few_words(d) ? d->dw != nullptr : is_few, x, w);
-  if (rc != TAM_OK) return rc;
+  matrix x = {}, w = {};
   const uint64_t piece = piece_of(d, size), widest = d->vocabulary < piece ? d->vocabulary : piece;
+  // otherwise dz comes from the z that was kept, or straight from x and w
+  const bool is_few = few(d), tiles = !few_words(d) && !(is_few && widest == d->vocabulary);
+  const int rc = operands(d, c, r, is_few ? nullptr : d->kept, true, tiles || d->dw, tiles || d->dx, x, w);
+  if (rc != TAM_OK) return rc;
   const uint32_t ld = aligned_ld((uint32_t)widest, size);
   void* dz = c.ws.take((uint64_t)rows * ld * size);
   const int tile_z = tile_of(rows, widest, inputs, c.dtype);
   const pair_shape both = choose_pair(rows, inputs, widest, d->dw, d->dx, c.dtype);
   if (c.tiles) {
-    c.tiles[0] = is_few && widest == d->vocabulary ? 0 : (uint32_t)tile_z;
+    c.tiles[0] = tiles ? (uint32_t)tile_z : 0;
     c.tiles[1] = (uint32_t)piece;
     c.tiles[2] = (uint32_t)both.tile;
     c.tiles[3] = both.x_parts << 16 | both.w_parts;
@@ -1276,11 +1279,6 @@ int backward(const TamCross* d, call& c) {
   if (c.dry) return TAM_OK;
   for (uint64_t first = 0; first < d->vocabulary; first += piece) {
     const uint32_t cols = (uint32_t)(d->vocabulary - first < piece ? d->vocabulary - first : piece);
-    cross_logits_args a = logits_of(d, x, w, r, first, cols, tile_z, size);
-    if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
-    a.row = row;
-    a.dz = dz;
-    a.ld = ld;
     if (few_words(d)) {
       const uint32_t ldz = words_ld(d);
       const float* const kept = (const float*)((const char*)d->kept + rows_bytes(rows));
@@ -1288,7 +1286,7 @@ int backward(const TamCross* d, call& c) {
 #define TAM_WORDS_DZ(T) \
   hipLaunchKernelGGL(tam_k_cross_words_dz<T>, grid, block, 0, c.stream, kept, ldz, cols, r, row, (T*)dz, (uint64_t)ld)
       TAM_OF_TYPE(c, TAM_WORDS_DZ);
-    } else if (is_few && cols == d->vocabulary) {
+    } else if (!tiles) {
       cross_few_args f = {};
       f.x = d->x;
       f.w = d->w;
@@ -1306,6 +1304,11 @@ int backward(const TamCross* d, call& c) {
 #define TAM_FEW_DZ(T) hipLaunchKernelGGL((tam_k_cross_few<T, 2, true>), grid, block, 0, c.stream, f)
       TAM_OF_TYPE(c, TAM_FEW_DZ);
     } else {
+      cross_logits_args a = logits_of(d, x, w, r, first, cols, tile_z, size);
+      if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+      a.row = row;
+      a.dz = dz;
+      a.ld = ld;
 #define TAM_DZ(T) launch_logits<T, true>(tile_z, a, c.stream)
       TAM_OF_TYPE(c, TAM_DZ);
     }
