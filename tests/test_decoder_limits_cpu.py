@@ -54,3 +54,26 @@ def test_cross_takes_no_memory_for_copies_that_nothing_reads():
     assert w < need(dw=None, **few) < w + 72376 * 82 + dz + 33 * 8 * 7191 * 4  # with w's, and dx's sums in parts
     assert need(dw=None, rows=8, inputs=8000, vocabulary=40) < 8 * 128 + 4096
     assert need(dw=None, dx=None, **few) == 0
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+def test_launches_of_too_many_threads_are_refused_before_any(backward):
+    """A launch takes fewer than 2^32 threads: 2^24 workgroups of 256. What needs more is refused where the workspace's size
+    is asked, and what is just below is not."""
+    lib, f32, bf16 = _lib.load(), _lib.TAM_DTYPE_F32, _lib.TAM_DTYPE_BF16
+    most = 1 << 31
+    for entry, make, kw, code in [
+            # 64-tiles of short rows: 2^25 of them, and 2^23
+            (lib.tam_gated_workspace, _gated, dict(rows=most - 1, inputs=8, outputs=16), 4),
+            (lib.tam_gated_workspace, _gated, dict(rows=most >> 3, inputs=8, outputs=16), 0),
+            (lib.tam_cross_workspace, _cross, dict(rows=most - 1, inputs=8, vocabulary=1000), 4),
+            (lib.tam_cross_workspace, _cross, dict(rows=1 << 20, inputs=8, vocabulary=1000), 0),
+            # copies of odd rows: 2^32 units of 8, and 2^28
+            (lib.tam_gated_workspace, _gated, dict(rows=1 << 27, inputs=249, outputs=8), 4),
+            (lib.tam_gated_workspace, _gated, dict(rows=1 << 23, inputs=249, outputs=8), 0),
+            # columns of few rows: 2^27 of them are 2^32 threads, but a backward pass takes 2^20 at a time
+            (lib.tam_cross_workspace, _cross, dict(rows=2, inputs=8, vocabulary=1 << 28), 0 if backward else 4),
+            (lib.tam_cross_workspace, _cross, dict(rows=2, inputs=8, vocabulary=1 << 20), 0)]:
+        for dtype in (f32, bf16):
+            rc, _, msg = _need(entry, make(dtype=dtype, **kw), backward)
+            assert rc == code and (rc == 0 or "2^32" in msg), (kw, dtype, rc, msg)

@@ -882,11 +882,6 @@ __global__ __launch_bounds__(256) void tam_k_cross_clear(tam_f16* dx, uint64_t r
   }
 }
 
-__global__ __launch_bounds__(256) void tam_k_cross_zero(tam_f16* out, uint64_t n) {
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) out[i] = (tam_f16)0.0f;  // zero has the same bits in every type
-}
-
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -972,8 +967,11 @@ int operands(const TamCross* d, call& c, const cross_rows& r, void* kept, bool b
   }
   if (!read_x) return TAM_OK;
   x = {kept ? (char*)kept + rows_bytes(d->rows) : c.ws.take(d->rows * ld * size), ld, d->rows, inputs, true};
-  if (!c.dry && inputs && !(back && kept)) {
-    const dim3 grid((uint32_t)tam_div_up(d->rows * (ld * halves / 8), 256)), block(256);
+  const uint64_t copies = back && kept ? 0 : tam_div_up(d->rows * (ld * halves / 8), 256);
+  const int rc = room(copies, 256);
+  if (rc != TAM_OK) return rc;
+  if (!c.dry && inputs && copies) {
+    const dim3 grid((uint32_t)copies), block(256);
     hipLaunchKernelGGL(tam_k_cross_gather, grid, block, 0, c.stream, (const tam_f16*)d->x, d->ldx * halves, inputs * halves, r,
                        (uint32_t)d->rows, (tam_f16*)x.p, ld * halves);
     TAM_OP_LAUNCHED("the rows' copy");
@@ -1115,6 +1113,8 @@ int forward(const TamCross* d, call& c) {
     } else if (is_few) {
       const uint32_t groups = (uint32_t)tam_div_up(d->vocabulary, 16);
       float2* parts = (float2*)c.ws.take(8ull * rows * groups);
+      const int rc = room(groups, 64 * TAM_FEW_WAVES);
+      if (rc != TAM_OK) return rc;
       if (!c.dry) {
         if (d->kept) {
           const int rc = number_rows(d, r, nullptr, c.stream);
@@ -1157,10 +1157,11 @@ int forward(const TamCross* d, call& c) {
       const int tile = tile_of(rows, d->vocabulary, d->inputs, c.dtype);
       if (c.tiles) c.tiles[0] = (uint32_t)tile;
       matrix x, w;
-      const int rc = operands(d, c, r, d->kept, false, true, true, x, w);
+      int rc = operands(d, c, r, d->kept, false, true, true, x, w);
+      if (rc == TAM_OK) rc = room_of_tiles(tam_div_up(rows, tile) * tam_div_up(d->vocabulary, tile), tile, true);
+      if (rc == TAM_OK) rc = room(tam_div_up(rows, 64), 1024);
       if (rc != TAM_OK) return rc;
       cross_logits_args a = logits_of(d, x, w, r, 0, d->vocabulary, tile, kSize[c.dtype]);
-      if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
       a.parts = (float2*)c.ws.take(8ull * rows * a.tn);
       a.hit = hit;
       if (!c.dry) {
@@ -1234,18 +1235,10 @@ uint64_t piece_of(const TamCross* d, uint32_t size) {
   return best;
 }
 
-int zero(const call& c, void* p, uint64_t elements) {
-  if (c.dry || !p || !elements) return TAM_OK;
-  const uint64_t halves = elements * (kSize[c.dtype] / 2);
-  hipLaunchKernelGGL(tam_k_cross_zero, dim3((uint32_t)tam_div_up(halves, 256)), dim3(256), 0, c.stream, (tam_f16*)p, halves);
-  TAM_OP_LAUNCHED("an empty sum");
-  return TAM_OK;
-}
-
 int backward(const TamCross* d, call& c) {
   if (!d->dx && !d->dw) return TAM_OK;
   const uint32_t rows = (uint32_t)d->rows, inputs = (uint32_t)d->inputs, size = kSize[c.dtype];
-  if (!rows || !inputs) return zero(c, d->dw, d->vocabulary * d->inputs);
+  if (!rows || !inputs) return zeros(c, d->dw, d->vocabulary * d->inputs);
   const cross_rows r = rows_in(d->kept, rows);
   cross_row* row = (cross_row*)c.ws.take(sizeof(cross_row) * (uint64_t)rows);
   float* scale = (float*)c.ws.take(4);
@@ -1259,7 +1252,7 @@ int backward(const TamCross* d, call& c) {
   const uint64_t piece = piece_of(d, size), widest = d->vocabulary < piece ? d->vocabulary : piece;
   // otherwise dz comes from the z that was kept, or straight from x and w
   const bool is_few = few(d), tiles = !few_words(d) && !(is_few && widest == d->vocabulary);
-  const int rc = operands(d, c, r, is_few ? nullptr : d->kept, true, tiles || d->dw, tiles || d->dx, x, w);
+  int rc = operands(d, c, r, is_few ? nullptr : d->kept, true, tiles || d->dw, tiles || d->dx, x, w);
   if (rc != TAM_OK) return rc;
   const uint32_t ld = aligned_ld((uint32_t)widest, size);
   void* dz = c.ws.take((uint64_t)rows * ld * size);
@@ -1276,7 +1269,15 @@ int backward(const TamCross* d, call& c) {
   float* dx_sums = d->dx && !direct ? (float*)c.ws.take(4ull * both.x_parts * rows * inputs) : nullptr;
   float* dw_sums = d->dw && both.w_parts > 1 ? (float*)c.ws.take(4ull * both.w_parts * widest * inputs) : nullptr;
   const uint32_t across = (uint32_t)tam_div_up(inputs, both.tile);
-  if (c.dry) return TAM_OK;
+  const uint64_t eights = tam_div_up(inputs, 8), joins_w = tam_div_up(widest * eights, 256), joins_x = tam_div_up(rows * eights, 256);
+  const uint64_t units_w = d->dw ? tam_div_up(widest, both.tile) * across * both.w_parts : 0;
+  const uint64_t units_x = d->dx ? tam_div_up(rows, both.tile) * (uint64_t)across * both.x_parts : 0;
+  rc = tiles ? room_of_tiles(tam_div_up(rows, tile_z) * tam_div_up(widest, tile_z), tile_z, true)
+             : room(tam_div_up(widest, 16), 64 * TAM_FEW_WAVES);
+  if (rc == TAM_OK) rc = room_of_tiles(units_w + units_x, both.tile, false);
+  if (rc == TAM_OK && dw_sums) rc = room(joins_w, 256);
+  if (rc == TAM_OK && d->dx && !direct) rc = room(joins_x, 256);
+  if (rc != TAM_OK || c.dry) return rc;
   for (uint64_t first = 0; first < d->vocabulary; first += piece) {
     const uint32_t cols = (uint32_t)(d->vocabulary - first < piece ? d->vocabulary - first : piece);
     if (few_words(d)) {
@@ -1305,7 +1306,6 @@ int backward(const TamCross* d, call& c) {
       TAM_OF_TYPE(c, TAM_FEW_DZ);
     } else {
       cross_logits_args a = logits_of(d, x, w, r, first, cols, tile_z, size);
-      if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
       a.row = row;
       a.dz = dz;
       a.ld = ld;
@@ -1351,12 +1351,11 @@ int backward(const TamCross* d, call& c) {
       if (units && (uint64_t)cols * both.w_parts > (uint64_t)rows * both.x_parts) p.w_first = (uint32_t)x_units;
       units += x_units;
     }
-    if (units >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
 #define TAM_PRODUCTS(T) launch_products<T>(both.tile, p, (uint32_t)units, c.stream)
     TAM_OF_TYPE(c, TAM_PRODUCTS);
     TAM_OP_LAUNCHED("dx and dw");
     if (dw_sums) {
-      const dim3 grid((uint32_t)tam_div_up((uint64_t)cols * tam_div_up(inputs, 8), 256)), block(256);
+      const dim3 grid((uint32_t)tam_div_up(cols * eights, 256)), block(256);
 #define TAM_DW_OUT(T)                                                                                                     \
   hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dw_sums, both.w_parts, (uint64_t)cols, inputs, nullptr, \
                      nullptr, 0u, 0ull, scale, (T*)p.w.out)
@@ -1370,7 +1369,7 @@ int backward(const TamCross* d, call& c) {
     hipLaunchKernelGGL(tam_k_cross_clear, grid, block, 0, c.stream, (tam_f16*)d->dx, (uint64_t)rows, halves, r.place);
     TAM_OP_LAUNCHED("rows without a gradient");
   } else if (d->dx) {
-    const dim3 grid((uint32_t)tam_div_up((uint64_t)rows * tam_div_up(inputs, 8), 256)), block(256);
+    const dim3 grid((uint32_t)joins_x), block(256);
 #define TAM_DX_OUT(T)                                                                                                        \
   hipLaunchKernelGGL(tam_k_cross_out<T>, grid, block, 0, c.stream, dx_sums, both.x_parts, (uint64_t)rows, inputs, r.place, \
                      r.count, (uint32_t)both.tile, widest, scale, (T*)d->dx)

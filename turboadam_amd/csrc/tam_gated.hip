@@ -399,11 +399,6 @@ __global__ __launch_bounds__(256) void tam_k_gated_sum(const float* partial, uin
   gated_put<T>(e, row, col, v);
 }
 
-__global__ __launch_bounds__(256) void tam_k_gated_zero(uint32_t* out, uint64_t words, uint64_t halves) {
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < words) out[i] = 0;
-  if (i == 0 && halves & 1) reinterpret_cast<uint16_t*>(out)[halves - 1] = 0;
-}
 
 // ---------------------------------------------------------------------------
 // host side
@@ -524,15 +519,6 @@ int choose_both(extent& w, extent& x, uint32_t dtype) {
   return best;
 }
 
-int zero(call& c, void* p, uint64_t elements) {
-  if (c.dry || !p || !elements) return TAM_OK;
-  const uint64_t halves = elements * kSize[c.dtype] / 2;
-  hipLaunchKernelGGL(tam_k_gated_zero, dim3((uint32_t)tam_div_up(halves / 2 + 1, 256)), dim3(256), 0, c.stream, (uint32_t*)p,
-                     halves / 2, halves);
-  TAM_OP_LAUNCHED("an empty sum");
-  return TAM_OK;
-}
-
 int forward(const TamGated* d, call& c) {
   if (d->rows == 0 || d->outputs == 0) return TAM_OK;
   const gated_epilogue e = {d->h, (char*)d->kept, (uint32_t)d->rows, (uint32_t)d->outputs, d->activation};
@@ -556,24 +542,27 @@ int forward(const TamGated* d, call& c) {
     c.tiles[1] = s.parts;
   }
   matrix x = x_of(d), gate = w_of(d, d->gate), up = w_of(d, d->up);
-  const int rc = whole_rows(c, {&x, &gate, &up});
+  int rc = whole_rows(c, {&x, &gate, &up});
   if (rc != TAM_OK) return rc;
   gated_args a = {};
   if (s.parts > 1) a.partial = (float*)c.ws.take(2ull * s.parts * e.rows * e.cols * 4);
-  if (c.dry) return TAM_OK;
+  const uint64_t tm = tam_div_up(e.rows, s.tile), tn = tam_div_up(e.cols, s.tile / 2);
+  const uint64_t joins = tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256);
+  rc = room_of_tiles(tm * tn, s.tile, true);
+  if (rc == TAM_OK && s.parts > 1) rc = room(joins, 256);
+  if (rc != TAM_OK || c.dry) return rc;
   a.P = {operand_of(gate, e.cols, size), operand_of(up, e.cols, size)};
   a.Q = operand_of(x, e.rows, size);
   a.k = d->inputs;
   a.k_part = s.parts > 1 ? tam_up(tam_div_up(a.k, s.parts), 64) : a.k;
-  a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
-  a.tn = (uint32_t)tam_div_up(e.cols, s.tile / 2);
+  a.tm = (uint32_t)tm;
+  a.tn = (uint32_t)tn;
   a.e = e;
-  if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
 #define TAM_GATED(T) launch_gated<T>(s.tile, !d->w_in_out, a, s.parts, c.stream)
   TAM_OF_TYPE(c, TAM_GATED);
   TAM_OP_LAUNCHED("the gated products");
   if (s.parts > 1) {
-    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
+    const dim3 grid((uint32_t)joins), block(256);
 #define TAM_JOIN(T) hipLaunchKernelGGL(tam_k_gated_join<T>, grid, block, 0, c.stream, a.partial, s.parts, e)
     TAM_OF_TYPE(c, TAM_JOIN);
     TAM_OP_LAUNCHED("the parts' sum");
@@ -597,9 +586,11 @@ uint64_t lay_out(call& c, gated_product_args& a, const matrix& P, const matrix& 
   return (uint64_t)a.tm * a.tn * of.parts;
 }
 
+uint64_t joins_of(const gated_out& e) { return tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256); }
+
 int join(call& c, const gated_product_args& a, uint32_t parts) {
   if (parts == 1) return TAM_OK;
-  const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(a.e.cols, 8) * a.e.rows, 256)), block(256);
+  const dim3 grid((uint32_t)joins_of(a.e)), block(256);
 #define TAM_SUM(T) hipLaunchKernelGGL(tam_k_gated_sum<T>, grid, block, 0, c.stream, a.partial, parts, a.e)
   TAM_OF_TYPE(c, TAM_SUM);
   TAM_OP_LAUNCHED("the parts' sum");
@@ -609,17 +600,20 @@ int join(call& c, const gated_product_args& a, uint32_t parts) {
 int backward(const TamGated* d, call& c) {
   const uint32_t size = kSize[c.dtype];
   if (d->rows == 0 || d->outputs == 0 || d->inputs == 0) {  // empty sums
-    int rc = zero(c, d->dx, d->rows * d->inputs);
-    if (rc == TAM_OK) rc = zero(c, d->dgate, d->outputs * d->inputs);
-    return rc == TAM_OK ? zero(c, d->dup, d->outputs * d->inputs) : rc;
+    int rc = zeros(c, d->dx, d->rows * d->inputs);
+    if (rc == TAM_OK) rc = zeros(c, d->dgate, d->outputs * d->inputs);
+    return rc == TAM_OK ? zeros(c, d->dup, d->outputs * d->inputs) : rc;
   }
   if (!d->dx && !d->dgate && !d->dup) return TAM_OK;
   const uint32_t rows = (uint32_t)d->rows, inputs = (uint32_t)d->inputs, outputs = (uint32_t)d->outputs;
   const uint32_t ld = aligned_ld(outputs, size);
   const matrix both = {c.ws.take((uint64_t)rows * 2 * ld * size), 2ull * ld, rows, 2 * ld, true};
+  const uint64_t slopes = tam_div_up((uint64_t)tam_div_up(outputs, 8) * rows, 256);
+  int rc = room(slopes, 256);
+  if (rc != TAM_OK) return rc;
   if (!c.dry) {
     const gated_slope_args a = {d->dh, (const char*)d->kept, (void*)both.p, rows, outputs, ld, d->activation};
-    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(outputs, 8) * rows, 256)), block(256);
+    const dim3 grid((uint32_t)slopes), block(256);
 #define TAM_SLOPE(T) hipLaunchKernelGGL(tam_k_gated_slope<T>, grid, block, 0, c.stream, a)
     TAM_OF_TYPE(c, TAM_SLOPE);
     TAM_OP_LAUNCHED("the activation's gradient");
@@ -628,7 +622,7 @@ int backward(const TamGated* d, call& c) {
   const bool want_w = d->dgate || d->dup;
   // dx's sum goes from one weight to the other in its stride: they are copied both or not at all
   if (in_words(gate, size) != in_words(up, size)) gate.whole = up.whole = false;
-  int rc = d->dx && want_w ? whole_rows(c, {&gate, &up, &x}) : (d->dx ? whole_rows(c, {&gate, &up}) : whole_rows(c, {&x}));
+  rc = d->dx && want_w ? whole_rows(c, {&gate, &up, &x}) : (d->dx ? whole_rows(c, {&gate, &up}) : whole_rows(c, {&x}));
   if (rc != TAM_OK) return rc;
   // dgate and dup lie as the weights do, one product: of dg's and du's columns, a row's padding between them
   gated_out ew = {{d->dgate, d->dup}, 2 * ld, inputs, ld, outputs, false};
@@ -652,8 +646,10 @@ int backward(const TamGated* d, call& c) {
     if (units && in.k / in.parts > w.k / w.parts) a.w_first = (uint32_t)x_units;
     units += x_units;
   }
-  if (c.dry) return TAM_OK;
-  if (units >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
+  rc = room_of_tiles(units, tile, false);
+  if (rc == TAM_OK && want_w && w.parts > 1) rc = room(joins_of(ew), 256);
+  if (rc == TAM_OK && d->dx && in.parts > 1) rc = room(joins_of(ex), 256);
+  if (rc != TAM_OK || c.dry) return rc;
 #define TAM_PRODUCTS(T) launch_products<T>(tile, d->w_in_out != 0, a, (uint32_t)units, c.stream)
   TAM_OF_TYPE(c, TAM_PRODUCTS);
   TAM_OP_LAUNCHED("the gradients' products");

@@ -323,12 +323,6 @@ __global__ __launch_bounds__(1024) void tam_k_column_sum(const float* sums, uint
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void tam_k_zero(T* out, uint32_t n) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n) out[i] = (T)0.0f;
-}
-
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -496,13 +490,9 @@ int backward(const TamLinear* d, call& c) {
       else
         TAM_SLOPE(tam_f16);
     }
-  } else if (d->db && d->outputs && !c.dry) {  // no rows: an empty sum
-    const dim3 grid((uint32_t)tam_div_up(d->outputs, 256)), block(256);
-    if (size == 4)
-      hipLaunchKernelGGL(tam_k_zero<float>, grid, block, 0, c.stream, (float*)d->db, (uint32_t)d->outputs);
-    else  // zero has the same 16 bits in both types
-      hipLaunchKernelGGL(tam_k_zero<tam_f16>, grid, block, 0, c.stream, (tam_f16*)d->db, (uint32_t)d->outputs);
-    TAM_OP_LAUNCHED("the bias's gradient");
+  } else {  // no rows
+    const int rc = zeros(c, d->db, d->outputs);
+    if (rc != TAM_OK) return rc;
   }
   if (!products) return TAM_OK;
   if (d->dx && d->rows) {

@@ -51,6 +51,13 @@ static __global__ __launch_bounds__(256) void tam_k_align_all(tam_align_args a) 
       tam_some(m.src + r * m.ld_src + c, c < m.cols ? m.cols - c : 0);
 }
 
+// Zeros, whose bits are the same in every type, for n 16-bit units.
+static __global__ __launch_bounds__(256) void tam_k_zeros(tam_f16* out, uint64_t n) {
+  const float v[8] = {};
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (uint64_t)gridDim.x * 2048)
+    tam_store_some(out + i, n - i < 8 ? (uint32_t)(n - i) : 8u, v);
+}
+
 namespace {
 
 constexpr uint32_t kSize[3] = {4, 2, 2};
@@ -95,6 +102,27 @@ struct call {
   bool dry;  // lay out the workspace only
   uint32_t* tiles;  // where a product's tile and parts are told (tam_linear_tiles), or null
 };
+
+// A launch takes fewer than 2^32 threads. Asked on both walks, so that the workspace's size is refused already.
+inline int room(uint64_t workgroups, uint32_t threads) {
+  if (workgroups < (1ull << 32) / threads) return TAM_OK;
+  return tam_op_fail(TAM_E_UNSUPPORTED, "a launch of 2^32 threads or more");
+}
+
+// Of tiles, whose numbers are 31 bits; the largest take turns on the compute units where there are more (`turns`).
+inline int room_of_tiles(uint64_t tiles, int tile, bool turns) {
+  if (tile == 256 && turns && tiles < 1ull << 31) return TAM_OK;
+  return room(tiles, tile == 256 ? 512 : 256);
+}
+
+// An empty sum: p, if it is wanted, of `elements`.
+inline int zeros(const call& c, void* p, uint64_t elements) {
+  if (c.dry || !p || !elements) return TAM_OK;
+  const uint64_t halves = elements * (kSize[c.dtype] / 2), wgs = tam_div_up(halves, 2048);
+  hipLaunchKernelGGL(tam_k_zeros, dim3((uint32_t)(wgs < 65536 ? wgs : 65536)), dim3(256), 0, c.stream, (tam_f16*)p, halves);
+  TAM_OP_LAUNCHED("an empty sum");
+  return TAM_OK;
+}
 
 // ---- products ----
 
@@ -182,7 +210,8 @@ inline int whole_rows(call& c, std::initializer_list<matrix*> all) {
     ++a.n;
     *m = {p, ld, m->rows, m->cols, true};
   }
-  if (c.dry || !a.n) return TAM_OK;
+  const int rc = room(tam_div_up(a.units, 256), 256);
+  if (rc != TAM_OK || c.dry || !a.n) return rc;
   hipLaunchKernelGGL(tam_k_align_all, dim3((uint32_t)tam_div_up(a.units, 256)), dim3(256), 0, c.stream, a);
   TAM_OP_LAUNCHED("the aligned copies");
   return TAM_OK;
