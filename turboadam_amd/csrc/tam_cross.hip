@@ -944,17 +944,6 @@ int number_rows(const TamCross* d, const cross_rows& r, float* loss, hipStream_t
   return TAM_OK;
 }
 
-#define TAM_OF_TYPE(c, CALL)                               \
-  do {                                                     \
-    if ((c).dtype == TAM_DTYPE_F32) {                      \
-      CALL(float);                                         \
-    } else if ((c).dtype == TAM_DTYPE_BF16) {              \
-      CALL(tam_bf16);                                      \
-    } else {                                               \
-      CALL(tam_f16);                                       \
-    }                                                      \
-  } while (0)
-
 // The rows of x that count, and w, as the tiles read them, where a product does. kept: where the rows lie or, in
 // the forward pass, are to lie (the workspace where it is null).
 int operands(const TamCross* d, call& c, const cross_rows& r, void* kept, bool back, bool read_x, bool read_w, matrix& x,
@@ -962,7 +951,7 @@ int operands(const TamCross* d, call& c, const cross_rows& r, void* kept, bool b
   const uint32_t size = kSize[c.dtype], halves = size / 2, inputs = (uint32_t)d->inputs, ld = aligned_ld(inputs, size);
   if (read_w) {
     w = matrix_of(d->w, d->ldw, d->vocabulary, d->inputs, size);
-    const int rc = whole_rows(c, {&w});
+    const int rc = whole_rows(c, &w);
     if (rc != TAM_OK) return rc;
   }
   if (!read_x) return TAM_OK;

@@ -429,17 +429,6 @@ matrix w_of(const TamGated* d, const void* w) {
   return matrix_of(w, d->ldw, d->w_in_out ? d->inputs : d->outputs, d->w_in_out ? d->outputs : d->inputs, kSize[d->dtype]);
 }
 
-#define TAM_OF_TYPE(c, CALL)                               \
-  do {                                                     \
-    if ((c).dtype == TAM_DTYPE_F32) {                      \
-      CALL(float);                                         \
-    } else if ((c).dtype == TAM_DTYPE_BF16) {              \
-      CALL(tam_bf16);                                      \
-    } else {                                               \
-      CALL(tam_f16);                                       \
-    }                                                      \
-  } while (0)
-
 template <typename T>
 void launch_gated(int tile, bool pk, const gated_args& a, uint32_t parts, hipStream_t s) {
   const uint32_t tiles = a.tm * a.tn, cus = tam_op_cus();
@@ -542,7 +531,7 @@ int forward(const TamGated* d, call& c) {
     c.tiles[1] = s.parts;
   }
   matrix x = x_of(d), gate = w_of(d, d->gate), up = w_of(d, d->up);
-  int rc = whole_rows(c, {&x, &gate, &up});
+  int rc = whole_rows(c, &x, &gate, &up);
   if (rc != TAM_OK) return rc;
   gated_args a = {};
   if (s.parts > 1) a.partial = (float*)c.ws.take(2ull * s.parts * e.rows * e.cols * 4);
@@ -622,7 +611,7 @@ int backward(const TamGated* d, call& c) {
   const bool want_w = d->dgate || d->dup;
   // dx's sum goes from one weight to the other in its stride: they are copied both or not at all
   if (in_words(gate, size) != in_words(up, size)) gate.whole = up.whole = false;
-  rc = d->dx && want_w ? whole_rows(c, {&gate, &up, &x}) : (d->dx ? whole_rows(c, {&gate, &up}) : whole_rows(c, {&x}));
+  rc = d->dx && want_w ? whole_rows(c, &gate, &up, &x) : (d->dx ? whole_rows(c, &gate, &up) : whole_rows(c, &x));
   if (rc != TAM_OK) return rc;
   // dgate and dup lie as the weights do, one product: of dg's and du's columns, a row's padding between them
   gated_out ew = {{d->dgate, d->dup}, 2 * ld, inputs, ld, outputs, false};

@@ -294,6 +294,8 @@ enum tam_ahead { TAM_AHEAD_PASS, TAM_AHEAD_ROUND, TAM_AHEAD_ALL };
 // of it is fetched in the last step but one (to LDS, where nobody reads it: that takes
 // no registers). Otherwise all compute units, whose tiles end together, wait for
 // memory: of 45 us that a tile of k = 256 took, 11 were the wait for x's low part.
+// The 256 tiles have no LDS left for it, and do without: their ring gained more than the
+// fetch had (tam_k_mu_square's p 378 -> 354 us, tam_k_mu_apply 1540 -> 1422).
 struct tam_soon {
   const char* base;         // of the tile's first element, on 4 bytes; null: nothing
   uint64_t ld;              // bytes, a multiple of 4
@@ -333,6 +335,7 @@ struct tam_tile {
   static constexpr int DUMP = STAGES * STAGE > TURN ? STAGES * STAGE : TURN;
   static constexpr int LDS = RING ? 5 * SP::BYTES : DUMP + NW * 256;  // the words that `soon` fetches
   static_assert(TM % 2 == 0, "rounds of 32 rows");
+  static_assert(!(RING && EXACT && !(PK && QK)), "the ring's loads have no bound at the operand's end");
 
   tam_f4 acc[TN][TM];
 

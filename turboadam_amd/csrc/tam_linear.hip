@@ -371,6 +371,13 @@ void launch_gemm(int tile, bool pk, bool qk, bool rest, const tam_gemm_args& a, 
   rest ? launch_tile<T, 64, 2, 2, true>(pk, qk, a, parts, s) : launch_tile<T, 64, 2, 2, false>(pk, qk, a, parts, s);
 }
 
+// Whether m is read as it lies, and not a copy whose rows are whole lines. Rows that may end inside 16 bytes
+// have kernels of their own (REST), as the bound on their loads and the rest of their
+// sums would cost the others 1% (x [8192, 768], w [768, 3072], bf16, both ways: 206 -> 208
+// us), and a copy of [2018, 13611] fp32 would be 25 of 110 us. The 256 tile is for
+// products so large that the copy is less than 3% of them.
+bool readable(const matrix& m, const shape& s, uint32_t size) { return in_words(m, size) && (m.whole || s.tile != 256); }
+
 // out[rows][cols] = sum over k of Q's row and P's row: P and Q as they lie in
 // memory, p_k / q_k: rows of the matrix are the operand's rows (contiguous along k).
 int product(call& c, matrix P, bool p_k, matrix Q, bool q_k, uint64_t k, const tam_epilogue& e) {
@@ -379,23 +386,25 @@ int product(call& c, matrix P, bool p_k, matrix Q, bool q_k, uint64_t k, const t
     c.tiles[0] = (uint32_t)s.tile;
     c.tiles[1] = s.parts;
   }
-  int rc = readable(c, P, s);
-  if (rc == TAM_OK) rc = readable(c, Q, s);
+  const uint32_t size = kSize[c.dtype];
+  int rc = copy_rows(c, {readable(P, s, size) ? nullptr : &P, readable(Q, s, size) ? nullptr : &Q});
   if (rc != TAM_OK) return rc;
   float* partial = s.parts > 1 ? (float*)c.ws.take((uint64_t)s.parts * e.rows * e.cols * 4) : nullptr;
-  if (c.dry) return TAM_OK;
-  const uint32_t size = kSize[c.dtype];
+  const uint64_t tm = tam_div_up(e.rows, s.tile), tn = tam_div_up(e.cols, s.tile);
+  const uint64_t joins = tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256);
+  rc = room_of_tiles(tm * tn, s.tile, false);
+  if (rc == TAM_OK && s.parts > 1) rc = room(joins, 256);
+  if (rc != TAM_OK || c.dry) return rc;
   tam_gemm_args a = {};
   a.P = operand_of(P, e.cols, size);
   a.Q = operand_of(Q, e.rows, size);
   a.k_all = k;
   a.k = (!p_k || P.whole) && (!q_k || Q.whole) ? k : k - k % (16 / size);
   a.k_part = s.parts > 1 ? tam_up(tam_div_up(a.k, s.parts), 64) : a.k;
-  a.tm = (uint32_t)tam_div_up(e.rows, s.tile);
-  a.tn = (uint32_t)tam_div_up(e.cols, s.tile);
+  a.tm = (uint32_t)tm;
+  a.tn = (uint32_t)tn;
   a.partial = partial;
   a.e = e;
-  if ((uint64_t)a.tm * a.tn >= 1ull << 31) return tam_op_fail(TAM_E_UNSUPPORTED, "a product of too many tiles");
   if (c.dtype == TAM_DTYPE_BF16)
     launch_gemm<tam_bf16>(s.tile, p_k, q_k, !(P.whole && Q.whole), a, s.parts, c.stream);
   else if (c.dtype == TAM_DTYPE_F16)
@@ -404,7 +413,7 @@ int product(call& c, matrix P, bool p_k, matrix Q, bool q_k, uint64_t k, const t
     launch_gemm<float>(s.tile, p_k, q_k, !(P.whole && Q.whole), a, s.parts, c.stream);
   TAM_OP_LAUNCHED("the product");
   if (s.parts > 1) {
-    const dim3 grid((uint32_t)tam_div_up((uint64_t)tam_div_up(e.cols, 8) * e.rows, 256)), block(256);
+    const dim3 grid((uint32_t)joins), block(256);
     if (c.dtype == TAM_DTYPE_BF16)
       hipLaunchKernelGGL(tam_k_split<tam_bf16>, grid, block, 0, c.stream, partial, s.parts, e);
     else if (c.dtype == TAM_DTYPE_F16)

@@ -11,19 +11,8 @@
 // ---------------------------------------------------------------------------
 // alignment
 // ---------------------------------------------------------------------------
-// dst[r][0 .. ld_dst) = src[r][0 .. cols) of 16-bit elements, zeros behind: a thread
-// moves 8 elements and none of their bits.
-static __global__ __launch_bounds__(256) void tam_k_align(const tam_f16* src, uint64_t ld_src, uint64_t rows, uint32_t cols,
-                                                   tam_f16* dst, uint32_t ld_dst) {
-  const uint32_t per = ld_dst / 8;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (uint64_t)per * rows) return;
-  const uint64_t r = i / per;
-  const uint32_t c = (uint32_t)(i - r * per) * 8;
-  *reinterpret_cast<tam_oct<tam_f16>*>(dst + r * ld_dst + c) = tam_some(src + r * ld_src + c, c < cols ? cols - c : 0);
-}
-
-// Up to three matrices of 16-bit units, one behind the other.
+// dst[r][0 .. ld_dst) = src[r][0 .. cols) of up to three matrices of 16-bit units, one behind the other, zeros
+// behind a row: a thread moves 8 units and none of their bits.
 struct tam_align_item {
   const tam_f16* src;
   tam_f16* dst;
@@ -36,7 +25,7 @@ struct tam_align_args {
   int n;
 };
 
-static __global__ __launch_bounds__(256) void tam_k_align_all(tam_align_args a) {
+static __global__ __launch_bounds__(256) void tam_k_align(tam_align_args a) {
   uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= a.units) return;
   tam_align_item m = a.item[0];
@@ -102,6 +91,18 @@ struct call {
   bool dry;  // lay out the workspace only
   uint32_t* tiles;  // where a product's tile and parts are told (tam_linear_tiles), or null
 };
+
+// CALL(T) with the type of call c.
+#define TAM_OF_TYPE(c, CALL)                               \
+  do {                                                     \
+    if ((c).dtype == TAM_DTYPE_F32) {                      \
+      CALL(float);                                         \
+    } else if ((c).dtype == TAM_DTYPE_BF16) {              \
+      CALL(tam_bf16);                                      \
+    } else {                                               \
+      CALL(tam_f16);                                       \
+    }                                                      \
+  } while (0)
 
 // A launch takes fewer than 2^32 threads. Asked on both walks, so that the workspace's size is refused already.
 inline int room(uint64_t workgroups, uint32_t threads) {
@@ -177,32 +178,13 @@ inline double units_us(const tam_tile_rate& t, uint64_t n1, double k1, uint64_t 
   return 0.5 * t.start + (late && late_at > early_at ? late_at : early_at);
 }
 
-// m, or a copy of it whose rows are whole lines. Rows that may end inside 16 bytes
-// have kernels of their own (REST), as the bound on their loads and the rest of their
-// sums would cost the others 1% (x [8192, 768], w [768, 3072], bf16, both ways: 206 -> 208
-// us), and a copy of [2018, 13611] fp32 would be 25 of 110 us. The 256 tile is for
-// products so large that the copy is less than 3% of them.
-inline int readable(call& c, matrix& m, const shape& s) {
-  const uint32_t size = kSize[c.dtype];
-  if ((in_words(m, size) && (m.whole || s.tile != 256)) || !m.cols || !m.rows) return TAM_OK;  // no elements: nothing is read
-  const uint32_t ld = aligned_ld(m.cols, size);
-  void* p = c.ws.take(m.rows * ld * size);
-  if (!c.dry) {
-    const dim3 grid((uint32_t)tam_div_up(m.rows * (ld / 8), 256)), block(256);
-    hipLaunchKernelGGL(tam_k_align, grid, block, 0, c.stream, (const tam_f16*)m.p, m.ld, m.rows, m.cols, (tam_f16*)p, ld);
-    TAM_OP_LAUNCHED("the aligned copy");
-  }
-  m = {p, ld, m.rows, m.cols, true};
-  return TAM_OK;
-}
-
-// The matrices, or copies of them: rows of whole 16 bytes that begin on 4, for kernels without a REST
-// form. All copies are one launch (three of 5 us each were a tenth of a small layer's time).
-inline int whole_rows(call& c, std::initializer_list<matrix*> all) {
+// Copies, in rows of whole lines, in place of those matrices that are given. All are one launch (three of 5 us each
+// were a tenth of a small layer's time). Matrices of no elements stay: nothing of them is read.
+inline int copy_rows(call& c, std::initializer_list<matrix*> all) {
   const uint32_t size = kSize[c.dtype], halves = size / 2;
   tam_align_args a = {};
   for (matrix* m : all) {
-    if ((in_words(*m, size) && m->whole) || !m->cols || !m->rows) continue;
+    if (!m || !m->cols || !m->rows) continue;
     const uint32_t ld = aligned_ld(m->cols, size);
     void* p = c.ws.take(m->rows * ld * size);
     a.item[a.n] = {(const tam_f16*)m->p, (tam_f16*)p, m->ld * halves, m->rows, a.units, m->cols * halves, ld * halves};
@@ -212,9 +194,17 @@ inline int whole_rows(call& c, std::initializer_list<matrix*> all) {
   }
   const int rc = room(tam_div_up(a.units, 256), 256);
   if (rc != TAM_OK || c.dry || !a.n) return rc;
-  hipLaunchKernelGGL(tam_k_align_all, dim3((uint32_t)tam_div_up(a.units, 256)), dim3(256), 0, c.stream, a);
+  hipLaunchKernelGGL(tam_k_align, dim3((uint32_t)tam_div_up(a.units, 256)), dim3(256), 0, c.stream, a);
   TAM_OP_LAUNCHED("the aligned copies");
   return TAM_OK;
+}
+
+// The matrices, or copies of them: rows of whole 16 bytes that begin on 4, for kernels without a REST form.
+inline int whole_rows(call& c, matrix* m0, matrix* m1 = nullptr, matrix* m2 = nullptr) {
+  const uint32_t size = kSize[c.dtype];
+  for (matrix** m : {&m0, &m1, &m2})
+    if (*m && in_words(**m, size) && (*m)->whole) *m = nullptr;
+  return copy_rows(c, {m0, m1, m2});
 }
 
 // m as an operand of a product: `count` rows or columns of it are the operand's.
