@@ -44,7 +44,9 @@ __device__ __forceinline__ float cross_exp(float x) {
     return expf(x);
 }
 
-constexpr float kFarTop = 1073741824.0f;  // 2^30
+// What multiplies 16-bit types' logits ahead of the hardware's 2^x. Past 2^30 they are 64 or more apart, and any base
+// tells the largest from the others; log2e times them may be infinite.
+__device__ __forceinline__ float cross_rate(float at) { return fabsf(at) < 1073741824.0f ? kLog2e : 1.0f; }
 
 // The sum of exp(z - top) over a lane's values, top their maximum or more, but in 16-bit types for the
 // factor that cross_settled takes out. A top of -inf (words that cannot be, or columns past the last one) counts as
@@ -53,13 +55,13 @@ template <typename T, int N>
 __device__ __forceinline__ float cross_terms(const float (&z)[N], float top) {
   const float at = top == -INFINITY ? 0.0f : top;
   float sum = 0.f;
-  if (sizeof(T) == 2 && fabsf(at) < kFarTop) {  // one multiplication and addition ahead of the hardware's 2^x
-    const float shift = -kLog2e * at;
+  if constexpr (sizeof(T) == 2) {  // one multiplication and addition ahead of the hardware's 2^x
+    const float rate = cross_rate(at), shift = -rate * at;
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], kLog2e, shift));
+    for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], rate, shift));
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum += cross_exp<T>(z[j] - at);
+    for (int j = 0; j < N; ++j) sum += expf(z[j] - at);
   }
   return sum;
 }
@@ -69,7 +71,8 @@ __device__ __forceinline__ float cross_terms(const float (&z)[N], float top) {
 template <typename T>
 __device__ __forceinline__ float cross_settled(float sum, float top) {
   if constexpr (sizeof(T) == 2) {
-    if (fabsf(top) < kFarTop) sum *= __builtin_amdgcn_exp2f(__builtin_fmaf(-kLog2e, top, kLog2e * top));
+    const float at = top == -INFINITY ? 0.0f : top, rate = cross_rate(at);
+    sum *= __builtin_amdgcn_exp2f(__builtin_fmaf(-rate, at, rate * at));
   }
   return sum;
 }
@@ -238,14 +241,15 @@ __device__ __forceinline__ void cross_forward(const cross_logits_args& a, Tile& 
   sync();
   const uint32_t row = m * TILE + threadIdx.x;
   if (threadIdx.x < TILE && row < count) {
-    float2 all = {-INFINITY, 0.f};
-#pragma unroll
-    for (int w = 0; w < WN; ++w) all.x = fmaxf(all.x, at[threadIdx.x * WN + w].x);
+    float2 part[WN], all = {-INFINITY, 0.f};
 #pragma unroll
     for (int w = 0; w < WN; ++w) {
-      const float2 p = at[threadIdx.x * WN + w];
-      if (p.y != 0.f) all.y += cross_settled<T>(p.y, p.x) * cross_exp<T>(p.x - all.x);
+      part[w] = at[threadIdx.x * WN + w];
+      all.x = fmaxf(all.x, part[w].x);
     }
+    const float top = all.x == -INFINITY ? 0.0f : all.x;  // a part of no words is 0 times exp(-inf)
+#pragma unroll
+    for (int w = 0; w < WN; ++w) all.y += cross_settled<T>(part[w].y, part[w].x) * cross_exp<T>(part[w].x - top);
     a.parts[(uint64_t)n * a.rows + row] = all;
   }
 }
