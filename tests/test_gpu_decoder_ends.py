@@ -224,3 +224,13 @@ def test_cross_gradients_of_one_argument(rows, inputs, words, dt):
         some = [v.detach().requires_grad_(j == i) for j, v in enumerate((x, w))]
         got, = torch.autograd.grad(linear_cross_entropy(*some, t), [some[i]])
         assert float((got.double() - both[i].double()).norm()) <= (2 * UNIT[dt] + 2.0 ** -18) * float(both[i].double().norm()), i
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_cross_few_rows_over_more_words_than_a_piece(dt):
+    """Past 2^20 words the backward pass of few rows takes pieces by tiles; the bounds are those of the other tests."""
+    from tests.test_gpu_decoder import _check_cross, _cross_case
+
+    log(f"cross of few rows over more words than a piece {dt}")
+    _check_cross(*_cross_case(5, 24, (1 << 20) + 777, dt, 0.3), dt, "mean")
+    _check_cross(*_cross_case(30, 9, (1 << 20) + 2, dt, 0.3), dt, "none")
