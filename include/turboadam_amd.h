@@ -396,8 +396,8 @@ int tam_norm_backward(const TamNorm* d, void* workspace, size_t ws_bytes, void* 
 
 /* The first half of a gated feed-forward block: h = act(x gate^T) * (x up^T), and its
  * gradients.  Both products are one; the backward pass sees g = x gate^T and u = x up^T
- * with 8 bits more than dtype, and dg = dh u act'(g) and du = dh act(g) are rounded to it
- * before the products that make dx, dgate and dup.  Every array is of `dtype`; arrays without a stride
+ * as the upper 24 bits of fp32 (fp32: whole), and dg = dh u act'(g) and du = dh act(g) are
+ * rounded to dtype before the products that make dx, dgate and dup.  Every array is of `dtype`; arrays without a stride
  * are contiguous.  Arrays may lie at any element's address; operands whose rows are not
  * whole 16 bytes on 4 bytes are first copied to the workspace: ask for its size with the
  * pointers and strides of the call. */

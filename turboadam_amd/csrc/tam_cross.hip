@@ -309,9 +309,9 @@ __device__ __forceinline__ void cross_backward(const cross_logits_args& a, Tile&
 // Bound by the matrix cores and, at small k, by what follows the sums: exponentials, and
 // in the backward pass the stores. 16-bit tiles of 256: a workgroup to a compute unit, which begins
 // its next tile before it goes through the last one's sums. bf16, 7680 rows that count x 4096 over
-// 128256 words: 6104 us (1322 TFLOP/s), in four pieces of dz 6362 (1268); 8192 x 768 over 50257 words
-// 587 (1077), two pieces of dz 651 (971, 1.3 TB/s written beside it). fp32 619 x 515 over 9973 words, 64
-// tiles: 68 and 70 (91 to 93 TFLOP/s).
+// 128256 words: 6123 us (1318 TFLOP/s), in four pieces of dz 6347 (1271); 8192 x 768 over 50257 words
+// 598 (1057), two pieces of dz 660 (958, 1.2 TB/s written beside it). fp32 619 x 515 over 9973 words, 64
+// tiles: 68 and 69 (91 to 93 TFLOP/s).
 template <typename T, int TILE, int WM, int WN, bool BACK>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_logits(cross_logits_args a) {
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), true, true> Tile;
@@ -504,7 +504,7 @@ struct cross_few_args {
 
 // One workgroup: 16 columns of z for up to 16 * MT rows of x, as tam_k_few. BACK: dz of rows that
 // count, of the whole vocabulary. Bound by memory: 1 x 4096 over 128256 words bf16 176 us, 6.0 TB/s; 8 x
-// 7191 over 72376 480, 2.2, as rows that begin on odd addresses take loads of their own.
+// 7191 over 72376 487, 2.1, as rows that begin on odd addresses take loads of their own.
 template <typename T, int MT, bool BACK>
 __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_cross_few(cross_few_args a) {
   constexpr int N = 16 / (int)sizeof(T), U = 4;
@@ -830,9 +830,9 @@ __device__ __forceinline__ void cross_product(cross_product_args& a, uint32_t un
       [](uint32_t, uint32_t, const float*, int) {});
 }
 
-// Bound by the matrix cores: bf16, 7680 rows that count x 4096 over 128256 words, four pieces 11850 us
-// for 16.1 Tflop (1362 TFLOP/s); 8192 x 768 over 50257 words, two pieces 983 (1287). fp32 619 x 515 over 9973
-// words, 64 tiles: 140 (91).
+// Bound by the matrix cores: bf16, 7680 rows that count x 4096 over 128256 words, four pieces 11920 us
+// for 16.1 Tflop (1354 TFLOP/s); 8192 x 768 over 50257 words, two pieces 1003 (1261). fp32 619 x 515 over 9973
+// words, 64 tiles: 129 (99).
 template <typename T, int TILE, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_cross_products(cross_products_args a) {
   typedef tam_tile<T, TILE, TILE, WM, WN, tam_stages<T, TILE>(), false, true> Tile;

@@ -110,8 +110,8 @@ struct gated_args {
 
 // Bound by the matrix cores, small ones by rounds that do not fill the card. 256 tiles: a workgroup to a
 // compute unit, which begins its next tile before it stores the last. 8192 x 4096 -> 14336 bf16
-// with what is kept: 1560 us, 1234 TFLOP/s (0.94 GB written beside it, of it 0.7 kept); 2048 x 768 -> 2048
-// fp16: 24; fp32 1531 x 777 -> 1001, 64 tiles: 47.
+// with what is kept: 1572 us, 1224 TFLOP/s (0.94 GB written beside it, of it 0.7 kept); 2048 x 768 -> 2048
+// fp16: 25; fp32 1531 x 777 -> 1001, 64 tiles: 47.
 template <typename T, int BM, int BN, int WM, int WN, bool PK>
 __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 3 : 2) void tam_k_gated(gated_args a) {
   typedef tam_tile<T, BM, BN, WM, WN, tam_stages<T, BM>(), PK, true, false, true> Tile;
@@ -204,7 +204,7 @@ struct gated_few_args {
 
 // One workgroup: 16 columns of h for up to 16 * MT rows of x, as tam_k_few; a wave's
 // turn of k is half as long, as it loads two weights. Bound by memory: 1 x 4096 -> 14336 bf16
-// 45.9 us, 5.1 TB/s.
+// 41 us where the weights stay in the memory-side cache, 46 to 48 where they do not (4.9 TB/s).
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * TAM_FEW_WAVES) void tam_k_gated_few(gated_few_args a) {
   constexpr int N = 16 / (int)sizeof(T), U = 4;
@@ -275,7 +275,7 @@ struct gated_slope_args {
   uint32_t cols, ld, act;
 };
 
-// A thread: one record. Bound by memory: 8192 x 14336 bf16 244 us, 5.8 TB/s.
+// A thread: one record. Bound by memory: 8192 x 14336 bf16 246 us, 5.7 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void tam_k_gated_slope(gated_slope_args a) {
   const uint32_t per = (a.cols + 7) / 8;
@@ -366,8 +366,8 @@ __device__ __forceinline__ void gated_product(const gated_product_args& a, uint3
 
 // One launch for both products, the longer sums first (dx's, where 2 outputs in its parts are more than the rows
 // in theirs), so that the second fills the places that the first leaves empty in its last round (2048 x 2048 -> 8192 bf16
-// both ways 387 us, 427 with dx behind). Bound by the matrix cores: 8192 x 4096 -> 14336 bf16 2739 us
-// for 3.85 Tflop, 1405 TFLOP/s; 2048 x 768 -> 2048 fp16 48, fp32 1531 x 777 -> 1001 104.
+// both ways 387 us, 427 with dx behind). Bound by the matrix cores: 8192 x 4096 -> 14336 bf16 2765 us
+// for 3.85 Tflop, 1392 TFLOP/s; 2048 x 768 -> 2048 fp16 46, fp32 1531 x 777 -> 1001 101.
 // IN_OUT: of weights stored [inputs][outputs], along which dx's sums run.
 template <typename T, int TILE, int WM, int WN, bool IN_OUT>
 __global__ __launch_bounds__(64 * WM * WN, TILE == 64 ? 3 : 2) void tam_k_gated_products(gated_products_args a) {

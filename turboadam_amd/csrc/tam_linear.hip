@@ -98,7 +98,7 @@ struct tam_gemm_args {
 // Bound by the matrix cores and, beside them, by LDS (operands in, fragments out).
 // 8192 x 14336 x 4096 bf16, 256 tiles (means over 200 passes, from card to card 5%
 // either way): 681 us with both operands along k (1413 TFLOP/s), 715 for dx (one
-// m-major), 755 for dw (both); a library product of 8192^3 reaches 1398 TFLOP/s, and on
+// m-major), 755 for dw (both); a library product of 8192^3 reaches 1398 to 1564 TFLOP/s from card to card, and on
 // operands of zeros, at the clock that they leave, this one 1900.
 // 8192 x 768 x 3072, 128 tiles: 70 us for y and z (its 100 MB of stores are the second
 // bound), 47 for dx and dw each. fp32 1531 x 1001 x 777, 64 tiles: 30, 34 and 39 us;

@@ -180,9 +180,10 @@ __device__ __forceinline__ float inverse_root(float x) {
 
 // A wave takes a bundle's rows in turns, queries' first; a turn's rows are all of one part, and their
 // addresses a base that the lanes share and an offset that a lane keeps. Bound by memory and,
-// nearly as much, by the vector unit: 16384 tokens of 32 + 8 heads of 128 bf16 with norms 73 us forward
-// (4.6 TB/s), 111 backward (4.6). One token: 4.5, a launch and three trips to memory one after another
-// (position, heads, results). 8192 tokens of 24 heads of 64 fp32, pairs side by side: 27 (3.7).
+// nearly as much, by the vector unit: 16384 tokens of 32 + 8 heads of 128 bf16 with norms 74 us forward
+// (4.6 TB/s), 113 backward (4.5). One token: 4.6, a launch and three trips to memory one after another
+// (position, heads, results). 8192 tokens of 24 heads of 64 fp32, pairs side by side: 28 (3.6; not at a
+// limit).
 // NORM: both parts have a weight, or none. BACK: dx and the weights' sums of a norm's backward pass (without
 // a norm it is the forward pass with the angles' sign turned).
 template <typename T, bool SIDE, bool NORM, bool BACK>
