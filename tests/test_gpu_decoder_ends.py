@@ -234,3 +234,21 @@ def test_cross_few_rows_over_more_words_than_a_piece(dt):
     log(f"cross of few rows over more words than a piece {dt}")
     _check_cross(*_cross_case(5, 24, (1 << 20) + 777, dt, 0.3), dt, "mean")
     _check_cross(*_cross_case(30, 9, (1 << 20) + 2, dt, 0.3), dt, "none")
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 21, 2.0 ** 26, 2.0 ** 28, 2.0 ** 40])
+@pytest.mark.parametrize("rows,words", [(20, 3001), (50, 60), (300, 2777)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_cross_loss_of_exact_logits_past_single_steps(rows, words, dt, scale):
+    """Logits that lie a thousandth of themselves apart or are the same: a loss is the difference to the largest and the
+    logarithm of how many of those there are, 2^-23 of either."""
+    from turboadam_amd import linear_cross_entropy
+
+    log(f"cross of exact logits {rows}x{words} {dt} scale {scale}")
+    x, w, t = _exact_case(rows, 16, words, dt, scale)
+    z = x.double() @ w.double().t()
+    number = (z == z.amax(1, keepdim=True)).sum(1).double().log()
+    want = z.amax(1) - z.gather(1, t[:, None])[:, 0] + number  # in 64 bits too a sum with the logarithm would be rounded
+    away = torch.where(z < z.amax(1, keepdim=True), z.amax(1, keepdim=True) - z, math.inf).amin(1)
+    assert bool((away > 100).all())  # nothing else counts
+    _within(linear_cross_entropy(x, w, t, reduction="none"), want, 2.0 ** -22 * (want.abs() + number), "loss")
